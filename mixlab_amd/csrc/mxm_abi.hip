@@ -10,93 +10,26 @@
 
 #include <algorithm>
 #include <array>
-#include <cstdarg>
 #include <cstdlib>
-#include <cstdio>
 #include <cstring>
 #include <map>
 #include <memory>
 #include <mutex>
-#include <stdexcept>
 #include <string>
 #include <vector>
 
 #include "../../include/mixmoe.h"
+#include "mxm_host.h"
 #include "mxm_kernels.h"
+
+thread_local std::string g_last_error;
 
 namespace {
 
-thread_local std::string g_last_error;
 std::mutex g_mu;
 std::map<int64_t, std::unique_ptr<struct MoeOp>> g_ops;
 int64_t g_next_handle = 1;
 std::string g_device_name = "uninitialised";
-
-// Failure classes of the bridge's status codes (gpu/mlx_bridge.cpp:814-823):
-// an argument the call cannot accept (MXM_ERR_ARGS), a runtime that is not
-// initialised (MXM_ERR_INIT); every other failure -- a HIP error, a call out
-// of sequence -- is MXM_ERR.
-struct ArgError : std::runtime_error {
-  using std::runtime_error::runtime_error;
-};
-struct InitError : std::runtime_error {
-  using std::runtime_error::runtime_error;
-};
-
-template <class Ex>
-[[noreturn]] void vthrow(const char* fmt, va_list ap) {
-  char buf[512];
-  vsnprintf(buf, sizeof buf, fmt, ap);
-  throw Ex(buf);
-}
-
-// An argument error (shape, dtype, index, size limit, NULL pointer).
-[[noreturn]] void fail(const char* fmt, ...) {
-  va_list ap;
-  va_start(ap, fmt);
-  vthrow<ArgError>(fmt, ap);
-}
-// A runtime failure or a call out of sequence.
-[[noreturn]] void fail_rt(const char* fmt, ...) {
-  va_list ap;
-  va_start(ap, fmt);
-  vthrow<std::runtime_error>(fmt, ap);
-}
-// The HIP runtime or the device is not (or cannot be) initialised.
-[[noreturn]] void fail_init(const char* fmt, ...) {
-  va_list ap;
-  va_start(ap, fmt);
-  vthrow<InitError>(fmt, ap);
-}
-
-#define HIPCK(expr)                                                                       \
-  do {                                                                                    \
-    hipError_t _e = (expr);                                                               \
-    if (_e != hipSuccess)                                                                 \
-      fail_rt("HIP error %s at %s:%d", hipGetErrorString(_e), __FILE__, __LINE__);       \
-  } while (0)
-
-struct DevBuf {
-  void* p = nullptr;
-  size_t bytes = 0;
-  DevBuf() = default;
-  DevBuf(const DevBuf&) = delete;
-  DevBuf& operator=(const DevBuf&) = delete;
-  ~DevBuf() { reset(); }
-  void alloc(size_t n) {
-    reset();
-    if (n == 0) n = 256;
-    HIPCK(hipMalloc(&p, n));
-    bytes = n;
-  }
-  void reset() {
-    if (p) (void)hipFree(p);
-    p = nullptr;
-    bytes = 0;
-  }
-  template <typename T>
-  T* as() const { return static_cast<T*>(p); }
-};
 
 // Every device buffer a forward writes besides its outputs.  layout_workspace
 // places the pieces at 256-byte aligned offsets from one base; the ticket is
@@ -152,6 +85,7 @@ struct MoeOp {
   // H holds two bf16 planes [N*K][2F] and Y is fp32 (GemmArgs::h_split)
   bool hsplit = false;
   int family = MXM_TILE_AUTO;
+  std::shared_ptr<StreamRef> stream_ref;  // owns `stream`; other handles may hold it too
   hipStream_t stream = nullptr;
   int device = 0;  // the device current at create (the stream's)
 
@@ -249,10 +183,7 @@ struct MoeOp {
   size_t ev_used = 0;
 
   ~MoeOp() {
-    if (stream) {
-      (void)hipStreamSynchronize(stream);
-      (void)hipStreamDestroy(stream);
-    }
+    if (stream) (void)hipStreamSynchronize(stream);
     for (auto& set : ev_sets)
       for (auto& e : set)
         if (e) (void)hipEventDestroy(e);
@@ -264,25 +195,6 @@ MoeOp* get_op(int64_t h) {
   auto it = g_ops.find(h);
   if (it == g_ops.end()) return nullptr;
   return it->second.get();
-}
-
-template <typename F>
-int fenced(F&& f) {
-  try {
-    return f();
-  } catch (const ArgError& e) {
-    g_last_error = e.what();
-    return MXM_ERR_ARGS;
-  } catch (const InitError& e) {
-    g_last_error = e.what();
-    return MXM_ERR_INIT;
-  } catch (const std::exception& e) {
-    g_last_error = e.what();
-    return MXM_ERR;
-  } catch (...) {
-    g_last_error = "unknown exception";
-    return MXM_ERR;
-  }
 }
 
 #define OP_OR_RETURN(h)                                 \
@@ -947,6 +859,17 @@ char* device_scratch(hipStream_t capturing) {
 
 }  // namespace
 
+int64_t mxm_new_handle() {
+  std::lock_guard<std::mutex> lk(g_mu);
+  return g_next_handle++;
+}
+
+std::shared_ptr<StreamRef> mxm_op_stream(int64_t h) {
+  std::lock_guard<std::mutex> lk(g_mu);
+  const auto it = g_ops.find(h);
+  return it == g_ops.end() ? nullptr : it->second->stream_ref;
+}
+
 extern "C" {
 
 int mxm_init(void) {
@@ -1122,7 +1045,8 @@ int64_t mxm_moe_create(const float* float_params, int n_float_params, const int3
     o->have.assign((size_t)n_inputs, 0);
     HIPCK(hipGetDevice(&o->device));
     HIPCK(hipDeviceGetAttribute(&o->n_cu, hipDeviceAttributeMultiprocessorCount, o->device));
-    HIPCK(hipStreamCreateWithFlags(&o->stream, hipStreamNonBlocking));
+    o->stream_ref = std::make_shared<StreamRef>(o->device);
+    o->stream = o->stream_ref->stream;
     const size_t DE = (size_t)o->D * o->E, DF = (size_t)o->D * o->F, EE = (size_t)o->E;
     const size_t F1 = (size_t)o->Kx * o->Fk, F2 = (size_t)o->Fk * o->Dk;  // padded matrices
     o->router.alloc(DE * (o->bf16 ? 2 : 4));
