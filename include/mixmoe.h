@@ -296,6 +296,109 @@ int mxm_moe_stage_times(int64_t op, float* ms, int n);
  * n, at most 8). */
 int mxm_moe_info(int64_t op, int64_t* info, int n);
 
+/* ---- around the op's training step ----
+ *
+ * The handles below run on a stream of their own, or on that of another live
+ * handle (`stream_of`: an op, a residual norm or a gradient set; 0: a new
+ * stream on the current device).  Handles that share a stream run in call
+ * order without any wait on the host, so a block's norms, its op and its
+ * optimizer go on one stream; work on another stream is ordered by the caller
+ * (mxm_stream, mxm_synchronize).  The stream lives as long as its last handle.
+ * Calls on one handle are serialised by the caller, as an op's are; calls on
+ * handles that share nothing but the stream may come from several threads.
+ * Every call is asynchronous and runs on the handle's device, whichever device
+ * is current.  Tensors are contiguous device memory aligned to their elements.
+ * After creation (and mxm_grads_bind) no call allocates or waits, so all of
+ * them can be captured into a HIP graph on the handle's stream; the scalars
+ * given by value (rows, lr, max_norm, ...) are then the captured ones.  A
+ * handle's workspace is its own: two graphs captured from one handle must not
+ * run at once.  None of this has a counterpart in the reference's bridge,
+ * whose graph compiler fuses such work itself. */
+
+/* Residual norm: what stands between a block's branch and the next block.
+ * Row n, channel d; x the residual stream, delta the branch's output:
+ *   z = delta / sqrt(mean_d(delta^2) + eps) with MXM_RESNORM_POST_NORM, else delta
+ *   h = x + gate[n / gateRows] * branch_scale * post_scale * z
+ *   y = norm_scale * h / sqrt(mean_d(h^2) + eps)    with MXM_RESNORM_NORM
+ * (moe_scale and the residual Add of arch/moe.go:199-204, :164, and the RMSNorm
+ * of gpu/ir.cpp:4949-4960, in one pass).  y is computed from h as it is kept,
+ * i.e. after h's rounding to the stream's type; sums are in fp32. */
+#define MXM_RESNORM_BRANCH 1       /* h = x + ...; without it h is x itself */
+#define MXM_RESNORM_POST_NORM 2    /* the branch is normalised first */
+#define MXM_RESNORM_NORM 4         /* the sum is normalised: y */
+#define MXM_RESNORM_GATE_SIGMOID 8 /* the gate is the sigmoid of what is given */
+#define MXM_RESNORM_BACKWARD 16    /* the handle also runs backward (holds its workspace) */
+#define MXM_RESNORM_MAX_D 16384
+#define MXM_GATE_NONE 0
+#define MXM_GATE_ROW 1     /* gate [ceil(rows / gateRows)] */
+#define MXM_GATE_CHANNEL 2 /* gate [ceil(rows / gateRows)][D] */
+
+/* params = [D, maxRows, streamDtype, branchDtype, outDtype, scaleDtype,
+ * gradDtype, flags, gate, gateRows]; dtypes are MXM_DTYPE_F32 or
+ * MXM_DTYPE_BF16: x and h, delta, y, the scales and the gate, and the gradients
+ * dh, dy, dx and d_delta.  Returns a handle, 0 on failure. */
+int64_t mxm_resnorm_create(const int64_t* params, int n_params, float eps, int64_t stream_of);
+int mxm_resnorm_destroy(int64_t h);
+
+/* h and y for rows <= maxRows rows (rows behind them are left as they were).
+ * Scales may be NULL (ones); h may be x, y may be delta where the types agree.
+ * delta, h and gate are ignored without a branch or gate, y without a norm. */
+int mxm_resnorm_forward(int64_t handle, int64_t rows, const void* x, const void* delta,
+                        const void* post_scale, const void* branch_scale, const void* gate,
+                        const void* norm_scale, void* h, void* y);
+
+/* Gradients at the forward's h (x for a handle without a branch) and delta,
+ * for upstream gradients dh and dy.  With a norm dh may be NULL (zeros), without
+ * one dy is ignored and dx, which then equals dh, may be NULL.  dx may be dh
+ * and d_delta may be dy or delta where the types agree.  The
+ * scales' and the gate's gradients are fp32 (overwritten, not added to; NULL:
+ * not computed), summed in a fixed order: equal inputs give equal bits. */
+int mxm_resnorm_backward(int64_t handle, int64_t rows, const void* h, const void* delta,
+                         const void* post_scale, const void* branch_scale, const void* gate,
+                         const void* norm_scale, const void* dh, const void* dy, void* dx,
+                         void* d_delta, float* d_post_scale, float* d_branch_scale, float* d_gate,
+                         float* d_norm_scale);
+
+/* Gradient set: n tensors of sizes[i] elements whose gradients are dtypes[i]
+ * (MXM_DTYPE_F32 or MXM_DTYPE_BF16); decay[i] multiplies the weight decay of
+ * tensor i (NULL: 1 each).  Returns a handle, 0 on failure. */
+int64_t mxm_grads_create(const int64_t* sizes, const int32_t* dtypes, const float* decay, int n,
+                         int64_t stream_of);
+int mxm_grads_destroy(int64_t h);
+
+/* Where the tensors are: host arrays of n device pointers.  clipped (the type
+ * of the gradients) is where mxm_grads_clip writes, NULL: in place.  params, m
+ * and v (fp32) are AdamW's, all or none; params_bf16, or NULL, gets the updated
+ * params rounded to bf16.  Waits for the handle's stream; calls use the
+ * pointers bound last, those captured into a graph too. */
+int mxm_grads_bind(int64_t h, const void* const* grads, void* const* clipped, void* const* params,
+                   void* const* m, void* const* v, void* const* params_bf16);
+
+/* norm [1] fp32 = sqrt(sum of squares over all tensors), summed in 64 bits in a
+ * fixed order. */
+int mxm_grads_norm(int64_t h, float* norm);
+
+/* clipped = g * min(1, max_norm / (norm + 1e-6)); where the norm is not finite
+ * the gradients are copied as they are.  norm may be NULL. */
+int mxm_grads_clip(int64_t h, double max_norm, float* norm);
+
+/* One AdamW step on the clipped gradients (max_norm 0: not clipped), which are
+ * not written back: with t = ++*step (device memory)
+ *   m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2
+ *   p -= lr weight_decay decay[i] p + lr (m / (1 - beta1^t)) / (sqrt(v / (1 - beta2^t)) + eps)
+ * A gradient norm that is not finite leaves params, m, v, the bf16 copies and
+ * *step as they were (gpu/optimizer_step_guard.h:12-71 rejects such a step) and
+ * sets *skipped to 1, else to 0.  norm and skipped may be NULL. */
+int mxm_grads_adamw(int64_t h, double lr, double beta1, double beta2, double eps,
+                    double weight_decay, double max_norm, int64_t* step, float* norm,
+                    int32_t* skipped);
+
+/* The hipStream_t that a handle (an op's too) runs on, to order other work with
+ * it or to capture its calls. */
+int mxm_stream(int64_t handle, void** stream);
+/* Wait for all work queued on a handle's stream. */
+int mxm_synchronize(int64_t handle);
+
 #ifdef __cplusplus
 }
 #endif

@@ -29,6 +29,15 @@ MXM_FLAG_MFMA_TILE256x128 = 8
 MXM_FLAG_MFMA_TILE256x256 = 12
 MXM_FLAG_INT8_WEIGHTS = 16
 MXM_FLAG_KEEP_FOR_BACKWARD = 32
+MXM_RESNORM_BRANCH = 1
+MXM_RESNORM_POST_NORM = 2
+MXM_RESNORM_NORM = 4
+MXM_RESNORM_GATE_SIGMOID = 8
+MXM_RESNORM_BACKWARD = 16
+MXM_RESNORM_MAX_D = 16384
+MXM_GATE_NONE = 0
+MXM_GATE_ROW = 1
+MXM_GATE_CHANNEL = 2
 MXM_NUM_STAGES = 6
 MXM_NOALLOC_MAX_BYTES = 64 << 20
 STAGE_NAMES = ("router", "scan", "scatter", "gemm_up", "gemm_down", "combine")
@@ -79,6 +88,18 @@ SIGNATURES = {
     "mxm_moe_set_profiling": (ctypes.c_int, [ctypes.c_int64, ctypes.c_int]),
     "mxm_moe_stage_times": (ctypes.c_int, [ctypes.c_int64, _F32P, ctypes.c_int]),
     "mxm_moe_info": (ctypes.c_int, [ctypes.c_int64, _I64P, ctypes.c_int]),
+    "mxm_resnorm_create": (ctypes.c_int64, [_I64P, ctypes.c_int, ctypes.c_float, ctypes.c_int64]),
+    "mxm_resnorm_destroy": (ctypes.c_int, [ctypes.c_int64]),
+    "mxm_resnorm_forward": (ctypes.c_int, [ctypes.c_int64, ctypes.c_int64] + [_VP] * 8),
+    "mxm_resnorm_backward": (ctypes.c_int, [ctypes.c_int64, ctypes.c_int64] + [_VP] * 14),
+    "mxm_grads_create": (ctypes.c_int64, [_I64P, _I32P, _F32P, ctypes.c_int, ctypes.c_int64]),
+    "mxm_grads_destroy": (ctypes.c_int, [ctypes.c_int64]),
+    "mxm_grads_bind": (ctypes.c_int, [ctypes.c_int64] + [ctypes.POINTER(_VP)] * 6),
+    "mxm_grads_norm": (ctypes.c_int, [ctypes.c_int64, _VP]),
+    "mxm_grads_clip": (ctypes.c_int, [ctypes.c_int64, ctypes.c_double, _VP]),
+    "mxm_grads_adamw": (ctypes.c_int, [ctypes.c_int64] + [ctypes.c_double] * 6 + [_VP] * 3),
+    "mxm_stream": (ctypes.c_int, [ctypes.c_int64, ctypes.POINTER(_VP)]),
+    "mxm_synchronize": (ctypes.c_int, [ctypes.c_int64]),
 }
 
 _lib = None

@@ -29,6 +29,9 @@ SOURCES = [
     "mxm_prep.hip",
     "mxm_block.hip",
     "mxm_backward.hip",
+    "mxm_resnorm.hip",
+    "mxm_optim.hip",
+    "mxm_train.hip",
     "mxm_abi.hip",
 ]
 ARCH = os.environ.get("MIXMOE_OFFLOAD_ARCH", "gfx950")

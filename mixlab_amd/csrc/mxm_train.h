@@ -1,0 +1,95 @@
+// Kernels around the MoE op's training step and its residual stream: the
+// residual norm (mxm_resnorm.hip) and the gradient set's norm, clipping and
+// AdamW step (mxm_optim.hip).  mxm_train.hip owns every buffer; these structs
+// carry raw device pointers.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "mxm_numerics.h"
+
+// ---- residual norm ----
+//
+// Row n, channel d; stream x, branch delta, all sums in fp32:
+//   rp = 1 / sqrt(mean_d(delta^2) + eps)           (post norm; else 1)
+//   z = delta * rp,  f = scale * post,  a = gate or sigmoid(gate) of row n / gate_rows
+//   h = x + a * f * z                              rounded to the stream's type
+//   rn = 1 / sqrt(mean_d(h^2) + eps),  y = h * rn * w     of the rounded h
+// and backwards, given dh and dy:
+//   u = w * dy,  t = dh + rn * u - h * rn^3 * mean_d(u * h)
+//   dx = t,  dw = sum_n dy * h * rn
+//   e = t * a * f,  d_delta = rp * e - delta * rp^3 * mean_d(e * delta)  (post norm; else e)
+//   q = t * z,  d_scale = post * sum_n a q,  d_post = scale * sum_n a q,
+//   d_gate = a' * sum over the gate's rows (and over d, for a gate per row) of f q
+struct ResNormArgs {
+  int N, D;
+  float eps, inv_d;                     // inv_d = (float)(1.0 / D)
+  bool branch, post_norm, norm, sigmoid;
+  bool x_bf16, delta_bf16, y_bf16, p_bf16, g_bf16;  // stream, branch, y, scales and gate, gradients
+  int gate;                             // 0 none, 1 one value per row, 2 one per channel
+  int gate_rows;                        // rows of x per row of the gate
+  const void *x, *delta;                // [N, D]; x unused backwards
+  const void *post, *scale, *w, *gatep; // [D] each (null: ones), gate [ceil(N / gate_rows)][1 or D]
+  void* h;                              // [N, D]: out forwards, in backwards
+  void* y;                              // [N, D]
+  // backward
+  const void *dh, *dy;                  // [N, D]; dh null: zeros
+  void *dx, *d_delta;                   // [N, D]
+  float *d_post, *d_scale, *d_w, *d_gate;  // null: not wanted
+  // Column sums go over chunks of rows: part [2][chunks][D] (w, then a q) and
+  // gate_part [chunks][D] for gates per channel whose rows span several chunks.
+  float *part, *gate_part;
+  int chunks, chunk_rows;  // chunk c: rows c * chunk_rows ..., within one group of
+  int group_chunks;        // gate rows if group_chunks > 0 (chunks per group), else whole groups
+};
+void mxm_launch_resnorm(const ResNormArgs& a, hipStream_t s);
+void mxm_launch_resnorm_bw(const ResNormArgs& a, hipStream_t s);
+// The rows per chunk, chunks and chunks per group of a backward of N rows.
+void mxm_resnorm_plan(ResNormArgs& a, int n_cu);
+// Most chunks of any backward of up to max_rows rows.
+int64_t mxm_resnorm_max_chunks(int64_t max_rows, int D, int gate, int gate_rows, int n_cu);
+
+// ---- gradient sets ----
+struct GradTensor {
+  const void* g;      // gradients, fp32 or bf16
+  void* clipped;      // where clip writes (g itself: in place)
+  float *p, *m, *v;
+  uint16_t* p16;      // bf16 copy of p, or null
+  int64_t n;
+  float decay;        // multiplies the call's weight decay
+  int32_t bf16;       // the gradients' type
+};
+struct GradChunk {
+  int32_t tensor;
+  int32_t count;      // elements
+  int64_t start;      // first element in its tensor
+};
+// What the norm leaves for the launches after it.
+struct GradScalars {
+  float coef;         // multiplies every gradient
+  float step_size;    // lr / (1 - beta1^t)
+  float root2;        // 1 / sqrt(1 - beta2^t)
+  int32_t skip;       // the norm is not finite
+};
+struct GradArgs {
+  const GradTensor* tensors;
+  const GradChunk* chunks;
+  int n_chunks;
+  double* partial;       // [n_chunks or fewer]
+  int32_t* ticket;       // zero between calls
+  GradScalars* scalars;
+  double max_norm;       // 0: no clipping
+  float* norm;           // or null
+  // AdamW
+  bool adamw;
+  int64_t* step;
+  int32_t* skipped;      // or null
+  // (in 64 bits: 1 - beta in 32 loses digits for beta next to 1)
+  double lr, beta1, beta2, eps, weight_decay;
+};
+int mxm_grad_chunk_elems(int64_t total, int n_cu);
+int mxm_grad_norm_blocks(int n_chunks);
+void mxm_launch_grad_norm(const GradArgs& a, hipStream_t s);
+void mxm_launch_grad_clip(const GradArgs& a, hipStream_t s);
+void mxm_launch_grad_adamw(const GradArgs& a, hipStream_t s);
