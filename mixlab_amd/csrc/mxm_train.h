@@ -51,19 +51,16 @@ void mxm_resnorm_plan(ResNormArgs& a, int n_cu);
 int64_t mxm_resnorm_max_chunks(int64_t max_rows, int D, int gate, int gate_rows, int n_cu);
 
 // ---- gradient sets ----
-struct GradTensor {
+// A piece of one tensor, with where it is (a launch reads one descriptor and
+// then the data).
+struct GradChunk {
   const void* g;      // gradients, fp32 or bf16
   void* clipped;      // where clip writes (g itself: in place)
   float *p, *m, *v;
   uint16_t* p16;      // bf16 copy of p, or null
-  int64_t n;
-  float decay;        // multiplies the call's weight decay
-  int32_t bf16;       // the gradients' type
-};
-struct GradChunk {
-  int32_t tensor;
   int32_t count;      // elements
-  int64_t start;      // first element in its tensor
+  float decay;        // multiplies the call's weight decay
+  int64_t bf16;       // the gradients' type
 };
 // What the norm leaves for the launches after it.
 struct GradScalars {
@@ -73,7 +70,6 @@ struct GradScalars {
   int32_t skip;       // the norm is not finite
 };
 struct GradArgs {
-  const GradTensor* tensors;
   const GradChunk* chunks;
   int n_chunks;
   double* partial;       // [n_chunks or fewer]

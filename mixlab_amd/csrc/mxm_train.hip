@@ -3,6 +3,7 @@
 // the op's handles (mxm_abi.hip): int64 handles, status codes, an exception
 // fence around every entry point; every argument is checked before the device
 // is touched.
+#include <algorithm>
 #include <cmath>
 #include <map>
 #include <mutex>
@@ -33,9 +34,15 @@ struct ResNorm : TrainHandle {
 };
 
 struct GradSet : TrainHandle {
-  std::vector<GradTensor> tensors;
+  struct Tensor {
+    int64_t n;
+    bool bf16;
+    float decay;
+  };
+  std::vector<Tensor> tensors;
+  int64_t chunk_elems = 0;
   GradArgs base{};
-  DevBuf table, chunks, partial, small;  // small: ticket, then the scalars at byte 64
+  DevBuf chunks, partial, small;  // small: ticket, then the scalars at byte 64
   bool bound = false, has_params = false;
   ~GradSet() override {
     if (stream_ref) (void)hipStreamSynchronize(stream());
@@ -333,30 +340,21 @@ int64_t mxm_grads_create(const int64_t* sizes, const int32_t* dtypes, const floa
     g->stream_ref = choose_stream(shared);
     g->n_cu = cu_count(g->stream_ref->device);
     const int64_t per = mxm_grad_chunk_elems(total, g->n_cu);
-    std::vector<GradChunk> chunks;
+    int64_t pieces = 0;
     for (int i = 0; i < n; ++i) {
-      GradTensor t{};
-      t.n = sizes[i];
-      t.bf16 = dtypes[i] == MXM_DTYPE_BF16;
-      t.decay = decay ? decay[i] : 1.0f;
-      g->tensors.push_back(t);
-      for (int64_t at = 0; at < sizes[i]; at += per)
-        chunks.push_back({i, (int32_t)(sizes[i] - at < per ? sizes[i] - at : per), at});
+      g->tensors.push_back({sizes[i], dtypes[i] == MXM_DTYPE_BF16, decay ? decay[i] : 1.0f});
+      pieces += (sizes[i] + per - 1) / per;
     }
-    if (chunks.size() > (size_t)INT32_MAX)
-      fail(GRADSET " too many pieces (%zu)", chunks.size());
-    g->table.alloc(g->tensors.size() * sizeof(GradTensor));
-    g->chunks.alloc(chunks.size() * sizeof(GradChunk));
-    g->partial.alloc((size_t)mxm_grad_norm_blocks((int)chunks.size()) * sizeof(double));
+    if (pieces > INT32_MAX) fail(GRADSET " too many pieces (%lld)", (long long)pieces);
+    g->chunk_elems = per;
+    g->chunks.alloc((size_t)pieces * sizeof(GradChunk));
+    g->partial.alloc((size_t)mxm_grad_norm_blocks((int)pieces) * sizeof(double));
     g->small.alloc(256);
-    HIPCK(hipMemcpyAsync(g->chunks.p, chunks.data(), chunks.size() * sizeof(GradChunk),
-                         hipMemcpyHostToDevice, g->stream()));
     HIPCK(hipMemsetAsync(g->small.p, 0, 256, g->stream()));
     HIPCK(hipStreamSynchronize(g->stream()));
     GradArgs& a = g->base;
-    a.tensors = g->table.as<GradTensor>();
     a.chunks = g->chunks.as<GradChunk>();
-    a.n_chunks = (int)chunks.size();
+    a.n_chunks = (int)pieces;
     a.partial = g->partial.as<double>();
     a.ticket = g->small.as<int32_t>();
     a.scalars = reinterpret_cast<GradScalars*>(g->small.as<char>() + 64);
@@ -376,39 +374,49 @@ int mxm_grads_bind(int64_t h, const void* const* grads, void* const* clipped, vo
     if ((params != nullptr) != (m != nullptr) || (params != nullptr) != (v != nullptr))
       fail(GRADSET " params, m and v are bound together");
     if (params_bf16 && !params) fail(GRADSET " params_bf16 needs params");
-    std::vector<GradTensor> t = g->tensors;
-    for (size_t i = 0; i < t.size(); ++i) {
-      auto take = [&](const char* name, const void* p, bool bf16) {
-        if (t[i].n == 0) return;
+    std::vector<GradChunk> chunks;
+    chunks.reserve((size_t)g->base.n_chunks);
+    for (size_t i = 0; i < g->tensors.size(); ++i) {
+      const GradSet::Tensor& t = g->tensors[i];
+      if (t.n == 0) continue;
+      // tensor i's pointer in a list (null: the list is not bound)
+      auto take = [&](const char* name, const void* const* list, bool bf16) {
+        if (!list) return (char*)nullptr;
+        const void* p = list[i];
         if (!p) fail(GRADSET " tensor %zu: %s is NULL", i, name);
         if (reinterpret_cast<uintptr_t>(p) % (bf16 ? 2 : 4) != 0)
           fail(GRADSET " tensor %zu: %s is not aligned to its elements", i, name);
+        return static_cast<char*>(const_cast<void*>(p));
       };
-      t[i].g = grads[i];
-      take("grads", t[i].g, t[i].bf16);
-      t[i].clipped = clipped ? clipped[i] : const_cast<void*>(grads[i]);
-      take("clipped", t[i].clipped, t[i].bf16);
-      t[i].p = t[i].m = t[i].v = nullptr;
-      t[i].p16 = nullptr;
-      if (params) {
-        take("params", params[i], false);
-        take("m", m[i], false);
-        take("v", v[i], false);
-        t[i].p = static_cast<float*>(params[i]);
-        t[i].m = static_cast<float*>(m[i]);
-        t[i].v = static_cast<float*>(v[i]);
-      }
-      if (params_bf16) {
-        take("params_bf16", params_bf16[i], true);
-        t[i].p16 = static_cast<uint16_t*>(params_bf16[i]);
+      char* const gp = take("grads", grads, t.bf16);
+      char* const cp = clipped ? take("clipped", clipped, t.bf16) : gp;
+      char* const pp = take("params", params, false);
+      char* const mp = take("m", m, false);
+      char* const vp = take("v", v, false);
+      char* const hp = take("params_bf16", params_bf16, true);
+      for (int64_t at = 0; at < t.n; at += g->chunk_elems) {
+        const int64_t wide = at * 4, own = at * (t.bf16 ? 2 : 4);
+        GradChunk c{};
+        c.g = gp + own;
+        c.clipped = cp + own;
+        if (pp) {
+          c.p = reinterpret_cast<float*>(pp + wide);
+          c.m = reinterpret_cast<float*>(mp + wide);
+          c.v = reinterpret_cast<float*>(vp + wide);
+        }
+        if (hp) c.p16 = reinterpret_cast<uint16_t*>(hp + at * 2);
+        c.count = (int32_t)std::min(t.n - at, g->chunk_elems);
+        c.decay = t.decay;
+        c.bf16 = t.bf16;
+        chunks.push_back(c);
       }
     }
     const DeviceGuard guard(g->stream_ref->device);
     // (waits for the calls that read the table, then for the copy)
-    HIPCK(hipMemcpyAsync(g->table.p, t.data(), t.size() * sizeof(GradTensor), hipMemcpyHostToDevice,
-                         g->stream()));
+    if (!chunks.empty())
+      HIPCK(hipMemcpyAsync(g->chunks.p, chunks.data(), chunks.size() * sizeof(GradChunk),
+                           hipMemcpyHostToDevice, g->stream()));
     HIPCK(hipStreamSynchronize(g->stream()));
-    g->tensors = std::move(t);
     g->bound = true;
     g->has_params = params != nullptr;
     return MXM_OK;
