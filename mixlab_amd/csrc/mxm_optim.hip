@@ -108,8 +108,14 @@ __device__ __forceinline__ void finish_norm(const GradArgs& a, double total) {
   *a.scalars = r;
 }
 
-// The squares of whole chunks per workgroup; the last workgroup to finish adds
-// the workgroups' sums in their order.
+// The squares of whole chunks per workgroup, one sum each.  Up to TICKET_BLOCKS
+// workgroups the last one to finish adds them; past that a second launch does:
+// every ticket costs about 45 ns (its release writes an L2 back), one after the
+// other.  Ticket / second launch at 32 workgroups 3.9 / 5.4 us, at 64 6.5 /
+// 6.7, at 256 8.1 / 5.3, and for 805 MB (2048 / 1024 workgroups) 213 / 119 us,
+// which is 6.8 TB/s.
+constexpr int TICKET_BLOCKS = 32, MOST_BLOCKS = 1024;
+
 __global__ __launch_bounds__(THREADS) void grad_norm_kernel(GradArgs a) {
   __shared__ double red[THREADS / 64];
   __shared__ int s_last;
@@ -124,7 +130,7 @@ __global__ __launch_bounds__(THREADS) void grad_norm_kernel(GradArgs a) {
     if (bf) {
       const u4* g = reinterpret_cast<const u4*>(static_cast<const uint16_t*>(k.g) + head);
       u4 w[UNROLL];
-      each_vector(n, [&](int i, int j) { w[j] = g[i]; },
+      each_vector(n, [&](int i, int j) { w[j] = __builtin_nontemporal_load(g + i); },
                   [&](int, int j) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
@@ -135,7 +141,7 @@ __global__ __launch_bounds__(THREADS) void grad_norm_kernel(GradArgs a) {
     } else {
       const f4* g = reinterpret_cast<const f4*>(static_cast<const float*>(k.g) + head);
       f4 w[UNROLL];
-      each_vector(n, [&](int i, int j) { w[j] = g[i]; },
+      each_vector(n, [&](int i, int j) { w[j] = __builtin_nontemporal_load(g + i); },
                   [&](int, int j) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) add(w[j][e]);
@@ -144,6 +150,10 @@ __global__ __launch_bounds__(THREADS) void grad_norm_kernel(GradArgs a) {
     each_rest(head, head + n * V, k.count, [&](int i) { add(grad_at(k.g, bf, i)); });
   }
   s = block_sum(s, red);
+  if (gridDim.x > TICKET_BLOCKS) {
+    if (threadIdx.x == 0) a.partial[blockIdx.x] = s;
+    return;
+  }
   // One thread stores the sum and takes the ticket, so the ticket's release
   // covers its store; the last workgroup's acquire covers everybody's.
   if (threadIdx.x == 0) {
@@ -154,8 +164,8 @@ __global__ __launch_bounds__(THREADS) void grad_norm_kernel(GradArgs a) {
   __syncthreads();
   if (!s_last) return;
   s = 0.0;
-  for (int b = threadIdx.x; b < (int)gridDim.x; b += THREADS)
-    s += __hip_atomic_load(a.partial + b, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  if (threadIdx.x < gridDim.x)
+    s = __hip_atomic_load(a.partial + threadIdx.x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   s = block_sum(s, red);
   if (threadIdx.x == 0) {
     finish_norm(a, s);
@@ -163,44 +173,65 @@ __global__ __launch_bounds__(THREADS) void grad_norm_kernel(GradArgs a) {
   }
 }
 
-// (Clip and AdamW walk the chunks backwards: what the norm read last is what the
-// last-level cache still holds.)
+// Adds the workgroups' sums in their order.
+__global__ __launch_bounds__(THREADS) void grad_norm_finish_kernel(GradArgs a, int blocks) {
+  __shared__ double red[THREADS / 64];
+  double s = 0.0;
+  for (int b = threadIdx.x; b < blocks; b += THREADS) s += a.partial[b];
+  s = block_sum(s, red);
+  if (threadIdx.x == 0) finish_norm(a, s);
+}
+
+// Clip and AdamW run one vector a thread and no loop: every workgroup takes one
+// slice of THREADS vectors of a chunk, the last slices first (what the norm
+// read last is what the last-level cache still holds).  Streams of such short
+// workgroups in address order, past the caches' usual replacement, reach 6.1
+// (AdamW) and 6.6 TB/s (one tensor in, one out) over 1 GiB tensors; workgroups
+// that stay and loop over chunks 5.1-5.4 and 5.3-5.7.
+struct Slice {
+  int head, n, at;  // scalar elements in front, vectors, this thread's vector
+};
+__device__ __forceinline__ Slice slice_of(int head, int count, int V, int sub) {
+  return {head, (count - head) / V, sub * THREADS + (int)threadIdx.x};
+}
+// f(i) for the elements outside the chunk's vectors, spread over its slices.
+template <class F>
+__device__ __forceinline__ void each_other(const Slice& s, int V, int count, int slices, F f) {
+  for (int i = s.at; i < s.head; i += slices * THREADS) f(i);
+  for (int i = s.head + s.n * V + s.at; i < count; i += slices * THREADS) f(i);
+}
+
 __global__ __launch_bounds__(THREADS) void grad_clip_kernel(GradArgs a) {
+  const int b = (int)gridDim.x - 1 - (int)blockIdx.x;
+  const GradChunk k = a.chunks[b / a.slices];
   const float coef = a.scalars->coef;
-  for (int c = a.n_chunks - 1 - (int)blockIdx.x; c >= 0; c -= gridDim.x) {
-    const GradChunk k = a.chunks[c];
-    const bool bf = k.bf16 != 0;
-    const int V = bf ? 8 : 4, size = bf ? 2 : 4;
-    int head = min(head_of(k.g, size, V), k.count);
-    if (!meets(k.clipped, size, V, head)) head = k.count;
-    const int n = (k.count - head) / V;
+  const bool bf = k.bf16 != 0;
+  const int V = bf ? 8 : 4, size = bf ? 2 : 4;
+  int head = min(head_of(k.g, size, V), k.count);
+  if (!meets(k.clipped, size, V, head)) head = k.count;
+  const Slice s = slice_of(head, k.count, V, b % a.slices);
+  if (s.at < s.n) {
     if (bf) {
       const u4* g = reinterpret_cast<const u4*>(static_cast<const uint16_t*>(k.g) + head);
       u4* out = reinterpret_cast<u4*>(static_cast<uint16_t*>(k.clipped) + head);
-      u4 w[UNROLL];
-      each_vector(n, [&](int i, int j) { w[j] = g[i]; },
-                  [&](int i, int j) {
-                    u4 r;
+      const u4 w = __builtin_nontemporal_load(g + s.at);
+      u4 r;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                      r[e] = (uint32_t)mxm_f2bf(lo16(w[j][e]) * coef) |
-                             (uint32_t)mxm_f2bf(hi16(w[j][e]) * coef) << 16;
-                    out[i] = r;
-                  });
+      for (int e = 0; e < 4; ++e) r[e] = mxm_pack_bf2_fast(lo16(w[e]) * coef, hi16(w[e]) * coef);
+      __builtin_nontemporal_store(r, out + s.at);
     } else {
       const f4* g = reinterpret_cast<const f4*>(static_cast<const float*>(k.g) + head);
       f4* out = reinterpret_cast<f4*>(static_cast<float*>(k.clipped) + head);
-      f4 w[UNROLL];
-      each_vector(n, [&](int i, int j) { w[j] = g[i]; }, [&](int i, int j) { out[i] = w[j] * coef; });
+      __builtin_nontemporal_store(__builtin_nontemporal_load(g + s.at) * coef, out + s.at);
     }
-    each_rest(head, head + n * V, k.count, [&](int i) {
-      const float g = grad_at(k.g, bf, i) * coef;
-      if (bf)
-        static_cast<uint16_t*>(k.clipped)[i] = mxm_f2bf(g);
-      else
-        static_cast<float*>(k.clipped)[i] = g;
-    });
   }
+  each_other(s, V, k.count, a.slices, [&](int i) {
+    const float g = grad_at(k.g, bf, i) * coef;
+    if (bf)
+      static_cast<uint16_t*>(k.clipped)[i] = mxm_f2bf(g);
+    else
+      static_cast<float*>(k.clipped)[i] = g;
+  });
 }
 
 struct AdamScalars {
@@ -215,51 +246,59 @@ __device__ __forceinline__ void adamw_one(const AdamScalars& r, float g, float& 
   p = p - __builtin_fmaf(r.decay, p, u);
 }
 
-template <bool BF>
-__device__ __forceinline__ void adamw_chunk(const GradChunk& k, const AdamScalars& r) {
+__global__ __launch_bounds__(THREADS) void grad_adamw_kernel(GradArgs a) {
+  const int b = (int)gridDim.x - 1 - (int)blockIdx.x;
+  const GradChunk k = a.chunks[b / a.slices];
+  const GradScalars sc = *a.scalars;
+  if (sc.skip) return;
+  const bool bf = k.bf16 != 0;
   int head = min(head_of(k.p, 4, 4), k.count);
-  if (!meets(k.m, 4, 4, head) || !meets(k.v, 4, 4, head) || !meets(k.g, BF ? 2 : 4, 4, head) ||
+  if (!meets(k.m, 4, 4, head) || !meets(k.v, 4, 4, head) || !meets(k.g, bf ? 2 : 4, 4, head) ||
       (k.p16 && !meets(k.p16, 2, 4, head)))
     head = k.count;
-  const int n = (k.count - head) / 4;
-  f4 *p = reinterpret_cast<f4*>(k.p + head), *m = reinterpret_cast<f4*>(k.m + head),
-     *v = reinterpret_cast<f4*>(k.v + head);
-  u2* p16 = k.p16 ? reinterpret_cast<u2*>(k.p16 + head) : nullptr;
-  const f4* g32 = reinterpret_cast<const f4*>(static_cast<const float*>(k.g) + head);
-  const u2* g16 = reinterpret_cast<const u2*>(static_cast<const uint16_t*>(k.g) + head);
-  f4 wp[UNROLL], wm[UNROLL], wv[UNROLL], wg[UNROLL];
-  u2 wh[UNROLL];
-  each_vector(n,
-              [&](int i, int j) {
-                if (BF)
-                  wh[j] = g16[i];
-                else
-                  wg[j] = g32[i];
-                wm[j] = m[i];
-                wv[j] = v[i];
-                wp[j] = p[i];
-              },
-              [&](int i, int j) {
-                f4 g = wg[j];
-                if (BF) g = f4{lo16(wh[j][0]), hi16(wh[j][0]), lo16(wh[j][1]), hi16(wh[j][1])};
+  const Slice s = slice_of(head, k.count, 4, b % a.slices);
+  AdamScalars r;
+  r.coef = sc.coef;
+  r.step_size = sc.step_size;
+  r.root2 = sc.root2;
+  r.b1 = a.b1;
+  r.c1 = a.c1;
+  r.b2 = a.b2;
+  r.c2 = a.c2;
+  r.eps = a.eps32;
+  r.decay = a.lr_decay * k.decay;
+  if (s.at < s.n) {
+    f4 *pp = reinterpret_cast<f4*>(k.p + head) + s.at, *mp = reinterpret_cast<f4*>(k.m + head) + s.at,
+       *vp = reinterpret_cast<f4*>(k.v + head) + s.at;
+    f4 g;
+    if (bf) {
+      const u2 w = __builtin_nontemporal_load(
+          reinterpret_cast<const u2*>(static_cast<const uint16_t*>(k.g) + head) + s.at);
+      g = f4{lo16(w[0]), hi16(w[0]), lo16(w[1]), hi16(w[1])};
+    } else {
+      g = __builtin_nontemporal_load(
+          reinterpret_cast<const f4*>(static_cast<const float*>(k.g) + head) + s.at);
+    }
+    f4 m = __builtin_nontemporal_load(mp), v = __builtin_nontemporal_load(vp),
+       p = __builtin_nontemporal_load(pp);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                  float pe = wp[j][e], me = wm[j][e], ve = wv[j][e];
-                  adamw_one(r, g[e], pe, me, ve);
-                  wp[j][e] = pe;
-                  wm[j][e] = me;
-                  wv[j][e] = ve;
-                }
-                m[i] = wm[j];
-                v[i] = wv[j];
-                p[i] = wp[j];
-                if (p16)
-                  p16[i] = u2{mxm_pack_bf2_fast(wp[j][0], wp[j][1]),
-                              mxm_pack_bf2_fast(wp[j][2], wp[j][3])};
-              });
-  each_rest(head, head + n * 4, k.count, [&](int i) {
+    for (int e = 0; e < 4; ++e) {
+      float pe = p[e], me = m[e], ve = v[e];
+      adamw_one(r, g[e], pe, me, ve);
+      p[e] = pe;
+      m[e] = me;
+      v[e] = ve;
+    }
+    __builtin_nontemporal_store(m, mp);
+    __builtin_nontemporal_store(v, vp);
+    __builtin_nontemporal_store(p, pp);
+    if (k.p16)
+      __builtin_nontemporal_store(u2{mxm_pack_bf2_fast(p[0], p[1]), mxm_pack_bf2_fast(p[2], p[3])},
+                                  reinterpret_cast<u2*>(k.p16 + head) + s.at);
+  }
+  each_other(s, 4, k.count, a.slices, [&](int i) {
     float p = k.p[i], m = k.m[i], v = k.v[i];
-    adamw_one(r, grad_at(k.g, BF, i), p, m, v);
+    adamw_one(r, grad_at(k.g, bf, i), p, m, v);
     k.m[i] = m;
     k.v[i] = v;
     k.p[i] = p;
@@ -267,49 +306,39 @@ __device__ __forceinline__ void adamw_chunk(const GradChunk& k, const AdamScalar
   });
 }
 
-__global__ __launch_bounds__(THREADS) void grad_adamw_kernel(GradArgs a) {
-  const GradScalars s = *a.scalars;
-  if (s.skip) return;
-  AdamScalars r;
-  r.coef = s.coef;
-  r.step_size = s.step_size;
-  r.root2 = s.root2;
-  r.b1 = (float)a.beta1;
-  r.c1 = (float)(1.0 - a.beta1);
-  r.b2 = (float)a.beta2;
-  r.c2 = (float)(1.0 - a.beta2);
-  r.eps = (float)a.eps;
-  for (int c = a.n_chunks - 1 - (int)blockIdx.x; c >= 0; c -= gridDim.x) {
-    const GradChunk k = a.chunks[c];
-    r.decay = (float)(a.lr * a.weight_decay * (double)k.decay);
-    if (k.bf16)
-      adamw_chunk<true>(k, r);
-    else
-      adamw_chunk<false>(k, r);
-  }
-}
-
 }  // namespace
 
-// Pieces of about an eighth of a CU's share, in whole rounds of the workgroups'
-// vectors.
+// Pieces that still make eight workgroups a CU for the norm, and at most 64 KB of
+// fp32.
 int mxm_grad_chunk_elems(int64_t total, int n_cu) {
-  constexpr int64_t round = THREADS * 4 * UNROLL;
-  const int64_t share = total / (8 * (int64_t)n_cu);
-  const int64_t rounds = (share + round - 1) / round;
-  return (int)(round * std::max<int64_t>(1, std::min<int64_t>(rounds, 8)));
+  int64_t per = 4096;
+  while (per < 16384 && total / (per * 2) >= 8 * (int64_t)n_cu) per *= 2;
+  return (int)per;
 }
 
-int mxm_grad_norm_blocks(int n_chunks) { return std::max(1, std::min(n_chunks, 2048)); }
+int mxm_grad_norm_blocks(int n_chunks) { return std::max(1, std::min(n_chunks, MOST_BLOCKS)); }
 
 void mxm_launch_grad_norm(const GradArgs& a, hipStream_t s) {
-  hipLaunchKernelGGL(grad_norm_kernel, dim3(mxm_grad_norm_blocks(a.n_chunks)), dim3(THREADS), 0, s, a);
+  const int blocks = mxm_grad_norm_blocks(a.n_chunks);
+  hipLaunchKernelGGL(grad_norm_kernel, dim3(blocks), dim3(THREADS), 0, s, a);
+  if (blocks > TICKET_BLOCKS)
+    hipLaunchKernelGGL(grad_norm_finish_kernel, dim3(1), dim3(THREADS), 0, s, a, blocks);
 }
-void mxm_launch_grad_clip(const GradArgs& a, hipStream_t s) {
+void mxm_launch_grad_clip(const GradArgs& args, hipStream_t s) {
+  GradArgs a = args;
+  a.slices = a.chunk_elems / (THREADS * (a.all_bf16 ? 8 : 4));
   if (a.n_chunks > 0)
-    hipLaunchKernelGGL(grad_clip_kernel, dim3(std::min(a.n_chunks, 2048)), dim3(THREADS), 0, s, a);
+    hipLaunchKernelGGL(grad_clip_kernel, dim3(a.n_chunks * a.slices), dim3(THREADS), 0, s, a);
 }
-void mxm_launch_grad_adamw(const GradArgs& a, hipStream_t s) {
+void mxm_launch_grad_adamw(const GradArgs& args, hipStream_t s) {
+  GradArgs a = args;
+  a.slices = a.chunk_elems / (THREADS * 4);
+  a.b1 = (float)a.beta1;
+  a.c1 = (float)(1.0 - a.beta1);
+  a.b2 = (float)a.beta2;
+  a.c2 = (float)(1.0 - a.beta2);
+  a.eps32 = (float)a.eps;
+  a.lr_decay = (float)(a.lr * a.weight_decay);
   if (a.n_chunks > 0)
-    hipLaunchKernelGGL(grad_adamw_kernel, dim3(std::min(a.n_chunks, 2048)), dim3(THREADS), 0, s, a);
+    hipLaunchKernelGGL(grad_adamw_kernel, dim3(a.n_chunks * a.slices), dim3(THREADS), 0, s, a);
 }

@@ -72,6 +72,9 @@ struct GradScalars {
 struct GradArgs {
   const GradChunk* chunks;
   int n_chunks;
+  int chunk_elems;       // elements of a chunk (a tensor's last one may be shorter)
+  bool all_bf16;         // every tensor's gradients are bf16
+  int slices;            // workgroups per chunk (set by the launchers of clip and AdamW)
   double* partial;       // [n_chunks or fewer]
   int32_t* ticket;       // zero between calls
   GradScalars* scalars;
@@ -83,6 +86,7 @@ struct GradArgs {
   int32_t* skipped;      // or null
   // (in 64 bits: 1 - beta in 32 loses digits for beta next to 1)
   double lr, beta1, beta2, eps, weight_decay;
+  float b1, c1, b2, c2, eps32, lr_decay;  // set by the launcher: c = 1 - b
 };
 int mxm_grad_chunk_elems(int64_t total, int n_cu);
 int mxm_grad_norm_blocks(int n_chunks);

@@ -40,7 +40,6 @@ struct GradSet : TrainHandle {
     float decay;
   };
   std::vector<Tensor> tensors;
-  int64_t chunk_elems = 0;
   GradArgs base{};
   DevBuf chunks, partial, small;  // small: ticket, then the scalars at byte 64
   bool bound = false, has_params = false;
@@ -345,8 +344,8 @@ int64_t mxm_grads_create(const int64_t* sizes, const int32_t* dtypes, const floa
       g->tensors.push_back({sizes[i], dtypes[i] == MXM_DTYPE_BF16, decay ? decay[i] : 1.0f});
       pieces += (sizes[i] + per - 1) / per;
     }
-    if (pieces > INT32_MAX) fail(GRADSET " too many pieces (%lld)", (long long)pieces);
-    g->chunk_elems = per;
+    // (a launch's workgroups, at most 16 a piece, are counted in 31 bits)
+    if (pieces > (INT32_MAX >> 4)) fail(GRADSET " too many pieces (%lld)", (long long)pieces);
     g->chunks.alloc((size_t)pieces * sizeof(GradChunk));
     g->partial.alloc((size_t)mxm_grad_norm_blocks((int)pieces) * sizeof(double));
     g->small.alloc(256);
@@ -355,6 +354,9 @@ int64_t mxm_grads_create(const int64_t* sizes, const int32_t* dtypes, const floa
     GradArgs& a = g->base;
     a.chunks = g->chunks.as<GradChunk>();
     a.n_chunks = (int)pieces;
+    a.chunk_elems = (int)per;
+    a.all_bf16 = true;
+    for (const auto& t : g->tensors) a.all_bf16 = a.all_bf16 && t.bf16;
     a.partial = g->partial.as<double>();
     a.ticket = g->small.as<int32_t>();
     a.scalars = reinterpret_cast<GradScalars*>(g->small.as<char>() + 64);
@@ -374,6 +376,7 @@ int mxm_grads_bind(int64_t h, const void* const* grads, void* const* clipped, vo
     if ((params != nullptr) != (m != nullptr) || (params != nullptr) != (v != nullptr))
       fail(GRADSET " params, m and v are bound together");
     if (params_bf16 && !params) fail(GRADSET " params_bf16 needs params");
+    const int64_t per = g->base.chunk_elems;
     std::vector<GradChunk> chunks;
     chunks.reserve((size_t)g->base.n_chunks);
     for (size_t i = 0; i < g->tensors.size(); ++i) {
@@ -394,7 +397,7 @@ int mxm_grads_bind(int64_t h, const void* const* grads, void* const* clipped, vo
       char* const mp = take("m", m, false);
       char* const vp = take("v", v, false);
       char* const hp = take("params_bf16", params_bf16, true);
-      for (int64_t at = 0; at < t.n; at += g->chunk_elems) {
+      for (int64_t at = 0; at < t.n; at += per) {
         const int64_t wide = at * 4, own = at * (t.bf16 ? 2 : 4);
         GradChunk c{};
         c.g = gp + own;
@@ -405,7 +408,7 @@ int mxm_grads_bind(int64_t h, const void* const* grads, void* const* clipped, vo
           c.v = reinterpret_cast<float*>(vp + wide);
         }
         if (hp) c.p16 = reinterpret_cast<uint16_t*>(hp + at * 2);
-        c.count = (int32_t)std::min(t.n - at, g->chunk_elems);
+        c.count = (int32_t)std::min(t.n - at, per);
         c.decay = t.decay;
         c.bf16 = t.bf16;
         chunks.push_back(c);
