@@ -30,6 +30,7 @@ SOURCES = [
     "mxm_block.hip",
     "mxm_backward.hip",
     "mxm_resnorm.hip",
+    "mxm_resnorm_bw.hip",
     "mxm_optim.hip",
     "mxm_train.hip",
     "mxm_abi.hip",

@@ -1,0 +1,134 @@
+// Shared by the residual norm's two directions: how a row lies in threads, typed
+// loads and stores, sums over a row.
+//
+// A row is held in registers from its one load to its last use.  V consecutive
+// elements (a 16-byte piece of fp32) lie in a thread, NV such vectors a thread;
+// LPR threads of a wave hold a row (rows side by side in the wave), or, with
+// LPR = 0, a workgroup of a row's length does.  V = 4 needs D % 4 == 0 and
+// aligned tensors; V = 1 takes any.
+#pragma once
+
+#include "mxm_kernels.h"
+#include "mxm_train.h"
+
+namespace resnorm {
+
+constexpr int THREADS = 256;  // of a workgroup that holds several rows
+
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+
+enum Kind { F32 = 0, BF16 = 1, ANY = 2 };  // ANY: `bf` says
+
+template <int K, int V>
+__device__ __forceinline__ void load(const void* p, bool bf, size_t i, float* out) {
+  if constexpr (V == 4) {
+    if (K == BF16) {
+      const u2 w = __builtin_nontemporal_load(
+          reinterpret_cast<const u2*>(static_cast<const uint16_t*>(p) + i));
+      out[0] = mxm_u2f(w[0] << 16);
+      out[1] = mxm_u2f(w[0] & 0xffff0000u);
+      out[2] = mxm_u2f(w[1] << 16);
+      out[3] = mxm_u2f(w[1] & 0xffff0000u);
+    } else {
+      const f4 w = __builtin_nontemporal_load(
+          reinterpret_cast<const f4*>(static_cast<const float*>(p) + i));
+#pragma unroll
+      for (int j = 0; j < 4; ++j) out[j] = w[j];
+    }
+  } else {
+    out[0] = bf ? mxm_bf2f(static_cast<const uint16_t*>(p)[i]) : static_cast<const float*>(p)[i];
+  }
+}
+
+// Rounds v to the type it is kept in; v holds the kept values afterwards.
+template <int K, int V>
+__device__ __forceinline__ void store(void* p, bool bf, size_t i, float* v) {
+  if constexpr (V == 4) {
+    if (K == BF16) {
+      const u2 w = {mxm_pack_bf2_fast(v[0], v[1]), mxm_pack_bf2_fast(v[2], v[3])};
+      __builtin_nontemporal_store(w, reinterpret_cast<u2*>(static_cast<uint16_t*>(p) + i));
+      v[0] = mxm_u2f(w[0] << 16);
+      v[1] = mxm_u2f(w[0] & 0xffff0000u);
+      v[2] = mxm_u2f(w[1] << 16);
+      v[3] = mxm_u2f(w[1] & 0xffff0000u);
+    } else {
+      __builtin_nontemporal_store(f4{v[0], v[1], v[2], v[3]},
+                                  reinterpret_cast<f4*>(static_cast<float*>(p) + i));
+    }
+  } else {
+    if (bf) {
+      const uint16_t b = mxm_f2bf(v[0]);
+      static_cast<uint16_t*>(p)[i] = b;
+      v[0] = mxm_bf2f(b);
+    } else {
+      static_cast<float*>(p)[i] = v[0];
+    }
+  }
+}
+
+// V values of a scale or a gate, which many rows read; null: ones.
+template <int V>
+__device__ __forceinline__ void load_scale(const void* p, bool bf, size_t i, float* out) {
+  if (!p) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) out[j] = 1.0f;
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < V; ++j)
+    out[j] = bf ? mxm_bf2f(static_cast<const uint16_t*>(p)[i + j])
+                : static_cast<const float*>(p)[i + j];
+}
+
+__device__ __forceinline__ float gate_of(const ResNormArgs& a, float g) {
+  return a.sigmoid ? mxm_sigmoid(g) : g;
+}
+
+// Sums of K values over a row's threads, in each of them.  LPR = 0: `red` holds
+// K floats a wave and is not written again before another barrier of the
+// workgroup (callers alternate buffers).
+template <int LPR, int K>
+__device__ __forceinline__ void row_sum(float (&v)[K], float* red) {
+#pragma unroll
+  for (int s = (LPR ? LPR : 64) / 2; s >= 1; s >>= 1)
+#pragma unroll
+    for (int k = 0; k < K; ++k) v[k] = v[k] + mxm_xor_lane_f(v[k], s);
+  if constexpr (LPR == 0) {
+    const int wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+    if ((threadIdx.x & 63) == 0)
+#pragma unroll
+      for (int k = 0; k < K; ++k) red[wave * K + k] = v[k];
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < K; ++k) v[k] = 0.0f;
+    for (int w = 0; w < waves; ++w)
+#pragma unroll
+      for (int k = 0; k < K; ++k) v[k] += red[w * K + k];
+  }
+}
+
+// How rows of D elements lie in threads.
+struct Shape {
+  int V, NV, lpr, threads;
+  int rows() const { return lpr ? threads / lpr : 1; }  // rows a workgroup holds at once
+};
+inline Shape shape_of(int D, bool vectors) {
+  if (vectors) {
+    if (D <= 64) return {4, 1, 16, THREADS};
+    if (D <= 128) return {4, 1, 32, THREADS};
+    if (D <= 256) return {4, 1, 64, THREADS};
+    if (D <= 512) return {4, 2, 64, THREADS};
+    const int nv = D <= 8192 ? 2 : 4;
+    return {4, nv, 0, (D + 4 * nv * 64 - 1) / (4 * nv * 64) * 64};
+  }
+  if (D <= 256) return {1, 4, 64, THREADS};
+  const int nv = D <= 4096 ? 4 : 16;
+  return {1, nv, 0, (D + nv * 64 - 1) / (nv * 64) * 64};
+}
+
+inline bool aligned(const void* p, bool bf16) {
+  return reinterpret_cast<uintptr_t>(p) % (bf16 ? 8 : 16) == 0;
+}
+
+}  // namespace resnorm

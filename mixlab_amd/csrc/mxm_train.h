@@ -37,18 +37,19 @@ struct ResNormArgs {
   const void *dh, *dy;                  // [N, D]; dh null: zeros
   void *dx, *d_delta;                   // [N, D]
   float *d_post, *d_scale, *d_w, *d_gate;  // null: not wanted
-  // Column sums go over chunks of rows: part [2][chunks][D] (w, then a q) and
-  // gate_part [chunks][D] for gates per channel whose rows span several chunks.
+  // Column sums go over chunks of rows: part [2][parts][D] (w, then a q; a part
+  // is a workgroup's chunks) and gate_part [chunks][1 or D] for gates whose rows
+  // span several chunks.  Set by the launcher.
   float *part, *gate_part;
-  int chunks, chunk_rows;  // chunk c: rows c * chunk_rows ..., within one group of
-  int group_chunks;        // gate rows if group_chunks > 0 (chunks per group), else whole groups
+  int chunks, parts, chunk_rows;  // (forwards chunk_rows: rows a thread walks)
+  int group_chunks;  // chunks per group of gate rows, each within one; 0: chunks of whole groups
+  int n_cu;
 };
 void mxm_launch_resnorm(const ResNormArgs& a, hipStream_t s);
 void mxm_launch_resnorm_bw(const ResNormArgs& a, hipStream_t s);
-// The rows per chunk, chunks and chunks per group of a backward of N rows.
-void mxm_resnorm_plan(ResNormArgs& a, int n_cu);
-// Most chunks of any backward of up to max_rows rows.
-int64_t mxm_resnorm_max_chunks(int64_t max_rows, int D, int gate, int gate_rows, int n_cu);
+// Most chunks (and so parts) of any backward of up to max_rows rows; groups: of
+// several rows per row of the gate.
+int64_t mxm_resnorm_max_chunks(int64_t max_rows, int D, bool groups, int n_cu);
 
 // ---- gradient sets ----
 // A piece of one tensor, with where it is (a launch reads one descriptor and

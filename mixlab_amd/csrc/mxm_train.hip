@@ -194,6 +194,7 @@ int64_t mxm_resnorm_create(const int64_t* params, int n_params, float eps, int64
     a.D = (int)D;
     a.eps = eps;
     a.inv_d = (float)(1.0 / (double)D);
+    a.n_cu = r->n_cu;
     a.branch = branch;
     a.post_norm = post;
     a.norm = (flags & MXM_RESNORM_NORM) != 0;
@@ -206,8 +207,7 @@ int64_t mxm_resnorm_create(const int64_t* params, int n_params, float eps, int64
     a.gate = (int)gate;
     a.gate_rows = gate == MXM_GATE_NONE ? 1 : (int)gate_rows;
     if (r->backward) {
-      const size_t chunks =
-          (size_t)mxm_resnorm_max_chunks(rows, a.D, a.gate, a.gate_rows, r->n_cu);
+      const size_t chunks = (size_t)mxm_resnorm_max_chunks(rows, a.D, a.gate_rows > 1, a.n_cu);
       r->part.alloc(2 * chunks * (size_t)D * 4);
       if (a.gate && a.gate_rows > 1)
         r->gate_part.alloc(chunks * (size_t)(gate == MXM_GATE_CHANNEL ? D : 1) * 4);
@@ -307,7 +307,6 @@ int mxm_resnorm_backward(int64_t h, int64_t rows, const void* h_in, const void* 
     a.d_scale = d_branch_scale;
     a.d_gate = d_gate;
     a.d_w = d_norm_scale;
-    mxm_resnorm_plan(a, r->n_cu);
     mxm_launch_resnorm_bw(a, r->stream());
     HIPCK(hipGetLastError());
     return MXM_OK;
