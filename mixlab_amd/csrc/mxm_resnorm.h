@@ -8,6 +8,8 @@
 // aligned tensors; V = 1 takes any.
 #pragma once
 
+#include <type_traits>
+
 #include "mxm_kernels.h"
 #include "mxm_train.h"
 
@@ -118,17 +120,52 @@ inline Shape shape_of(int D, bool vectors) {
     if (D <= 64) return {4, 1, 16, THREADS};
     if (D <= 128) return {4, 1, 32, THREADS};
     if (D <= 256) return {4, 1, 64, THREADS};
-    if (D <= 512) return {4, 2, 64, THREADS};
+    if (D <= 1024) return {4, (D + 255) / 256, 64, THREADS};
     const int nv = D <= 8192 ? 2 : 4;
     return {4, nv, 0, (D + 4 * nv * 64 - 1) / (4 * nv * 64) * 64};
   }
   if (D <= 256) return {1, 4, 64, THREADS};
-  const int nv = D <= 4096 ? 4 : 16;
+  const int nv = D <= 4096 ? 4 : D <= 8192 ? 8 : 16;
   return {1, nv, 0, (D + nv * 64 - 1) / (nv * 64) * 64};
 }
 
 inline bool aligned(const void* p, bool bf16) {
   return reinterpret_cast<uintptr_t>(p) % (bf16 ? 8 : 16) == 0;
+}
+
+// f(NV, LPR) of a shape with vectors of 4, or of one without (std::integral_constants).
+template <class F>
+void with_shape4(const Shape& sh, F f) {
+  using std::integral_constant;
+#define MXM_CASE(nv, l) return f(integral_constant<int, nv>(), integral_constant<int, l>())
+  if (sh.lpr == 16) MXM_CASE(1, 16);
+  if (sh.lpr == 32) MXM_CASE(1, 32);
+  if (sh.lpr == 64) {
+    if (sh.NV == 1) MXM_CASE(1, 64);
+    if (sh.NV == 2) MXM_CASE(2, 64);
+    if (sh.NV == 3) MXM_CASE(3, 64);
+    MXM_CASE(4, 64);
+  }
+  if (sh.NV == 2) MXM_CASE(2, 0);
+  MXM_CASE(4, 0);
+}
+template <class F>
+void with_shape1(const Shape& sh, F f) {
+  using std::integral_constant;
+  if (sh.lpr == 64) MXM_CASE(4, 64);
+  if (sh.NV == 4) MXM_CASE(4, 0);
+  if (sh.NV == 8) MXM_CASE(8, 0);
+  MXM_CASE(16, 0);
+#undef MXM_CASE
+}
+// f(K0, K1, K2) of three types.
+template <class F>
+void with_types(bool bf0, bool bf1, bool bf2, F f) {
+  using std::integral_constant;
+  auto k = [](auto bf) { return integral_constant<int, decltype(bf)::value ? BF16 : F32>(); };
+  auto third = [&](auto a, auto b) { bf2 ? f(a, b, k(std::true_type())) : f(a, b, k(std::false_type())); };
+  auto second = [&](auto a) { bf1 ? third(a, k(std::true_type())) : third(a, k(std::false_type())); };
+  bf0 ? second(k(std::true_type())) : second(k(std::false_type()));
 }
 
 }  // namespace resnorm

@@ -111,21 +111,6 @@ void launch(const ResNormArgs& args, const Shape& sh, hipStream_t s) {
                      dim3(sh.threads), 0, s, a);
 }
 
-template <int NV, int LPR>
-void launch_typed(const ResNormArgs& a, const Shape& sh, hipStream_t s) {
-  const int types = (a.x_bf16 ? 4 : 0) | (a.delta_bf16 ? 2 : 0) | (a.y_bf16 ? 1 : 0);
-  switch (types) {
-    case 0: return launch<4, NV, LPR, F32, F32, F32>(a, sh, s);
-    case 1: return launch<4, NV, LPR, F32, F32, BF16>(a, sh, s);
-    case 2: return launch<4, NV, LPR, F32, BF16, F32>(a, sh, s);
-    case 3: return launch<4, NV, LPR, F32, BF16, BF16>(a, sh, s);
-    case 4: return launch<4, NV, LPR, BF16, F32, F32>(a, sh, s);
-    case 5: return launch<4, NV, LPR, BF16, F32, BF16>(a, sh, s);
-    case 6: return launch<4, NV, LPR, BF16, BF16, F32>(a, sh, s);
-    default: return launch<4, NV, LPR, BF16, BF16, BF16>(a, sh, s);
-  }
-}
-
 }  // namespace
 
 void mxm_launch_resnorm(const ResNormArgs& a, hipStream_t s) {
@@ -134,12 +119,12 @@ void mxm_launch_resnorm(const ResNormArgs& a, hipStream_t s) {
                        (!a.branch || (aligned(a.delta, a.delta_bf16) && aligned(a.h, a.x_bf16))) &&
                        (!a.norm || aligned(a.y, a.y_bf16));
   const Shape sh = shape_of(a.D, vectors);
-  if (vectors) {
-    if (sh.lpr == 16) return launch_typed<1, 16>(a, sh, s);
-    if (sh.lpr == 32) return launch_typed<1, 32>(a, sh, s);
-    if (sh.lpr == 64) return sh.NV == 1 ? launch_typed<1, 64>(a, sh, s) : launch_typed<2, 64>(a, sh, s);
-    return sh.NV == 2 ? launch_typed<2, 0>(a, sh, s) : launch_typed<4, 0>(a, sh, s);
-  }
-  if (sh.lpr == 64) return launch<1, 4, 64, ANY, ANY, ANY>(a, sh, s);
-  return sh.NV == 4 ? launch<1, 4, 0, ANY, ANY, ANY>(a, sh, s) : launch<1, 16, 0, ANY, ANY, ANY>(a, sh, s);
+  if (vectors)
+    with_shape4(sh, [&](auto nv, auto lpr) {
+      with_types(a.x_bf16, a.delta_bf16, a.y_bf16, [&](auto xt, auto dt, auto yt) {
+        launch<4, nv(), lpr(), xt(), dt(), yt()>(a, sh, s);
+      });
+    });
+  else
+    with_shape1(sh, [&](auto nv, auto lpr) { launch<1, nv(), lpr(), ANY, ANY, ANY>(a, sh, s); });
 }

@@ -154,62 +154,61 @@ __global__ __launch_bounds__(LPR ? THREADS : 1024) void resnorm_bw_kernel(ResNor
 #pragma unroll
     for (int i = 0; i < NV; ++i)
       if (valid && at[i] < D && a.dx) store<GT, V>(a.dx, a.g_bf16, row + at[i], t + i * V);
-    // the group's last row here: its gate's gradient goes out
+    // the group's last row here
     if (a.gate && valid && (--left == 0 || n + 1 == hi)) {
-      if (a.d_gate) {
-        float* out = a.group_chunks > 0 ? a.gate_part + (size_t)c * (CH ? D : 1)
-                                        : a.d_gate + (size_t)group * (CH ? D : 1);
-        if (CH) {
+      if (a.sigmoid) {
 #pragma unroll
-          for (int i = 0; i < NV; ++i)
+        for (int e = 0; e < (CH ? E : 1); ++e) ag[e] = ag[e] * (ga[e] * (1.0f - ga[e]));
+      }
+      if (a.group_chunks == 0) {  // the group is whole: its gate's gradient goes out
+        if (a.d_gate) {
+          float* out = a.d_gate + (size_t)group * (CH ? D : 1);
+          if (CH) {
 #pragma unroll
-            for (int j = 0; j < V; ++j) {
-              const int e = CH ? i * V + j : 0;
-              if (at[i] < D) out[at[i] + j] = a.sigmoid ? ag[e] * (ga[e] * (1.0f - ga[e])) : ag[e];
-              ag[e] = 0.0f;
-            }
-        } else {
-          if (lane == 0) out[0] = a.sigmoid ? ag[0] * (ga[0] * (1.0f - ga[0])) : ag[0];
-          ag[0] = 0.0f;
+            for (int i = 0; i < NV; ++i)
+              if (at[i] < D)
+#pragma unroll
+                for (int j = 0; j < V; ++j) out[at[i] + j] = ag[CH ? i * V + j : 0];
+          } else if (lane == 0) {
+            out[0] = ag[0];
+          }
         }
+#pragma unroll
+        for (int e = 0; e < (CH ? E : 1); ++e) ag[e] = 0.0f;
       }
       ++group;
       left = a.gate_rows;
       fresh = true;
     }
   }
-  if (a.gate && a.group_chunks > 0 && a.d_gate && lo >= hi && c < a.chunks) {
-    // (a chunk past the last row of a short group)
-    if (CH) {
-#pragma unroll
-      for (int i = 0; i < NV; ++i)
-#pragma unroll
-        for (int j = 0; j < V; ++j)
-          if (at[i] < D) a.gate_part[(size_t)c * D + at[i] + j] = 0.0f;
-    } else if (lane == 0) {
-      a.gate_part[c] = 0.0f;
-    }
-  }
-  auto join = [&](float(&acc)[E], int kind) {
-    float* part = a.part + ((size_t)kind * a.parts + blockIdx.x) * D;
+  // One partial a workgroup, of its rows' sums in their order: n values a thread
+  // in columns, or one (a gate per row).
+  auto join = [&](auto& acc, float* part) {
+    constexpr int n = sizeof acc / sizeof acc[0];
     if (LPR) {
       __syncthreads();
 #pragma unroll
-      for (int e = 0; e < E; ++e) red[LPR ? e * THREADS + threadIdx.x : 0] = acc[e];
+      for (int e = 0; e < n; ++e) red[LPR ? e * THREADS + threadIdx.x : 0] = acc[e];
       __syncthreads();
       if (proc > 0) return;
 #pragma unroll
-      for (int e = 0; e < E; ++e)
+      for (int e = 0; e < n; ++e)
         for (int p = 1; p < rows; ++p) acc[e] += red[LPR ? e * THREADS + p * LPR + lane : 0];
     }
+    if constexpr (n == 1) {
+      if (lane == 0) part[0] = acc[0];
+    } else {
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
+      for (int i = 0; i < NV; ++i)
+        if (at[i] < D)
 #pragma unroll
-      for (int j = 0; j < V; ++j)
-        if (at[i] < D) part[at[i] + j] = acc[i * V + j];
+          for (int j = 0; j < V; ++j) part[at[i] + j] = acc[i * V + j];
+    }
   };
-  if (a.norm && a.d_w) join(aw, 0);
-  if (a.branch && (a.d_scale || a.d_post)) join(aq, 1);
+  if (a.norm && a.d_w) join(aw, a.part + (size_t)blockIdx.x * D);
+  if (a.branch && (a.d_scale || a.d_post)) join(aq, a.part + ((size_t)a.parts + blockIdx.x) * D);
+  if (a.gate && a.group_chunks > 0 && a.d_gate)
+    join(ag, a.gate_part + (size_t)blockIdx.x * (CH ? D : 1));
 }
 
 // Joins the workgroups' column sums: 32 columns a workgroup, 32 slices of the
@@ -225,12 +224,21 @@ __global__ __launch_bounds__(JOIN_COLS* JOIN_SLICES) void resnorm_join_kernel(Re
   if (kind == 1 && !(a.branch && (a.d_scale || a.d_post))) return;
   const int d = blockIdx.x * JOIN_COLS + col;
   const int group = (int)blockIdx.y - 2;
-  const int count = kind == 2 ? a.group_chunks : a.parts;
-  const float* src = kind == 2 ? a.gate_part + (size_t)group * a.group_chunks * width
+  const int count = kind == 2 ? a.group_parts : a.parts;
+  const float* src = kind == 2 ? a.gate_part + (size_t)group * a.group_parts * width
                                : a.part + (size_t)kind * a.parts * a.D;
   float s = 0.0f;
-  if (d < width)
-    for (int p = slice; p < count; p += JOIN_SLICES) s += src[(size_t)p * width + d];
+  if (d < width) {
+    int p = slice;
+    for (; p + 7 * JOIN_SLICES < count; p += 8 * JOIN_SLICES) {
+      float v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = src[(size_t)(p + k * JOIN_SLICES) * width + d];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) s += v[k];
+    }
+    for (; p < count; p += JOIN_SLICES) s += src[(size_t)p * width + d];
+  }
   red[slice][col] = s;
   __syncthreads();
   if (slice != 0 || d >= width) return;
@@ -249,28 +257,36 @@ __global__ __launch_bounds__(JOIN_COLS* JOIN_SLICES) void resnorm_join_kernel(Re
   }
 }
 
-// Chunks that a backward aims at, and the fewest rows of one.
-constexpr int WGS_PER_CU = 4, MIN_CHUNK_ROWS = 4;
-int64_t target_chunks(const Shape& sh, int n_cu) { return (int64_t)WGS_PER_CU * n_cu * sh.rows(); }
+// Chunks that a backward of N rows aims at: WGS_PER_CU workgroups a CU, of no
+// fewer rows than pay for a partial.
+constexpr int WGS_PER_CU = 4;
+int fewest_rows(const Shape& sh) { return sh.lpr > 0 && sh.lpr < 64 ? 1 : 2; }
+int rows_per_chunk(const Shape& sh, int64_t N, int n_cu) {
+  const int64_t target = (int64_t)WGS_PER_CU * n_cu * sh.rows();
+  return (int)std::max<int64_t>((N + target - 1) / target, fewest_rows(sh));
+}
 
 // Splits a.N rows into chunks.
 void plan(ResNormArgs& a, const Shape& sh) {
-  const int64_t target = target_chunks(sh, a.n_cu);
-  const int rows = (int)std::max<int64_t>((a.N + target - 1) / target, MIN_CHUNK_ROWS);
-  a.group_chunks = 0;
-  a.chunk_rows = rows;
+  const int rows = rows_per_chunk(sh, a.N, a.n_cu);
   const int T = std::min(a.gate_rows, a.N);  // rows of the longest group
-  if (a.gate && a.gate_rows > 1 && T > rows) {
-    a.group_chunks = (T + rows - 1) / rows;
-    a.chunk_rows = (T + a.group_chunks - 1) / a.group_chunks;
-    a.group_chunks = (T + a.chunk_rows - 1) / a.chunk_rows;
+  a.group_chunks = a.group_parts = 0;
+  a.chunk_rows = rows;
+  if (a.gate && a.gate_rows > 1) {
     const int groups = (int)(((int64_t)a.N + a.gate_rows - 1) / a.gate_rows);
-    a.chunks = groups * a.group_chunks;
-  } else {
-    // whole groups (or part of the only one)
-    if (a.gate && a.gate_rows <= rows) a.chunk_rows = rows / a.gate_rows * a.gate_rows;
-    a.chunks = (a.N + a.chunk_rows - 1) / a.chunk_rows;
+    if (T >= (int64_t)rows * sh.rows()) {
+      // a group fills workgroups: whole workgroups of chunks for each
+      a.group_parts = (int)(((int64_t)T + (int64_t)rows * sh.rows() - 1) / ((int64_t)rows * sh.rows()));
+      a.group_chunks = a.group_parts * sh.rows();
+      a.chunk_rows = (T + a.group_chunks - 1) / a.group_chunks;
+      a.chunks = groups * a.group_chunks;
+      a.parts = groups * a.group_parts;
+      return;
+    }
+    // chunks of whole groups (or of the only one)
+    a.chunk_rows = T <= rows ? rows / T * T : T;
   }
+  a.chunks = (a.N + a.chunk_rows - 1) / a.chunk_rows;
   a.parts = (a.chunks + sh.rows() - 1) / sh.rows();
 }
 
@@ -284,61 +300,53 @@ void launch(const ResNormArgs& a, const Shape& sh, hipStream_t s) {
                        dim3(sh.threads), 0, s, a);
 }
 
-template <int NV, int LPR>
-void launch_typed(const ResNormArgs& a, const Shape& sh, hipStream_t s) {
-  const int types = (a.x_bf16 ? 4 : 0) | (a.delta_bf16 ? 2 : 0) | (a.g_bf16 ? 1 : 0);
-  switch (types) {
-    case 0: return launch<4, NV, LPR, F32, F32, F32>(a, sh, s);
-    case 1: return launch<4, NV, LPR, F32, F32, BF16>(a, sh, s);
-    case 2: return launch<4, NV, LPR, F32, BF16, F32>(a, sh, s);
-    case 3: return launch<4, NV, LPR, F32, BF16, BF16>(a, sh, s);
-    case 4: return launch<4, NV, LPR, BF16, F32, F32>(a, sh, s);
-    case 5: return launch<4, NV, LPR, BF16, F32, BF16>(a, sh, s);
-    case 6: return launch<4, NV, LPR, BF16, BF16, F32>(a, sh, s);
-    default: return launch<4, NV, LPR, BF16, BF16, BF16>(a, sh, s);
-  }
-}
-
 void launch_rows(const ResNormArgs& a, const Shape& sh, hipStream_t s) {
-  if (sh.V == 4) {
-    if (sh.lpr == 16) return launch_typed<1, 16>(a, sh, s);
-    if (sh.lpr == 32) return launch_typed<1, 32>(a, sh, s);
-    if (sh.lpr == 64) return sh.NV == 1 ? launch_typed<1, 64>(a, sh, s) : launch_typed<2, 64>(a, sh, s);
-    return sh.NV == 2 ? launch_typed<2, 0>(a, sh, s) : launch_typed<4, 0>(a, sh, s);
-  }
-  if (sh.lpr == 64) return launch<1, 4, 64, ANY, ANY, ANY>(a, sh, s);
-  return sh.NV == 4 ? launch<1, 4, 0, ANY, ANY, ANY>(a, sh, s) : launch<1, 16, 0, ANY, ANY, ANY>(a, sh, s);
+  if (sh.V == 4)
+    with_shape4(sh, [&](auto nv, auto lpr) {
+      with_types(a.x_bf16, a.delta_bf16, a.g_bf16, [&](auto xt, auto dt, auto gt) {
+        launch<4, nv(), lpr(), xt(), dt(), gt()>(a, sh, s);
+      });
+    });
+  else
+    with_shape1(sh, [&](auto nv, auto lpr) { launch<1, nv(), lpr(), ANY, ANY, ANY>(a, sh, s); });
 }
 
 }  // namespace
 
-int64_t mxm_resnorm_max_chunks(int64_t max_rows, int D, bool groups, int n_cu) {
-  // Without groups at most the target's; whole groups make chunks of at least
-  // half the rows aimed at; chunks within groups are at most one more per group
-  // than rows / chunk rows, and the groups fewer than that.
+int64_t mxm_resnorm_max_parts(int64_t max_rows, int D, bool groups, int n_cu) {
+  // A workgroup's R = rows() * rows_per_chunk rows.  Without groups ceil(N / R)
+  // parts, at most the target and at most ceil(N / (rows() * fewest)); chunks of
+  // whole groups hold more than half of the rows aimed at; groups that fill
+  // workgroups (T >= R) have at most T / R + 1 parts each, and there are at most
+  // N / T + 1 of them: N / R + T / R + N / T + 1 <= 3 N / R + 1.
   int64_t most = 0;
-  for (const bool vectors : {false, true})
-    most = std::max(most, target_chunks(shape_of(D, vectors), n_cu));
-  most = std::min(most, (max_rows + MIN_CHUNK_ROWS - 1) / MIN_CHUNK_ROWS);
+  for (const bool vectors : {false, true}) {
+    const Shape sh = shape_of(D, vectors);
+    const int64_t R = (int64_t)sh.rows() * fewest_rows(sh);
+    most = std::max(most, std::min<int64_t>((int64_t)WGS_PER_CU * n_cu, (max_rows + R - 1) / R));
+  }
   return groups ? 3 * most + 1 : most;
 }
 
-void mxm_launch_resnorm_bw(const ResNormArgs& args, hipStream_t s) {
+bool mxm_launch_resnorm_bw(const ResNormArgs& args, hipStream_t s) {
   ResNormArgs a = args;
   const bool vectors =
       a.D % 4 == 0 && (!a.norm || (aligned(a.h, a.x_bf16) && aligned(a.dy, a.g_bf16))) &&
       (!a.branch || (aligned(a.delta, a.delta_bf16) && aligned(a.d_delta, a.g_bf16))) &&
       aligned(a.dh, a.g_bf16) && aligned(a.dx, a.g_bf16);
   const Shape sh = shape_of(a.D, vectors);
-  a.chunks = a.parts = a.group_chunks = 0;
+  a.chunks = a.parts = a.group_chunks = a.group_parts = 0;
   if (a.N > 0) {
     plan(a, sh);
+    if (a.parts > a.max_parts) return false;
     launch_rows(a, sh, s);
   }
   // (without rows the scales' gradients are zero)
   const bool columns = (a.norm && a.d_w) || (a.branch && (a.d_scale || a.d_post));
   const bool gates = a.gate && a.group_chunks > 0 && a.d_gate;
-  if (!columns && !gates) return;
-  const dim3 grid((a.D + JOIN_COLS - 1) / JOIN_COLS, 2 + (gates ? a.chunks / a.group_chunks : 0));
-  hipLaunchKernelGGL(resnorm_join_kernel, grid, dim3(JOIN_COLS * JOIN_SLICES), 0, s, a);
+  if (columns || gates) {
+    const dim3 grid((a.D + JOIN_COLS - 1) / JOIN_COLS, 2 + (gates ? a.parts / a.group_parts : 0));
+    hipLaunchKernelGGL(resnorm_join_kernel, grid, dim3(JOIN_COLS * JOIN_SLICES), 0, s, a);
+  }
+  return true;
 }

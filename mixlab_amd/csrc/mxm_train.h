@@ -37,19 +37,21 @@ struct ResNormArgs {
   const void *dh, *dy;                  // [N, D]; dh null: zeros
   void *dx, *d_delta;                   // [N, D]
   float *d_post, *d_scale, *d_w, *d_gate;  // null: not wanted
-  // Column sums go over chunks of rows: part [2][parts][D] (w, then a q; a part
-  // is a workgroup's chunks) and gate_part [chunks][1 or D] for gates whose rows
-  // span several chunks.  Set by the launcher.
+  // Column sums go over chunks of rows, one a row's threads; a workgroup's chunks
+  // make a part: part [2][parts][D] (w, then a q) and, for gates whose rows span
+  // several parts, gate_part [parts][1 or D].  Set by the launcher.
   float *part, *gate_part;
-  int chunks, parts, chunk_rows;  // (forwards chunk_rows: rows a thread walks)
-  int group_chunks;  // chunks per group of gate rows, each within one; 0: chunks of whole groups
+  int chunks, parts, chunk_rows;   // (forwards chunk_rows: rows a thread walks)
+  int group_chunks, group_parts;   // per group of gate rows, each within one; 0: whole groups
+  int max_parts;                   // that part and gate_part have room for
   int n_cu;
 };
 void mxm_launch_resnorm(const ResNormArgs& a, hipStream_t s);
-void mxm_launch_resnorm_bw(const ResNormArgs& a, hipStream_t s);
-// Most chunks (and so parts) of any backward of up to max_rows rows; groups: of
-// several rows per row of the gate.
-int64_t mxm_resnorm_max_chunks(int64_t max_rows, int D, bool groups, int n_cu);
+// false, and no launch, where max_parts is too few.
+bool mxm_launch_resnorm_bw(const ResNormArgs& a, hipStream_t s);
+// Most parts of any backward of up to max_rows rows; groups: of several rows per
+// row of the gate.
+int64_t mxm_resnorm_max_parts(int64_t max_rows, int D, bool groups, int n_cu);
 
 // ---- gradient sets ----
 // A piece of one tensor, with where it is (a launch reads one descriptor and

@@ -207,10 +207,11 @@ int64_t mxm_resnorm_create(const int64_t* params, int n_params, float eps, int64
     a.gate = (int)gate;
     a.gate_rows = gate == MXM_GATE_NONE ? 1 : (int)gate_rows;
     if (r->backward) {
-      const size_t chunks = (size_t)mxm_resnorm_max_chunks(rows, a.D, a.gate_rows > 1, a.n_cu);
-      r->part.alloc(2 * chunks * (size_t)D * 4);
+      a.max_parts = (int)mxm_resnorm_max_parts(rows, a.D, a.gate_rows > 1, a.n_cu);
+      const size_t parts = (size_t)a.max_parts;
+      r->part.alloc(2 * parts * (size_t)D * 4);
       if (a.gate && a.gate_rows > 1)
-        r->gate_part.alloc(chunks * (size_t)(gate == MXM_GATE_CHANNEL ? D : 1) * 4);
+        r->gate_part.alloc(parts * (size_t)(gate == MXM_GATE_CHANNEL ? D : 1) * 4);
       a.part = r->part.as<float>();
       a.gate_part = r->gate_part.as<float>();
     }
@@ -307,7 +308,8 @@ int mxm_resnorm_backward(int64_t h, int64_t rows, const void* h_in, const void* 
     a.d_scale = d_branch_scale;
     a.d_gate = d_gate;
     a.d_w = d_norm_scale;
-    mxm_launch_resnorm_bw(a, r->stream());
+    if (!mxm_launch_resnorm_bw(a, r->stream()))
+      fail_rt(RESNORM " internal error: backward workspace too small");
     HIPCK(hipGetLastError());
     return MXM_OK;
   });

@@ -17,10 +17,6 @@ from .op import _DTYPES
 _GATES = {None: _lib.MXM_GATE_NONE, "row": _lib.MXM_GATE_ROW, "channel": _lib.MXM_GATE_CHANNEL}
 
 
-def _vp(ptr: Optional[int]):
-    return ctypes.c_void_p(ptr) if ptr else None
-
-
 class _Handle:
     """A handle of the library: its stream, waiting for it, its release."""
 
@@ -88,17 +84,17 @@ class ResidualNorm(_Handle):
                 post_scale: int = 0, branch_scale: int = 0, gate: int = 0,
                 norm_scale: int = 0) -> None:
         _lib.check(self._lib.mxm_resnorm_forward(
-            self.handle, rows, _vp(x), _vp(delta), _vp(post_scale), _vp(branch_scale), _vp(gate),
-            _vp(norm_scale), _vp(h), _vp(y)), "mxm_resnorm_forward")
+            self.handle, rows, x or None, delta or None, post_scale or None, branch_scale or None, gate or None,
+            norm_scale or None, h or None, y or None), "mxm_resnorm_forward")
 
     def backward(self, rows: int, h: int = 0, delta: int = 0, dh: int = 0, dy: int = 0, dx: int = 0,
                  d_delta: int = 0, post_scale: int = 0, branch_scale: int = 0, gate: int = 0,
                  norm_scale: int = 0, d_post_scale: int = 0, d_branch_scale: int = 0,
                  d_gate: int = 0, d_norm_scale: int = 0) -> None:
         _lib.check(self._lib.mxm_resnorm_backward(
-            self.handle, rows, _vp(h), _vp(delta), _vp(post_scale), _vp(branch_scale), _vp(gate),
-            _vp(norm_scale), _vp(dh), _vp(dy), _vp(dx), _vp(d_delta), _vp(d_post_scale),
-            _vp(d_branch_scale), _vp(d_gate), _vp(d_norm_scale)), "mxm_resnorm_backward")
+            self.handle, rows, h or None, delta or None, post_scale or None, branch_scale or None, gate or None,
+            norm_scale or None, dh or None, dy or None, dx or None, d_delta or None, d_post_scale or None,
+            d_branch_scale or None, d_gate or None, d_norm_scale or None), "mxm_resnorm_backward")
 
 
 class GradientSet(_Handle):
@@ -139,13 +135,13 @@ class GradientSet(_Handle):
             grads, clipped, params, m, v, params_bf16))), "mxm_grads_bind")
 
     def norm(self, norm: int) -> None:
-        _lib.check(self._lib.mxm_grads_norm(self.handle, _vp(norm)), "mxm_grads_norm")
+        _lib.check(self._lib.mxm_grads_norm(self.handle, norm or None), "mxm_grads_norm")
 
     def clip(self, max_norm: float, norm: int = 0) -> None:
-        _lib.check(self._lib.mxm_grads_clip(self.handle, max_norm, _vp(norm)), "mxm_grads_clip")
+        _lib.check(self._lib.mxm_grads_clip(self.handle, max_norm, norm or None), "mxm_grads_clip")
 
     def adamw(self, lr: float, beta1: float, beta2: float, eps: float, weight_decay: float,
               max_norm: float, step: int, norm: int = 0, skipped: int = 0) -> None:
         _lib.check(self._lib.mxm_grads_adamw(self.handle, lr, beta1, beta2, eps, weight_decay,
-                                             max_norm, _vp(step), _vp(norm), _vp(skipped)),
+                                             max_norm, step or None, norm or None, skipped or None),
                    "mxm_grads_adamw")
