@@ -9,15 +9,13 @@ namespace {
 
 using namespace resnorm;
 
-constexpr int ROWS_PER_WG_LOOP = 4;  // row rounds of a workgroup that loops
-
 template <int V, int NV, int LPR, int XT, int DT, int YT>
-__global__ __launch_bounds__(LPR ? THREADS : 1024) void resnorm_kernel(ResNormArgs a) {
+__global__ __launch_bounds__(most_threads(LPR)) void resnorm_kernel(ResNormArgs a) {
   constexpr int E = V * NV;
-  __shared__ float red[2][2][LPR ? 1 : 16];
-  const int lane = LPR ? threadIdx.x % (LPR ? LPR : 1) : threadIdx.x;
-  const int stride = LPR ? LPR : blockDim.x;
-  const int rows = LPR ? THREADS / (LPR ? LPR : 1) : 1;
+  __shared__ float red[2][2][LPR > 0 ? 1 : 16];
+  const int lane = LPR > 0 ? threadIdx.x % (LPR > 0 ? LPR : 1) : threadIdx.x;
+  const int stride = LPR > 0 ? LPR : blockDim.x;
+  const int rows = LPR > 0 ? THREADS / (LPR > 0 ? LPR : 1) : 1;
   const int D = a.D;
   int at[NV];
   float f[E], w[E];
@@ -27,48 +25,58 @@ __global__ __launch_bounds__(LPR ? THREADS : 1024) void resnorm_kernel(ResNormAr
 #pragma unroll
     for (int j = 0; j < V; ++j) f[i * V + j] = w[i * V + j] = 0.0f;
     if (at[i] < D) {
-      float p[V];
-      load_scale<V>(a.scale, a.p_bf16, at[i], f + i * V);
-      load_scale<V>(a.post, a.p_bf16, at[i], p);
+      if (a.branch) {
+        float p[V];
+        load_scale<V>(a.scale, a.p_bf16, at[i], f + i * V);
+        load_scale<V>(a.post, a.p_bf16, at[i], p);
 #pragma unroll
-      for (int j = 0; j < V; ++j) f[i * V + j] *= p[j];
+        for (int j = 0; j < V; ++j) f[i * V + j] *= p[j];
+      }
       if (a.norm) load_scale<V>(a.w, a.p_bf16, at[i], w + i * V);
     }
   }
   // (at most 2^30 rows and a workgroup's more)
-  const int first =
-      (int)blockIdx.x * rows * a.chunk_rows + (LPR ? (int)threadIdx.x / (LPR ? LPR : 1) : 0);
+  const int first = (int)blockIdx.x * rows * a.chunk_rows + row_slot<LPR>();
+  Raw<XT, V> rx[NV];
+  Raw<DT, V> rd[NV];
+  float rg = 0.0f;  // a gate per row
+  // (values past the row's end and rows past the last are zero)
+  auto fetch = [&](int n) {
+    const size_t row = (size_t)n * D;
+    if (a.gate == 1 && n < a.N) load_scale<1>(a.gatep, a.p_bf16, (size_t)(n / a.gate_rows), &rg);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      rx[i] = Raw<XT, V>{};
+      rd[i] = Raw<DT, V>{};
+      if (n < a.N && at[i] < D) {
+        rx[i] = load<XT, V>(a.x, a.x_bf16, row + at[i]);
+        if (a.branch) rd[i] = load<DT, V>(a.delta, a.delta_bf16, row + at[i]);
+      }
+    }
+  };
+  fetch(first);
   for (int it = 0; it < a.chunk_rows; ++it) {
     const int n = first + it * rows;
     const bool valid = n < a.N;  // (a workgroup of one row: for all of it)
     const size_t row = (size_t)n * D;
     float h[E], dl[E], ga[E], sum[1];
-    // (values past the row's end and rows past the last stay zero)
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-#pragma unroll
-      for (int j = 0; j < V; ++j) h[i * V + j] = dl[i * V + j] = ga[i * V + j] = 0.0f;
-      if (valid && at[i] < D) {
-        load<XT, V>(a.x, a.x_bf16, row + at[i], h + i * V);
-        if (a.branch) load<DT, V>(a.delta, a.delta_bf16, row + at[i], dl + i * V);
-      }
+      unpack<XT, V>(rx[i], h + i * V);
+      unpack<DT, V>(rd[i], dl + i * V);
     }
+    float g = a.gate == 1 ? rg : 1.0f;
+    if (it + 1 < a.chunk_rows) fetch(n + rows);
     if (a.branch) {
+      // (the gate's values go through the sigmoid after the sum, which hides its load)
       if (a.gate == 2) {
         const size_t grow = (size_t)(n / a.gate_rows) * D;
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
+        for (int i = 0; i < NV; ++i) {
+#pragma unroll
+          for (int j = 0; j < V; ++j) ga[i * V + j] = 0.0f;
           if (valid && at[i] < D) load_scale<V>(a.gatep, a.p_bf16, grow + at[i], ga + i * V);
-#pragma unroll
-        for (int e = 0; e < E; ++e) ga[e] = gate_of(a, ga[e]) * f[e];
-      } else {
-        float g = 1.0f;
-        if (a.gate == 1 && valid) {
-          load_scale<1>(a.gatep, a.p_bf16, (size_t)(n / a.gate_rows), &g);
-          g = gate_of(a, g);
         }
-#pragma unroll
-        for (int e = 0; e < E; ++e) ga[e] = g * f[e];
       }
       float rp = 1.0f;
       if (a.post_norm) {
@@ -79,7 +87,10 @@ __global__ __launch_bounds__(LPR ? THREADS : 1024) void resnorm_kernel(ResNormAr
         rp = 1.0f / __builtin_sqrtf(sum[0] * a.inv_d + a.eps);
       }
 #pragma unroll
-      for (int e = 0; e < E; ++e) h[e] = h[e] + ga[e] * (dl[e] * rp);
+      for (int e = 0; e < E; ++e) ga[e] = a.gate == 2 ? gate_of(a, ga[e]) * f[e] : f[e];
+      g = (a.gate == 1 ? gate_of(a, g) : 1.0f) * rp;
+#pragma unroll
+      for (int e = 0; e < E; ++e) h[e] = __builtin_fmaf(g * dl[e], ga[e], h[e]);
 #pragma unroll
       for (int i = 0; i < NV; ++i)
         if (valid && at[i] < D) store<XT, V>(a.h, a.x_bf16, row + at[i], h + i * V);
@@ -101,13 +112,22 @@ __global__ __launch_bounds__(LPR ? THREADS : 1024) void resnorm_kernel(ResNormAr
   }
 }
 
+// Rows that a thread walks, which share its loads of the scales: few enough that
+// all CUs have several workgroups.  134 M elements at 1024 and 2048 channels with
+// 1 / 2 / 4 / 8 rows, fp32 302-328 / 302-305 / 320-332 / 341-349 us, bf16 206-210 /
+// 178-182 / 174-178 / 174-194: rows of half the bytes pay for twice as many.
+int rows_per_thread(const ResNormArgs& a, const Shape& sh) {
+  const int64_t rounds = ((int64_t)a.N + sh.rows() - 1) / sh.rows();
+  const int most = a.x_bf16 && (a.delta_bf16 || !a.branch) ? 4 : 2;
+  return (int)std::min<int64_t>(std::max<int64_t>(rounds / (8 * a.n_cu), 1), most);
+}
+
 template <int V, int NV, int LPR, int XT, int DT, int YT>
 void launch(const ResNormArgs& args, const Shape& sh, hipStream_t s) {
   ResNormArgs a = args;
-  const int64_t rounds = ((int64_t)a.N + sh.rows() - 1) / sh.rows();
-  a.chunk_rows = rounds >= 4096 * ROWS_PER_WG_LOOP ? ROWS_PER_WG_LOOP : 1;
-  const int64_t blocks = (rounds + a.chunk_rows - 1) / a.chunk_rows;
-  hipLaunchKernelGGL((resnorm_kernel<V, NV, LPR, XT, DT, YT>), dim3((unsigned)blocks),
+  a.chunk_rows = rows_per_thread(a, sh);
+  const int64_t per = (int64_t)a.chunk_rows * sh.rows();
+  hipLaunchKernelGGL((resnorm_kernel<V, NV, LPR, XT, DT, YT>), dim3((unsigned)((a.N + per - 1) / per)),
                      dim3(sh.threads), 0, s, a);
 }
 
@@ -118,7 +138,7 @@ void mxm_launch_resnorm(const ResNormArgs& a, hipStream_t s) {
   const bool vectors = a.D % 4 == 0 && aligned(a.x, a.x_bf16) &&
                        (!a.branch || (aligned(a.delta, a.delta_bf16) && aligned(a.h, a.x_bf16))) &&
                        (!a.norm || aligned(a.y, a.y_bf16));
-  const Shape sh = shape_of(a.D, vectors);
+  const Shape sh = shape_of(a.D, vectors, false);
   if (vectors)
     with_shape4(sh, [&](auto nv, auto lpr) {
       with_types(a.x_bf16, a.delta_bf16, a.y_bf16, [&](auto xt, auto dt, auto yt) {

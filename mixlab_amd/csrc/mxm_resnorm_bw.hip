@@ -10,34 +10,39 @@ namespace {
 
 using namespace resnorm;
 
-// Rows [*lo, *hi) of chunk c.
-__device__ __forceinline__ void chunk_range(const ResNormArgs& a, int c, int* lo, int* hi) {
-  int64_t r0, r1;
-  if (c >= a.chunks) {
-    r0 = r1 = a.N;
-  } else if (a.group_chunks > 0) {
-    const int64_t g = c / a.group_chunks, sub = c % a.group_chunks;
-    r0 = g * a.gate_rows + sub * a.chunk_rows;
-    r1 = min(r0 + a.chunk_rows, (g + 1) * (int64_t)a.gate_rows);
-  } else {
-    r0 = (int64_t)c * a.chunk_rows;
-    r1 = r0 + a.chunk_rows;
+// The rows of a chunk: first, first + step, ... (count of them).  Neighbouring
+// chunks hold neighbouring rows, so that the workgroups sweep over memory side
+// by side; chunks of whole groups of gate rows hold theirs in a row.
+struct Rows {
+  int first, step, count;
+};
+__device__ __forceinline__ Rows rows_of(const ResNormArgs& a, int c) {
+  if (c >= a.chunks) return {0, 1, 0};
+  int first = c, step = a.chunks, end = a.N;
+  if (a.group_chunks > 0) {
+    const int g = c / a.group_chunks;
+    first = (int)min((int64_t)g * a.gate_rows + c % a.group_chunks, (int64_t)a.N);
+    step = a.group_chunks;
+    end = (int)min((int64_t)(g + 1) * a.gate_rows, (int64_t)a.N);
+  } else if (a.gate && a.gate_rows > 1) {
+    first = (int)min((int64_t)c * a.chunk_rows, (int64_t)a.N);
+    step = 1;
+    end = (int)min((int64_t)first + a.chunk_rows, (int64_t)a.N);
   }
-  *lo = (int)min(r0, (int64_t)a.N);
-  *hi = (int)min(r1, (int64_t)a.N);
+  return {first, step, first < end ? (int)(((int64_t)end - first + step - 1) / step) : 0};
 }
 
 // CH: a gate per channel.  A row's threads walk one chunk; the chunks of a
 // workgroup add their column sums in LDS and store one partial.
 template <int V, int NV, int LPR, int XT, int DT, int GT, bool CH>
-__global__ __launch_bounds__(LPR ? THREADS : 1024) void resnorm_bw_kernel(ResNormArgs a) {
+__global__ __launch_bounds__(most_threads(LPR)) void resnorm_bw_kernel(ResNormArgs a) {
   constexpr int E = V * NV;
-  // of a row's sums (LPR = 0), or of the workgroup's column sums at the end
-  __shared__ float red[LPR ? THREADS * E : 2 * 2 * 16 * 3];
-  const int lane = LPR ? threadIdx.x % (LPR ? LPR : 1) : threadIdx.x;
-  const int stride = LPR ? LPR : blockDim.x;
-  const int rows = LPR ? THREADS / (LPR ? LPR : 1) : 1;
-  const int proc = LPR ? threadIdx.x / (LPR ? LPR : 1) : 0;
+  // of a row's sums (a workgroup a row), or of the workgroup's column sums at the end
+  __shared__ float red[LPR > 0 ? THREADS * E : 2 * 16 * 3 + 2 * 16];
+  const int lane = LPR > 0 ? threadIdx.x % (LPR > 0 ? LPR : 1) : threadIdx.x;
+  const int stride = LPR > 0 ? LPR : blockDim.x;
+  const int rows = LPR > 0 ? THREADS / (LPR > 0 ? LPR : 1) : 1;
+  const int proc = row_slot<LPR>();
   const int c = blockIdx.x * rows + proc, D = a.D;
   const bool post = a.branch && a.post_norm;
   int at[NV];
@@ -66,53 +71,77 @@ __global__ __launch_bounds__(LPR ? THREADS : 1024) void resnorm_bw_kernel(ResNor
     ag[0] = 0.0f;
     ga[0] = 1.0f;
   }
-  int lo, hi;
-  chunk_range(a, c, &lo, &hi);
-  int group = a.gate ? lo / a.gate_rows : 0;
-  int left = a.gate ? a.gate_rows - (lo - group * a.gate_rows) : 0;  // rows to the group's end
-  bool fresh = true;                                                  // the gate is not loaded yet
-  // (the same number of rounds in every lane: the sums use whole waves)
-  const int rounds = LPR ? a.chunk_rows : hi - lo;
-  for (int it = 0; it < rounds; ++it) {
-    const int n = lo + it;
-    const bool valid = n < hi;
-    const size_t row = (size_t)n * D;
-    float h[E], dl[E], t[E], dy[E];
+  const Rows mine = rows_of(a, c);
+  int group = a.gate ? mine.first / a.gate_rows : 0;
+  // the chunk's rows before its group ends: whole groups (in a row), or one group
+  int left = a.group_chunks > 0 ? mine.count : a.gate_rows;
+  bool fresh = true;  // the group's gate is not loaded yet
+  Raw<XT, V> rh[NV];
+  Raw<DT, V> rd[NV];
+  Raw<GT, V> rt[NV], ry[NV];
+  float rg = 0.0f;  // a gate of the row alone
+  const bool row_gate = !CH && a.gate && a.gate_rows == 1;
+  // (values past the row's end and rows past the chunk's are zero)
+  auto fetch = [&](int it) {
+    const size_t row = ((size_t)mine.first + (size_t)it * mine.step) * D;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const int e = i * V + j;
-        h[e] = dl[e] = t[e] = dy[e] = 0.0f;
+      rh[i] = Raw<XT, V>{};
+      rd[i] = Raw<DT, V>{};
+      rt[i] = Raw<GT, V>{};
+      ry[i] = Raw<GT, V>{};
+      if (it < mine.count && at[i] < D) {
+        if (a.norm) {
+          rh[i] = load<XT, V>(a.h, a.x_bf16, row + at[i]);
+          ry[i] = load<GT, V>(a.dy, a.g_bf16, row + at[i]);
+        }
+        if (a.branch) rd[i] = load<DT, V>(a.delta, a.delta_bf16, row + at[i]);
+        if (a.dh) rt[i] = load<GT, V>(a.dh, a.g_bf16, row + at[i]);
       }
-      if (!valid || at[i] >= D) continue;
-      if (a.norm) {
-        load<XT, V>(a.h, a.x_bf16, row + at[i], h + i * V);
-        load<GT, V>(a.dy, a.g_bf16, row + at[i], dy + i * V);
-      }
-      if (a.branch) load<DT, V>(a.delta, a.delta_bf16, row + at[i], dl + i * V);
-      if (a.dh) load<GT, V>(a.dh, a.g_bf16, row + at[i], t + i * V);
     }
-    if (a.gate && fresh && valid) {
+    if (row_gate && it < mine.count)
+      load_scale<1>(a.gatep, a.p_bf16, (size_t)mine.first + (size_t)it * mine.step, &rg);
+  };
+  if (LPR >= 0) fetch(0);
+  // (the same number of rounds in every lane: the sums use whole waves)
+  const int rounds = LPR > 0 ? a.chunk_rows : mine.count;
+  for (int it = 0; it < rounds; ++it) {
+    const bool valid = it < mine.count;
+    const size_t row = ((size_t)mine.first + (size_t)it * mine.step) * D;
+    float h[E], dl[E], t[E], dy[E];
+    if (LPR < 0) fetch(it);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      unpack<XT, V>(rh[i], h + i * V);
+      unpack<DT, V>(rd[i], dl + i * V);
+      unpack<GT, V>(rt[i], t + i * V);
+      unpack<GT, V>(ry[i], dy + i * V);
+    }
+    // (the gate's values go through the sigmoid after the sums, which hide its load)
+    const bool new_gate = a.gate && fresh && valid;
+    if (row_gate) ga[0] = rg;
+    if (LPR >= 0 && it + 1 < rounds) fetch(it + 1);
+    if (new_gate && !row_gate) {
       if (CH) {
 #pragma unroll
         for (int i = 0; i < NV; ++i)
           if (at[i] < D)
             load_scale<V>(a.gatep, a.p_bf16, (size_t)group * D + at[i], ga + (CH ? i * V : 0));
-#pragma unroll
-        for (int e = 0; e < (CH ? E : 1); ++e) ga[e] = gate_of(a, ga[e]);
       } else {
         load_scale<1>(a.gatep, a.p_bf16, (size_t)group, ga);
-        ga[0] = gate_of(a, ga[0]);
       }
-      fresh = false;
     }
     float s[3] = {0.0f, 0.0f, 0.0f};
+    if (a.norm) {
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      s[0] = __builtin_fmaf(h[e], h[e], s[0]);
-      s[1] = __builtin_fmaf(w[e] * dy[e], h[e], s[1]);
-      s[2] = __builtin_fmaf(dl[e], dl[e], s[2]);
+      for (int e = 0; e < E; ++e) {
+        s[0] = __builtin_fmaf(h[e], h[e], s[0]);
+        s[1] = __builtin_fmaf(w[e] * dy[e], h[e], s[1]);
+      }
+    }
+    if (post) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) s[2] = __builtin_fmaf(dl[e], dl[e], s[2]);
     }
     if (a.norm || post) row_sum<LPR>(s, red + (it & 1) * 48);
     if (a.norm) {
@@ -120,42 +149,54 @@ __global__ __launch_bounds__(LPR ? THREADS : 1024) void resnorm_bw_kernel(ResNor
       const float kn = rn * rn * rn * (s[1] * a.inv_d);
 #pragma unroll
       for (int e = 0; e < E; ++e) {
-        t[e] = t[e] + (rn * (w[e] * dy[e]) - h[e] * kn);
-        if (valid) aw[e] = aw[e] + dy[e] * h[e] * rn;
+        t[e] = __builtin_fmaf(-kn, h[e], __builtin_fmaf(rn, w[e] * dy[e], t[e]));
+        aw[e] = __builtin_fmaf(rn, dy[e] * h[e], aw[e]);  // (rows past the chunk's: dy is 0)
       }
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      if (!(valid && at[i] < D && a.dx)) continue;
+      float out[V];
+#pragma unroll
+      for (int j = 0; j < V; ++j) out[j] = t[i * V + j];
+      store<GT, V>(a.dx, a.g_bf16, row + at[i], out);
+    }
+    if (new_gate) {
+#pragma unroll
+      for (int e = 0; e < (CH ? E : 1); ++e) ga[e] = gate_of(a, ga[e]);
+      fresh = false;
     }
     if (a.branch) {
       const float rp = post ? 1.0f / __builtin_sqrtf(s[2] * a.inv_d + a.eps) : 1.0f;
-      float q[2] = {0.0f, 0.0f};
+      // q = sum f t delta, times the gate where that differs by channel
+      float q[1] = {0.0f};
+      const float g = CH ? 1.0f : ga[0];
 #pragma unroll
       for (int e = 0; e < E; ++e) {
-        const float td = f[e] * t[e] * dl[e];
-        q[0] = __builtin_fmaf(ga[CH ? e : 0], td, q[0]);  // e * delta
-        q[1] = q[1] + td * rp;                            // f * q
+        const float td = t[e] * dl[e];  // (0 in rows past the chunk's: delta is)
+        const float gt = CH ? ga[CH ? e : 0] * td : td;
+        aq[e] = __builtin_fmaf(g * rp, gt, aq[e]);
+        if (CH) ag[CH ? e : 0] = __builtin_fmaf(rp * f[e], td, ag[CH ? e : 0]);
+        q[0] = __builtin_fmaf(f[e], gt, q[0]);
       }
-      if (post || a.gate == 1) row_sum<LPR>(q, red + 96 + (it & 1) * 32);
-      const float kp = post ? rp * rp * rp * (q[0] * a.inv_d) : 0.0f;
-      float d[E];
+      if (post || a.gate == 1) row_sum<LPR>(q, red + 96 + (it & 1) * 16);
+      if (!CH && valid) ag[0] = __builtin_fmaf(rp, q[0], ag[0]);
+      const float kp = post ? rp * rp * rp * (g * q[0] * a.inv_d) : 0.0f;
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const float g = ga[CH ? e : 0];
-        const float tz = t[e] * (dl[e] * rp);
-        if (valid) {
-          aq[e] = aq[e] + g * tz;
-          if (CH) ag[CH ? e : 0] = ag[CH ? e : 0] + f[e] * tz;
+      for (int i = 0; i < NV; ++i) {
+        if (!(valid && at[i] < D)) continue;
+        float out[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const int e = i * V + j;
+          const float gf = CH ? ga[CH ? e : 0] * f[e] : f[e];
+          out[j] = __builtin_fmaf(-kp, dl[e], (g * rp) * (gf * t[e]));
         }
-        d[e] = rp * (t[e] * (g * f[e])) - dl[e] * kp;
+        store<GT, V>(a.d_delta, a.g_bf16, row + at[i], out);
       }
-      if (!CH && valid) ag[0] = ag[0] + q[1];
-#pragma unroll
-      for (int i = 0; i < NV; ++i)
-        if (valid && at[i] < D) store<GT, V>(a.d_delta, a.g_bf16, row + at[i], d + i * V);
     }
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-      if (valid && at[i] < D && a.dx) store<GT, V>(a.dx, a.g_bf16, row + at[i], t + i * V);
     // the group's last row here
-    if (a.gate && valid && (--left == 0 || n + 1 == hi)) {
+    if (a.gate && valid && (--left == 0 || it + 1 == mine.count)) {
       if (a.sigmoid) {
 #pragma unroll
         for (int e = 0; e < (CH ? E : 1); ++e) ag[e] = ag[e] * (ga[e] * (1.0f - ga[e]));
@@ -176,7 +217,7 @@ __global__ __launch_bounds__(LPR ? THREADS : 1024) void resnorm_bw_kernel(ResNor
 #pragma unroll
         for (int e = 0; e < (CH ? E : 1); ++e) ag[e] = 0.0f;
       }
-      ++group;
+      group += a.gate_rows == 1 ? mine.step : 1;
       left = a.gate_rows;
       fresh = true;
     }
@@ -185,15 +226,15 @@ __global__ __launch_bounds__(LPR ? THREADS : 1024) void resnorm_bw_kernel(ResNor
   // in columns, or one (a gate per row).
   auto join = [&](auto& acc, float* part) {
     constexpr int n = sizeof acc / sizeof acc[0];
-    if (LPR) {
+    if (LPR > 0) {
       __syncthreads();
 #pragma unroll
-      for (int e = 0; e < n; ++e) red[LPR ? e * THREADS + threadIdx.x : 0] = acc[e];
+      for (int e = 0; e < n; ++e) red[LPR > 0 ? e * THREADS + threadIdx.x : 0] = acc[e];
       __syncthreads();
       if (proc > 0) return;
 #pragma unroll
       for (int e = 0; e < n; ++e)
-        for (int p = 1; p < rows; ++p) acc[e] += red[LPR ? e * THREADS + p * LPR + lane : 0];
+        for (int p = 1; p < rows; ++p) acc[e] += red[LPR > 0 ? e * THREADS + p * LPR + lane : 0];
     }
     if constexpr (n == 1) {
       if (lane == 0) part[0] = acc[0];
@@ -258,8 +299,12 @@ __global__ __launch_bounds__(JOIN_COLS* JOIN_SLICES) void resnorm_join_kernel(Re
 }
 
 // Chunks that a backward of N rows aims at: WGS_PER_CU workgroups a CU, of no
-// fewer rows than pay for a partial.
-constexpr int WGS_PER_CU = 4;
+// fewer rows than pay for a partial.  134 M elements in fp32 at 64, 512, 1024,
+// 2048 and 4096 channels with 2 / 4 / 8 workgroups a CU: 556 / 599 / 612, 545 /
+// 603 / 608, 576 / 589 / 593, 568 / 659 / 645 and 564 / 628 / 664 us (5.7 TB/s
+// with 2): each has its next row's loads on their way, and fewer streams at once
+// suit the memory better.
+constexpr int WGS_PER_CU = 2;
 int fewest_rows(const Shape& sh) { return sh.lpr > 0 && sh.lpr < 64 ? 1 : 2; }
 int rows_per_chunk(const Shape& sh, int64_t N, int n_cu) {
   const int64_t target = (int64_t)WGS_PER_CU * n_cu * sh.rows();
@@ -287,6 +332,7 @@ void plan(ResNormArgs& a, const Shape& sh) {
     a.chunk_rows = T <= rows ? rows / T * T : T;
   }
   a.chunks = (a.N + a.chunk_rows - 1) / a.chunk_rows;
+  if (!(a.gate && a.gate_rows > 1)) a.chunk_rows = (a.N + a.chunks - 1) / a.chunks;
   a.parts = (a.chunks + sh.rows() - 1) / sh.rows();
 }
 
@@ -321,7 +367,7 @@ int64_t mxm_resnorm_max_parts(int64_t max_rows, int D, bool groups, int n_cu) {
   // N / T + 1 of them: N / R + T / R + N / T + 1 <= 3 N / R + 1.
   int64_t most = 0;
   for (const bool vectors : {false, true}) {
-    const Shape sh = shape_of(D, vectors);
+    const Shape sh = shape_of(D, vectors, true);
     const int64_t R = (int64_t)sh.rows() * fewest_rows(sh);
     most = std::max(most, std::min<int64_t>((int64_t)WGS_PER_CU * n_cu, (max_rows + R - 1) / R));
   }
@@ -334,7 +380,7 @@ bool mxm_launch_resnorm_bw(const ResNormArgs& args, hipStream_t s) {
       a.D % 4 == 0 && (!a.norm || (aligned(a.h, a.x_bf16) && aligned(a.dy, a.g_bf16))) &&
       (!a.branch || (aligned(a.delta, a.delta_bf16) && aligned(a.d_delta, a.g_bf16))) &&
       aligned(a.dh, a.g_bf16) && aligned(a.dx, a.g_bf16);
-  const Shape sh = shape_of(a.D, vectors);
+  const Shape sh = shape_of(a.D, vectors, true);
   a.chunks = a.parts = a.group_chunks = a.group_parts = 0;
   if (a.N > 0) {
     plan(a, sh);
