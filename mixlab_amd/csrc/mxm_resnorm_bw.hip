@@ -84,6 +84,8 @@ __global__ __launch_bounds__(most_threads(LPR)) void resnorm_bw_kernel(ResNormAr
   // (values past the row's end and rows past the chunk's are zero)
   auto fetch = [&](int it) {
     const size_t row = ((size_t)mine.first + (size_t)it * mine.step) * D;
+    if (row_gate && it < mine.count)
+      load_scale<1>(a.gatep, a.p_bf16, (size_t)mine.first + (size_t)it * mine.step, &rg);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       rh[i] = Raw<XT, V>{};
@@ -99,8 +101,6 @@ __global__ __launch_bounds__(most_threads(LPR)) void resnorm_bw_kernel(ResNormAr
         if (a.dh) rt[i] = load<GT, V>(a.dh, a.g_bf16, row + at[i]);
       }
     }
-    if (row_gate && it < mine.count)
-      load_scale<1>(a.gatep, a.p_bf16, (size_t)mine.first + (size_t)it * mine.step, &rg);
   };
   if (LPR >= 0) fetch(0);
   // (the same number of rounds in every lane: the sums use whole waves)
@@ -298,16 +298,17 @@ __global__ __launch_bounds__(JOIN_COLS* JOIN_SLICES) void resnorm_join_kernel(Re
   }
 }
 
-// Chunks that a backward of N rows aims at: WGS_PER_CU workgroups a CU, of no
-// fewer rows than pay for a partial.  134 M elements in fp32 at 64, 512, 1024,
-// 2048 and 4096 channels with 2 / 4 / 8 workgroups a CU: 556 / 599 / 612, 545 /
-// 603 / 608, 576 / 589 / 593, 568 / 659 / 645 and 564 / 628 / 664 us (5.7 TB/s
-// with 2): each has its next row's loads on their way, and fewer streams at once
-// suit the memory better.
-constexpr int WGS_PER_CU = 2;
+// Chunks that a backward of N rows aims at: some workgroups a CU, of no fewer
+// rows than pay for a partial.  134 M elements in fp32 at 512, 1024, 2048 and 4096
+// channels with 2 / 4 / 8 workgroups a CU: 545 / 603 / 608, 576 / 589 / 593, 568 /
+// 659 / 645 and 564 / 628 / 664 us (5.7 TB/s with 2): each has its next row's loads
+// on their way, and fewer streams at once suit the memory better.  Rows of one
+// vector a thread need 4 for as many bytes on their way (64 and 256 channels 655
+// / 629 and 637 / 629).
+int wgs_per_cu(const Shape& sh) { return sh.NV == 1 ? 4 : 2; }
 int fewest_rows(const Shape& sh) { return sh.lpr > 0 && sh.lpr < 64 ? 1 : 2; }
 int rows_per_chunk(const Shape& sh, int64_t N, int n_cu) {
-  const int64_t target = (int64_t)WGS_PER_CU * n_cu * sh.rows();
+  const int64_t target = (int64_t)wgs_per_cu(sh) * n_cu * sh.rows();
   return (int)std::max<int64_t>((N + target - 1) / target, fewest_rows(sh));
 }
 
@@ -369,7 +370,7 @@ int64_t mxm_resnorm_max_parts(int64_t max_rows, int D, bool groups, int n_cu) {
   for (const bool vectors : {false, true}) {
     const Shape sh = shape_of(D, vectors, true);
     const int64_t R = (int64_t)sh.rows() * fewest_rows(sh);
-    most = std::max(most, std::min<int64_t>((int64_t)WGS_PER_CU * n_cu, (max_rows + R - 1) / R));
+    most = std::max(most, std::min<int64_t>((int64_t)wgs_per_cu(sh) * n_cu, (max_rows + R - 1) / R));
   }
   return groups ? 3 * most + 1 : most;
 }
