@@ -55,6 +55,13 @@ class Dev:
         d.ptr = d.buf.value + shift * item
         return d
 
+    def put(self, a):
+        """Other values of the same type (fp32 or whole numbers) in place."""
+        a = np.ascontiguousarray(a, self.np_dtype)
+        assert a.size == self.size and self.dtype != "bf16"
+        if a.size:
+            _lib.check(_lib.load().mxm_memcpy_h2d(self.ptr, a.ctypes.data, a.nbytes), "mxm_memcpy_h2d")
+
     def get(self):
         """The values (bf16 widened to fp32); whatever lies around them is untouched."""
         item = self.np_dtype.itemsize
