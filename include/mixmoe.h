@@ -366,10 +366,11 @@ int64_t mxm_grads_create(const int64_t* sizes, const int32_t* dtypes, const floa
                          int64_t stream_of);
 int mxm_grads_destroy(int64_t h);
 
-/* Where the tensors are: host arrays of n device pointers.  clipped (the type
- * of the gradients) is where mxm_grads_clip writes, NULL: in place.  params, m
- * and v (fp32) are AdamW's, all or none; params_bf16, or NULL, gets the updated
- * params rounded to bf16.  Waits for the handle's stream; calls use the
+/* Where the tensors are: host arrays of n device pointers (any value for a tensor
+ * of no elements).  clipped (the type of the gradients) is where mxm_grads_clip
+ * writes, NULL or the gradient's own pointer: in place.  params, m and v (fp32)
+ * are AdamW's, all or none; params_bf16, or NULL, gets the updated params
+ * rounded to bf16.  No two of the tensors may overlap.  Waits for the handle's stream; calls use the
  * pointers bound last, those captured into a graph too. */
 int mxm_grads_bind(int64_t h, const void* const* grads, void* const* clipped, void* const* params,
                    void* const* m, void* const* v, void* const* params_bf16);

@@ -202,7 +202,7 @@ __device__ __forceinline__ void each_other(const Slice& s, int V, int count, int
 }
 
 __global__ __launch_bounds__(THREADS) void grad_clip_kernel(GradArgs a) {
-  const int b = (int)gridDim.x - 1 - (int)blockIdx.x;
+  const int b = a.first_slice - (int)blockIdx.x;
   const GradChunk k = a.chunks[b / a.slices];
   const float coef = a.scalars->coef;
   const bool bf = k.bf16 != 0;
@@ -247,7 +247,7 @@ __device__ __forceinline__ void adamw_one(const AdamScalars& r, float g, float& 
 }
 
 __global__ __launch_bounds__(THREADS) void grad_adamw_kernel(GradArgs a) {
-  const int b = (int)gridDim.x - 1 - (int)blockIdx.x;
+  const int b = a.first_slice - (int)blockIdx.x;
   const GradChunk k = a.chunks[b / a.slices];
   const GradScalars sc = *a.scalars;
   if (sc.skip) return;
@@ -324,11 +324,22 @@ void mxm_launch_grad_norm(const GradArgs& a, hipStream_t s) {
   if (blocks > TICKET_BLOCKS)
     hipLaunchKernelGGL(grad_norm_finish_kernel, dim3(1), dim3(THREADS), 0, s, a, blocks);
 }
+// f(a, workgroups) for all of a's slices, the last first, in launches whose threads
+// are counted in 32 bits.
+template <class F>
+void each_launch(GradArgs a, F f) {
+  constexpr int MOST = 1 << 23;
+  for (int64_t left = (int64_t)a.n_chunks * a.slices; left > 0; left -= MOST) {
+    a.first_slice = (int)(left - 1);
+    f(a, (unsigned)std::min<int64_t>(left, MOST));
+  }
+}
 void mxm_launch_grad_clip(const GradArgs& args, hipStream_t s) {
   GradArgs a = args;
   a.slices = a.chunk_elems / (THREADS * (a.all_bf16 ? 8 : 4));
-  if (a.n_chunks > 0)
-    hipLaunchKernelGGL(grad_clip_kernel, dim3(a.n_chunks * a.slices), dim3(THREADS), 0, s, a);
+  each_launch(a, [&](const GradArgs& l, unsigned blocks) {
+    hipLaunchKernelGGL(grad_clip_kernel, dim3(blocks), dim3(THREADS), 0, s, l);
+  });
 }
 void mxm_launch_grad_adamw(const GradArgs& args, hipStream_t s) {
   GradArgs a = args;
@@ -339,6 +350,7 @@ void mxm_launch_grad_adamw(const GradArgs& args, hipStream_t s) {
   a.c2 = (float)(1.0 - a.beta2);
   a.eps32 = (float)a.eps;
   a.lr_decay = (float)(a.lr * a.weight_decay);
-  if (a.n_chunks > 0)
-    hipLaunchKernelGGL(grad_adamw_kernel, dim3(a.n_chunks * a.slices), dim3(THREADS), 0, s, a);
+  each_launch(a, [&](const GradArgs& l, unsigned blocks) {
+    hipLaunchKernelGGL(grad_adamw_kernel, dim3(blocks), dim3(THREADS), 0, s, l);
+  });
 }

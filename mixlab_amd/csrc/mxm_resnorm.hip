@@ -119,7 +119,9 @@ __global__ __launch_bounds__(most_threads(LPR)) void resnorm_kernel(ResNormArgs 
 int rows_per_thread(const ResNormArgs& a, const Shape& sh) {
   const int64_t rounds = ((int64_t)a.N + sh.rows() - 1) / sh.rows();
   const int most = a.x_bf16 && (a.delta_bf16 || !a.branch) ? 4 : 2;
-  return (int)std::min<int64_t>(std::max<int64_t>(rounds / (8 * a.n_cu), 1), most);
+  // (a launch's threads are counted in 32 bits)
+  const int64_t least = (rounds * sh.threads + ((int64_t)1 << 31) - 1) >> 31;
+  return (int)std::max(std::min<int64_t>(std::max<int64_t>(rounds / (8 * a.n_cu), 1), most), least);
 }
 
 template <int V, int NV, int LPR, int XT, int DT, int YT>

@@ -106,7 +106,7 @@ __global__ __launch_bounds__(most_threads(LPR)) void resnorm_bw_kernel(ResNormAr
   // (the same number of rounds in every lane: the sums use whole waves)
   const int rounds = LPR > 0 ? a.chunk_rows : mine.count;
   for (int it = 0; it < rounds; ++it) {
-    const bool valid = it < mine.count;
+    const bool valid = LPR <= 0 || it < mine.count;
     const size_t row = ((size_t)mine.first + (size_t)it * mine.step) * D;
     float h[E], dl[E], t[E], dy[E];
     if (LPR < 0) fetch(it);
@@ -150,7 +150,7 @@ __global__ __launch_bounds__(most_threads(LPR)) void resnorm_bw_kernel(ResNormAr
 #pragma unroll
       for (int e = 0; e < E; ++e) {
         t[e] = __builtin_fmaf(-kn, h[e], __builtin_fmaf(rn, w[e] * dy[e], t[e]));
-        aw[e] = __builtin_fmaf(rn, dy[e] * h[e], aw[e]);  // (rows past the chunk's: dy is 0)
+        if (valid) aw[e] = __builtin_fmaf(rn, dy[e] * h[e], aw[e]);
       }
     }
 #pragma unroll
@@ -173,10 +173,12 @@ __global__ __launch_bounds__(most_threads(LPR)) void resnorm_bw_kernel(ResNormAr
       const float g = CH ? 1.0f : ga[0];
 #pragma unroll
       for (int e = 0; e < E; ++e) {
-        const float td = t[e] * dl[e];  // (0 in rows past the chunk's: delta is)
+        const float td = t[e] * dl[e];
         const float gt = CH ? ga[CH ? e : 0] * td : td;
-        aq[e] = __builtin_fmaf(g * rp, gt, aq[e]);
-        if (CH) ag[CH ? e : 0] = __builtin_fmaf(rp * f[e], td, ag[CH ? e : 0]);
+        if (valid) {  // (past the chunk's rows 1 / sqrt(eps) or a gate times 0 need not be 0)
+          aq[e] = __builtin_fmaf(g * rp, gt, aq[e]);
+          if (CH) ag[CH ? e : 0] = __builtin_fmaf(rp * f[e], td, ag[CH ? e : 0]);
+        }
         q[0] = __builtin_fmaf(f[e], gt, q[0]);
       }
       if (post || a.gate == 1) row_sum<LPR>(q, red + 96 + (it & 1) * 16);

@@ -77,7 +77,8 @@ struct GradArgs {
   int n_chunks;
   int chunk_elems;       // elements of a chunk (a tensor's last one may be shorter)
   bool all_bf16;         // every tensor's gradients are bf16
-  int slices;            // workgroups per chunk (set by the launchers of clip and AdamW)
+  int slices;            // workgroups per chunk, and the one that a launch's first
+  int first_slice;       // workgroup takes (set by the launchers of clip and AdamW)
   double* partial;       // [n_chunks or fewer]
   int32_t* ticket;       // zero between calls
   GradScalars* scalars;

@@ -345,7 +345,7 @@ int64_t mxm_grads_create(const int64_t* sizes, const int32_t* dtypes, const floa
       g->tensors.push_back({sizes[i], dtypes[i] == MXM_DTYPE_BF16, decay ? decay[i] : 1.0f});
       pieces += (sizes[i] + per - 1) / per;
     }
-    // (a launch's workgroups, at most 16 a piece, are counted in 31 bits)
+    // (slices, at most 16 a piece, are counted in 31 bits)
     if (pieces > (INT32_MAX >> 4)) fail(GRADSET " too many pieces (%lld)", (long long)pieces);
     g->chunks.alloc((size_t)pieces * sizeof(GradChunk));
     g->partial.alloc((size_t)mxm_grad_norm_blocks((int)pieces) * sizeof(double));
@@ -378,6 +378,12 @@ int mxm_grads_bind(int64_t h, const void* const* grads, void* const* clipped, vo
       fail(GRADSET " params, m and v are bound together");
     if (params_bf16 && !params) fail(GRADSET " params_bf16 needs params");
     const int64_t per = g->base.chunk_elems;
+    struct Extent {
+      uintptr_t from, to;
+      size_t tensor;
+      const char* name;
+    };
+    std::vector<Extent> extents;
     std::vector<GradChunk> chunks;
     chunks.reserve((size_t)g->base.n_chunks);
     for (size_t i = 0; i < g->tensors.size(); ++i) {
@@ -390,10 +396,12 @@ int mxm_grads_bind(int64_t h, const void* const* grads, void* const* clipped, vo
         if (!p) fail(GRADSET " tensor %zu: %s is NULL", i, name);
         if (reinterpret_cast<uintptr_t>(p) % (bf16 ? 2 : 4) != 0)
           fail(GRADSET " tensor %zu: %s is not aligned to its elements", i, name);
+        const uintptr_t from = reinterpret_cast<uintptr_t>(p);
+        extents.push_back({from, from + (uintptr_t)t.n * (bf16 ? 2 : 4), i, name});
         return static_cast<char*>(const_cast<void*>(p));
       };
       char* const gp = take("grads", grads, t.bf16);
-      char* const cp = clipped ? take("clipped", clipped, t.bf16) : gp;
+      char* const cp = clipped && clipped[i] != gp ? take("clipped", clipped, t.bf16) : gp;
       char* const pp = take("params", params, false);
       char* const mp = take("m", m, false);
       char* const vp = take("v", v, false);
@@ -415,6 +423,12 @@ int mxm_grads_bind(int64_t h, const void* const* grads, void* const* clipped, vo
         chunks.push_back(c);
       }
     }
+    std::sort(extents.begin(), extents.end(),
+              [](const Extent& a, const Extent& b) { return a.from < b.from; });
+    for (size_t k = 1; k < extents.size(); ++k)
+      if (extents[k].from < extents[k - 1].to)
+        fail(GRADSET " tensor %zu: %s overlaps tensor %zu's %s", extents[k].tensor, extents[k].name,
+             extents[k - 1].tensor, extents[k - 1].name);
     const DeviceGuard guard(g->stream_ref->device);
     // (waits for the calls that read the table, then for the copy)
     if (!chunks.empty())

@@ -181,6 +181,9 @@ def test_refusals(gpu_lib):
     a = Dev(np.zeros(64, np.float32))
     step = Dev(np.zeros(1, np.int64), "int64")
     E = _lib.MixMoEError
+    with GradientSet([8, 8]) as s:
+        with pytest.raises(E, match="tensor 1: grads overlaps tensor 0's grads|tensor 0: grads overlaps"):
+            s.bind([a.ptr, a.ptr])
     with GradientSet([16, 0]) as s:
         with pytest.raises(E, match="before mxm_grads_bind"):
             s.norm(a.ptr)
@@ -188,6 +191,10 @@ def test_refusals(gpu_lib):
             s.bind([0, 0])
         with pytest.raises(E, match="tensor 0: grads is not aligned"):
             s.bind([a.ptr + 2, 0])
+        with pytest.raises(E, match="tensor 0: clipped overlaps tensor 0's grads"):
+            s.bind([a.ptr, 0], clipped=[a.ptr + 4, 0])
+        with pytest.raises(E, match="overlaps"):
+            s.bind([a.ptr, 0], params=[a.ptr + 64, 0], m=[a.ptr + 128, 0], v=[a.ptr + 128, 0])
         with pytest.raises(E, match="bound together"):
             s.bind([a.ptr, 0], params=[a.ptr, 0])
         with pytest.raises(E, match="needs params"):

@@ -285,6 +285,29 @@ def test_in_place(gpu_lib, D, dtype):
         assert np.array_equal(dh.get(), g["dx"]) and np.array_equal(dy.get(), g["d_delta"])
 
 
+@pytest.mark.parametrize("N,D", [(7, 20), (33, 100), (9, 300), (21, 1000)])
+@pytest.mark.parametrize("gate", [None, "channel"])
+def test_no_epsilon_and_an_infinite_gate(gpu_lib, N, D, gate):
+    """eps 0, numbers of rows that leave threads without one, and an infinite gate in
+    the last group: only what reads it is not finite."""
+    c = dict(gate=gate, gate_rows=4)
+    v = _case(N, N, D, **c)
+    from mixlab_amd.train import ResidualNorm
+    with ResidualNorm(D, N, out_dtype="fp32", post_norm=True, eps=0.0, gate=gate, gate_rows=4) as r:
+        good = run_backward(v, N, D, handle=r, **c)
+        assert all(np.isfinite(a).all() for a in good.values())
+        if gate:
+            v["gate"][-1, 3] = np.inf
+            bad = run_backward(v, N, D, handle=r, **c)
+            rows = (N - 1) // 4 * 4
+            assert np.array_equal(bad["dx"], good["dx"])
+            assert np.array_equal(bad["d_delta"][:rows], good["d_delta"][:rows])
+            other = np.arange(D) != 3
+            for k in ("d_scale", "d_post"):
+                assert np.array_equal(bad[k][other], good[k][other]) and not np.isfinite(bad[k][3])
+            assert np.array_equal(bad["d_gate"], good["d_gate"])
+
+
 def test_refusals(gpu_lib):
     N, D = 4, 32
     v = _case(0, N, D)
