@@ -2,11 +2,17 @@
 // loads and stores, sums over a row.
 //
 // A row is held in registers from its one load to its last use, and the next
-// row's loads are on their way meanwhile.  V consecutive elements (16 bytes of
-// fp32) lie in a thread, NV such vectors a thread; LPR threads of a wave hold a
-// row (rows side by side in the wave), or, with LPR 0, a workgroup of a row's
+// row's loads are on their way meanwhile.  V = 4 consecutive elements (16 bytes
+// of fp32) lie in a thread, NV such vectors a thread; LPR threads of a wave hold
+// a row (rows side by side in the wave), or, with LPR 0, a workgroup of a row's
 // length does (LPR -1: one of over 512 threads, whose registers do not hold a
-// second row).  V = 4 needs D % 4 == 0 and aligned tensors; V = 1 takes any.
+// second row).
+//
+// Kernels of known types need D % 4 == 0 and tensors aligned to their vectors;
+// those of Kind ANY take the rest: the part's vector loads and stores need no
+// more than an element's alignment, and a row's last vector may be short.
+// Element loads instead took 599 us for 130,308 rows of 1030 channels, forwards
+// in fp32, where aligned rows of 1024 take 303.
 #pragma once
 
 #include <type_traits>
@@ -21,86 +27,133 @@ constexpr int THREADS = 256;  // of a workgroup that holds several rows
 typedef float f4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u2 __attribute__((ext_vector_type(2)));
 
+// The same at any element's address.
+typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t u2u __attribute__((ext_vector_type(2), aligned(2)));
+
 enum Kind { F32 = 0, BF16 = 1, ANY = 2 };  // ANY: `bf` says
 
-// V elements as they come from memory.
-template <int K, int V>
-using Raw = std::conditional_t<V == 4, std::conditional_t<K == BF16, u2, f4>, float>;
+constexpr int V = 4;
 
-template <int K, int V>
-__device__ __forceinline__ Raw<K, V> load(const void* p, bool bf, size_t i) {
-  if constexpr (V == 4 && K == BF16)
-    return __builtin_nontemporal_load(
-        reinterpret_cast<const u2*>(static_cast<const uint16_t*>(p) + i));
-  else if constexpr (V == 4)
-    return __builtin_nontemporal_load(
-        reinterpret_cast<const f4*>(static_cast<const float*>(p) + i));
-  else
-    return bf ? mxm_bf2f(static_cast<const uint16_t*>(p)[i]) : static_cast<const float*>(p)[i];
+// V elements as they come from memory (ANY: bf16 in the first two words).
+template <int K>
+using Raw = std::conditional_t<K == BF16, u2, f4>;
+
+__device__ __forceinline__ void widen(u2 w, float* out) {
+  out[0] = mxm_u2f(w[0] << 16);
+  out[1] = mxm_u2f(w[0] & 0xffff0000u);
+  out[2] = mxm_u2f(w[1] << 16);
+  out[3] = mxm_u2f(w[1] & 0xffff0000u);
 }
-template <int K, int V>
-__device__ __forceinline__ void unpack(const Raw<K, V>& w, float* out) {
-  if constexpr (V == 4 && K == BF16) {
-    out[0] = mxm_u2f(w[0] << 16);
-    out[1] = mxm_u2f(w[0] & 0xffff0000u);
-    out[2] = mxm_u2f(w[1] << 16);
-    out[3] = mxm_u2f(w[1] & 0xffff0000u);
-  } else if constexpr (V == 4) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) out[j] = w[j];
+
+// Elements [at, at + V) of a row of D that starts at p[row].  Of a row's short last
+// vector (ANY) these are the row's last V, which unpack moves down; a row
+// shorter than that is read by elements.
+template <int K>
+__device__ __forceinline__ Raw<K> load(const void* p, bool bf, size_t row, int at, int D) {
+  if constexpr (K == BF16) {
+    return __builtin_nontemporal_load(
+        reinterpret_cast<const u2*>(static_cast<const uint16_t*>(p) + row + at));
+  } else if constexpr (K == F32) {
+    return __builtin_nontemporal_load(
+        reinterpret_cast<const f4*>(static_cast<const float*>(p) + row + at));
   } else {
-    out[0] = w;
+    f4 r = {};
+    if (D < V) {  // (at is 0)
+      if (bf) {
+        u2 w = {};
+        for (int j = 0; j < D; ++j)
+          w[j >> 1] |= (uint32_t) static_cast<const uint16_t*>(p)[row + j] << (16 * (j & 1));
+        return f4{mxm_u2f(w[0]), mxm_u2f(w[1]), 0.0f, 0.0f};
+      }
+      r[0] = static_cast<const float*>(p)[row];
+      if (D > 1) r[1] = static_cast<const float*>(p)[row + 1];
+      if (D > 2) r[2] = static_cast<const float*>(p)[row + 2];
+      return r;
+    }
+    const size_t i = row + min(at, D - V);
+    if (bf) {
+      const u2 w = *reinterpret_cast<const u2u*>(static_cast<const uint16_t*>(p) + i);
+      return f4{mxm_u2f(w[0]), mxm_u2f(w[1]), 0.0f, 0.0f};
+    }
+    return *reinterpret_cast<const f4u*>(static_cast<const float*>(p) + i);
+  }
+}
+// Their values, zeros behind the row.
+template <int K>
+__device__ __forceinline__ void unpack(const Raw<K>& raw, bool bf, int at, int D, float* out) {
+  if constexpr (K == BF16) {
+    widen(raw, out);
+  } else if constexpr (K == F32) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) out[j] = raw[j];
+  } else {
+    const int over = D < V ? 0 : max(at + V - D, 0) & 3;  // (past the row all is 0)
+    if (bf) {
+      const uint64_t w = ((uint64_t)mxm_f2u(raw[1]) << 32 | mxm_f2u(raw[0])) >> (16 * over);
+      widen(u2{(uint32_t)w, (uint32_t)(w >> 32)}, out);
+    } else {
+      f4 w = raw;
+      if (over & 1) w = f4{w[1], w[2], w[3], 0.0f};
+      if (over & 2) w = f4{w[2], w[3], 0.0f, 0.0f};
+#pragma unroll
+      for (int j = 0; j < V; ++j) out[j] = w[j];
+    }
   }
 }
 
 // Rounds v to the type it is kept in; v holds the kept values afterwards.
-template <int K, int V>
-__device__ __forceinline__ void store(void* p, bool bf, size_t i, float* v) {
-  if constexpr (V == 4) {
-    if (K == BF16) {
-      const u2 w = {mxm_pack_bf2_fast(v[0], v[1]), mxm_pack_bf2_fast(v[2], v[3])};
-      __builtin_nontemporal_store(w, reinterpret_cast<u2*>(static_cast<uint16_t*>(p) + i));
-      v[0] = mxm_u2f(w[0] << 16);
-      v[1] = mxm_u2f(w[0] & 0xffff0000u);
-      v[2] = mxm_u2f(w[1] << 16);
-      v[3] = mxm_u2f(w[1] & 0xffff0000u);
+template <int K>
+__device__ __forceinline__ void store(void* p, bool bf, size_t i, int n, float* v) {
+  const u2 w = {mxm_pack_bf2_fast(v[0], v[1]), mxm_pack_bf2_fast(v[2], v[3])};
+  if constexpr (K == BF16) {
+    __builtin_nontemporal_store(w, reinterpret_cast<u2*>(static_cast<uint16_t*>(p) + i));
+    widen(w, v);
+  } else if constexpr (K == F32) {
+    __builtin_nontemporal_store(f4{v[0], v[1], v[2], v[3]},
+                                reinterpret_cast<f4*>(static_cast<float*>(p) + i));
+  } else if (bf) {
+    uint16_t* q = static_cast<uint16_t*>(p) + i;
+    if (n >= V) {
+      *reinterpret_cast<u2u*>(q) = w;
     } else {
-      __builtin_nontemporal_store(f4{v[0], v[1], v[2], v[3]},
-                                  reinterpret_cast<f4*>(static_cast<float*>(p) + i));
+      q[0] = (uint16_t)w[0];
+      if (n > 1) q[1] = (uint16_t)(w[0] >> 16);
+      if (n > 2) q[2] = (uint16_t)w[1];
     }
+    widen(w, v);
   } else {
-    if (bf) {
-      const uint16_t b = mxm_f2bf(v[0]);
-      static_cast<uint16_t*>(p)[i] = b;
-      v[0] = mxm_bf2f(b);
+    float* q = static_cast<float*>(p) + i;
+    if (n >= V) {
+      *reinterpret_cast<f4u*>(q) = f4u{v[0], v[1], v[2], v[3]};
     } else {
-      static_cast<float*>(p)[i] = v[0];
+      q[0] = v[0];
+      if (n > 1) q[1] = v[1];
+      if (n > 2) q[2] = v[2];
     }
   }
 }
 
-// V values of a scale or a gate, which many rows read; null: ones.
-template <int V>
-__device__ __forceinline__ void load_scale(const void* p, bool bf, size_t i, float* out) {
+__device__ __forceinline__ float load_one(const void* p, bool bf, size_t i) {
+  return bf ? mxm_bf2f(static_cast<const uint16_t*>(p)[i]) : static_cast<const float*>(p)[i];
+}
+// Values [at, at + V) of a scale, or of a gate's row, of D channels, which many rows
+// read; zeros behind them; null: ones.  K as the kernel's: unless ANY, D % V == 0.
+template <int K>
+__device__ __forceinline__ void load_scale(const void* p, bool bf, size_t row, int at, int D,
+                                           float* out) {
   if (!p) {
 #pragma unroll
-    for (int j = 0; j < V; ++j) out[j] = 1.0f;
-    return;
-  }
-  if constexpr (V == 4) {  // (whole vectors where the tensor starts at one's boundary)
-    if (!bf && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
-      unpack<F32, 4>(*reinterpret_cast<const f4*>(static_cast<const float*>(p) + i), out);
-      return;
-    }
-    if (bf && (reinterpret_cast<uintptr_t>(p) & 7) == 0) {
-      unpack<BF16, 4>(*reinterpret_cast<const u2*>(static_cast<const uint16_t*>(p) + i), out);
-      return;
-    }
-  }
+    for (int j = 0; j < V; ++j) out[j] = K != ANY || at + j < D ? 1.0f : 0.0f;
+  } else if constexpr (K == ANY) {
+    unpack<ANY>(load<ANY>(p, bf, row, at, D), bf, at, D, out);
+  } else if (bf) {
+    widen(*reinterpret_cast<const u2u*>(static_cast<const uint16_t*>(p) + row + at), out);
+  } else {
+    const f4u w = *reinterpret_cast<const f4u*>(static_cast<const float*>(p) + row + at);
 #pragma unroll
-  for (int j = 0; j < V; ++j)
-    out[j] = bf ? mxm_bf2f(static_cast<const uint16_t*>(p)[i + j])
-                : static_cast<const float*>(p)[i + j];
+    for (int j = 0; j < V; ++j) out[j] = w[j];
+  }
 }
 
 __device__ __forceinline__ float gate_of(const ResNormArgs& a, float g) {
@@ -141,23 +194,16 @@ __device__ __forceinline__ int row_slot() {
 
 // How rows of D elements lie in threads.
 struct Shape {
-  int V, NV, lpr, threads;
+  int NV, lpr, threads;
   int rows() const { return lpr > 0 ? threads / lpr : 1; }  // rows a workgroup holds at once
 };
-inline Shape shape_of(int D, bool vectors, bool backward) {
-  auto workgroup = [&](int V, int nv) {
-    const int per = V * nv * 64;
-    const int threads = (D + per - 1) / per * 64;
-    return Shape{V, nv, threads > 512 ? -1 : 0, threads};
-  };
-  if (vectors) {
-    if (D <= 64) return {4, 1, 16, THREADS};
-    if (D <= 128) return {4, 1, 32, THREADS};
-    if (D <= 1024) return {4, (D + 255) / 256, 64, THREADS};
-    return workgroup(4, D <= (backward ? 8192 : 4096) ? 2 : 4);
-  }
-  if (D <= 256) return {1, 4, 64, THREADS};
-  return workgroup(1, D <= 2048 ? 4 : D <= 4096 ? 8 : 16);
+inline Shape shape_of(int D, bool backward) {
+  if (D <= 64) return {1, 16, THREADS};
+  if (D <= 128) return {1, 32, THREADS};
+  if (D <= 1024) return {(D + 255) / 256, 64, THREADS};
+  const int nv = D <= (backward ? 8192 : 4096) ? 2 : 4, per = V * nv * 64;
+  const int threads = (D + per - 1) / per * 64;
+  return {nv, threads > 512 ? -1 : 0, threads};
 }
 constexpr int most_threads(int lpr) { return lpr > 0 ? THREADS : lpr == 0 ? 512 : 1024; }
 
@@ -165,9 +211,9 @@ inline bool aligned(const void* p, bool bf16) {
   return reinterpret_cast<uintptr_t>(p) % (bf16 ? 8 : 16) == 0;
 }
 
-// f(NV, LPR) of a shape with vectors of 4, or of one without (std::integral_constants).
-template <class F>
-void with_shape4(const Shape& sh, F f) {
+// f(NV, LPR) of a shape_of(D, BACKWARD) (std::integral_constants).
+template <bool BACKWARD, class F>
+void with_shape(const Shape& sh, F f) {
   using std::integral_constant;
 #define MXM_CASE(nv, l) return f(integral_constant<int, nv>(), integral_constant<int, l>())
   if (sh.lpr == 16) MXM_CASE(1, 16);
@@ -179,24 +225,22 @@ void with_shape4(const Shape& sh, F f) {
     MXM_CASE(4, 64);
   }
   if (sh.NV == 2 && sh.lpr == 0) MXM_CASE(2, 0);
-  if (sh.NV == 2) MXM_CASE(2, -1);
-  if (sh.lpr == 0) MXM_CASE(4, 0);
+  if constexpr (BACKWARD) {
+    if (sh.NV == 2) MXM_CASE(2, -1);
+  } else {
+    if (sh.lpr == 0) MXM_CASE(4, 0);
+  }
   MXM_CASE(4, -1);
-}
-template <class F>
-void with_shape1(const Shape& sh, F f) {
-  using std::integral_constant;
-  if (sh.lpr == 64) MXM_CASE(4, 64);
-  if (sh.NV == 4) MXM_CASE(4, 0);
-  if (sh.NV == 8) MXM_CASE(8, 0);
-  if (sh.lpr == 0) MXM_CASE(16, 0);
-  MXM_CASE(16, -1);
 #undef MXM_CASE
 }
-// f(K0, K1, K2) of three types.
+// f(K0, K1, K2) of three types, or of ANY.
 template <class F>
-void with_types(bool bf0, bool bf1, bool bf2, F f) {
+void with_types(bool known, bool bf0, bool bf1, bool bf2, F f) {
   using std::integral_constant;
+  if (!known) {
+    constexpr integral_constant<int, ANY> any;
+    return f(any, any, any);
+  }
   auto k = [](auto bf) { return integral_constant<int, decltype(bf)::value ? BF16 : F32>(); };
   auto third = [&](auto a, auto b) { bf2 ? f(a, b, k(std::true_type())) : f(a, b, k(std::false_type())); };
   auto second = [&](auto a) { bf1 ? third(a, k(std::true_type())) : third(a, k(std::false_type())); };

@@ -34,9 +34,10 @@ __device__ __forceinline__ Rows rows_of(const ResNormArgs& a, int c) {
 
 // CH: a gate per channel.  A row's threads walk one chunk; the chunks of a
 // workgroup add their column sums in LDS and store one partial.
-template <int V, int NV, int LPR, int XT, int DT, int GT, bool CH>
+template <int NV, int LPR, int XT, int DT, int GT, bool CH>
 __global__ __launch_bounds__(most_threads(LPR)) void resnorm_bw_kernel(ResNormArgs a) {
   constexpr int E = V * NV;
+  constexpr bool full = XT != ANY;  // every vector of a row is whole
   // of a row's sums (a workgroup a row), or of the workgroup's column sums at the end
   __shared__ float red[LPR > 0 ? THREADS * E : 2 * 16 * 3 + 2 * 16];
   const int lane = LPR > 0 ? threadIdx.x % (LPR > 0 ? LPR : 1) : threadIdx.x;
@@ -59,12 +60,12 @@ __global__ __launch_bounds__(most_threads(LPR)) void resnorm_bw_kernel(ResNormAr
     if (at[i] < D) {
       if (a.branch) {
         float p[V];
-        load_scale<V>(a.scale, a.p_bf16, at[i], f + i * V);
-        load_scale<V>(a.post, a.p_bf16, at[i], p);
+        load_scale<XT>(a.scale, a.p_bf16, 0, at[i], D, f + i * V);
+        load_scale<XT>(a.post, a.p_bf16, 0, at[i], D, p);
 #pragma unroll
         for (int j = 0; j < V; ++j) f[i * V + j] *= p[j];
       }
-      if (a.norm) load_scale<V>(a.w, a.p_bf16, at[i], w + i * V);
+      if (a.norm) load_scale<XT>(a.w, a.p_bf16, 0, at[i], D, w + i * V);
     }
   }
   if (!CH) {
@@ -76,29 +77,29 @@ __global__ __launch_bounds__(most_threads(LPR)) void resnorm_bw_kernel(ResNormAr
   // the chunk's rows before its group ends: whole groups (in a row), or one group
   int left = a.group_chunks > 0 ? mine.count : a.gate_rows;
   bool fresh = true;  // the group's gate is not loaded yet
-  Raw<XT, V> rh[NV];
-  Raw<DT, V> rd[NV];
-  Raw<GT, V> rt[NV], ry[NV];
+  Raw<XT> rh[NV];
+  Raw<DT> rd[NV];
+  Raw<GT> rt[NV], ry[NV];
   float rg = 0.0f;  // a gate of the row alone
   const bool row_gate = !CH && a.gate && a.gate_rows == 1;
   // (values past the row's end and rows past the chunk's are zero)
   auto fetch = [&](int it) {
     const size_t row = ((size_t)mine.first + (size_t)it * mine.step) * D;
     if (row_gate && it < mine.count)
-      load_scale<1>(a.gatep, a.p_bf16, (size_t)mine.first + (size_t)it * mine.step, &rg);
+      rg = load_one(a.gatep, a.p_bf16, (size_t)mine.first + (size_t)it * mine.step);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      rh[i] = Raw<XT, V>{};
-      rd[i] = Raw<DT, V>{};
-      rt[i] = Raw<GT, V>{};
-      ry[i] = Raw<GT, V>{};
+      rh[i] = Raw<XT>{};
+      rd[i] = Raw<DT>{};
+      rt[i] = Raw<GT>{};
+      ry[i] = Raw<GT>{};
       if (it < mine.count && at[i] < D) {
         if (a.norm) {
-          rh[i] = load<XT, V>(a.h, a.x_bf16, row + at[i]);
-          ry[i] = load<GT, V>(a.dy, a.g_bf16, row + at[i]);
+          rh[i] = load<XT>(a.h, a.x_bf16, row, at[i], D);
+          ry[i] = load<GT>(a.dy, a.g_bf16, row, at[i], D);
         }
-        if (a.branch) rd[i] = load<DT, V>(a.delta, a.delta_bf16, row + at[i]);
-        if (a.dh) rt[i] = load<GT, V>(a.dh, a.g_bf16, row + at[i]);
+        if (a.branch) rd[i] = load<DT>(a.delta, a.delta_bf16, row, at[i], D);
+        if (a.dh) rt[i] = load<GT>(a.dh, a.g_bf16, row, at[i], D);
       }
     }
   };
@@ -112,10 +113,10 @@ __global__ __launch_bounds__(most_threads(LPR)) void resnorm_bw_kernel(ResNormAr
     if (LPR < 0) fetch(it);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      unpack<XT, V>(rh[i], h + i * V);
-      unpack<DT, V>(rd[i], dl + i * V);
-      unpack<GT, V>(rt[i], t + i * V);
-      unpack<GT, V>(ry[i], dy + i * V);
+      unpack<XT>(rh[i], a.x_bf16, at[i], D, h + i * V);
+      unpack<DT>(rd[i], a.delta_bf16, at[i], D, dl + i * V);
+      unpack<GT>(rt[i], a.g_bf16, at[i], D, t + i * V);
+      unpack<GT>(ry[i], a.g_bf16, at[i], D, dy + i * V);
     }
     // (the gate's values go through the sigmoid after the sums, which hide its load)
     const bool new_gate = a.gate && fresh && valid;
@@ -126,9 +127,9 @@ __global__ __launch_bounds__(most_threads(LPR)) void resnorm_bw_kernel(ResNormAr
 #pragma unroll
         for (int i = 0; i < NV; ++i)
           if (at[i] < D)
-            load_scale<V>(a.gatep, a.p_bf16, (size_t)group * D + at[i], ga + (CH ? i * V : 0));
+            load_scale<XT>(a.gatep, a.p_bf16, (size_t)group * D, at[i], D, ga + (CH ? i * V : 0));
       } else {
-        load_scale<1>(a.gatep, a.p_bf16, (size_t)group, ga);
+        ga[0] = load_one(a.gatep, a.p_bf16, (size_t)group);
       }
     }
     float s[3] = {0.0f, 0.0f, 0.0f};
@@ -159,7 +160,7 @@ __global__ __launch_bounds__(most_threads(LPR)) void resnorm_bw_kernel(ResNormAr
       float out[V];
 #pragma unroll
       for (int j = 0; j < V; ++j) out[j] = t[i * V + j];
-      store<GT, V>(a.dx, a.g_bf16, row + at[i], out);
+      store<GT>(a.dx, a.g_bf16, row + at[i], D - at[i], out);
     }
     if (new_gate) {
 #pragma unroll
@@ -194,7 +195,7 @@ __global__ __launch_bounds__(most_threads(LPR)) void resnorm_bw_kernel(ResNormAr
           const float gf = CH ? ga[CH ? e : 0] * f[e] : f[e];
           out[j] = __builtin_fmaf(-kp, dl[e], (g * rp) * (gf * t[e]));
         }
-        store<GT, V>(a.d_delta, a.g_bf16, row + at[i], out);
+        store<GT>(a.d_delta, a.g_bf16, row + at[i], D - at[i], out);
       }
     }
     // the group's last row here
@@ -211,7 +212,8 @@ __global__ __launch_bounds__(most_threads(LPR)) void resnorm_bw_kernel(ResNormAr
             for (int i = 0; i < NV; ++i)
               if (at[i] < D)
 #pragma unroll
-                for (int j = 0; j < V; ++j) out[at[i] + j] = ag[CH ? i * V + j : 0];
+                for (int j = 0; j < V; ++j)
+                  if (full || at[i] + j < D) out[at[i] + j] = ag[CH ? i * V + j : 0];
           } else if (lane == 0) {
             out[0] = ag[0];
           }
@@ -245,7 +247,8 @@ __global__ __launch_bounds__(most_threads(LPR)) void resnorm_bw_kernel(ResNormAr
       for (int i = 0; i < NV; ++i)
         if (at[i] < D)
 #pragma unroll
-          for (int j = 0; j < V; ++j) part[at[i] + j] = acc[i * V + j];
+          for (int j = 0; j < V; ++j)
+            if (full || at[i] + j < D) part[at[i] + j] = acc[i * V + j];
     }
   };
   if (a.norm && a.d_w) join(aw, a.part + (size_t)blockIdx.x * D);
@@ -287,14 +290,11 @@ __global__ __launch_bounds__(JOIN_COLS* JOIN_SLICES) void resnorm_join_kernel(Re
   if (slice != 0 || d >= width) return;
   s = 0.0f;
   for (int i = 0; i < JOIN_SLICES; ++i) s += red[i][col];
-  float other[1];
   if (kind == 0) {
     a.d_w[d] = s;
   } else if (kind == 1) {
-    load_scale<1>(a.post, a.p_bf16, d, other);
-    if (a.d_scale) a.d_scale[d] = s * other[0];
-    load_scale<1>(a.scale, a.p_bf16, d, other);
-    if (a.d_post) a.d_post[d] = s * other[0];
+    if (a.d_scale) a.d_scale[d] = a.post ? s * load_one(a.post, a.p_bf16, d) : s;
+    if (a.d_post) a.d_post[d] = a.scale ? s * load_one(a.scale, a.p_bf16, d) : s;
   } else {
     a.d_gate[(size_t)group * width + d] = s;
   }
@@ -339,25 +339,14 @@ void plan(ResNormArgs& a, const Shape& sh) {
   a.parts = (a.chunks + sh.rows() - 1) / sh.rows();
 }
 
-template <int V, int NV, int LPR, int XT, int DT, int GT>
+template <int NV, int LPR, int XT, int DT, int GT>
 void launch(const ResNormArgs& a, const Shape& sh, hipStream_t s) {
   if (a.gate == 2)
-    hipLaunchKernelGGL((resnorm_bw_kernel<V, NV, LPR, XT, DT, GT, true>), dim3(a.parts),
+    hipLaunchKernelGGL((resnorm_bw_kernel<NV, LPR, XT, DT, GT, true>), dim3(a.parts),
                        dim3(sh.threads), 0, s, a);
   else
-    hipLaunchKernelGGL((resnorm_bw_kernel<V, NV, LPR, XT, DT, GT, false>), dim3(a.parts),
+    hipLaunchKernelGGL((resnorm_bw_kernel<NV, LPR, XT, DT, GT, false>), dim3(a.parts),
                        dim3(sh.threads), 0, s, a);
-}
-
-void launch_rows(const ResNormArgs& a, const Shape& sh, hipStream_t s) {
-  if (sh.V == 4)
-    with_shape4(sh, [&](auto nv, auto lpr) {
-      with_types(a.x_bf16, a.delta_bf16, a.g_bf16, [&](auto xt, auto dt, auto gt) {
-        launch<4, nv(), lpr(), xt(), dt(), gt()>(a, sh, s);
-      });
-    });
-  else
-    with_shape1(sh, [&](auto nv, auto lpr) { launch<1, nv(), lpr(), ANY, ANY, ANY>(a, sh, s); });
 }
 
 }  // namespace
@@ -368,12 +357,9 @@ int64_t mxm_resnorm_max_parts(int64_t max_rows, int D, bool groups, int n_cu) {
   // whole groups hold more than half of the rows aimed at; groups that fill
   // workgroups (T >= R) have at most T / R + 1 parts each, and there are at most
   // N / T + 1 of them: N / R + T / R + N / T + 1 <= 3 N / R + 1.
-  int64_t most = 0;
-  for (const bool vectors : {false, true}) {
-    const Shape sh = shape_of(D, vectors, true);
-    const int64_t R = (int64_t)sh.rows() * fewest_rows(sh);
-    most = std::max(most, std::min<int64_t>((int64_t)wgs_per_cu(sh) * n_cu, (max_rows + R - 1) / R));
-  }
+  const Shape sh = shape_of(D, true);
+  const int64_t R = (int64_t)sh.rows() * fewest_rows(sh);
+  const int64_t most = std::min<int64_t>((int64_t)wgs_per_cu(sh) * n_cu, (max_rows + R - 1) / R);
   return groups ? 3 * most + 1 : most;
 }
 
@@ -383,12 +369,16 @@ bool mxm_launch_resnorm_bw(const ResNormArgs& args, hipStream_t s) {
       a.D % 4 == 0 && (!a.norm || (aligned(a.h, a.x_bf16) && aligned(a.dy, a.g_bf16))) &&
       (!a.branch || (aligned(a.delta, a.delta_bf16) && aligned(a.d_delta, a.g_bf16))) &&
       aligned(a.dh, a.g_bf16) && aligned(a.dx, a.g_bf16);
-  const Shape sh = shape_of(a.D, vectors, true);
+  const Shape sh = shape_of(a.D, true);
   a.chunks = a.parts = a.group_chunks = a.group_parts = 0;
   if (a.N > 0) {
     plan(a, sh);
     if (a.parts > a.max_parts) return false;
-    launch_rows(a, sh, s);
+    with_shape<true>(sh, [&](auto nv, auto lpr) {
+      with_types(vectors, a.x_bf16, a.delta_bf16, a.g_bf16, [&](auto xt, auto dt, auto gt) {
+        launch<nv(), lpr(), xt(), dt(), gt()>(a, sh, s);
+      });
+    });
   }
   // (without rows the scales' gradients are zero)
   const bool columns = (a.norm && a.d_w) || (a.branch && (a.d_scale || a.d_post));
