@@ -21,6 +21,26 @@ constexpr int UNROLL = 4;  // vectors in flight per thread and tensor
 typedef float f4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+// The same at any element's address.
+typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t u2u __attribute__((ext_vector_type(2), aligned(2)));
+typedef uint32_t u4u __attribute__((ext_vector_type(4), aligned(2)));
+
+// A vector that is read or written once; EVEN: at its own boundary.
+template <bool EVEN, class T, class U>
+__device__ __forceinline__ T get(const void* p, int i) {
+  if constexpr (EVEN)
+    return __builtin_nontemporal_load(static_cast<const T*>(p) + i);
+  else
+    return static_cast<const U*>(p)[i];
+}
+template <bool EVEN, class T, class U>
+__device__ __forceinline__ void put(void* p, int i, T v) {
+  if constexpr (EVEN)
+    __builtin_nontemporal_store(v, static_cast<T*>(p) + i);
+  else
+    static_cast<U*>(p)[i] = v;
+}
 
 __device__ __forceinline__ float lo16(uint32_t w) { return mxm_u2f(w << 16); }
 __device__ __forceinline__ float hi16(uint32_t w) { return mxm_u2f(w & 0xffff0000u); }
@@ -201,29 +221,37 @@ __device__ __forceinline__ void each_other(const Slice& s, int V, int count, int
   for (int i = s.head + s.n * V + s.at; i < count; i += slices * THREADS) f(i);
 }
 
+template <bool EVEN>
+__device__ __forceinline__ void clip_vector(const void* g, void* out, bool bf, int i, float coef) {
+  if (bf) {
+    const u4 w = get<EVEN, u4, u4u>(g, i);
+    u4 r;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) r[e] = mxm_pack_bf2_fast(lo16(w[e]) * coef, hi16(w[e]) * coef);
+    put<EVEN, u4, u4u>(out, i, r);
+  } else {
+    put<EVEN, f4, f4u>(out, i, get<EVEN, f4, f4u>(g, i) * coef);
+  }
+}
+
 __global__ __launch_bounds__(THREADS) void grad_clip_kernel(GradArgs a) {
   const int b = a.first_slice - (int)blockIdx.x;
   const GradChunk k = a.chunks[b / a.slices];
   const float coef = a.scalars->coef;
   const bool bf = k.bf16 != 0;
   const int V = bf ? 8 : 4, size = bf ? 2 : 4;
+  // (tensors out of step with each other: vectors at any address, from the start on)
   int head = min(head_of(k.g, size, V), k.count);
-  if (!meets(k.clipped, size, V, head)) head = k.count;
+  const bool even = meets(k.clipped, size, V, head);
+  if (!even) head = 0;
   const Slice s = slice_of(head, k.count, V, b % a.slices);
+  const char* g = static_cast<const char*>(k.g) + head * size;
+  char* out = static_cast<char*>(k.clipped) + head * size;
   if (s.at < s.n) {
-    if (bf) {
-      const u4* g = reinterpret_cast<const u4*>(static_cast<const uint16_t*>(k.g) + head);
-      u4* out = reinterpret_cast<u4*>(static_cast<uint16_t*>(k.clipped) + head);
-      const u4 w = __builtin_nontemporal_load(g + s.at);
-      u4 r;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) r[e] = mxm_pack_bf2_fast(lo16(w[e]) * coef, hi16(w[e]) * coef);
-      __builtin_nontemporal_store(r, out + s.at);
-    } else {
-      const f4* g = reinterpret_cast<const f4*>(static_cast<const float*>(k.g) + head);
-      f4* out = reinterpret_cast<f4*>(static_cast<float*>(k.clipped) + head);
-      __builtin_nontemporal_store(__builtin_nontemporal_load(g + s.at) * coef, out + s.at);
-    }
+    if (even)
+      clip_vector<true>(g, out, bf, s.at, coef);
+    else
+      clip_vector<false>(g, out, bf, s.at, coef);
   }
   each_other(s, V, k.count, a.slices, [&](int i) {
     const float g = grad_at(k.g, bf, i) * coef;
@@ -246,6 +274,34 @@ __device__ __forceinline__ void adamw_one(const AdamScalars& r, float g, float& 
   p = p - __builtin_fmaf(r.decay, p, u);
 }
 
+template <bool EVEN>
+__device__ __forceinline__ void adamw_vector(const GradChunk& k, const AdamScalars& r, int head,
+                                             int i) {
+  f4 g;
+  if (k.bf16) {
+    const u2 w = get<EVEN, u2, u2u>(static_cast<const uint16_t*>(k.g) + head, i);
+    g = f4{lo16(w[0]), hi16(w[0]), lo16(w[1]), hi16(w[1])};
+  } else {
+    g = get<EVEN, f4, f4u>(static_cast<const float*>(k.g) + head, i);
+  }
+  f4 m = get<EVEN, f4, f4u>(k.m + head, i), v = get<EVEN, f4, f4u>(k.v + head, i),
+     p = get<EVEN, f4, f4u>(k.p + head, i);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    float pe = p[e], me = m[e], ve = v[e];
+    adamw_one(r, g[e], pe, me, ve);
+    p[e] = pe;
+    m[e] = me;
+    v[e] = ve;
+  }
+  put<EVEN, f4, f4u>(k.m + head, i, m);
+  put<EVEN, f4, f4u>(k.v + head, i, v);
+  put<EVEN, f4, f4u>(k.p + head, i, p);
+  if (k.p16)
+    put<EVEN, u2, u2u>(k.p16 + head, i,
+                       u2{mxm_pack_bf2_fast(p[0], p[1]), mxm_pack_bf2_fast(p[2], p[3])});
+}
+
 __global__ __launch_bounds__(THREADS) void grad_adamw_kernel(GradArgs a) {
   const int b = a.first_slice - (int)blockIdx.x;
   const GradChunk k = a.chunks[b / a.slices];
@@ -253,9 +309,9 @@ __global__ __launch_bounds__(THREADS) void grad_adamw_kernel(GradArgs a) {
   if (sc.skip) return;
   const bool bf = k.bf16 != 0;
   int head = min(head_of(k.p, 4, 4), k.count);
-  if (!meets(k.m, 4, 4, head) || !meets(k.v, 4, 4, head) || !meets(k.g, bf ? 2 : 4, 4, head) ||
-      (k.p16 && !meets(k.p16, 2, 4, head)))
-    head = k.count;
+  const bool even = meets(k.m, 4, 4, head) && meets(k.v, 4, 4, head) &&
+                    meets(k.g, bf ? 2 : 4, 4, head) && (!k.p16 || meets(k.p16, 2, 4, head));
+  if (!even) head = 0;
   const Slice s = slice_of(head, k.count, 4, b % a.slices);
   AdamScalars r;
   r.coef = sc.coef;
@@ -268,33 +324,10 @@ __global__ __launch_bounds__(THREADS) void grad_adamw_kernel(GradArgs a) {
   r.eps = a.eps32;
   r.decay = a.lr_decay * k.decay;
   if (s.at < s.n) {
-    f4 *pp = reinterpret_cast<f4*>(k.p + head) + s.at, *mp = reinterpret_cast<f4*>(k.m + head) + s.at,
-       *vp = reinterpret_cast<f4*>(k.v + head) + s.at;
-    f4 g;
-    if (bf) {
-      const u2 w = __builtin_nontemporal_load(
-          reinterpret_cast<const u2*>(static_cast<const uint16_t*>(k.g) + head) + s.at);
-      g = f4{lo16(w[0]), hi16(w[0]), lo16(w[1]), hi16(w[1])};
-    } else {
-      g = __builtin_nontemporal_load(
-          reinterpret_cast<const f4*>(static_cast<const float*>(k.g) + head) + s.at);
-    }
-    f4 m = __builtin_nontemporal_load(mp), v = __builtin_nontemporal_load(vp),
-       p = __builtin_nontemporal_load(pp);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      float pe = p[e], me = m[e], ve = v[e];
-      adamw_one(r, g[e], pe, me, ve);
-      p[e] = pe;
-      m[e] = me;
-      v[e] = ve;
-    }
-    __builtin_nontemporal_store(m, mp);
-    __builtin_nontemporal_store(v, vp);
-    __builtin_nontemporal_store(p, pp);
-    if (k.p16)
-      __builtin_nontemporal_store(u2{mxm_pack_bf2_fast(p[0], p[1]), mxm_pack_bf2_fast(p[2], p[3])},
-                                  reinterpret_cast<u2*>(k.p16 + head) + s.at);
+    if (even)
+      adamw_vector<true>(k, r, head, s.at);
+    else
+      adamw_vector<false>(k, r, head, s.at);
   }
   each_other(s, 4, k.count, a.slices, [&](int i) {
     float p = k.p[i], m = k.m[i], v = k.v[i];

@@ -8,11 +8,12 @@
 // length does (LPR -1: one of over 512 threads, whose registers do not hold a
 // second row).
 //
-// Kernels of known types need D % 4 == 0 and tensors aligned to their vectors;
-// those of Kind ANY take the rest: the part's vector loads and stores need no
-// more than an element's alignment, and a row's last vector may be short.
-// Element loads instead took 599 us for 130,308 rows of 1030 channels, forwards
-// in fp32, where aligned rows of 1024 take 303.
+// Kernels with ODD 0 need D % 4 == 0 and tensors aligned to their vectors; the
+// others take the rest: the part's vector loads and stores need no more than an
+// element's alignment, and a row's last vector may be short.  134 M elements of
+// 1024 / 1030 / 1023 channels take 301 / 456 / 384 us forwards and 564 / 663 /
+// 628 backwards in fp32, 180 / 290 / 226 and 265 / 453 / 345 in bf16; such rows
+// share cache lines, so their loads stay in the caches' usual replacement.
 #pragma once
 
 #include <type_traits>
@@ -31,13 +32,15 @@ typedef uint32_t u2 __attribute__((ext_vector_type(2)));
 typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
 typedef uint32_t u2u __attribute__((ext_vector_type(2), aligned(2)));
 
-enum Kind { F32 = 0, BF16 = 1, ANY = 2 };  // ANY: `bf` says
+enum Kind { F32 = 0, BF16 = 1 };
 
 constexpr int V = 4;
 
-// V elements as they come from memory (ANY: bf16 in the first two words).
+// V elements as they come from memory.
 template <int K>
 using Raw = std::conditional_t<K == BF16, u2, f4>;
+template <int K>
+using Element = std::conditional_t<K == BF16, uint16_t, float>;
 
 __device__ __forceinline__ void widen(u2 w, float* out) {
   out[0] = mxm_u2f(w[0] << 16);
@@ -47,89 +50,75 @@ __device__ __forceinline__ void widen(u2 w, float* out) {
 }
 
 // Elements [at, at + V) of a row of D that starts at p[row].  Of a row's short last
-// vector (ANY) these are the row's last V, which unpack moves down; a row
-// shorter than that is read by elements.
-template <int K>
-__device__ __forceinline__ Raw<K> load(const void* p, bool bf, size_t row, int at, int D) {
-  if constexpr (K == BF16) {
-    return __builtin_nontemporal_load(
-        reinterpret_cast<const u2*>(static_cast<const uint16_t*>(p) + row + at));
-  } else if constexpr (K == F32) {
-    return __builtin_nontemporal_load(
-        reinterpret_cast<const f4*>(static_cast<const float*>(p) + row + at));
+// vector (ODD) these are the row's last V, which unpack moves down; a row
+// shorter than that (ODD 2: possible) is read by elements.
+template <int K, int ODD>
+__device__ __forceinline__ Raw<K> load(const void* p, size_t row, int at, int D) {
+  const Element<K>* q = static_cast<const Element<K>*>(p) + row;
+  if constexpr (!ODD) {
+    return __builtin_nontemporal_load(reinterpret_cast<const Raw<K>*>(q + at));
   } else {
-    f4 r = {};
-    if (D < V) {  // (at is 0)
-      if (bf) {
-        u2 w = {};
-        for (int j = 0; j < D; ++j)
-          w[j >> 1] |= (uint32_t) static_cast<const uint16_t*>(p)[row + j] << (16 * (j & 1));
-        return f4{mxm_u2f(w[0]), mxm_u2f(w[1]), 0.0f, 0.0f};
+    if (ODD == 2 && D < V) {  // (at is 0)
+      Raw<K> r = {};
+      if constexpr (K == BF16) {
+        r[0] = q[0] | (D > 1 ? (uint32_t)q[1] << 16 : 0u);
+        if (D > 2) r[1] = q[2];
+      } else {
+        r[0] = q[0];
+        if (D > 1) r[1] = q[1];
+        if (D > 2) r[2] = q[2];
       }
-      r[0] = static_cast<const float*>(p)[row];
-      if (D > 1) r[1] = static_cast<const float*>(p)[row + 1];
-      if (D > 2) r[2] = static_cast<const float*>(p)[row + 2];
       return r;
     }
-    const size_t i = row + min(at, D - V);
-    if (bf) {
-      const u2 w = *reinterpret_cast<const u2u*>(static_cast<const uint16_t*>(p) + i);
-      return f4{mxm_u2f(w[0]), mxm_u2f(w[1]), 0.0f, 0.0f};
-    }
-    return *reinterpret_cast<const f4u*>(static_cast<const float*>(p) + i);
+    using Any = std::conditional_t<K == BF16, u2u, f4u>;
+    return *reinterpret_cast<const Any*>(q + min(at, D - V));
   }
 }
 // Their values, zeros behind the row.
-template <int K>
-__device__ __forceinline__ void unpack(const Raw<K>& raw, bool bf, int at, int D, float* out) {
+template <int K, int ODD>
+__device__ __forceinline__ void unpack(Raw<K> w, int at, int D, float* out) {
+  const int over = !ODD || (ODD == 2 && D < V) ? 0 : max(at + V - D, 0) & 3;  // (past the row all is 0)
   if constexpr (K == BF16) {
-    widen(raw, out);
-  } else if constexpr (K == F32) {
-#pragma unroll
-    for (int j = 0; j < V; ++j) out[j] = raw[j];
+    if (ODD) {
+      const uint64_t u = ((uint64_t)w[1] << 32 | w[0]) >> (16 * over);
+      w = u2{(uint32_t)u, (uint32_t)(u >> 32)};
+    }
+    widen(w, out);
   } else {
-    const int over = D < V ? 0 : max(at + V - D, 0) & 3;  // (past the row all is 0)
-    if (bf) {
-      const uint64_t w = ((uint64_t)mxm_f2u(raw[1]) << 32 | mxm_f2u(raw[0])) >> (16 * over);
-      widen(u2{(uint32_t)w, (uint32_t)(w >> 32)}, out);
-    } else {
-      f4 w = raw;
+    if (ODD) {
       if (over & 1) w = f4{w[1], w[2], w[3], 0.0f};
       if (over & 2) w = f4{w[2], w[3], 0.0f, 0.0f};
-#pragma unroll
-      for (int j = 0; j < V; ++j) out[j] = w[j];
     }
+#pragma unroll
+    for (int j = 0; j < V; ++j) out[j] = w[j];
   }
 }
 
-// Rounds v to the type it is kept in; v holds the kept values afterwards.
-template <int K>
-__device__ __forceinline__ void store(void* p, bool bf, size_t i, int n, float* v) {
-  const u2 w = {mxm_pack_bf2_fast(v[0], v[1]), mxm_pack_bf2_fast(v[2], v[3])};
+// Rounds v to the type it is kept in and stores what of it lies in the row; v holds
+// the kept values afterwards.
+template <int K, int ODD>
+__device__ __forceinline__ void store(void* p, size_t row, int at, int D, float* v) {
+  Element<K>* q = static_cast<Element<K>*>(p) + row + at;
+  Raw<K> w;
   if constexpr (K == BF16) {
-    __builtin_nontemporal_store(w, reinterpret_cast<u2*>(static_cast<uint16_t*>(p) + i));
-    widen(w, v);
-  } else if constexpr (K == F32) {
-    __builtin_nontemporal_store(f4{v[0], v[1], v[2], v[3]},
-                                reinterpret_cast<f4*>(static_cast<float*>(p) + i));
-  } else if (bf) {
-    uint16_t* q = static_cast<uint16_t*>(p) + i;
-    if (n >= V) {
-      *reinterpret_cast<u2u*>(q) = w;
-    } else {
-      q[0] = (uint16_t)w[0];
-      if (n > 1) q[1] = (uint16_t)(w[0] >> 16);
-      if (n > 2) q[2] = (uint16_t)w[1];
-    }
+    w = u2{mxm_pack_bf2_fast(v[0], v[1]), mxm_pack_bf2_fast(v[2], v[3])};
     widen(w, v);
   } else {
-    float* q = static_cast<float*>(p) + i;
-    if (n >= V) {
-      *reinterpret_cast<f4u*>(q) = f4u{v[0], v[1], v[2], v[3]};
-    } else {
-      q[0] = v[0];
-      if (n > 1) q[1] = v[1];
-      if (n > 2) q[2] = v[2];
+    w = f4{v[0], v[1], v[2], v[3]};
+  }
+  if constexpr (!ODD) {
+    __builtin_nontemporal_store(w, reinterpret_cast<Raw<K>*>(q));
+  } else if (at + V <= D) {
+    using Any = std::conditional_t<K == BF16, u2u, f4u>;
+    *reinterpret_cast<Any*>(q) = w;
+  } else {
+#pragma unroll
+    for (int j = 0; j < V - 1; ++j) {
+      if (at + j >= D) continue;
+      if constexpr (K == BF16)
+        q[j] = (uint16_t)(mxm_f2u(v[j]) >> 16);
+      else
+        q[j] = v[j];
     }
   }
 }
@@ -138,15 +127,18 @@ __device__ __forceinline__ float load_one(const void* p, bool bf, size_t i) {
   return bf ? mxm_bf2f(static_cast<const uint16_t*>(p)[i]) : static_cast<const float*>(p)[i];
 }
 // Values [at, at + V) of a scale, or of a gate's row, of D channels, which many rows
-// read; zeros behind them; null: ones.  K as the kernel's: unless ANY, D % V == 0.
-template <int K>
+// read; zeros behind them; null: ones.
+template <int ODD>
 __device__ __forceinline__ void load_scale(const void* p, bool bf, size_t row, int at, int D,
                                            float* out) {
   if (!p) {
 #pragma unroll
-    for (int j = 0; j < V; ++j) out[j] = K != ANY || at + j < D ? 1.0f : 0.0f;
-  } else if constexpr (K == ANY) {
-    unpack<ANY>(load<ANY>(p, bf, row, at, D), bf, at, D, out);
+    for (int j = 0; j < V; ++j) out[j] = !ODD || at + j < D ? 1.0f : 0.0f;
+  } else if constexpr (ODD) {
+    if (bf)
+      unpack<BF16, ODD>(load<BF16, ODD>(p, row, at, D), at, D, out);
+    else
+      unpack<F32, ODD>(load<F32, ODD>(p, row, at, D), at, D, out);
   } else if (bf) {
     widen(*reinterpret_cast<const u2u*>(static_cast<const uint16_t*>(p) + row + at), out);
   } else {
@@ -233,18 +225,16 @@ void with_shape(const Shape& sh, F f) {
   MXM_CASE(4, -1);
 #undef MXM_CASE
 }
-// f(K0, K1, K2) of three types, or of ANY.
+// f(K0, K1, K2, ODD) of three types.
 template <class F>
-void with_types(bool known, bool bf0, bool bf1, bool bf2, F f) {
-  using std::integral_constant;
-  if (!known) {
-    constexpr integral_constant<int, ANY> any;
-    return f(any, any, any);
-  }
-  auto k = [](auto bf) { return integral_constant<int, decltype(bf)::value ? BF16 : F32>(); };
-  auto third = [&](auto a, auto b) { bf2 ? f(a, b, k(std::true_type())) : f(a, b, k(std::false_type())); };
-  auto second = [&](auto a) { bf1 ? third(a, k(std::true_type())) : third(a, k(std::false_type())); };
-  bf0 ? second(k(std::true_type())) : second(k(std::false_type()));
+void with_types(bool bf0, bool bf1, bool bf2, bool odd, F f) {
+  auto as = [](bool on, auto g) { on ? g(std::true_type()) : g(std::false_type()); };
+  auto k = [](auto bf) { return std::integral_constant<int, decltype(bf)::value ? BF16 : F32>(); };
+  as(bf0, [&](auto a) {
+    as(bf1, [&](auto b) {
+      as(bf2, [&](auto c) { as(odd, [&](auto o) { f(k(a), k(b), k(c), o); }); });
+    });
+  });
 }
 
 }  // namespace resnorm

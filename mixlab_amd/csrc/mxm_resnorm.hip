@@ -9,7 +9,7 @@ namespace {
 
 using namespace resnorm;
 
-template <int NV, int LPR, int XT, int DT, int YT>
+template <int NV, int LPR, int XT, int DT, int YT, int ODD>
 __global__ __launch_bounds__(most_threads(LPR)) void resnorm_kernel(ResNormArgs a) {
   constexpr int E = V * NV;
   __shared__ float red[2][2][LPR > 0 ? 1 : 16];
@@ -27,12 +27,12 @@ __global__ __launch_bounds__(most_threads(LPR)) void resnorm_kernel(ResNormArgs 
     if (at[i] < D) {
       if (a.branch) {
         float p[V];
-        load_scale<XT>(a.scale, a.p_bf16, 0, at[i], D, f + i * V);
-        load_scale<XT>(a.post, a.p_bf16, 0, at[i], D, p);
+        load_scale<ODD>(a.scale, a.p_bf16, 0, at[i], D, f + i * V);
+        load_scale<ODD>(a.post, a.p_bf16, 0, at[i], D, p);
 #pragma unroll
         for (int j = 0; j < V; ++j) f[i * V + j] *= p[j];
       }
-      if (a.norm) load_scale<XT>(a.w, a.p_bf16, 0, at[i], D, w + i * V);
+      if (a.norm) load_scale<ODD>(a.w, a.p_bf16, 0, at[i], D, w + i * V);
     }
   }
   // (at most 2^30 rows and a workgroup's more)
@@ -49,8 +49,8 @@ __global__ __launch_bounds__(most_threads(LPR)) void resnorm_kernel(ResNormArgs 
       rx[i] = Raw<XT>{};
       rd[i] = Raw<DT>{};
       if (n < a.N && at[i] < D) {
-        rx[i] = load<XT>(a.x, a.x_bf16, row, at[i], D);
-        if (a.branch) rd[i] = load<DT>(a.delta, a.delta_bf16, row, at[i], D);
+        rx[i] = load<XT, ODD>(a.x, row, at[i], D);
+        if (a.branch) rd[i] = load<DT, ODD>(a.delta, row, at[i], D);
       }
     }
   };
@@ -62,8 +62,8 @@ __global__ __launch_bounds__(most_threads(LPR)) void resnorm_kernel(ResNormArgs 
     float h[E], dl[E], ga[E], sum[1];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      unpack<XT>(rx[i], a.x_bf16, at[i], D, h + i * V);
-      unpack<DT>(rd[i], a.delta_bf16, at[i], D, dl + i * V);
+      unpack<XT, ODD>(rx[i], at[i], D, h + i * V);
+      unpack<DT, ODD>(rd[i], at[i], D, dl + i * V);
     }
     float g = a.gate == 1 ? rg : 1.0f;
     if (it + 1 < a.chunk_rows) fetch(n + rows);
@@ -75,7 +75,7 @@ __global__ __launch_bounds__(most_threads(LPR)) void resnorm_kernel(ResNormArgs 
         for (int i = 0; i < NV; ++i) {
 #pragma unroll
           for (int j = 0; j < V; ++j) ga[i * V + j] = 0.0f;
-          if (valid && at[i] < D) load_scale<XT>(a.gatep, a.p_bf16, grow, at[i], D, ga + i * V);
+          if (valid && at[i] < D) load_scale<ODD>(a.gatep, a.p_bf16, grow, at[i], D, ga + i * V);
         }
       }
       float rp = 1.0f;
@@ -93,7 +93,7 @@ __global__ __launch_bounds__(most_threads(LPR)) void resnorm_kernel(ResNormArgs 
       for (int e = 0; e < E; ++e) h[e] = __builtin_fmaf(g * dl[e], ga[e], h[e]);
 #pragma unroll
       for (int i = 0; i < NV; ++i)
-        if (valid && at[i] < D) store<XT>(a.h, a.x_bf16, row + at[i], D - at[i], h + i * V);
+        if (valid && at[i] < D) store<XT, ODD>(a.h, row, at[i], D, h + i * V);
     }
     if (!a.norm) continue;
     sum[0] = 0.0f;
@@ -107,7 +107,7 @@ __global__ __launch_bounds__(most_threads(LPR)) void resnorm_kernel(ResNormArgs 
       float y[V];
 #pragma unroll
       for (int j = 0; j < V; ++j) y[j] = (h[i * V + j] * rn) * w[i * V + j];
-      store<YT>(a.y, a.y_bf16, row + at[i], D - at[i], y);
+      store<YT, ODD>(a.y, row, at[i], D, y);
     }
   }
 }
@@ -124,12 +124,12 @@ int rows_per_thread(const ResNormArgs& a, const Shape& sh) {
   return (int)std::max(std::min<int64_t>(std::max<int64_t>(rounds / (8 * a.n_cu), 1), most), least);
 }
 
-template <int NV, int LPR, int XT, int DT, int YT>
+template <int NV, int LPR, int XT, int DT, int YT, int ODD>
 void launch(const ResNormArgs& args, const Shape& sh, hipStream_t s) {
   ResNormArgs a = args;
   a.chunk_rows = rows_per_thread(a, sh);
   const int64_t per = (int64_t)a.chunk_rows * sh.rows();
-  hipLaunchKernelGGL((resnorm_kernel<NV, LPR, XT, DT, YT>), dim3((unsigned)((a.N + per - 1) / per)),
+  hipLaunchKernelGGL((resnorm_kernel<NV, LPR, XT, DT, YT, ODD>), dim3((unsigned)((a.N + per - 1) / per)),
                      dim3(sh.threads), 0, s, a);
 }
 
@@ -142,8 +142,8 @@ void mxm_launch_resnorm(const ResNormArgs& a, hipStream_t s) {
                        (!a.norm || aligned(a.y, a.y_bf16));
   const Shape sh = shape_of(a.D, false);
   with_shape<false>(sh, [&](auto nv, auto lpr) {
-    with_types(vectors, a.x_bf16, a.delta_bf16, a.y_bf16, [&](auto xt, auto dt, auto yt) {
-      launch<nv(), lpr(), xt(), dt(), yt()>(a, sh, s);
+    with_types(a.x_bf16, a.delta_bf16, a.y_bf16, !vectors, [&](auto xt, auto dt, auto yt, auto odd) {
+      launch<nv(), lpr(), xt(), dt(), yt(), odd() ? lpr() == 16 ? 2 : 1 : 0>(a, sh, s);
     });
   });
 }

@@ -34,10 +34,9 @@ __device__ __forceinline__ Rows rows_of(const ResNormArgs& a, int c) {
 
 // CH: a gate per channel.  A row's threads walk one chunk; the chunks of a
 // workgroup add their column sums in LDS and store one partial.
-template <int NV, int LPR, int XT, int DT, int GT, bool CH>
+template <int NV, int LPR, int XT, int DT, int GT, int ODD, bool CH>
 __global__ __launch_bounds__(most_threads(LPR)) void resnorm_bw_kernel(ResNormArgs a) {
   constexpr int E = V * NV;
-  constexpr bool full = XT != ANY;  // every vector of a row is whole
   // of a row's sums (a workgroup a row), or of the workgroup's column sums at the end
   __shared__ float red[LPR > 0 ? THREADS * E : 2 * 16 * 3 + 2 * 16];
   const int lane = LPR > 0 ? threadIdx.x % (LPR > 0 ? LPR : 1) : threadIdx.x;
@@ -60,12 +59,12 @@ __global__ __launch_bounds__(most_threads(LPR)) void resnorm_bw_kernel(ResNormAr
     if (at[i] < D) {
       if (a.branch) {
         float p[V];
-        load_scale<XT>(a.scale, a.p_bf16, 0, at[i], D, f + i * V);
-        load_scale<XT>(a.post, a.p_bf16, 0, at[i], D, p);
+        load_scale<ODD>(a.scale, a.p_bf16, 0, at[i], D, f + i * V);
+        load_scale<ODD>(a.post, a.p_bf16, 0, at[i], D, p);
 #pragma unroll
         for (int j = 0; j < V; ++j) f[i * V + j] *= p[j];
       }
-      if (a.norm) load_scale<XT>(a.w, a.p_bf16, 0, at[i], D, w + i * V);
+      if (a.norm) load_scale<ODD>(a.w, a.p_bf16, 0, at[i], D, w + i * V);
     }
   }
   if (!CH) {
@@ -95,11 +94,11 @@ __global__ __launch_bounds__(most_threads(LPR)) void resnorm_bw_kernel(ResNormAr
       ry[i] = Raw<GT>{};
       if (it < mine.count && at[i] < D) {
         if (a.norm) {
-          rh[i] = load<XT>(a.h, a.x_bf16, row, at[i], D);
-          ry[i] = load<GT>(a.dy, a.g_bf16, row, at[i], D);
+          rh[i] = load<XT, ODD>(a.h, row, at[i], D);
+          ry[i] = load<GT, ODD>(a.dy, row, at[i], D);
         }
-        if (a.branch) rd[i] = load<DT>(a.delta, a.delta_bf16, row, at[i], D);
-        if (a.dh) rt[i] = load<GT>(a.dh, a.g_bf16, row, at[i], D);
+        if (a.branch) rd[i] = load<DT, ODD>(a.delta, row, at[i], D);
+        if (a.dh) rt[i] = load<GT, ODD>(a.dh, row, at[i], D);
       }
     }
   };
@@ -113,10 +112,10 @@ __global__ __launch_bounds__(most_threads(LPR)) void resnorm_bw_kernel(ResNormAr
     if (LPR < 0) fetch(it);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      unpack<XT>(rh[i], a.x_bf16, at[i], D, h + i * V);
-      unpack<DT>(rd[i], a.delta_bf16, at[i], D, dl + i * V);
-      unpack<GT>(rt[i], a.g_bf16, at[i], D, t + i * V);
-      unpack<GT>(ry[i], a.g_bf16, at[i], D, dy + i * V);
+      unpack<XT, ODD>(rh[i], at[i], D, h + i * V);
+      unpack<DT, ODD>(rd[i], at[i], D, dl + i * V);
+      unpack<GT, ODD>(rt[i], at[i], D, t + i * V);
+      unpack<GT, ODD>(ry[i], at[i], D, dy + i * V);
     }
     // (the gate's values go through the sigmoid after the sums, which hide its load)
     const bool new_gate = a.gate && fresh && valid;
@@ -127,7 +126,7 @@ __global__ __launch_bounds__(most_threads(LPR)) void resnorm_bw_kernel(ResNormAr
 #pragma unroll
         for (int i = 0; i < NV; ++i)
           if (at[i] < D)
-            load_scale<XT>(a.gatep, a.p_bf16, (size_t)group * D, at[i], D, ga + (CH ? i * V : 0));
+            load_scale<ODD>(a.gatep, a.p_bf16, (size_t)group * D, at[i], D, ga + (CH ? i * V : 0));
       } else {
         ga[0] = load_one(a.gatep, a.p_bf16, (size_t)group);
       }
@@ -160,7 +159,7 @@ __global__ __launch_bounds__(most_threads(LPR)) void resnorm_bw_kernel(ResNormAr
       float out[V];
 #pragma unroll
       for (int j = 0; j < V; ++j) out[j] = t[i * V + j];
-      store<GT>(a.dx, a.g_bf16, row + at[i], D - at[i], out);
+      store<GT, ODD>(a.dx, row, at[i], D, out);
     }
     if (new_gate) {
 #pragma unroll
@@ -195,7 +194,7 @@ __global__ __launch_bounds__(most_threads(LPR)) void resnorm_bw_kernel(ResNormAr
           const float gf = CH ? ga[CH ? e : 0] * f[e] : f[e];
           out[j] = __builtin_fmaf(-kp, dl[e], (g * rp) * (gf * t[e]));
         }
-        store<GT>(a.d_delta, a.g_bf16, row + at[i], D - at[i], out);
+        store<GT, ODD>(a.d_delta, row, at[i], D, out);
       }
     }
     // the group's last row here
@@ -213,7 +212,7 @@ __global__ __launch_bounds__(most_threads(LPR)) void resnorm_bw_kernel(ResNormAr
               if (at[i] < D)
 #pragma unroll
                 for (int j = 0; j < V; ++j)
-                  if (full || at[i] + j < D) out[at[i] + j] = ag[CH ? i * V + j : 0];
+                  if (!ODD || at[i] + j < D) out[at[i] + j] = ag[CH ? i * V + j : 0];
           } else if (lane == 0) {
             out[0] = ag[0];
           }
@@ -248,7 +247,7 @@ __global__ __launch_bounds__(most_threads(LPR)) void resnorm_bw_kernel(ResNormAr
         if (at[i] < D)
 #pragma unroll
           for (int j = 0; j < V; ++j)
-            if (full || at[i] + j < D) part[at[i] + j] = acc[i * V + j];
+            if (!ODD || at[i] + j < D) part[at[i] + j] = acc[i * V + j];
     }
   };
   if (a.norm && a.d_w) join(aw, a.part + (size_t)blockIdx.x * D);
@@ -306,17 +305,20 @@ __global__ __launch_bounds__(JOIN_COLS* JOIN_SLICES) void resnorm_join_kernel(Re
 // 659 / 645 and 564 / 628 / 664 us (5.7 TB/s with 2): each has its next row's loads
 // on their way, and fewer streams at once suit the memory better.  Rows of one
 // vector a thread need 4 for as many bytes on their way (64 and 256 channels 655
-// / 629 and 637 / 629).
-int wgs_per_cu(const Shape& sh) { return sh.NV == 1 ? 4 : 2; }
+// / 629 and 637 / 629), and three waves a row in bf16 3 (1032 and 1536 channels
+// 537 / 421 and 377 / 311).
+int wgs_per_cu(const Shape& sh, bool bf16) {
+  return sh.NV == 1 ? 4 : bf16 && sh.lpr == 0 && sh.threads < 256 ? 3 : 2;
+}
 int fewest_rows(const Shape& sh) { return sh.lpr > 0 && sh.lpr < 64 ? 1 : 2; }
-int rows_per_chunk(const Shape& sh, int64_t N, int n_cu) {
-  const int64_t target = (int64_t)wgs_per_cu(sh) * n_cu * sh.rows();
+int rows_per_chunk(const Shape& sh, bool bf16, int64_t N, int n_cu) {
+  const int64_t target = (int64_t)wgs_per_cu(sh, bf16) * n_cu * sh.rows();
   return (int)std::max<int64_t>((N + target - 1) / target, fewest_rows(sh));
 }
 
 // Splits a.N rows into chunks.
 void plan(ResNormArgs& a, const Shape& sh) {
-  const int rows = rows_per_chunk(sh, a.N, a.n_cu);
+  const int rows = rows_per_chunk(sh, a.x_bf16 && a.g_bf16, a.N, a.n_cu);
   const int T = std::min(a.gate_rows, a.N);  // rows of the longest group
   a.group_chunks = a.group_parts = 0;
   a.chunk_rows = rows;
@@ -339,19 +341,19 @@ void plan(ResNormArgs& a, const Shape& sh) {
   a.parts = (a.chunks + sh.rows() - 1) / sh.rows();
 }
 
-template <int NV, int LPR, int XT, int DT, int GT>
+template <int NV, int LPR, int XT, int DT, int GT, int ODD>
 void launch(const ResNormArgs& a, const Shape& sh, hipStream_t s) {
   if (a.gate == 2)
-    hipLaunchKernelGGL((resnorm_bw_kernel<NV, LPR, XT, DT, GT, true>), dim3(a.parts),
+    hipLaunchKernelGGL((resnorm_bw_kernel<NV, LPR, XT, DT, GT, ODD, true>), dim3(a.parts),
                        dim3(sh.threads), 0, s, a);
   else
-    hipLaunchKernelGGL((resnorm_bw_kernel<NV, LPR, XT, DT, GT, false>), dim3(a.parts),
+    hipLaunchKernelGGL((resnorm_bw_kernel<NV, LPR, XT, DT, GT, ODD, false>), dim3(a.parts),
                        dim3(sh.threads), 0, s, a);
 }
 
 }  // namespace
 
-int64_t mxm_resnorm_max_parts(int64_t max_rows, int D, bool groups, int n_cu) {
+int64_t mxm_resnorm_max_parts(int64_t max_rows, int D, bool bf16, bool groups, int n_cu) {
   // A workgroup's R = rows() * rows_per_chunk rows.  Without groups ceil(N / R)
   // parts, at most the target and at most ceil(N / (rows() * fewest)); chunks of
   // whole groups hold more than half of the rows aimed at; groups that fill
@@ -359,7 +361,7 @@ int64_t mxm_resnorm_max_parts(int64_t max_rows, int D, bool groups, int n_cu) {
   // N / T + 1 of them: N / R + T / R + N / T + 1 <= 3 N / R + 1.
   const Shape sh = shape_of(D, true);
   const int64_t R = (int64_t)sh.rows() * fewest_rows(sh);
-  const int64_t most = std::min<int64_t>((int64_t)wgs_per_cu(sh) * n_cu, (max_rows + R - 1) / R);
+  const int64_t most = std::min<int64_t>((int64_t)wgs_per_cu(sh, bf16) * n_cu, (max_rows + R - 1) / R);
   return groups ? 3 * most + 1 : most;
 }
 
@@ -375,8 +377,8 @@ bool mxm_launch_resnorm_bw(const ResNormArgs& args, hipStream_t s) {
     plan(a, sh);
     if (a.parts > a.max_parts) return false;
     with_shape<true>(sh, [&](auto nv, auto lpr) {
-      with_types(vectors, a.x_bf16, a.delta_bf16, a.g_bf16, [&](auto xt, auto dt, auto gt) {
-        launch<nv(), lpr(), xt(), dt(), gt()>(a, sh, s);
+      with_types(a.x_bf16, a.delta_bf16, a.g_bf16, !vectors, [&](auto xt, auto dt, auto gt, auto odd) {
+        launch<nv(), lpr(), xt(), dt(), gt(), odd() ? lpr() == 16 ? 2 : 1 : 0>(a, sh, s);
       });
     });
   }

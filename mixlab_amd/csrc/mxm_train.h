@@ -49,9 +49,9 @@ struct ResNormArgs {
 void mxm_launch_resnorm(const ResNormArgs& a, hipStream_t s);
 // false, and no launch, where max_parts is too few.
 bool mxm_launch_resnorm_bw(const ResNormArgs& a, hipStream_t s);
-// Most parts of any backward of up to max_rows rows; groups: of several rows per
-// row of the gate.
-int64_t mxm_resnorm_max_parts(int64_t max_rows, int D, bool groups, int n_cu);
+// Most parts of any backward of up to max_rows rows; bf16: stream and gradients;
+// groups: of several rows per row of the gate.
+int64_t mxm_resnorm_max_parts(int64_t max_rows, int D, bool bf16, bool groups, int n_cu);
 
 // ---- gradient sets ----
 // A piece of one tensor, with where it is (a launch reads one descriptor and

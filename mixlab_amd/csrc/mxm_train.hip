@@ -207,7 +207,8 @@ int64_t mxm_resnorm_create(const int64_t* params, int n_params, float eps, int64
     a.gate = (int)gate;
     a.gate_rows = gate == MXM_GATE_NONE ? 1 : (int)gate_rows;
     if (r->backward) {
-      a.max_parts = (int)mxm_resnorm_max_parts(rows, a.D, a.gate_rows > 1, a.n_cu);
+      a.max_parts = (int)mxm_resnorm_max_parts(rows, a.D, a.x_bf16 && a.g_bf16, a.gate_rows > 1,
+                                               a.n_cu);
       const size_t parts = (size_t)a.max_parts;
       r->part.alloc(2 * parts * (size_t)D * 4);
       if (a.gate && a.gate_rows > 1)

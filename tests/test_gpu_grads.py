@@ -128,6 +128,32 @@ def test_adamw(gpu_lib, name, dtype, max_norm):
             assert step.get()[0] == t and skipped.get()[0] == 0
 
 
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_tensors_out_of_step(gpu_lib, dtype):
+    """Gradients, outputs and state that start at different places between two
+    vectors' boundaries give what aligned ones give."""
+    from mixlab_amd.train import GradientSet
+
+    sizes = [4099, 20003, 2]
+    rng = np.random.default_rng(8)
+    grads = [as_kept(rng.standard_normal(n, dtype=np.float32), dtype) for n in sizes]
+    ps, ms, vs = ([np.abs(rng.standard_normal(n, dtype=np.float32)) for n in sizes] for _ in range(3))
+    got = []
+    for shifts in ((0, 0, 0, 0, 0, 0), (1, 2, 3, 1, 2, 1), (3, 1, 0, 3, 3, 3)):
+        with GradientSet(sizes, dtype) as s:
+            lists = [[Dev(a, t, shift=k) for a in arrays] for arrays, t, k in zip(
+                (grads, grads, ps, ms, vs, ps), (dtype, dtype, "fp32", "fp32", "fp32", "bf16"), shifts)]
+            step = Dev(np.zeros(1, np.int64), "int64")
+            s.bind(*[[d.ptr for d in one] for one in lists])
+            s.clip(0.25)
+            s.adamw(1e-2, 0.9, 0.99, 1e-8, 0.1, 0.25, step.ptr)
+            s.synchronize()
+            got.append([d.get() for one in lists for d in one])
+    for other in got[1:]:
+        for a, b in zip(other, got[0]):
+            assert np.array_equal(a, b)
+
+
 @pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
 def test_non_finite_gradients(gpu_lib, bad):
     """AdamW leaves everything as it was, clip copies, and the next step runs."""
