@@ -140,7 +140,7 @@ void mxm_launch_resnorm(const ResNormArgs& a, hipStream_t s) {
   const bool vectors = a.D % 4 == 0 && aligned(a.x, a.x_bf16) &&
                        (!a.branch || (aligned(a.delta, a.delta_bf16) && aligned(a.h, a.x_bf16))) &&
                        (!a.norm || aligned(a.y, a.y_bf16));
-  const Shape sh = shape_of(a.D, false);
+  const Shape sh = shape_of(a.D, false, a.N);
   with_shape<false>(sh, [&](auto nv, auto lpr) {
     with_types(a.x_bf16, a.delta_bf16, a.y_bf16, !vectors, [&](auto xt, auto dt, auto yt, auto odd) {
       launch<nv(), lpr(), xt(), dt(), yt(), odd() ? lpr() == 16 ? 2 : 1 : 0>(a, sh, s);

@@ -359,9 +359,12 @@ int64_t mxm_resnorm_max_parts(int64_t max_rows, int D, bool bf16, bool groups, i
   // whole groups hold more than half of the rows aimed at; groups that fill
   // workgroups (T >= R) have at most T / R + 1 parts each, and there are at most
   // N / T + 1 of them: N / R + T / R + N / T + 1 <= 3 N / R + 1.
-  const Shape sh = shape_of(D, true);
-  const int64_t R = (int64_t)sh.rows() * fewest_rows(sh);
-  const int64_t most = std::min<int64_t>((int64_t)wgs_per_cu(sh, bf16) * n_cu, (max_rows + R - 1) / R);
+  int64_t most = 0;
+  for (const int64_t rows : {max_rows, std::min<int64_t>(max_rows, FEW_ROWS)}) {
+    const Shape sh = shape_of(D, true, rows);
+    const int64_t R = (int64_t)sh.rows() * fewest_rows(sh);
+    most = std::max(most, std::min<int64_t>((int64_t)wgs_per_cu(sh, bf16) * n_cu, (rows + R - 1) / R));
+  }
   return groups ? 3 * most + 1 : most;
 }
 
@@ -371,7 +374,7 @@ bool mxm_launch_resnorm_bw(const ResNormArgs& args, hipStream_t s) {
       a.D % 4 == 0 && (!a.norm || (aligned(a.h, a.x_bf16) && aligned(a.dy, a.g_bf16))) &&
       (!a.branch || (aligned(a.delta, a.delta_bf16) && aligned(a.d_delta, a.g_bf16))) &&
       aligned(a.dh, a.g_bf16) && aligned(a.dx, a.g_bf16);
-  const Shape sh = shape_of(a.D, true);
+  const Shape sh = shape_of(a.D, true, a.N);
   a.chunks = a.parts = a.group_chunks = a.group_parts = 0;
   if (a.N > 0) {
     plan(a, sh);
