@@ -15,7 +15,7 @@ import numpy as np
 
 from . import _lib
 from .moe import (DEFAULT_FFN_MULTIPLIER, MOE_EXPERT_MLP, OP_MOE_FEED_FORWARD, OP_RMSNORM, BlockSpec,
-                  Op, Program, effective_moe_load_balance_loss_weight, emit_moe_ir,
+                  Op, Program, WeightMeta, effective_moe_load_balance_loss_weight, emit_moe_ir,
                   moe_weight_shapes)
 
 _DTYPES = {"fp32": _lib.MXM_DTYPE_F32, "float32": _lib.MXM_DTYPE_F32,
@@ -262,11 +262,14 @@ class MoEBlock:
     op 74, aux weight, optional moe_scale, residual add -- run as one fused
     call (mxm_moe_block_forward).  Weights follow the block's metas
     (arch/moe.go:112-150): moe_norm_scale, router_w, per-expert matrices,
-    then moe_scale when block_scales is on."""
+    then moe_scale when block_scales is on.  With post_norm the op's output is
+    normalised before the scale and the residual add (weight
+    moe_post_norm_scale, after the others; no counterpart in the reference):
+    the block then runs as its entry norm, the op and its exit."""
 
     def __init__(self, spec: BlockSpec, B: int, T: int, D: int,
                  mlp_mult: float = DEFAULT_FFN_MULTIPLIER, block_scales: bool = False,
-                 compute_dtype: str = "fp32", flags: int = 0):
+                 compute_dtype: str = "fp32", flags: int = 0, post_norm: bool = False):
         prog = Program()
         emit_moe_ir(prog, spec, "x", 0, D, T, B, 0, mlp_mult, block_scales)
         norm = next(op for op in prog.ops if op.code == OP_RMSNORM)
@@ -281,6 +284,10 @@ class MoEBlock:
         self.op = MoEFeedForward.from_op(ff, compute_dtype=compute_dtype, flags=flags)
         self.norm_scale = None
         self.moe_scale = None
+        self.post_scale = None
+        self.post_norm = post_norm
+        if post_norm:
+            self.metas.append(WeightMeta("moe_post_norm_scale", [D], is_norm_scale=True, init_one=True))
 
     def _conv(self, a):
         from .workloads import bf16_bits
@@ -296,10 +303,11 @@ class MoEBlock:
                 raise ValueError(f"{m.name}: shape {list(np.shape(w))}, want {m.shape}")
         self.norm_scale = self._conv(weights[0])
         self.op.set_input(1, self._conv(weights[1]))
-        n_exp = len(self.metas) - 2 - (1 if self.block_scales else 0)
+        n_exp = sum(m.name.startswith("expert_") for m in self.metas)
         for i in range(n_exp):
             self.op.set_input(2 + i, self._conv(weights[2 + i]))
-        self.moe_scale = self._conv(weights[-1]) if self.block_scales else None
+        self.moe_scale = self._conv(weights[2 + n_exp]) if self.block_scales else None
+        self.post_scale = self._conv(weights[-1]) if self.post_norm else None
 
     def load(self, path: str, first_index: int = 0) -> None:
         """Bind the block's weights from a native checkpoint (tensors
@@ -322,20 +330,50 @@ class MoEBlock:
         dense = [g.dequantize() if isinstance(g, QuantizedWeight) else g for g in got]
         self.norm_scale = self._conv(dense[0])
         self.op.set_input(1, self._conv(dense[1]))
-        n_exp = len(self.metas) - 2 - (1 if self.block_scales else 0)
+        n_exp = sum(m.name.startswith("expert_") for m in self.metas)
         for i in range(n_exp):
             g = got[2 + i]
             q, sc = g.per_channel() if isinstance(g, QuantizedWeight) else quantize_per_channel(g)
             self.op.set_input_q8(2 + i, q, sc)
-        self.moe_scale = self._conv(dense[-1]) if self.block_scales else None
+        self.moe_scale = self._conv(dense[2 + n_exp]) if self.block_scales else None
+        self.post_scale = self._conv(dense[-1]) if self.post_norm else None
 
     def forward_host(self, x: np.ndarray):
         """x [B*T, D] (fp32, or bf16 bits) -> (x + delta [B*T, D] fp32,
         aux = load-balance weight * aux_raw, router entropy)."""
         if self.norm_scale is None:
             raise ValueError("moe block weights are not set")
+        if self.post_norm:
+            return self._forward_post_norm(x)
         return self.op.block_forward_host(x, self.norm_scale, self.moe_scale, self.eps,
                                           self.aux_weight)
+
+    def _forward_post_norm(self, x: np.ndarray):
+        from .train import ResidualNorm
+        from .workloads import from_bits
+        dev, N, D = _lib.DeviceBuffer, self.op.N, self.op.D
+        kept = "bf16" if self.bf16 else "fp32"
+        x = np.ascontiguousarray(x)
+        if x.shape != (N, D):
+            raise ValueError(f"x must be [{N}, {D}]")
+        # (the result is fp32 whatever x is, as the fused block's)
+        bx = dev.from_array(from_bits(x) if x.dtype == np.uint16 else x.astype(np.float32, copy=False))
+        xn, delta, out = dev(N * D * (2 if self.bf16 else 4)), dev(N * D * 4), dev(N * D * 4)
+        aux, ent = dev(4), dev(4)
+        ns, ps = dev.from_array(self.norm_scale), dev.from_array(self.post_scale)
+        ms = dev.from_array(self.moe_scale) if self.block_scales else None
+        with ResidualNorm(D, N, out_dtype=kept, scale_dtype=kept, eps=self.eps, branch=False,
+                          backward=False, share=self.op) as entry, \
+                ResidualNorm(D, N, scale_dtype=kept, eps=self.eps, post_norm=True, norm=False,
+                             backward=False, share=self.op) as leave:
+            entry.forward(N, bx.value, y=xn.value, norm_scale=ns.value)
+            self.op.forward(xn.value, _lib.MXM_DTYPE_BF16 if self.bf16 else _lib.MXM_DTYPE_F32, N,
+                            delta.value, aux.value, ent.value)
+            leave.forward(N, bx.value, delta.value, out.value, post_scale=ps.value,
+                          branch_scale=ms.value if ms else 0)
+            self.op.synchronize()
+        one = lambda b: float(b.download(np.float32, (1,))[0])  # noqa: E731
+        return out.download(np.float32, (N, D)), self.aux_weight * one(aux), one(ent)
 
     def close(self) -> None:
         self.op.close()

@@ -249,6 +249,29 @@ def test_zero_and_non_finite_rows(gpu_lib, D):
     assert np.isnan(got["d_scale"]).any()
 
 
+@pytest.mark.parametrize("N,D", [(1025, 520), (1300, 767), (1100, 1000), (1030, 1021), (3, 5000),
+                                 (2, 9001)])
+@pytest.mark.parametrize("types", ["fp32", "bf16"])
+def test_more_rows_and_wide_rows(gpu_lib, N, D, types):
+    """Rows in a wave past the few, and rows over 512 threads."""
+    c = dict(gate="channel", gate_rows=7, sigmoid=True)
+    if types == "bf16":
+        c.update(stream="bf16", delta="bf16", out="bf16", grad="bf16")
+    v = _case(N + D, N, D, **c)
+    h, y = run_forward(v, N, D, **c)
+    check_forward(v, h.get(), y.get(), N, D, c)
+    check_backward(v, run_backward(v, N, D, **c), N, D, c)
+
+
+@pytest.mark.parametrize("rows", [1, 700, 1024, 1025, 3000])
+def test_one_handle_for_many_sizes(gpu_lib, rows):
+    """The workspace made for the most rows holds any fewer, whatever shape they take."""
+    c = dict(gate="channel", gate_rows=100)
+    v = _case(rows, rows, 600, **c)
+    with _handle(3000, 600, **c) as r:
+        check_backward(v, run_backward(v, rows, 600, handle=r, **c), rows, 600, c)
+
+
 @pytest.mark.parametrize("N,D", [(5000, 64), (3000, 1030), (2100, 2048)])
 def test_many_rows_and_equal_bits(gpu_lib, N, D):
     """More chunks than workgroups fit at once; two runs agree bit for bit."""

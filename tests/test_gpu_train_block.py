@@ -149,6 +149,32 @@ def test_entry_and_op_match_the_fused_block(gpu_lib):
     assert abs(got["aux"] - aux) <= 1e-5 * abs(aux)
 
 
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("N,D,scales", [(1, 96, True), (8, 256, False), (70, 160, True)])
+def test_post_norm_block_serves_what_it_trained(gpu_lib, dtype, N, D, scales):
+    """The inference block with a post norm, from one token on, gives the training
+    forward's output on the trained weights."""
+    from mixlab_amd.op import MoEBlock
+    from mixlab_amd.train import MoEBlockTrainer
+
+    spec = moe.BlockSpec.from_dict({"type": "moe", "num_experts": 4, "top_k": 2})
+    rng = np.random.default_rng(N)
+    x, d_out = (rng.standard_normal((N, D), dtype=np.float32) for _ in range(2))
+    with MoEBlockTrainer(spec, 1, N, D, 1.0, scales, post_norm=True, compute_dtype=dtype) as tr, \
+            MoEBlock(spec, 1, N, D, 1.0, scales, compute_dtype=dtype, post_norm=True) as blk:
+        tr.set_weights(_weights(rng, tr.metas))
+        tr.step_host(x, d_out, 1e-2)
+        assert [m.name for m in blk.metas] == [m.name for m in tr.metas]
+        blk.set_weights(tr.weights())
+        out, aux, ent = blk.forward_host(x)
+        want = tr.step_host(x, d_out, 0.0)
+        # (a bf16 op of few rows streams its weights: other sums of the same products)
+        tol = 1e-5 if dtype == "fp32" else TOL[dtype]
+        assert rel_l2(out - x, want["out"] - x) <= tol
+        assert abs(aux - want["aux"]) <= tol * abs(want["aux"])
+        assert abs(ent - want["entropy"]) <= tol * abs(want["entropy"])
+
+
 def test_refusals(gpu_lib):
     from mixlab_amd.train import MoEBlockTrainer
 
