@@ -1,6 +1,9 @@
 // The residual norm forwards (formulas in mxm_train.h): the branch's output
 // normalised, scaled and gated, added to the stream, and the next sublayer's
-// norm of the sum, in one pass over the rows.
+// norm of the sum, in one pass over the rows.  Bound by memory: 65,536 rows of
+// 2048 channels, fp32 with a bf16 y and a gate per token, 306 us (1.88 GB at 6.1
+// TB/s; 383 us at a large copy's rate), few rows by one row's chain of load, sum,
+// root, sum, root, store (3.9 us for 8 rows of 1024).
 #include <algorithm>
 
 #include "mxm_resnorm.h"
