@@ -384,7 +384,7 @@ int mxm_grads_norm(int64_t h, float* norm);
 int mxm_grads_clip(int64_t h, double max_norm, float* norm);
 
 /* One AdamW step on the clipped gradients (max_norm 0: not clipped), which are
- * not written back: with t = ++*step (device memory)
+ * not written back: with t = ++*step (device memory; below 0 taken as 0)
  *   m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2
  *   p -= lr weight_decay decay[i] p + lr (m / (1 - beta1^t)) / (sqrt(v / (1 - beta2^t)) + eps)
  * A gradient norm that is not finite leaves params, m, v, the bf16 copies and

@@ -122,7 +122,7 @@ __device__ __forceinline__ void finish_norm(const GradArgs& a, double total) {
   if (a.adamw) {
     if (a.skipped) *a.skipped = !finite;
     if (finite) {
-      const int64_t t = *a.step + 1;
+      const int64_t done = *a.step, t = (done > 0 ? done : 0) + 1;
       *a.step = t;
       r.step_size = (float)(a.lr / (1.0 - pow(a.beta1, (double)t)));
       r.root2 = (float)(1.0 / sqrt(1.0 - pow(a.beta2, (double)t)));

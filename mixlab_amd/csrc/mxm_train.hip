@@ -276,7 +276,7 @@ int mxm_resnorm_backward(int64_t h, int64_t rows, const void* h_in, const void* 
     check_pointer(RESNORM, "delta", delta, a.delta_bf16, any && a.branch);
     check_pointer(RESNORM, "dh", dh, a.g_bf16, any && !a.norm);
     check_pointer(RESNORM, "dy", dy, a.g_bf16, any && a.norm);
-    check_pointer(RESNORM, "dx", dx, a.g_bf16, any && !a.branch);
+    check_pointer(RESNORM, "dx", dx, a.g_bf16, any && (a.norm || !a.branch));
     check_pointer(RESNORM, "d_delta", d_delta, a.g_bf16, any && a.branch);
     check_pointer(RESNORM, "gate", gate, a.p_bf16, any && a.gate != 0);
     check_pointer(RESNORM, "post_scale", post_scale, a.p_bf16, false);

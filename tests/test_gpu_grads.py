@@ -184,6 +184,28 @@ def test_non_finite_gradients(gpu_lib, bad):
         assert not np.array_equal(p.get(), np.concatenate(ps))
 
 
+def test_step_count(gpu_lib):
+    """A count past 32 bits, and one below zero, which is taken as zero."""
+    from mixlab_amd.train import GradientSet
+
+    g = _set("small", "fp32")
+    ps, ms, vs = _adam_state("small")
+    with GradientSet(SETS["small"]) as s:
+        for start, t in ((2 ** 40, 2 ** 40 + 1), (-7, 1), (0, 1)):
+            (p, pp), (m, mp), (v, vp) = _flat(ps), _flat(ms), _flat(vs)
+            gd, gp = _flat(g)
+            step = Dev(np.full(1, start, np.int64), "int64")
+            s.bind(gp, params=pp, m=mp, v=vp)
+            s.adamw(1e-2, 0.9, 0.999, 1e-8, 0.0, 0.0, step.ptr)
+            s.synchronize()
+            assert step.get()[0] == t
+            flat = [np.concatenate(a) for a in (ps, ms, vs, g)]
+            want = ot.adamw(*flat, t, 1e-2, 0.9, 0.999, 1e-8, 0.0)
+            size = (0.9 * np.abs(flat[1]) + 0.1 * np.abs(flat[3])) / (1 - 0.9 ** t)
+            update = 1e-2 * size / (np.sqrt(want[2] / (1 - 0.999 ** t)) + 1e-8)
+            close(p.get(), want[0], 16 * U32 * update + 2 * U32 * np.abs(flat[0]), "fp32", "p")
+
+
 def test_mixed_types_and_equal_bits(gpu_lib):
     from mixlab_amd.train import GradientSet
 

@@ -346,6 +346,8 @@ def test_refusals(gpu_lib):
                 r.forward(**a)
         with pytest.raises(_lib.MixMoEError, match="dy must be non-NULL"):
             r.backward(N, x.ptr, d.ptr, x.ptr, 0, h.ptr, y.ptr)
+        with pytest.raises(_lib.MixMoEError, match="dx must be non-NULL"):
+            r.backward(N, x.ptr, d.ptr, x.ptr, x.ptr, 0, y.ptr)
         with pytest.raises(_lib.MixMoEError, match="d_gate given without a gate"):
             r.backward(N, x.ptr, d.ptr, x.ptr, x.ptr, h.ptr, y.ptr, d_gate=h.ptr)
     with _handle(N, D, backward=False, post=False) as r:
