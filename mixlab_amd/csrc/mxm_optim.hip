@@ -196,12 +196,10 @@ __global__ __launch_bounds__(THREADS) void grad_norm_kernel(GradArgs a) {
   }
 }
 
-// Adds the workgroups' sums in their order.
-__global__ __launch_bounds__(THREADS) void grad_norm_finish_kernel(GradArgs a, int blocks) {
-  __shared__ double red[THREADS / 64];
-  double s = 0.0;
-  for (int b = threadIdx.x; b < blocks; b += THREADS) s += a.partial[b];
-  s = block_sum(s, red);
+// Adds the workgroups' sums, one a thread.
+__global__ __launch_bounds__(MOST_BLOCKS) void grad_norm_finish_kernel(GradArgs a, int blocks) {
+  __shared__ double red[MOST_BLOCKS / 64];
+  const double s = block_sum((int)threadIdx.x < blocks ? a.partial[threadIdx.x] : 0.0, red);
   if (threadIdx.x == 0) finish_norm(a, s);
 }
 
@@ -241,6 +239,7 @@ __global__ __launch_bounds__(THREADS) void grad_clip_kernel(GradArgs a) {
   const int b = a.first_slice - (int)blockIdx.x;
   const GradChunk k = a.chunks[b / a.slices];
   const float coef = a.scalars->coef;
+  if (coef == 1.0f && k.clipped == k.g) return;  // (in place, and nothing to clip)
   const bool bf = k.bf16 != 0;
   const int V = bf ? 8 : 4, size = bf ? 2 : 4;
   // (tensors out of step with each other: vectors at any address, from the start on)
@@ -358,7 +357,7 @@ void mxm_launch_grad_norm(const GradArgs& a, hipStream_t s) {
   const int blocks = mxm_grad_norm_blocks(a.n_chunks);
   hipLaunchKernelGGL(grad_norm_kernel, dim3(blocks), dim3(THREADS), 0, s, a);
   if (blocks > TICKET_BLOCKS)
-    hipLaunchKernelGGL(grad_norm_finish_kernel, dim3(1), dim3(THREADS), 0, s, a, blocks);
+    hipLaunchKernelGGL(grad_norm_finish_kernel, dim3(1), dim3((blocks + 63) / 64 * 64), 0, s, a, blocks);
 }
 // f(a, workgroups) for all of a's slices, the last first, in launches whose threads
 // are counted in 32 bits.

@@ -62,6 +62,9 @@ def test_norm_and_clip(gpu_lib, name, dtype, shift):
             close(out.get(), want, 3 * U32 * np.abs(want), dtype, "clipped")
             assert np.array_equal(g.get(), np.concatenate(grads))
         s.bind(gp)  # in place
+        s.clip(norm * 3)
+        s.synchronize()
+        assert np.array_equal(g.get(), np.concatenate(grads))
         s.clip(norm / 3)
         s.synchronize()
         want = ot.clip_coef(norm, norm / 3) * np.concatenate(grads).astype(np.float64)
