@@ -9,7 +9,7 @@
 // A norm that is not finite leaves p, m, v and the step count as they were.
 // Bound by memory: the norm of 201 M fp32 gradients 120 us (6.7 TB/s; 115 at the
 // rate of a plain read stream), AdamW over 403 M parameters with bf16 copies 2.09
-// ms of 12.1 GB (5.8 TB/s) after the norm's 0.24.
+// ms of 12.1 GB (5.8 TB/s) after the norm's 0.15-0.24.
 #include <algorithm>
 
 #include "mxm_kernels.h"
@@ -131,6 +131,44 @@ __device__ __forceinline__ void finish_norm(const GradArgs& a, double total) {
   *a.scalars = r;
 }
 
+// s and the squares of a chunk; ONCE: it is not read again soon.
+template <bool ONCE>
+__device__ __forceinline__ double add_squares(const GradChunk& k, double s) {
+  auto add = [&](float v) { s = __builtin_fma((double)v, (double)v, s); };
+  auto read = [](const auto* p) {
+    if constexpr (ONCE)
+      return __builtin_nontemporal_load(p);
+    else
+      return *p;
+  };
+  const bool bf = k.bf16 != 0;
+  const int V = bf ? 8 : 4;  // elements of 16 bytes
+  const int head = min(head_of(k.g, bf ? 2 : 4, V), k.count);
+  const int n = (k.count - head) / V;
+  if (bf) {
+    const u4* g = reinterpret_cast<const u4*>(static_cast<const uint16_t*>(k.g) + head);
+    u4 w[UNROLL];
+    each_vector(n, [&](int i, int j) { w[j] = read(g + i); },
+                [&](int, int j) {
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) {
+                    add(lo16(w[j][e]));
+                    add(hi16(w[j][e]));
+                  }
+                });
+  } else {
+    const f4* g = reinterpret_cast<const f4*>(static_cast<const float*>(k.g) + head);
+    f4 w[UNROLL];
+    each_vector(n, [&](int i, int j) { w[j] = read(g + i); },
+                [&](int, int j) {
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) add(w[j][e]);
+                });
+  }
+  each_rest(head, head + n * V, k.count, [&](int i) { add(grad_at(k.g, bf, i)); });
+  return s;
+}
+
 // The squares of whole chunks per workgroup, one sum each.  Up to TICKET_BLOCKS
 // workgroups the last one to finish adds them; past that a second launch does:
 // every ticket costs about 45 ns (its release writes an L2 back), one after the
@@ -143,34 +181,12 @@ __global__ __launch_bounds__(THREADS) void grad_norm_kernel(GradArgs a) {
   __shared__ double red[THREADS / 64];
   __shared__ int s_last;
   double s = 0.0;
-  auto add = [&](float v) { s = __builtin_fma((double)v, (double)v, s); };
   for (int c = blockIdx.x; c < a.n_chunks; c += gridDim.x) {
     const GradChunk k = a.chunks[c];
-    const bool bf = k.bf16 != 0;
-    const int V = bf ? 8 : 4;  // elements of 16 bytes
-    const int head = min(head_of(k.g, bf ? 2 : 4, V), k.count);
-    const int n = (k.count - head) / V;
-    if (bf) {
-      const u4* g = reinterpret_cast<const u4*>(static_cast<const uint16_t*>(k.g) + head);
-      u4 w[UNROLL];
-      each_vector(n, [&](int i, int j) { w[j] = __builtin_nontemporal_load(g + i); },
-                  [&](int, int j) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                      add(lo16(w[j][e]));
-                      add(hi16(w[j][e]));
-                    }
-                  });
-    } else {
-      const f4* g = reinterpret_cast<const f4*>(static_cast<const float*>(k.g) + head);
-      f4 w[UNROLL];
-      each_vector(n, [&](int i, int j) { w[j] = __builtin_nontemporal_load(g + i); },
-                  [&](int, int j) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) add(w[j][e]);
-                  });
-    }
-    each_rest(head, head + n * V, k.count, [&](int i) { add(grad_at(k.g, bf, i)); });
+    if (c < a.keep_from)
+      s = add_squares<true>(k, s);
+    else
+      s = add_squares<false>(k, s);
   }
   s = block_sum(s, red);
   if (gridDim.x > TICKET_BLOCKS) {
@@ -351,9 +367,21 @@ int mxm_grad_chunk_elems(int64_t total, int n_cu) {
   return (int)per;
 }
 
+// Of gradients that clip or AdamW reads next, the norm leaves about what the
+// last-level cache holds there, the rest it reads past it.  None / 64 / 128 / 192 /
+// 256 MB / all kept: clipping 134 M bf16 130.6 / 130.4 / 128.8 / 126.9 / 125.9 /
+// 125.2 us, AdamW over 16.8 M 95.7 / 88.1 / 88.0 / 88.0 / 88.0 / 88.1, over 403 M
+// 2298 / 2287 / 2280 / 2266 / 2244 / 2272; a norm alone 119.4 with none kept, 133
+// with all.
+constexpr int64_t KEPT_BYTES = 256ll << 20;
+
 int mxm_grad_norm_blocks(int n_chunks) { return std::max(1, std::min(n_chunks, MOST_BLOCKS)); }
 
-void mxm_launch_grad_norm(const GradArgs& a, hipStream_t s) {
+void mxm_launch_grad_norm(const GradArgs& args, bool again, hipStream_t s) {
+  GradArgs a = args;
+  a.keep_from = again ? (int)std::max<int64_t>(
+                            a.n_chunks - KEPT_BYTES / ((int64_t)a.chunk_elems * (a.all_bf16 ? 2 : 4)), 0)
+                      : a.n_chunks;
   const int blocks = mxm_grad_norm_blocks(a.n_chunks);
   hipLaunchKernelGGL(grad_norm_kernel, dim3(blocks), dim3(THREADS), 0, s, a);
   if (blocks > TICKET_BLOCKS)

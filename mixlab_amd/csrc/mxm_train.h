@@ -77,6 +77,7 @@ struct GradArgs {
   int n_chunks;
   int chunk_elems;       // elements of a chunk (a tensor's last one may be shorter)
   bool all_bf16;         // every tensor's gradients are bf16
+  int keep_from;         // (set by the norm's launcher) chunks from here on stay in the caches
   int slices;            // workgroups per chunk, and the one that a launch's first
   int first_slice;       // workgroup takes (set by the launchers of clip and AdamW)
   double* partial;       // [n_chunks or fewer]
@@ -94,6 +95,7 @@ struct GradArgs {
 };
 int mxm_grad_chunk_elems(int64_t total, int n_cu);
 int mxm_grad_norm_blocks(int n_chunks);
-void mxm_launch_grad_norm(const GradArgs& a, hipStream_t s);
+// again: a launch that reads the gradients again follows.
+void mxm_launch_grad_norm(const GradArgs& a, bool again, hipStream_t s);
 void mxm_launch_grad_clip(const GradArgs& a, hipStream_t s);
 void mxm_launch_grad_adamw(const GradArgs& a, hipStream_t s);

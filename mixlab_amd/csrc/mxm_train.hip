@@ -450,7 +450,7 @@ int mxm_grads_norm(int64_t h, float* norm) {
     const DeviceGuard guard(g->stream_ref->device);
     GradArgs a = g->base;
     a.norm = norm;
-    mxm_launch_grad_norm(a, g->stream());
+    mxm_launch_grad_norm(a, false, g->stream());
     HIPCK(hipGetLastError());
     return MXM_OK;
   });
@@ -467,7 +467,7 @@ int mxm_grads_clip(int64_t h, double max_norm, float* norm) {
     GradArgs a = g->base;
     a.norm = norm;
     a.max_norm = max_norm;
-    mxm_launch_grad_norm(a, g->stream());
+    mxm_launch_grad_norm(a, true, g->stream());
     HIPCK(hipGetLastError());
     mxm_launch_grad_clip(a, g->stream());
     HIPCK(hipGetLastError());
@@ -505,7 +505,7 @@ int mxm_grads_adamw(int64_t h, double lr, double beta1, double beta2, double eps
     a.beta2 = beta2;
     a.eps = eps;
     a.weight_decay = weight_decay;
-    mxm_launch_grad_norm(a, g->stream());
+    mxm_launch_grad_norm(a, true, g->stream());
     HIPCK(hipGetLastError());
     mxm_launch_grad_adamw(a, g->stream());
     HIPCK(hipGetLastError());
