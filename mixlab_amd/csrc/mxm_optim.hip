@@ -8,8 +8,8 @@
 //   p = p - lr decay p - lr (m / (1 - beta1^t)) / (sqrt(v / (1 - beta2^t)) + eps)
 // A norm that is not finite leaves p, m, v and the step count as they were.
 // Bound by memory: the norm of 201 M fp32 gradients 120 us (6.7 TB/s; 115 at the
-// rate of a plain read stream), AdamW over 403 M parameters with bf16 copies 2.09
-// ms of 12.1 GB (5.8 TB/s) after the norm's 0.15-0.24.
+// rate of a plain read stream), AdamW over 403 M parameters with bf16 copies 2.00
+// ms of 12.1 GB (6.0 TB/s) after the norm's 0.23.
 #include <algorithm>
 
 #include "mxm_kernels.h"
@@ -367,12 +367,14 @@ int mxm_grad_chunk_elems(int64_t total, int n_cu) {
   return (int)per;
 }
 
-// Of gradients that clip or AdamW reads next, the norm leaves about what the
-// last-level cache holds there, the rest it reads past it.  None / 64 / 128 / 192 /
-// 256 MB / all kept: clipping 134 M bf16 130.6 / 130.4 / 128.8 / 126.9 / 125.9 /
+// Of gradients that clip or AdamW reads next, the norm reads the last ones, about
+// as much as the last-level cache holds, with plain loads and the rest with
+// nontemporal ones.  None / 64 / 128 / 192 / 256 MB / all with plain loads (one
+// sweep; runs of the last case differ by up to 1.7 %, so 192 MB to all are not told
+// apart there): clipping 134 M bf16 130.6 / 130.4 / 128.8 / 126.9 / 125.9 /
 // 125.2 us, AdamW over 16.8 M 95.7 / 88.1 / 88.0 / 88.0 / 88.0 / 88.1, over 403 M
-// 2298 / 2287 / 2280 / 2266 / 2244 / 2272; a norm alone 119.4 with none kept, 133
-// with all.
+// 2298 / 2287 / 2280 / 2266 / 2244 / 2272; a norm alone, of 201 M fp32,
+// 119.6 with none, 133 with all.
 constexpr int64_t KEPT_BYTES = 256ll << 20;
 
 int mxm_grad_norm_blocks(int n_chunks) { return std::max(1, std::min(n_chunks, MOST_BLOCKS)); }
