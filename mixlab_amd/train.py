@@ -184,7 +184,7 @@ class MoEBlockTrainer:
             self.metas.append(WeightMeta("moe_post_norm_scale", [D], is_norm_scale=True, init_one=True))
         self.hyper = dict(beta1=beta1, beta2=beta2, eps=adam_eps, weight_decay=weight_decay,
                           max_norm=grad_clip)
-        self.gate = gate
+        self.gate, self.gate_rows = gate, gate_rows
         self.op = MoEFeedForward.from_op(ff, compute_dtype=compute_dtype,
                                          flags=flags | _lib.MXM_FLAG_KEEP_FOR_BACKWARD)
         kept = "bf16" if self.bf16 else "fp32"
@@ -339,11 +339,19 @@ class MoEBlockTrainer:
 
     def step_host(self, x: np.ndarray, d_out: np.ndarray, lr: float, gate: Optional[np.ndarray] = None):
         """Forward, backward and update on host arrays: a dict of out, aux (weighted),
-        entropy, dx, d_gate (with a gate), norm and applied."""
+        entropy, dx, d_gate (with a gate), norm and applied.  gate is fp32 [ceil(N /
+        gate_rows), 1 or D] (axes of one more or less are the same), d_gate as it."""
         x = np.ascontiguousarray(x, np.float32)
         d_out = np.ascontiguousarray(d_out, np.float32)
         if x.shape != (self.N, self.D) or d_out.shape != x.shape:
             raise ValueError(f"x and d_out must be [{self.N}, {self.D}]")
+        if (gate is not None) != (self.gate is not None):
+            raise ValueError("a step takes a gate where the block has one, else none")
+        if gate is not None:
+            want = [-(-self.N // self.gate_rows), self.D if self.gate == "channel" else 1]
+            long = lambda shape: [n for n in shape if n != 1]  # noqa: E731
+            if long(np.shape(gate)) != long(want):
+                raise ValueError(f"gate must be {want}, got {list(np.shape(gate))}")
         dev = _lib.DeviceBuffer
         bx, bo, bd = dev.from_array(x), dev(x.nbytes), dev.from_array(d_out)
         bg = bdg = None
