@@ -371,7 +371,8 @@ int mxm_grads_destroy(int64_t h);
  * writes, NULL or the gradient's own pointer: in place.  params, m and v (fp32)
  * are AdamW's, all or none; params_bf16, or NULL, gets the updated params
  * rounded to bf16.  No two of the tensors may overlap.  Waits for the handle's stream; calls use the
- * pointers bound last, those captured into a graph too. */
+ * pointers bound last, those captured into a graph too (a captured mxm_grads_adamw
+ * that runs while no params are bound updates nothing and sets *skipped to 1). */
 int mxm_grads_bind(int64_t h, const void* const* grads, void* const* clipped, void* const* params,
                    void* const* m, void* const* v, void* const* params_bf16);
 

@@ -107,6 +107,8 @@ __device__ __forceinline__ double block_sum(double v, double* red) {
 }
 
 __device__ __forceinline__ void finish_norm(const GradArgs& a, double total) {
+  // (a captured step may be replayed after a bind without params: it updates nothing)
+  const bool bound = !a.adamw || a.n_chunks == 0 || a.chunks[0].p != nullptr;
   const double norm = sqrt(total);
   const bool finite = total <= 1.7976931348623157e308;  // false for NaN too
   if (a.norm) *a.norm = (float)norm;
@@ -117,11 +119,11 @@ __device__ __forceinline__ void finish_norm(const GradArgs& a, double total) {
   }
   GradScalars r;
   r.coef = (float)coef;
-  r.skip = !finite;
+  r.skip = !finite || !bound;
   r.step_size = r.root2 = 0.0f;
   if (a.adamw) {
-    if (a.skipped) *a.skipped = !finite;
-    if (finite) {
+    if (a.skipped) *a.skipped = r.skip;
+    if (!r.skip) {
       const int64_t done = *a.step, t = (done > 0 ? done : 0) + 1;
       *a.step = t;
       r.step_size = (float)(a.lr / (1.0 - pow(a.beta1, (double)t)));

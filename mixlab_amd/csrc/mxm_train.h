@@ -70,7 +70,7 @@ struct GradScalars {
   float coef;         // multiplies every gradient
   float step_size;    // lr / (1 - beta1^t)
   float root2;        // 1 / sqrt(1 - beta2^t)
-  int32_t skip;       // the norm is not finite
+  int32_t skip;       // the norm is not finite, or no params are bound
 };
 struct GradArgs {
   const GradChunk* chunks;
