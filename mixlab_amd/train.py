@@ -203,6 +203,7 @@ class MoEBlockTrainer:
         self.step = buf(8)
         self.step.upload(np.zeros(1, np.int64))
         self._x = 0  # the last forward's input
+        self._ready = False  # _g holds gradients that no update has taken
 
     def _place(self) -> None:
         """The tensors' places in the flat buffers: the expert matrices side by side
@@ -224,7 +225,7 @@ class MoEBlockTrainer:
         self._p, self._g, self._m, self._v = (buf(self._total * 4) for _ in range(4))
         self._p16 = buf(self._total * 2) if self.bf16 else None
         zeros = np.zeros(self._total, np.float32)
-        for b in (self._p, self._m, self._v):
+        for b in (self._p, self._g, self._m, self._v):
             b.upload(zeros)
         self.grads = GradientSet(sizes, decay=[0.0 if len(m.shape) == 1 else 1.0 for m in self.metas],
                                  share=self.op)
@@ -275,6 +276,7 @@ class MoEBlockTrainer:
         self._m.upload(zeros)
         self._v.upload(zeros)
         self.step.upload(np.zeros(1, np.int64))
+        self._ready = False
         self._bind()
 
     def _read(self, b) -> list:
@@ -310,6 +312,7 @@ class MoEBlockTrainer:
         the loss's gradient d_out [N, D] at its output and the weighted aux loss."""
         if not self._x:
             raise _lib.MixMoEError("backward without a forward")
+        self._ready = False
         self.exit.backward(self.N, delta=self._delta.value, dh=d_out, d_delta=self._d_delta.value,
                            gate=self._gate, d_gate=d_gate,
                            post_scale=self._weight("moe_post_norm_scale"),
@@ -323,11 +326,15 @@ class MoEBlockTrainer:
         self.entry.backward(self.N, self._x, dh=d_out, dy=self._d_xn.value, dx=dx,
                             norm_scale=self._weight("moe_norm_scale"),
                             d_norm_scale=self._grad("moe_norm_scale"))
-        self._x = 0
+        self._x, self._ready = 0, True
 
     def update(self, lr: float) -> bool:
-        """One AdamW step on the last backward's gradients; the op gets the new
-        weights.  False where a gradient was not finite and nothing changed."""
+        """One AdamW step on the last backward's gradients, which it uses up; the op
+        gets the new weights.  False where a gradient was not finite and nothing
+        changed."""
+        if not self._ready:
+            raise _lib.MixMoEError("update without a backward on these weights since the last update")
+        self._ready = False
         h = self.hyper
         self.grads.adamw(lr, h["beta1"], h["beta2"], h["eps"], h["weight_decay"], h["max_norm"],
                          self.step.value, self.norm.value, self.skipped.value)

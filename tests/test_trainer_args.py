@@ -4,6 +4,8 @@ from __future__ import annotations
 import numpy as np
 import pytest
 
+from mixlab_amd import _lib
+from mixlab_amd.moe import WeightMeta
 from mixlab_amd.train import MoEBlockTrainer
 
 
@@ -35,3 +37,60 @@ def test_gate_where_the_block_has_one():
         _trainer().step_host(X, X, 1e-3, np.zeros((10, 1), np.float32))
     with pytest.raises(ValueError, match="gate"):
         _trainer(gate="row").step_host(X, X, 1e-3)
+
+
+class _Calls:
+    """Stands in for the handles and the device: every method is noted by name."""
+
+    def __init__(self, fail=()):
+        self.names, self.fail, self.handle, self.value = [], set(fail), 1, 4096
+
+    def __getattr__(self, name):
+        def call(*a, **kw):
+            self.names.append(name)
+            if name in self.fail:
+                raise _lib.MixMoEError(name)
+            return np.zeros(1, np.int32) if name == "download" else 0
+        return call
+
+
+@pytest.fixture
+def stub(monkeypatch):
+    """A trainer on such stand-ins, and what was called."""
+    calls = _Calls()
+    monkeypatch.setattr(_lib, "load", lambda: calls)
+    metas = [WeightMeta("expert_0_w_up", [8, 8])]
+    hyper = dict(beta1=0.9, beta2=0.95, eps=1e-8, weight_decay=0.0, max_norm=1.0)
+    tr = _trainer(op=calls, entry=calls, exit=calls, grads=calls, metas=metas, _at=[0], _total=64,
+                  hyper=hyper, aux_weight=0.0, _x=0, _ready=False)
+    for name in ("_xn", "_delta", "_d_delta", "_d_xn", "_p", "_g", "_m", "_v", "aux", "entropy", "norm",
+                 "skipped", "step"):
+        setattr(tr, name, calls)
+    return tr, calls
+
+
+def test_update_needs_a_backward(stub):
+    """An update takes the gradients of a backward that ran on the present weights, once."""
+    tr, calls = stub
+
+    def refused():
+        before = calls.names.count("adamw")
+        with pytest.raises(_lib.MixMoEError, match="update without a backward"):
+            tr.update(1e-3)
+        assert calls.names.count("adamw") == before
+
+    def step():
+        tr.forward(64, 128)
+        tr.backward(64, 128)
+
+    refused()
+    step()
+    assert tr.update(1e-3)
+    refused()
+    step()
+    tr.set_weights([np.zeros((8, 8))])
+    refused()
+    tr.forward(64, 128)
+    refused()
+    tr.backward(64, 128)
+    assert tr.update(1e-3)
