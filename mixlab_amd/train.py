@@ -299,6 +299,7 @@ class MoEBlockTrainer:
             raise ValueError("the block's training forward keeps x: out must be another buffer")
         if (gate != 0) != (self.gate is not None):
             raise ValueError("the forward takes a gate where the block has one, else none")
+        self._x = 0  # (until all of it is queued)
         self.entry.forward(self.N, x, y=self._xn.value, norm_scale=self._weight("moe_norm_scale"))
         self.op.forward(self._xn.value, _lib.MXM_DTYPE_BF16 if self.bf16 else _lib.MXM_DTYPE_F32,
                         self.N, self._delta.value, self.aux.value, self.entropy.value)

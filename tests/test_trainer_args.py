@@ -94,3 +94,16 @@ def test_update_needs_a_backward(stub):
     refused()
     tr.backward(64, 128)
     assert tr.update(1e-3)
+
+
+def test_backward_after_a_failed_forward(stub):
+    """The op may have kept what a forward that failed gave it: an earlier forward's
+    input does not go with that."""
+    tr, calls = stub
+    tr.forward(64, 128)
+    calls.fail = {"forward"}
+    with pytest.raises(_lib.MixMoEError, match="forward"):
+        tr.forward(256, 512)
+    calls.fail = set()
+    with pytest.raises(_lib.MixMoEError, match="backward without a forward"):
+        tr.backward(64, 128)
