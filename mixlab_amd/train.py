@@ -23,6 +23,15 @@ from .op import _DTYPES, MoEFeedForward
 _GATES = {None: _lib.MXM_GATE_NONE, "row": _lib.MXM_GATE_ROW, "channel": _lib.MXM_GATE_CHANNEL}
 
 
+def _stream_of(share) -> int:
+    """The handle whose stream a new one runs on, 0: a stream of its own."""
+    if share is None:
+        return 0
+    if not share.handle:
+        raise ValueError("share is closed")
+    return share.handle
+
+
 class _Handle:
     """A handle of the library: its stream, waiting for it, its release."""
 
@@ -73,6 +82,7 @@ class ResidualNorm(_Handle):
                  eps: float = 1e-5, branch: bool = True, post_norm: bool = False, norm: bool = True,
                  gate: Optional[str] = None, gate_rows: int = 1, gate_sigmoid: bool = False,
                  backward: bool = True, share=None):
+        stream_of = _stream_of(share)
         self._lib = _lib.init()
         flags = ((_lib.MXM_RESNORM_BRANCH if branch else 0)
                  | (_lib.MXM_RESNORM_POST_NORM if post_norm else 0)
@@ -83,8 +93,7 @@ class ResidualNorm(_Handle):
                                                     scale_dtype, grad_dtype)),
                 flags, _GATES[gate], gate_rows]
         arr = (ctypes.c_int64 * len(vals))(*vals)
-        self._open(self._lib.mxm_resnorm_create(arr, len(vals), float(eps),
-                                                share.handle if share is not None else 0))
+        self._open(self._lib.mxm_resnorm_create(arr, len(vals), float(eps), stream_of))
 
     def forward(self, rows: int, x: int, delta: int = 0, h: int = 0, y: int = 0,
                 post_scale: int = 0, branch_scale: int = 0, gate: int = 0,
@@ -112,6 +121,7 @@ class GradientSet(_Handle):
 
     def __init__(self, sizes: Sequence[int], dtypes: Union[str, Sequence[str]] = "fp32",
                  decay: Optional[Sequence[float]] = None, share=None):
+        stream_of = _stream_of(share)
         self._lib = _lib.init()
         n = len(sizes)
         if isinstance(dtypes, str):
@@ -123,8 +133,7 @@ class GradientSet(_Handle):
         cs = (ctypes.c_int64 * max(1, n))(*[int(s) for s in sizes])
         cd = (ctypes.c_int32 * max(1, n))(*[_DTYPES[t] for t in dtypes])
         cw = None if decay is None else (ctypes.c_float * max(1, n))(*decay)
-        self._open(self._lib.mxm_grads_create(cs, cd, cw, n,
-                                              share.handle if share is not None else 0))
+        self._open(self._lib.mxm_grads_create(cs, cd, cw, n, stream_of))
 
     def bind(self, grads: Sequence[int], clipped: Optional[Sequence[int]] = None,
              params: Optional[Sequence[int]] = None, m: Optional[Sequence[int]] = None,

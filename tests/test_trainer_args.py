@@ -6,7 +6,7 @@ import pytest
 
 from mixlab_amd import _lib
 from mixlab_amd.moe import WeightMeta
-from mixlab_amd.train import MoEBlockTrainer
+from mixlab_amd.train import GradientSet, MoEBlockTrainer, ResidualNorm
 
 
 def _trainer(**kw):
@@ -107,3 +107,13 @@ def test_backward_after_a_failed_forward(stub):
     calls.fail = set()
     with pytest.raises(_lib.MixMoEError, match="backward without a forward"):
         tr.backward(64, 128)
+
+
+@pytest.mark.parametrize("make", [lambda share: ResidualNorm(8, 4, share=share),
+                                  lambda share: GradientSet([8], share=share)])
+def test_sharing_the_stream_of_a_closed_handle(make):
+    """A closed object has no stream: a new one would not be in order with anything."""
+    closed = object.__new__(ResidualNorm)
+    closed.handle = 0
+    with pytest.raises(ValueError, match="share is closed"):
+        make(closed)
