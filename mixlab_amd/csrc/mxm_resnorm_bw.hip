@@ -148,11 +148,12 @@ __global__ __launch_bounds__(most_threads(LPR)) void resnorm_bw_kernel(ResNormAr
     if (a.norm || post) row_sum<LPR>(s, red + (it & 1) * 48);
     if (a.norm) {
       const float rn = 1.0f / __builtin_sqrtf(s[0] * a.inv_d + a.eps);
-      const float kn = rn * rn * rn * (s[1] * a.inv_d);
+      const float k = rn * (s[1] * a.inv_d);  // (rn^3 leaves fp32's range where rn does not)
 #pragma unroll
       for (int e = 0; e < E; ++e) {
-        t[e] = __builtin_fmaf(-kn, h[e], __builtin_fmaf(rn, w[e] * dy[e], t[e]));
-        if (valid) aw[e] = __builtin_fmaf(rn, dy[e] * h[e], aw[e]);
+        const float hn = rn * h[e];
+        t[e] = __builtin_fmaf(rn, __builtin_fmaf(-k, hn, w[e] * dy[e]), t[e]);
+        if (valid) aw[e] = __builtin_fmaf(dy[e], hn, aw[e]);
       }
     }
 #pragma unroll
@@ -170,22 +171,23 @@ __global__ __launch_bounds__(most_threads(LPR)) void resnorm_bw_kernel(ResNormAr
     }
     if (a.branch) {
       const float rp = post ? 1.0f / __builtin_sqrtf(s[2] * a.inv_d + a.eps) : 1.0f;
-      // q = sum f t delta, times the gate where that differs by channel
+      // q = sum f t z, times the gate where that differs by channel
       float q[1] = {0.0f};
       const float g = CH ? 1.0f : ga[0];
 #pragma unroll
       for (int e = 0; e < E; ++e) {
-        const float td = t[e] * dl[e];
-        const float gt = CH ? ga[CH ? e : 0] * td : td;
+        dl[e] = rp * dl[e];  // z
+        const float tz = t[e] * dl[e];
+        const float gt = CH ? ga[CH ? e : 0] * tz : tz;
         if (valid) {  // (past the chunk's rows 1 / sqrt(eps) or a gate times 0 need not be 0)
-          aq[e] = __builtin_fmaf(g * rp, gt, aq[e]);
-          if (CH) ag[CH ? e : 0] = __builtin_fmaf(rp * f[e], td, ag[CH ? e : 0]);
+          aq[e] = __builtin_fmaf(g, gt, aq[e]);
+          if (CH) ag[CH ? e : 0] = __builtin_fmaf(f[e], tz, ag[CH ? e : 0]);
         }
         q[0] = __builtin_fmaf(f[e], gt, q[0]);
       }
       if (post || a.gate == 1) row_sum<LPR>(q, red + 96 + (it & 1) * 16);
-      if (!CH && valid) ag[0] = __builtin_fmaf(rp, q[0], ag[0]);
-      const float kp = post ? rp * rp * rp * (g * q[0] * a.inv_d) : 0.0f;
+      if (!CH && valid) ag[0] = ag[0] + q[0];
+      const float k = post ? q[0] * a.inv_d : 0.0f;
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         if (!(valid && at[i] < D)) continue;
@@ -194,7 +196,7 @@ __global__ __launch_bounds__(most_threads(LPR)) void resnorm_bw_kernel(ResNormAr
         for (int j = 0; j < V; ++j) {
           const int e = i * V + j;
           const float gf = CH ? ga[CH ? e : 0] * f[e] : f[e];
-          out[j] = __builtin_fmaf(-kp, dl[e], (g * rp) * (gf * t[e]));
+          out[j] = (g * rp) * __builtin_fmaf(-k, dl[e], gf * t[e]);
         }
         store<GT, ODD>(a.d_delta, row, at[i], D, out);
       }

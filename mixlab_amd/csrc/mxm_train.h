@@ -17,9 +17,9 @@
 //   h = x + a * f * z                              rounded to the stream's type
 //   rn = 1 / sqrt(mean_d(h^2) + eps),  y = h * rn * w     of the rounded h
 // and backwards, given dh and dy:
-//   u = w * dy,  t = dh + rn * u - h * rn^3 * mean_d(u * h)
-//   dx = t,  dw = sum_n dy * h * rn
-//   e = t * a * f,  d_delta = rp * e - delta * rp^3 * mean_d(e * delta)  (post norm; else e)
+//   u = w * dy,  hn = rn * h,  t = dh + rn * (u - hn * mean_d(u * hn))
+//   dx = t,  dw = sum_n dy * hn
+//   e = t * a * f,  d_delta = rp * (e - z * mean_d(e * z))               (post norm; else e)
 //   q = t * z,  d_scale = post * sum_n a q,  d_post = scale * sum_n a q,
 //   d_gate = a' * sum over the gate's rows (and over d, for a gate per row) of f q
 struct ResNormArgs {

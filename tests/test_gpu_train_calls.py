@@ -3,9 +3,11 @@ buffers that a program can come to."""
 import numpy as np
 import pytest
 
+from mixlab_amd.train import GradientSet, ResidualNorm
 from oracle import train as ot
+from tests.test_gpu_resnorm import _case, _col_c, run_backward
 from tests.test_gpu_train_streams import Graph
-from tests.train_testutil import Dev, close
+from tests.train_testutil import Dev, as_kept, close
 
 pytestmark = pytest.mark.gpu
 
@@ -13,8 +15,6 @@ pytestmark = pytest.mark.gpu
 def test_replayed_update_after_a_bind_without_params(gpu_lib):
     """A captured AdamW step reads the pointers bound last: with none for params it
     updates nothing, and goes on once they are bound again."""
-    from mixlab_amd.train import GradientSet
-
     sizes = [1000, 0, 3]
     rng = np.random.default_rng(0)
     with GradientSet(sizes) as s:
@@ -43,3 +43,31 @@ def test_replayed_update_after_a_bind_without_params(gpu_lib):
         assert not np.array_equal(state()[0], once[0])
         assert step.get()[0] == 2 and skipped.get()[0] == 0
         graph.close()
+
+
+def _check_backward(v, got, D, size_bound, **kw):
+    """Row and column gradients within size_bound of the sums over absolute values."""
+    f = lambda k: v[k].astype(np.float64)  # noqa: E731
+    args = (f("h"), f("delta"), None, f("dy"), v["post_scale"], v["branch_scale"], v.get("gate"))
+    want = ot.resnorm_backward(*args, post_norm=True, norm_scale=v["norm_scale"], **kw)
+    size = ot.resnorm_backward(*args, post_norm=True, norm_scale=v["norm_scale"], absolute=True, **kw)
+    for k in want:
+        close(got[k], want[k], size_bound * size[k], v["dtype"] if k in ("dx", "d_delta") else "fp32", k)
+
+
+@pytest.mark.parametrize("N,D", [(5, 64), (9, 300), (4, 1024), (3, 2049), (2, 9000)])
+@pytest.mark.parametrize("size,eps", [(1e15, 1e-5), (1e17, 1e-5), (1e-16, 0.0)])
+@pytest.mark.parametrize("gate", [None, "row", "channel"])
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_backward_of_large_and_tiny_rows(gpu_lib, N, D, size, eps, gate, dtype):
+    """Rows whose 1 / rms has a cube outside fp32's range (the sums' squares are
+    inside it) keep both terms of their gradients.  dh is left out and dy as large
+    as the rows, so that every gradient is far from the range's ends."""
+    c = dict(stream=dtype, delta=dtype, grad=dtype, gate=gate)
+    v = _case(N + D, N, D, **c)
+    for k in ("h", "delta", "dy"):
+        v[k] = as_kept(v[k] * np.float32(size), dtype)
+    with ResidualNorm(D, N, stream_dtype=dtype, delta_dtype=dtype, out_dtype="fp32", grad_dtype=dtype,
+                      post_norm=True, eps=eps, gate=gate) as r:
+        got = run_backward(v, N, D, handle=r, use_dh=False, **c)
+    _check_backward(dict(v, dtype=dtype), got, D, _col_c(N, D), eps=eps)
