@@ -196,7 +196,8 @@ __global__ __launch_bounds__(most_threads(LPR)) void resnorm_bw_kernel(ResNormAr
         for (int j = 0; j < V; ++j) {
           const int e = i * V + j;
           const float gf = CH ? ga[CH ? e : 0] * f[e] : f[e];
-          out[j] = (g * rp) * __builtin_fmaf(-k, dl[e], gf * t[e]);
+          // (without a post norm nothing of delta, which may be infinite)
+          out[j] = (g * rp) * (post ? __builtin_fmaf(-k, dl[e], gf * t[e]) : gf * t[e]);
         }
         store<GT, ODD>(a.d_delta, row, at[i], D, out);
       }

@@ -71,3 +71,21 @@ def test_backward_of_large_and_tiny_rows(gpu_lib, N, D, size, eps, gate, dtype):
                       post_norm=True, eps=eps, gate=gate) as r:
         got = run_backward(v, N, D, handle=r, use_dh=False, **c)
     _check_backward(dict(v, dtype=dtype), got, D, _col_c(N, D), eps=eps)
+
+
+@pytest.mark.parametrize("N,D", [(6, 64), (6, 300), (5, 1024), (3, 2051)])
+@pytest.mark.parametrize("gate", [None, "row", "channel"])
+def test_non_finite_branch_without_a_post_norm(gpu_lib, N, D, gate):
+    """d_delta does not depend on delta then: an infinite or NaN element of it only
+    shows in the sums that read it."""
+    c = dict(post=False, norm=False, gate=gate, gate_rows=2)
+    v = _case(N, N, D, **c)
+    good = run_backward(v, N, D, **c)
+    bad = dict(v, delta=v["delta"].copy())
+    bad["delta"][1, 5], bad["delta"][2, 9] = np.inf, np.nan
+    got = run_backward(bad, N, D, **c)
+    for k in ("dx", "d_delta"):
+        assert np.array_equal(got[k], good[k]), k
+    other = ~np.isin(np.arange(D), (5, 9))
+    assert np.array_equal(got["d_scale"][other], good["d_scale"][other])
+    assert not np.isfinite(got["d_scale"][[5, 9]]).any()
