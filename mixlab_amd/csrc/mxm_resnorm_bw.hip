@@ -187,18 +187,19 @@ __global__ __launch_bounds__(most_threads(LPR)) void resnorm_bw_kernel(ResNormAr
       }
       if (post || a.gate == 1) row_sum<LPR>(q, red + 96 + (it & 1) * 16);
       if (!CH && valid) ag[0] = ag[0] + q[0];
-      const float k = post ? q[0] * a.inv_d : 0.0f;
+#pragma unroll
+      for (int e = 0; e < E; ++e) t[e] = (CH ? ga[CH ? e : 0] * f[e] : f[e]) * t[e];
+      if (post) {  // (else nothing of delta, which may be infinite)
+        const float k = q[0] * a.inv_d;
+#pragma unroll
+        for (int e = 0; e < E; ++e) t[e] = __builtin_fmaf(-k, dl[e], t[e]);
+      }
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         if (!(valid && at[i] < D)) continue;
         float out[V];
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          const int e = i * V + j;
-          const float gf = CH ? ga[CH ? e : 0] * f[e] : f[e];
-          // (without a post norm nothing of delta, which may be infinite)
-          out[j] = (g * rp) * (post ? __builtin_fmaf(-k, dl[e], gf * t[e]) : gf * t[e]);
-        }
+        for (int j = 0; j < V; ++j) out[j] = (g * rp) * t[i * V + j];
         store<GT, ODD>(a.d_delta, row, at[i], D, out);
       }
     }
