@@ -34,6 +34,24 @@ __device__ __forceinline__ Rows rows_of(const ResNormArgs& a, int c) {
   return {first, step, first < end ? (int)(((int64_t)end - first + step - 1) / step) : 0};
 }
 
+// A gate between its load and its gradient.  Of a sigmoid a that is a where a < 1/2,
+// else -(1 - a), for its slope a (1 - a): 1 - a has few digits where a is next to 1
+// (the slope 10 % off at 15 and 0 past 17), and two values an element do not fit
+// the registers.  k - floor(k) is a again, at most 1 - 2^-24.
+constexpr float LEAST_TAIL = 1.17549435e-38f;  // (so that 1 has a sign)
+__device__ __forceinline__ float gate_kept(const ResNormArgs& a, float g) {
+  if (!a.sigmoid) return g;
+  const float tail = mxm_sigmoid(-__builtin_fabsf(g));
+  return g < 0.0f ? tail : tail < LEAST_TAIL ? -LEAST_TAIL : -tail;
+}
+__device__ __forceinline__ float gate_value(const ResNormArgs& a, float k) {
+  return a.sigmoid ? __builtin_amdgcn_fractf(k) : k;
+}
+__device__ __forceinline__ float gate_slope(float k) {
+  const float tail = __builtin_fabsf(k);
+  return tail <= LEAST_TAIL ? 0.0f : tail * (1.0f - tail);
+}
+
 // CH: a gate per channel.  A row's threads walk one chunk; the chunks of a
 // workgroup add their column sums in LDS and store one partial.
 template <int NV, int LPR, int XT, int DT, int GT, int ODD, bool CH>
@@ -166,29 +184,29 @@ __global__ __launch_bounds__(most_threads(LPR)) void resnorm_bw_kernel(ResNormAr
     }
     if (new_gate) {
 #pragma unroll
-      for (int e = 0; e < (CH ? E : 1); ++e) ga[e] = gate_of(a, ga[e]);
+      for (int e = 0; e < (CH ? E : 1); ++e) ga[e] = gate_kept(a, ga[e]);
       fresh = false;
     }
     if (a.branch) {
       const float rp = post ? 1.0f / __builtin_sqrtf(s[2] * a.inv_d + a.eps) : 1.0f;
       // q = sum f t z, times the gate where that differs by channel
       float q[1] = {0.0f};
-      const float g = CH ? 1.0f : ga[0];
+      const float g = CH || !a.gate ? 1.0f : gate_value(a, ga[0]);
 #pragma unroll
       for (int e = 0; e < E; ++e) {
         dl[e] = rp * dl[e];  // z
         const float tz = t[e] * dl[e];
-        const float gt = CH ? ga[CH ? e : 0] * tz : tz;
+        const float gv = CH ? gate_value(a, ga[CH ? e : 0]) : 1.0f;
+        const float gt = CH ? gv * tz : tz;
         if (valid) {  // (past the chunk's rows 1 / sqrt(eps) or a gate times 0 need not be 0)
           aq[e] = __builtin_fmaf(g, gt, aq[e]);
           if (CH) ag[CH ? e : 0] = __builtin_fmaf(f[e], tz, ag[CH ? e : 0]);
         }
         q[0] = __builtin_fmaf(f[e], gt, q[0]);
+        t[e] = (CH ? gv * f[e] : f[e]) * t[e];
       }
       if (post || a.gate == 1) row_sum<LPR>(q, red + 96 + (it & 1) * 16);
       if (!CH && valid) ag[0] = ag[0] + q[0];
-#pragma unroll
-      for (int e = 0; e < E; ++e) t[e] = (CH ? ga[CH ? e : 0] * f[e] : f[e]) * t[e];
       if (post) {  // (else nothing of delta, which may be infinite)
         const float k = q[0] * a.inv_d;
 #pragma unroll
@@ -207,7 +225,7 @@ __global__ __launch_bounds__(most_threads(LPR)) void resnorm_bw_kernel(ResNormAr
     if (a.gate && valid && (--left == 0 || it + 1 == mine.count)) {
       if (a.sigmoid) {
 #pragma unroll
-        for (int e = 0; e < (CH ? E : 1); ++e) ag[e] = ag[e] * (ga[e] * (1.0f - ga[e]));
+        for (int e = 0; e < (CH ? E : 1); ++e) ag[e] = ag[e] * gate_slope(ga[e]);
       }
       if (a.group_chunks == 0) {  // the group is whole: its gate's gradient goes out
         if (a.d_gate) {

@@ -22,7 +22,7 @@ def gate_values(gate, sigmoid):
     if not sigmoid:
         return g, np.ones_like(g)
     a = 1.0 / (1.0 + np.exp(-g))
-    return a, a * (1.0 - a)
+    return a, a * (1.0 / (1.0 + np.exp(g)))  # (1 - a loses its digits next to 1)
 
 
 def resnorm_sum(x, delta, post_scale=None, branch_scale=None, gate=None, gate_rows=1, sigmoid=False,

@@ -5,7 +5,7 @@ import pytest
 
 from mixlab_amd.train import GradientSet, ResidualNorm
 from oracle import train as ot
-from tests.test_gpu_resnorm import _case, _col_c, run_backward
+from tests.test_gpu_resnorm import _case, _col_c, _row_c, run_backward
 from tests.test_gpu_train_streams import Graph
 from tests.train_testutil import Dev, as_kept, close
 
@@ -89,3 +89,43 @@ def test_non_finite_branch_without_a_post_norm(gpu_lib, N, D, gate):
     other = ~np.isin(np.arange(D), (5, 9))
     assert np.array_equal(got["d_scale"][other], good["d_scale"][other])
     assert not np.isfinite(got["d_scale"][[5, 9]]).any()
+
+
+@pytest.mark.parametrize("gate,gate_rows", [("row", 1), ("row", 7), ("row", 40), ("channel", 1), ("channel", 7),
+                                            ("channel", 40)])
+@pytest.mark.parametrize("N,D", [(40, 64), (40, 544), (9, 2051)])
+@pytest.mark.parametrize("post", [False, True])
+def test_gradient_of_a_saturated_gate(gpu_lib, N, D, gate, gate_rows, post):
+    """A sigmoid's slope a (1 - a) keeps its digits where a is next to 1: gates from
+    -60 to 60 (slopes from 9e-27 on).  The exponential and the slope add about ten
+    roundings, within the handful that the bound counts."""
+    c = dict(post=post, norm=False, gate=gate, gate_rows=gate_rows, sigmoid=True)
+    v = _case(N + D, N, D, **c)
+    v["gate"] = np.random.default_rng(D).uniform(-60, 60, v["gate"].shape).astype(np.float32)
+    got = run_backward(v, N, D, **c)
+    f = lambda k: v[k].astype(np.float64)  # noqa: E731
+    args = (None, f("delta"), f("dh"), None, v.get("post_scale"), v["branch_scale"], v["gate"], gate_rows,
+            True, post)
+    want, size = ot.resnorm_backward(*args), ot.resnorm_backward(*args, absolute=True)
+    for k in got:
+        close(got[k], want[k], (_row_c(D) if k == "d_delta" else _col_c(N, D)) * size[k], "fp32", k)
+
+
+def test_gates_of_any_value(gpu_lib):
+    """Infinite and NaN gates through the sigmoid, both zeros, and the largest."""
+    N, D = 8, 96
+    c = dict(post=True, norm=False, gate="row", gate_rows=1, sigmoid=True)
+    v = _case(1, N, D, **c)
+    v["gate"][:, 0] = (np.inf, -np.inf, 0.0, -0.0, 3e38, -3e38, np.nan, 1.0)
+    got = run_backward(v, N, D, **c)
+    with np.errstate(over="ignore"):
+        a = 1.0 / (1.0 + np.exp(-v["gate"].astype(np.float64)))
+    assert np.isnan(got["d_delta"][6]).all() and np.isnan(got["d_gate"][6])
+    assert np.all(got["d_delta"][[1, 5]] == 0) and np.all(got["d_gate"][[0, 1, 4, 5]] == 0)
+    keep = [n for n in range(N) if n != 6]
+    args = [x[keep].astype(np.float64) for x in (v["delta"], v["dh"], v["gate"])]
+    want = ot.resnorm_backward(None, args[0], args[1], None, v["post_scale"], v["branch_scale"], a[keep],
+                               1, False, True)
+    size = ot.resnorm_backward(None, args[0], args[1], None, v["post_scale"], v["branch_scale"], a[keep],
+                               1, False, True, absolute=True)
+    close(got["d_delta"][keep], want["d_delta"], _row_c(D) * size["d_delta"], "fp32", "d_delta")
