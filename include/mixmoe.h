@@ -377,11 +377,12 @@ int mxm_grads_bind(int64_t h, const void* const* grads, void* const* clipped, vo
                    void* const* m, void* const* v, void* const* params_bf16);
 
 /* norm [1] fp32 = sqrt(sum of squares over all tensors), summed in 64 bits in a
- * fixed order. */
+ * fixed order; infinite where it is past fp32's largest value.  The two calls
+ * below go by this fp32 value. */
 int mxm_grads_norm(int64_t h, float* norm);
 
-/* clipped = g * min(1, max_norm / (norm + 1e-6)); where the norm is not finite
- * the gradients are copied as they are.  norm may be NULL. */
+/* clipped = g * min(1, max_norm / (norm + 1e-6)), a factor in fp32; where the norm
+ * is not finite the gradients are copied as they are.  norm may be NULL. */
 int mxm_grads_clip(int64_t h, double max_norm, float* norm);
 
 /* One AdamW step on the clipped gradients (max_norm 0: not clipped), which are

@@ -2,11 +2,11 @@
 // with that clipping in it.
 //
 //   norm = sqrt(sum g^2)                                   in 64 bits
-//   coef = min(1, max_norm / (norm + 1e-6))                (1 where the norm is not finite)
+//   coef = min(1, max_norm / (norm + 1e-6))                (1 where the norm is not finite in fp32)
 //   g' = coef g
 //   m = beta1 m + (1 - beta1) g',  v = beta2 v + (1 - beta2) g'^2
 //   p = p - lr decay p - lr (m / (1 - beta1^t)) / (sqrt(v / (1 - beta2^t)) + eps)
-// A norm that is not finite leaves p, m, v and the step count as they were.
+// Such a norm leaves p, m, v and the step count as they were.
 // Bound by memory: the norm of 201 M fp32 gradients 120 us (6.7 TB/s; 115 at the
 // rate of a plain read stream), AdamW over 403 M parameters with bf16 copies 2.00
 // ms of 12.1 GB (6.0 TB/s) after the norm's 0.23.
@@ -110,8 +110,9 @@ __device__ __forceinline__ void finish_norm(const GradArgs& a, double total) {
   // (a captured step may be replayed after a bind without params: it updates nothing)
   const bool bound = !a.adamw || a.n_chunks == 0 || a.chunks[0].p != nullptr;
   const double norm = sqrt(total);
-  const bool finite = total <= 1.7976931348623157e308;  // false for NaN too
-  if (a.norm) *a.norm = (float)norm;
+  const float shown = (float)norm;
+  const bool finite = shown <= 3.40282347e38f;  // (what *norm says; false for NaN too)
+  if (a.norm) *a.norm = shown;
   double coef = 1.0;
   if (finite && a.max_norm > 0.0) {
     coef = a.max_norm / (norm + 1e-6);

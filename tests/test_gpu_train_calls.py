@@ -7,7 +7,7 @@ from mixlab_amd.train import GradientSet, ResidualNorm
 from oracle import train as ot
 from tests.test_gpu_resnorm import _case, _col_c, _row_c, run_backward
 from tests.test_gpu_train_streams import Graph
-from tests.train_testutil import Dev, as_kept, close
+from tests.train_testutil import U32, Dev, as_kept, close
 
 pytestmark = pytest.mark.gpu
 
@@ -129,3 +129,60 @@ def test_gates_of_any_value(gpu_lib):
     size = ot.resnorm_backward(None, args[0], args[1], None, v["post_scale"], v["branch_scale"], a[keep],
                                1, False, True, absolute=True)
     close(got["d_delta"][keep], want["d_delta"], _row_c(D) * size["d_delta"], "fp32", "d_delta")
+
+
+@pytest.mark.parametrize("max_norm", [0.0, 1.0, 1e30])
+def test_norm_beyond_fp32(gpu_lib, max_norm):
+    """Finite gradients whose norm is infinite as fp32: *norm says so, and so do the
+    step that changes nothing and the clip that copies."""
+    g = np.array([3e38, 0.0, -3e38, 1.0, 2.0], np.float32)
+    old = [np.full(5, x, np.float32) for x in (0.5, 0.25, 0.125)]
+    with GradientSet([5]) as s:
+        d, out, (p, m, v) = Dev(g), Dev.out((5,)), (Dev(a) for a in old)
+        step, norm, skipped = Dev(np.full(1, 7, np.int64), "int64"), Dev.out((1,)), Dev.out((1,), np.int32)
+        s.bind([d.ptr], [out.ptr], [p.ptr], [m.ptr], [v.ptr])
+        s.adamw(1e-2, 0.9, 0.99, 1e-8, 0.1, max_norm, step.ptr, norm.ptr, skipped.ptr)
+        s.synchronize()
+        assert norm.get()[0] == np.inf and skipped.get()[0] == 1 and step.get()[0] == 7
+        for a, b in zip((p, m, v), old):
+            assert np.array_equal(a.get(), b)
+        if max_norm:
+            s.clip(max_norm, norm.ptr)
+            s.synchronize()
+            assert norm.get()[0] == np.inf and np.array_equal(out.get(), g)
+
+
+def test_largest_norm_of_fp32(gpu_lib):
+    """A norm next to fp32's largest value is finite: the step runs and clips.  The
+    coefficient is a subnormal, off by 2^-150, half of fp32's smallest step."""
+    g = np.array([2e38, -2e38, 1e38, 1.5e38, 0.5], np.float32)
+    n = ot.global_norm([g])
+    coef = ot.clip_coef(n, 1.0)
+    bound = (2.0 ** -150 + 3 * U32 * coef) * np.abs(g.astype(np.float64))
+    with GradientSet([5]) as s:
+        d, out, (p, m, v) = Dev(g), Dev.out((5,)), (Dev(np.zeros(5, np.float32)) for _ in range(3))
+        step, norm, skipped = Dev(np.zeros(1, np.int64), "int64"), Dev.out((1,)), Dev.out((1,), np.int32)
+        s.bind([d.ptr], [out.ptr], [p.ptr], [m.ptr], [v.ptr])
+        s.clip(1.0, norm.ptr)
+        s.adamw(1e-2, 0.9, 0.99, 1e-8, 0.0, 1.0, step.ptr, norm.ptr, skipped.ptr)
+        s.synchronize()
+        close(norm.get(), [n], 0, "fp32", "norm")
+        assert skipped.get()[0] == 0 and step.get()[0] == 1
+        close(out.get(), coef * g.astype(np.float64), bound, "fp32", "clipped")
+        close(m.get(), 0.1 * coef * g.astype(np.float64), bound, "fp32", "m")
+
+
+@pytest.mark.parametrize("size", [1e-40, 1e-38, 1e-44])
+@pytest.mark.parametrize("n", [3, 1000, 200000])
+def test_norm_of_subnormal_gradients(gpu_lib, size, n):
+    """Subnormal gradients are not flushed, and neither is a subnormal norm: half of
+    fp32's smallest step, or of the value's."""
+    a = (np.random.default_rng(n).standard_normal(n) * size).astype(np.float32)
+    assert np.any(a)
+    with GradientSet([n]) as s:
+        d, norm = Dev(a), Dev.out((1,))
+        s.bind([d.ptr])
+        s.norm(norm.ptr)
+        s.synchronize()
+        want = ot.global_norm([a])
+        assert abs(float(norm.get()[0]) - want) <= max(2.0 ** -150, U32 * want) * (1 + 1e-9)
