@@ -316,8 +316,11 @@ __global__ __launch_bounds__(JOIN_COLS* JOIN_SLICES) void resnorm_join_kernel(Re
   if (kind == 0) {
     a.d_w[d] = s;
   } else if (kind == 1) {
-    if (a.d_scale) a.d_scale[d] = a.post ? s * load_one(a.post, a.p_bf16, d) : s;
-    if (a.d_post) a.d_post[d] = a.scale ? s * load_one(a.scale, a.p_bf16, d) : s;
+    // (both before the stores: a gradient may take its scale's place)
+    const float post = a.post ? load_one(a.post, a.p_bf16, d) : 1.0f;
+    const float scale = a.scale ? load_one(a.scale, a.p_bf16, d) : 1.0f;
+    if (a.d_scale) a.d_scale[d] = s * post;
+    if (a.d_post) a.d_post[d] = s * scale;
   } else {
     a.d_gate[(size_t)group * width + d] = s;
   }

@@ -123,6 +123,46 @@ void check_pointer(const char* what, const char* name, const void* p, bool bf16,
     fail("%s %s is not aligned to its elements", what, name);
 }
 
+// Where a call's tensors lie.  An output may be one of the inputs that it is
+// computed beside, element for element (`in_place`, a mask of kinds); every other
+// overlap of an output is refused.
+struct Tensors {
+  struct One {
+    const char* name;
+    uintptr_t from, to;
+    int item;
+    unsigned kind;      // of an input
+    unsigned in_place;  // of an output: kinds of inputs
+  };
+  One all[14];
+  int n = 0;
+  void add(const char* name, const void* p, int64_t elements, bool bf16, unsigned kind, unsigned in_place) {
+    if (!p || elements <= 0) return;
+    const uintptr_t from = reinterpret_cast<uintptr_t>(p);
+    const int item = bf16 ? 2 : 4;
+    all[n++] = {name, from, from + (uintptr_t)elements * item, item, kind, in_place};
+  }
+  void in(const char* name, const void* p, int64_t elements, bool bf16, unsigned kind) {
+    add(name, p, elements, bf16, kind, 0);
+  }
+  void out(const char* name, const void* p, int64_t elements, bool bf16, unsigned in_place) {
+    add(name, p, elements, bf16, 0, in_place);
+  }
+  void check(const char* what) const {
+    for (int i = 0; i < n; ++i) {
+      const One& o = all[i];
+      if (!o.in_place) continue;
+      for (int j = 0; j < n; ++j) {
+        const One& t = all[j];
+        if (i == j || t.from >= o.to || o.from >= t.to) continue;
+        if ((o.in_place & t.kind) && t.from == o.from && t.to == o.to && t.item == o.item) continue;
+        fail("%s %s overlaps %s", what, o.name, t.name);
+      }
+    }
+  }
+};
+enum : unsigned { ROWS = 1, POST = 2, SCALE = 4, GATE = 8, NORM = 16 };
+
 // The stream of `stream_of`, or a new one on the current device.
 std::shared_ptr<StreamRef> choose_stream(std::shared_ptr<StreamRef> shared) {
   if (shared) return shared;
@@ -136,6 +176,10 @@ std::shared_ptr<StreamRef> shared_stream(const char* what, int64_t stream_of) {
   auto s = stream_of_handle(stream_of);
   if (!s) fail("%s stream_of %lld is not a live handle", what, (long long)stream_of);
   return s;
+}
+
+int64_t gate_elements(const ResNormArgs& a, int64_t rows) {
+  return a.gate ? (rows + a.gate_rows - 1) / a.gate_rows * (a.gate == 2 ? a.D : 1) : 0;
 }
 
 int cu_count(int device) {
@@ -244,6 +288,17 @@ int mxm_resnorm_forward(int64_t h, int64_t rows, const void* x, const void* delt
     if (post_scale && !a.post_norm) fail(RESNORM " post_scale given without MXM_RESNORM_POST_NORM");
     if (branch_scale && !a.branch) fail(RESNORM " branch_scale given without MXM_RESNORM_BRANCH");
     if (norm_scale && !a.norm) fail(RESNORM " norm_scale given without MXM_RESNORM_NORM");
+    const int64_t n = rows * a.D, gates = gate_elements(a, rows);
+    Tensors t;
+    t.in("x", x, n, a.x_bf16, ROWS);
+    if (a.branch) t.in("delta", delta, n, a.delta_bf16, ROWS);
+    t.in("post_scale", post_scale, a.D, a.p_bf16, POST);
+    t.in("branch_scale", branch_scale, a.D, a.p_bf16, SCALE);
+    t.in("norm_scale", norm_scale, a.D, a.p_bf16, NORM);
+    t.in("gate", gate, gates, a.p_bf16, GATE);
+    if (a.branch) t.out("h", h_out, n, a.x_bf16, ROWS);
+    if (a.norm) t.out("y", y, n, a.y_bf16, ROWS);
+    t.check(RESNORM);
     const DeviceGuard guard(r->stream_ref->device);
     a.N = (int)rows;
     a.x = x;
@@ -293,6 +348,23 @@ int mxm_resnorm_backward(int64_t h, int64_t rows, const void* h_in, const void* 
     if ((norm_scale || d_norm_scale) && !a.norm)
       fail(RESNORM " norm_scale given without MXM_RESNORM_NORM");
     if (d_gate && !a.gate) fail(RESNORM " d_gate given without a gate");
+    const int64_t n = rows * a.D, gates = gate_elements(a, rows);
+    Tensors t;
+    if (a.norm) t.in("h", h_in, n, a.x_bf16, ROWS);
+    if (a.branch) t.in("delta", delta, n, a.delta_bf16, ROWS);
+    t.in("dh", dh, n, a.g_bf16, ROWS);
+    if (a.norm) t.in("dy", dy, n, a.g_bf16, ROWS);
+    t.in("post_scale", post_scale, a.D, a.p_bf16, POST);
+    t.in("branch_scale", branch_scale, a.D, a.p_bf16, SCALE);
+    t.in("norm_scale", norm_scale, a.D, a.p_bf16, NORM);
+    t.in("gate", gate, gates, a.p_bf16, GATE);
+    t.out("dx", dx, n, a.g_bf16, ROWS);
+    if (a.branch) t.out("d_delta", d_delta, n, a.g_bf16, ROWS);
+    t.out("d_post_scale", d_post_scale, a.D, false, POST);
+    t.out("d_branch_scale", d_branch_scale, a.D, false, SCALE);
+    t.out("d_gate", d_gate, gates, false, GATE);
+    t.out("d_norm_scale", d_norm_scale, a.D, false, NORM);
+    t.check(RESNORM);
     const DeviceGuard guard(r->stream_ref->device);
     a.N = (int)rows;
     a.delta = delta;

@@ -3,6 +3,7 @@ buffers that a program can come to."""
 import numpy as np
 import pytest
 
+from mixlab_amd import _lib
 from mixlab_amd.train import GradientSet, ResidualNorm
 from oracle import train as ot
 from tests.test_gpu_resnorm import _case, _col_c, _row_c, run_backward
@@ -186,3 +187,91 @@ def test_norm_of_subnormal_gradients(gpu_lib, size, n):
         s.synchronize()
         want = ot.global_norm([a])
         assert abs(float(norm.get()[0]) - want) <= max(2.0 ** -150, U32 * want) * (1 + 1e-9)
+
+
+N, D = 6, 24
+ITEM = {"fp32": 4, "bf16": 2}
+
+
+def _spare(dtype="fp32", rows=N):
+    return Dev.out((rows, D), dtype)
+
+
+@pytest.mark.parametrize("types", ["fp32", "mixed"])
+def test_overlaps_of_a_forward(gpu_lib, types):
+    """An output in the place of an input of its type is fine; the rest is refused
+    before anything runs."""
+    b = "bf16" if types == "mixed" else "fp32"
+    with ResidualNorm(D, N, delta_dtype=b, out_dtype="fp32", post_norm=True, gate="channel", gate_rows=4) as r:
+        x, delta, h, y = _spare(rows=3 * N), _spare(b, 3 * N), _spare(), _spare(rows=3 * N)
+        s, g = _spare(rows=4), _spare(rows=4)
+        ok = dict(rows=N, x=x.ptr, delta=delta.ptr, h=h.ptr, y=y.ptr, branch_scale=s.ptr, gate=g.ptr)
+        bad = [("h overlaps x", dict(h=x.ptr + 4)), ("h overlaps x", dict(x=x.ptr + 4 * D, h=x.ptr)),
+               ("y overlaps x", dict(y=x.ptr + 4 * (N * D - 1))), ("h overlaps y", dict(h=y.ptr)),
+               ("h overlaps y", dict(h=y.ptr + 4 * D)), ("h overlaps branch_scale", dict(branch_scale=h.ptr + 8)),
+               ("y overlaps gate", dict(gate=y.ptr + 4 * D)),
+               ("y overlaps post_scale", dict(post_scale=y.ptr + 4 * (N - 1) * D)),
+               ("y overlaps norm_scale", dict(norm_scale=y.ptr)), ("h overlaps y", dict(h=x.ptr, y=x.ptr))]
+        if types == "mixed":
+            bad += [("y overlaps delta", dict(y=delta.ptr)), ("h overlaps delta", dict(h=delta.ptr))]
+        for text, kw in bad:
+            with pytest.raises(_lib.MixMoEError, match=text):
+                r.forward(**dict(ok, **kw))
+        good = [dict(h=x.ptr), dict(y=x.ptr), dict(h=x.ptr, y=y.ptr), dict(x=x.ptr, h=x.ptr + 4 * N * D),
+                dict(delta=x.ptr) if types == "fp32" else {}, dict(post_scale=s.ptr, norm_scale=s.ptr, gate=s.ptr)]
+        if types == "fp32":
+            good += [dict(h=delta.ptr), dict(y=delta.ptr), dict(h=delta.ptr, y=x.ptr)]
+        for kw in good:
+            r.forward(**dict(ok, **kw))
+        r.synchronize()
+
+
+def test_overlaps_of_a_backward(gpu_lib):
+    with ResidualNorm(D, N, out_dtype="fp32", post_norm=True, gate="channel", gate_rows=4) as r, \
+            ResidualNorm(D, N, scale_dtype="bf16", gate="row", gate_rows=2) as rb:
+        h, delta, dh, dy, dx, dd = (_spare(rows=2 * N) for _ in range(6))
+        v = {k: _spare(rows=2) for k in ("post", "scale", "w", "gate", "dp", "ds", "dw", "dg")}
+        ok = dict(rows=N, h=h.ptr, delta=delta.ptr, dh=dh.ptr, dy=dy.ptr, dx=dx.ptr, d_delta=dd.ptr,
+                  post_scale=v["post"].ptr, branch_scale=v["scale"].ptr, norm_scale=v["w"].ptr,
+                  gate=v["gate"].ptr, d_post_scale=v["dp"].ptr, d_branch_scale=v["ds"].ptr,
+                  d_norm_scale=v["dw"].ptr, d_gate=v["dg"].ptr)
+        for text, kw in [
+                ("dx overlaps d_delta", dict(dx=dd.ptr)), ("dx overlaps dh", dict(dx=dh.ptr + 4)),
+                ("d_delta overlaps dy", dict(d_delta=dy.ptr + 4 * D)), ("dx overlaps h", dict(h=dx.ptr + 4 * D)),
+                ("d_delta overlaps gate", dict(d_delta=v["gate"].ptr)),
+                ("d_post_scale overlaps d_branch_scale", dict(d_post_scale=v["ds"].ptr)),
+                ("d_branch_scale overlaps post_scale", dict(d_branch_scale=v["post"].ptr)),
+                ("d_norm_scale overlaps branch_scale", dict(d_norm_scale=v["scale"].ptr)),
+                ("d_gate overlaps post_scale", dict(d_gate=v["post"].ptr)),
+                ("d_gate overlaps gate", dict(d_gate=v["gate"].ptr + 4 * D)),
+                ("d_norm_scale overlaps dy|d_norm_scale overlaps d", dict(d_norm_scale=dy.ptr))]:
+            with pytest.raises(_lib.MixMoEError, match=text):
+                r.backward(**dict(ok, **kw))
+        both = dict(rows=N, h=h.ptr, delta=delta.ptr, dh=dh.ptr, dy=dy.ptr, dx=dx.ptr, d_delta=dd.ptr,
+                    branch_scale=v["scale"].ptr, gate=v["gate"].ptr)
+        for text, kw in [("d_branch_scale overlaps branch_scale", dict(d_branch_scale=v["scale"].ptr)),
+                         ("d_gate overlaps gate", dict(d_gate=v["gate"].ptr))]:
+            with pytest.raises(_lib.MixMoEError, match=text):  # bf16 under fp32
+                rb.backward(**dict(both, **kw))
+        for kw in (dict(dx=dh.ptr), dict(d_delta=dy.ptr), dict(d_delta=delta.ptr, dx=h.ptr), dict(dh=dy.ptr),
+                   dict(d_delta=dh.ptr, dx=dy.ptr)):
+            r.backward(**dict(ok, **kw))
+        r.synchronize()
+
+
+@pytest.mark.parametrize("N,D,gate_rows", [(40, 64, 1), (40, 300, 7), (700, 64, 700), (9, 1030, 2)])
+def test_gradients_in_their_scales_places(gpu_lib, N, D, gate_rows):
+    """The scales' and the gate's gradients over the scales and the gate themselves."""
+    c = dict(gate="channel", gate_rows=gate_rows, sigmoid=True)
+    v = _case(N, N, D, **c)
+    want = run_backward(v, N, D, **c)
+    t = {k: Dev(v[k]) for k in ("h", "delta", "dh", "dy", "post_scale", "branch_scale", "norm_scale", "gate")}
+    with ResidualNorm(D, N, out_dtype="fp32", post_norm=True, gate="channel", gate_rows=gate_rows,
+                      gate_sigmoid=True) as r:
+        r.backward(N, dx=t["dh"].ptr, d_delta=t["dy"].ptr, d_post_scale=t["post_scale"].ptr,
+                   d_branch_scale=t["branch_scale"].ptr, d_gate=t["gate"].ptr,
+                   d_norm_scale=t["norm_scale"].ptr, **{k: d.ptr for k, d in t.items()})
+        r.synchronize()
+    for k, place in (("dx", "dh"), ("d_delta", "dy"), ("d_post", "post_scale"), ("d_scale", "branch_scale"),
+                     ("d_w", "norm_scale"), ("d_gate", "gate")):
+        assert np.array_equal(t[place].get(), want[k]), k
