@@ -173,7 +173,8 @@ class MoEBlockTrainer:
     (arch/moe.go:112-150), then ``moe_post_norm_scale`` with post_norm.  Matrices
     decay, vectors do not.  ``gate`` is None, "row" or "channel": values given to
     the forward for each group of gate_rows rows (a sequence: gate_rows=T).  All
-    calls but ``update`` are asynchronous on the op's stream; the stream is fp32."""
+    calls but ``update`` are asynchronous on the op's stream.  The residual stream
+    and all gradients are fp32, the gate's values are what the compute is in."""
 
     def __init__(self, spec: BlockSpec, B: int, T: int, D: int,
                  mlp_mult: float = DEFAULT_FFN_MULTIPLIER, block_scales: bool = False,
@@ -303,7 +304,9 @@ class MoEBlockTrainer:
         return self._read(self._g)
 
     def forward(self, x: int, out: int, gate: int = 0) -> None:
-        """out [N, D] fp32 (not x's buffer: the backward reads x) for x [N, D] fp32."""
+        """out [N, D] fp32 (not x's buffer: the backward reads x) for x [N, D] fp32.
+        gate [ceil(N / gate_rows), 1 or D] is bf16 under bf16 compute, else fp32;
+        the backward reads it again."""
         if x == out:
             raise ValueError("the block's training forward keeps x: out must be another buffer")
         if (gate != 0) != (self.gate is not None):
@@ -319,7 +322,8 @@ class MoEBlockTrainer:
 
     def backward(self, d_out: int, dx: int, d_gate: int = 0) -> None:
         """dx [N, D] (may be d_out) and the weights' gradients of the last forward, for
-        the loss's gradient d_out [N, D] at its output and the weighted aux loss."""
+        the loss's gradient d_out [N, D] at its output and the weighted aux loss.
+        d_gate, or 0, gets the gate's gradient in fp32."""
         if not self._x:
             raise _lib.MixMoEError("backward without a forward")
         self._ready = False

@@ -3,8 +3,8 @@ buffers that a program can come to."""
 import numpy as np
 import pytest
 
-from mixlab_amd import _lib
-from mixlab_amd.train import GradientSet, ResidualNorm
+from mixlab_amd import _lib, moe
+from mixlab_amd.train import GradientSet, MoEBlockTrainer, ResidualNorm
 from oracle import train as ot
 from tests.test_gpu_resnorm import _case, _col_c, _row_c, run_backward
 from tests.test_gpu_train_streams import Graph
@@ -275,3 +275,26 @@ def test_gradients_in_their_scales_places(gpu_lib, N, D, gate_rows):
     for k, place in (("dx", "dh"), ("d_delta", "dy"), ("d_post", "post_scale"), ("d_scale", "branch_scale"),
                      ("d_w", "norm_scale"), ("d_gate", "gate")):
         assert np.array_equal(t[place].get(), want[k]), k
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("gate", ["row", "channel"])
+def test_trainer_gates_on_the_device(gpu_lib, dtype, gate):
+    """A gate on the device in the compute's type gives what step_host gives for its
+    values in fp32; its gradient is fp32 in both."""
+    spec = moe.BlockSpec.from_dict({"type": "moe", "num_experts": 4, "top_k": 2})
+    B, T, width = 2, 15, 96
+    rng = np.random.default_rng(3)
+    x, d_out = (rng.standard_normal((B * T, width), dtype=np.float32) for _ in range(2))
+    g = rng.standard_normal((B, width) if gate == "channel" else (B, 1), dtype=np.float32)
+    with MoEBlockTrainer(spec, B, T, width, 1.0, post_norm=True, gate=gate, gate_rows=T,
+                         compute_dtype=dtype) as tr:
+        tr.set_weights([np.ones(m.shape) if len(m.shape) == 1 else 0.05 * rng.standard_normal(m.shape)
+                        for m in tr.metas])
+        want = tr.step_host(x, d_out, 0.0, g)
+        bx, bd, bo, bg, dg = Dev(x), Dev(d_out), Dev.out(x.shape), Dev(g, dtype), Dev.out(g.shape)
+        tr.forward(bx.ptr, bo.ptr, bg.ptr)
+        tr.backward(bd.ptr, bd.ptr, dg.ptr)
+        assert tr.update(0.0)
+        assert np.array_equal(bo.get(), want["out"]) and np.array_equal(bd.get(), want["dx"])
+        assert np.array_equal(dg.get(), want["d_gate"])
