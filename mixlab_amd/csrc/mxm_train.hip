@@ -558,6 +558,8 @@ int mxm_grads_adamw(int64_t h, double lr, double beta1, double beta2, double eps
     if (!((float)eps > 0.0f) || !std::isfinite(eps)) fail(GRADSET " eps must be finite and > 0");
     if (!(weight_decay >= 0.0) || !std::isfinite(weight_decay))
       fail(GRADSET " weight_decay must be finite and >= 0");
+    if (!std::isfinite((float)lr) || !std::isfinite((float)(lr * weight_decay)))
+      fail(GRADSET " lr and lr * weight_decay must be finite in fp32");
     if (!(max_norm >= 0.0) || !std::isfinite(max_norm))
       fail(GRADSET " max_norm must be finite and >= 0 (0: no clipping)");
     if (!step || reinterpret_cast<uintptr_t>(step) % 8 != 0)

@@ -298,3 +298,20 @@ def test_trainer_gates_on_the_device(gpu_lib, dtype, gate):
         assert tr.update(0.0)
         assert np.array_equal(bo.get(), want["out"]) and np.array_equal(bd.get(), want["dx"])
         assert np.array_equal(dg.get(), want["d_gate"])
+
+
+@pytest.mark.parametrize("kw", [dict(lr=1e39), dict(lr=1e30, weight_decay=1e30), dict(lr=1.0, weight_decay=1e39)])
+def test_rates_past_fp32(gpu_lib, kw):
+    """Finite rates that are infinite in the update's fp32 are refused: they would make
+    weights of zero gradient NaN."""
+    with GradientSet([4]) as s:
+        g, p, m, v = (Dev(np.zeros(4, np.float32)) for _ in range(4))
+        step = Dev(np.zeros(1, np.int64), "int64")
+        s.bind([g.ptr], params=[p.ptr], m=[m.ptr], v=[v.ptr])
+        args = dict(dict(dict(lr=1e-3, weight_decay=0.0), **kw), beta1=0.9, beta2=0.99, eps=1e-8, max_norm=1.0,
+                    step=step.ptr)
+        with pytest.raises(_lib.MixMoEError, match="fp32"):
+            s.adamw(**args)
+        s.adamw(**dict(args, lr=1e30, weight_decay=1.0))
+        s.synchronize()
+        assert step.get()[0] == 1 and not p.get().any()
