@@ -312,7 +312,7 @@ int mxm_moe_info(int64_t op, int64_t* info, int n);
  * them can be captured into a HIP graph on the handle's stream; the scalars
  * given by value (rows, lr, max_norm, ...) are then the captured ones.  A
  * handle's workspace is its own: two graphs captured from one handle must not
- * run at once.  None of this has a counterpart in the reference's bridge,
+ * run at once, and none runs after the handle's destruction.  None of this has a counterpart in the reference's bridge,
  * whose graph compiler fuses such work itself. */
 
 /* Residual norm: what stands between a block's branch and the next block.
@@ -322,7 +322,8 @@ int mxm_moe_info(int64_t op, int64_t* info, int n);
  *   y = norm_scale * h / sqrt(mean_d(h^2) + eps)    with MXM_RESNORM_NORM
  * (moe_scale and the residual Add of arch/moe.go:199-204, :164, and the RMSNorm
  * of gpu/ir.cpp:4949-4960, in one pass).  y is computed from h as it is kept,
- * i.e. after h's rounding to the stream's type; sums are in fp32. */
+ * i.e. after h's rounding to the stream's type; sums are in fp32, so a row's
+ * squares have to add up to less than 3.4e38. */
 #define MXM_RESNORM_BRANCH 1       /* h = x + ...; without it h is x itself */
 #define MXM_RESNORM_POST_NORM 2    /* the branch is normalised first */
 #define MXM_RESNORM_NORM 4         /* the sum is normalised: y */

@@ -11,9 +11,11 @@
 // Kernels with ODD 0 need D % 4 == 0 and tensors aligned to their vectors; the
 // others take the rest: the part's vector loads and stores need no more than an
 // element's alignment, and a row's last vector may be short.  134 M elements of
-// 1024 / 1030 / 1023 channels take 301 / 456 / 384 us forwards and 564 / 663 /
-// 628 backwards in fp32, 180 / 290 / 226 and 265 / 453 / 345 in bf16; such rows
-// share cache lines, so their loads stay in the caches' usual replacement.
+// 1024 / 1030 / 1023 channels take 312 / 458 / 384 us forwards and 571 / 658 /
+// 645 backwards in fp32, 180 / 290 / 227 and 265 / 459 / 342 in bf16; such rows
+// share cache lines, so their loads stay in the caches' usual replacement.  Just
+// past a shape's widths lanes idle as well: 65 channels 410 and 651 us in fp32,
+// 312 and 523 in bf16, 2049 channels 552 and 640, 332 and 590.
 #pragma once
 
 #include <type_traits>

@@ -2,8 +2,8 @@
 // with the gradients of the stream and the branch, column sums of the scales'
 // and the gate's gradients kept in registers over a chunk of rows, and a second
 // launch that joins the chunks in their order.  Bound by memory: 65,536 rows of
-// 2048 channels in fp32 565 us (3.22 GB over six streams at 5.7 TB/s; 656 us at a
-// large copy's rate), the join 4.6 of them.
+// 2048 channels in fp32 559 us (3.22 GB over six streams at 5.8 TB/s; 656 us at a
+// large copy's rate), the join 4.8 of them.
 #include <algorithm>
 
 #include "mxm_resnorm.h"
