@@ -342,8 +342,9 @@ int64_t mxm_resnorm_create(const int64_t* params, int n_params, float eps, int64
 int mxm_resnorm_destroy(int64_t h);
 
 /* h and y for rows <= maxRows rows (rows behind them are left as they were).
- * Scales may be NULL (ones).  h or y may be x or delta where the types agree; any
- * other overlap of an output with a tensor of the call is refused.
+ * Scales may be NULL (ones).  h or y may be x or delta where the types agree, or
+ * one buffer, which then holds y; any other overlap of an output with a tensor of
+ * the call is refused.
  * delta, h and gate are ignored without a branch or gate, y without a norm. */
 int mxm_resnorm_forward(int64_t handle, int64_t rows, const void* x, const void* delta,
                         const void* post_scale, const void* branch_scale, const void* gate,
@@ -352,9 +353,9 @@ int mxm_resnorm_forward(int64_t handle, int64_t rows, const void* x, const void*
 /* Gradients at the forward's h (x for a handle without a branch) and delta,
  * for upstream gradients dh and dy.  With a norm dh may be NULL (zeros), without
  * one dy is ignored and dx, which then equals dh, may be NULL.  dx or d_delta may
- * be any of h, delta, dh and dy where the types agree, and the gradient of an
- * fp32 scale or gate may take its place; any other overlap of an output is
- * refused.  The scales' and the gate's gradients are fp32 (overwritten, not added to; NULL:
+ * be any of h, delta, dh and dy where the types agree, or one buffer, which then
+ * holds d_delta, and the gradient of an fp32 scale or gate may take its place; any
+ * other overlap of an output is refused.  The scales' and the gate's gradients are fp32 (overwritten, not added to; NULL:
  * not computed), summed in a fixed order: equal inputs give equal bits. */
 int mxm_resnorm_backward(int64_t handle, int64_t rows, const void* h, const void* delta,
                          const void* post_scale, const void* branch_scale, const void* gate,

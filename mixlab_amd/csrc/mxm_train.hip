@@ -123,15 +123,18 @@ void check_pointer(const char* what, const char* name, const void* p, bool bf16,
     fail("%s %s is not aligned to its elements", what, name);
 }
 
+enum : unsigned { ROWS = 1, POST = 2, SCALE = 4, GATE = 8, NORM = 16 };
+
 // Where a call's tensors lie.  An output may be one of the inputs that it is
-// computed beside, element for element (`in_place`, a mask of kinds); every other
-// overlap of an output is refused.
+// computed beside, element for element (`in_place`, a mask of kinds), and rows of
+// results may take each other's place (the thread that stores both leaves the
+// later one); every other overlap of an output is refused.
 struct Tensors {
   struct One {
     const char* name;
     uintptr_t from, to;
     int item;
-    unsigned kind;      // of an input
+    unsigned kind;
     unsigned in_place;  // of an output: kinds of inputs
   };
   One all[14];
@@ -146,7 +149,7 @@ struct Tensors {
     add(name, p, elements, bf16, kind, 0);
   }
   void out(const char* name, const void* p, int64_t elements, bool bf16, unsigned in_place) {
-    add(name, p, elements, bf16, 0, in_place);
+    add(name, p, elements, bf16, in_place & ROWS, in_place);
   }
   void check(const char* what) const {
     for (int i = 0; i < n; ++i) {
@@ -161,8 +164,6 @@ struct Tensors {
     }
   }
 };
-enum : unsigned { ROWS = 1, POST = 2, SCALE = 4, GATE = 8, NORM = 16 };
-
 // The stream of `stream_of`, or a new one on the current device.
 std::shared_ptr<StreamRef> choose_stream(std::shared_ptr<StreamRef> shared) {
   if (shared) return shared;

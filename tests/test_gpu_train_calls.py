@@ -6,7 +6,7 @@ import pytest
 from mixlab_amd import _lib, moe
 from mixlab_amd.train import GradientSet, MoEBlockTrainer, ResidualNorm
 from oracle import train as ot
-from tests.test_gpu_resnorm import _case, _col_c, _row_c, run_backward
+from tests.test_gpu_resnorm import _case, _col_c, _handle, _row_c, run_backward, run_forward
 from tests.test_gpu_train_streams import Graph
 from tests.train_testutil import U32, Dev, as_kept, close
 
@@ -207,11 +207,11 @@ def test_overlaps_of_a_forward(gpu_lib, types):
         s, g = _spare(rows=4), _spare(rows=4)
         ok = dict(rows=N, x=x.ptr, delta=delta.ptr, h=h.ptr, y=y.ptr, branch_scale=s.ptr, gate=g.ptr)
         bad = [("h overlaps x", dict(h=x.ptr + 4)), ("h overlaps x", dict(x=x.ptr + 4 * D, h=x.ptr)),
-               ("y overlaps x", dict(y=x.ptr + 4 * (N * D - 1))), ("h overlaps y", dict(h=y.ptr)),
+               ("y overlaps x", dict(y=x.ptr + 4 * (N * D - 1))),
                ("h overlaps y", dict(h=y.ptr + 4 * D)), ("h overlaps branch_scale", dict(branch_scale=h.ptr + 8)),
                ("y overlaps gate", dict(gate=y.ptr + 4 * D)),
                ("y overlaps post_scale", dict(post_scale=y.ptr + 4 * (N - 1) * D)),
-               ("y overlaps norm_scale", dict(norm_scale=y.ptr)), ("h overlaps y", dict(h=x.ptr, y=x.ptr))]
+               ("y overlaps norm_scale", dict(norm_scale=y.ptr))]
         if types == "mixed":
             bad += [("y overlaps delta", dict(y=delta.ptr)), ("h overlaps delta", dict(h=delta.ptr))]
         for text, kw in bad:
@@ -236,7 +236,7 @@ def test_overlaps_of_a_backward(gpu_lib):
                   gate=v["gate"].ptr, d_post_scale=v["dp"].ptr, d_branch_scale=v["ds"].ptr,
                   d_norm_scale=v["dw"].ptr, d_gate=v["dg"].ptr)
         for text, kw in [
-                ("dx overlaps d_delta", dict(dx=dd.ptr)), ("dx overlaps dh", dict(dx=dh.ptr + 4)),
+                ("dx overlaps d_delta", dict(dx=dd.ptr + 4 * D)), ("dx overlaps dh", dict(dx=dh.ptr + 4)),
                 ("d_delta overlaps dy", dict(d_delta=dy.ptr + 4 * D)), ("dx overlaps h", dict(h=dx.ptr + 4 * D)),
                 ("d_delta overlaps gate", dict(d_delta=v["gate"].ptr)),
                 ("d_post_scale overlaps d_branch_scale", dict(d_post_scale=v["ds"].ptr)),
@@ -315,3 +315,29 @@ def test_rates_past_fp32(gpu_lib, kw):
         s.adamw(**dict(args, lr=1e30, weight_decay=1.0))
         s.synchronize()
         assert step.get()[0] == 1 and not p.get().any()
+
+
+@pytest.mark.parametrize("N,D", [(9, 64), (9, 301), (5, 1030), (3, 4100)])
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_results_that_are_not_wanted(gpu_lib, N, D, dtype):
+    """h in y's buffer, or dx in d_delta's: the later result is what is left."""
+    c = dict(stream=dtype, delta=dtype, out=dtype, grad=dtype)
+    v = _case(N, N, D, **c)
+    y = run_forward(v, N, D, **c)[1].get()
+    dd = run_backward(v, N, D, **c)["d_delta"]
+    t = {k: Dev(v[k], dtype) for k in ("x", "delta", "h", "dh", "dy")}
+    s = {k: Dev(v[k]) for k in ("post_scale", "branch_scale", "norm_scale")}
+    scales = {k: d.ptr for k, d in s.items()}
+    with _handle(N, D, **c) as r:
+        for x, place in ((t["x"], Dev.out((N, D), dtype)), (t["x"], t["x"])):
+            r.forward(N, x.ptr, t["delta"].ptr, place.ptr, place.ptr, **scales)
+            r.synchronize()
+            assert np.array_equal(place.get(), y)
+        place = Dev.out((N, D), dtype)
+        r.backward(N, t["h"].ptr, t["delta"].ptr, t["dh"].ptr, t["dy"].ptr, place.ptr, place.ptr, **scales)
+        r.synchronize()
+        assert np.array_equal(place.get(), dd)
+    if dtype == "fp32":
+        with _handle(N, D, out="bf16") as r:
+            with pytest.raises(_lib.MixMoEError, match="h overlaps y"):
+                r.forward(N, t["x"].ptr, t["delta"].ptr, place.ptr, place.ptr, **scales)
