@@ -299,7 +299,7 @@ int mxm_moe_info(int64_t op, int64_t* info, int n);
 /* ---- around the op's training step ----
  *
  * The handles below run on a stream of their own, or on that of another live
- * handle (`stream_of`: an op, a residual norm or a gradient set; 0: a new
+ * handle (`stream_of`: an op or any of these; 0: a new
  * stream on the current device).  Handles that share a stream run in call
  * order without any wait on the host, so a block's norms, its op and its
  * optimizer go on one stream; work on another stream is ordered by the caller
@@ -399,6 +399,69 @@ int mxm_grads_clip(int64_t h, double max_norm, float* norm);
 int mxm_grads_adamw(int64_t h, double lr, double beta1, double beta2, double eps,
                     double weight_decay, double max_norm, int64_t* step, float* norm,
                     int32_t* skipped);
+
+/* ---- the vocabulary's two ends of a training step ----
+ *
+ * Handles as the residual norm's and the gradient set's above: shared streams,
+ * asynchronous calls without allocation or waiting (all can be captured), contiguous
+ * device tensors aligned to their elements, a workspace that is the handle's own.
+ * An output may not overlap any other tensor of its call.  Every sum is taken in
+ * an order that the call's sizes and whole-number inputs decide: equal inputs give
+ * equal bits. */
+#define MXM_VOCAB_MAX 16777216
+
+/* Token embedding: out[n] = scale * table[tokens[n]], n < rows, for a table [V, D];
+ * a token outside [0, V) gives a row of zeros.
+ * params = [V, D, maxRows, tableDtype, outDtype, gradDtype, tableGradDtype, flags];
+ * dtypes (MXM_DTYPE_F32 or MXM_DTYPE_BF16) are those of table, out, d_out and
+ * d_table.  D is at most MXM_RESNORM_MAX_D, V at most MXM_VOCAB_MAX.  Returns a
+ * handle, 0 on failure. */
+#define MXM_EMBED_BACKWARD 1 /* the handle also runs backward (holds its workspace) */
+int64_t mxm_embed_create(const int64_t* params, int n_params, float scale, int64_t stream_of);
+int mxm_embed_destroy(int64_t h);
+
+/* tokens [rows] int32, rows <= maxRows; rows of out behind them are left as they were. */
+int mxm_embed_forward(int64_t h, int64_t rows, const int32_t* tokens, const void* table, void* out);
+
+/* d_table[v] = scale * sum of d_out[n] over the n with tokens[n] = v, for every v
+ * (zeros where there is none); with accumulate the sums are added to d_table, and
+ * the rows of tokens that do not occur are left as they were (a table tied to a
+ * token loss: its dw first).  Sums in fp32, one rounding.  d_out's rows of tokens
+ * outside [0, V) are not read. */
+int mxm_embed_backward(int64_t h, int64_t rows, const int32_t* tokens, const void* d_out,
+                       void* d_table, int accumulate);
+
+/* Token loss: softmax cross entropy of hidden rows x [rows, D] against a table
+ * weight [V, D] (the embedding's, where they are tied), without keeping the logits
+ * of more than a piece of the rows.  A row takes part where its target is in [0, V)
+ * and its weight is not 0; of any other row nothing else is read, and its loss, lse
+ * and dx are 0.
+ *   l = x . weight[v]                      with a softcap: softcap * tanh(l / softcap)
+ *   lse[n] = log sum_v exp(l[v]),  loss[n] = lse[n] - l[targets[n]]
+ *   total = sum of row_weights[n] * loss[n]    MXM_XENT_MEAN: / sum of row_weights[n]
+ * over the rows that take part (0 where none does).
+ * params = [V, D, maxRows, dtype, dxDtype, dwDtype, flags]; dtype is that of x and
+ * weight.  Under fp32 the products are as exact as fp32 ones; under bf16 they are
+ * exact products summed in fp32, and the backward rounds the logits' gradient to
+ * bf16 before the products with it.  softcap 0: none.  Returns a handle, 0 on
+ * failure. */
+#define MXM_XENT_MEAN 1
+#define MXM_XENT_BACKWARD 2 /* the handle also runs backward (holds its workspace) */
+int64_t mxm_xent_create(const int64_t* params, int n_params, float softcap, int64_t stream_of);
+int mxm_xent_destroy(int64_t h);
+
+/* targets [rows] int32, row_weights [rows] fp32 or NULL (ones); loss and lse [rows]
+ * and total [1] fp32, each NULL where it is not wanted, not all of them. */
+int mxm_xent_forward(int64_t h, int64_t rows, const void* x, const void* weight,
+                     const int32_t* targets, const float* row_weights, float* loss, float* lse,
+                     float* total);
+
+/* The forward and the gradients of d_total * total: dx [rows, D] and dw [V, D]
+ * (overwritten), either NULL where it is not wanted.  loss, lse and total may all be
+ * NULL.  It runs the forward on what it is given: no mxm_xent_forward before it. */
+int mxm_xent_backward(int64_t h, int64_t rows, const void* x, const void* weight,
+                      const int32_t* targets, const float* row_weights, float d_total, float* loss,
+                      float* lse, float* total, void* dx, void* dw);
 
 /* The hipStream_t that a handle (an op's too) runs on, to order other work with
  * it or to capture its calls. */

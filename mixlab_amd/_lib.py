@@ -38,6 +38,10 @@ MXM_RESNORM_MAX_D = 16384
 MXM_GATE_NONE = 0
 MXM_GATE_ROW = 1
 MXM_GATE_CHANNEL = 2
+MXM_VOCAB_MAX = 16777216
+MXM_EMBED_BACKWARD = 1
+MXM_XENT_MEAN = 1
+MXM_XENT_BACKWARD = 2
 MXM_NUM_STAGES = 6
 MXM_NOALLOC_MAX_BYTES = 64 << 20
 STAGE_NAMES = ("router", "scan", "scatter", "gemm_up", "gemm_down", "combine")
@@ -98,6 +102,16 @@ SIGNATURES = {
     "mxm_grads_norm": (ctypes.c_int, [ctypes.c_int64, _VP]),
     "mxm_grads_clip": (ctypes.c_int, [ctypes.c_int64, ctypes.c_double, _VP]),
     "mxm_grads_adamw": (ctypes.c_int, [ctypes.c_int64] + [ctypes.c_double] * 6 + [_VP] * 3),
+    "mxm_embed_create": (ctypes.c_int64, [_I64P, ctypes.c_int, ctypes.c_float, ctypes.c_int64]),
+    "mxm_embed_destroy": (ctypes.c_int, [ctypes.c_int64]),
+    "mxm_embed_forward": (ctypes.c_int, [ctypes.c_int64, ctypes.c_int64] + [_VP] * 3),
+    "mxm_embed_backward": (ctypes.c_int, [ctypes.c_int64, ctypes.c_int64] + [_VP] * 3
+                           + [ctypes.c_int]),
+    "mxm_xent_create": (ctypes.c_int64, [_I64P, ctypes.c_int, ctypes.c_float, ctypes.c_int64]),
+    "mxm_xent_destroy": (ctypes.c_int, [ctypes.c_int64]),
+    "mxm_xent_forward": (ctypes.c_int, [ctypes.c_int64, ctypes.c_int64] + [_VP] * 7),
+    "mxm_xent_backward": (ctypes.c_int, [ctypes.c_int64, ctypes.c_int64] + [_VP] * 4
+                          + [ctypes.c_float] + [_VP] * 5),
     "mxm_stream": (ctypes.c_int, [ctypes.c_int64, ctypes.POINTER(_VP)]),
     "mxm_synchronize": (ctypes.c_int, [ctypes.c_int64]),
 }

@@ -33,6 +33,9 @@ SOURCES = [
     "mxm_resnorm_bw.hip",
     "mxm_optim.hip",
     "mxm_train.hip",
+    "mxm_embed.hip",
+    "mxm_xent.hip",
+    "mxm_vocab.hip",
     "mxm_abi.hip",
 ]
 ARCH = os.environ.get("MIXMOE_OFFLOAD_ARCH", "gfx950")

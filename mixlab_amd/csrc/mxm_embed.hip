@@ -1,0 +1,352 @@
+// The token embedding (mxm_vocab.h): lookup with scaling, and its gradient by
+// sorted tokens.
+#include <algorithm>
+
+#include "mxm_vocab.h"
+
+namespace {
+
+typedef unsigned int u32x4_t __attribute__((ext_vector_type(4)));
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
+
+// U elements at p as fp32, U = 8 from 16-byte aligned rows, else 1.
+template <int U>
+__device__ __forceinline__ void load_unit(const void* p, bool bf16, int64_t at, float (&v)[U]) {
+  if constexpr (U == 8) {
+    if (bf16) {
+      const u32x4_t q = *reinterpret_cast<const u32x4_t*>(static_cast<const uint16_t*>(p) + at);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v[2 * i] = mxm_u2f(q[i] << 16);
+        v[2 * i + 1] = mxm_u2f(q[i] & 0xffff0000u);
+      }
+    } else {
+      const f32x4_t* q = reinterpret_cast<const f32x4_t*>(static_cast<const float*>(p) + at);
+      const f32x4_t a = q[0], b = q[1];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = a[i], v[4 + i] = b[i];
+    }
+  } else {
+    v[0] = bf16 ? mxm_bf2f(static_cast<const uint16_t*>(p)[at]) : static_cast<const float*>(p)[at];
+  }
+}
+template <int U>
+__device__ __forceinline__ void store_unit(void* p, bool bf16, int64_t at, const float (&v)[U]) {
+  if constexpr (U == 8) {
+    if (bf16) {
+      u32x4_t q;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) q[i] = mxm_pack_bf2_fast(v[2 * i], v[2 * i + 1]);
+      *reinterpret_cast<u32x4_t*>(static_cast<uint16_t*>(p) + at) = q;
+    } else {
+      f32x4_t a, b;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) a[i] = v[i], b[i] = v[4 + i];
+      f32x4_t* q = reinterpret_cast<f32x4_t*>(static_cast<float*>(p) + at);
+      q[0] = a;
+      q[1] = b;
+    }
+  } else if (bf16) {
+    static_cast<uint16_t*>(p)[at] = mxm_f2bf_fast(v[0]);
+  } else {
+    static_cast<float*>(p)[at] = v[0];
+  }
+}
+
+constexpr int NT = 256;
+
+// A row per T threads.
+template <int U>
+__global__ __launch_bounds__(NT) void embed_kernel(EmbedArgs a, int T) {
+  const int per = NT / T, sub = threadIdx.x / T, t = threadIdx.x % T;
+  for (int64_t n = (int64_t)blockIdx.x * per + sub; n < a.rows; n += (int64_t)gridDim.x * per) {
+    const int v = a.tokens[n];
+    const bool in = v >= 0 && v < a.V;
+    for (int d = t * U; d < a.D; d += T * U) {
+      float e[U];
+#pragma unroll
+      for (int i = 0; i < U; ++i) e[i] = 0.0f;
+      if (in) load_unit<U>(a.table, a.table_bf16, (int64_t)v * a.D + d, e);
+#pragma unroll
+      for (int i = 0; i < U; ++i) e[i] = in ? e[i] * a.scale : 0.0f;
+      store_unit<U>(a.out, a.out_bf16, n * a.D + d, e);
+    }
+  }
+}
+
+// ---- backward: the places sorted by token ----
+//
+// Workgroup o owns the tokens [o * span, (o + 1) * span).  Its waves each walk
+// their own stretch of the tokens twice: counting, per wave, how often each owned
+// token occurs (and how many tokens are smaller than the first owned one, which is
+// where the owned ones start), then writing the owned places in order.
+constexpr int SORT_WAVES = 16;
+constexpr int SORT_SPAN = 512;  // most tokens a workgroup owns
+constexpr int SORT_AHEAD = 4;   // tokens in flight per lane
+
+// LDS written by lanes of this wave is read by other lanes of it afterwards.
+__device__ __forceinline__ void wave_lds_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+__global__ __launch_bounds__(64 * SORT_WAVES) void embed_sort_kernel(EmbedArgs a, int span) {
+  __shared__ int cnt[SORT_WAVES][SORT_SPAN];
+  __shared__ int tot[SORT_SPAN];
+  __shared__ int lower[SORT_WAVES];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lo = blockIdx.x * span, own = min(span, a.V - lo);
+  for (int i = threadIdx.x; i < SORT_WAVES * SORT_SPAN; i += blockDim.x) (&cnt[0][0])[i] = 0;
+  __syncthreads();
+  // stretches of whole groups of 64
+  const int64_t groups = (a.rows + 63) / 64, each = (groups + SORT_WAVES - 1) / SORT_WAVES;
+  const int64_t from = min((int64_t)wave * each * 64, a.rows);
+  const int64_t to = min(from + each * 64, a.rows);
+  int below = 0;
+  for (int64_t n = from; n < to; n += 64 * SORT_AHEAD) {
+    int v[SORT_AHEAD];
+#pragma unroll
+    for (int q = 0; q < SORT_AHEAD; ++q) {
+      const int64_t i = n + 64 * q + lane;
+      v[q] = i < to ? a.tokens[i] : -1;
+    }
+#pragma unroll
+    for (int q = 0; q < SORT_AHEAD; ++q) {
+      below += v[q] >= 0 && v[q] < lo;
+      const unsigned b = (unsigned)(v[q] - lo);
+      if (v[q] >= lo && b < (unsigned)own) atomicAdd(&cnt[wave][b], 1);
+    }
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) below += __shfl_xor(below, o);
+  if (lane == 0) lower[wave] = below;
+  __syncthreads();
+  // where each wave's first place of each token goes
+  for (int b = threadIdx.x; b < own; b += blockDim.x) {
+    int s = 0;
+#pragma unroll
+    for (int w = 0; w < SORT_WAVES; ++w) {
+      const int c = cnt[w][b];
+      cnt[w][b] = s;
+      s += c;
+    }
+    tot[b] = s;
+  }
+  __syncthreads();
+  if (wave == 0) {
+    int base = 0;
+#pragma unroll
+    for (int w = 0; w < SORT_WAVES; ++w) base += lower[w];
+    for (int b0 = 0; b0 < own; b0 += 64) {
+      const int b = b0 + lane, c = b < own ? tot[b] : 0;
+      int x = c;
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const int y = __shfl_up(x, o);
+        if (lane >= o) x += y;
+      }
+      if (b < own) {
+        tot[b] = base + x - c;
+        a.starts[lo + b] = base + x - c;
+      }
+      base += __shfl(x, 63);
+    }
+    if (lane == 0 && lo + own == a.V) a.starts[a.V] = base;
+  }
+  __syncthreads();
+  for (int64_t n = from; n < to; n += 64 * SORT_AHEAD) {
+    int v[SORT_AHEAD];
+#pragma unroll
+    for (int q = 0; q < SORT_AHEAD; ++q) {
+      const int64_t i = n + 64 * q + lane;
+      v[q] = i < to ? a.tokens[i] : -1;
+    }
+#pragma unroll
+    for (int q = 0; q < SORT_AHEAD; ++q) {
+      const bool mine = v[q] >= lo && v[q] - lo < own;
+      const int b = v[q] - lo;
+      unsigned long long left = __ballot(mine);
+      while (left) {  // one token that occurs in this group at a time
+        const int lead = __ffsll(left) - 1;
+        const int tok = __shfl(b, lead);
+        const bool same = mine && b == tok;
+        const unsigned long long all = __ballot(same);
+        const int at = tot[tok] + cnt[wave][tok];
+        if (same) {
+          const int rank = __popcll(all & ((1ull << lane) - 1));
+          a.sorted[at + rank] = make_int2((int)(n + 64 * q + lane), v[q]);
+        }
+        wave_lds_sync();  // every lane has read the count
+        if (lane == lead) cnt[wave][tok] += __popcll(all);
+        wave_lds_sync();
+        left &= ~all;
+      }
+    }
+  }
+}
+
+// Sorted places [c * C, (c + 1) * C) per T threads: each run of one token that lies
+// within them to the table, the first and last run's sums to part where they go on
+// outside.  Workgroups behind the chunks': zeros for the tokens that occur nowhere.
+template <int U>
+__device__ __forceinline__ void put_row(const EmbedArgs& a, int v, int d, float (&s)[U]) {
+#pragma unroll
+  for (int i = 0; i < U; ++i) s[i] *= a.scale;
+  const int64_t at = (int64_t)v * a.D + d;
+  if (a.accumulate) {
+    float o[U];
+    load_unit<U>(a.d_table, a.dtable_bf16, at, o);
+#pragma unroll
+    for (int i = 0; i < U; ++i) s[i] += o[i];
+  }
+  store_unit<U>(a.d_table, a.dtable_bf16, at, s);
+}
+
+template <int U>
+__device__ __forceinline__ void sum_chunk(const EmbedArgs& a, int T, int t, int C, int64_t c, int64_t all) {
+  const int64_t from = c * C, to = min(from + C, all);
+  if (from >= to) return;
+  for (int d = t * U; d < a.D; d += T * U) {
+    float s[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i) s[i] = 0.0f;
+    int v = a.sorted[from].y;
+    bool first = true;  // the chunk's first run
+    for (int64_t p = from; p < to; ++p) {
+      const int2 e = a.sorted[p];
+      if (e.y != v) {
+        if (first && a.starts[v] < from) {
+          float* q = a.part + c * 2 * a.D + d;
+#pragma unroll
+          for (int i = 0; i < U; ++i) q[i] = s[i];
+        } else {
+          put_row<U>(a, v, d, s);
+        }
+        first = false;
+        v = e.y;
+#pragma unroll
+        for (int i = 0; i < U; ++i) s[i] = 0.0f;
+      }
+      float g[U];
+      load_unit<U>(a.d_out, a.grad_bf16, (int64_t)e.x * a.D + d, g);
+#pragma unroll
+      for (int i = 0; i < U; ++i) s[i] += g[i];
+    }
+    const bool before = first && a.starts[v] < from, after = a.starts[v + 1] > to;
+    if (before || after) {
+      float* q = a.part + (c * 2 + (before ? 0 : 1)) * a.D + d;
+#pragma unroll
+      for (int i = 0; i < U; ++i) q[i] = s[i];
+    } else {
+      put_row<U>(a, v, d, s);
+    }
+  }
+}
+
+template <int U>
+__global__ __launch_bounds__(NT) void embed_sum_kernel(EmbedArgs a, int T, int C, int64_t chunks,
+                                                       int64_t items) {
+  const int per = NT / T, sub = threadIdx.x / T, t = threadIdx.x % T;
+  const int64_t all = a.starts[a.V];
+  for (int64_t i = (int64_t)blockIdx.x * per + sub; i < items; i += (int64_t)gridDim.x * per) {
+    if (i < chunks) {
+      sum_chunk<U>(a, T, t, C, i, all);
+    } else {
+      const int64_t v = i - chunks;
+      if (a.starts[v] != a.starts[v + 1]) continue;
+      float z[U];
+#pragma unroll
+      for (int k = 0; k < U; ++k) z[k] = 0.0f;
+      for (int d = t * U; d < a.D; d += T * U) store_unit<U>(a.d_table, a.dtable_bf16, v * a.D + d, z);
+    }
+  }
+}
+
+// The run that starts in chunk c and goes on behind it: its sums in order.
+template <int U>
+__device__ __forceinline__ void join_chunk(const EmbedArgs& a, int T, int t, int C, int64_t c, int64_t all) {
+  if ((c + 1) * C >= all) return;
+  const int v = a.sorted[(c + 1) * C - 1].y;
+  const int64_t from = a.starts[v], to = a.starts[v + 1];
+  if (from < c * C || to <= (c + 1) * C) return;
+  const int64_t last = (to - 1) / C;
+  for (int d = t * U; d < a.D; d += T * U) {
+    float s[U];
+    const float* q = a.part + (c * 2 + 1) * a.D + d;
+#pragma unroll
+    for (int i = 0; i < U; ++i) s[i] = q[i];
+    for (int64_t k = c + 1; k <= last; ++k) {
+      q = a.part + k * 2 * a.D + d;
+#pragma unroll
+      for (int i = 0; i < U; ++i) s[i] += q[i];
+    }
+    put_row<U>(a, v, d, s);
+  }
+}
+
+template <int U>
+__global__ __launch_bounds__(NT) void embed_join_kernel(EmbedArgs a, int T, int C, int64_t chunks) {
+  const int per = NT / T, sub = threadIdx.x / T, t = threadIdx.x % T;
+  const int64_t all = a.starts[a.V];
+  for (int64_t c = (int64_t)blockIdx.x * per + sub; c < chunks; c += (int64_t)gridDim.x * per)
+    join_chunk<U>(a, T, t, C, c, all);
+}
+
+bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// Threads that walk one row of `units`: the least power of two that covers it, at
+// most a workgroup.
+int threads_per_row(int64_t units) {
+  int t = 8;
+  while (t < NT && t < units) t *= 2;
+  return t;
+}
+
+// Sorted places per chunk.
+constexpr int64_t LONG_BATCH = 32768;
+int chunk_rows(int64_t rows) { return rows >= LONG_BATCH ? 32 : 8; }
+
+unsigned grid_of(int64_t items, int per, int n_cu) {
+  return (unsigned)std::min<int64_t>((items + per - 1) / per, (int64_t)n_cu * 64);
+}
+
+}  // namespace
+
+int64_t mxm_embed_max_chunks(int64_t max_rows) {
+  return std::max((std::min(max_rows, LONG_BATCH - 1) + 7) / 8, (max_rows + 31) / 32);
+}
+
+void mxm_launch_embed(const EmbedArgs& a, hipStream_t s) {
+  if (a.rows == 0) return;
+  const bool wide = a.D % 8 == 0 && aligned(a.table) && aligned(a.out);
+  const int T = threads_per_row(wide ? a.D / 8 : a.D);
+  const unsigned grid = grid_of(a.rows, NT / T, a.n_cu);
+  if (wide)
+    embed_kernel<8><<<grid, NT, 0, s>>>(a, T);
+  else
+    embed_kernel<1><<<grid, NT, 0, s>>>(a, T);
+}
+
+void mxm_launch_embed_bw(const EmbedArgs& a, hipStream_t s) {
+  const bool wide = a.D % 8 == 0 && aligned(a.d_out) && aligned(a.d_table);
+  const int T = threads_per_row(wide ? a.D / 8 : a.D), per = NT / T;
+  const int span = std::min(SORT_SPAN, std::max(16, (a.V + a.n_cu - 1) / a.n_cu));
+  embed_sort_kernel<<<(a.V + span - 1) / span, 64 * SORT_WAVES, 0, s>>>(a, span);
+  const int C = chunk_rows(a.rows);
+  const int64_t chunks = (a.rows + C - 1) / C, items = chunks + (a.accumulate ? 0 : a.V);
+  if (items > 0) {
+    const unsigned grid = grid_of(items, per, a.n_cu);
+    if (wide)
+      embed_sum_kernel<8><<<grid, NT, 0, s>>>(a, T, C, chunks, items);
+    else
+      embed_sum_kernel<1><<<grid, NT, 0, s>>>(a, T, C, chunks, items);
+  }
+  if (chunks > 1) {
+    const unsigned grid = grid_of(chunks, per, a.n_cu);
+    if (wide)
+      embed_join_kernel<8><<<grid, NT, 0, s>>>(a, T, C, chunks);
+    else
+      embed_join_kernel<1><<<grid, NT, 0, s>>>(a, T, C, chunks);
+  }
+}

@@ -5,22 +5,13 @@
 // is touched.
 #include <algorithm>
 #include <cmath>
-#include <map>
-#include <mutex>
 #include <vector>
 
 #include "../../include/mixmoe.h"
-#include "mxm_host.h"
+#include "mxm_handles.h"
 #include "mxm_train.h"
 
 namespace {
-
-struct TrainHandle {
-  std::shared_ptr<StreamRef> stream_ref;
-  int n_cu = 256;
-  virtual ~TrainHandle() = default;
-  hipStream_t stream() const { return stream_ref->stream; }
-};
 
 struct ResNorm : TrainHandle {
   ResNormArgs base{};  // what every call shares
@@ -47,81 +38,6 @@ struct GradSet : TrainHandle {
     if (stream_ref) (void)hipStreamSynchronize(stream());
   }
 };
-
-std::mutex g_train_mu;
-std::map<int64_t, std::shared_ptr<TrainHandle>> g_train;
-
-std::shared_ptr<TrainHandle> find(int64_t h) {
-  std::lock_guard<std::mutex> lk(g_train_mu);
-  const auto it = g_train.find(h);
-  return it == g_train.end() ? nullptr : it->second;
-}
-template <class T>
-std::shared_ptr<T> get(int64_t h) {
-  return std::dynamic_pointer_cast<T>(find(h));
-}
-
-std::shared_ptr<StreamRef> stream_of_handle(int64_t h) {
-  if (auto s = mxm_op_stream(h)) return s;
-  const auto t = find(h);
-  return t ? t->stream_ref : nullptr;
-}
-
-// Makes `dev` current for a call and puts the caller's device back.
-struct DeviceGuard {
-  int prev = -1;
-  bool moved = false;
-  explicit DeviceGuard(int dev) {
-    HIPCK(hipGetDevice(&prev));
-    if (prev != dev) {
-      HIPCK(hipSetDevice(dev));
-      moved = true;
-    }
-  }
-  ~DeviceGuard() {
-    if (moved) (void)hipSetDevice(prev);
-  }
-};
-
-int64_t keep(std::shared_ptr<TrainHandle> t) {
-  const int64_t h = mxm_new_handle();
-  std::lock_guard<std::mutex> lk(g_train_mu);
-  g_train[h] = std::move(t);
-  return h;
-}
-
-template <class T>
-int destroy(int64_t h, const char* what) {
-  return fenced([&] {
-    std::shared_ptr<TrainHandle> victim;
-    {
-      std::lock_guard<std::mutex> lk(g_train_mu);
-      const auto it = g_train.find(h);
-      if (it == g_train.end() || !dynamic_cast<T*>(it->second.get())) {
-        g_last_error = std::string(what) + " invalid handle";
-        return MXM_ERR_OP;
-      }
-      victim = std::move(it->second);
-      g_train.erase(it);
-    }
-    return MXM_OK;
-  });
-}
-
-#define HANDLE_OR_RETURN(T, var, h, what)          \
-  const std::shared_ptr<T> var = get<T>(h);        \
-  if (!var) {                                      \
-    g_last_error = what " invalid handle";         \
-    return MXM_ERR_OP;                             \
-  }
-
-bool float_dtype(int64_t t) { return t == MXM_DTYPE_F32 || t == MXM_DTYPE_BF16; }
-
-void check_pointer(const char* what, const char* name, const void* p, bool bf16, bool required) {
-  if (!p && required) fail("%s %s must be non-NULL", what, name);
-  if (reinterpret_cast<uintptr_t>(p) % (bf16 ? 2 : 4) != 0)
-    fail("%s %s is not aligned to its elements", what, name);
-}
 
 enum : unsigned { ROWS = 1, POST = 2, SCALE = 4, GATE = 8, NORM = 16 };
 
@@ -164,29 +80,9 @@ struct Tensors {
     }
   }
 };
-// The stream of `stream_of`, or a new one on the current device.
-std::shared_ptr<StreamRef> choose_stream(std::shared_ptr<StreamRef> shared) {
-  if (shared) return shared;
-  int dev = 0;
-  HIPCK(hipGetDevice(&dev));
-  return std::make_shared<StreamRef>(dev);
-}
-
-std::shared_ptr<StreamRef> shared_stream(const char* what, int64_t stream_of) {
-  if (stream_of == 0) return nullptr;
-  auto s = stream_of_handle(stream_of);
-  if (!s) fail("%s stream_of %lld is not a live handle", what, (long long)stream_of);
-  return s;
-}
 
 int64_t gate_elements(const ResNormArgs& a, int64_t rows) {
   return a.gate ? (rows + a.gate_rows - 1) / a.gate_rows * (a.gate == 2 ? a.D : 1) : 0;
-}
-
-int cu_count(int device) {
-  int n = 0;
-  HIPCK(hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, device));
-  return n;
 }
 
 #define RESNORM "RESIDUAL_NORM"
@@ -226,11 +122,7 @@ int64_t mxm_resnorm_create(const int64_t* params, int n_params, float eps, int64
     auto shared = shared_stream(RESNORM, stream_of);
 
     auto r = std::make_shared<ResNorm>();
-    const DeviceGuard guard(shared ? shared->device : [] {
-      int dev = 0;
-      HIPCK(hipGetDevice(&dev));
-      return dev;
-    }());
+    const DeviceGuard guard(device_of(shared));
     r->stream_ref = choose_stream(shared);
     r->n_cu = cu_count(r->stream_ref->device);
     r->max_rows = rows;
@@ -406,11 +298,7 @@ int64_t mxm_grads_create(const int64_t* sizes, const int32_t* dtypes, const floa
     auto shared = shared_stream(GRADSET, stream_of);
 
     auto g = std::make_shared<GradSet>();
-    const DeviceGuard guard(shared ? shared->device : [] {
-      int dev = 0;
-      HIPCK(hipGetDevice(&dev));
-      return dev;
-    }());
+    const DeviceGuard guard(device_of(shared));
     g->stream_ref = choose_stream(shared);
     g->n_cu = cu_count(g->stream_ref->device);
     const int64_t per = mxm_grad_chunk_elems(total, g->n_cu);
