@@ -408,7 +408,7 @@ int mxm_grads_adamw(int64_t h, double lr, double beta1, double beta2, double eps
  * An output may not overlap any other tensor of its call.  Every sum is taken in
  * an order that the call's sizes and whole-number inputs decide: equal inputs give
  * equal bits. */
-#define MXM_VOCAB_MAX 16777216
+#define MXM_VOCAB_MAX 4194304
 
 /* Token embedding: out[n] = scale * table[tokens[n]], n < rows, for a table [V, D];
  * a token outside [0, V) gives a row of zeros.

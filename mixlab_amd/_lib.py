@@ -38,7 +38,7 @@ MXM_RESNORM_MAX_D = 16384
 MXM_GATE_NONE = 0
 MXM_GATE_ROW = 1
 MXM_GATE_CHANNEL = 2
-MXM_VOCAB_MAX = 16777216
+MXM_VOCAB_MAX = 4194304
 MXM_EMBED_BACKWARD = 1
 MXM_XENT_MEAN = 1
 MXM_XENT_BACKWARD = 2

@@ -35,6 +35,7 @@ SOURCES = [
     "mxm_train.hip",
     "mxm_embed.hip",
     "mxm_xent.hip",
+    "mxm_xent_gemm.hip",
     "mxm_vocab.hip",
     "mxm_abi.hip",
 ]

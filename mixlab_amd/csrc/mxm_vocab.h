@@ -45,8 +45,27 @@ int64_t mxm_embed_max_chunks(int64_t max_rows);
 //   total = sum_n w_n loss_n             (mean: / sum_n w_n)
 //   g_n = d_total w_n                    (mean: / sum_n w_n)
 //   dz = g (softmax(l) - [v = t]) (1 - (l / cap)^2),  dx = dz W,  dW = dz^T x
-// Rows that take part are gathered (in order); the logits of a piece of them
-// exist at a time.
+// The rows that take part are packed (in order) into x_pack, zero-padded to whole
+// 64-wide stages; under fp32 as three bf16 planes hi, mid and lo whose sum is the
+// value, and a product of two values as the six products of planes that matter.
+// Then, for a piece of these rows at a time:
+//   product 1 (mxm_xent_gemm.hip): logits of a tile of vocabulary x rows in the
+//     accumulators; of each row and block of the vocabulary the sum over v != t of
+//     2^(l log2 e - ref) with a whole-number ref of the block; backwards also each
+//     summand (times 1 - (l / cap)^2), relative to that ref;
+//   join (mxm_xent.hip): each row's loss and the factors of its gradient;
+//   finish: the summands to dz, in place (fp32: to three planes);
+//   product 2: dx = dz W;  product 3: dW (+)= dz^T x.
+struct XentScalars {
+  double weight_sum;        // of the rows that take part
+  int32_t rows;             // that take part
+};
+struct XentRow {            // of a row that takes part
+  float ref;                // M: the summands' common exponent
+  float scale;              // g / sum of all 2^(l log2 e - M)
+  float at_target;          // dz of the target
+  int32_t target;
+};
 struct XentArgs {
   int64_t rows;
   int V, D;
@@ -63,16 +82,40 @@ struct XentArgs {
   void *dx, *dw;            // [rows, D], [V, D], or null
   bool backward;
   // workspace
-  int32_t* map;             // [rows] the rows that take part
-  struct XentScalars* scalars;
+  int Dp, Vp;               // D and V rounded up to whole stages
+  int planes;               // 1 (bf16) or 3
+  int32_t* slot;            // [rows] a row's place among those that take part, or -1
+  int32_t* map;             // [rows] and back
+  XentScalars* scalars;
   float* nll;               // [rows] loss of the rows that take part
-  float* logits;            // [piece_rows][V]
-  float* dw32;              // [V][D] or null: dw is fp32 itself
-  int64_t piece_rows;
+  float* at_target;         // [rows] their target's logit
+  XentRow* row;             // [rows]
+  uint16_t* x_pack;         // [planes][x_rows][Dp]
+  int64_t x_rows;
+  uint16_t* w_pack;         // [planes][V][Dp], unused where weight is read in place
+  bool w_direct;            // weight itself: bf16 rows of whole 16 bytes
+  float2* stat;             // [blocks][stat_ld]: sum, ref
+  void* summands;           // [piece_rows][Vp]: fp16 (bf16) or fp32
+  uint16_t* dz;             // [planes][piece_rows][Vp]: the summands' place under bf16
+  float* partial;           // tiles of products that are split along their sums
+  float* dw32;              // [V][D] sums of the pieces before the last, or null: dw itself
+  const uint16_t* zeros;    // 4 KB of zeros
+  int64_t piece_rows, stat_ld;
   int n_cu;
 };
-struct XentScalars {
-  double weight_sum;        // of the rows that take part
-  int32_t rows;             // that take part
-};
+// Bytes of partial, for handles that run backward.
+int64_t mxm_xent_partial_bytes(int n_cu);
+// Most blocks of stat times rows, for pieces of `rows`.
+int64_t mxm_xent_stats(int64_t rows, int V);
+// Columns of the vocabulary per block of stat, for a piece of `rows` rows.
+int mxm_xent_block(int64_t rows);
+void mxm_launch_xent_logits(const XentArgs& a, int64_t r0, int64_t rows, hipStream_t s);
+void mxm_launch_xent_dx(const XentArgs& a, int64_t r0, int64_t rows, hipStream_t s);
+void mxm_launch_xent_dw(const XentArgs& a, int64_t r0, int64_t rows, bool last, hipStream_t s);
 void mxm_launch_xent(const XentArgs& a, hipStream_t s);
+
+// Rows of the piece that starts at row r0 of those that take part.
+__device__ __forceinline__ int mxm_xent_rows(const XentArgs& a, int64_t r0) {
+  const int64_t left = a.scalars->rows - r0;
+  return left <= 0 ? 0 : (int)(left < a.piece_rows ? left : a.piece_rows);
+}

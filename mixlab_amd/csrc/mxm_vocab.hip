@@ -26,7 +26,7 @@ struct Xent : TrainHandle {
   XentArgs base{};
   int64_t max_rows = 0;
   bool backward = false;
-  DevBuf map, scalars, nll, logits, dw32;
+  DevBuf slot, map, scalars, nll, at_target, row, x_pack, w_pack, stat, summands, dz, partial, dw32, zeros;
   ~Xent() override {
     if (stream_ref) (void)hipStreamSynchronize(stream());
   }
@@ -69,9 +69,9 @@ void check_rows(const char* what, int64_t rows, int64_t max_rows) {
 }
 int item(bool bf16) { return bf16 ? 2 : 4; }
 
-// Bytes of logits that a loss's workspace holds at most (but for tables of which a
-// few rows' logits are more).
-constexpr int64_t XENT_LOGIT_BYTES = (int64_t)2 << 30;
+// Bytes that a loss's workspace holds of a piece of the rows at most (but for tables
+// of which a tile's rows take more).
+constexpr int64_t XENT_PIECE_BYTES = (int64_t)2 << 30;
 
 #define EMBED "TOKEN_EMBEDDING"
 #define XENT "TOKEN_LOSS"
@@ -250,19 +250,48 @@ int64_t mxm_xent_create(const int64_t* params, int n_params, float softcap, int6
     a.bf16 = params[3] == MXM_DTYPE_BF16;
     a.dx_bf16 = params[4] == MXM_DTYPE_BF16;
     a.dw_bf16 = params[5] == MXM_DTYPE_BF16;
-    int64_t bytes = XENT_LOGIT_BYTES;
+    const auto up = [](int64_t n) { return (n + 63) / 64 * 64; };
+    a.Dp = (int)up(D);
+    a.Vp = (int)up(V);
+    a.planes = a.bf16 ? 1 : 3;
+    a.x_rows = std::max<int64_t>(rows, 1);
+    // a row's share of the workspace: its blocks' sums, and backwards its summands
+    // (and under fp32 their gradient's planes)
+    int64_t bytes = XENT_PIECE_BYTES;
     if (const char* env = std::getenv("MXM_XENT_PIECE_BYTES")) bytes = std::max(0ll, std::atoll(env));
-    a.piece_rows = std::max<int64_t>(64, std::min((rows + 63) / 64, bytes / 4 / V / 64) * 64);
+    const int64_t row_bytes = (V + 127) / 128 * 8 + (x->backward ? a.Vp * (int64_t)(a.bf16 ? 2 : 10) : 0);
+    a.piece_rows = std::max<int64_t>(256, std::min(up(rows), bytes / row_bytes / 256 * 256));
+    if (rows < a.piece_rows) a.piece_rows = std::max<int64_t>(64, up(rows));
+    x->slot.alloc((size_t)rows * 4);
     x->map.alloc((size_t)rows * 4);
     x->scalars.alloc(sizeof(XentScalars));
     x->nll.alloc((size_t)rows * 4);
-    x->logits.alloc((size_t)a.piece_rows * (size_t)V * 4);
+    x->at_target.alloc((size_t)rows * 4);
+    x->x_pack.alloc((size_t)a.x_rows * a.Dp * 2 * a.planes);
+    x->w_pack.alloc((size_t)V * a.Dp * 2 * a.planes);
+    x->stat.alloc((size_t)mxm_xent_stats(a.piece_rows, a.V) * sizeof(float2));
+    x->zeros.alloc(4096);
+    HIPCK(hipMemsetAsync(x->zeros.p, 0, 4096, x->stream()));
+    a.slot = x->slot.as<int32_t>();
     a.map = x->map.as<int32_t>();
     a.scalars = x->scalars.as<XentScalars>();
     a.nll = x->nll.as<float>();
-    a.logits = x->logits.as<float>();
-    if (x->backward && a.dw_bf16 && rows > a.piece_rows) {
-      x->dw32.alloc((size_t)V * (size_t)D * 4);
+    a.at_target = x->at_target.as<float>();
+    a.x_pack = x->x_pack.as<uint16_t>();
+    a.w_pack = x->w_pack.as<uint16_t>();
+    a.stat = x->stat.as<float2>();
+    a.zeros = x->zeros.as<uint16_t>();
+    if (x->backward) {
+      const size_t cells = (size_t)a.piece_rows * (size_t)a.Vp;
+      x->row.alloc((size_t)rows * sizeof(XentRow));
+      x->summands.alloc(cells * (a.bf16 ? 2 : 4));
+      if (!a.bf16) x->dz.alloc(cells * 6);
+      x->partial.alloc((size_t)mxm_xent_partial_bytes(a.n_cu));
+      if (a.dw_bf16 && rows > a.piece_rows) x->dw32.alloc((size_t)V * (size_t)D * 4);
+      a.row = x->row.as<XentRow>();
+      a.summands = x->summands.p;
+      a.dz = a.bf16 ? x->summands.as<uint16_t>() : x->dz.as<uint16_t>();
+      a.partial = x->partial.as<float>();
       a.dw32 = x->dw32.as<float>();
     }
     handle = keep(std::move(x));

@@ -1,19 +1,15 @@
-// The token loss (mxm_vocab.h): softmax cross entropy of hidden rows against the
-// vocabulary's table.
+// The token loss (mxm_vocab.h) around its three products: which rows take part,
+// the operands' planes, the rows' losses and the logits' gradient.
 #include <algorithm>
 
 #include "mxm_vocab.h"
 
 namespace {
 
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+
 __device__ __forceinline__ float load1(const void* p, bool bf16, int64_t at) {
   return bf16 ? mxm_bf2f(static_cast<const uint16_t*>(p)[at]) : static_cast<const float*>(p)[at];
-}
-__device__ __forceinline__ void store1(void* p, bool bf16, int64_t at, float v) {
-  if (bf16)
-    static_cast<uint16_t*>(p)[at] = mxm_f2bf(v);
-  else
-    static_cast<float*>(p)[at] = v;
 }
 
 __device__ __forceinline__ bool takes_part(const XentArgs& a, int64_t n, float& w) {
@@ -35,10 +31,6 @@ __global__ __launch_bounds__(PLAN_NT) void xent_plan_kernel(XentArgs a) {
     const int64_t n = n0 + threadIdx.x;
     float w = 0.0f;
     const bool in = n < a.rows && takes_part(a, n, w);
-    if (n < a.rows && !in) {
-      if (a.loss) a.loss[n] = 0.0f;
-      if (a.lse) a.lse[n] = 0.0f;
-    }
     const unsigned long long m = __ballot(in);
     if (lane == 0) wave_count[wave] = __popcll(m);
     __syncthreads();
@@ -47,10 +39,15 @@ __global__ __launch_bounds__(PLAN_NT) void xent_plan_kernel(XentArgs a) {
       before += i < wave ? wave_count[i] : 0;
       all += wave_count[i];
     }
+    const int64_t at = base + before + __popcll(m & ((1ull << lane) - 1));
     if (in) {
-      a.map[base + before + __popcll(m & ((1ull << lane) - 1))] = (int32_t)n;
+      a.map[at] = (int32_t)n;
       sum += (double)w;
+    } else if (n < a.rows) {
+      if (a.loss) a.loss[n] = 0.0f;
+      if (a.lse) a.lse[n] = 0.0f;
     }
+    if (n < a.rows) a.slot[n] = in ? (int32_t)at : -1;
     base += all;
     __syncthreads();
   }
@@ -66,175 +63,163 @@ __global__ __launch_bounds__(PLAN_NT) void xent_plan_kernel(XentArgs a) {
   }
 }
 
-// A 64 x 64 tile of sum_k A(m, k) B(k, n), 16 x 16 threads of 4 x 4.
-template <class FA, class FB>
-__device__ __forceinline__ void tile64(int K, FA A, FB B, float (&c)[4][4]) {
-  __shared__ float sa[16][65], sb[16][65];
-  const int t = threadIdx.x, tm = t / 16, tn = t % 16;
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) c[i][j] = 0.0f;
-  for (int k0 = 0; k0 < K; k0 += 16) {
-    for (int i = t; i < 1024; i += 256) {
-      sa[i % 16][i / 16] = k0 + i % 16 < K ? A(i / 16, k0 + i % 16) : 0.0f;
-      sb[i / 64][i % 64] = k0 + i / 64 < K ? B(k0 + i / 64, i % 64) : 0.0f;
+// v as hi + mid + lo, each a bf16: 24 bits, all of v's.  The differences are exact.
+// Infinities become the largest bf16 (an infinite plane times another operand's
+// mid plane, of any sign or zero, would make a NaN of every product).
+__device__ __forceinline__ void planes3(float v, uint16_t& hi, uint16_t& mid, uint16_t& lo) {
+  const float c = v != v ? v : fminf(fmaxf(v, -3.3895313892515355e38f), 3.3895313892515355e38f);
+  hi = mxm_f2bf_fast(c);
+  const float r = c - mxm_bf2f(hi);
+  mid = mxm_f2bf_fast(r);
+  lo = mxm_f2bf_fast(r - mxm_bf2f(mid));
+}
+
+constexpr int NT = 256;
+
+// Row `src` of x or weight to row `to` of its pack of `rows` rows, zeros behind D.
+__device__ __forceinline__ void pack_row(const XentArgs& a, const void* p, int64_t src, uint16_t* pack,
+                                         int64_t rows, int64_t to, int t, int T) {
+  for (int d = t; d < a.Dp; d += T) {
+    const int64_t at = to * a.Dp + d;
+    if (a.planes == 1) {
+      pack[at] = d < a.D ? static_cast<const uint16_t*>(p)[src * a.D + d] : (uint16_t)0;
+    } else {
+      uint16_t hi = 0, mid = 0, lo = 0;
+      if (d < a.D) planes3(static_cast<const float*>(p)[src * a.D + d], hi, mid, lo);
+      const int64_t plane = rows * a.Dp;
+      pack[at] = hi;
+      pack[at + plane] = mid;
+      pack[at + 2 * plane] = lo;
     }
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < 16; ++k) {
-      float av[4], bv[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) av[i] = sa[k][tm * 4 + i], bv[i] = sb[k][tn * 4 + i];
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) c[i][j] = fmaf(av[i], bv[j], c[i][j]);
-    }
-    __syncthreads();
   }
 }
 
-// The rows of the piece that starts at row r0.
-__device__ __forceinline__ int piece_rows(const XentArgs& a, int64_t r0) {
-  const int64_t left = a.scalars->rows - r0;
-  return left <= 0 ? 0 : (int)(left < a.piece_rows ? left : a.piece_rows);
-}
-
-__global__ __launch_bounds__(256) void xent_logits_kernel(XentArgs a, int64_t r0) {
-  const int rows = piece_rows(a, r0), tm = threadIdx.x / 16, tn = threadIdx.x % 16;
-  const int n0 = blockIdx.x * 64;
-  for (int m0 = blockIdx.y * 64; m0 < rows; m0 += gridDim.y * 64) {
-    float c[4][4];
-    tile64(
-        a.D,
-        [&](int m, int k) {
-          return m0 + m < rows ? load1(a.x, a.bf16, (int64_t)a.map[r0 + m0 + m] * a.D + k) : 0.0f;
-        },
-        [&](int k, int n) {
-          return n0 + n < a.V ? load1(a.weight, a.bf16, (int64_t)(n0 + n) * a.D + k) : 0.0f;
-        },
-        c);
-    for (int i = 0; i < 4; ++i)
-      for (int j = 0; j < 4; ++j) {
-        const int m = m0 + tm * 4 + i, n = n0 + tn * 4 + j;
-        if (m < rows && n < a.V) {
-          float z = c[i][j];
-          if (a.softcap > 0.0f) z = a.softcap * tanhf(z / a.softcap);
-          a.logits[(int64_t)m * a.V + n] = z;
-        }
+// x's rows that take part to their places, and dx's others to zeros.
+__global__ __launch_bounds__(NT) void xent_pack_x_kernel(XentArgs a) {
+  const int lane = threadIdx.x & 63;
+  for (int64_t n = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); n < a.rows; n += (int64_t)gridDim.x * 4) {
+    const int to = a.slot[n];
+    if (to >= 0) {
+      pack_row(a, a.x, n, a.x_pack, a.x_rows, to, lane, 64);
+    } else if (a.dx) {
+      for (int d = lane; d < a.D; d += 64) {
+        if (a.dx_bf16)
+          static_cast<uint16_t*>(a.dx)[n * a.D + d] = 0;
+        else
+          static_cast<float*>(a.dx)[n * a.D + d] = 0.0f;
       }
+    }
   }
 }
 
-__device__ __forceinline__ float block_reduce(float v, bool max_of, float* lds) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    const float u = __shfl_xor(v, o);
-    v = max_of ? fmaxf(v, u) : v + u;
+__global__ __launch_bounds__(NT) void xent_pack_w_kernel(XentArgs a) {
+  const int lane = threadIdx.x & 63;
+  for (int64_t v = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); v < a.V; v += (int64_t)gridDim.x * 4)
+    pack_row(a, a.weight, v, a.w_pack, a.V, v, lane, 64);
+}
+
+// 16 rows by 16 threads: each row's blocks joined.
+constexpr int JOIN_ROWS = 16;
+__global__ __launch_bounds__(NT) void xent_join_kernel(XentArgs a, int64_t r0, int blocks) {
+  __shared__ float red[2][16][JOIN_ROWS];
+  const int rows = mxm_xent_rows(a, r0);
+  const int m = blockIdx.x * JOIN_ROWS + (threadIdx.x & 15), part = threadIdx.x >> 4;
+  if (blockIdx.x * JOIN_ROWS >= rows) return;
+  const bool in = m < rows;
+  float top = -__builtin_inff(), sum = 0.0f;
+  for (int b = part; in && b < blocks; b += 16) {
+    const float2 e = a.stat[(int64_t)b * a.stat_ld + m];
+    const float up = fmaxf(top, e.y);
+    // (ref and top agree where both are infinite: no difference to take)
+    sum = sum * (top == up ? 1.0f : __builtin_amdgcn_exp2f(top - up)) +
+          e.x * (e.y == up ? 1.0f : __builtin_amdgcn_exp2f(e.y - up));
+    top = up;
   }
-  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+  red[0][part][threadIdx.x & 15] = top;
+  red[1][part][threadIdx.x & 15] = sum;
   __syncthreads();
-  v = lds[0];
-  for (int i = 1; i < 4; ++i) v = max_of ? fmaxf(v, lds[i]) : v + lds[i];
-  __syncthreads();
-  return v;
-}
-
-// A row's loss, and its logits' gradient in their place.
-__global__ __launch_bounds__(256) void xent_row_kernel(XentArgs a, int64_t r0) {
-  __shared__ float lds[4];
-  const int rows = piece_rows(a, r0);
-  for (int m = blockIdx.x; m < rows; m += gridDim.x) {
-    float* l = a.logits + (int64_t)m * a.V;
-    const int64_t n = a.map[r0 + m];
-    const int t = a.targets[n];
-    const float lt = l[t];
-    float top = -__builtin_inff();
-    for (int v = threadIdx.x; v < a.V; v += 256)
-      if (v != t) top = fmaxf(top, l[v]);
-    top = fmaxf(block_reduce(top, true, lds), lt);
-    float s = 0.0f;
-    for (int v = threadIdx.x; v < a.V; v += 256)
-      if (v != t) s += expf(l[v] - top);
-    s = block_reduce(s, false, lds);
-    const float et = expf(lt - top), whole = s + et;
-    const float loss = lt == top ? log1pf(s) : logf(whole) + (top - lt);
-    if (threadIdx.x == 0) {
-      a.nll[r0 + m] = loss;
-      if (a.loss) a.loss[n] = loss;
-      if (a.lse) a.lse[n] = lt == top ? log1pf(s) + lt : logf(whole) + top;
+  if (part != 0 || !in) return;
+  for (int p = 1; p < 16; ++p) {
+    const float t = red[0][p][m & 15], s = red[1][p][m & 15], up = fmaxf(top, t);
+    sum = sum * (top == up ? 1.0f : __builtin_amdgcn_exp2f(top - up)) +
+          s * (t == up ? 1.0f : __builtin_amdgcn_exp2f(t - up));
+    top = up;
+  }
+  // the others' sum is sum * 2^top, the target's exponential 2^(top - d)
+  const float lt = a.at_target[r0 + m], d = fmaf(-lt, LOG2E, top);
+  const float et = __builtin_amdgcn_exp2f(-d), whole = sum + et;
+  // (next to the target's probability of one the loss keeps its digits)
+  const bool near = d <= 60.0f;
+  const float over = logf(whole);
+  const float loss = near ? log1pf(sum * __builtin_amdgcn_exp2f(d)) : d * LN2 + over;
+  const int64_t n = a.map[r0 + m];
+  a.nll[r0 + m] = loss;
+  if (a.loss) a.loss[n] = loss;
+  if (a.lse) a.lse[n] = near ? lt + loss : top * LN2 + over;
+  if (a.backward) {
+    const double w = a.row_weights ? (double)a.row_weights[n] : 1.0;
+    const float g = (float)((double)a.d_total * w / (a.mean ? a.scalars->weight_sum : 1.0));
+    XentRow r;
+    r.ref = top;
+    r.scale = g / whole;
+    float slope = 1.0f;
+    if (a.softcap > 0.0f) {
+      const float u = lt / a.softcap;
+      slope = 1.0f - u * u;
     }
-    if (a.backward) {
-      const float w = a.row_weights ? a.row_weights[n] : 1.0f;
-      const float g = (float)((double)a.d_total * w / (a.mean ? a.scalars->weight_sum : 1.0));
-      for (int v = threadIdx.x; v < a.V; v += 256) {
-        const float z = l[v];
-        float d = v == t ? -s / whole : expf(z - top) / whole;
-        d *= g;
-        if (a.softcap > 0.0f) {
-          const float u = z / a.softcap;
-          d *= 1.0f - u * u;
-        }
-        l[v] = d;
-      }
-    }
+    r.at_target = -g * (sum / whole) * slope;
+    r.target = a.targets[n];
+    a.row[r0 + m] = r;
   }
 }
 
-__global__ __launch_bounds__(256) void xent_dx_kernel(XentArgs a, int64_t r0) {
-  const int rows = piece_rows(a, r0), tm = threadIdx.x / 16, tn = threadIdx.x % 16;
-  const int d0 = blockIdx.x * 64;
-  for (int m0 = blockIdx.y * 64; m0 < rows; m0 += gridDim.y * 64) {
-    float c[4][4];
-    tile64(
-        a.V, [&](int m, int k) { return m0 + m < rows ? a.logits[(int64_t)(m0 + m) * a.V + k] : 0.0f; },
-        [&](int k, int n) {
-          return d0 + n < a.D ? load1(a.weight, a.bf16, (int64_t)k * a.D + d0 + n) : 0.0f;
-        },
-        c);
-    for (int i = 0; i < 4; ++i)
-      for (int j = 0; j < 4; ++j) {
-        const int m = m0 + tm * 4 + i, d = d0 + tn * 4 + j;
-        if (m < rows && d < a.D)
-          store1(a.dx, a.dx_bf16, (int64_t)a.map[r0 + m] * a.D + d, c[i][j]);
+// The summands of a piece to dz, 8 of a row per thread.
+typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+typedef unsigned int u32x4_t __attribute__((ext_vector_type(4)));
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
+template <int PLANES>
+__global__ __launch_bounds__(NT) void xent_finish_kernel(XentArgs a, int64_t r0, int block) {
+  const int rows = mxm_xent_rows(a, r0), units = a.Vp / 8;
+  for (int m = blockIdx.y; m < rows; m += gridDim.y) {
+    const XentRow r = a.row[r0 + m];
+    for (int u = blockIdx.x * NT + threadIdx.x; u < units; u += gridDim.x * NT) {
+      const int v = u * 8;
+      // (the last units may lie in padding behind the last block)
+      const float ref = v < a.V ? a.stat[(int64_t)(v / block) * a.stat_ld + m].y : r.ref;
+      const float f = r.scale * (ref == r.ref ? 1.0f : __builtin_amdgcn_exp2f(ref - r.ref));
+      float e[8];
+      const int64_t at = (int64_t)m * a.Vp + v;
+      if constexpr (PLANES == 1) {
+        const f16x8_t h = *reinterpret_cast<const f16x8_t*>(static_cast<const uint16_t*>(a.summands) + at);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) e[i] = (float)h[i] * f;
+      } else {
+        const f32x4_t* q = reinterpret_cast<const f32x4_t*>(static_cast<const float*>(a.summands) + at);
+        const f32x4_t lo = q[0], hi = q[1];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) e[i] = lo[i] * f, e[4 + i] = hi[i] * f;
       }
-  }
-}
-
-__global__ __launch_bounds__(256) void xent_dw_kernel(XentArgs a, int64_t r0, bool last) {
-  const int rows = piece_rows(a, r0), tm = threadIdx.x / 16, tn = threadIdx.x % 16;
-  const int d0 = blockIdx.x * 64;
-  for (int v0 = blockIdx.y * 64; v0 < a.V; v0 += gridDim.y * 64) {
-    float c[4][4];
-    tile64(
-        rows, [&](int m, int k) { return v0 + m < a.V ? a.logits[(int64_t)k * a.V + v0 + m] : 0.0f; },
-        [&](int k, int n) {
-          return d0 + n < a.D ? load1(a.x, a.bf16, (int64_t)a.map[r0 + k] * a.D + d0 + n) : 0.0f;
-        },
-        c);
-    float* acc = a.dw_bf16 ? a.dw32 : static_cast<float*>(a.dw);
-    for (int i = 0; i < 4; ++i)
-      for (int j = 0; j < 4; ++j) {
-        const int v = v0 + tm * 4 + i, d = d0 + tn * 4 + j;
-        if (v < a.V && d < a.D) {
-          const int64_t at = (int64_t)v * a.D + d;
-          const float s = r0 > 0 ? acc[at] + c[i][j] : c[i][j];
-          if (last)
-            store1(a.dw, a.dw_bf16, at, s);
-          else
-            acc[at] = s;
+      const int t = r.target - v;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) e[i] = i == t ? r.at_target : (v + i < a.V ? e[i] : 0.0f);
+      if constexpr (PLANES == 1) {
+        u32x4_t o;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i] = mxm_pack_bf2_fast(e[2 * i], e[2 * i + 1]);
+        *reinterpret_cast<u32x4_t*>(a.dz + at) = o;
+      } else {
+        uint16_t p[3][8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) planes3(e[i], p[0][i], p[1][i], p[2][i]);
+#pragma unroll
+        for (int k = 0; k < 3; ++k) {
+          u32x4_t o;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[i] = p[k][2 * i] | (uint32_t)p[k][2 * i + 1] << 16;
+          *reinterpret_cast<u32x4_t*>(a.dz + (int64_t)k * a.piece_rows * a.Vp + at) = o;
         }
       }
-  }
-}
-
-// Zeros in dx for the rows that take no part.
-__global__ __launch_bounds__(256) void xent_zero_kernel(XentArgs a) {
-  for (int64_t n = blockIdx.x; n < a.rows; n += gridDim.x) {
-    float w;
-    if (takes_part(a, n, w)) continue;
-    for (int d = threadIdx.x; d < a.D; d += 256) store1(a.dx, a.dx_bf16, n * a.D + d, 0.0f);
+    }
   }
 }
 
@@ -257,19 +242,35 @@ __global__ __launch_bounds__(PLAN_NT) void xent_total_kernel(XentArgs a) {
 
 }  // namespace
 
-void mxm_launch_xent(const XentArgs& a, hipStream_t s) {
+void mxm_launch_xent(const XentArgs& a0, hipStream_t s) {
+  XentArgs a = a0;
+  a.w_direct = a.bf16 && a.D % 8 == 0 && (reinterpret_cast<uintptr_t>(a.weight) & 15) == 0;
+  const auto rows_grid = [&](int64_t n) { return (unsigned)std::min<int64_t>((n + 3) / 4, (int64_t)a.n_cu * 16); };
   xent_plan_kernel<<<1, PLAN_NT, 0, s>>>(a);
+  if (a.rows > 0) {
+    xent_pack_x_kernel<<<rows_grid(a.rows), NT, 0, s>>>(a);
+    if (!a.w_direct) xent_pack_w_kernel<<<rows_grid(a.V), NT, 0, s>>>(a);
+  }
   const int64_t pieces = std::max<int64_t>(1, (a.rows + a.piece_rows - 1) / a.piece_rows);
-  const auto tiles = [](int64_t n, int64_t most) { return (unsigned)std::min((n + 63) / 64, most); };
   for (int64_t p = 0; p < pieces; ++p) {
     const int64_t r0 = p * a.piece_rows, rows = std::min(a.rows - r0, a.piece_rows);
     if (rows > 0) {
-      xent_logits_kernel<<<dim3(tiles(a.V, 1 << 20), tiles(rows, 64)), 256, 0, s>>>(a, r0);
-      xent_row_kernel<<<(unsigned)std::min<int64_t>(rows, 8192), 256, 0, s>>>(a, r0);
+      const int block = mxm_xent_block(rows);
+      a.stat_ld = rows;
+      mxm_launch_xent_logits(a, r0, rows, s);
+      xent_join_kernel<<<(unsigned)((rows + JOIN_ROWS - 1) / JOIN_ROWS), NT, 0, s>>>(
+          a, r0, (a.V + block - 1) / block);
+      if (a.backward) {
+        const unsigned gx = (unsigned)std::min((a.Vp / 8 + NT - 1) / NT, 64);
+        const dim3 grid(gx, (unsigned)std::min<int64_t>(rows, std::max(1u, (unsigned)a.n_cu * 32 / gx)));
+        if (a.planes == 1)
+          xent_finish_kernel<1><<<grid, NT, 0, s>>>(a, r0, block);
+        else
+          xent_finish_kernel<3><<<grid, NT, 0, s>>>(a, r0, block);
+      }
+      if (a.dx) mxm_launch_xent_dx(a, r0, rows, s);
     }
-    if (rows > 0 && a.dx) xent_dx_kernel<<<dim3(tiles(a.D, 1024), tiles(rows, 4096)), 256, 0, s>>>(a, r0);
-    if (a.dw) xent_dw_kernel<<<dim3(tiles(a.D, 1024), tiles(a.V, 4096)), 256, 0, s>>>(a, r0, p == pieces - 1);
+    if (a.dw) mxm_launch_xent_dw(a, r0, rows, p == pieces - 1, s);
   }
-  if (a.dx && a.rows > 0) xent_zero_kernel<<<(unsigned)std::min<int64_t>(a.rows, 8192), 256, 0, s>>>(a);
   if (a.total) xent_total_kernel<<<1, PLAN_NT, 0, s>>>(a);
 }

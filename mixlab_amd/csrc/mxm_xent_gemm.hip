@@ -1,0 +1,703 @@
+// The token loss's three products on bf16 MFMA (gfx950, v_mfma_f32_32x32x16_bf16).
+//
+//   C[m][n] = sum over pairs of planes and k of A(m, k) B(n, k)
+//   logits:  m a vocabulary entry, n a row;  A = weight,        B = x
+//   dx:      m a channel,          n a row;  A = weight (k out), B = dz
+//   dw:      m a channel, n an entry;        A = x (k out),      B = dz (k out)
+// An operand is either k-inner (a row holds consecutive k of one m or n) or k-out
+// (a row holds one k, consecutive m or n); dz and weight are read both ways, so
+// nothing is stored transposed.  Register r of lane l holds C[(r / 4) * 8 + (l / 32)
+// * 4 + r % 4][l % 32] of a 32 x 32 MFMA tile.  With the vocabulary along m a lane
+// owns one row's logits: the softmax's sums over a block of the vocabulary stay in
+// its registers but for one exchange between the wave's halves.  With the channels
+// along m a lane owns consecutive channels of one output row and stores them as
+// vectors.
+//
+// Tiles move global -> LDS with global_load_lds_dwordx4 into a ring of NS stages of
+// 64 k.  k-inner tiles come out by ds_read_b128 (16-byte chunks swizzled by the row),
+// k-out ones by the transposing ds_read_b64_tr_b16: within 16 lanes, lane 4r + q
+// supplies the address of row r, columns 4q..4q+3 of a 4 x 16 block and lane i
+// receives column i (chunks swizzled by 4 * (k % 4)).  The fragments of the next
+// 16-wide k step are read between the MFMAs of the current one, the next stage's
+// loads go out over its first two.
+//
+// fp32 operands are three bf16 planes hi, mid, lo; of the nine products of planes the
+// six of at least 2^-16 relative are summed, the small ones first: what is left out is
+// below 2^-23 of |A| |B|.
+//
+// The grid is persistent; each XCD (workgroup L runs on XCD L % 8) takes an eighth of
+// the tile list, in groups of GN n-tiles by all m-tiles.  Products with few tiles and
+// a long sum are split along k; the splits' tiles go to scratch in fp32 and are added
+// in order by a second launch.
+#include <algorithm>
+
+#include "mxm_lanes.h"
+#include "mxm_vocab.h"
+
+namespace {
+
+typedef __bf16 bf16x4_t __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
+typedef float f32x16_t __attribute__((ext_vector_type(16)));
+typedef unsigned int u32x2_t __attribute__((ext_vector_type(2)));
+typedef unsigned int u32x4_t __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) bf16x4_t* lds_bf16x4_p;
+
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr int BK = 64;  // k per stage
+constexpr int GN = 8;   // n-tiles per scheduling group
+
+// global_load_lds_dwordx4: lane l's 16 bytes land at LDS `lds` + 16 l.  Inline asm,
+// so that the compiler's tracking of LDS DMA does not drain the ring; the waits are
+// explicit.  M0 holds the LDS base.
+__device__ __forceinline__ void dma16(const void* g, const void* lds) {
+  const unsigned base = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)lds);
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off"
+               :
+               : "v"(g), "s"(base)
+               : "memory", "m0");
+}
+// From a uniform 64-bit base plus the lane's 32-bit byte offset.
+__device__ __forceinline__ void dma16s(const void* base, unsigned off_bytes, const void* lds) {
+  const unsigned lb = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)lds);
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
+               :
+               : "v"(off_bytes), "s"(base), "s"(lb)
+               : "memory", "m0");
+}
+// At most N of this thread's loads in flight, its LDS reads done, then the barrier.
+template <int N>
+__device__ __forceinline__ void stage_barrier() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(N) : "memory");
+}
+
+// BM x BN per workgroup of WM x WN waves, each (BM / WM) x (BN / WN).
+template <int BM_, int BN_, int WM_, int WN_, int NS_, int WPS_>
+struct Tile {
+  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, NS = NS_, WPS = WPS_;
+  static constexpr int NW = WM * WN, NT = 64 * NW;
+  static constexpr int TM = BM / WM / 32, TN = BN / WN / 32;
+  static constexpr int A_BYTES = BM * BK * 2, B_BYTES = BN * BK * 2, BUF = A_BYTES + B_BYTES;
+};
+using Big = Tile<256, 256, 2, 4, 2, 2>;     // one workgroup per CU, 128 KB of LDS
+using Small = Tile<128, 128, 2, 2, 2, 2>;   // two per CU, 64 KB each
+using Few = Tile<128, 32, 4, 1, 4, 2>;      // few rows: a stream of the table, 80 KB
+
+// One operand: `rows` of m (n) that exist, `k` of its reduction; beyond them k-inner
+// rows repeat the last one (for outputs that are not stored), k beyond come from zeros.
+struct Operand {
+  const uint16_t* p;
+  int64_t plane;  // elements between planes
+  int ld;         // elements between rows
+  int rows, k;
+};
+struct Product {
+  Operand a, b;
+  int nk;          // stages of 64 k
+  int pairs;       // pairs of planes
+  uint32_t amap, bmap;  // their planes, two bits each
+  const uint16_t* zeros;
+};
+
+// The loads of one operand's W x 64 (k-inner) or 64 x W (k-out) tile by NW waves.
+template <int W, int NW, bool INNER>
+struct Loads {
+  static constexpr int RPW = INNER ? 8 : 64 / (W / 8);  // tile rows per wave-load of 1 KB
+  static constexpr int Q = INNER ? W / 8 / NW : BK / RPW / NW;
+  static_assert(Q >= 1 && Q * RPW * NW == (INNER ? W : BK), "whole wave-loads");
+  static_assert((NW * RPW) % (INNER ? 16 : 4) == 0, "swizzle phase is the same for every load");
+  unsigned off[Q];  // bytes from the stage's base
+  int r0, chunk;    // the lane's row in load 0, its chunk's first element
+  __device__ __forceinline__ void init(const Operand& o, int x0, int wave, int lane) {
+    if constexpr (INNER) {
+      r0 = wave * 8 + lane / 8;
+      chunk = ((lane % 8) ^ ((r0 / 2) % 8)) * 8;
+#pragma unroll
+      for (int q = 0; q < Q; ++q)
+        off[q] = 2u * ((unsigned)min(r0 + q * NW * 8, o.rows - 1 - x0) * (unsigned)o.ld + (unsigned)chunk);
+    } else {
+      r0 = wave * RPW + lane / (W / 8);
+      chunk = ((lane % (W / 8)) ^ ((r0 & 3) << 2)) * 8;
+      const int col = min(x0 + chunk, o.rows - 8);
+#pragma unroll
+      for (int q = 0; q < Q; ++q)
+        off[q] = 2u * ((unsigned)(r0 + q * NW * RPW) * (unsigned)o.ld + (unsigned)col);
+    }
+  }
+  // load q of the stage at k0 of plane `pl` into `lds` (the operand's part of a stage)
+  __device__ __forceinline__ void load(const Operand& o, const uint16_t* zeros, int x0, int pl, int k0,
+                                       int q, int wave, unsigned char* lds) const {
+    const uint16_t* base = o.p + pl * o.plane + (INNER ? (int64_t)x0 * o.ld + k0 : (int64_t)k0 * o.ld);
+    unsigned char* to = lds + (wave + NW * q) * 1024;
+    if (k0 + BK <= o.k) {
+      dma16s(base, off[q], to);
+    } else {
+      const int k = k0 + (INNER ? chunk : r0 + q * NW * RPW);
+      const char* from = reinterpret_cast<const char*>(base) + off[q];
+      dma16(k < o.k ? from : reinterpret_cast<const char*>(zeros), to);
+    }
+  }
+};
+
+// The MFMA fragment of k step ks of tile rows (columns) col .. col + 31: lane l has
+// m (n) = col + l % 32, k = 16 ks + 8 (l / 32) .. + 7.
+template <int W, bool INNER>
+__device__ __forceinline__ bf16x8_t fragment(const unsigned char* t, int ks, int col, int lane) {
+  if constexpr (INNER) {
+    const int row = col + (lane & 31), kc = ks * 2 + (lane >> 5);
+    return __builtin_bit_cast(
+        bf16x8_t, *reinterpret_cast<const u32x4_t*>(t + (row * 8 + (kc ^ ((row / 2) % 8))) * 16));
+  } else {
+    const int li = lane & 15, lg = lane >> 4;
+    u32x2_t v[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int r = ks * 16 + 8 * (lg >> 1) + 4 * h + (li >> 2);
+      const int c = col + 16 * (lg & 1) + 4 * (li & 3);
+      const unsigned char* p = t + r * (W * 2) + ((c >> 3) ^ ((r & 3) << 2)) * 16 + (c & 7) * 2;
+      v[h] = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4_p)(p)));
+    }
+    const u32x4_t w = {v[0].x, v[0].y, v[1].x, v[1].y};
+    return __builtin_bit_cast(bf16x8_t, w);
+  }
+}
+
+// Stages s_lo .. s_hi - 1 (of pairs * nk) of the tile at (m0, n0) into acc.
+template <class TL, bool AIN, bool BIN>
+__device__ __forceinline__ void product_tile(const Product& p, unsigned char* lds, int m0, int n0,
+                                             int s_lo, int s_hi, f32x16_t (&acc)[TL::TM][TL::TN]) {
+  constexpr int TM = TL::TM, TN = TL::TN, NW = TL::NW, NS = TL::NS, KS = BK / 16;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave / TL::WN, wn = wave % TL::WN;
+  using LA = Loads<TL::BM, NW, AIN>;
+  using LB = Loads<TL::BN, NW, BIN>;
+  constexpr int LDPS = LA::Q + LB::Q;
+  static_assert((NS - 1) * LDPS <= 63, "vmcnt counts");
+  LA la;
+  LB lb;
+  la.init(p.a, m0, wave, lane);
+  lb.init(p.b, n0, wave, lane);
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int j = 0; j < TN; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
+
+  // the next stage to load: pair of planes and stage within it
+  int dp = s_lo / max(p.nk, 1), dk = s_lo - dp * p.nk;
+  auto next = [&] {
+    if (++dk == p.nk) dk = 0, ++dp;
+  };
+  auto load = [&](int slot, int from, int to) {
+    unsigned char* st = lds + slot * TL::BUF;
+    const int pa = (p.amap >> (2 * dp)) & 3, pb = (p.bmap >> (2 * dp)) & 3;
+#pragma unroll
+    for (int q = 0; q < LDPS; ++q) {
+      if (q < from || q >= to) continue;
+      if (q < LA::Q)
+        la.load(p.a, p.zeros, m0, pa, dk * BK, q, wave, st);
+      else
+        lb.load(p.b, p.zeros, n0, pb, dk * BK, q - LA::Q, wave, st + TL::A_BYTES);
+    }
+  };
+  const int n = s_hi - s_lo;
+#pragma unroll
+  for (int s = 0; s < NS - 1; ++s)
+    if (s < n) {
+      load(s, 0, LDPS);
+      next();
+    }
+  bf16x8_t af[2][TM], bf[2][TN];
+  auto frags = [&](const unsigned char* st, int set, int ks) {
+#pragma unroll
+    for (int j = 0; j < TN; ++j)
+      bf[set][j] = fragment<TL::BN, BIN>(st + TL::A_BYTES, ks, (wn * TN + j) * 32, lane);
+#pragma unroll
+    for (int i = 0; i < TM; ++i) af[set][i] = fragment<TL::BM, AIN>(st, ks, (wm * TM + i) * 32, lane);
+  };
+  constexpr int READS = TM * (AIN ? 1 : 2) + TN * (BIN ? 1 : 2);
+  constexpr int DSTEPS = 2;  // k steps that the next stage's loads are spread over
+  int slot = 0;
+  for (int kt = 0; kt < n; ++kt) {
+    // stage kt has landed (at most NS - 2 later ones in flight) and the stage read at
+    // kt - 1 is free: it receives stage kt + NS - 1
+    const int ahead = min(NS - 2, n - 1 - kt);
+    if (NS >= 4 && ahead >= 2) stage_barrier<2 * LDPS>();
+    else if (NS >= 3 && ahead >= 1) stage_barrier<LDPS>();
+    else stage_barrier<0>();
+    const unsigned char* st = lds + slot * TL::BUF;
+    const bool more = kt + NS - 1 < n;
+    const int free = slot == 0 ? NS - 1 : slot - 1;
+    frags(st, 0, 0);
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      if (ks + 1 < KS) frags(st, (ks + 1) & 1, ks + 1);
+#pragma unroll
+      for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(af[ks & 1][i], bf[ks & 1][j], acc[i][j], 0, 0, 0);
+      if (ks + 1 < KS) {
+        if (ks == 0) __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
+#pragma unroll
+        for (int q = 0; q < TM * TN; ++q) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+          const int nr = READS * (q + 1) / (TM * TN) - READS * q / (TM * TN);
+          if (nr == 1) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+          else if (nr == 2) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+          else if (nr == 3) __builtin_amdgcn_sched_group_barrier(0x100, 3, 0);
+          else if (nr >= 4) __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+        }
+      }
+      if (more && ks < DSTEPS) {
+        load(free, ks * LDPS / DSTEPS, (ks + 1) * LDPS / DSTEPS);
+        if (ks == DSTEPS - 1) next();
+      }
+    }
+    slot = slot + 1 == NS ? 0 : slot + 1;
+  }
+  stage_barrier<0>();  // every wave is done reading before the next tile's loads
+}
+
+// Tile `t` of mt x nt tiles, in groups of GN n-tiles by all m-tiles.
+__device__ __forceinline__ void tile_at(int t, int mt, int nt, int& m, int& n) {
+  const int g = t / (GN * mt), left = t - g * GN * mt, width = min(GN, nt - g * GN);
+  m = left / width;
+  n = g * GN + left - m * width;
+}
+// Calls f(item) for this workgroup's items of `items`.
+template <class F>
+__device__ __forceinline__ void each_item(int items, F f) {
+  const int xcd = blockIdx.x % 8, workers = gridDim.x / 8, per = (items + 7) / 8;
+  const int end = min((xcd + 1) * per, items);
+  for (int i = xcd * per + blockIdx.x / 8; i < end; i += workers) f(i);
+}
+
+// ---- logits ----
+
+__device__ __forceinline__ float softcapped(float z, float cap, float inv) {
+  // tanh(u) = (1 - t) / (1 + t), t = exp(-2 |u|): off by a few 2^-24 of 1
+  const float t = __builtin_amdgcn_exp2f(-2.0f * LOG2E * __builtin_fabsf(z * inv));
+  return __builtin_copysignf(cap * ((1.0f - t) * __builtin_amdgcn_rcpf(1.0f + t)), z);
+}
+
+template <class TL, bool STORE, int PLANES>
+__global__ __launch_bounds__(TL::NT, TL::WPS) void xent_logits_kernel(XentArgs a, Product p, int64_t r0) {
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[TL::NS * TL::BUF];
+  constexpr int TM = TL::TM, TN = TL::TN;
+  const int rows = mxm_xent_rows(a, r0);
+  p.b.rows = rows;
+  p.b.p += r0 * p.b.ld;
+  const int mt = (a.V + TL::BM - 1) / TL::BM, nt = (rows + TL::BN - 1) / TL::BN;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int wm = wave / TL::WN, wn = wave % TL::WN;
+  const float cap = a.softcap, inv = cap > 0.0f ? 1.0f / cap : 0.0f;
+  each_item(mt * nt, [&](int item) {
+    int tm, tn;
+    tile_at(item, mt, nt, tm, tn);
+    const int m0 = tm * TL::BM, n0 = tn * TL::BN;
+    int target[TN];
+#pragma unroll
+    for (int j = 0; j < TN; ++j) {
+      const int n = n0 + (wn * TN + j) * 32 + (lane & 31);
+      target[j] = n < rows ? a.targets[a.map[r0 + n]] : -1;
+    }
+    f32x16_t acc[TM][TN];
+    product_tile<TL, true, true>(p, lds, m0, n0, 0, p.nk * p.pairs, acc);
+    const int mw = m0 + wm * TM * 32;  // the wave's block of the vocabulary
+    if (mw >= a.V && !STORE) return;
+#pragma unroll
+    for (int j = 0; j < TN; ++j) {
+      const int n = n0 + (wn * TN + j) * 32 + (lane & 31);
+      if (cap > 0.0f) {
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) acc[i][j][r] = softcapped(acc[i][j][r], cap, inv);
+      }
+      // entries behind the vocabulary, and the target (whose logit is kept apart)
+      const int first = mw + (lane >> 5) * 4;
+      if (mw + TM * 32 > a.V) {
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (first + i * 32 + (r >> 2) * 8 + (r & 3) >= a.V) acc[i][j][r] = -__builtin_inff();
+      }
+      const int at = target[j] - first;
+      if (__ballot(target[j] >= mw && target[j] < mw + TM * 32)) {
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (at == i * 32 + (r >> 2) * 8 + (r & 3)) {
+              a.at_target[r0 + n] = acc[i][j][r];
+              acc[i][j][r] = -__builtin_inff();
+            }
+      }
+      float top = acc[0][j][0];
+#pragma unroll
+      for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) top = fmaxf(top, acc[i][j][r]);
+      top = fmaxf(top, mxm_xor_lane_f(top, 32));
+      // 2^(l log2 e - ref) lies in (0, 2^15]: fp16 keeps 12 bits of summands down to
+      // 2^-29 of the block's largest and 2^-39 of it at all
+      const float ref = top > -3.0e38f ? ceilf(top * LOG2E) - 15.0f : -1.0e30f;
+      float s[2] = {0.0f, 0.0f};
+#pragma unroll
+      for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const float l = acc[i][j][r];
+          float e = __builtin_amdgcn_exp2f(fmaf(l, LOG2E, -ref));
+          s[r & 1] += e;
+          if constexpr (STORE) {
+            if (cap > 0.0f) {
+              const float u = l * inv;
+              e *= l > -3.0e38f ? 1.0f - u * u : 0.0f;
+            }
+            acc[i][j][r] = e;
+          }
+        }
+      float sum = s[0] + s[1];
+      sum += mxm_xor_lane_f(sum, 32);
+      if (n < rows && mw < a.V && lane < 32)
+        a.stat[(int64_t)(mw / (TM * 32)) * a.stat_ld + n] = make_float2(sum, ref);
+      if constexpr (STORE) {
+        const int64_t row = (int64_t)n * a.Vp;
+#pragma unroll
+        for (int i = 0; i < TM; ++i) {
+          if constexpr (PLANES == 1) {
+            // quads q and q + 1 of the two half-waves exchanged: 8 consecutive entries a lane
+#pragma unroll
+            for (int q = 0; q < 4; q += 2) {
+              uint32_t w[2][2];
+#pragma unroll
+              for (int k = 0; k < 2; ++k)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                  const f16x2_t v = {(_Float16)acc[i][j][(q + k) * 4 + 2 * h],
+                                     (_Float16)acc[i][j][(q + k) * 4 + 2 * h + 1]};
+                  w[k][h] = __builtin_bit_cast(uint32_t, v);
+                }
+              const auto x = __builtin_amdgcn_permlane32_swap(w[0][0], w[1][0], false, false);
+              const auto y = __builtin_amdgcn_permlane32_swap(w[0][1], w[1][1], false, false);
+              const u32x4_t o = {x[0], y[0], x[1], y[1]};
+              const int m = mw + i * 32 + (q + (lane >> 5)) * 8;
+              if (n < rows && m < a.Vp)
+                *reinterpret_cast<u32x4_t*>(static_cast<uint16_t*>(a.summands) + row + m) = o;
+            }
+          } else {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const f32x4_t o = {acc[i][j][q * 4], acc[i][j][q * 4 + 1], acc[i][j][q * 4 + 2],
+                                 acc[i][j][q * 4 + 3]};
+              const int m = first + i * 32 + q * 8;
+              if (n < rows && m < a.Vp)
+                *reinterpret_cast<f32x4_t*>(static_cast<float*>(a.summands) + row + m) = o;
+            }
+          }
+        }
+      }
+    }
+  });
+}
+
+// ---- dx and dw ----
+
+// Where C goes: rows n of M elements.
+struct Out {
+  void* out;
+  const float* add;      // earlier sums of the same elements, or null
+  const int32_t* map;    // the row that n is, or null: n
+  int M;
+  bool bf16, vec;        // vec: rows of whole aligned 16 bytes
+};
+
+// Row n's elements m .. m + 3 of an MFMA tile, as each quad of registers holds them.
+__device__ __forceinline__ void put_tile(const Out& o, int m_first, int n, bool in, int lane, f32x16_t c) {
+  const int64_t row = in ? (int64_t)(o.map ? o.map[n] : n) * o.M : 0;
+  if (o.add && in) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int m = m_first + (r >> 2) * 8 + (lane >> 5) * 4 + (r & 3);
+      if (m < o.M) c[r] += o.add[row + m];
+    }
+  }
+  if (o.bf16 && o.vec) {
+#pragma unroll
+    for (int q = 0; q < 4; q += 2) {
+      uint32_t w[2][2];
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          w[k][h] = mxm_pack_bf2_fast(c[(q + k) * 4 + 2 * h], c[(q + k) * 4 + 2 * h + 1]);
+      const auto x = __builtin_amdgcn_permlane32_swap(w[0][0], w[1][0], false, false);
+      const auto y = __builtin_amdgcn_permlane32_swap(w[0][1], w[1][1], false, false);
+      const u32x4_t v = {x[0], y[0], x[1], y[1]};
+      const int m = m_first + (q + (lane >> 5)) * 8;
+      if (in && m < o.M) *reinterpret_cast<u32x4_t*>(static_cast<uint16_t*>(o.out) + row + m) = v;
+    }
+  } else {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int m = m_first + q * 8 + (lane >> 5) * 4;
+      if (!in) continue;
+      if (o.vec) {
+        const f32x4_t v = {c[q * 4], c[q * 4 + 1], c[q * 4 + 2], c[q * 4 + 3]};
+        if (m < o.M) *reinterpret_cast<f32x4_t*>(static_cast<float*>(o.out) + row + m) = v;
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (m + k < o.M) {
+            if (o.bf16)
+              static_cast<uint16_t*>(o.out)[row + m + k] = mxm_f2bf_fast(c[q * 4 + k]);
+            else
+              static_cast<float*>(o.out)[row + m + k] = c[q * 4 + k];
+          }
+      }
+    }
+  }
+}
+
+// What a launch needs of the device's count of rows: n of dx, k of dw.
+template <bool DW>
+__device__ __forceinline__ void fit(const XentArgs& a, Product& p, int64_t r0) {
+  const int rows = mxm_xent_rows(a, r0);
+  if constexpr (DW) {
+    p.a.p += r0 * p.a.ld;
+    p.a.k = p.b.k = rows;
+    p.nk = (rows + BK - 1) / BK;
+  } else {
+    p.b.rows = rows;
+  }
+}
+
+template <class TL, bool DW>
+__global__ __launch_bounds__(TL::NT, TL::WPS) void xent_grad_kernel(XentArgs a, Product p, Out o, int64_t r0,
+                                                                    int splits) {
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[TL::NS * TL::BUF];
+  constexpr int TM = TL::TM, TN = TL::TN;
+  fit<DW>(a, p, r0);
+  const int N = DW ? a.V : p.b.rows;
+  const int mt = (a.D + TL::BM - 1) / TL::BM, nt = (N + TL::BN - 1) / TL::BN;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int wm = wave / TL::WN, wn = wave % TL::WN;
+  const int stages = p.nk * p.pairs, tiles = mt * nt;
+  each_item(tiles * splits, [&](int item) {
+    const int split = item / tiles;
+    int tm, tn;
+    tile_at(item - split * tiles, mt, nt, tm, tn);
+    f32x16_t acc[TM][TN];
+    product_tile<TL, false, !DW>(p, lds, tm * TL::BM, tn * TL::BN, (int)((int64_t)split * stages / splits),
+                               (int)((int64_t)(split + 1) * stages / splits), acc);
+    if (splits > 1) {
+      f32x4_t* to = reinterpret_cast<f32x4_t*>(a.partial) + (int64_t)item * (TL::BM * TL::BN / 4) +
+                    wave * (TM * TN * 4 * 64) + lane;
+#pragma unroll
+      for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const f32x4_t v = {acc[i][j][q * 4], acc[i][j][q * 4 + 1], acc[i][j][q * 4 + 2],
+                               acc[i][j][q * 4 + 3]};
+            to[((i * TN + j) * 4 + q) * 64] = v;
+          }
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+      for (int j = 0; j < TN; ++j) {
+        const int n = tn * TL::BN + (wn * TN + j) * 32 + (lane & 31);
+        put_tile(o, tm * TL::BM + (wm * TM + i) * 32, n, n < N, lane, acc[i][j]);
+      }
+  });
+}
+
+// The splits of a tile added in order; a workgroup per MFMA tile of each wave.
+template <class TL, bool DW>
+__global__ __launch_bounds__(TL::NT) void xent_grad_join_kernel(XentArgs a, Out o, int64_t r0, int splits) {
+  constexpr int TM = TL::TM, TN = TL::TN;
+  const int N = DW ? a.V : mxm_xent_rows(a, r0);
+  const int mt = (a.D + TL::BM - 1) / TL::BM, nt = (N + TL::BN - 1) / TL::BN, tiles = mt * nt;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int wm = wave / TL::WN, wn = wave % TL::WN;
+  const int tile = blockIdx.x / (TM * TN), ij = blockIdx.x % (TM * TN), i = ij / TN, j = ij % TN;
+  if (tile >= tiles) return;
+  int tm, tn;
+  tile_at(tile, mt, nt, tm, tn);
+  f32x16_t c;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) c[r] = 0.0f;
+  for (int s = 0; s < splits; ++s) {
+    const f32x4_t* from = reinterpret_cast<const f32x4_t*>(a.partial) +
+                          ((int64_t)s * tiles + tile) * (TL::BM * TL::BN / 4) + wave * (TM * TN * 4 * 64) +
+                          ij * 4 * 64 + lane;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const f32x4_t v = from[q * 64];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) c[q * 4 + k] += v[k];
+    }
+  }
+  const int n = tn * TL::BN + (wn * TN + j) * 32 + (lane & 31);
+  put_tile(o, tm * TL::BM + (wm * TM + i) * 32, n, n < N, lane, c);
+}
+
+// ---- launches ----
+
+bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+int64_t tiles_of(int64_t m, int64_t n, int bm, int bn) { return (m + bm - 1) / bm * ((n + bn - 1) / bn); }
+unsigned grid_of(int64_t items, int64_t slots) {
+  return (unsigned)((std::min(items, slots) + 7) / 8 * 8);
+}
+// pairs of planes: (hi, lo), (lo, hi), (mid, mid), (hi, mid), (mid, hi), (hi, hi)
+constexpr uint32_t map_of(int p0, int p1, int p2, int p3, int p4, int p5) {
+  return p0 | p1 << 2 | p2 << 4 | p3 << 6 | p4 << 8 | p5 << 10;
+}
+void set_planes(const XentArgs& a, Product& p) {
+  p.pairs = a.planes == 1 ? 1 : 6;
+  p.amap = a.planes == 1 ? 0 : map_of(0, 2, 1, 0, 1, 0);
+  p.bmap = a.planes == 1 ? 0 : map_of(2, 0, 1, 1, 0, 0);
+  p.zeros = a.zeros;
+}
+// The table, its rows' k or (k-out) its columns.
+Operand table(const XentArgs& a, bool inner) {
+  Operand o{};
+  o.p = a.w_direct ? static_cast<const uint16_t*>(a.weight) : a.w_pack;
+  o.ld = a.w_direct ? a.D : a.Dp;
+  o.plane = (int64_t)a.V * o.ld;
+  o.rows = inner ? a.V : o.ld;
+  o.k = inner ? o.ld : a.V;
+  return o;
+}
+Operand hidden(const XentArgs& a, bool inner) {
+  Operand o{};
+  o.p = a.x_pack;
+  o.ld = a.Dp;
+  o.plane = a.x_rows * a.Dp;
+  o.rows = a.Dp;  // (k-out; k-inner: the rows that take part, on the device)
+  o.k = inner ? a.Dp : 0;
+  return o;
+}
+Operand grad(const XentArgs& a) {
+  Operand o{};
+  o.p = a.dz;
+  o.ld = a.Vp;
+  o.plane = a.piece_rows * a.Vp;
+  o.rows = a.Vp;
+  o.k = a.Vp;
+  return o;
+}
+
+enum Shape { FEW, SMALL, BIG };
+Shape logits_shape(int64_t rows) { return rows <= 32 ? FEW : rows <= 128 ? SMALL : BIG; }
+
+template <class TL, bool STORE, int PLANES>
+void launch_logits(const XentArgs& a, const Product& p, int64_t r0, int64_t rows, int per_cu, hipStream_t s) {
+  const unsigned grid = grid_of(tiles_of(a.V, rows, TL::BM, TL::BN), (int64_t)a.n_cu * per_cu);
+  xent_logits_kernel<TL, STORE, PLANES><<<grid, TL::NT, 0, s>>>(a, p, r0);
+}
+template <class TL>
+void launch_logits(const XentArgs& a, const Product& p, int64_t r0, int64_t rows, int per_cu, hipStream_t s) {
+  if (!a.backward) return launch_logits<TL, false, 1>(a, p, r0, rows, per_cu, s);
+  if (a.planes == 1) return launch_logits<TL, true, 1>(a, p, r0, rows, per_cu, s);
+  return launch_logits<TL, true, 3>(a, p, r0, rows, per_cu, s);
+}
+
+// How often a product of `tiles` tiles and `stages` stages is split: the least of
+// rounds of the CUs times a split's stages and its fixed cost (a tile's start and
+// end, and with splits its way through scratch), in stages.
+constexpr int TILE_COST = 8, SPLIT_COST = 12, MIN_STAGES = 4;
+int splits_of(int64_t tiles, int64_t stages, int64_t slots, int64_t scratch_tiles) {
+  int best = 1;
+  double least = 0;
+  for (int64_t s = 1; s == 1 || (s * tiles <= scratch_tiles && s * MIN_STAGES <= stages); ++s) {
+    const double rounds = (double)((tiles * s + slots - 1) / slots);
+    const double cost = rounds * ((double)((stages + s - 1) / s) + TILE_COST + (s > 1 ? SPLIT_COST : 0));
+    if (s == 1 || cost < least) best = (int)s, least = cost;
+  }
+  return best;
+}
+
+template <class TL, bool DW>
+void launch_grad(const XentArgs& a, const Product& p, const Out& o, int64_t r0, int64_t N, int64_t stages,
+                 int per_cu, hipStream_t s) {
+  const int64_t tiles = tiles_of(a.D, N, TL::BM, TL::BN), slots = (int64_t)a.n_cu * per_cu;
+  const int splits = splits_of(tiles, stages, slots, mxm_xent_partial_bytes(a.n_cu) / (TL::BM * TL::BN * 4));
+  xent_grad_kernel<TL, DW><<<grid_of(tiles * splits, slots), TL::NT, 0, s>>>(a, p, o, r0, splits);
+  if (splits > 1)
+    xent_grad_join_kernel<TL, DW><<<(unsigned)(tiles * TL::TM * TL::TN), TL::NT, 0, s>>>(a, o, r0, splits);
+}
+
+}  // namespace
+
+int64_t mxm_xent_partial_bytes(int n_cu) { return (int64_t)n_cu * 2 * 256 * 256 * 4; }
+
+int mxm_xent_block(int64_t rows) {
+  const Shape s = logits_shape(rows);
+  return s == FEW ? Few::TM * 32 : s == SMALL ? Small::TM * 32 : Big::TM * 32;
+}
+
+int64_t mxm_xent_stats(int64_t rows, int V) {
+  // (the narrower blocks of fewer rows among them)
+  const auto of = [&](int64_t n, int block) { return n * ((V + block - 1) / block); };
+  return std::max({of(rows, 128), of(std::min<int64_t>(rows, 128), 64), of(std::min<int64_t>(rows, 32), 32)});
+}
+
+void mxm_launch_xent_logits(const XentArgs& a, int64_t r0, int64_t rows, hipStream_t s) {
+  Product p{};
+  set_planes(a, p);
+  p.a = table(a, true);
+  p.b = hidden(a, true);
+  p.nk = a.Dp / BK;
+  switch (logits_shape(rows)) {
+    case FEW: return launch_logits<Few>(a, p, r0, rows, 2, s);
+    case SMALL: return launch_logits<Small>(a, p, r0, rows, 2, s);
+    default: return launch_logits<Big>(a, p, r0, rows, 1, s);
+  }
+}
+
+void mxm_launch_xent_dx(const XentArgs& a, int64_t r0, int64_t rows, hipStream_t s) {
+  Product p{};
+  set_planes(a, p);
+  p.a = table(a, false);
+  p.b = grad(a);
+  p.nk = a.Vp / BK;
+  Out o{};
+  o.out = a.dx;
+  o.map = a.map + r0;
+  o.M = a.D;
+  o.bf16 = a.dx_bf16;
+  o.vec = aligned(a.dx) && a.D % (a.dx_bf16 ? 8 : 4) == 0;
+  if (a.D <= 128 || rows <= 128)
+    launch_grad<Small, false>(a, p, o, r0, rows, (int64_t)p.nk * p.pairs, 2, s);
+  else
+    launch_grad<Big, false>(a, p, o, r0, rows, (int64_t)p.nk * p.pairs, 1, s);
+}
+
+void mxm_launch_xent_dw(const XentArgs& a, int64_t r0, int64_t rows, bool last, hipStream_t s) {
+  Product p{};
+  set_planes(a, p);
+  p.a = hidden(a, false);
+  p.b = grad(a);
+  Out o{};
+  float* sums = a.dw32 ? a.dw32 : static_cast<float*>(a.dw);
+  o.out = last ? a.dw : sums;
+  o.bf16 = last && a.dw_bf16;
+  o.add = r0 > 0 ? sums : nullptr;
+  o.M = a.D;
+  o.vec = aligned(o.out) && a.D % (o.bf16 ? 8 : 4) == 0;
+  const int64_t stages = (rows + BK - 1) / BK * p.pairs;
+  if (a.D <= 128 || a.V <= 128)
+    launch_grad<Small, true>(a, p, o, r0, a.V, stages, 2, s);
+  else
+    launch_grad<Big, true>(a, p, o, r0, a.V, stages, 1, s);
+}

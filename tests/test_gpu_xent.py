@@ -35,6 +35,11 @@ def tolerances(x, w, ref, dtype, softcap, V):
     rounding = (UBF + UBF / 4) if dtype == "bf16" else 8 * U32
     dz, dl = np.abs(ref["dz"]), np.abs(ref["dl"])
     edz = dz * (ep + rounding)
+    if dtype == "bf16":
+        # p is kept in fp16 between its two passes, in units of which the largest of a
+        # block of the vocabulary is over 2^14: half a step of fp16's subnormal numbers,
+        # 2^-25, is 2^-39 of that largest one, which is at most the row's largest p
+        edz = edz + dl.max(axis=1, keepdims=True) * 2.0 ** -39
     if softcap:                             # of 1 - (l / cap)^2
         edz = edz + dl * (2 * el / softcap + 16 * U32)
     per = 2 * (6 if dtype == "fp32" else 1)
