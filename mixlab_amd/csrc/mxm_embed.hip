@@ -55,21 +55,32 @@ __device__ __forceinline__ void store_unit(void* p, bool bf16, int64_t at, const
 
 constexpr int NT = 256;
 
-// A row per T threads.
+// A row per T threads, ROWS of them in flight: their tokens, then their elements.
+constexpr int ROWS = 4;
 template <int U>
 __global__ __launch_bounds__(NT) void embed_kernel(EmbedArgs a, int T) {
   const int per = NT / T, sub = threadIdx.x / T, t = threadIdx.x % T;
-  for (int64_t n = (int64_t)blockIdx.x * per + sub; n < a.rows; n += (int64_t)gridDim.x * per) {
-    const int v = a.tokens[n];
-    const bool in = v >= 0 && v < a.V;
+  const int64_t step = (int64_t)gridDim.x * per;
+  for (int64_t n0 = (int64_t)blockIdx.x * per + sub; n0 < a.rows; n0 += ROWS * step) {
+    int v[ROWS];
+#pragma unroll
+    for (int k = 0; k < ROWS; ++k) v[k] = n0 + k * step < a.rows ? a.tokens[n0 + k * step] : -1;
     for (int d = t * U; d < a.D; d += T * U) {
-      float e[U];
+      float e[ROWS][U];
 #pragma unroll
-      for (int i = 0; i < U; ++i) e[i] = 0.0f;
-      if (in) load_unit<U>(a.table, a.table_bf16, (int64_t)v * a.D + d, e);
+      for (int k = 0; k < ROWS; ++k) {
+        if (v[k] >= 0 && v[k] < a.V) {
+          load_unit<U>(a.table, a.table_bf16, (int64_t)v[k] * a.D + d, e[k]);
 #pragma unroll
-      for (int i = 0; i < U; ++i) e[i] = in ? e[i] * a.scale : 0.0f;
-      store_unit<U>(a.out, a.out_bf16, n * a.D + d, e);
+          for (int i = 0; i < U; ++i) e[k][i] *= a.scale;
+        } else {
+#pragma unroll
+          for (int i = 0; i < U; ++i) e[k][i] = 0.0f;
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < ROWS; ++k)
+        if (n0 + k * step < a.rows) store_unit<U>(a.out, a.out_bf16, (n0 + k * step) * a.D + d, e[k]);
     }
   }
 }
@@ -114,8 +125,8 @@ __global__ __launch_bounds__(64 * SORT_WAVES) void embed_sort_kernel(EmbedArgs a
 #pragma unroll
     for (int q = 0; q < SORT_AHEAD; ++q) {
       below += v[q] >= 0 && v[q] < lo;
-      const unsigned b = (unsigned)(v[q] - lo);
-      if (v[q] >= lo && b < (unsigned)own) atomicAdd(&cnt[wave][b], 1);
+      const unsigned b = (unsigned)v[q] - (unsigned)lo;
+      if (b < (unsigned)own) atomicAdd(&cnt[wave][b], 1);
     }
   }
 #pragma unroll
@@ -164,24 +175,26 @@ __global__ __launch_bounds__(64 * SORT_WAVES) void embed_sort_kernel(EmbedArgs a
     }
 #pragma unroll
     for (int q = 0; q < SORT_AHEAD; ++q) {
-      const bool mine = v[q] >= lo && v[q] - lo < own;
-      const int b = v[q] - lo;
-      unsigned long long left = __ballot(mine);
-      while (left) {  // one token that occurs in this group at a time
-        const int lead = __ffsll(left) - 1;
-        const int tok = __shfl(b, lead);
-        const bool same = mine && b == tok;
-        const unsigned long long all = __ballot(same);
-        const int at = tot[tok] + cnt[wave][tok];
-        if (same) {
-          const int rank = __popcll(all & ((1ull << lane) - 1));
-          a.sorted[at + rank] = make_int2((int)(n + 64 * q + lane), v[q]);
-        }
-        wave_lds_sync();  // every lane has read the count
-        if (lane == lead) cnt[wave][tok] += __popcll(all);
-        wave_lds_sync();
-        left &= ~all;
+      const unsigned b = (unsigned)v[q] - (unsigned)lo;
+      const bool mine = b < (unsigned)own;
+      // the lanes that hold the same token: a ballot per bit of its place in the span
+      unsigned long long same = __ballot(mine);
+      if (!same) continue;
+      for (unsigned bit = 1; bit < (unsigned)span; bit <<= 1) {
+        const bool set = b & bit;
+        const unsigned long long m = __ballot(set);
+        same &= set ? m : ~m;
       }
+      int left = 0;  // of the first of them: how many there are
+      if (mine) {
+        const unsigned long long before = same & ((1ull << lane) - 1);
+        const int at = tot[b] + cnt[wave][b];
+        a.sorted[at + __popcll(before)] = make_int2((int)(n + 64 * q + lane), v[q]);
+        if (!before) left = __popcll(same);
+      }
+      wave_lds_sync();  // every lane has read its count
+      if (left) cnt[wave][b] += left;
+      wave_lds_sync();
     }
   }
 }
@@ -203,6 +216,7 @@ __device__ __forceinline__ void put_row(const EmbedArgs& a, int v, int d, float 
   store_unit<U>(a.d_table, a.dtable_bf16, at, s);
 }
 
+constexpr int AHEAD = 4;  // rows in flight
 template <int U>
 __device__ __forceinline__ void sum_chunk(const EmbedArgs& a, int T, int t, int C, int64_t c, int64_t all) {
   const int64_t from = c * C, to = min(from + C, all);
@@ -213,25 +227,32 @@ __device__ __forceinline__ void sum_chunk(const EmbedArgs& a, int T, int t, int 
     for (int i = 0; i < U; ++i) s[i] = 0.0f;
     int v = a.sorted[from].y;
     bool first = true;  // the chunk's first run
-    for (int64_t p = from; p < to; ++p) {
-      const int2 e = a.sorted[p];
-      if (e.y != v) {
-        if (first && a.starts[v] < from) {
-          float* q = a.part + c * 2 * a.D + d;
+    for (int64_t p0 = from; p0 < to; p0 += AHEAD) {
+      int2 e[AHEAD];
+      float g[AHEAD][U];
 #pragma unroll
-          for (int i = 0; i < U; ++i) q[i] = s[i];
-        } else {
-          put_row<U>(a, v, d, s);
+      for (int k = 0; k < AHEAD; ++k) e[k] = a.sorted[min(p0 + k, to - 1)];
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) load_unit<U>(a.d_out, a.grad_bf16, (int64_t)e[k].x * a.D + d, g[k]);
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) {
+        if (p0 + k >= to) break;
+        if (e[k].y != v) {
+          if (first && a.starts[v] < from) {
+            float* q = a.part + c * 2 * a.D + d;
+#pragma unroll
+            for (int i = 0; i < U; ++i) q[i] = s[i];
+          } else {
+            put_row<U>(a, v, d, s);
+          }
+          first = false;
+          v = e[k].y;
+#pragma unroll
+          for (int i = 0; i < U; ++i) s[i] = 0.0f;
         }
-        first = false;
-        v = e.y;
 #pragma unroll
-        for (int i = 0; i < U; ++i) s[i] = 0.0f;
+        for (int i = 0; i < U; ++i) s[i] += g[k][i];
       }
-      float g[U];
-      load_unit<U>(a.d_out, a.grad_bf16, (int64_t)e.x * a.D + d, g);
-#pragma unroll
-      for (int i = 0; i < U; ++i) s[i] += g[i];
     }
     const bool before = first && a.starts[v] < from, after = a.starts[v + 1] > to;
     if (before || after) {
@@ -276,10 +297,21 @@ __device__ __forceinline__ void join_chunk(const EmbedArgs& a, int T, int t, int
     const float* q = a.part + (c * 2 + 1) * a.D + d;
 #pragma unroll
     for (int i = 0; i < U; ++i) s[i] = q[i];
-    for (int64_t k = c + 1; k <= last; ++k) {
-      q = a.part + k * 2 * a.D + d;
+    int64_t k = c + 1;
+    for (; k + 8 <= last + 1; k += 8) {
+      float e[8][U];
 #pragma unroll
-      for (int i = 0; i < U; ++i) s[i] += q[i];
+      for (int h = 0; h < 8; ++h) load_unit<U>(a.part, false, (k + h) * 2 * a.D + d, e[h]);
+#pragma unroll
+      for (int h = 0; h < 8; ++h)
+#pragma unroll
+        for (int i = 0; i < U; ++i) s[i] += e[h][i];
+    }
+    for (; k <= last; ++k) {
+      float e[U];
+      load_unit<U>(a.part, false, k * 2 * a.D + d, e);
+#pragma unroll
+      for (int i = 0; i < U; ++i) s[i] += e[i];
     }
     put_row<U>(a, v, d, s);
   }

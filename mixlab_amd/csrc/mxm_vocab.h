@@ -86,6 +86,7 @@ struct XentArgs {
   int planes;               // 1 (bf16) or 3
   int32_t* slot;            // [rows] a row's place among those that take part, or -1
   int32_t* map;             // [rows] and back
+  int32_t* target;          // [rows] of those that take part
   XentScalars* scalars;
   float* nll;               // [rows] loss of the rows that take part
   float* at_target;         // [rows] their target's logit

@@ -26,7 +26,7 @@ struct Xent : TrainHandle {
   XentArgs base{};
   int64_t max_rows = 0;
   bool backward = false;
-  DevBuf slot, map, scalars, nll, at_target, row, x_pack, w_pack, stat, summands, dz, partial, dw32, zeros;
+  DevBuf slot, map, target, scalars, nll, at_target, row, x_pack, w_pack, stat, summands, dz, partial, dw32, zeros;
   ~Xent() override {
     if (stream_ref) (void)hipStreamSynchronize(stream());
   }
@@ -264,6 +264,7 @@ int64_t mxm_xent_create(const int64_t* params, int n_params, float softcap, int6
     if (rows < a.piece_rows) a.piece_rows = std::max<int64_t>(64, up(rows));
     x->slot.alloc((size_t)rows * 4);
     x->map.alloc((size_t)rows * 4);
+    x->target.alloc((size_t)rows * 4);
     x->scalars.alloc(sizeof(XentScalars));
     x->nll.alloc((size_t)rows * 4);
     x->at_target.alloc((size_t)rows * 4);
@@ -274,6 +275,7 @@ int64_t mxm_xent_create(const int64_t* params, int n_params, float softcap, int6
     HIPCK(hipMemsetAsync(x->zeros.p, 0, 4096, x->stream()));
     a.slot = x->slot.as<int32_t>();
     a.map = x->map.as<int32_t>();
+    a.target = x->target.as<int32_t>();
     a.scalars = x->scalars.as<XentScalars>();
     a.nll = x->nll.as<float>();
     a.at_target = x->at_target.as<float>();

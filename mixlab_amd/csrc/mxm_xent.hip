@@ -6,16 +6,20 @@
 
 namespace {
 
+typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+typedef unsigned int u32x4_t __attribute__((ext_vector_type(4)));
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
+
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
-__device__ __forceinline__ float load1(const void* p, bool bf16, int64_t at) {
-  return bf16 ? mxm_bf2f(static_cast<const uint16_t*>(p)[at]) : static_cast<const float*>(p)[at];
-}
-
-__device__ __forceinline__ bool takes_part(const XentArgs& a, int64_t n, float& w) {
-  const int t = a.targets[n];
+__device__ __forceinline__ bool takes_part(const XentArgs& a, int64_t n, int& t, float& w) {
+  t = a.targets[n];
   w = a.row_weights ? a.row_weights[n] : 1.0f;
   return t >= 0 && t < a.V && w != 0.0f;
+}
+__device__ __forceinline__ void leave_out(const XentArgs& a, int64_t n) {
+  if (a.loss) a.loss[n] = 0.0f;
+  if (a.lse) a.lse[n] = 0.0f;
 }
 
 // The rows that take part, in order, and the sum of their weights; zeros for the
@@ -29,8 +33,9 @@ __global__ __launch_bounds__(PLAN_NT) void xent_plan_kernel(XentArgs a) {
   double sum = 0.0;
   for (int64_t n0 = 0; n0 < a.rows; n0 += PLAN_NT) {
     const int64_t n = n0 + threadIdx.x;
+    int t;
     float w = 0.0f;
-    const bool in = n < a.rows && takes_part(a, n, w);
+    const bool in = n < a.rows && takes_part(a, n, t, w);
     const unsigned long long m = __ballot(in);
     if (lane == 0) wave_count[wave] = __popcll(m);
     __syncthreads();
@@ -42,10 +47,10 @@ __global__ __launch_bounds__(PLAN_NT) void xent_plan_kernel(XentArgs a) {
     const int64_t at = base + before + __popcll(m & ((1ull << lane) - 1));
     if (in) {
       a.map[at] = (int32_t)n;
+      a.target[at] = t;
       sum += (double)w;
     } else if (n < a.rows) {
-      if (a.loss) a.loss[n] = 0.0f;
-      if (a.lse) a.lse[n] = 0.0f;
+      leave_out(a, n);
     }
     if (n < a.rows) a.slot[n] = in ? (int32_t)at : -1;
     base += all;
@@ -74,11 +79,47 @@ __device__ __forceinline__ void planes3(float v, uint16_t& hi, uint16_t& mid, ui
   lo = mxm_f2bf_fast(r - mxm_bf2f(mid));
 }
 
+__device__ __forceinline__ void planes3x8(const float (&v)[8], u32x4_t (&q)[3]) {
+  uint16_t p[3][8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) planes3(v[i], p[0][i], p[1][i], p[2][i]);
+#pragma unroll
+  for (int k = 0; k < 3; ++k)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) q[k][i] = p[k][2 * i] | (uint32_t)p[k][2 * i + 1] << 16;
+}
+
 constexpr int NT = 256;
 
-// Row `src` of x or weight to row `to` of its pack of `rows` rows, zeros behind D.
-__device__ __forceinline__ void pack_row(const XentArgs& a, const void* p, int64_t src, uint16_t* pack,
-                                         int64_t rows, int64_t to, int t, int T) {
+// Row `src` of x or weight to row `to` of its pack of `rows` rows, zeros behind D, by
+// T threads; wide: rows of whole aligned 16 bytes.
+__device__ __forceinline__ void pack_row(const XentArgs& a, const void* p, bool wide, int64_t src,
+                                         uint16_t* pack, int64_t rows, int64_t to, int t, int T) {
+  const int64_t plane = rows * a.Dp;
+  if (wide) {
+    for (int d = t * 8; d < a.Dp; d += T * 8) {
+      const int64_t at = to * a.Dp + d;
+      const u32x4_t none = {0, 0, 0, 0};
+      if (a.planes == 1) {
+        u32x4_t q = none;
+        if (d < a.D) q = *reinterpret_cast<const u32x4_t*>(static_cast<const uint16_t*>(p) + src * a.D + d);
+        *reinterpret_cast<u32x4_t*>(pack + at) = q;
+      } else {
+        u32x4_t q[3] = {none, none, none};
+        if (d < a.D) {
+          const f32x4_t* f = reinterpret_cast<const f32x4_t*>(static_cast<const float*>(p) + src * a.D + d);
+          const f32x4_t lo = f[0], hi = f[1];
+          float v[8];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) v[i] = lo[i], v[4 + i] = hi[i];
+          planes3x8(v, q);
+        }
+#pragma unroll
+        for (int k = 0; k < 3; ++k) *reinterpret_cast<u32x4_t*>(pack + at + k * plane) = q[k];
+      }
+    }
+    return;
+  }
   for (int d = t; d < a.Dp; d += T) {
     const int64_t at = to * a.Dp + d;
     if (a.planes == 1) {
@@ -86,7 +127,6 @@ __device__ __forceinline__ void pack_row(const XentArgs& a, const void* p, int64
     } else {
       uint16_t hi = 0, mid = 0, lo = 0;
       if (d < a.D) planes3(static_cast<const float*>(p)[src * a.D + d], hi, mid, lo);
-      const int64_t plane = rows * a.Dp;
       pack[at] = hi;
       pack[at + plane] = mid;
       pack[at + 2 * plane] = lo;
@@ -94,13 +134,72 @@ __device__ __forceinline__ void pack_row(const XentArgs& a, const void* p, int64
   }
 }
 
-// x's rows that take part to their places, and dx's others to zeros.
+__device__ __forceinline__ bool wide_rows(const XentArgs& a, const void* p) {
+  return a.D % 8 == 0 && (reinterpret_cast<uintptr_t>(p) & 15) == 0;
+}
+
+// x's rows that take part to their places, and dx's others to zeros; a wave per row.
+// PLAN: for up to PLAN_ROWS rows, every workgroup counts those before its own, and the
+// plan's launch is saved.
+constexpr int PLAN_ROWS = 1024;
+template <bool PLAN>
 __global__ __launch_bounds__(NT) void xent_pack_x_kernel(XentArgs a) {
-  const int lane = threadIdx.x & 63;
-  for (int64_t n = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); n < a.rows; n += (int64_t)gridDim.x * 4) {
-    const int to = a.slot[n];
+  __shared__ int count[2][4];
+  __shared__ double weight[4];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const bool wide = wide_rows(a, a.x);
+  for (int64_t first = (int64_t)blockIdx.x * 4; first < a.rows; first += (int64_t)gridDim.x * 4) {
+    const int64_t n = first + wave;
+    int to = -1;
+    if constexpr (PLAN) {
+      int before = 0, all = 0;
+      double sum = 0.0;
+#pragma unroll
+      for (int i = 0; i < PLAN_ROWS; i += NT) {
+        const int64_t k = i + threadIdx.x;
+        int t;
+        float w = 0.0f;
+        if (k < a.rows && takes_part(a, k, t, w)) {
+          before += k < n - wave;
+          ++all;
+          sum += (double)w;
+        }
+      }
+#pragma unroll
+      for (int o = 32; o > 0; o >>= 1) {
+        before += __shfl_xor(before, o);
+        all += __shfl_xor(all, o);
+        sum += __shfl_xor(sum, o);
+      }
+      if (lane == 0) count[0][wave] = before, count[1][wave] = all, weight[wave] = sum;
+      __syncthreads();
+      if (first == 0 && threadIdx.x == 0) {
+        a.scalars->rows = count[1][0] + count[1][1] + count[1][2] + count[1][3];
+        a.scalars->weight_sum = ((weight[0] + weight[1]) + weight[2]) + weight[3];
+      }
+      int at = count[0][0] + count[0][1] + count[0][2] + count[0][3];
+      int t = -1;
+      for (int64_t k = first; k <= n && k < a.rows; ++k) {  // (uniform in the wave)
+        float w;
+        const bool in = takes_part(a, k, t, w);
+        if (k == n) to = in ? at : -1;
+        at += in;
+      }
+      if (n < a.rows && lane == 0) {
+        if (to >= 0) {
+          a.map[to] = (int32_t)n;
+          a.target[to] = t;
+        } else {
+          leave_out(a, n);
+        }
+      }
+      __syncthreads();
+    } else if (n < a.rows) {
+      to = a.slot[n];
+    }
+    if (n >= a.rows) continue;
     if (to >= 0) {
-      pack_row(a, a.x, n, a.x_pack, a.x_rows, to, lane, 64);
+      pack_row(a, a.x, wide, n, a.x_pack, a.x_rows, to, lane, 64);
     } else if (a.dx) {
       for (int d = lane; d < a.D; d += 64) {
         if (a.dx_bf16)
@@ -114,38 +213,46 @@ __global__ __launch_bounds__(NT) void xent_pack_x_kernel(XentArgs a) {
 
 __global__ __launch_bounds__(NT) void xent_pack_w_kernel(XentArgs a) {
   const int lane = threadIdx.x & 63;
+  const bool wide = wide_rows(a, a.weight);
   for (int64_t v = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); v < a.V; v += (int64_t)gridDim.x * 4)
-    pack_row(a, a.weight, v, a.w_pack, a.V, v, lane, 64);
+    pack_row(a, a.weight, wide, v, a.w_pack, a.V, v, lane, 64);
 }
 
-// 16 rows by 16 threads: each row's blocks joined.
-constexpr int JOIN_ROWS = 16;
-__global__ __launch_bounds__(NT) void xent_join_kernel(XentArgs a, int64_t r0, int blocks) {
-  __shared__ float red[2][16][JOIN_ROWS];
-  const int rows = mxm_xent_rows(a, r0);
-  const int m = blockIdx.x * JOIN_ROWS + (threadIdx.x & 15), part = threadIdx.x >> 4;
-  if (blockIdx.x * JOIN_ROWS >= rows) return;
-  const bool in = m < rows;
-  float top = -__builtin_inff(), sum = 0.0f;
-  for (int b = part; in && b < blocks; b += 16) {
-    const float2 e = a.stat[(int64_t)b * a.stat_ld + m];
-    const float up = fmaxf(top, e.y);
-    // (ref and top agree where both are infinite: no difference to take)
-    sum = sum * (top == up ? 1.0f : __builtin_amdgcn_exp2f(top - up)) +
-          e.x * (e.y == up ? 1.0f : __builtin_amdgcn_exp2f(e.y - up));
-    top = up;
+// What a set of exponentials sums to: sum * 2^top.
+struct Sum {
+  float top, sum;
+};
+__device__ __forceinline__ Sum join(Sum p, Sum q) {
+  // (no difference of equal ones: they may be infinite)
+  const float up = fmaxf(p.top, q.top);
+  return {up, p.sum * (p.top == up ? 1.0f : __builtin_amdgcn_exp2f(p.top - up)) +
+                  q.sum * (q.top == up ? 1.0f : __builtin_amdgcn_exp2f(q.top - up))};
+}
+// Blocks part, part + parts, ... of row m.
+__device__ __forceinline__ Sum blocks_of(const XentArgs& a, int m, int part, int parts, int blocks) {
+  constexpr int AHEAD = 8;
+  Sum all = {-__builtin_inff(), 0.0f};
+  for (int b = part; b < blocks; b += AHEAD * parts) {
+    float2 e[AHEAD];
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k)
+      e[k] = b + k * parts < blocks ? a.stat[(int64_t)(b + k * parts) * a.stat_ld + m]
+                                    : make_float2(0.0f, -__builtin_inff());
+    float up = all.top;
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) up = fmaxf(up, e[k].y);
+    float s = all.sum * (all.top == up ? 1.0f : __builtin_amdgcn_exp2f(all.top - up));
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) s += e[k].x * (e[k].y == up ? 1.0f : __builtin_amdgcn_exp2f(e[k].y - up));
+    all = {up, s};
   }
-  red[0][part][threadIdx.x & 15] = top;
-  red[1][part][threadIdx.x & 15] = sum;
-  __syncthreads();
-  if (part != 0 || !in) return;
-  for (int p = 1; p < 16; ++p) {
-    const float t = red[0][p][m & 15], s = red[1][p][m & 15], up = fmaxf(top, t);
-    sum = sum * (top == up ? 1.0f : __builtin_amdgcn_exp2f(top - up)) +
-          s * (t == up ? 1.0f : __builtin_amdgcn_exp2f(t - up));
-    top = up;
-  }
+  return all;
+}
+
+// Row m's loss and the factors of its gradient from the others' sum.
+__device__ __forceinline__ float finish_row(const XentArgs& a, int64_t r0, int m, Sum others) {
   // the others' sum is sum * 2^top, the target's exponential 2^(top - d)
+  const float top = others.top, sum = others.sum;
   const float lt = a.at_target[r0 + m], d = fmaf(-lt, LOG2E, top);
   const float et = __builtin_amdgcn_exp2f(-d), whole = sum + et;
   // (next to the target's probability of one the loss keeps its digits)
@@ -168,15 +275,57 @@ __global__ __launch_bounds__(NT) void xent_join_kernel(XentArgs a, int64_t r0, i
       slope = 1.0f - u * u;
     }
     r.at_target = -g * (sum / whole) * slope;
-    r.target = a.targets[n];
+    r.target = a.target[r0 + m];
     a.row[r0 + m] = r;
+  }
+  return loss;
+}
+
+// Few rows: a wave each.  With one workgroup for all of them it also sums the total.
+constexpr int JOIN_WAVES = 16, JOIN_FEW = 512;
+__global__ __launch_bounds__(64 * JOIN_WAVES) void xent_join_few_kernel(XentArgs a, int64_t r0, int blocks,
+                                                                        bool total) {
+  __shared__ double part[JOIN_WAVES];
+  const int rows = mxm_xent_rows(a, r0), lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int m = blockIdx.x * JOIN_WAVES + wave;
+  double sum = 0.0;
+  if (m < rows) {
+    Sum s = blocks_of(a, m, lane, 64, blocks);
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) s = join(s, {__shfl_xor(s.top, o), __shfl_xor(s.sum, o)});
+    if (lane == 0) {
+      const float loss = finish_row(a, r0, m, s);
+      sum = (double)loss * (a.row_weights ? (double)a.row_weights[a.map[r0 + m]] : 1.0);
+    }
+  }
+  if (!total) return;
+  if (lane == 0) part[wave] = sum;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    sum = 0.0;
+    for (int i = 0; i < JOIN_WAVES; ++i) sum += part[i];
+    if (a.mean && rows > 0) sum /= a.scalars->weight_sum;
+    a.total[0] = (float)sum;
   }
 }
 
+// 16 rows by 16 threads.
+constexpr int JOIN_ROWS = 16;
+__global__ __launch_bounds__(NT) void xent_join_kernel(XentArgs a, int64_t r0, int blocks) {
+  __shared__ Sum red[4][JOIN_ROWS];
+  const int rows = mxm_xent_rows(a, r0);
+  const int k = threadIdx.x & 15, m = blockIdx.x * JOIN_ROWS + k;
+  if (blockIdx.x * JOIN_ROWS >= rows) return;
+  Sum s = blocks_of(a, min(m, rows - 1), threadIdx.x >> 4, 16, blocks);
+  s = join(s, {__shfl_xor(s.top, 16), __shfl_xor(s.sum, 16)});
+  s = join(s, {__shfl_xor(s.top, 32), __shfl_xor(s.sum, 32)});
+  if ((threadIdx.x & 63) < 16) red[threadIdx.x >> 6][k] = s;
+  __syncthreads();
+  if (threadIdx.x < 16 && m < rows)
+    finish_row(a, r0, m, join(join(red[0][k], red[1][k]), join(red[2][k], red[3][k])));
+}
+
 // The summands of a piece to dz, 8 of a row per thread.
-typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
-typedef unsigned int u32x4_t __attribute__((ext_vector_type(4)));
-typedef float f32x4_t __attribute__((ext_vector_type(4)));
 template <int PLANES>
 __global__ __launch_bounds__(NT) void xent_finish_kernel(XentArgs a, int64_t r0, int block) {
   const int rows = mxm_xent_rows(a, r0), units = a.Vp / 8;
@@ -208,16 +357,11 @@ __global__ __launch_bounds__(NT) void xent_finish_kernel(XentArgs a, int64_t r0,
         for (int i = 0; i < 4; ++i) o[i] = mxm_pack_bf2_fast(e[2 * i], e[2 * i + 1]);
         *reinterpret_cast<u32x4_t*>(a.dz + at) = o;
       } else {
-        uint16_t p[3][8];
+        u32x4_t q[3];
+        planes3x8(e, q);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) planes3(e[i], p[0][i], p[1][i], p[2][i]);
-#pragma unroll
-        for (int k = 0; k < 3; ++k) {
-          u32x4_t o;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) o[i] = p[k][2 * i] | (uint32_t)p[k][2 * i + 1] << 16;
-          *reinterpret_cast<u32x4_t*>(a.dz + (int64_t)k * a.piece_rows * a.Vp + at) = o;
-        }
+        for (int k = 0; k < 3; ++k)
+          *reinterpret_cast<u32x4_t*>(a.dz + (int64_t)k * a.piece_rows * a.Vp + at) = q[k];
       }
     }
   }
@@ -246,20 +390,29 @@ void mxm_launch_xent(const XentArgs& a0, hipStream_t s) {
   XentArgs a = a0;
   a.w_direct = a.bf16 && a.D % 8 == 0 && (reinterpret_cast<uintptr_t>(a.weight) & 15) == 0;
   const auto rows_grid = [&](int64_t n) { return (unsigned)std::min<int64_t>((n + 3) / 4, (int64_t)a.n_cu * 16); };
-  xent_plan_kernel<<<1, PLAN_NT, 0, s>>>(a);
+  const bool plan = a.rows > 0 && a.rows <= PLAN_ROWS;
+  if (!plan) xent_plan_kernel<<<1, PLAN_NT, 0, s>>>(a);
   if (a.rows > 0) {
-    xent_pack_x_kernel<<<rows_grid(a.rows), NT, 0, s>>>(a);
+    if (plan)
+      xent_pack_x_kernel<true><<<rows_grid(a.rows), NT, 0, s>>>(a);
+    else
+      xent_pack_x_kernel<false><<<rows_grid(a.rows), NT, 0, s>>>(a);
     if (!a.w_direct) xent_pack_w_kernel<<<rows_grid(a.V), NT, 0, s>>>(a);
   }
   const int64_t pieces = std::max<int64_t>(1, (a.rows + a.piece_rows - 1) / a.piece_rows);
+  const bool total_there = a.total && a.rows > 0 && a.rows <= JOIN_WAVES;  // (one piece)
   for (int64_t p = 0; p < pieces; ++p) {
     const int64_t r0 = p * a.piece_rows, rows = std::min(a.rows - r0, a.piece_rows);
     if (rows > 0) {
       const int block = mxm_xent_block(rows);
       a.stat_ld = rows;
       mxm_launch_xent_logits(a, r0, rows, s);
-      xent_join_kernel<<<(unsigned)((rows + JOIN_ROWS - 1) / JOIN_ROWS), NT, 0, s>>>(
-          a, r0, (a.V + block - 1) / block);
+      const int blocks = (a.V + block - 1) / block;
+      if (rows <= JOIN_FEW)
+        xent_join_few_kernel<<<(unsigned)((rows + JOIN_WAVES - 1) / JOIN_WAVES), 64 * JOIN_WAVES, 0, s>>>(
+            a, r0, blocks, total_there);
+      else
+        xent_join_kernel<<<(unsigned)((rows + JOIN_ROWS - 1) / JOIN_ROWS), NT, 0, s>>>(a, r0, blocks);
       if (a.backward) {
         const unsigned gx = (unsigned)std::min((a.Vp / 8 + NT - 1) / NT, 64);
         const dim3 grid(gx, (unsigned)std::min<int64_t>(rows, std::max(1u, (unsigned)a.n_cu * 32 / gx)));
@@ -272,5 +425,5 @@ void mxm_launch_xent(const XentArgs& a0, hipStream_t s) {
     }
     if (a.dw) mxm_launch_xent_dw(a, r0, rows, p == pieces - 1, s);
   }
-  if (a.total) xent_total_kernel<<<1, PLAN_NT, 0, s>>>(a);
+  if (a.total && !total_there) xent_total_kernel<<<1, PLAN_NT, 0, s>>>(a);
 }

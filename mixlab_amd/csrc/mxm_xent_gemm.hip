@@ -303,7 +303,7 @@ __global__ __launch_bounds__(TL::NT, TL::WPS) void xent_logits_kernel(XentArgs a
 #pragma unroll
     for (int j = 0; j < TN; ++j) {
       const int n = n0 + (wn * TN + j) * 32 + (lane & 31);
-      target[j] = n < rows ? a.targets[a.map[r0 + n]] : -1;
+      target[j] = n < rows ? a.target[r0 + n] : -1;
     }
     f32x16_t acc[TM][TN];
     product_tile<TL, true, true>(p, lds, m0, n0, 0, p.nk * p.pairs, acc);
