@@ -107,12 +107,12 @@ struct XentArgs {
 // Bytes of partial, for handles that run backward.
 int64_t mxm_xent_partial_bytes(int n_cu);
 // Most blocks of stat times rows, for pieces of `rows`.
-int64_t mxm_xent_stats(int64_t rows, int V);
+int64_t mxm_xent_stats(int64_t rows, int V, int n_cu);
 // Columns of the vocabulary per block of stat, for a piece of `rows` rows.
-int mxm_xent_block(int64_t rows);
+int mxm_xent_block(int64_t rows, int V, int n_cu);
 void mxm_launch_xent_logits(const XentArgs& a, int64_t r0, int64_t rows, hipStream_t s);
 void mxm_launch_xent_dx(const XentArgs& a, int64_t r0, int64_t rows, hipStream_t s);
-void mxm_launch_xent_dw(const XentArgs& a, int64_t r0, int64_t rows, bool last, hipStream_t s);
+void mxm_launch_xent_dw(const XentArgs& a, int64_t r0, bool last, hipStream_t s);
 void mxm_launch_xent(const XentArgs& a, hipStream_t s);
 
 // Rows of the piece that starts at row r0 of those that take part.

@@ -270,7 +270,7 @@ int64_t mxm_xent_create(const int64_t* params, int n_params, float softcap, int6
     x->at_target.alloc((size_t)rows * 4);
     x->x_pack.alloc((size_t)a.x_rows * a.Dp * 2 * a.planes);
     x->w_pack.alloc((size_t)V * a.Dp * 2 * a.planes);
-    x->stat.alloc((size_t)mxm_xent_stats(a.piece_rows, a.V) * sizeof(float2));
+    x->stat.alloc((size_t)mxm_xent_stats(a.piece_rows, a.V, a.n_cu) * sizeof(float2));
     x->zeros.alloc(4096);
     HIPCK(hipMemsetAsync(x->zeros.p, 0, 4096, x->stream()));
     a.slot = x->slot.as<int32_t>();

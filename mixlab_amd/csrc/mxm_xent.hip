@@ -404,7 +404,7 @@ void mxm_launch_xent(const XentArgs& a0, hipStream_t s) {
   for (int64_t p = 0; p < pieces; ++p) {
     const int64_t r0 = p * a.piece_rows, rows = std::min(a.rows - r0, a.piece_rows);
     if (rows > 0) {
-      const int block = mxm_xent_block(rows);
+      const int block = mxm_xent_block(rows, a.V, a.n_cu);
       a.stat_ld = rows;
       mxm_launch_xent_logits(a, r0, rows, s);
       const int blocks = (a.V + block - 1) / block;
@@ -423,7 +423,7 @@ void mxm_launch_xent(const XentArgs& a0, hipStream_t s) {
       }
       if (a.dx) mxm_launch_xent_dx(a, r0, rows, s);
     }
-    if (a.dw) mxm_launch_xent_dw(a, r0, rows, p == pieces - 1, s);
+    if (a.dw) mxm_launch_xent_dw(a, r0, p == pieces - 1, s);
   }
   if (a.total && !total_there) xent_total_kernel<<<1, PLAN_NT, 0, s>>>(a);
 }

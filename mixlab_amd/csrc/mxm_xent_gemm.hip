@@ -262,19 +262,48 @@ __device__ __forceinline__ void product_tile(const Product& p, unsigned char* ld
   stage_barrier<0>();  // every wave is done reading before the next tile's loads
 }
 
+// How a product's tiles are worked off: `whole` of them (whole rounds of the CUs) in one
+// piece, each of the others, the last round's, split along the sum so that they fill
+// the CUs too.
+struct Split {
+  int whole, tail, splits;
+};
+// Costs in stages: a tile's start and end, a split's way through scratch, and the
+// second launch's addition per split.
+constexpr int TILE_COST = 3, SPLIT_COST = 6, MIN_STAGES = 4;
+__host__ __device__ inline Split split_of(int tiles, int stages, int slots, int scratch_tiles) {
+  Split p{tiles / slots * slots, 0, 1};
+  p.tail = tiles - p.whole;
+  if (p.tail == 0) return p;
+  int least = stages + TILE_COST;
+  for (int rounds = 1; rounds <= 2; ++rounds) {
+    int n = rounds * slots / p.tail;
+    if (n > stages / MIN_STAGES) n = stages / MIN_STAGES;
+    if (n * p.tail > scratch_tiles) n = scratch_tiles / p.tail;
+    if (n < 2) continue;
+    const int need = (n * p.tail + slots - 1) / slots;
+    const int cost = need * ((stages + n - 1) / n + TILE_COST) + SPLIT_COST + n / 2;
+    if (cost < least) least = cost, p.splits = n;
+  }
+  return p;
+}
+
 // Tile `t` of mt x nt tiles, in groups of GN n-tiles by all m-tiles.
 __device__ __forceinline__ void tile_at(int t, int mt, int nt, int& m, int& n) {
   const int g = t / (GN * mt), left = t - g * GN * mt, width = min(GN, nt - g * GN);
   m = left / width;
   n = g * GN + left - m * width;
 }
-// Calls f(item) for this workgroup's items of `items`.
-template <class F>
-__device__ __forceinline__ void each_item(int items, F f) {
-  const int xcd = blockIdx.x % 8, workers = gridDim.x / 8, per = (items + 7) / 8;
-  const int end = min((xcd + 1) * per, items);
-  for (int i = xcd * per + blockIdx.x / 8; i < end; i += workers) f(i);
-}
+// This workgroup's items of `items`: first, first + step, ... below end.
+struct Items {
+  int first, step, end;
+  __device__ __forceinline__ explicit Items(int items) {
+    const int xcd = blockIdx.x % 8, per = (items + 7) / 8;
+    first = xcd * per + blockIdx.x / 8;
+    step = gridDim.x / 8;
+    end = min((xcd + 1) * per, items);
+  }
+};
 
 // ---- logits ----
 
@@ -295,7 +324,8 @@ __global__ __launch_bounds__(TL::NT, TL::WPS) void xent_logits_kernel(XentArgs a
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int wm = wave / TL::WN, wn = wave % TL::WN;
   const float cap = a.softcap, inv = cap > 0.0f ? 1.0f / cap : 0.0f;
-  each_item(mt * nt, [&](int item) {
+  const Items items(mt * nt);
+  for (int item = items.first; item < items.end; item += items.step) {
     int tm, tn;
     tile_at(item, mt, nt, tm, tn);
     const int m0 = tm * TL::BM, n0 = tn * TL::BN;
@@ -308,7 +338,7 @@ __global__ __launch_bounds__(TL::NT, TL::WPS) void xent_logits_kernel(XentArgs a
     f32x16_t acc[TM][TN];
     product_tile<TL, true, true>(p, lds, m0, n0, 0, p.nk * p.pairs, acc);
     const int mw = m0 + wm * TM * 32;  // the wave's block of the vocabulary
-    if (mw >= a.V && !STORE) return;
+    if (mw >= a.V && !STORE) continue;
 #pragma unroll
     for (int j = 0; j < TN; ++j) {
       const int n = n0 + (wn * TN + j) * 32 + (lane & 31);
@@ -404,7 +434,7 @@ __global__ __launch_bounds__(TL::NT, TL::WPS) void xent_logits_kernel(XentArgs a
         }
       }
     }
-  });
+  }
 }
 
 // ---- dx and dw ----
@@ -480,7 +510,7 @@ __device__ __forceinline__ void fit(const XentArgs& a, Product& p, int64_t r0) {
 
 template <class TL, bool DW>
 __global__ __launch_bounds__(TL::NT, TL::WPS) void xent_grad_kernel(XentArgs a, Product p, Out o, int64_t r0,
-                                                                    int splits) {
+                                                                    int slots, int scratch_tiles) {
   __shared__ __attribute__((aligned(1024))) unsigned char lds[TL::NS * TL::BUF];
   constexpr int TM = TL::TM, TN = TL::TN;
   fit<DW>(a, p, r0);
@@ -488,16 +518,17 @@ __global__ __launch_bounds__(TL::NT, TL::WPS) void xent_grad_kernel(XentArgs a, 
   const int mt = (a.D + TL::BM - 1) / TL::BM, nt = (N + TL::BN - 1) / TL::BN;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int wm = wave / TL::WN, wn = wave % TL::WN;
-  const int stages = p.nk * p.pairs, tiles = mt * nt;
-  each_item(tiles * splits, [&](int item) {
-    const int split = item / tiles;
+  const int stages = p.nk * p.pairs;
+  const Split plan = split_of(mt * nt, stages, slots, scratch_tiles);
+  auto work = [&](int tile, int split, int splits) {
     int tm, tn;
-    tile_at(item - split * tiles, mt, nt, tm, tn);
+    tile_at(tile, mt, nt, tm, tn);
     f32x16_t acc[TM][TN];
     product_tile<TL, false, !DW>(p, lds, tm * TL::BM, tn * TL::BN, (int)((int64_t)split * stages / splits),
-                               (int)((int64_t)(split + 1) * stages / splits), acc);
+                                 (int)((int64_t)(split + 1) * stages / splits), acc);
     if (splits > 1) {
-      f32x4_t* to = reinterpret_cast<f32x4_t*>(a.partial) + (int64_t)item * (TL::BM * TL::BN / 4) +
+      f32x4_t* to = reinterpret_cast<f32x4_t*>(a.partial) +
+                    (int64_t)(split * plan.tail + tile - plan.whole) * (TL::BM * TL::BN / 4) +
                     wave * (TM * TN * 4 * 64) + lane;
 #pragma unroll
       for (int i = 0; i < TM; ++i)
@@ -518,34 +549,58 @@ __global__ __launch_bounds__(TL::NT, TL::WPS) void xent_grad_kernel(XentArgs a, 
         const int n = tn * TL::BN + (wn * TN + j) * 32 + (lane & 31);
         put_tile(o, tm * TL::BM + (wm * TM + i) * 32, n, n < N, lane, acc[i][j]);
       }
-  });
+  };
+  // (one loop over both lists: the tile's code once)
+  const Items whole(plan.whole), tail(plan.tail * plan.splits);
+  int item = whole.first;
+  bool rest = item >= whole.end;
+  if (rest) item = tail.first;
+  while (!rest || item < tail.end) {
+    const int split = rest ? item / plan.tail : 0;
+    work(rest ? plan.whole + item - split * plan.tail : item, split, rest ? plan.splits : 1);
+    item += whole.step;
+    if (!rest && item >= whole.end) {
+      rest = true;
+      item = tail.first;
+    }
+  }
 }
 
-// The splits of a tile added in order; a workgroup per MFMA tile of each wave.
+// The splits of the last round's tiles added in order; a workgroup per MFMA tile of
+// each wave.
 template <class TL, bool DW>
-__global__ __launch_bounds__(TL::NT) void xent_grad_join_kernel(XentArgs a, Out o, int64_t r0, int splits) {
-  constexpr int TM = TL::TM, TN = TL::TN;
-  const int N = DW ? a.V : mxm_xent_rows(a, r0);
-  const int mt = (a.D + TL::BM - 1) / TL::BM, nt = (N + TL::BN - 1) / TL::BN, tiles = mt * nt;
+__global__ __launch_bounds__(TL::NT) void xent_grad_join_kernel(XentArgs a, Product p, Out o, int64_t r0,
+                                                                int slots, int scratch_tiles) {
+  constexpr int TM = TL::TM, TN = TL::TN, AHEAD = 4;
+  fit<DW>(a, p, r0);
+  const int N = DW ? a.V : p.b.rows;
+  const int mt = (a.D + TL::BM - 1) / TL::BM, nt = (N + TL::BN - 1) / TL::BN;
+  const Split plan = split_of(mt * nt, p.nk * p.pairs, slots, scratch_tiles);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int wm = wave / TL::WN, wn = wave % TL::WN;
   const int tile = blockIdx.x / (TM * TN), ij = blockIdx.x % (TM * TN), i = ij / TN, j = ij % TN;
-  if (tile >= tiles) return;
+  if (plan.splits == 1 || tile >= plan.tail) return;
   int tm, tn;
-  tile_at(tile, mt, nt, tm, tn);
+  tile_at(plan.whole + tile, mt, nt, tm, tn);
   f32x16_t c;
 #pragma unroll
   for (int r = 0; r < 16; ++r) c[r] = 0.0f;
-  for (int s = 0; s < splits; ++s) {
-    const f32x4_t* from = reinterpret_cast<const f32x4_t*>(a.partial) +
-                          ((int64_t)s * tiles + tile) * (TL::BM * TL::BN / 4) + wave * (TM * TN * 4 * 64) +
-                          ij * 4 * 64 + lane;
+  const int64_t step = (int64_t)plan.tail * (TL::BM * TL::BN / 4);
+  const f32x4_t* from = reinterpret_cast<const f32x4_t*>(a.partial) + (int64_t)tile * (TL::BM * TL::BN / 4) +
+                        wave * (TM * TN * 4 * 64) + ij * 4 * 64 + lane;
+  for (int s = 0; s < plan.splits; s += AHEAD) {
+    f32x4_t v[AHEAD][4];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const f32x4_t v = from[q * 64];
+    for (int h = 0; h < AHEAD; ++h)
 #pragma unroll
-      for (int k = 0; k < 4; ++k) c[q * 4 + k] += v[k];
-    }
+      for (int q = 0; q < 4; ++q)
+        v[h][q] = s + h < plan.splits ? from[(s + h) * step + q * 64] : f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int h = 0; h < AHEAD; ++h)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) c[q * 4 + k] += v[h][q][k];
   }
   const int n = tn * TL::BN + (wn * TN + j) * 32 + (lane & 31);
   put_tile(o, tm * TL::BM + (wm * TM + i) * 32, n, n < N, lane, c);
@@ -598,7 +653,10 @@ Operand grad(const XentArgs& a) {
 }
 
 enum Shape { FEW, SMALL, BIG };
-Shape logits_shape(int64_t rows) { return rows <= 32 ? FEW : rows <= 128 ? SMALL : BIG; }
+Shape logits_shape(int64_t rows, int V, int n_cu) {
+  if (rows <= 32) return FEW;
+  return rows <= 128 || tiles_of(V, rows, Big::BM, Big::BN) <= n_cu / 2 ? SMALL : BIG;
+}
 
 template <class TL, bool STORE, int PLANES>
 void launch_logits(const XentArgs& a, const Product& p, int64_t r0, int64_t rows, int per_cu, hipStream_t s) {
@@ -612,44 +670,36 @@ void launch_logits(const XentArgs& a, const Product& p, int64_t r0, int64_t rows
   return launch_logits<TL, true, 3>(a, p, r0, rows, per_cu, s);
 }
 
-// How often a product of `tiles` tiles and `stages` stages is split: the least of
-// rounds of the CUs times a split's stages and its fixed cost (a tile's start and
-// end, and with splits its way through scratch), in stages.
-constexpr int TILE_COST = 8, SPLIT_COST = 12, MIN_STAGES = 4;
-int splits_of(int64_t tiles, int64_t stages, int64_t slots, int64_t scratch_tiles) {
-  int best = 1;
-  double least = 0;
-  for (int64_t s = 1; s == 1 || (s * tiles <= scratch_tiles && s * MIN_STAGES <= stages); ++s) {
-    const double rounds = (double)((tiles * s + slots - 1) / slots);
-    const double cost = rounds * ((double)((stages + s - 1) / s) + TILE_COST + (s > 1 ? SPLIT_COST : 0));
-    if (s == 1 || cost < least) best = (int)s, least = cost;
-  }
-  return best;
-}
-
+// The device counts the rows that take part, so it decides how tiles are split: the
+// second launch is there wherever it may.
 template <class TL, bool DW>
-void launch_grad(const XentArgs& a, const Product& p, const Out& o, int64_t r0, int64_t N, int64_t stages,
-                 int per_cu, hipStream_t s) {
-  const int64_t tiles = tiles_of(a.D, N, TL::BM, TL::BN), slots = (int64_t)a.n_cu * per_cu;
-  const int splits = splits_of(tiles, stages, slots, mxm_xent_partial_bytes(a.n_cu) / (TL::BM * TL::BN * 4));
-  xent_grad_kernel<TL, DW><<<grid_of(tiles * splits, slots), TL::NT, 0, s>>>(a, p, o, r0, splits);
-  if (splits > 1)
-    xent_grad_join_kernel<TL, DW><<<(unsigned)(tiles * TL::TM * TL::TN), TL::NT, 0, s>>>(a, o, r0, splits);
+void launch_grad(const XentArgs& a, const Product& p, const Out& o, int64_t r0, int64_t N, int per_cu,
+                 hipStream_t s) {
+  const int64_t tiles = tiles_of(a.D, N, TL::BM, TL::BN);
+  const int slots = a.n_cu * per_cu / 8 * 8;
+  const int scratch = (int)(mxm_xent_partial_bytes(a.n_cu) / (TL::BM * TL::BN * 4));
+  xent_grad_kernel<TL, DW><<<(unsigned)slots, TL::NT, 0, s>>>(a, p, o, r0, slots, scratch);
+  const int64_t most = DW ? tiles % slots : std::min<int64_t>(tiles, slots - 1);
+  if (most > 0)
+    xent_grad_join_kernel<TL, DW><<<(unsigned)(most * TL::TM * TL::TN), TL::NT, 0, s>>>(a, p, o, r0, slots, scratch);
 }
 
 }  // namespace
 
 int64_t mxm_xent_partial_bytes(int n_cu) { return (int64_t)n_cu * 2 * 256 * 256 * 4; }
 
-int mxm_xent_block(int64_t rows) {
-  const Shape s = logits_shape(rows);
+int mxm_xent_block(int64_t rows, int V, int n_cu) {
+  const Shape s = logits_shape(rows, V, n_cu);
   return s == FEW ? Few::TM * 32 : s == SMALL ? Small::TM * 32 : Big::TM * 32;
 }
 
-int64_t mxm_xent_stats(int64_t rows, int V) {
-  // (the narrower blocks of fewer rows among them)
+int64_t mxm_xent_stats(int64_t rows, int V, int n_cu) {
+  // the most of any number of rows: 32-wide blocks for up to 32 of them, 64-wide ones
+  // for up to 128 or for half a round of big tiles, 128-wide ones
   const auto of = [&](int64_t n, int block) { return n * ((V + block - 1) / block); };
-  return std::max({of(rows, 128), of(std::min<int64_t>(rows, 128), 64), of(std::min<int64_t>(rows, 32), 32)});
+  const int64_t half = (n_cu / 2) / ((V + Big::BM - 1) / Big::BM) * Big::BN;
+  return std::max({of(rows, 128), of(std::min(rows, std::max<int64_t>(128, half)), 64),
+                   of(std::min<int64_t>(rows, 32), 32)});
 }
 
 void mxm_launch_xent_logits(const XentArgs& a, int64_t r0, int64_t rows, hipStream_t s) {
@@ -658,7 +708,7 @@ void mxm_launch_xent_logits(const XentArgs& a, int64_t r0, int64_t rows, hipStre
   p.a = table(a, true);
   p.b = hidden(a, true);
   p.nk = a.Dp / BK;
-  switch (logits_shape(rows)) {
+  switch (logits_shape(rows, a.V, a.n_cu)) {
     case FEW: return launch_logits<Few>(a, p, r0, rows, 2, s);
     case SMALL: return launch_logits<Small>(a, p, r0, rows, 2, s);
     default: return launch_logits<Big>(a, p, r0, rows, 1, s);
@@ -678,12 +728,12 @@ void mxm_launch_xent_dx(const XentArgs& a, int64_t r0, int64_t rows, hipStream_t
   o.bf16 = a.dx_bf16;
   o.vec = aligned(a.dx) && a.D % (a.dx_bf16 ? 8 : 4) == 0;
   if (a.D <= 128 || rows <= 128)
-    launch_grad<Small, false>(a, p, o, r0, rows, (int64_t)p.nk * p.pairs, 2, s);
+    launch_grad<Small, false>(a, p, o, r0, rows, 2, s);
   else
-    launch_grad<Big, false>(a, p, o, r0, rows, (int64_t)p.nk * p.pairs, 1, s);
+    launch_grad<Big, false>(a, p, o, r0, rows, 1, s);
 }
 
-void mxm_launch_xent_dw(const XentArgs& a, int64_t r0, int64_t rows, bool last, hipStream_t s) {
+void mxm_launch_xent_dw(const XentArgs& a, int64_t r0, bool last, hipStream_t s) {
   Product p{};
   set_planes(a, p);
   p.a = hidden(a, false);
@@ -695,9 +745,8 @@ void mxm_launch_xent_dw(const XentArgs& a, int64_t r0, int64_t rows, bool last, 
   o.add = r0 > 0 ? sums : nullptr;
   o.M = a.D;
   o.vec = aligned(o.out) && a.D % (o.bf16 ? 8 : 4) == 0;
-  const int64_t stages = (rows + BK - 1) / BK * p.pairs;
   if (a.D <= 128 || a.V <= 128)
-    launch_grad<Small, true>(a, p, o, r0, a.V, stages, 2, s);
+    launch_grad<Small, true>(a, p, o, r0, a.V, 2, s);
   else
-    launch_grad<Big, true>(a, p, o, r0, a.V, stages, 1, s);
+    launch_grad<Big, true>(a, p, o, r0, a.V, 1, s);
 }
