@@ -82,7 +82,7 @@ struct XentArgs {
   void *dx, *dw;            // [rows, D], [V, D], or null
   bool backward;
   // workspace
-  int Dp, Vp;               // D and V rounded up to whole stages
+  int Dp, Vp;               // D rounded up to whole stages; V to an odd number of them
   int planes;               // 1 (bf16) or 3
   int32_t* slot;            // [rows] a row's place among those that take part, or -1
   int32_t* map;             // [rows] and back

@@ -252,7 +252,9 @@ int64_t mxm_xent_create(const int64_t* params, int n_params, float softcap, int6
     a.dw_bf16 = params[5] == MXM_DTYPE_BF16;
     const auto up = [](int64_t n) { return (n + 63) / 64 * 64; };
     a.Dp = (int)up(D);
-    a.Vp = (int)up(V);
+    // (rows of the summands an odd number of 128-byte lines apart: a power of two would
+    // put a tile's rows into few memory channels)
+    a.Vp = (int)(up(V) | 64);
     a.planes = a.bf16 ? 1 : 3;
     a.x_rows = std::max<int64_t>(rows, 1);
     // a row's share of the workspace: its blocks' sums, and backwards its summands

@@ -73,6 +73,11 @@ __device__ __forceinline__ void stage_barrier() {
   asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(N) : "memory");
 }
 
+// The barrier alone, this wave's LDS accesses done.
+__device__ __forceinline__ void lds_barrier() {
+  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" : : : "memory");
+}
+
 // BM x BN per workgroup of WM x WN waves, each (BM / WM) x (BN / WN).
 template <int BM_, int BN_, int WM_, int WN_, int NS_, int WPS_>
 struct Tile {
@@ -305,6 +310,65 @@ struct Items {
   }
 };
 
+// A wave's block of 32 n by M = 32 TM m, from the accumulators' layout to whole rows:
+// through LDS of the wave's own (16-byte chunks swizzled by the row), then 16 bytes a
+// lane with M / 8 (of 16 bits) or M / 4 (of 32) lanes to a row.  Stored as they lie in
+// the accumulators, a store instruction covers 32 bytes of 32 rows: at D 544 and 32768
+// entries the logits' tiles took 34 us with such stores.
+template <int TM, int BITS>
+struct Rows {
+  static constexpr int CR = TM * (BITS == 16 ? 4 : 8);  // chunks per row
+  static constexpr int BYTES = 32 * CR * 16;
+  unsigned char* st;
+  int lane;
+  __device__ __forceinline__ void put(int chunk, u32x4_t v) const {
+    const int n = lane & 31;
+    *reinterpret_cast<u32x4_t*>(st + (n * CR + (chunk ^ (n % CR))) * 16) = v;
+  }
+  // f(row, chunk, 16 bytes) for all of the block
+  template <class F>
+  __device__ __forceinline__ void get(F f) const {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll
+    for (int it = 0; it < CR / 2; ++it) {
+      const int row = it * (64 / CR) + lane / CR, c = lane % CR;
+      f(row, c, *reinterpret_cast<const u32x4_t*>(st + (row * CR + (c ^ (row % CR))) * 16));
+    }
+    // (read before the next block is put)
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_wave_barrier();
+  }
+  // The MFMA tile i's values, rounded by pack(a, b) to two 16-bit halves of a word:
+  // quads q and q + 1 of the two half-waves exchanged, 8 consecutive m a lane
+  template <class P>
+  __device__ __forceinline__ void put16(int i, const f32x16_t& c, P pack) const {
+#pragma unroll
+    for (int q = 0; q < 4; q += 2) {
+      uint32_t w[2][2];
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) w[k][h] = pack(c[(q + k) * 4 + 2 * h], c[(q + k) * 4 + 2 * h + 1]);
+      const auto x = __builtin_amdgcn_permlane32_swap(w[0][0], w[1][0], false, false);
+      const auto y = __builtin_amdgcn_permlane32_swap(w[0][1], w[1][1], false, false);
+      put(i * 4 + q + (lane >> 5), u32x4_t{x[0], y[0], x[1], y[1]});
+    }
+  }
+  __device__ __forceinline__ void put32(int i, const f32x16_t& c) const {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const f32x4_t v = {c[q * 4], c[q * 4 + 1], c[q * 4 + 2], c[q * 4 + 3]};
+      put(i * 8 + q * 2 + (lane >> 5), __builtin_bit_cast(u32x4_t, v));
+    }
+  }
+};
+__device__ __forceinline__ uint32_t pack_f16(float a, float b) {
+  const f16x2_t v = {(_Float16)a, (_Float16)b};
+  return __builtin_bit_cast(uint32_t, v);
+}
+
 // ---- logits ----
 
 __device__ __forceinline__ float softcapped(float z, float cap, float inv) {
@@ -398,42 +462,27 @@ __global__ __launch_bounds__(TL::NT, TL::WPS) void xent_logits_kernel(XentArgs a
       if (n < rows && mw < a.V && lane < 32)
         a.stat[(int64_t)(mw / (TM * 32)) * a.stat_ld + n] = make_float2(sum, ref);
       if constexpr (STORE) {
-        const int64_t row = (int64_t)n * a.Vp;
+        constexpr int BITS = PLANES == 1 ? 16 : 32, PER = 128 / BITS;
+        using R = Rows<TM, BITS>;
+        static_assert(TL::NW * R::BYTES <= TL::NS * TL::BUF, "staging fits the ring");
+        const R block{lds + wave * R::BYTES, lane};
 #pragma unroll
         for (int i = 0; i < TM; ++i) {
-          if constexpr (PLANES == 1) {
-            // quads q and q + 1 of the two half-waves exchanged: 8 consecutive entries a lane
-#pragma unroll
-            for (int q = 0; q < 4; q += 2) {
-              uint32_t w[2][2];
-#pragma unroll
-              for (int k = 0; k < 2; ++k)
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                  const f16x2_t v = {(_Float16)acc[i][j][(q + k) * 4 + 2 * h],
-                                     (_Float16)acc[i][j][(q + k) * 4 + 2 * h + 1]};
-                  w[k][h] = __builtin_bit_cast(uint32_t, v);
-                }
-              const auto x = __builtin_amdgcn_permlane32_swap(w[0][0], w[1][0], false, false);
-              const auto y = __builtin_amdgcn_permlane32_swap(w[0][1], w[1][1], false, false);
-              const u32x4_t o = {x[0], y[0], x[1], y[1]};
-              const int m = mw + i * 32 + (q + (lane >> 5)) * 8;
-              if (n < rows && m < a.Vp)
-                *reinterpret_cast<u32x4_t*>(static_cast<uint16_t*>(a.summands) + row + m) = o;
-            }
-          } else {
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              const f32x4_t o = {acc[i][j][q * 4], acc[i][j][q * 4 + 1], acc[i][j][q * 4 + 2],
-                                 acc[i][j][q * 4 + 3]};
-              const int m = first + i * 32 + q * 8;
-              if (n < rows && m < a.Vp)
-                *reinterpret_cast<f32x4_t*>(static_cast<float*>(a.summands) + row + m) = o;
-            }
-          }
+          if constexpr (PLANES == 1)
+            block.put16(i, acc[i][j], pack_f16);
+          else
+            block.put32(i, acc[i][j]);
         }
+        const int nw = n0 + (wn * TN + j) * 32;
+        block.get([&](int row, int c, u32x4_t v) {
+          const int m = mw + c * PER;
+          if (nw + row < rows && m < a.Vp)
+            *reinterpret_cast<u32x4_t*>(static_cast<char*>(a.summands) +
+                                        ((int64_t)(nw + row) * a.Vp + m) * (BITS / 8)) = v;
+        });
       }
     }
+    if constexpr (STORE) lds_barrier();  // before the next tile's loads
   }
 }
 
@@ -720,7 +769,7 @@ void mxm_launch_xent_dx(const XentArgs& a, int64_t r0, int64_t rows, hipStream_t
   set_planes(a, p);
   p.a = table(a, false);
   p.b = grad(a);
-  p.nk = a.Vp / BK;
+  p.nk = (a.V + BK - 1) / BK;
   Out o{};
   o.out = a.dx;
   o.map = a.map + r0;
