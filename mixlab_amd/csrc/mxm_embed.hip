@@ -6,50 +6,53 @@
 
 namespace {
 
-typedef unsigned int u32x4_t __attribute__((ext_vector_type(4)));
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 
-// U elements at p as fp32, U = 8 from 16-byte aligned rows, else 1.
+// U elements at p as fp32: 8 or 4 of rows of whole such units at aligned places, or 1.
 template <int U>
 __device__ __forceinline__ void load_unit(const void* p, bool bf16, int64_t at, float (&v)[U]) {
-  if constexpr (U == 8) {
-    if (bf16) {
-      const u32x4_t q = *reinterpret_cast<const u32x4_t*>(static_cast<const uint16_t*>(p) + at);
+  if constexpr (U == 1) {
+    v[0] = bf16 ? mxm_bf2f(static_cast<const uint16_t*>(p)[at]) : static_cast<const float*>(p)[at];
+  } else if (bf16) {
+    typedef unsigned int words_t __attribute__((ext_vector_type(U / 2)));
+    const words_t q = *reinterpret_cast<const words_t*>(static_cast<const uint16_t*>(p) + at);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        v[2 * i] = mxm_u2f(q[i] << 16);
-        v[2 * i + 1] = mxm_u2f(q[i] & 0xffff0000u);
-      }
-    } else {
-      const f32x4_t* q = reinterpret_cast<const f32x4_t*>(static_cast<const float*>(p) + at);
-      const f32x4_t a = q[0], b = q[1];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = a[i], v[4 + i] = b[i];
+    for (int i = 0; i < U / 2; ++i) {
+      v[2 * i] = mxm_u2f(q[i] << 16);
+      v[2 * i + 1] = mxm_u2f(q[i] & 0xffff0000u);
     }
   } else {
-    v[0] = bf16 ? mxm_bf2f(static_cast<const uint16_t*>(p)[at]) : static_cast<const float*>(p)[at];
+    const f32x4_t* q = reinterpret_cast<const f32x4_t*>(static_cast<const float*>(p) + at);
+#pragma unroll
+    for (int h = 0; h < U / 4; ++h) {
+      const f32x4_t a = q[h];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[4 * h + i] = a[i];
+    }
   }
 }
 template <int U>
 __device__ __forceinline__ void store_unit(void* p, bool bf16, int64_t at, const float (&v)[U]) {
-  if constexpr (U == 8) {
-    if (bf16) {
-      u32x4_t q;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) q[i] = mxm_pack_bf2_fast(v[2 * i], v[2 * i + 1]);
-      *reinterpret_cast<u32x4_t*>(static_cast<uint16_t*>(p) + at) = q;
-    } else {
-      f32x4_t a, b;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) a[i] = v[i], b[i] = v[4 + i];
-      f32x4_t* q = reinterpret_cast<f32x4_t*>(static_cast<float*>(p) + at);
-      q[0] = a;
-      q[1] = b;
-    }
+  if constexpr (U == 1) {
+    if (bf16)
+      static_cast<uint16_t*>(p)[at] = mxm_f2bf_fast(v[0]);
+    else
+      static_cast<float*>(p)[at] = v[0];
   } else if (bf16) {
-    static_cast<uint16_t*>(p)[at] = mxm_f2bf_fast(v[0]);
+    typedef unsigned int words_t __attribute__((ext_vector_type(U / 2)));
+    words_t q;
+#pragma unroll
+    for (int i = 0; i < U / 2; ++i) q[i] = mxm_pack_bf2_fast(v[2 * i], v[2 * i + 1]);
+    __builtin_nontemporal_store(q, reinterpret_cast<words_t*>(static_cast<uint16_t*>(p) + at));
   } else {
-    static_cast<float*>(p)[at] = v[0];
+    f32x4_t* q = reinterpret_cast<f32x4_t*>(static_cast<float*>(p) + at);
+#pragma unroll
+    for (int h = 0; h < U / 4; ++h) {
+      f32x4_t a;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) a[i] = v[4 * h + i];
+      __builtin_nontemporal_store(a, q + h);
+    }
   }
 }
 
@@ -87,13 +90,18 @@ __global__ __launch_bounds__(NT) void embed_kernel(EmbedArgs a, int T) {
 
 // ---- backward: the places sorted by token ----
 //
-// Workgroup o owns the tokens [o * span, (o + 1) * span).  Its waves each walk
-// their own stretch of the tokens twice: counting, per wave, how often each owned
-// token occurs (and how many tokens are smaller than the first owned one, which is
-// where the owned ones start), then writing the owned places in order.
+// Workgroup o owns the tokens [o * span, (o + 1) * span).  Its waves each take their
+// own stretch of the places: they count, per wave, how often each owned token occurs
+// (and how many tokens are smaller than the first owned one, which is where the owned
+// ones start), then write the owned places in order.  What bounds it is the tokens'
+// latency and, where one span holds many of them, their ranks, which are one CU's: 65536
+// places take 18 us of tokens spread evenly over 50257, 30 where token v occurs like
+// 1 / (v + 1) (49 with a ballot per bit of the token instead of the bits' word).  The
+// next batch is loaded while one is worked on; the loops stay rolled (unrolled over 64
+// places a lane, with the tokens kept in registers between the two walks, the code's
+// own way into the instruction cache made it 57 us).
 constexpr int SORT_WAVES = 16;
 constexpr int SORT_SPAN = 512;  // most tokens a workgroup owns
-constexpr int SORT_AHEAD = 4;   // tokens in flight per lane
 
 // LDS written by lanes of this wave is read by other lanes of it afterwards.
 __device__ __forceinline__ void wave_lds_sync() {
@@ -102,45 +110,67 @@ __device__ __forceinline__ void wave_lds_sync() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
+// f(first place, token) for the wave's groups of 64 places in from .. to - 1; behind
+// them ~0.  (As unsigned numbers, tokens below 0 are past the vocabulary.)
+template <int AHEAD, class F>
+__device__ __forceinline__ void each_group(const int32_t* tokens, int64_t from, int64_t to, int lane, F f) {
+  unsigned v[AHEAD];
+  auto fetch = [&](int64_t n) {
+    const int32_t* t = tokens + n + lane;
+    if (n + 64 * AHEAD <= to) {
+#pragma unroll
+      for (int q = 0; q < AHEAD; ++q) v[q] = (unsigned)t[64 * q];
+    } else {
+#pragma unroll
+      for (int q = 0; q < AHEAD; ++q) v[q] = n + 64 * q + lane < to ? (unsigned)t[64 * q] : ~0u;
+    }
+  };
+  fetch(from);
+  for (int64_t n = from; n < to; n += 64 * AHEAD) {
+    unsigned now[AHEAD];
+#pragma unroll
+    for (int q = 0; q < AHEAD; ++q) now[q] = v[q];
+    if (n + 64 * AHEAD < to) fetch(n + 64 * AHEAD);
+#pragma unroll
+    for (int q = 0; q < AHEAD; ++q) f(n + 64 * q, now[q]);
+  }
+}
+
 __global__ __launch_bounds__(64 * SORT_WAVES) void embed_sort_kernel(EmbedArgs a, int span) {
   __shared__ int cnt[SORT_WAVES][SORT_SPAN];
+  __shared__ unsigned long long same[SORT_WAVES][SORT_SPAN];
   __shared__ int tot[SORT_SPAN];
   __shared__ int lower[SORT_WAVES];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int lo = blockIdx.x * span, own = min(span, a.V - lo);
-  for (int i = threadIdx.x; i < SORT_WAVES * SORT_SPAN; i += blockDim.x) (&cnt[0][0])[i] = 0;
-  __syncthreads();
   // stretches of whole groups of 64
-  const int64_t groups = (a.rows + 63) / 64, each = (groups + SORT_WAVES - 1) / SORT_WAVES;
-  const int64_t from = min((int64_t)wave * each * 64, a.rows);
-  const int64_t to = min(from + each * 64, a.rows);
-  int below = 0;
-  for (int64_t n = from; n < to; n += 64 * SORT_AHEAD) {
-    int v[SORT_AHEAD];
-#pragma unroll
-    for (int q = 0; q < SORT_AHEAD; ++q) {
-      const int64_t i = n + 64 * q + lane;
-      v[q] = i < to ? a.tokens[i] : -1;
-    }
-#pragma unroll
-    for (int q = 0; q < SORT_AHEAD; ++q) {
-      below += v[q] >= 0 && v[q] < lo;
-      const unsigned b = (unsigned)v[q] - (unsigned)lo;
-      if (b < (unsigned)own) atomicAdd(&cnt[wave][b], 1);
-    }
+  const int64_t groups = (a.rows + 63) / 64, each = (groups + SORT_WAVES - 1) / SORT_WAVES * 64;
+  const int64_t from = min(wave * each, a.rows), to = min(from + each, a.rows);
+  for (int i = threadIdx.x; i < SORT_WAVES * span; i += blockDim.x) {
+    const int w = i / span, b = i - w * span;
+    cnt[w][b] = 0;
+    same[w][b] = 0;
   }
+  __syncthreads();
+  int below = 0;
+  each_group<16>(a.tokens, from, to, lane, [&](int64_t, unsigned v) {
+    below += v < (unsigned)lo;
+    const unsigned b = v - (unsigned)lo;
+    if (__ballot(b < (unsigned)own) && b < (unsigned)own) atomicAdd(&cnt[wave][b], 1);
+  });
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) below += __shfl_xor(below, o);
   if (lane == 0) lower[wave] = below;
   __syncthreads();
-  // where each wave's first place of each token goes
+  // where each wave's first place of each token goes, within the token's
   for (int b = threadIdx.x; b < own; b += blockDim.x) {
-    int s = 0;
+    int c[SORT_WAVES], s = 0;
+#pragma unroll
+    for (int w = 0; w < SORT_WAVES; ++w) c[w] = cnt[w][b];
 #pragma unroll
     for (int w = 0; w < SORT_WAVES; ++w) {
-      const int c = cnt[w][b];
       cnt[w][b] = s;
-      s += c;
+      s += c[w];
     }
     tot[b] = s;
   }
@@ -166,37 +196,33 @@ __global__ __launch_bounds__(64 * SORT_WAVES) void embed_sort_kernel(EmbedArgs a
     if (lane == 0 && lo + own == a.V) a.starts[a.V] = base;
   }
   __syncthreads();
-  for (int64_t n = from; n < to; n += 64 * SORT_AHEAD) {
-    int v[SORT_AHEAD];
-#pragma unroll
-    for (int q = 0; q < SORT_AHEAD; ++q) {
-      const int64_t i = n + 64 * q + lane;
-      v[q] = i < to ? a.tokens[i] : -1;
-    }
-#pragma unroll
-    for (int q = 0; q < SORT_AHEAD; ++q) {
-      const unsigned b = (unsigned)v[q] - (unsigned)lo;
-      const bool mine = b < (unsigned)own;
-      // the lanes that hold the same token: a ballot per bit of its place in the span
-      unsigned long long same = __ballot(mine);
-      if (!same) continue;
-      for (unsigned bit = 1; bit < (unsigned)span; bit <<= 1) {
-        const bool set = b & bit;
-        const unsigned long long m = __ballot(set);
-        same &= set ? m : ~m;
-      }
-      int left = 0;  // of the first of them: how many there are
-      if (mine) {
-        const unsigned long long before = same & ((1ull << lane) - 1);
-        const int at = tot[b] + cnt[wave][b];
-        a.sorted[at + __popcll(before)] = make_int2((int)(n + 64 * q + lane), v[q]);
-        if (!before) left = __popcll(same);
-      }
-      wave_lds_sync();  // every lane has read its count
-      if (left) cnt[wave][b] += left;
+  each_group<8>(a.tokens, from, to, lane, [&](int64_t n, unsigned v) {
+    const unsigned b = v - (unsigned)lo;
+    const bool mine = b < (unsigned)own;
+    const unsigned long long any = __ballot(mine);
+    if (!any) return;
+    // the lanes that hold the same token: a bit each, in the token's word (64 lanes of one
+    // token would go there one after the other: those need no word)
+    const unsigned lead = __builtin_amdgcn_readlane(b, __builtin_ctzll(any));
+    const bool one = __ballot(mine && b == lead) == any;
+    if (!one) {
+      if (mine) atomicOr(&same[wave][b], 1ull << lane);
       wave_lds_sync();
     }
-  }
+    int before = 0, all = 0;
+    if (mine) {
+      const unsigned long long m = one ? any : same[wave][b];
+      before = __popcll(m & ((1ull << lane) - 1));
+      all = __popcll(m);
+      a.sorted[tot[b] + cnt[wave][b] + before] = make_int2((int)(n + lane), (int)v);
+    }
+    wave_lds_sync();  // every lane has read its word and count
+    if (mine && before == 0) {
+      cnt[wave][b] += all;
+      same[wave][b] = 0;
+    }
+    wave_lds_sync();
+  });
 }
 
 // Sorted places [c * C, (c + 1) * C) per T threads: each run of one token that lies
@@ -214,6 +240,21 @@ __device__ __forceinline__ void put_row(const EmbedArgs& a, int v, int d, float 
     for (int i = 0; i < U; ++i) s[i] += o[i];
   }
   store_unit<U>(a.d_table, a.dtable_bf16, at, s);
+}
+
+// (read again by the join: kept in the caches)
+template <int U>
+__device__ __forceinline__ void store_part(const EmbedArgs& a, int64_t row, int d, const float (&s)[U]) {
+  float* q = a.part + row * a.D + d;
+  if constexpr (U == 1) {
+    q[0] = s[0];
+  } else {
+#pragma unroll
+    for (int h = 0; h < U / 4; ++h) {
+      const f32x4_t v = {s[4 * h], s[4 * h + 1], s[4 * h + 2], s[4 * h + 3]};
+      reinterpret_cast<f32x4_t*>(q)[h] = v;
+    }
+  }
 }
 
 constexpr int AHEAD = 4;  // rows in flight
@@ -239,9 +280,7 @@ __device__ __forceinline__ void sum_chunk(const EmbedArgs& a, int T, int t, int 
         if (p0 + k >= to) break;
         if (e[k].y != v) {
           if (first && a.starts[v] < from) {
-            float* q = a.part + c * 2 * a.D + d;
-#pragma unroll
-            for (int i = 0; i < U; ++i) q[i] = s[i];
+            store_part<U>(a, c * 2, d, s);
           } else {
             put_row<U>(a, v, d, s);
           }
@@ -256,9 +295,7 @@ __device__ __forceinline__ void sum_chunk(const EmbedArgs& a, int T, int t, int 
     }
     const bool before = first && a.starts[v] < from, after = a.starts[v + 1] > to;
     if (before || after) {
-      float* q = a.part + (c * 2 + (before ? 0 : 1)) * a.D + d;
-#pragma unroll
-      for (int i = 0; i < U; ++i) q[i] = s[i];
+      store_part<U>(a, c * 2 + (before ? 0 : 1), d, s);
     } else {
       put_row<U>(a, v, d, s);
     }
@@ -285,6 +322,7 @@ __global__ __launch_bounds__(NT) void embed_sum_kernel(EmbedArgs a, int T, int C
 }
 
 // The run that starts in chunk c and goes on behind it: its sums in order.
+constexpr int JOIN_AHEAD = 16;
 template <int U>
 __device__ __forceinline__ void join_chunk(const EmbedArgs& a, int T, int t, int C, int64_t c, int64_t all) {
   if ((c + 1) * C >= all) return;
@@ -294,16 +332,14 @@ __device__ __forceinline__ void join_chunk(const EmbedArgs& a, int T, int t, int
   const int64_t last = (to - 1) / C;
   for (int d = t * U; d < a.D; d += T * U) {
     float s[U];
-    const float* q = a.part + (c * 2 + 1) * a.D + d;
-#pragma unroll
-    for (int i = 0; i < U; ++i) s[i] = q[i];
+    load_unit<U>(a.part, false, (c * 2 + 1) * a.D + d, s);
     int64_t k = c + 1;
-    for (; k + 8 <= last + 1; k += 8) {
-      float e[8][U];
+    for (; k + JOIN_AHEAD <= last + 1; k += JOIN_AHEAD) {
+      float e[JOIN_AHEAD][U];
 #pragma unroll
-      for (int h = 0; h < 8; ++h) load_unit<U>(a.part, false, (k + h) * 2 * a.D + d, e[h]);
+      for (int h = 0; h < JOIN_AHEAD; ++h) load_unit<U>(a.part, false, (k + h) * 2 * a.D + d, e[h]);
 #pragma unroll
-      for (int h = 0; h < 8; ++h)
+      for (int h = 0; h < JOIN_AHEAD; ++h)
 #pragma unroll
         for (int i = 0; i < U; ++i) s[i] += e[h][i];
     }
@@ -325,7 +361,17 @@ __global__ __launch_bounds__(NT) void embed_join_kernel(EmbedArgs a, int T, int 
     join_chunk<U>(a, T, t, C, c, all);
 }
 
-bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+// Elements per thread and step: 4 where fp32 is among the tensors (16 bytes of it, so
+// that a wave's accesses lie side by side: two halves of 32 bytes a lane took 221 us for
+// a backward's sums of 65536 x 2048, against 197), 8 of bf16 alone, 1 of rows that no
+// aligned unit divides.
+int unit_of(int D, const void* p, bool p_bf16, const void* q, bool q_bf16) {
+  const int u = p_bf16 && q_bf16 ? 8 : 4;
+  const auto fits = [&](const void* at, bool bf16) {
+    return reinterpret_cast<uintptr_t>(at) % (u * (bf16 ? 2 : 4) < 16 ? u * (bf16 ? 2 : 4) : 16) == 0;
+  };
+  return D % u == 0 && fits(p, p_bf16) && fits(q, q_bf16) ? u : 1;
+}
 
 // Threads that walk one row of `units`: the least power of two that covers it, at
 // most a workgroup.
@@ -343,6 +389,14 @@ unsigned grid_of(int64_t items, int per, int n_cu) {
   return (unsigned)std::min<int64_t>((items + per - 1) / per, (int64_t)n_cu * 64);
 }
 
+template <int U>
+void launch_bw(const EmbedArgs& a, hipStream_t s) {
+  const int T = threads_per_row(a.D / U), per = NT / T, C = chunk_rows(a.rows);
+  const int64_t chunks = (a.rows + C - 1) / C, items = chunks + (a.accumulate ? 0 : a.V);
+  if (items > 0) embed_sum_kernel<U><<<grid_of(items, per, a.n_cu), NT, 0, s>>>(a, T, C, chunks, items);
+  if (chunks > 1) embed_join_kernel<U><<<grid_of(chunks, per, a.n_cu), NT, 0, s>>>(a, T, C, chunks);
+}
+
 }  // namespace
 
 int64_t mxm_embed_max_chunks(int64_t max_rows) {
@@ -351,34 +405,26 @@ int64_t mxm_embed_max_chunks(int64_t max_rows) {
 
 void mxm_launch_embed(const EmbedArgs& a, hipStream_t s) {
   if (a.rows == 0) return;
-  const bool wide = a.D % 8 == 0 && aligned(a.table) && aligned(a.out);
-  const int T = threads_per_row(wide ? a.D / 8 : a.D);
+  const int U = unit_of(a.D, a.table, a.table_bf16, a.out, a.out_bf16);
+  const int T = threads_per_row(a.D / U);
   const unsigned grid = grid_of(a.rows, NT / T, a.n_cu);
-  if (wide)
+  if (U == 8)
     embed_kernel<8><<<grid, NT, 0, s>>>(a, T);
+  else if (U == 4)
+    embed_kernel<4><<<grid, NT, 0, s>>>(a, T);
   else
     embed_kernel<1><<<grid, NT, 0, s>>>(a, T);
 }
 
 void mxm_launch_embed_bw(const EmbedArgs& a, hipStream_t s) {
-  const bool wide = a.D % 8 == 0 && aligned(a.d_out) && aligned(a.d_table);
-  const int T = threads_per_row(wide ? a.D / 8 : a.D), per = NT / T;
   const int span = std::min(SORT_SPAN, std::max(16, (a.V + a.n_cu - 1) / a.n_cu));
-  embed_sort_kernel<<<(a.V + span - 1) / span, 64 * SORT_WAVES, 0, s>>>(a, span);
-  const int C = chunk_rows(a.rows);
-  const int64_t chunks = (a.rows + C - 1) / C, items = chunks + (a.accumulate ? 0 : a.V);
-  if (items > 0) {
-    const unsigned grid = grid_of(items, per, a.n_cu);
-    if (wide)
-      embed_sum_kernel<8><<<grid, NT, 0, s>>>(a, T, C, chunks, items);
-    else
-      embed_sum_kernel<1><<<grid, NT, 0, s>>>(a, T, C, chunks, items);
-  }
-  if (chunks > 1) {
-    const unsigned grid = grid_of(chunks, per, a.n_cu);
-    if (wide)
-      embed_join_kernel<8><<<grid, NT, 0, s>>>(a, T, C, chunks);
-    else
-      embed_join_kernel<1><<<grid, NT, 0, s>>>(a, T, C, chunks);
-  }
+  const unsigned grid = (unsigned)((a.V + span - 1) / span);
+  embed_sort_kernel<<<grid, 64 * SORT_WAVES, 0, s>>>(a, span);
+  const int U = unit_of(a.D, a.d_out, a.grad_bf16, a.d_table, a.dtable_bf16);
+  if (U == 8)
+    launch_bw<8>(a, s);
+  else if (U == 4)
+    launch_bw<4>(a, s);
+  else
+    launch_bw<1>(a, s);
 }

@@ -138,17 +138,24 @@ __device__ __forceinline__ bool wide_rows(const XentArgs& a, const void* p) {
   return a.D % 8 == 0 && (reinterpret_cast<uintptr_t>(p) & 15) == 0;
 }
 
-// x's rows that take part to their places, and dx's others to zeros; a wave per row.
+// x's rows that take part to their places, dx's others to zeros; a wave per row.
 // PLAN: for up to PLAN_ROWS rows, every workgroup counts those before its own, and the
 // plan's launch is saved.
 constexpr int PLAN_ROWS = 1024;
+// The workgroups behind the first x_blocks pack the table.
 template <bool PLAN>
-__global__ __launch_bounds__(NT) void xent_pack_x_kernel(XentArgs a) {
+__global__ __launch_bounds__(NT) void xent_pack_kernel(XentArgs a, int x_blocks) {
   __shared__ int count[2][4];
   __shared__ double weight[4];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  if ((int)blockIdx.x >= x_blocks) {
+    const bool wide = wide_rows(a, a.weight);
+    for (int64_t v = (int64_t)(blockIdx.x - x_blocks) * 4 + wave; v < a.V; v += (int64_t)(gridDim.x - x_blocks) * 4)
+      pack_row(a, a.weight, wide, v, a.w_pack, a.V, v, lane, 64);
+    return;
+  }
   const bool wide = wide_rows(a, a.x);
-  for (int64_t first = (int64_t)blockIdx.x * 4; first < a.rows; first += (int64_t)gridDim.x * 4) {
+  for (int64_t first = (int64_t)blockIdx.x * 4; first < a.rows; first += (int64_t)x_blocks * 4) {
     const int64_t n = first + wave;
     int to = -1;
     if constexpr (PLAN) {
@@ -209,13 +216,6 @@ __global__ __launch_bounds__(NT) void xent_pack_x_kernel(XentArgs a) {
       }
     }
   }
-}
-
-__global__ __launch_bounds__(NT) void xent_pack_w_kernel(XentArgs a) {
-  const int lane = threadIdx.x & 63;
-  const bool wide = wide_rows(a, a.weight);
-  for (int64_t v = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); v < a.V; v += (int64_t)gridDim.x * 4)
-    pack_row(a, a.weight, wide, v, a.w_pack, a.V, v, lane, 64);
 }
 
 // What a set of exponentials sums to: sum * 2^top.
@@ -393,11 +393,11 @@ void mxm_launch_xent(const XentArgs& a0, hipStream_t s) {
   const bool plan = a.rows > 0 && a.rows <= PLAN_ROWS;
   if (!plan) xent_plan_kernel<<<1, PLAN_NT, 0, s>>>(a);
   if (a.rows > 0) {
+    const unsigned gx = rows_grid(a.rows), gw = a.w_direct ? 0 : rows_grid(a.V);
     if (plan)
-      xent_pack_x_kernel<true><<<rows_grid(a.rows), NT, 0, s>>>(a);
+      xent_pack_kernel<true><<<gx + gw, NT, 0, s>>>(a, (int)gx);
     else
-      xent_pack_x_kernel<false><<<rows_grid(a.rows), NT, 0, s>>>(a);
-    if (!a.w_direct) xent_pack_w_kernel<<<rows_grid(a.V), NT, 0, s>>>(a);
+      xent_pack_kernel<false><<<gx + gw, NT, 0, s>>>(a, (int)gx);
   }
   const int64_t pieces = std::max<int64_t>(1, (a.rows + a.piece_rows - 1) / a.piece_rows);
   const bool total_there = a.total && a.rows > 0 && a.rows <= JOIN_WAVES;  // (one piece)

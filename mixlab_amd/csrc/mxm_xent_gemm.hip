@@ -451,8 +451,9 @@ __global__ __launch_bounds__(TL::NT, TL::WPS) void xent_logits_kernel(XentArgs a
           s[r & 1] += e;
           if constexpr (STORE) {
             if (cap > 0.0f) {
-              const float u = l * inv;
-              e *= l > -3.0e38f ? 1.0f - u * u : 0.0f;
+              // (a masked logit counts as -cap: a factor of 0)
+              const float u = fmaxf(l * inv, -1.0f);
+              e *= fmaf(-u, u, 1.0f);
             }
             acc[i][j][r] = e;
           }
@@ -620,7 +621,7 @@ __global__ __launch_bounds__(TL::NT, TL::WPS) void xent_grad_kernel(XentArgs a, 
 template <class TL, bool DW>
 __global__ __launch_bounds__(TL::NT) void xent_grad_join_kernel(XentArgs a, Product p, Out o, int64_t r0,
                                                                 int slots, int scratch_tiles) {
-  constexpr int TM = TL::TM, TN = TL::TN, AHEAD = 4;
+  constexpr int TM = TL::TM, TN = TL::TN, AHEAD = 8;
   fit<DW>(a, p, r0);
   const int N = DW ? a.V : p.b.rows;
   const int mt = (a.D + TL::BM - 1) / TL::BM, nt = (N + TL::BN - 1) / TL::BN;
