@@ -31,6 +31,29 @@ __device__ __forceinline__ void load_unit(const void* p, bool bf16, int64_t at, 
     }
   }
 }
+// (rows of gradients are read once)
+template <int U>
+__device__ __forceinline__ void load_once(const void* p, bool bf16, int64_t at, float (&v)[U]) {
+  if constexpr (U == 1) {
+    load_unit<U>(p, bf16, at, v);
+  } else if (bf16) {
+    typedef unsigned int words_t __attribute__((ext_vector_type(U / 2)));
+    const words_t q = __builtin_nontemporal_load(reinterpret_cast<const words_t*>(static_cast<const uint16_t*>(p) + at));
+#pragma unroll
+    for (int i = 0; i < U / 2; ++i) {
+      v[2 * i] = mxm_u2f(q[i] << 16);
+      v[2 * i + 1] = mxm_u2f(q[i] & 0xffff0000u);
+    }
+  } else {
+    const f32x4_t* q = reinterpret_cast<const f32x4_t*>(static_cast<const float*>(p) + at);
+#pragma unroll
+    for (int h = 0; h < U / 4; ++h) {
+      const f32x4_t a = __builtin_nontemporal_load(q + h);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[4 * h + i] = a[i];
+    }
+  }
+}
 template <int U>
 __device__ __forceinline__ void store_unit(void* p, bool bf16, int64_t at, const float (&v)[U]) {
   if constexpr (U == 1) {
@@ -100,8 +123,8 @@ __global__ __launch_bounds__(NT) void embed_kernel(EmbedArgs a, int T) {
 // next batch is loaded while one is worked on; the loops stay rolled (unrolled over 64
 // places a lane, with the tokens kept in registers between the two walks, the code's
 // own way into the instruction cache made it 57 us).
-constexpr int SORT_WAVES = 16;
-constexpr int SORT_SPAN = 512;  // most tokens a workgroup owns
+constexpr int SORT_SPAN = 512;    // most tokens a workgroup owns
+constexpr int SORT_FEW = 2048;    // places up to which it has 4 waves, not 16
 
 // LDS written by lanes of this wave is read by other lanes of it afterwards.
 __device__ __forceinline__ void wave_lds_sync() {
@@ -136,6 +159,7 @@ __device__ __forceinline__ void each_group(const int32_t* tokens, int64_t from, 
   }
 }
 
+template <int SORT_WAVES>
 __global__ __launch_bounds__(64 * SORT_WAVES) void embed_sort_kernel(EmbedArgs a, int span) {
   __shared__ int cnt[SORT_WAVES][SORT_SPAN];
   __shared__ unsigned long long same[SORT_WAVES][SORT_SPAN];
@@ -227,7 +251,7 @@ __global__ __launch_bounds__(64 * SORT_WAVES) void embed_sort_kernel(EmbedArgs a
 
 // Sorted places [c * C, (c + 1) * C) per T threads: each run of one token that lies
 // within them to the table, the first and last run's sums to part where they go on
-// outside.  Workgroups behind the chunks': zeros for the tokens that occur nowhere.
+// outside.
 template <int U>
 __device__ __forceinline__ void put_row(const EmbedArgs& a, int v, int d, float (&s)[U]) {
 #pragma unroll
@@ -257,7 +281,7 @@ __device__ __forceinline__ void store_part(const EmbedArgs& a, int64_t row, int 
   }
 }
 
-constexpr int AHEAD = 4;  // rows in flight
+constexpr int AHEAD = 8;  // rows in flight
 template <int U>
 __device__ __forceinline__ void sum_chunk(const EmbedArgs& a, int T, int t, int C, int64_t c, int64_t all) {
   const int64_t from = c * C, to = min(from + C, all);
@@ -274,7 +298,7 @@ __device__ __forceinline__ void sum_chunk(const EmbedArgs& a, int T, int t, int 
 #pragma unroll
       for (int k = 0; k < AHEAD; ++k) e[k] = a.sorted[min(p0 + k, to - 1)];
 #pragma unroll
-      for (int k = 0; k < AHEAD; ++k) load_unit<U>(a.d_out, a.grad_bf16, (int64_t)e[k].x * a.D + d, g[k]);
+      for (int k = 0; k < AHEAD; ++k) load_once<U>(a.d_out, a.grad_bf16, (int64_t)e[k].x * a.D + d, g[k]);
 #pragma unroll
       for (int k = 0; k < AHEAD; ++k) {
         if (p0 + k >= to) break;
@@ -303,22 +327,11 @@ __device__ __forceinline__ void sum_chunk(const EmbedArgs& a, int T, int t, int 
 }
 
 template <int U>
-__global__ __launch_bounds__(NT) void embed_sum_kernel(EmbedArgs a, int T, int C, int64_t chunks,
-                                                       int64_t items) {
+__global__ __launch_bounds__(NT) void embed_sum_kernel(EmbedArgs a, int T, int C, int64_t chunks) {
   const int per = NT / T, sub = threadIdx.x / T, t = threadIdx.x % T;
   const int64_t all = a.starts[a.V];
-  for (int64_t i = (int64_t)blockIdx.x * per + sub; i < items; i += (int64_t)gridDim.x * per) {
-    if (i < chunks) {
-      sum_chunk<U>(a, T, t, C, i, all);
-    } else {
-      const int64_t v = i - chunks;
-      if (a.starts[v] != a.starts[v + 1]) continue;
-      float z[U];
-#pragma unroll
-      for (int k = 0; k < U; ++k) z[k] = 0.0f;
-      for (int d = t * U; d < a.D; d += T * U) store_unit<U>(a.d_table, a.dtable_bf16, v * a.D + d, z);
-    }
-  }
+  for (int64_t c = (int64_t)blockIdx.x * per + sub; c < chunks; c += (int64_t)gridDim.x * per)
+    sum_chunk<U>(a, T, t, C, c, all);
 }
 
 // The run that starts in chunk c and goes on behind it: its sums in order.
@@ -353,12 +366,24 @@ __device__ __forceinline__ void join_chunk(const EmbedArgs& a, int T, int t, int
   }
 }
 
+// The runs over several chunks, then zeros for the tokens that occur nowhere (behind the
+// runs, whose partials come one after the other: a launch of theirs took 15 us more).
 template <int U>
-__global__ __launch_bounds__(NT) void embed_join_kernel(EmbedArgs a, int T, int C, int64_t chunks) {
+__global__ __launch_bounds__(NT) void embed_join_kernel(EmbedArgs a, int T, int C, int64_t joins, int64_t items) {
   const int per = NT / T, sub = threadIdx.x / T, t = threadIdx.x % T;
   const int64_t all = a.starts[a.V];
-  for (int64_t c = (int64_t)blockIdx.x * per + sub; c < chunks; c += (int64_t)gridDim.x * per)
-    join_chunk<U>(a, T, t, C, c, all);
+  for (int64_t i = (int64_t)blockIdx.x * per + sub; i < items; i += (int64_t)gridDim.x * per) {
+    if (i < joins) {
+      join_chunk<U>(a, T, t, C, i, all);
+    } else {
+      const int64_t v = i - joins;
+      if (a.starts[v] != a.starts[v + 1]) continue;
+      float z[U];
+#pragma unroll
+      for (int k = 0; k < U; ++k) z[k] = 0.0f;
+      for (int d = t * U; d < a.D; d += T * U) store_unit<U>(a.d_table, a.dtable_bf16, v * a.D + d, z);
+    }
+  }
 }
 
 // Elements per thread and step: 4 where fp32 is among the tensors (16 bytes of it, so
@@ -392,9 +417,10 @@ unsigned grid_of(int64_t items, int per, int n_cu) {
 template <int U>
 void launch_bw(const EmbedArgs& a, hipStream_t s) {
   const int T = threads_per_row(a.D / U), per = NT / T, C = chunk_rows(a.rows);
-  const int64_t chunks = (a.rows + C - 1) / C, items = chunks + (a.accumulate ? 0 : a.V);
-  if (items > 0) embed_sum_kernel<U><<<grid_of(items, per, a.n_cu), NT, 0, s>>>(a, T, C, chunks, items);
-  if (chunks > 1) embed_join_kernel<U><<<grid_of(chunks, per, a.n_cu), NT, 0, s>>>(a, T, C, chunks);
+  const int64_t chunks = (a.rows + C - 1) / C, joins = chunks > 1 ? chunks - 1 : 0;
+  const int64_t items = joins + (a.accumulate ? 0 : a.V);
+  if (chunks > 0) embed_sum_kernel<U><<<grid_of(chunks, per, a.n_cu), NT, 0, s>>>(a, T, C, chunks);
+  if (items > 0) embed_join_kernel<U><<<grid_of(items, per, a.n_cu), NT, 0, s>>>(a, T, C, joins, items);
 }
 
 }  // namespace
@@ -419,7 +445,10 @@ void mxm_launch_embed(const EmbedArgs& a, hipStream_t s) {
 void mxm_launch_embed_bw(const EmbedArgs& a, hipStream_t s) {
   const int span = std::min(SORT_SPAN, std::max(16, (a.V + a.n_cu - 1) / a.n_cu));
   const unsigned grid = (unsigned)((a.V + span - 1) / span);
-  embed_sort_kernel<<<grid, 64 * SORT_WAVES, 0, s>>>(a, span);
+  if (a.rows <= SORT_FEW)
+    embed_sort_kernel<4><<<grid, 256, 0, s>>>(a, span);
+  else
+    embed_sort_kernel<16><<<grid, 1024, 0, s>>>(a, span);
   const int U = unit_of(a.D, a.d_out, a.grad_bf16, a.d_table, a.dtable_bf16);
   if (U == 8)
     launch_bw<8>(a, s);
