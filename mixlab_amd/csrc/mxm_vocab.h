@@ -46,25 +46,42 @@ int64_t mxm_embed_max_chunks(int64_t max_rows);
 //   g_n = d_total w_n                    (mean: / sum_n w_n)
 //   dz = g (softmax(l) - [v = t]) (1 - (l / cap)^2),  dx = dz W,  dW = dz^T x
 // The rows that take part are packed (in order) into x_pack, zero-padded to whole
-// 64-wide stages; under fp32 as three bf16 planes hi, mid and lo whose sum is the
-// value, and a product of two values as the six products of planes that matter.
-// Then, for a piece of these rows at a time:
+// 64-wide stages.
+//
+// fp32 operands become two fp16 planes: a row of x or weight is 2^exp (hi + lo) with
+// its largest element's hi in [2^14, 2^15), 22 bits of every element down to 2^-17 of
+// the largest and 2^-40 of the largest below.  Products of two such operands are
+// hi lo + lo hi + hi hi (lo lo is below 2^-23 of the product), each exact in fp32.
+// Exponents of rows along m or n of a product are applied to its sums; along k they
+// have to agree:  with E_n from the row's largest |dz| and W_v = 2^w_v W'_v
+//   dz'[n, v] = dz 2^(w_v - E_n),  dx = 2^E_n dz' W'
+//   x''_n = x'_n 2^(E_n + X_n - C),  dW_v = 2^(C - w_v) dz'^T x'',  C = max_n (E_n + X_n)
+// so that dW's terms keep 2^-40 of the largest row's, however small their own is.
+// A row of weight with infinite elements is its infinities' signs and the exponent
+// XENT_INF.
+//
+// Then, for a piece of the rows that take part at a time:
 //   product 1 (mxm_xent_gemm.hip): logits of a tile of vocabulary x rows in the
 //     accumulators; of each row and block of the vocabulary the sum over v != t of
 //     2^(l log2 e - ref) with a whole-number ref of the block; backwards also each
 //     summand (times 1 - (l / cap)^2), relative to that ref;
 //   join (mxm_xent.hip): each row's loss and the factors of its gradient;
-//   finish: the summands to dz, in place (fp32: to three planes);
+//   finish: the summands to dz, in place (fp32: to planes; x' to x'');
 //   product 2: dx = dz W;  product 3: dW (+)= dz^T x.
 struct XentScalars {
   double weight_sum;        // of the rows that take part
   int32_t rows;             // that take part
+  int32_t dw_exp;           // C
 };
+constexpr int XENT_INF = 1 << 20;
+constexpr int XENT_NO_EXP = -(1 << 20);  // of no row
 struct XentRow {            // of a row that takes part
   float ref;                // M: the summands' common exponent
   float scale;              // g / sum of all 2^(l log2 e - M)
   float at_target;          // dz of the target
   int32_t target;
+  int32_t exp;              // E (fp32)
+  int32_t x_factor;         // E + X, XENT_NO_EXP for a row without a gradient
 };
 struct XentArgs {
   int64_t rows;
@@ -83,7 +100,7 @@ struct XentArgs {
   bool backward;
   // workspace
   int Dp, Vp;               // D rounded up to whole stages; V to an odd number of them
-  int planes;               // 1 (bf16) or 3
+  int planes;               // 1 (bf16) or 2 (fp32)
   int32_t* slot;            // [rows] a row's place among those that take part, or -1
   int32_t* map;             // [rows] and back
   int32_t* target;          // [rows] of those that take part
@@ -95,6 +112,9 @@ struct XentArgs {
   int64_t x_rows;
   uint16_t* w_pack;         // [planes][V][Dp], unused where weight is read in place
   bool w_direct;            // weight itself: bf16 rows of whole 16 bytes
+  int32_t *x_exp, *w_exp;   // [rows], [V up to whole tiles]: X, w (fp32)
+  int32_t *w_part, *c_part; // the largest of w and of E + X of each workgroup that packs
+  int w_parts, c_parts;     // the table, or joins rows
   float2* stat;             // [blocks][stat_ld]: sum, ref
   void* summands;           // [piece_rows][Vp]: fp16 (bf16) or fp32
   uint16_t* dz;             // [planes][piece_rows][Vp]: the summands' place under bf16
@@ -104,6 +124,7 @@ struct XentArgs {
   int64_t piece_rows, stat_ld;
   int n_cu;
 };
+constexpr int XENT_W_PARTS = 4096;  // most workgroups that pack the table
 // Bytes of partial, for handles that run backward.
 int64_t mxm_xent_partial_bytes(int n_cu);
 // Most blocks of stat times rows, for pieces of `rows`.

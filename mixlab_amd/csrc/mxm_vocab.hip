@@ -26,7 +26,7 @@ struct Xent : TrainHandle {
   XentArgs base{};
   int64_t max_rows = 0;
   bool backward = false;
-  DevBuf slot, map, target, scalars, nll, at_target, row, x_pack, w_pack, stat, summands, dz, partial, dw32, zeros;
+  DevBuf slot, map, target, scalars, nll, at_target, row, x_pack, w_pack, exps, stat, summands, dz, partial, dw32, zeros;
   ~Xent() override {
     if (stream_ref) (void)hipStreamSynchronize(stream());
   }
@@ -255,13 +255,13 @@ int64_t mxm_xent_create(const int64_t* params, int n_params, float softcap, int6
     // (rows of the summands an odd number of 128-byte lines apart: a power of two would
     // put a tile's rows into few memory channels)
     a.Vp = (int)(up(V) | 64);
-    a.planes = a.bf16 ? 1 : 3;
+    a.planes = a.bf16 ? 1 : 2;
     a.x_rows = std::max<int64_t>(rows, 1);
     // a row's share of the workspace: its blocks' sums, and backwards its summands
     // (and under fp32 their gradient's planes)
     int64_t bytes = XENT_PIECE_BYTES;
     if (const char* env = std::getenv("MXM_XENT_PIECE_BYTES")) bytes = std::max(0ll, std::atoll(env));
-    const int64_t row_bytes = (V + 127) / 128 * 8 + (x->backward ? a.Vp * (int64_t)(a.bf16 ? 2 : 10) : 0);
+    const int64_t row_bytes = (V + 127) / 128 * 8 + (x->backward ? a.Vp * (int64_t)(a.bf16 ? 2 : 8) : 0);
     a.piece_rows = std::max<int64_t>(256, std::min(up(rows), bytes / row_bytes / 256 * 256));
     if (rows < a.piece_rows) a.piece_rows = std::max<int64_t>(64, up(rows));
     x->slot.alloc((size_t)rows * 4);
@@ -273,6 +273,14 @@ int64_t mxm_xent_create(const int64_t* params, int n_params, float softcap, int6
     x->x_pack.alloc((size_t)a.x_rows * a.Dp * 2 * a.planes);
     x->w_pack.alloc((size_t)V * a.Dp * 2 * a.planes);
     x->stat.alloc((size_t)mxm_xent_stats(a.piece_rows, a.V, a.n_cu) * sizeof(float2));
+    if (!a.bf16) {
+      const size_t v_tiles = ((size_t)V + 255) / 256 * 256, n = (size_t)rows, joins = (size_t)rows / 16 + 1;
+      x->exps.alloc((n + v_tiles + XENT_W_PARTS + joins) * 4 + 64);
+      a.w_exp = x->exps.as<int32_t>();  // (first: read by vectors)
+      a.x_exp = a.w_exp + v_tiles;
+      a.w_part = a.x_exp + n;
+      a.c_part = a.w_part + XENT_W_PARTS;
+    }
     x->zeros.alloc(4096);
     HIPCK(hipMemsetAsync(x->zeros.p, 0, 4096, x->stream()));
     a.slot = x->slot.as<int32_t>();
@@ -289,7 +297,7 @@ int64_t mxm_xent_create(const int64_t* params, int n_params, float softcap, int6
       const size_t cells = (size_t)a.piece_rows * (size_t)a.Vp;
       x->row.alloc((size_t)rows * sizeof(XentRow));
       x->summands.alloc(cells * (a.bf16 ? 2 : 4));
-      if (!a.bf16) x->dz.alloc(cells * 6);
+      if (!a.bf16) x->dz.alloc(cells * 4);
       x->partial.alloc((size_t)mxm_xent_partial_bytes(a.n_cu));
       if (a.dw_bf16 && rows > a.piece_rows) x->dw32.alloc((size_t)V * (size_t)D * 4);
       a.row = x->row.as<XentRow>();

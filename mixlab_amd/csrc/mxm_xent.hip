@@ -9,6 +9,7 @@ namespace {
 typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 typedef unsigned int u32x4_t __attribute__((ext_vector_type(4)));
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
+typedef int i32x4_t __attribute__((ext_vector_type(4)));
 
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
@@ -68,70 +69,109 @@ __global__ __launch_bounds__(PLAN_NT) void xent_plan_kernel(XentArgs a) {
   }
 }
 
-// v as hi + mid + lo, each a bf16: 24 bits, all of v's.  The differences are exact.
-// Infinities become the largest bf16 (an infinite plane times another operand's
-// mid plane, of any sign or zero, would make a NaN of every product).
-__device__ __forceinline__ void planes3(float v, uint16_t& hi, uint16_t& mid, uint16_t& lo) {
-  const float c = v != v ? v : fminf(fmaxf(v, -3.3895313892515355e38f), 3.3895313892515355e38f);
-  hi = mxm_f2bf_fast(c);
-  const float r = c - mxm_bf2f(hi);
-  mid = mxm_f2bf_fast(r);
-  lo = mxm_f2bf_fast(r - mxm_bf2f(mid));
+// v as hi + lo of fp16 (the difference is exact; an infinity has no lo).
+__device__ __forceinline__ void planes2(float v, uint16_t& hi, uint16_t& lo) {
+  const _Float16 h = (_Float16)v;
+  const _Float16 l = (_Float16)(__builtin_isinf((float)h) ? 0.0f : v - (float)h);
+  hi = __builtin_bit_cast(uint16_t, h);
+  lo = __builtin_bit_cast(uint16_t, l);
 }
-
-__device__ __forceinline__ void planes3x8(const float (&v)[8], u32x4_t (&q)[3]) {
-  uint16_t p[3][8];
+__device__ __forceinline__ void planes2x8(const float (&v)[8], u32x4_t (&q)[2]) {
+  uint16_t p[2][8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) planes3(v[i], p[0][i], p[1][i], p[2][i]);
+  for (int i = 0; i < 8; ++i) planes2(v[i], p[0][i], p[1][i]);
 #pragma unroll
-  for (int k = 0; k < 3; ++k)
+  for (int k = 0; k < 2; ++k)
 #pragma unroll
     for (int i = 0; i < 4; ++i) q[k][i] = p[k][2 * i] | (uint32_t)p[k][2 * i + 1] << 16;
 }
 
 constexpr int NT = 256;
 
-// Row `src` of x or weight to row `to` of its pack of `rows` rows, zeros behind D, by
-// T threads; wide: rows of whole aligned 16 bytes.
+// Row `src` of x or weight to row `to` of its pack of `rows` rows, zeros behind D, by a
+// wave; wide: rows of whole aligned 16 bytes.
 __device__ __forceinline__ void pack_row(const XentArgs& a, const void* p, bool wide, int64_t src,
-                                         uint16_t* pack, int64_t rows, int64_t to, int t, int T) {
-  const int64_t plane = rows * a.Dp;
+                                         uint16_t* pack, int64_t to, int lane) {
+  const uint16_t* from = static_cast<const uint16_t*>(p) + src * a.D;
+  pack += to * a.Dp;
   if (wide) {
-    for (int d = t * 8; d < a.Dp; d += T * 8) {
-      const int64_t at = to * a.Dp + d;
-      const u32x4_t none = {0, 0, 0, 0};
-      if (a.planes == 1) {
-        u32x4_t q = none;
-        if (d < a.D) q = *reinterpret_cast<const u32x4_t*>(static_cast<const uint16_t*>(p) + src * a.D + d);
-        *reinterpret_cast<u32x4_t*>(pack + at) = q;
-      } else {
-        u32x4_t q[3] = {none, none, none};
-        if (d < a.D) {
-          const f32x4_t* f = reinterpret_cast<const f32x4_t*>(static_cast<const float*>(p) + src * a.D + d);
-          const f32x4_t lo = f[0], hi = f[1];
-          float v[8];
+    for (int d = lane * 8; d < a.Dp; d += 512) {
+      u32x4_t q = {0, 0, 0, 0};
+      if (d < a.D) q = *reinterpret_cast<const u32x4_t*>(from + d);
+      *reinterpret_cast<u32x4_t*>(pack + d) = q;
+    }
+  } else {
+    for (int d = lane; d < a.Dp; d += 64) pack[d] = d < a.D ? from[d] : (uint16_t)0;
+  }
+}
+
+// The same of an fp32 row, to planes; returns its exponent.
+template <bool WEIGHT>
+__device__ __forceinline__ int pack_row32(const XentArgs& a, const void* p, bool wide, int64_t src,
+                                          uint16_t* pack, int64_t rows, int64_t to, int lane) {
+  const float* from = static_cast<const float*>(p) + src * a.D;
+  const int64_t plane = rows * a.Dp;
+  pack += to * a.Dp;
+  // the largest finite element (of their bits, which are ordered alike), any infinity
+  uint32_t top = 0;
+  bool inf = false;
+  auto look = [&](float v) {
+    const uint32_t u = mxm_f2u(v) & 0x7fffffffu;
+    if (u < 0x7f800000u) top = max(top, u);
+    inf |= u == 0x7f800000u;
+  };
+  if (wide) {
+    for (int d = lane * 4; d < a.D; d += 256) {
+      const f32x4_t v = *reinterpret_cast<const f32x4_t*>(from + d);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) v[i] = lo[i], v[4 + i] = hi[i];
-          planes3x8(v, q);
-        }
+      for (int i = 0; i < 4; ++i) look(v[i]);
+    }
+  } else {
+    for (int d = lane; d < a.D; d += 64) look(from[d]);
+  }
 #pragma unroll
-        for (int k = 0; k < 3; ++k) *reinterpret_cast<u32x4_t*>(pack + at + k * plane) = q[k];
+  for (int o = 32; o > 0; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o));
+  const bool signs = WEIGHT && __ballot(inf) != 0;
+  int e = 0;
+  if (top != 0) {
+    (void)frexpf(mxm_u2f(top), &e);
+    e = max(e - 15, -126);
+  }
+  auto scaled = [&](float v) {
+    if (!signs) return ldexpf(v, -e);
+    return v != v ? v : __builtin_isinf(v) ? __builtin_copysignf(1.0f, v) : 0.0f;
+  };
+  if (wide) {
+    for (int d = lane * 8; d < a.Dp; d += 512) {
+      float v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+      if (d < a.D) {
+        const f32x4_t* f = reinterpret_cast<const f32x4_t*>(from + d);
+        const f32x4_t lo = f[0], hi = f[1];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = scaled(lo[i]), v[4 + i] = scaled(hi[i]);
       }
+      u32x4_t q[2];
+      planes2x8(v, q);
+      *reinterpret_cast<u32x4_t*>(pack + d) = q[0];
+      *reinterpret_cast<u32x4_t*>(pack + plane + d) = q[1];
     }
-    return;
-  }
-  for (int d = t; d < a.Dp; d += T) {
-    const int64_t at = to * a.Dp + d;
-    if (a.planes == 1) {
-      pack[at] = d < a.D ? static_cast<const uint16_t*>(p)[src * a.D + d] : (uint16_t)0;
-    } else {
-      uint16_t hi = 0, mid = 0, lo = 0;
-      if (d < a.D) planes3(static_cast<const float*>(p)[src * a.D + d], hi, mid, lo);
-      pack[at] = hi;
-      pack[at + plane] = mid;
-      pack[at + 2 * plane] = lo;
+  } else {
+    for (int d = lane; d < a.Dp; d += 64) {
+      uint16_t hi, lo;
+      planes2(d < a.D ? scaled(from[d]) : 0.0f, hi, lo);
+      pack[d] = hi;
+      pack[plane + d] = lo;
     }
   }
+  return signs ? XENT_INF : e;
+}
+
+__device__ __forceinline__ int wave_max(int v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v = max(v, __shfl_xor(v, o));
+  return v;
 }
 
 __device__ __forceinline__ bool wide_rows(const XentArgs& a, const void* p) {
@@ -150,8 +190,22 @@ __global__ __launch_bounds__(NT) void xent_pack_kernel(XentArgs a, int x_blocks)
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   if ((int)blockIdx.x >= x_blocks) {
     const bool wide = wide_rows(a, a.weight);
-    for (int64_t v = (int64_t)(blockIdx.x - x_blocks) * 4 + wave; v < a.V; v += (int64_t)(gridDim.x - x_blocks) * 4)
-      pack_row(a, a.weight, wide, v, a.w_pack, a.V, v, lane, 64);
+    int most = XENT_NO_EXP;
+    for (int64_t v = (int64_t)(blockIdx.x - x_blocks) * 4 + wave; v < a.V; v += (int64_t)(gridDim.x - x_blocks) * 4) {
+      if (a.planes == 1) {
+        pack_row(a, a.weight, wide, v, a.w_pack, v, lane);
+      } else {
+        const int e = pack_row32<true>(a, a.weight, wide, v, a.w_pack, a.V, v, lane);
+        if (lane == 0) a.w_exp[v] = e;
+        if (e < XENT_INF) most = max(most, e);
+      }
+    }
+    if (a.planes != 1) {
+      if (lane == 0) count[0][wave] = most;
+      __syncthreads();
+      if (threadIdx.x == 0)
+        a.w_part[blockIdx.x - x_blocks] = max(max(count[0][0], count[0][1]), max(count[0][2], count[0][3]));
+    }
     return;
   }
   const bool wide = wide_rows(a, a.x);
@@ -206,7 +260,12 @@ __global__ __launch_bounds__(NT) void xent_pack_kernel(XentArgs a, int x_blocks)
     }
     if (n >= a.rows) continue;
     if (to >= 0) {
-      pack_row(a, a.x, wide, n, a.x_pack, a.x_rows, to, lane, 64);
+      if (a.planes == 1) {
+        pack_row(a, a.x, wide, n, a.x_pack, to, lane);
+      } else {
+        const int e = pack_row32<false>(a, a.x, wide, n, a.x_pack, a.x_rows, to, lane);
+        if (lane == 0) a.x_exp[to] = e;
+      }
     } else if (a.dx) {
       for (int d = lane; d < a.D; d += 64) {
         if (a.dx_bf16)
@@ -249,8 +308,10 @@ __device__ __forceinline__ Sum blocks_of(const XentArgs& a, int m, int part, int
   return all;
 }
 
-// Row m's loss and the factors of its gradient from the others' sum.
-__device__ __forceinline__ float finish_row(const XentArgs& a, int64_t r0, int m, Sum others) {
+// Row m's loss and the factors of its gradient from the others' sum; w_top: the largest
+// w.  The row's E + X goes to x_factor.
+__device__ __forceinline__ float finish_row(const XentArgs& a, int64_t r0, int m, Sum others, int w_top,
+                                            int& x_factor) {
   // the others' sum is sum * 2^top, the target's exponential 2^(top - d)
   const float top = others.top, sum = others.sum;
   const float lt = a.at_target[r0 + m], d = fmaf(-lt, LOG2E, top);
@@ -276,9 +337,37 @@ __device__ __forceinline__ float finish_row(const XentArgs& a, int64_t r0, int m
     }
     r.at_target = -g * (sum / whole) * slope;
     r.target = a.target[r0 + m];
+    r.exp = 0;
+    r.x_factor = XENT_NO_EXP;
+    if (a.planes != 1) {
+      // no |dz| of the row is above |g| times the others' share
+      const float most = __builtin_fabsf(g) * (sum / whole);
+      if (most > 0.0f && most < __builtin_inff()) {
+        int e;
+        (void)frexpf(most, &e);
+        r.exp = e + w_top - 15;
+        r.x_factor = r.exp + a.x_exp[r0 + m];
+      }
+      r.at_target = ldexpf(r.at_target, a.w_exp[r.target] - r.exp);
+    }
+    x_factor = r.x_factor;
     a.row[r0 + m] = r;
   }
   return loss;
+}
+
+// The largest w of all that packed the table (0: none but zeros and infinities).
+template <int T>
+__device__ __forceinline__ int largest_w(const XentArgs& a, int* lds) {
+  if (!a.backward || a.planes == 1) return 0;
+  int most = XENT_NO_EXP;
+  for (int i = threadIdx.x; i < a.w_parts; i += T) most = max(most, a.w_part[i]);
+  most = wave_max(most);
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = most;
+  __syncthreads();
+  for (int i = 0; i < T / 64; ++i) most = max(most, lds[i]);
+  __syncthreads();
+  return most == XENT_NO_EXP ? 0 : most;
 }
 
 // Few rows: a wave each.  With one workgroup for all of them it also sums the total.
@@ -286,16 +375,28 @@ constexpr int JOIN_WAVES = 16, JOIN_FEW = 512;
 __global__ __launch_bounds__(64 * JOIN_WAVES) void xent_join_few_kernel(XentArgs a, int64_t r0, int blocks,
                                                                         bool total) {
   __shared__ double part[JOIN_WAVES];
+  __shared__ int exps[JOIN_WAVES];
   const int rows = mxm_xent_rows(a, r0), lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int m = blockIdx.x * JOIN_WAVES + wave;
+  const int w_top = largest_w<64 * JOIN_WAVES>(a, exps);
+  int x_factor = XENT_NO_EXP;
   double sum = 0.0;
   if (m < rows) {
     Sum s = blocks_of(a, m, lane, 64, blocks);
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) s = join(s, {__shfl_xor(s.top, o), __shfl_xor(s.sum, o)});
     if (lane == 0) {
-      const float loss = finish_row(a, r0, m, s);
+      const float loss = finish_row(a, r0, m, s, w_top, x_factor);
       sum = (double)loss * (a.row_weights ? (double)a.row_weights[a.map[r0 + m]] : 1.0);
+    }
+  }
+  if (a.backward && a.planes != 1) {
+    if (lane == 0) exps[wave] = x_factor;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      int most = exps[0];
+      for (int i = 1; i < JOIN_WAVES; ++i) most = max(most, exps[i]);
+      a.c_part[blockIdx.x] = most;
     }
   }
   if (!total) return;
@@ -313,24 +414,64 @@ __global__ __launch_bounds__(64 * JOIN_WAVES) void xent_join_few_kernel(XentArgs
 constexpr int JOIN_ROWS = 16;
 __global__ __launch_bounds__(NT) void xent_join_kernel(XentArgs a, int64_t r0, int blocks) {
   __shared__ Sum red[4][JOIN_ROWS];
+  __shared__ int exps[4];
   const int rows = mxm_xent_rows(a, r0);
   const int k = threadIdx.x & 15, m = blockIdx.x * JOIN_ROWS + k;
-  if (blockIdx.x * JOIN_ROWS >= rows) return;
+  const bool exponents = a.backward && a.planes != 1;
+  if (blockIdx.x * JOIN_ROWS >= rows) {
+    if (exponents && threadIdx.x == 0) a.c_part[blockIdx.x] = XENT_NO_EXP;
+    return;
+  }
+  const int w_top = largest_w<NT>(a, exps);
   Sum s = blocks_of(a, min(m, rows - 1), threadIdx.x >> 4, 16, blocks);
   s = join(s, {__shfl_xor(s.top, 16), __shfl_xor(s.sum, 16)});
   s = join(s, {__shfl_xor(s.top, 32), __shfl_xor(s.sum, 32)});
   if ((threadIdx.x & 63) < 16) red[threadIdx.x >> 6][k] = s;
   __syncthreads();
+  if (threadIdx.x >= 64) return;
+  int x_factor = XENT_NO_EXP;
   if (threadIdx.x < 16 && m < rows)
-    finish_row(a, r0, m, join(join(red[0][k], red[1][k]), join(red[2][k], red[3][k])));
+    finish_row(a, r0, m, join(join(red[0][k], red[1][k]), join(red[2][k], red[3][k])), w_top, x_factor);
+  if (exponents) {
+    x_factor = wave_max(x_factor);
+    if (threadIdx.x == 0) a.c_part[blockIdx.x] = x_factor;
+  }
 }
 
-// The summands of a piece to dz, 8 of a row per thread.
-template <int PLANES>
+// The summands of a piece to dz, 8 of a row per thread; under fp32 the first workgroups
+// of the rows also take x' to x'' (in place: the piece's logits are done).
+template <bool F16>
 __global__ __launch_bounds__(NT) void xent_finish_kernel(XentArgs a, int64_t r0, int block) {
   const int rows = mxm_xent_rows(a, r0), units = a.Vp / 8;
+  int c_top = 0;
+  if constexpr (F16) {
+    __shared__ int exps[4];
+    if (blockIdx.x == 0 && a.dw) {
+      c_top = XENT_NO_EXP;
+      for (int i = threadIdx.x; i < a.c_parts; i += NT) c_top = max(c_top, a.c_part[i]);
+      c_top = wave_max(c_top);
+      if ((threadIdx.x & 63) == 0) exps[threadIdx.x >> 6] = c_top;
+      __syncthreads();
+      c_top = max(max(exps[0], exps[1]), max(exps[2], exps[3]));
+      if (blockIdx.y == 0 && threadIdx.x == 0) a.scalars->dw_exp = c_top == XENT_NO_EXP ? 0 : c_top;
+    }
+  }
   for (int m = blockIdx.y; m < rows; m += gridDim.y) {
     const XentRow r = a.row[r0 + m];
+    if constexpr (F16) {
+      if (blockIdx.x == 0 && a.dw) {
+        const float f = r.x_factor == XENT_NO_EXP ? 0.0f : ldexpf(1.0f, r.x_factor - c_top);
+        for (int u = threadIdx.x; u < 2 * (a.Dp / 8); u += NT) {
+          const int pl = u >= a.Dp / 8;
+          f16x8_t* q = reinterpret_cast<f16x8_t*>(a.x_pack + pl * (a.x_rows * a.Dp) + (r0 + m) * a.Dp) +
+                       (u - pl * (a.Dp / 8));
+          f16x8_t v = *q;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[i] = (_Float16)((float)v[i] * f);
+          *q = v;
+        }
+      }
+    }
     for (int u = blockIdx.x * NT + threadIdx.x; u < units; u += gridDim.x * NT) {
       const int v = u * 8;
       // (the last units may lie in padding behind the last block)
@@ -338,30 +479,37 @@ __global__ __launch_bounds__(NT) void xent_finish_kernel(XentArgs a, int64_t r0,
       const float f = r.scale * (ref == r.ref ? 1.0f : __builtin_amdgcn_exp2f(ref - r.ref));
       float e[8];
       const int64_t at = (int64_t)m * a.Vp + v;
-      if constexpr (PLANES == 1) {
+      if constexpr (!F16) {
         const f16x8_t h = *reinterpret_cast<const f16x8_t*>(static_cast<const uint16_t*>(a.summands) + at);
 #pragma unroll
         for (int i = 0; i < 8; ++i) e[i] = (float)h[i] * f;
       } else {
         const f32x4_t* q = reinterpret_cast<const f32x4_t*>(static_cast<const float*>(a.summands) + at);
         const f32x4_t lo = q[0], hi = q[1];
+        i32x4_t wl = {0, 0, 0, 0}, wh = {0, 0, 0, 0};
+        if (v < a.V) {
+          wl = *reinterpret_cast<const i32x4_t*>(a.w_exp + v);
+          wh = *reinterpret_cast<const i32x4_t*>(a.w_exp + v + 4);
+        }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) e[i] = lo[i] * f, e[4 + i] = hi[i] * f;
+        for (int i = 0; i < 4; ++i) {
+          e[i] = ldexpf(lo[i] * f, wl[i] - r.exp);
+          e[4 + i] = ldexpf(hi[i] * f, wh[i] - r.exp);
+        }
       }
       const int t = r.target - v;
 #pragma unroll
       for (int i = 0; i < 8; ++i) e[i] = i == t ? r.at_target : (v + i < a.V ? e[i] : 0.0f);
-      if constexpr (PLANES == 1) {
+      if constexpr (!F16) {
         u32x4_t o;
 #pragma unroll
         for (int i = 0; i < 4; ++i) o[i] = mxm_pack_bf2_fast(e[2 * i], e[2 * i + 1]);
         *reinterpret_cast<u32x4_t*>(a.dz + at) = o;
       } else {
-        u32x4_t q[3];
-        planes3x8(e, q);
-#pragma unroll
-        for (int k = 0; k < 3; ++k)
-          *reinterpret_cast<u32x4_t*>(a.dz + (int64_t)k * a.piece_rows * a.Vp + at) = q[k];
+        u32x4_t q[2];
+        planes2x8(e, q);
+        *reinterpret_cast<u32x4_t*>(a.dz + at) = q[0];
+        *reinterpret_cast<u32x4_t*>(a.dz + a.piece_rows * a.Vp + at) = q[1];
       }
     }
   }
@@ -393,7 +541,8 @@ void mxm_launch_xent(const XentArgs& a0, hipStream_t s) {
   const bool plan = a.rows > 0 && a.rows <= PLAN_ROWS;
   if (!plan) xent_plan_kernel<<<1, PLAN_NT, 0, s>>>(a);
   if (a.rows > 0) {
-    const unsigned gx = rows_grid(a.rows), gw = a.w_direct ? 0 : rows_grid(a.V);
+    const unsigned gx = rows_grid(a.rows), gw = a.w_direct ? 0 : std::min<unsigned>(rows_grid(a.V), XENT_W_PARTS);
+    a.w_parts = (int)gw;
     if (plan)
       xent_pack_kernel<true><<<gx + gw, NT, 0, s>>>(a, (int)gx);
     else
@@ -408,18 +557,20 @@ void mxm_launch_xent(const XentArgs& a0, hipStream_t s) {
       a.stat_ld = rows;
       mxm_launch_xent_logits(a, r0, rows, s);
       const int blocks = (a.V + block - 1) / block;
-      if (rows <= JOIN_FEW)
-        xent_join_few_kernel<<<(unsigned)((rows + JOIN_WAVES - 1) / JOIN_WAVES), 64 * JOIN_WAVES, 0, s>>>(
-            a, r0, blocks, total_there);
-      else
-        xent_join_kernel<<<(unsigned)((rows + JOIN_ROWS - 1) / JOIN_ROWS), NT, 0, s>>>(a, r0, blocks);
+      if (rows <= JOIN_FEW) {
+        a.c_parts = (int)((rows + JOIN_WAVES - 1) / JOIN_WAVES);
+        xent_join_few_kernel<<<a.c_parts, 64 * JOIN_WAVES, 0, s>>>(a, r0, blocks, total_there);
+      } else {
+        a.c_parts = (int)((rows + JOIN_ROWS - 1) / JOIN_ROWS);
+        xent_join_kernel<<<a.c_parts, NT, 0, s>>>(a, r0, blocks);
+      }
       if (a.backward) {
         const unsigned gx = (unsigned)std::min((a.Vp / 8 + NT - 1) / NT, 64);
         const dim3 grid(gx, (unsigned)std::min<int64_t>(rows, std::max(1u, (unsigned)a.n_cu * 32 / gx)));
         if (a.planes == 1)
-          xent_finish_kernel<1><<<grid, NT, 0, s>>>(a, r0, block);
+          xent_finish_kernel<false><<<grid, NT, 0, s>>>(a, r0, block);
         else
-          xent_finish_kernel<3><<<grid, NT, 0, s>>>(a, r0, block);
+          xent_finish_kernel<true><<<grid, NT, 0, s>>>(a, r0, block);
       }
       if (a.dx) mxm_launch_xent_dx(a, r0, rows, s);
     }

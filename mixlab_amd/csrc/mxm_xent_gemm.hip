@@ -21,9 +21,10 @@
 // 16-wide k step are read between the MFMAs of the current one, the next stage's
 // loads go out over its first two.
 //
-// fp32 operands are three bf16 planes hi, mid, lo; of the nine products of planes the
-// six of at least 2^-16 relative are summed, the small ones first: what is left out is
-// below 2^-23 of |A| |B|.
+// fp32 operands are two fp16 planes with exponents of their rows (mxm_vocab.h); of the
+// four products of planes lo lo is left out, the small ones are summed first.  (As three
+// bf16 planes, of whose nine products six matter, the products took twice the time: a
+// step of 2048 rows, D 512 and 32768 entries 1.27 ms, 0.88 so.)
 //
 // The grid is persistent; each XCD (workgroup L runs on XCD L % 8) takes an eighth of
 // the tile list, in groups of GN n-tiles by all m-tiles.  Products with few tiles and
@@ -39,6 +40,8 @@ namespace {
 typedef __bf16 bf16x4_t __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+typedef int i32x4_t __attribute__((ext_vector_type(4)));
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 typedef float f32x16_t __attribute__((ext_vector_type(16)));
 typedef unsigned int u32x2_t __attribute__((ext_vector_type(2)));
@@ -102,7 +105,7 @@ struct Product {
   Operand a, b;
   int nk;          // stages of 64 k
   int pairs;       // pairs of planes
-  uint32_t amap, bmap;  // their planes, two bits each
+  uint32_t amap, bmap;  // their planes, a bit each
   const uint16_t* zeros;
 };
 
@@ -149,11 +152,10 @@ struct Loads {
 // The MFMA fragment of k step ks of tile rows (columns) col .. col + 31: lane l has
 // m (n) = col + l % 32, k = 16 ks + 8 (l / 32) .. + 7.
 template <int W, bool INNER>
-__device__ __forceinline__ bf16x8_t fragment(const unsigned char* t, int ks, int col, int lane) {
+__device__ __forceinline__ u32x4_t fragment(const unsigned char* t, int ks, int col, int lane) {
   if constexpr (INNER) {
     const int row = col + (lane & 31), kc = ks * 2 + (lane >> 5);
-    return __builtin_bit_cast(
-        bf16x8_t, *reinterpret_cast<const u32x4_t*>(t + (row * 8 + (kc ^ ((row / 2) % 8))) * 16));
+    return *reinterpret_cast<const u32x4_t*>(t + (row * 8 + (kc ^ ((row / 2) % 8))) * 16);
   } else {
     const int li = lane & 15, lg = lane >> 4;
     u32x2_t v[2];
@@ -164,13 +166,22 @@ __device__ __forceinline__ bf16x8_t fragment(const unsigned char* t, int ks, int
       const unsigned char* p = t + r * (W * 2) + ((c >> 3) ^ ((r & 3) << 2)) * 16 + (c & 7) * 2;
       v[h] = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4_p)(p)));
     }
-    const u32x4_t w = {v[0].x, v[0].y, v[1].x, v[1].y};
-    return __builtin_bit_cast(bf16x8_t, w);
+    return u32x4_t{v[0].x, v[0].y, v[1].x, v[1].y};
   }
 }
 
+template <bool F16>
+__device__ __forceinline__ f32x16_t mfma(u32x4_t a, u32x4_t b, f32x16_t c) {
+  if constexpr (F16)
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c,
+                                                  0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b),
+                                                   c, 0, 0, 0);
+}
+
 // Stages s_lo .. s_hi - 1 (of pairs * nk) of the tile at (m0, n0) into acc.
-template <class TL, bool AIN, bool BIN>
+template <class TL, bool AIN, bool BIN, bool F16>
 __device__ __forceinline__ void product_tile(const Product& p, unsigned char* lds, int m0, int n0,
                                              int s_lo, int s_hi, f32x16_t (&acc)[TL::TM][TL::TN]) {
   constexpr int TM = TL::TM, TN = TL::TN, NW = TL::NW, NS = TL::NS, KS = BK / 16;
@@ -198,7 +209,7 @@ __device__ __forceinline__ void product_tile(const Product& p, unsigned char* ld
   };
   auto load = [&](int slot, int from, int to) {
     unsigned char* st = lds + slot * TL::BUF;
-    const int pa = (p.amap >> (2 * dp)) & 3, pb = (p.bmap >> (2 * dp)) & 3;
+    const int pa = (p.amap >> dp) & 1, pb = (p.bmap >> dp) & 1;
 #pragma unroll
     for (int q = 0; q < LDPS; ++q) {
       if (q < from || q >= to) continue;
@@ -215,7 +226,7 @@ __device__ __forceinline__ void product_tile(const Product& p, unsigned char* ld
       load(s, 0, LDPS);
       next();
     }
-  bf16x8_t af[2][TM], bf[2][TN];
+  u32x4_t af[2][TM], bf[2][TN];
   auto frags = [&](const unsigned char* st, int set, int ks) {
 #pragma unroll
     for (int j = 0; j < TN; ++j)
@@ -244,7 +255,7 @@ __device__ __forceinline__ void product_tile(const Product& p, unsigned char* ld
       for (int i = 0; i < TM; ++i)
 #pragma unroll
         for (int j = 0; j < TN; ++j)
-          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(af[ks & 1][i], bf[ks & 1][j], acc[i][j], 0, 0, 0);
+          acc[i][j] = mfma<F16>(af[ks & 1][i], bf[ks & 1][j], acc[i][j]);
       if (ks + 1 < KS) {
         if (ks == 0) __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
 #pragma unroll
@@ -377,7 +388,7 @@ __device__ __forceinline__ float softcapped(float z, float cap, float inv) {
   return __builtin_copysignf(cap * ((1.0f - t) * __builtin_amdgcn_rcpf(1.0f + t)), z);
 }
 
-template <class TL, bool STORE, int PLANES>
+template <class TL, bool STORE, bool F16>
 __global__ __launch_bounds__(TL::NT, TL::WPS) void xent_logits_kernel(XentArgs a, Product p, int64_t r0) {
   __shared__ __attribute__((aligned(1024))) unsigned char lds[TL::NS * TL::BUF];
   constexpr int TM = TL::TM, TN = TL::TN;
@@ -400,12 +411,24 @@ __global__ __launch_bounds__(TL::NT, TL::WPS) void xent_logits_kernel(XentArgs a
       target[j] = n < rows ? a.target[r0 + n] : -1;
     }
     f32x16_t acc[TM][TN];
-    product_tile<TL, true, true>(p, lds, m0, n0, 0, p.nk * p.pairs, acc);
+    product_tile<TL, true, true, F16>(p, lds, m0, n0, 0, p.nk * p.pairs, acc);
     const int mw = m0 + wm * TM * 32;  // the wave's block of the vocabulary
     if (mw >= a.V && !STORE) continue;
 #pragma unroll
     for (int j = 0; j < TN; ++j) {
       const int n = n0 + (wn * TN + j) * 32 + (lane & 31);
+      if constexpr (F16) {
+        const int xe = n < rows ? a.x_exp[r0 + n] : 0;
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const i32x4_t we =
+                *reinterpret_cast<const i32x4_t*>(a.w_exp + mw + i * 32 + q * 8 + (lane >> 5) * 4);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) acc[i][j][q * 4 + k] = ldexpf(acc[i][j][q * 4 + k], we[k] + xe);
+          }
+      }
       if (cap > 0.0f) {
 #pragma unroll
         for (int i = 0; i < TM; ++i)
@@ -463,16 +486,16 @@ __global__ __launch_bounds__(TL::NT, TL::WPS) void xent_logits_kernel(XentArgs a
       if (n < rows && mw < a.V && lane < 32)
         a.stat[(int64_t)(mw / (TM * 32)) * a.stat_ld + n] = make_float2(sum, ref);
       if constexpr (STORE) {
-        constexpr int BITS = PLANES == 1 ? 16 : 32, PER = 128 / BITS;
+        constexpr int BITS = F16 ? 32 : 16, PER = 128 / BITS;
         using R = Rows<TM, BITS>;
         static_assert(TL::NW * R::BYTES <= TL::NS * TL::BUF, "staging fits the ring");
         const R block{lds + wave * R::BYTES, lane};
 #pragma unroll
         for (int i = 0; i < TM; ++i) {
-          if constexpr (PLANES == 1)
-            block.put16(i, acc[i][j], pack_f16);
-          else
+          if constexpr (F16)
             block.put32(i, acc[i][j]);
+          else
+            block.put16(i, acc[i][j], pack_f16);
         }
         const int nw = n0 + (wn * TN + j) * 32;
         block.get([&](int row, int c, u32x4_t v) {
@@ -494,12 +517,21 @@ struct Out {
   void* out;
   const float* add;      // earlier sums of the same elements, or null
   const int32_t* map;    // the row that n is, or null: n
+  const XentRow* row;    // fp32: the exponents of n's sums: dx's E,
+  const int32_t* w_exp;  // or dw's C - w
+  const XentScalars* scalars;
   int M;
   bool bf16, vec;        // vec: rows of whole aligned 16 bytes
 };
 
 // Row n's elements m .. m + 3 of an MFMA tile, as each quad of registers holds them.
+template <bool F16>
 __device__ __forceinline__ void put_tile(const Out& o, int m_first, int n, bool in, int lane, f32x16_t c) {
+  if constexpr (F16) {
+    const int e = !in ? 0 : o.row ? o.row[n].exp : o.scalars->dw_exp - o.w_exp[n];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) c[r] = ldexpf(c[r], e);
+  }
   const int64_t row = in ? (int64_t)(o.map ? o.map[n] : n) * o.M : 0;
   if (o.add && in) {
 #pragma unroll
@@ -558,7 +590,7 @@ __device__ __forceinline__ void fit(const XentArgs& a, Product& p, int64_t r0) {
   }
 }
 
-template <class TL, bool DW>
+template <class TL, bool DW, bool F16>
 __global__ __launch_bounds__(TL::NT, TL::WPS) void xent_grad_kernel(XentArgs a, Product p, Out o, int64_t r0,
                                                                     int slots, int scratch_tiles) {
   __shared__ __attribute__((aligned(1024))) unsigned char lds[TL::NS * TL::BUF];
@@ -574,7 +606,7 @@ __global__ __launch_bounds__(TL::NT, TL::WPS) void xent_grad_kernel(XentArgs a, 
     int tm, tn;
     tile_at(tile, mt, nt, tm, tn);
     f32x16_t acc[TM][TN];
-    product_tile<TL, false, !DW>(p, lds, tm * TL::BM, tn * TL::BN, (int)((int64_t)split * stages / splits),
+    product_tile<TL, false, !DW, F16>(p, lds, tm * TL::BM, tn * TL::BN, (int)((int64_t)split * stages / splits),
                                  (int)((int64_t)(split + 1) * stages / splits), acc);
     if (splits > 1) {
       f32x4_t* to = reinterpret_cast<f32x4_t*>(a.partial) +
@@ -597,7 +629,7 @@ __global__ __launch_bounds__(TL::NT, TL::WPS) void xent_grad_kernel(XentArgs a, 
 #pragma unroll
       for (int j = 0; j < TN; ++j) {
         const int n = tn * TL::BN + (wn * TN + j) * 32 + (lane & 31);
-        put_tile(o, tm * TL::BM + (wm * TM + i) * 32, n, n < N, lane, acc[i][j]);
+        put_tile<F16>(o, tm * TL::BM + (wm * TM + i) * 32, n, n < N, lane, acc[i][j]);
       }
   };
   // (one loop over both lists: the tile's code once)
@@ -618,7 +650,7 @@ __global__ __launch_bounds__(TL::NT, TL::WPS) void xent_grad_kernel(XentArgs a, 
 
 // The splits of the last round's tiles added in order; a workgroup per MFMA tile of
 // each wave.
-template <class TL, bool DW>
+template <class TL, bool DW, bool F16>
 __global__ __launch_bounds__(TL::NT) void xent_grad_join_kernel(XentArgs a, Product p, Out o, int64_t r0,
                                                                 int slots, int scratch_tiles) {
   constexpr int TM = TL::TM, TN = TL::TN, AHEAD = 8;
@@ -653,7 +685,7 @@ __global__ __launch_bounds__(TL::NT) void xent_grad_join_kernel(XentArgs a, Prod
         for (int k = 0; k < 4; ++k) c[q * 4 + k] += v[h][q][k];
   }
   const int n = tn * TL::BN + (wn * TN + j) * 32 + (lane & 31);
-  put_tile(o, tm * TL::BM + (wm * TM + i) * 32, n, n < N, lane, c);
+  put_tile<F16>(o, tm * TL::BM + (wm * TM + i) * 32, n, n < N, lane, c);
 }
 
 // ---- launches ----
@@ -663,14 +695,11 @@ int64_t tiles_of(int64_t m, int64_t n, int bm, int bn) { return (m + bm - 1) / b
 unsigned grid_of(int64_t items, int64_t slots) {
   return (unsigned)((std::min(items, slots) + 7) / 8 * 8);
 }
-// pairs of planes: (hi, lo), (lo, hi), (mid, mid), (hi, mid), (mid, hi), (hi, hi)
-constexpr uint32_t map_of(int p0, int p1, int p2, int p3, int p4, int p5) {
-  return p0 | p1 << 2 | p2 << 4 | p3 << 6 | p4 << 8 | p5 << 10;
-}
+// pairs of planes: (hi, lo), (lo, hi), (hi, hi)
 void set_planes(const XentArgs& a, Product& p) {
-  p.pairs = a.planes == 1 ? 1 : 6;
-  p.amap = a.planes == 1 ? 0 : map_of(0, 2, 1, 0, 1, 0);
-  p.bmap = a.planes == 1 ? 0 : map_of(2, 0, 1, 1, 0, 0);
+  p.pairs = a.planes == 1 ? 1 : 3;
+  p.amap = a.planes == 1 ? 0 : 0b010;
+  p.bmap = a.planes == 1 ? 0 : 0b001;
   p.zeros = a.zeros;
 }
 // The table, its rows' k or (k-out) its columns.
@@ -708,16 +737,14 @@ Shape logits_shape(int64_t rows, int V, int n_cu) {
   return rows <= 128 || tiles_of(V, rows, Big::BM, Big::BN) <= n_cu / 2 ? SMALL : BIG;
 }
 
-template <class TL, bool STORE, int PLANES>
-void launch_logits(const XentArgs& a, const Product& p, int64_t r0, int64_t rows, int per_cu, hipStream_t s) {
-  const unsigned grid = grid_of(tiles_of(a.V, rows, TL::BM, TL::BN), (int64_t)a.n_cu * per_cu);
-  xent_logits_kernel<TL, STORE, PLANES><<<grid, TL::NT, 0, s>>>(a, p, r0);
-}
 template <class TL>
 void launch_logits(const XentArgs& a, const Product& p, int64_t r0, int64_t rows, int per_cu, hipStream_t s) {
-  if (!a.backward) return launch_logits<TL, false, 1>(a, p, r0, rows, per_cu, s);
-  if (a.planes == 1) return launch_logits<TL, true, 1>(a, p, r0, rows, per_cu, s);
-  return launch_logits<TL, true, 3>(a, p, r0, rows, per_cu, s);
+  const unsigned grid = grid_of(tiles_of(a.V, rows, TL::BM, TL::BN), (int64_t)a.n_cu * per_cu);
+  const auto launch = [&](auto kernel) { kernel<<<grid, TL::NT, 0, s>>>(a, p, r0); };
+  if (a.planes == 1)
+    a.backward ? launch(xent_logits_kernel<TL, true, false>) : launch(xent_logits_kernel<TL, false, false>);
+  else
+    a.backward ? launch(xent_logits_kernel<TL, true, true>) : launch(xent_logits_kernel<TL, false, true>);
 }
 
 // The device counts the rows that take part, so it decides how tiles are split: the
@@ -728,10 +755,17 @@ void launch_grad(const XentArgs& a, const Product& p, const Out& o, int64_t r0, 
   const int64_t tiles = tiles_of(a.D, N, TL::BM, TL::BN);
   const int slots = a.n_cu * per_cu / 8 * 8;
   const int scratch = (int)(mxm_xent_partial_bytes(a.n_cu) / (TL::BM * TL::BN * 4));
-  xent_grad_kernel<TL, DW><<<(unsigned)slots, TL::NT, 0, s>>>(a, p, o, r0, slots, scratch);
   const int64_t most = DW ? tiles % slots : std::min<int64_t>(tiles, slots - 1);
-  if (most > 0)
-    xent_grad_join_kernel<TL, DW><<<(unsigned)(most * TL::TM * TL::TN), TL::NT, 0, s>>>(a, p, o, r0, slots, scratch);
+  const auto launch = [&](auto kernel, int64_t grid) {
+    if (grid > 0) kernel<<<(unsigned)grid, TL::NT, 0, s>>>(a, p, o, r0, slots, scratch);
+  };
+  if (a.planes == 1) {
+    launch(xent_grad_kernel<TL, DW, false>, slots);
+    launch(xent_grad_join_kernel<TL, DW, false>, most * TL::TM * TL::TN);
+  } else {
+    launch(xent_grad_kernel<TL, DW, true>, slots);
+    launch(xent_grad_join_kernel<TL, DW, true>, most * TL::TM * TL::TN);
+  }
 }
 
 }  // namespace
@@ -774,6 +808,7 @@ void mxm_launch_xent_dx(const XentArgs& a, int64_t r0, int64_t rows, hipStream_t
   Out o{};
   o.out = a.dx;
   o.map = a.map + r0;
+  o.row = a.row + r0;
   o.M = a.D;
   o.bf16 = a.dx_bf16;
   o.vec = aligned(a.dx) && a.D % (a.dx_bf16 ? 8 : 4) == 0;
@@ -793,6 +828,8 @@ void mxm_launch_xent_dw(const XentArgs& a, int64_t r0, bool last, hipStream_t s)
   o.out = last ? a.dw : sums;
   o.bf16 = last && a.dw_bf16;
   o.add = r0 > 0 ? sums : nullptr;
+  o.w_exp = a.w_exp;
+  o.scalars = a.scalars;
   o.M = a.D;
   o.vec = aligned(o.out) && a.D % (o.bf16 ? 8 : 4) == 0;
   if (a.D <= 128 || a.V <= 128)

@@ -18,13 +18,20 @@ def tolerances(x, w, ref, dtype, softcap, V):
     """Bounds of loss, lse, dx and dw (of the rows that take part), from the roundings.
 
     A logit is a sum of D products in fp32, of which each partial sum may lose a whole
-    step (2 U32) in the matrix cores; under fp32 the operands are split into planes whose
-    products number six, and what the planes leave out is under 4 U32 of the products.
+    step (2 U32) in the matrix cores.  Under fp32 a row of an operand is two fp16 planes
+    of 11 bits each, in units of which its largest element is over 2^14: 2^-23 of an
+    element (2 U32), or half a subnormal step, 2^-25 and so 2^-39 of the row's largest;
+    three products of planes are summed, and the fourth, left out, is below 2^-22 (4 U32).
     An exponential's argument l - ref is rounded once (U32 |l|), the exponential and
     each of the sum's additions once or twice."""
     D = x.shape[1]
-    sums = 2 * (D + 8) * (6 if dtype == "fp32" else 1) + 4
-    el = sums * U32 * ref["mass"]
+    fp32 = dtype == "fp32"
+    aw, ax = np.abs(w), np.abs(x)
+    xtop, wtop = ax.max(axis=1, keepdims=True), aw.max(axis=1, keepdims=True)
+    low = 2.0 ** -39
+    el = (2 * (D + 8) * (3 if fp32 else 1) + (8 if fp32 else 4)) * U32 * ref["mass"]
+    if fp32:
+        el = el + low * (xtop * aw.sum(axis=1) + ax.sum(axis=1, keepdims=True) * wtop.T)
     if softcap:
         el = el + 8 * U32 * softcap
     size = np.abs(ref["l"]).max(axis=1, keepdims=True)
@@ -32,21 +39,32 @@ def tolerances(x, w, ref, dtype, softcap, V):
     steps = U32 * (8 * size + 2 * (V / 64 + 160))
     row = (2 * top + steps)[:, 0]
     ep = (2 * top + steps) * 1.1            # of p, relative
-    rounding = (UBF + UBF / 4) if dtype == "bf16" else 8 * U32
+    rounding = 8 * U32 if fp32 else UBF + UBF / 4
     dz, dl = np.abs(ref["dz"]), np.abs(ref["dl"])
     edz = dz * (ep + rounding)
-    if dtype == "bf16":
+    # |g| times the others' share bounds a row's |dl|; the target's is that
+    most = dl.max(axis=1, keepdims=True)
+    if fp32:
+        # dz is kept in planes too, in units that the row's bound and the table's largest
+        # row set: half a subnormal step is 2^-39 of them, for entry v as many times more
+        # as its row of the table is smaller (powers of two: within a factor of 4)
+        edz = edz + low * 4 * most * (wtop.max() / np.maximum(wtop, 1e-300)).T
+    else:
         # p is kept in fp16 between its two passes, in units of which the largest of a
         # block of the vocabulary is over 2^14: half a step of fp16's subnormal numbers,
         # 2^-25, is 2^-39 of that largest one, which is at most the row's largest p
-        edz = edz + dl.max(axis=1, keepdims=True) * 2.0 ** -39
+        edz = edz + most * low
     if softcap:                             # of 1 - (l / cap)^2
         edz = edz + dl * (2 * el / softcap + 16 * U32)
-    per = 2 * (6 if dtype == "fp32" else 1)
+    per = 2 * (3 if fp32 else 1)
     N = x.shape[0]
-    aw, ax = np.abs(w), np.abs(x)
     bx = edz @ aw + per * (V + 64) * U32 * ((dz + edz) @ aw)
     bw = edz.T @ ax + per * (N + 64) * U32 * ((dz + edz).T @ ax)
+    if fp32:
+        bx = bx + dz @ (4 * U32 * aw + low * wtop)
+        # dw's rows of x share one exponent, set by the largest bound times row of x
+        share = np.divide(dz, most, out=np.zeros_like(dz), where=most > 0)
+        bw = bw + dz.T @ (4 * U32 * ax) + (low * 4 * (most * xtop).max()) * share.sum(axis=0)[:, None]
     return row, bx, bw
 
 
