@@ -106,7 +106,7 @@ struct XentArgs {
   int32_t* target;          // [rows] of those that take part
   XentScalars* scalars;
   float* nll;               // [rows] loss of the rows that take part
-  float* at_target;         // [rows] their target's logit
+  float* at_target;         // [rows] their target's logit, before the cap
   XentRow* row;             // [rows]
   uint16_t* x_pack;         // [planes][x_rows][Dp]
   int64_t x_rows;
@@ -140,4 +140,10 @@ void mxm_launch_xent(const XentArgs& a, hipStream_t s);
 __device__ __forceinline__ int mxm_xent_rows(const XentArgs& a, int64_t r0) {
   const int64_t left = a.scalars->rows - r0;
   return left <= 0 ? 0 : (int)(left < a.piece_rows ? left : a.piece_rows);
+}
+
+// tanh(z / cap) = 1 - 2 / (1 + exp(2 z / cap)), k2 = 2 log2 e / cap: off by a few 2^-24
+// of 1.
+__device__ __forceinline__ float mxm_xent_capped(float z, float k2) {
+  return fmaf(-2.0f, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * k2)), 1.0f);
 }

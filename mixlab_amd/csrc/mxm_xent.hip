@@ -27,35 +27,54 @@ __device__ __forceinline__ void leave_out(const XentArgs& a, int64_t n) {
 // others' loss and lse.
 constexpr int PLAN_NT = 1024;
 __global__ __launch_bounds__(PLAN_NT) void xent_plan_kernel(XentArgs a) {
-  __shared__ int wave_count[16];
+  constexpr int EACH = 8;  // rows per thread and turn, PLAN_NT apart
+  __shared__ int wave_count[2][EACH][16];
   __shared__ double wave_weight[16];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   int64_t base = 0;
   double sum = 0.0;
-  for (int64_t n0 = 0; n0 < a.rows; n0 += PLAN_NT) {
-    const int64_t n = n0 + threadIdx.x;
-    int t;
-    float w = 0.0f;
-    const bool in = n < a.rows && takes_part(a, n, t, w);
-    const unsigned long long m = __ballot(in);
-    if (lane == 0) wave_count[wave] = __popcll(m);
-    __syncthreads();
-    int before = 0, all = 0;
-    for (int i = 0; i < 16; ++i) {
-      before += i < wave ? wave_count[i] : 0;
-      all += wave_count[i];
+  int turn = 0;
+  for (int64_t n0 = 0; n0 < a.rows; n0 += PLAN_NT * EACH, turn ^= 1) {
+    int t[EACH];
+    float w[EACH];
+    bool in[EACH];
+    unsigned long long m[EACH];
+#pragma unroll
+    for (int k = 0; k < EACH; ++k) {
+      const int64_t n = n0 + k * PLAN_NT + threadIdx.x;
+      w[k] = 0.0f;
+      in[k] = n < a.rows && takes_part(a, n, t[k], w[k]);
     }
-    const int64_t at = base + before + __popcll(m & ((1ull << lane) - 1));
-    if (in) {
-      a.map[at] = (int32_t)n;
-      a.target[at] = t;
-      sum += (double)w;
-    } else if (n < a.rows) {
-      leave_out(a, n);
+#pragma unroll
+    for (int k = 0; k < EACH; ++k) {
+      sum += in[k] ? (double)w[k] : 0.0;
+      m[k] = __ballot(in[k]);
+      if (lane == 0) wave_count[turn][k][wave] = __popcll(m[k]);
     }
-    if (n < a.rows) a.slot[n] = in ? (int32_t)at : -1;
-    base += all;
     __syncthreads();
+#pragma unroll
+    for (int k = 0; k < EACH; ++k) {
+      const int64_t n = n0 + k * PLAN_NT + threadIdx.x;
+      const int c = lane < 16 ? wave_count[turn][k][lane] : 0;
+      int before = lane < wave ? c : 0, all = c;
+#pragma unroll
+      for (int o = 1; o < 16; o <<= 1) {
+        before += __shfl_xor(before, o);
+        all += __shfl_xor(all, o);
+      }
+      before = __builtin_amdgcn_readfirstlane(before);
+      const int64_t at = base + before + __popcll(m[k] & ((1ull << lane) - 1));
+      if (n < a.rows) {
+        a.slot[n] = in[k] ? (int32_t)at : -1;
+        if (in[k]) {
+          a.map[at] = (int32_t)n;
+          a.target[at] = t[k];
+        } else {
+          leave_out(a, n);
+        }
+      }
+      base += __builtin_amdgcn_readfirstlane(all);
+    }
   }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
@@ -314,7 +333,13 @@ __device__ __forceinline__ float finish_row(const XentArgs& a, int64_t r0, int m
                                             int& x_factor) {
   // the others' sum is sum * 2^top, the target's exponential 2^(top - d)
   const float top = others.top, sum = others.sum;
-  const float lt = a.at_target[r0 + m], d = fmaf(-lt, LOG2E, top);
+  float lt = a.at_target[r0 + m], slope = 1.0f;
+  if (a.softcap > 0.0f) {
+    const float th = mxm_xent_capped(lt, 2.0f * LOG2E / a.softcap);
+    lt = a.softcap * th;
+    slope = fmaf(-th, th, 1.0f);
+  }
+  const float d = fmaf(-lt, LOG2E, top);
   const float et = __builtin_amdgcn_exp2f(-d), whole = sum + et;
   // (next to the target's probability of one the loss keeps its digits)
   const bool near = d <= 60.0f;
@@ -330,11 +355,6 @@ __device__ __forceinline__ float finish_row(const XentArgs& a, int64_t r0, int m
     XentRow r;
     r.ref = top;
     r.scale = g / whole;
-    float slope = 1.0f;
-    if (a.softcap > 0.0f) {
-      const float u = lt / a.softcap;
-      slope = 1.0f - u * u;
-    }
     r.at_target = -g * (sum / whole) * slope;
     r.target = a.target[r0 + m];
     r.exp = 0;

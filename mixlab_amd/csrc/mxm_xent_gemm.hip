@@ -31,6 +31,7 @@
 // a long sum are split along k; the splits' tiles go to scratch in fp32 and are added
 // in order by a second launch.
 #include <algorithm>
+#include <type_traits>
 
 #include "mxm_lanes.h"
 #include "mxm_vocab.h"
@@ -116,8 +117,9 @@ struct Loads {
   static constexpr int Q = INNER ? W / 8 / NW : BK / RPW / NW;
   static_assert(Q >= 1 && Q * RPW * NW == (INNER ? W : BK), "whole wave-loads");
   static_assert((NW * RPW) % (INNER ? 16 : 4) == 0, "swizzle phase is the same for every load");
-  unsigned off[Q];  // bytes from the stage's base
-  int r0, chunk;    // the lane's row in load 0, its chunk's first element
+  unsigned off[Q];       // bytes from the stage's base
+  int r0, chunk;         // the lane's row in load 0, its chunk's first element
+  const uint16_t* base;  // of the next stage to load
   __device__ __forceinline__ void init(const Operand& o, int x0, int wave, int lane) {
     if constexpr (INNER) {
       r0 = wave * 8 + lane / 8;
@@ -134,18 +136,20 @@ struct Loads {
         off[q] = 2u * ((unsigned)(r0 + q * NW * RPW) * (unsigned)o.ld + (unsigned)col);
     }
   }
-  // load q of the stage at k0 of plane `pl` into `lds` (the operand's part of a stage)
-  __device__ __forceinline__ void load(const Operand& o, const uint16_t* zeros, int x0, int pl, int k0,
-                                       int q, int wave, unsigned char* lds) const {
-    const uint16_t* base = o.p + pl * o.plane + (INNER ? (int64_t)x0 * o.ld + k0 : (int64_t)k0 * o.ld);
-    unsigned char* to = lds + (wave + NW * q) * 1024;
-    if (k0 + BK <= o.k) {
-      dma16s(base, off[q], to);
-    } else {
-      const int k = k0 + (INNER ? chunk : r0 + q * NW * RPW);
-      const char* from = reinterpret_cast<const char*>(base) + off[q];
-      dma16(k < o.k ? from : reinterpret_cast<const char*>(zeros), to);
-    }
+  __device__ __forceinline__ void seek(const Operand& o, int x0, int plane, int k0) {
+    base = o.p + plane * o.plane + (INNER ? (int64_t)x0 * o.ld + k0 : (int64_t)k0 * o.ld);
+  }
+  __device__ __forceinline__ void step(const Operand& o) { base += INNER ? BK : (int64_t)BK * o.ld; }
+  // load q of the stage into `lds` (the operand's part of a stage)
+  __device__ __forceinline__ void load(int q, int wave, unsigned char* lds) const {
+    dma16s(base, off[q], lds + (wave + NW * q) * 1024);
+  }
+  // of a stage of which only `left` k exist: zeros behind them
+  __device__ __forceinline__ void load_part(int left, const uint16_t* zeros, int q, int wave,
+                                            unsigned char* lds) const {
+    const int k = INNER ? chunk : r0 + q * NW * RPW;
+    const char* from = reinterpret_cast<const char*>(base) + off[q];
+    dma16(k < left ? from : reinterpret_cast<const char*>(zeros), lds + (wave + NW * q) * 1024);
   }
 };
 
@@ -204,21 +208,43 @@ __device__ __forceinline__ void product_tile(const Product& p, unsigned char* ld
 
   // the next stage to load: pair of planes and stage within it
   int dp = s_lo / max(p.nk, 1), dk = s_lo - dp * p.nk;
-  auto next = [&] {
-    if (++dk == p.nk) dk = 0, ++dp;
+  auto seek = [&] {
+    la.seek(p.a, m0, (p.amap >> dp) & 1, dk * BK);
+    lb.seek(p.b, n0, (p.bmap >> dp) & 1, dk * BK);
   };
-  auto load = [&](int slot, int from, int to) {
-    unsigned char* st = lds + slot * TL::BUF;
-    const int pa = (p.amap >> dp) & 1, pb = (p.bmap >> dp) & 1;
-#pragma unroll
-    for (int q = 0; q < LDPS; ++q) {
-      if (q < from || q >= to) continue;
-      if (q < LA::Q)
-        la.load(p.a, p.zeros, m0, pa, dk * BK, q, wave, st);
-      else
-        lb.load(p.b, p.zeros, n0, pb, dk * BK, q - LA::Q, wave, st + TL::A_BYTES);
+  auto next = [&] {
+    la.step(p.a);
+    lb.step(p.b);
+    if (++dk == p.nk) {
+      dk = 0;
+      ++dp;
+      seek();
     }
   };
+  const bool partial = min(p.a.k, p.b.k) < p.nk * BK;
+  auto load = [&](int slot, int from, int to) {
+    unsigned char* st = lds + slot * TL::BUF;
+    if (!partial || dk + 1 < p.nk) {
+#pragma unroll
+      for (int q = 0; q < LDPS; ++q) {
+        if (q < from || q >= to) continue;
+        if (q < LA::Q)
+          la.load(q, wave, st);
+        else
+          lb.load(q - LA::Q, wave, st + TL::A_BYTES);
+      }
+    } else {
+#pragma unroll
+      for (int q = 0; q < LDPS; ++q) {
+        if (q < from || q >= to) continue;
+        if (q < LA::Q)
+          la.load_part(p.a.k - dk * BK, p.zeros, q, wave, st);
+        else
+          lb.load_part(p.b.k - dk * BK, p.zeros, q - LA::Q, wave, st + TL::A_BYTES);
+      }
+    }
+  };
+  seek();
   const int n = s_hi - s_lo;
 #pragma unroll
   for (int s = 0; s < NS - 1; ++s)
@@ -298,7 +324,7 @@ __host__ __device__ inline Split split_of(int tiles, int stages, int slots, int 
     if (n * p.tail > scratch_tiles) n = scratch_tiles / p.tail;
     if (n < 2) continue;
     const int need = (n * p.tail + slots - 1) / slots;
-    const int cost = need * ((stages + n - 1) / n + TILE_COST) + SPLIT_COST + n / 2;
+    const int cost = need * ((stages + n - 1) / n + TILE_COST) + SPLIT_COST + n / 8;
     if (cost < least) least = cost, p.splits = n;
   }
   return p;
@@ -351,17 +377,19 @@ struct Rows {
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_wave_barrier();
   }
-  // The MFMA tile i's values, rounded by pack(a, b) to two 16-bit halves of a word:
-  // quads q and q + 1 of the two half-waves exchanged, 8 consecutive m a lane
-  template <class P>
-  __device__ __forceinline__ void put16(int i, const f32x16_t& c, P pack) const {
+  // The MFMA tile i's values as fp16: quads q and q + 1 of the two half-waves exchanged,
+  // 8 consecutive m a lane
+  __device__ __forceinline__ void put16(int i, const f32x16_t& c) const {
 #pragma unroll
     for (int q = 0; q < 4; q += 2) {
       uint32_t w[2][2];
 #pragma unroll
       for (int k = 0; k < 2; ++k)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) w[k][h] = pack(c[(q + k) * 4 + 2 * h], c[(q + k) * 4 + 2 * h + 1]);
+        for (int h = 0; h < 2; ++h) {
+          const f16x2_t v = {(_Float16)c[(q + k) * 4 + 2 * h], (_Float16)c[(q + k) * 4 + 2 * h + 1]};
+          w[k][h] = __builtin_bit_cast(uint32_t, v);
+        }
       const auto x = __builtin_amdgcn_permlane32_swap(w[0][0], w[1][0], false, false);
       const auto y = __builtin_amdgcn_permlane32_swap(w[0][1], w[1][1], false, false);
       put(i * 4 + q + (lane >> 5), u32x4_t{x[0], y[0], x[1], y[1]});
@@ -375,83 +403,103 @@ struct Rows {
     }
   }
 };
-__device__ __forceinline__ uint32_t pack_f16(float a, float b) {
-  const f16x2_t v = {(_Float16)a, (_Float16)b};
-  return __builtin_bit_cast(uint32_t, v);
-}
 
 // ---- logits ----
 
-__device__ __forceinline__ float softcapped(float z, float cap, float inv) {
-  // tanh(u) = (1 - t) / (1 + t), t = exp(-2 |u|): off by a few 2^-24 of 1
-  const float t = __builtin_amdgcn_exp2f(-2.0f * LOG2E * __builtin_fabsf(z * inv));
-  return __builtin_copysignf(cap * ((1.0f - t) * __builtin_amdgcn_rcpf(1.0f + t)), z);
+// What bounds the epilogue is its transcendentals, one per logit and three with a
+// softcap, at a quarter of the other instructions' rate: about 4 us of a 256 x 256 tile
+// without and 8 with it, next to 1.5 us per stage of the sum.  The largest logit is
+// taken before the cap, which keeps their order.
+// (What the kernels take, and no more: every argument is a scalar register that the sum's
+// loop has to keep, and some forty more of them had it reading them back from vector
+// registers: 2720 us of 16384 x 50257 logits at D 2048 became 2940.)
+struct LogitsArgs {
+  const XentScalars* scalars;
+  int64_t r0, piece_rows;  // the piece; arrays of rows start at its first row
+  int V, Vp;
+  float softcap;
+  const int32_t *target, *x_exp, *w_exp;
+  float* at_target;
+  float2* stat;
+  int64_t stat_ld;
+  void* summands;
+};
+struct GradArgs {
+  const XentScalars* scalars;
+  int64_t r0, piece_rows;
+  int V, D;
+  float* partial;
+  int slots, scratch_tiles;
+};
+template <class A>
+__device__ __forceinline__ int rows_of(const A& a) {
+  const int64_t left = a.scalars->rows - a.r0;
+  return left <= 0 ? 0 : (int)(left < a.piece_rows ? left : a.piece_rows);
 }
 
-template <class TL, bool STORE, bool F16>
-__global__ __launch_bounds__(TL::NT, TL::WPS) void xent_logits_kernel(XentArgs a, Product p, int64_t r0) {
+template <class TL, bool STORE, bool F16, bool CAP>
+__global__ __launch_bounds__(TL::NT, TL::WPS) void xent_logits_kernel(LogitsArgs a, Product p) {
   __shared__ __attribute__((aligned(1024))) unsigned char lds[TL::NS * TL::BUF];
+  __shared__ __attribute__((aligned(16))) int w_exp[F16 ? TL::BM : 4];
   constexpr int TM = TL::TM, TN = TL::TN;
-  const int rows = mxm_xent_rows(a, r0);
+  const int rows = rows_of(a);
   p.b.rows = rows;
-  p.b.p += r0 * p.b.ld;
   const int mt = (a.V + TL::BM - 1) / TL::BM, nt = (rows + TL::BN - 1) / TL::BN;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int wm = wave / TL::WN, wn = wave % TL::WN;
-  const float cap = a.softcap, inv = cap > 0.0f ? 1.0f / cap : 0.0f;
+  const float k2 = 2.0f * LOG2E / a.softcap, cap2 = a.softcap * LOG2E;  // (CAP)
   const Items items(mt * nt);
   for (int item = items.first; item < items.end; item += items.step) {
     int tm, tn;
     tile_at(item, mt, nt, tm, tn);
     const int m0 = tm * TL::BM, n0 = tn * TL::BN;
-    int target[TN];
+    int targets[TN], x_exps[TN];
 #pragma unroll
     for (int j = 0; j < TN; ++j) {
       const int n = n0 + (wn * TN + j) * 32 + (lane & 31);
-      target[j] = n < rows ? a.target[r0 + n] : -1;
+      targets[j] = n < rows ? a.target[n] : -1;
+      if constexpr (F16) x_exps[j] = n < rows ? a.x_exp[n] : 0;
     }
+    // (the sum's barriers stand between this and the epilogue)
+    if constexpr (F16)
+      for (int i = threadIdx.x; i < TL::BM; i += TL::NT) w_exp[i] = a.w_exp[m0 + i];
     f32x16_t acc[TM][TN];
     product_tile<TL, true, true, F16>(p, lds, m0, n0, 0, p.nk * p.pairs, acc);
     const int mw = m0 + wm * TM * 32;  // the wave's block of the vocabulary
-    if (mw >= a.V && !STORE) continue;
+    const int first = mw + (lane >> 5) * 4;
 #pragma unroll
     for (int j = 0; j < TN; ++j) {
-      const int n = n0 + (wn * TN + j) * 32 + (lane & 31);
+      if (mw >= a.V && !STORE) continue;
+      const int nw = n0 + (wn * TN + j) * 32, n = nw + (lane & 31);
+      const int target = targets[j];
       if constexpr (F16) {
-        const int xe = n < rows ? a.x_exp[r0 + n] : 0;
 #pragma unroll
         for (int i = 0; i < TM; ++i)
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
-            const i32x4_t we =
-                *reinterpret_cast<const i32x4_t*>(a.w_exp + mw + i * 32 + q * 8 + (lane >> 5) * 4);
+            const i32x4_t we = *reinterpret_cast<const i32x4_t*>(w_exp + first - m0 + i * 32 + q * 8);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) acc[i][j][q * 4 + k] = ldexpf(acc[i][j][q * 4 + k], we[k] + xe);
+            for (int k = 0; k < 4; ++k) acc[i][j][q * 4 + k] = ldexpf(acc[i][j][q * 4 + k], we[k] + x_exps[j]);
           }
       }
-      if (cap > 0.0f) {
-#pragma unroll
-        for (int i = 0; i < TM; ++i)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) acc[i][j][r] = softcapped(acc[i][j][r], cap, inv);
-      }
       // entries behind the vocabulary, and the target (whose logit is kept apart)
-      const int first = mw + (lane >> 5) * 4;
       if (mw + TM * 32 > a.V) {
+        int end = a.V - first;
+        asm volatile("" : "+v"(end));  // (else the loop's comparisons move before it, into 128 scalar registers)
 #pragma unroll
         for (int i = 0; i < TM; ++i)
 #pragma unroll
           for (int r = 0; r < 16; ++r)
-            if (first + i * 32 + (r >> 2) * 8 + (r & 3) >= a.V) acc[i][j][r] = -__builtin_inff();
+            acc[i][j][r] = i * 32 + (r >> 2) * 8 + (r & 3) >= end ? -__builtin_inff() : acc[i][j][r];
       }
-      const int at = target[j] - first;
-      if (__ballot(target[j] >= mw && target[j] < mw + TM * 32)) {
+      if (__ballot(target >= mw && target < mw + TM * 32) != 0) {
+        const int at = target - first;
 #pragma unroll
         for (int i = 0; i < TM; ++i)
 #pragma unroll
           for (int r = 0; r < 16; ++r)
             if (at == i * 32 + (r >> 2) * 8 + (r & 3)) {
-              a.at_target[r0 + n] = acc[i][j][r];
+              a.at_target[n] = acc[i][j][r];
               acc[i][j][r] = -__builtin_inff();
             }
       }
@@ -463,24 +511,29 @@ __global__ __launch_bounds__(TL::NT, TL::WPS) void xent_logits_kernel(XentArgs a
       top = fmaxf(top, mxm_xor_lane_f(top, 32));
       // 2^(l log2 e - ref) lies in (0, 2^15]: fp16 keeps 12 bits of summands down to
       // 2^-29 of the block's largest and 2^-39 of it at all
-      const float ref = top > -3.0e38f ? ceilf(top * LOG2E) - 15.0f : -1.0e30f;
+      float ref = -1.0e30f;  // (of a block of minus infinities)
+      if (top > -__builtin_inff()) ref = ceilf(CAP ? cap2 * mxm_xent_capped(top, k2) : top * LOG2E) - 15.0f;
       float s[2] = {0.0f, 0.0f};
+      if constexpr (CAP) {
 #pragma unroll
-      for (int i = 0; i < TM; ++i)
+        for (int i = 0; i < TM; ++i)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const float l = acc[i][j][r];
-          float e = __builtin_amdgcn_exp2f(fmaf(l, LOG2E, -ref));
-          s[r & 1] += e;
-          if constexpr (STORE) {
-            if (cap > 0.0f) {
-              // (a masked logit counts as -cap: a factor of 0)
-              const float u = fmaxf(l * inv, -1.0f);
-              e *= fmaf(-u, u, 1.0f);
-            }
-            acc[i][j][r] = e;
+          for (int r = 0; r < 16; ++r) {
+            const float th = mxm_xent_capped(acc[i][j][r], k2);
+            float e = __builtin_amdgcn_exp2f(fmaf(th, cap2, -ref));
+            e = acc[i][j][r] == -__builtin_inff() ? 0.0f : e;
+            s[r & 1] += e;
+            acc[i][j][r] = e * fmaf(-th, th, 1.0f);
           }
-        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            acc[i][j][r] = __builtin_amdgcn_exp2f(fmaf(acc[i][j][r], LOG2E, -ref));
+            s[r & 1] += acc[i][j][r];
+          }
+      }
       float sum = s[0] + s[1];
       sum += mxm_xor_lane_f(sum, 32);
       if (n < rows && mw < a.V && lane < 32)
@@ -495,9 +548,8 @@ __global__ __launch_bounds__(TL::NT, TL::WPS) void xent_logits_kernel(XentArgs a
           if constexpr (F16)
             block.put32(i, acc[i][j]);
           else
-            block.put16(i, acc[i][j], pack_f16);
+            block.put16(i, acc[i][j]);
         }
-        const int nw = n0 + (wn * TN + j) * 32;
         block.get([&](int row, int c, u32x4_t v) {
           const int m = mw + c * PER;
           if (nw + row < rows && m < a.Vp)
@@ -506,7 +558,7 @@ __global__ __launch_bounds__(TL::NT, TL::WPS) void xent_logits_kernel(XentArgs a
         });
       }
     }
-    if constexpr (STORE) lds_barrier();  // before the next tile's loads
+    if constexpr (STORE || F16) lds_barrier();  // before the next tile's loads
   }
 }
 
@@ -577,12 +629,44 @@ __device__ __forceinline__ void put_tile(const Out& o, int m_first, int n, bool 
   }
 }
 
+// Elements m .. m + 3 of row n.
+template <bool F16>
+__device__ __forceinline__ void put_quad(const Out& o, int m, int n, f32x4_t c) {
+  if (m >= o.M) return;
+  if constexpr (F16) {
+    const int e = o.row ? o.row[n].exp : o.scalars->dw_exp - o.w_exp[n];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) c[k] = ldexpf(c[k], e);
+  }
+  const int64_t at = (int64_t)(o.map ? o.map[n] : n) * o.M + m;
+  if (o.vec) {
+    if (o.add) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) c[k] += o.add[at + k];
+    }
+    if (o.bf16)
+      *reinterpret_cast<u32x2_t*>(static_cast<uint16_t*>(o.out) + at) =
+          u32x2_t{mxm_pack_bf2_fast(c[0], c[1]), mxm_pack_bf2_fast(c[2], c[3])};
+    else
+      *reinterpret_cast<f32x4_t*>(static_cast<float*>(o.out) + at) = c;
+    return;
+  }
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    if (m + k < o.M) {
+      const float v = o.add ? c[k] + o.add[at + k] : c[k];
+      if (o.bf16)
+        static_cast<uint16_t*>(o.out)[at + k] = mxm_f2bf_fast(v);
+      else
+        static_cast<float*>(o.out)[at + k] = v;
+    }
+}
+
 // What a launch needs of the device's count of rows: n of dx, k of dw.
 template <bool DW>
-__device__ __forceinline__ void fit(const XentArgs& a, Product& p, int64_t r0) {
-  const int rows = mxm_xent_rows(a, r0);
+__device__ __forceinline__ void fit(const GradArgs& a, Product& p) {
+  const int rows = rows_of(a);
   if constexpr (DW) {
-    p.a.p += r0 * p.a.ld;
     p.a.k = p.b.k = rows;
     p.nk = (rows + BK - 1) / BK;
   } else {
@@ -591,17 +675,16 @@ __device__ __forceinline__ void fit(const XentArgs& a, Product& p, int64_t r0) {
 }
 
 template <class TL, bool DW, bool F16>
-__global__ __launch_bounds__(TL::NT, TL::WPS) void xent_grad_kernel(XentArgs a, Product p, Out o, int64_t r0,
-                                                                    int slots, int scratch_tiles) {
+__global__ __launch_bounds__(TL::NT, TL::WPS) void xent_grad_kernel(GradArgs a, Product p, Out o) {
   __shared__ __attribute__((aligned(1024))) unsigned char lds[TL::NS * TL::BUF];
   constexpr int TM = TL::TM, TN = TL::TN;
-  fit<DW>(a, p, r0);
+  fit<DW>(a, p);
   const int N = DW ? a.V : p.b.rows;
   const int mt = (a.D + TL::BM - 1) / TL::BM, nt = (N + TL::BN - 1) / TL::BN;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int wm = wave / TL::WN, wn = wave % TL::WN;
   const int stages = p.nk * p.pairs;
-  const Split plan = split_of(mt * nt, stages, slots, scratch_tiles);
+  const Split plan = split_of(mt * nt, stages, a.slots, a.scratch_tiles);
   auto work = [&](int tile, int split, int splits) {
     int tm, tn;
     tile_at(tile, mt, nt, tm, tn);
@@ -651,41 +734,38 @@ __global__ __launch_bounds__(TL::NT, TL::WPS) void xent_grad_kernel(XentArgs a, 
 // The splits of the last round's tiles added in order; a workgroup per MFMA tile of
 // each wave.
 template <class TL, bool DW, bool F16>
-__global__ __launch_bounds__(TL::NT) void xent_grad_join_kernel(XentArgs a, Product p, Out o, int64_t r0,
-                                                                int slots, int scratch_tiles) {
-  constexpr int TM = TL::TM, TN = TL::TN, AHEAD = 8;
-  fit<DW>(a, p, r0);
+__global__ __launch_bounds__(TL::NT) void xent_grad_join_kernel(GradArgs a, Product p, Out o) {
+  constexpr int TM = TL::TM, TN = TL::TN, AHEAD = 16;
+  fit<DW>(a, p);
   const int N = DW ? a.V : p.b.rows;
   const int mt = (a.D + TL::BM - 1) / TL::BM, nt = (N + TL::BN - 1) / TL::BN;
-  const Split plan = split_of(mt * nt, p.nk * p.pairs, slots, scratch_tiles);
+  const Split plan = split_of(mt * nt, p.nk * p.pairs, a.slots, a.scratch_tiles);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int wm = wave / TL::WN, wn = wave % TL::WN;
-  const int tile = blockIdx.x / (TM * TN), ij = blockIdx.x % (TM * TN), i = ij / TN, j = ij % TN;
-  if (plan.splits == 1 || tile >= plan.tail) return;
-  int tm, tn;
-  tile_at(plan.whole + tile, mt, nt, tm, tn);
-  f32x16_t c;
-#pragma unroll
-  for (int r = 0; r < 16; ++r) c[r] = 0.0f;
+  if (plan.splits == 1) return;
   const int64_t step = (int64_t)plan.tail * (TL::BM * TL::BN / 4);
-  const f32x4_t* from = reinterpret_cast<const f32x4_t*>(a.partial) + (int64_t)tile * (TL::BM * TL::BN / 4) +
-                        wave * (TM * TN * 4 * 64) + ij * 4 * 64 + lane;
-  for (int s = 0; s < plan.splits; s += AHEAD) {
-    f32x4_t v[AHEAD][4];
+  // a quad of each lane's registers at a time
+  for (int item = blockIdx.x; item < plan.tail * (TM * TN * 4); item += gridDim.x) {
+    const int tile = item / (TM * TN * 4), ijq = item % (TM * TN * 4);
+    const int i = ijq / (TN * 4), j = ijq / 4 % TN, q = ijq % 4;
+    int tm, tn;
+    tile_at(plan.whole + tile, mt, nt, tm, tn);
+    f32x4_t c = {0.0f, 0.0f, 0.0f, 0.0f};
+    const f32x4_t* from = reinterpret_cast<const f32x4_t*>(a.partial) + (int64_t)tile * (TL::BM * TL::BN / 4) +
+                          wave * (TM * TN * 4 * 64) + ijq * 64 + lane;
+    for (int s = 0; s < plan.splits; s += AHEAD) {
+      f32x4_t v[AHEAD];
 #pragma unroll
-    for (int h = 0; h < AHEAD; ++h)
+      for (int h = 0; h < AHEAD; ++h)
+        v[h] = s + h < plan.splits ? from[(s + h) * step] : f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
-        v[h][q] = s + h < plan.splits ? from[(s + h) * step + q * 64] : f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+      for (int h = 0; h < AHEAD; ++h)
 #pragma unroll
-    for (int h = 0; h < AHEAD; ++h)
-#pragma unroll
-      for (int q = 0; q < 4; ++q)
-#pragma unroll
-        for (int k = 0; k < 4; ++k) c[q * 4 + k] += v[h][q][k];
+        for (int k = 0; k < 4; ++k) c[k] += v[h][k];
+    }
+    const int n = tn * TL::BN + (wn * TN + j) * 32 + (lane & 31);
+    if (n < N) put_quad<F16>(o, tm * TL::BM + (wm * TM + i) * 32 + q * 8 + (lane >> 5) * 4, n, c);
   }
-  const int n = tn * TL::BN + (wn * TN + j) * 32 + (lane & 31);
-  put_tile<F16>(o, tm * TL::BM + (wm * TM + i) * 32, n, n < N, lane, c);
 }
 
 // ---- launches ----
@@ -712,9 +792,9 @@ Operand table(const XentArgs& a, bool inner) {
   o.k = inner ? o.ld : a.V;
   return o;
 }
-Operand hidden(const XentArgs& a, bool inner) {
+Operand hidden(const XentArgs& a, bool inner, int64_t r0) {
   Operand o{};
-  o.p = a.x_pack;
+  o.p = a.x_pack + r0 * a.Dp;
   o.ld = a.Dp;
   o.plane = a.x_rows * a.Dp;
   o.rows = a.Dp;  // (k-out; k-inner: the rows that take part, on the device)
@@ -733,18 +813,27 @@ Operand grad(const XentArgs& a) {
 
 enum Shape { FEW, SMALL, BIG };
 Shape logits_shape(int64_t rows, int V, int n_cu) {
-  if (rows <= 32) return FEW;
+  if (rows <= 32 || tiles_of(V, rows, Few::BM, Few::BN) <= 2 * n_cu) return FEW;
   return rows <= 128 || tiles_of(V, rows, Big::BM, Big::BN) <= n_cu / 2 ? SMALL : BIG;
 }
 
 template <class TL>
 void launch_logits(const XentArgs& a, const Product& p, int64_t r0, int64_t rows, int per_cu, hipStream_t s) {
   const unsigned grid = grid_of(tiles_of(a.V, rows, TL::BM, TL::BN), (int64_t)a.n_cu * per_cu);
-  const auto launch = [&](auto kernel) { kernel<<<grid, TL::NT, 0, s>>>(a, p, r0); };
-  if (a.planes == 1)
-    a.backward ? launch(xent_logits_kernel<TL, true, false>) : launch(xent_logits_kernel<TL, false, false>);
+  const LogitsArgs l{a.scalars, r0, a.piece_rows, a.V, a.Vp, a.softcap, a.target + r0,
+                     a.x_exp ? a.x_exp + r0 : nullptr, a.w_exp, a.at_target + r0, a.stat, a.stat_ld, a.summands};
+  const auto launch = [&](auto kernel) { kernel<<<grid, TL::NT, 0, s>>>(l, p); };
+  const auto typed = [&](auto cap) {
+    constexpr bool CAP = decltype(cap)::value;
+    if (a.planes == 1)
+      a.backward ? launch(xent_logits_kernel<TL, true, false, CAP>) : launch(xent_logits_kernel<TL, false, false, CAP>);
+    else
+      a.backward ? launch(xent_logits_kernel<TL, true, true, CAP>) : launch(xent_logits_kernel<TL, false, true, CAP>);
+  };
+  if (a.softcap > 0.0f)
+    typed(std::true_type{});
   else
-    a.backward ? launch(xent_logits_kernel<TL, true, true>) : launch(xent_logits_kernel<TL, false, true>);
+    typed(std::false_type{});
 }
 
 // The device counts the rows that take part, so it decides how tiles are split: the
@@ -755,16 +844,18 @@ void launch_grad(const XentArgs& a, const Product& p, const Out& o, int64_t r0, 
   const int64_t tiles = tiles_of(a.D, N, TL::BM, TL::BN);
   const int slots = a.n_cu * per_cu / 8 * 8;
   const int scratch = (int)(mxm_xent_partial_bytes(a.n_cu) / (TL::BM * TL::BN * 4));
-  const int64_t most = DW ? tiles % slots : std::min<int64_t>(tiles, slots - 1);
+  const int64_t most = std::min<int64_t>((DW ? tiles % slots : std::min<int64_t>(tiles, slots - 1)) * TL::TM * TL::TN * 4,
+                                         (int64_t)a.n_cu * 8);
+  const GradArgs g{a.scalars, r0, a.piece_rows, a.V, a.D, a.partial, slots, scratch};
   const auto launch = [&](auto kernel, int64_t grid) {
-    if (grid > 0) kernel<<<(unsigned)grid, TL::NT, 0, s>>>(a, p, o, r0, slots, scratch);
+    if (grid > 0) kernel<<<(unsigned)grid, TL::NT, 0, s>>>(g, p, o);
   };
   if (a.planes == 1) {
     launch(xent_grad_kernel<TL, DW, false>, slots);
-    launch(xent_grad_join_kernel<TL, DW, false>, most * TL::TM * TL::TN);
+    launch(xent_grad_join_kernel<TL, DW, false>, most);
   } else {
     launch(xent_grad_kernel<TL, DW, true>, slots);
-    launch(xent_grad_join_kernel<TL, DW, true>, most * TL::TM * TL::TN);
+    launch(xent_grad_join_kernel<TL, DW, true>, most);
   }
 }
 
@@ -778,19 +869,20 @@ int mxm_xent_block(int64_t rows, int V, int n_cu) {
 }
 
 int64_t mxm_xent_stats(int64_t rows, int V, int n_cu) {
-  // the most of any number of rows: 32-wide blocks for up to 32 of them, 64-wide ones
-  // for up to 128 or for half a round of big tiles, 128-wide ones
+  // the most of any number of rows: 32-wide blocks for up to 32 of them or a round of
+  // tiles for few rows, 64-wide ones for up to 128 or half a round of big tiles, 128-wide
   const auto of = [&](int64_t n, int block) { return n * ((V + block - 1) / block); };
-  const int64_t half = (n_cu / 2) / ((V + Big::BM - 1) / Big::BM) * Big::BN;
-  return std::max({of(rows, 128), of(std::min(rows, std::max<int64_t>(128, half)), 64),
-                   of(std::min<int64_t>(rows, 32), 32)});
+  const auto tiled = [&](int64_t tiles, int bm, int bn) { return tiles / ((V + bm - 1) / bm) * bn; };
+  const int64_t few = std::max<int64_t>(32, tiled(2 * n_cu, Few::BM, Few::BN));
+  const int64_t small = std::max<int64_t>(128, tiled(n_cu / 2, Big::BM, Big::BN));
+  return std::max({of(rows, 128), of(std::min(rows, small), 64), of(std::min(rows, few), 32)});
 }
 
 void mxm_launch_xent_logits(const XentArgs& a, int64_t r0, int64_t rows, hipStream_t s) {
   Product p{};
   set_planes(a, p);
   p.a = table(a, true);
-  p.b = hidden(a, true);
+  p.b = hidden(a, true, r0);
   p.nk = a.Dp / BK;
   switch (logits_shape(rows, a.V, a.n_cu)) {
     case FEW: return launch_logits<Few>(a, p, r0, rows, 2, s);
@@ -821,7 +913,7 @@ void mxm_launch_xent_dx(const XentArgs& a, int64_t r0, int64_t rows, hipStream_t
 void mxm_launch_xent_dw(const XentArgs& a, int64_t r0, bool last, hipStream_t s) {
   Product p{};
   set_planes(a, p);
-  p.a = hidden(a, false);
+  p.a = hidden(a, false, r0);
   p.b = grad(a);
   Out o{};
   float* sums = a.dw32 ? a.dw32 : static_cast<float*>(a.dw);
