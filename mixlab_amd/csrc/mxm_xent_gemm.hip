@@ -18,8 +18,9 @@
 // k-out ones by the transposing ds_read_b64_tr_b16: within 16 lanes, lane 4r + q
 // supplies the address of row r, columns 4q..4q+3 of a 4 x 16 block and lane i
 // receives column i (chunks swizzled by 4 * (k % 4)).  The fragments of the next
-// 16-wide k step are read between the MFMAs of the current one, the next stage's
-// loads go out over its first two.
+// 16-wide k step are read between the MFMAs of the current one; the next stage's
+// loads all go out before the first (over the first two k steps a step of 16384 rows of
+// D 2048 and 50257 entries took 9.70 ms, so 9.37).
 //
 // fp32 operands are two fp16 planes with exponents of their rows (mxm_vocab.h); of the
 // four products of planes lo lo is left out, the small ones are summed first.  (As three
@@ -51,7 +52,7 @@ typedef __attribute__((address_space(3))) bf16x4_t* lds_bf16x4_p;
 
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr int BK = 64;  // k per stage
-constexpr int GN = 8;   // n-tiles per scheduling group
+constexpr int GN = 4;   // n-tiles per scheduling group (8: 9.37 ms for that step, 4: 9.23)
 
 // global_load_lds_dwordx4: lane l's 16 bytes land at LDS `lds` + 16 l.  Inline asm,
 // so that the compiler's tracking of LDS DMA does not drain the ring; the waits are
@@ -261,7 +262,6 @@ __device__ __forceinline__ void product_tile(const Product& p, unsigned char* ld
     for (int i = 0; i < TM; ++i) af[set][i] = fragment<TL::BM, AIN>(st, ks, (wm * TM + i) * 32, lane);
   };
   constexpr int READS = TM * (AIN ? 1 : 2) + TN * (BIN ? 1 : 2);
-  constexpr int DSTEPS = 2;  // k steps that the next stage's loads are spread over
   int slot = 0;
   for (int kt = 0; kt < n; ++kt) {
     // stage kt has landed (at most NS - 2 later ones in flight) and the stage read at
@@ -273,6 +273,10 @@ __device__ __forceinline__ void product_tile(const Product& p, unsigned char* ld
     const unsigned char* st = lds + slot * TL::BUF;
     const bool more = kt + NS - 1 < n;
     const int free = slot == 0 ? NS - 1 : slot - 1;
+    if (more) {
+      load(free, 0, LDPS);
+      next();
+    }
     frags(st, 0, 0);
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
@@ -293,10 +297,6 @@ __device__ __forceinline__ void product_tile(const Product& p, unsigned char* ld
           else if (nr == 3) __builtin_amdgcn_sched_group_barrier(0x100, 3, 0);
           else if (nr >= 4) __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
         }
-      }
-      if (more && ks < DSTEPS) {
-        load(free, ks * LDPS / DSTEPS, (ks + 1) * LDPS / DSTEPS);
-        if (ks == DSTEPS - 1) next();
       }
     }
     slot = slot + 1 == NS ? 0 : slot + 1;
