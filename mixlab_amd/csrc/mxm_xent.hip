@@ -460,8 +460,16 @@ __global__ __launch_bounds__(NT) void xent_join_kernel(XentArgs a, int64_t r0, i
 
 // The summands of a piece to dz, 8 of a row per thread; under fp32 the first workgroups
 // of the rows also take x' to x'' (in place: the piece's logits are done).
-template <bool F16>
+// ONCE: past the last-level cache.
+template <bool F16, bool ONCE>
 __global__ __launch_bounds__(NT) void xent_finish_kernel(XentArgs a, int64_t r0, int block) {
+  constexpr int AHEAD = ONCE ? 4 : 1;  // units of a thread in flight
+  const auto put = [](u32x4_t v, u32x4_t* to) {
+    if constexpr (ONCE)
+      __builtin_nontemporal_store(v, to);
+    else
+      *to = v;
+  };
   const int rows = mxm_xent_rows(a, r0), units = a.Vp / 8;
   int c_top = 0;
   if constexpr (F16) {
@@ -492,44 +500,56 @@ __global__ __launch_bounds__(NT) void xent_finish_kernel(XentArgs a, int64_t r0,
         }
       }
     }
-    for (int u = blockIdx.x * NT + threadIdx.x; u < units; u += gridDim.x * NT) {
-      const int v = u * 8;
-      // (the last units may lie in padding behind the last block)
-      const float ref = v < a.V ? a.stat[(int64_t)(v / block) * a.stat_ld + m].y : r.ref;
-      const float f = r.scale * (ref == r.ref ? 1.0f : __builtin_amdgcn_exp2f(ref - r.ref));
-      float e[8];
-      const int64_t at = (int64_t)m * a.Vp + v;
-      if constexpr (!F16) {
-        const f16x8_t h = *reinterpret_cast<const f16x8_t*>(static_cast<const uint16_t*>(a.summands) + at);
+    for (int u0 = blockIdx.x * NT * AHEAD + threadIdx.x; u0 < units; u0 += gridDim.x * NT * AHEAD) {
+      u32x4_t raw[AHEAD][F16 ? 2 : 1];
+      float ref[AHEAD];
+      i32x4_t we[F16 ? AHEAD : 1][2];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) e[i] = (float)h[i] * f;
-      } else {
-        const f32x4_t* q = reinterpret_cast<const f32x4_t*>(static_cast<const float*>(a.summands) + at);
-        const f32x4_t lo = q[0], hi = q[1];
-        i32x4_t wl = {0, 0, 0, 0}, wh = {0, 0, 0, 0};
-        if (v < a.V) {
-          wl = *reinterpret_cast<const i32x4_t*>(a.w_exp + v);
-          wh = *reinterpret_cast<const i32x4_t*>(a.w_exp + v + 4);
+      for (int k = 0; k < AHEAD; ++k) {
+        // (units behind the last one: it again, not stored; a row's last ones may lie in
+        // padding behind the last block)
+        const int v = min(u0 + k * NT, units - 1) * 8;
+        const int64_t at = (int64_t)m * a.Vp + v;
+        const u32x4_t* from = reinterpret_cast<const u32x4_t*>(static_cast<const char*>(a.summands) + at * (F16 ? 4 : 2));
+        raw[k][0] = ONCE ? __builtin_nontemporal_load(from) : from[0];
+        if constexpr (F16) {
+          raw[k][1] = ONCE ? __builtin_nontemporal_load(from + 1) : from[1];
+          const i32x4_t* w = reinterpret_cast<const i32x4_t*>(a.w_exp + (v < a.V ? v : 0));
+          we[k][0] = w[0];
+          we[k][1] = w[1];
         }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          e[i] = ldexpf(lo[i] * f, wl[i] - r.exp);
-          e[4 + i] = ldexpf(hi[i] * f, wh[i] - r.exp);
-        }
+        ref[k] = v < a.V ? a.stat[(int64_t)(v / block) * a.stat_ld + m].y : r.ref;
       }
-      const int t = r.target - v;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) e[i] = i == t ? r.at_target : (v + i < a.V ? e[i] : 0.0f);
-      if constexpr (!F16) {
-        u32x4_t o;
+      for (int k = 0; k < AHEAD; ++k) {
+        if (u0 + k * NT >= units) break;
+        const int v = (u0 + k * NT) * 8;
+        const int64_t at = (int64_t)m * a.Vp + v;
+        const float f = r.scale * (ref[k] == r.ref ? 1.0f : __builtin_amdgcn_exp2f(ref[k] - r.ref));
+        float e[8];
+        if constexpr (!F16) {
+          const f16x8_t h = __builtin_bit_cast(f16x8_t, raw[k][0]);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o[i] = mxm_pack_bf2_fast(e[2 * i], e[2 * i + 1]);
-        *reinterpret_cast<u32x4_t*>(a.dz + at) = o;
-      } else {
-        u32x4_t q[2];
-        planes2x8(e, q);
-        *reinterpret_cast<u32x4_t*>(a.dz + at) = q[0];
-        *reinterpret_cast<u32x4_t*>(a.dz + a.piece_rows * a.Vp + at) = q[1];
+          for (int i = 0; i < 8; ++i) e[i] = (float)h[i] * f;
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            e[i] = ldexpf(mxm_u2f(raw[k][i / 4][i % 4]) * f, we[k][i / 4][i % 4] - r.exp);
+        }
+        const int t = r.target - v;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) e[i] = i == t ? r.at_target : (v + i < a.V ? e[i] : 0.0f);
+        if constexpr (!F16) {
+          u32x4_t o;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[i] = mxm_pack_bf2_fast(e[2 * i], e[2 * i + 1]);
+          put(o, reinterpret_cast<u32x4_t*>(a.dz + at));
+        } else {
+          u32x4_t q[2];
+          planes2x8(e, q);
+          put(q[0], reinterpret_cast<u32x4_t*>(a.dz + at));
+          put(q[1], reinterpret_cast<u32x4_t*>(a.dz + a.piece_rows * a.Vp + at));
+        }
       }
     }
   }
@@ -585,12 +605,17 @@ void mxm_launch_xent(const XentArgs& a0, hipStream_t s) {
         xent_join_kernel<<<a.c_parts, NT, 0, s>>>(a, r0, blocks);
       }
       if (a.backward) {
-        const unsigned gx = (unsigned)std::min((a.Vp / 8 + NT - 1) / NT, 64);
+        // What is past the 256 MB of the last-level cache goes around it: 2.0 GB of summands
+        // 691 us, so 605; 188 MB 69 us, so 77, and the products find less of it there.
+        const bool once = rows * a.Vp * (a.planes == 1 ? 2 : 8) > (int64_t)256 << 20;
+        const int per = NT * (once ? 4 : 1);
+        const unsigned gx = (unsigned)std::min((a.Vp / 8 + per - 1) / per, 64);
         const dim3 grid(gx, (unsigned)std::min<int64_t>(rows, std::max(1u, (unsigned)a.n_cu * 32 / gx)));
+        const auto launch = [&](auto kernel) { kernel<<<grid, NT, 0, s>>>(a, r0, block); };
         if (a.planes == 1)
-          xent_finish_kernel<false><<<grid, NT, 0, s>>>(a, r0, block);
+          once ? launch(xent_finish_kernel<false, true>) : launch(xent_finish_kernel<false, false>);
         else
-          xent_finish_kernel<true><<<grid, NT, 0, s>>>(a, r0, block);
+          once ? launch(xent_finish_kernel<true, true>) : launch(xent_finish_kernel<true, false>);
       }
       if (a.dx) mxm_launch_xent_dx(a, r0, rows, s);
     }

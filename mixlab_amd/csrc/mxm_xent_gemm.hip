@@ -93,6 +93,7 @@ struct Tile {
 };
 using Big = Tile<256, 256, 2, 4, 2, 2>;     // one workgroup per CU, 128 KB of LDS
 using Small = Tile<128, 128, 2, 2, 2, 2>;   // two per CU, 64 KB each
+using Thin = Tile<192, 256, 2, 4, 2, 2>;    // gradients of widths that 256 divides badly, 112 KB
 using Few = Tile<128, 32, 4, 1, 4, 2>;      // few rows: a stream of the table, 80 KB
 
 // One operand: `rows` of m (n) that exist, `k` of its reduction; beyond them k-inner
@@ -111,30 +112,43 @@ struct Product {
   const uint16_t* zeros;
 };
 
-// The loads of one operand's W x 64 (k-inner) or 64 x W (k-out) tile by NW waves.
+// A k-out tile's 16-byte chunk c of row k lies at c ^ swizzle: a read phase (4 rows of
+// 4 chunks) has to hit 16 distinct chunks of the 64 banks.  Rows of 256 or 128 elements
+// start at the same bank; of 192, every other one half the banks on.
+template <int W>
+__device__ __forceinline__ int out_swizzle(int k) {
+  return W == 192 ? (k & 2) << 1 : (k & 3) << 2;
+}
+
+// The loads of one operand's W x 64 (k-inner) or 64 x W (k-out) tile by NW waves; a
+// wave-load is 1 KB, 64 chunks of the tile as it lies in LDS.
 template <int W, int NW, bool INNER>
 struct Loads {
-  static constexpr int RPW = INNER ? 8 : 64 / (W / 8);  // tile rows per wave-load of 1 KB
-  static constexpr int Q = INNER ? W / 8 / NW : BK / RPW / NW;
-  static_assert(Q >= 1 && Q * RPW * NW == (INNER ? W : BK), "whole wave-loads");
-  static_assert((NW * RPW) % (INNER ? 16 : 4) == 0, "swizzle phase is the same for every load");
+  static constexpr int CR = INNER ? 8 : W / 8;          // chunks per tile row
+  static constexpr int Q = W / 8 / NW;
+  static_assert(Q >= 1 && Q * NW * 8 == W, "whole wave-loads");
+  static_assert(!INNER || (NW * 8) % 16 == 0, "swizzle phase is the same for every load");
+  // a k-out operand's rows of its loads, from the first one's: a whole number of rows, or
+  // (192 elements, 8 waves) 21 rows and a third
+  static constexpr bool EVEN = INNER || (NW * 64) % CR == 0;
   unsigned off[Q];       // bytes from the stage's base
-  int r0, chunk;         // the lane's row in load 0, its chunk's first element
+  int k[EVEN ? 1 : Q];   // the lane's k in the stage: of load 0, or of each
   const uint16_t* base;  // of the next stage to load
   __device__ __forceinline__ void init(const Operand& o, int x0, int wave, int lane) {
     if constexpr (INNER) {
-      r0 = wave * 8 + lane / 8;
-      chunk = ((lane % 8) ^ ((r0 / 2) % 8)) * 8;
+      const int r0 = wave * 8 + lane / 8, chunk = ((lane % 8) ^ ((r0 / 2) % 8)) * 8;
+      k[0] = chunk;
 #pragma unroll
       for (int q = 0; q < Q; ++q)
         off[q] = 2u * ((unsigned)min(r0 + q * NW * 8, o.rows - 1 - x0) * (unsigned)o.ld + (unsigned)chunk);
     } else {
-      r0 = wave * RPW + lane / (W / 8);
-      chunk = ((lane % (W / 8)) ^ ((r0 & 3) << 2)) * 8;
-      const int col = min(x0 + chunk, o.rows - 8);
 #pragma unroll
-      for (int q = 0; q < Q; ++q)
-        off[q] = 2u * ((unsigned)(r0 + q * NW * RPW) * (unsigned)o.ld + (unsigned)col);
+      for (int q = 0; q < Q; ++q) {
+        const int at = (wave + NW * q) * 64 + lane, r = at / CR;
+        const int col = min(x0 + ((at % CR) ^ out_swizzle<W>(r)) * 8, o.rows - 8);
+        off[q] = 2u * ((unsigned)r * (unsigned)o.ld + (unsigned)col);
+        if (q == 0 || !EVEN) k[EVEN ? 0 : q] = r;
+      }
     }
   }
   __device__ __forceinline__ void seek(const Operand& o, int x0, int plane, int k0) {
@@ -148,9 +162,9 @@ struct Loads {
   // of a stage of which only `left` k exist: zeros behind them
   __device__ __forceinline__ void load_part(int left, const uint16_t* zeros, int q, int wave,
                                             unsigned char* lds) const {
-    const int k = INNER ? chunk : r0 + q * NW * RPW;
+    const int kq = INNER ? k[0] : EVEN ? k[0] + q * (NW * 64 / CR) : k[EVEN ? 0 : q];
     const char* from = reinterpret_cast<const char*>(base) + off[q];
-    dma16(k < left ? from : reinterpret_cast<const char*>(zeros), lds + (wave + NW * q) * 1024);
+    dma16(kq < left ? from : reinterpret_cast<const char*>(zeros), lds + (wave + NW * q) * 1024);
   }
 };
 
@@ -168,7 +182,7 @@ __device__ __forceinline__ u32x4_t fragment(const unsigned char* t, int ks, int 
     for (int h = 0; h < 2; ++h) {
       const int r = ks * 16 + 8 * (lg >> 1) + 4 * h + (li >> 2);
       const int c = col + 16 * (lg & 1) + 4 * (li & 3);
-      const unsigned char* p = t + r * (W * 2) + ((c >> 3) ^ ((r & 3) << 2)) * 16 + (c & 7) * 2;
+      const unsigned char* p = t + r * (W * 2) + ((c >> 3) ^ out_swizzle<W>(r)) * 16 + (c & 7) * 2;
       v[h] = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4_p)(p)));
     }
     return u32x4_t{v[0].x, v[0].y, v[1].x, v[1].y};
@@ -859,6 +873,21 @@ void launch_grad(const XentArgs& a, const Product& p, const Out& o, int64_t r0, 
   }
 }
 
+// Small tiles where one of the product's sides is at most theirs; tiles of 192 channels
+// where they cover D with at least a tenth less than tiles of 256 (a step of 8192 rows
+// and 32768 entries at D 320: 982 us in tiles of 256, 930 of 192; D 384 1014 / 965; with
+// 6 per cent less at D 960 1681 / 1677).
+template <bool DW>
+void launch_grad(const XentArgs& a, const Product& p, const Out& o, int64_t r0, int64_t N, hipStream_t s) {
+  const auto cover = [&](int bm) { return (a.D + bm - 1) / bm * bm; };
+  if (a.D <= 128 || N <= 128)
+    launch_grad<Small, DW>(a, p, o, r0, N, 2, s);
+  else if (cover(192) * 10 <= cover(256) * 9)
+    launch_grad<Thin, DW>(a, p, o, r0, N, 1, s);
+  else
+    launch_grad<Big, DW>(a, p, o, r0, N, 1, s);
+}
+
 }  // namespace
 
 int64_t mxm_xent_partial_bytes(int n_cu) { return (int64_t)n_cu * 2 * 256 * 256 * 4; }
@@ -904,10 +933,7 @@ void mxm_launch_xent_dx(const XentArgs& a, int64_t r0, int64_t rows, hipStream_t
   o.M = a.D;
   o.bf16 = a.dx_bf16;
   o.vec = aligned(a.dx) && a.D % (a.dx_bf16 ? 8 : 4) == 0;
-  if (a.D <= 128 || rows <= 128)
-    launch_grad<Small, false>(a, p, o, r0, rows, 2, s);
-  else
-    launch_grad<Big, false>(a, p, o, r0, rows, 1, s);
+  launch_grad<false>(a, p, o, r0, rows, s);
 }
 
 void mxm_launch_xent_dw(const XentArgs& a, int64_t r0, bool last, hipStream_t s) {
@@ -924,8 +950,5 @@ void mxm_launch_xent_dw(const XentArgs& a, int64_t r0, bool last, hipStream_t s)
   o.scalars = a.scalars;
   o.M = a.D;
   o.vec = aligned(o.out) && a.D % (o.bf16 ? 8 : 4) == 0;
-  if (a.D <= 128 || a.V <= 128)
-    launch_grad<Small, true>(a, p, o, r0, a.V, 2, s);
-  else
-    launch_grad<Big, true>(a, p, o, r0, a.V, 1, s);
+  launch_grad<true>(a, p, o, r0, a.V, s);
 }
