@@ -133,7 +133,7 @@ int64_t mxm_xent_stats(int64_t rows, int V, int n_cu);
 int mxm_xent_block(int64_t rows, int V, int n_cu);
 void mxm_launch_xent_logits(const XentArgs& a, int64_t r0, int64_t rows, hipStream_t s);
 void mxm_launch_xent_dx(const XentArgs& a, int64_t r0, int64_t rows, hipStream_t s);
-void mxm_launch_xent_dw(const XentArgs& a, int64_t r0, bool last, hipStream_t s);
+void mxm_launch_xent_dw(const XentArgs& a, int64_t r0, int64_t rows, bool last, hipStream_t s);
 void mxm_launch_xent(const XentArgs& a, hipStream_t s);
 
 // Rows of the piece that starts at row r0 of those that take part.

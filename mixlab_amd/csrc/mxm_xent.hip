@@ -605,9 +605,9 @@ void mxm_launch_xent(const XentArgs& a0, hipStream_t s) {
         xent_join_kernel<<<a.c_parts, NT, 0, s>>>(a, r0, blocks);
       }
       if (a.backward) {
-        // What is past the 256 MB of the last-level cache goes around it: 2.0 GB of summands
-        // 691 us, so 605; 188 MB 69 us, so 77, and the products find less of it there.
-        const bool once = rows * a.Vp * (a.planes == 1 ? 2 : 8) > (int64_t)256 << 20;
+        // What is far past the 256 MB of the last-level cache goes around it: a step of
+        // 1.6 GB of summands 1856 us, so 1776; of 538 MB 784, so 792; of 188 MB 552, so 558.
+        const bool once = rows * a.Vp * (a.planes == 1 ? 2 : 8) > (int64_t)1 << 30;
         const int per = NT * (once ? 4 : 1);
         const unsigned gx = (unsigned)std::min((a.Vp / 8 + per - 1) / per, 64);
         const dim3 grid(gx, (unsigned)std::min<int64_t>(rows, std::max(1u, (unsigned)a.n_cu * 32 / gx)));
@@ -619,7 +619,7 @@ void mxm_launch_xent(const XentArgs& a0, hipStream_t s) {
       }
       if (a.dx) mxm_launch_xent_dx(a, r0, rows, s);
     }
-    if (a.dw) mxm_launch_xent_dw(a, r0, p == pieces - 1, s);
+    if (a.dw) mxm_launch_xent_dw(a, r0, rows, p == pieces - 1, s);
   }
   if (a.total && !total_there) xent_total_kernel<<<1, PLAN_NT, 0, s>>>(a);
 }

@@ -323,12 +323,13 @@ __device__ __forceinline__ void product_tile(const Product& p, unsigned char* ld
 // the CUs too.
 struct Split {
   int whole, tail, splits;
+  int cost;  // of all tiles, in stages of a tile
 };
 // Costs in stages: a tile's start and end, a split's way through scratch, and the
 // second launch's addition per split.
 constexpr int TILE_COST = 3, SPLIT_COST = 6, MIN_STAGES = 4;
 __host__ __device__ inline Split split_of(int tiles, int stages, int slots, int scratch_tiles) {
-  Split p{tiles / slots * slots, 0, 1};
+  Split p{tiles / slots * slots, 0, 1, tiles / slots * (stages + TILE_COST)};
   p.tail = tiles - p.whole;
   if (p.tail == 0) return p;
   int least = stages + TILE_COST;
@@ -341,6 +342,7 @@ __host__ __device__ inline Split split_of(int tiles, int stages, int slots, int 
     const int cost = need * ((stages + n - 1) / n + TILE_COST) + SPLIT_COST + n / 8;
     if (cost < least) least = cost, p.splits = n;
   }
+  p.cost += least;
   return p;
 }
 
@@ -873,16 +875,25 @@ void launch_grad(const XentArgs& a, const Product& p, const Out& o, int64_t r0, 
   }
 }
 
-// Small tiles where one of the product's sides is at most theirs; tiles of 192 channels
-// where they cover D with at least a tenth less than tiles of 256 (a step of 8192 rows
-// and 32768 entries at D 320: 982 us in tiles of 256, 930 of 192; D 384 1014 / 965; with
-// 6 per cent less at D 960 1681 / 1677).
+// The shape whose tiles take the least time by split_of's count of stages, at a stage's
+// time (Small: of two on a CU).  Measured: a step of 8192 rows and 32768 entries at D
+// 320 982 us in tiles of 256 channels, 930 of 192; D 384 1014 / 965; of 315 rows and 256
+// entries in fp32 at D 1528 89 us in tiles of 256, 76 so.
 template <bool DW>
-void launch_grad(const XentArgs& a, const Product& p, const Out& o, int64_t r0, int64_t N, hipStream_t s) {
-  const auto cover = [&](int bm) { return (a.D + bm - 1) / bm * bm; };
-  if (a.D <= 128 || N <= 128)
+void launch_grad(const XentArgs& a, const Product& p, const Out& o, int64_t r0, int64_t rows, hipStream_t s) {
+  const int64_t N = DW ? a.V : rows;
+  const int stages = (int)(DW ? (rows + BK - 1) / BK : p.nk) * p.pairs;
+  const auto time = [&](auto tile, int per_cu, double stage) {
+    using TL = decltype(tile);
+    const int slots = a.n_cu * per_cu / 8 * 8;
+    return stage * split_of((int)tiles_of(a.D, N, TL::BM, TL::BN), stages, slots,
+                            (int)(mxm_xent_partial_bytes(a.n_cu) / (TL::BM * TL::BN * 4)))
+                       .cost;
+  };
+  const double big = time(Big{}, 1, 1.0), thin = time(Thin{}, 1, 0.8), small = time(Small{}, 2, 0.65);
+  if (small < big && small < thin)
     launch_grad<Small, DW>(a, p, o, r0, N, 2, s);
-  else if (cover(192) * 10 <= cover(256) * 9)
+  else if (thin < big)
     launch_grad<Thin, DW>(a, p, o, r0, N, 1, s);
   else
     launch_grad<Big, DW>(a, p, o, r0, N, 1, s);
@@ -936,7 +947,7 @@ void mxm_launch_xent_dx(const XentArgs& a, int64_t r0, int64_t rows, hipStream_t
   launch_grad<false>(a, p, o, r0, rows, s);
 }
 
-void mxm_launch_xent_dw(const XentArgs& a, int64_t r0, bool last, hipStream_t s) {
+void mxm_launch_xent_dw(const XentArgs& a, int64_t r0, int64_t rows, bool last, hipStream_t s) {
   Product p{};
   set_planes(a, p);
   p.a = hidden(a, false, r0);
@@ -950,5 +961,5 @@ void mxm_launch_xent_dw(const XentArgs& a, int64_t r0, bool last, hipStream_t s)
   o.scalars = a.scalars;
   o.M = a.D;
   o.vec = aligned(o.out) && a.D % (o.bf16 ? 8 : 4) == 0;
-  launch_grad<true>(a, p, o, r0, a.V, s);
+  launch_grad<true>(a, p, o, r0, rows, s);
 }
