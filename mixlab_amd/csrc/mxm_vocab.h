@@ -53,12 +53,19 @@ int64_t mxm_embed_max_chunks(int64_t max_rows);
 // the largest and 2^-40 of the largest below.  Products of two such operands are
 // hi lo + lo hi + hi hi (lo lo is below 2^-23 of the product), each exact in fp32.
 // Exponents of rows along m or n of a product are applied to its sums; along k they
-// have to agree:  with E_n from the row's largest |dz| and W_v = 2^w_v W'_v
-//   dz'[n, v] = dz 2^(w_v - E_n),  dx = 2^E_n dz' W'
-//   x''_n = x'_n 2^(E_n + X_n - C),  dW_v = 2^(C - w_v) dz'^T x'',  C = max_n (E_n + X_n)
-// so that dW's terms keep 2^-40 of the largest row's, however small their own is.
+// have to agree.  With W_v = 2^c_v W'_v and x_n = 2^X_n x'_n:
+//   dz'[n, v] = dz 2^(c_v - E_n),  dx = 2^E_n dz' W'
+//   x''_n = x'_n 2^(E_n + X_n - C),  dW_v = 2^(C - c_v) dz'^T x'',  C = max_n (E_n + X_n)
+// E_n is the largest of |dz| 2^c_v, taken where the summands are, so that an entry of
+// any size without a share in the gradient has none in it.  c_v is the exponent w_v of
+// the row of weight, but where that is so small that dz' would lose digits, which dW_v
+// needs whatever the row holds (zeros, say): no smaller than L = max_n of the others'
+// largest |dz| 2^w_v over the largest |dz|, less XENT_SLACK (rows of W' below L are taken
+// down to it before product 2: with the slack, few if any of a table of alike rows; a
+// step of 733 rows of D 1528 and 256 entries took 206 us without, 76 with it).  So dx's
+// terms keep 2^-40 of their largest, and dW's 2^-36.
 // A row of weight with infinite elements is its infinities' signs and the exponent
-// XENT_INF.
+// XENT_INF, one of zeros has XENT_ZERO.
 //
 // Then, for a piece of the rows that take part at a time:
 //   product 1 (mxm_xent_gemm.hip): logits of a tile of vocabulary x rows in the
@@ -72,16 +79,20 @@ struct XentScalars {
   double weight_sum;        // of the rows that take part
   int32_t rows;             // that take part
   int32_t dw_exp;           // C
+  int32_t low[2];           // L of the pieces so far, by the last one's parity
 };
 constexpr int XENT_INF = 1 << 20;
-constexpr int XENT_NO_EXP = -(1 << 20);  // of no row
+constexpr int XENT_ZERO = -(1 << 18);
+constexpr int XENT_SLACK = 4;
+constexpr int XENT_NO_EXP = -(1 << 20);  // of nothing
 struct XentRow {            // of a row that takes part
   float ref;                // M: the summands' common exponent
   float scale;              // g / sum of all 2^(l log2 e - M)
   float at_target;          // dz of the target
   int32_t target;
-  int32_t exp;              // E (fp32)
-  int32_t x_factor;         // E + X, XENT_NO_EXP for a row without a gradient
+  // fp32: |dz| 2^w < 2^(e + 15) and |dz| < 2^(g + 15), XENT_NO_EXP for a row without a
+  // gradient
+  int32_t e, g;
 };
 struct XentArgs {
   int64_t rows;
@@ -113,9 +124,11 @@ struct XentArgs {
   uint16_t* w_pack;         // [planes][V][Dp], unused where weight is read in place
   bool w_direct;            // weight itself: bf16 rows of whole 16 bytes
   int32_t *x_exp, *w_exp;   // [rows], [V up to whole tiles]: X, w (fp32)
-  int32_t *w_part, *c_part; // the largest of w and of E + X of each workgroup that packs
-  int w_parts, c_parts;     // the table, or joins rows
+  int32_t* e_row;           // [rows]: E
+  int4* c_part;             // of each workgroup that joins rows the largest others' e - g,
+  int c_parts;              // e + X and g + X
   float2* stat;             // [blocks][stat_ld]: sum, ref
+  int32_t* stat_exp;        // [blocks][stat_ld] (fp32 backward): the exponent of summand 2^w
   void* summands;           // [piece_rows][Vp]: fp16 (bf16) or fp32
   uint16_t* dz;             // [planes][piece_rows][Vp]: the summands' place under bf16
   float* partial;           // tiles of products that are split along their sums
@@ -124,16 +137,17 @@ struct XentArgs {
   int64_t piece_rows, stat_ld;
   int n_cu;
 };
-constexpr int XENT_W_PARTS = 4096;  // most workgroups that pack the table
 // Bytes of partial, for handles that run backward.
 int64_t mxm_xent_partial_bytes(int n_cu);
 // Most blocks of stat times rows, for pieces of `rows`.
 int64_t mxm_xent_stats(int64_t rows, int V, int n_cu);
 // Columns of the vocabulary per block of stat, for a piece of `rows` rows.
 int mxm_xent_block(int64_t rows, int V, int n_cu);
-void mxm_launch_xent_logits(const XentArgs& a, int64_t r0, int64_t rows, hipStream_t s);
+// low: where the pieces before left L, or null.
+void mxm_launch_xent_logits(const XentArgs& a, int64_t r0, int64_t rows, const int32_t* low, hipStream_t s);
 void mxm_launch_xent_dx(const XentArgs& a, int64_t r0, int64_t rows, hipStream_t s);
-void mxm_launch_xent_dw(const XentArgs& a, int64_t r0, int64_t rows, bool last, hipStream_t s);
+void mxm_launch_xent_dw(const XentArgs& a, int64_t r0, int64_t rows, bool last, const int32_t* low,
+                        hipStream_t s);
 void mxm_launch_xent(const XentArgs& a, hipStream_t s);
 
 // Rows of the piece that starts at row r0 of those that take part.

@@ -26,7 +26,7 @@ struct Xent : TrainHandle {
   XentArgs base{};
   int64_t max_rows = 0;
   bool backward = false;
-  DevBuf slot, map, target, scalars, nll, at_target, row, x_pack, w_pack, exps, stat, summands, dz, partial, dw32, zeros;
+  DevBuf slot, map, target, scalars, nll, at_target, row, x_pack, w_pack, exps, parts, stat, stat_exp, summands, dz, partial, dw32, zeros;
   ~Xent() override {
     if (stream_ref) (void)hipStreamSynchronize(stream());
   }
@@ -261,7 +261,7 @@ int64_t mxm_xent_create(const int64_t* params, int n_params, float softcap, int6
     // (and under fp32 their gradient's planes)
     int64_t bytes = XENT_PIECE_BYTES;
     if (const char* env = std::getenv("MXM_XENT_PIECE_BYTES")) bytes = std::max(0ll, std::atoll(env));
-    const int64_t row_bytes = (V + 127) / 128 * 8 + (x->backward ? a.Vp * (int64_t)(a.bf16 ? 2 : 8) : 0);
+    const int64_t row_bytes = (V + 127) / 128 * (x->backward && !a.bf16 ? 12 : 8) + (x->backward ? a.Vp * (int64_t)(a.bf16 ? 2 : 8) : 0);
     a.piece_rows = std::max<int64_t>(256, std::min(up(rows), bytes / row_bytes / 256 * 256));
     if (rows < a.piece_rows) a.piece_rows = std::max<int64_t>(64, up(rows));
     x->slot.alloc((size_t)rows * 4);
@@ -274,12 +274,17 @@ int64_t mxm_xent_create(const int64_t* params, int n_params, float softcap, int6
     x->w_pack.alloc((size_t)V * a.Dp * 2 * a.planes);
     x->stat.alloc((size_t)mxm_xent_stats(a.piece_rows, a.V, a.n_cu) * sizeof(float2));
     if (!a.bf16) {
-      const size_t v_tiles = ((size_t)V + 255) / 256 * 256, n = (size_t)rows, joins = (size_t)rows / 16 + 1;
-      x->exps.alloc((n + v_tiles + XENT_W_PARTS + joins) * 4 + 64);
+      const size_t v_tiles = ((size_t)V + 255) / 256 * 256, n = (size_t)rows;
+      x->exps.alloc((v_tiles + 2 * n) * 4);
       a.w_exp = x->exps.as<int32_t>();  // (first: read by vectors)
       a.x_exp = a.w_exp + v_tiles;
-      a.w_part = a.x_exp + n;
-      a.c_part = a.w_part + XENT_W_PARTS;
+      a.e_row = a.x_exp + n;
+      if (x->backward) {
+        x->parts.alloc((n / 16 + 1) * sizeof(int4));
+        x->stat_exp.alloc((size_t)mxm_xent_stats(a.piece_rows, a.V, a.n_cu) * 4);
+        a.c_part = x->parts.as<int4>();
+        a.stat_exp = x->stat_exp.as<int32_t>();
+      }
     }
     x->zeros.alloc(4096);
     HIPCK(hipMemsetAsync(x->zeros.p, 0, 4096, x->stream()));

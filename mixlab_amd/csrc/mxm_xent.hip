@@ -151,7 +151,7 @@ __device__ __forceinline__ int pack_row32(const XentArgs& a, const void* p, bool
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o));
   const bool signs = WEIGHT && __ballot(inf) != 0;
-  int e = 0;
+  int e = WEIGHT ? XENT_ZERO : 0;
   if (top != 0) {
     (void)frexpf(mxm_u2f(top), &e);
     e = max(e - 15, -126);
@@ -209,21 +209,13 @@ __global__ __launch_bounds__(NT) void xent_pack_kernel(XentArgs a, int x_blocks)
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   if ((int)blockIdx.x >= x_blocks) {
     const bool wide = wide_rows(a, a.weight);
-    int most = XENT_NO_EXP;
     for (int64_t v = (int64_t)(blockIdx.x - x_blocks) * 4 + wave; v < a.V; v += (int64_t)(gridDim.x - x_blocks) * 4) {
       if (a.planes == 1) {
         pack_row(a, a.weight, wide, v, a.w_pack, v, lane);
       } else {
         const int e = pack_row32<true>(a, a.weight, wide, v, a.w_pack, a.V, v, lane);
         if (lane == 0) a.w_exp[v] = e;
-        if (e < XENT_INF) most = max(most, e);
       }
-    }
-    if (a.planes != 1) {
-      if (lane == 0) count[0][wave] = most;
-      __syncthreads();
-      if (threadIdx.x == 0)
-        a.w_part[blockIdx.x - x_blocks] = max(max(count[0][0], count[0][1]), max(count[0][2], count[0][3]));
     }
     return;
   }
@@ -296,22 +288,39 @@ __global__ __launch_bounds__(NT) void xent_pack_kernel(XentArgs a, int x_blocks)
   }
 }
 
-// What a set of exponentials sums to: sum * 2^top.
+// What a set of exponentials sums to: sum * 2^top; exp: that of the largest summand times
+// 2^w, over 2^top too.
 struct Sum {
   float top, sum;
+  int exp;
 };
+__device__ __forceinline__ int moved(int exp, float top, float up) {
+  return top == up ? exp : max(exp + (int)fmaxf(top - up, (float)XENT_NO_EXP), XENT_NO_EXP);
+}
 __device__ __forceinline__ Sum join(Sum p, Sum q) {
   // (no difference of equal ones: they may be infinite)
   const float up = fmaxf(p.top, q.top);
-  return {up, p.sum * (p.top == up ? 1.0f : __builtin_amdgcn_exp2f(p.top - up)) +
-                  q.sum * (q.top == up ? 1.0f : __builtin_amdgcn_exp2f(q.top - up))};
+  return {up,
+          p.sum * (p.top == up ? 1.0f : __builtin_amdgcn_exp2f(p.top - up)) +
+              q.sum * (q.top == up ? 1.0f : __builtin_amdgcn_exp2f(q.top - up)),
+          max(moved(p.exp, p.top, up), moved(q.exp, q.top, up))};
+}
+__device__ __forceinline__ Sum of_lane(Sum s, int mask) {
+  return {__shfl_xor(s.top, mask), __shfl_xor(s.sum, mask), __shfl_xor(s.exp, mask)};
 }
 // Blocks part, part + parts, ... of row m.
 __device__ __forceinline__ Sum blocks_of(const XentArgs& a, int m, int part, int parts, int blocks) {
   constexpr int AHEAD = 8;
-  Sum all = {-__builtin_inff(), 0.0f};
+  const bool exps = a.backward && a.planes != 1;
+  Sum all = {-__builtin_inff(), 0.0f, XENT_NO_EXP};
   for (int b = part; b < blocks; b += AHEAD * parts) {
     float2 e[AHEAD];
+    int x[AHEAD];
+    if (exps) {
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k)
+        x[k] = b + k * parts < blocks ? a.stat_exp[(int64_t)(b + k * parts) * a.stat_ld + m] : XENT_NO_EXP;
+    }
 #pragma unroll
     for (int k = 0; k < AHEAD; ++k)
       e[k] = b + k * parts < blocks ? a.stat[(int64_t)(b + k * parts) * a.stat_ld + m]
@@ -322,15 +331,36 @@ __device__ __forceinline__ Sum blocks_of(const XentArgs& a, int m, int part, int
     float s = all.sum * (all.top == up ? 1.0f : __builtin_amdgcn_exp2f(all.top - up));
 #pragma unroll
     for (int k = 0; k < AHEAD; ++k) s += e[k].x * (e[k].y == up ? 1.0f : __builtin_amdgcn_exp2f(e[k].y - up));
-    all = {up, s};
+    int most = XENT_NO_EXP;
+    if (exps) {
+      most = moved(all.exp, all.top, up);
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) most = max(most, moved(x[k], e[k].y, up));
+    }
+    all = {up, s, most};
   }
   return all;
 }
 
-// Row m's loss and the factors of its gradient from the others' sum; w_top: the largest
-// w.  The row's E + X goes to x_factor.
-__device__ __forceinline__ float finish_row(const XentArgs& a, int64_t r0, int m, Sum others, int w_top,
-                                            int& x_factor) {
+// Largest exponents of some rows: c_part's.
+struct Exps {
+  int low, e, g;
+  __device__ __forceinline__ void take(const Exps& o) {
+    low = max(low, o.low);
+    e = max(e, o.e);
+    g = max(g, o.g);
+  }
+  __device__ __forceinline__ void take_wave() {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1)
+      take({__shfl_xor(low, o), __shfl_xor(e, o), __shfl_xor(g, o)});
+  }
+};
+
+constexpr Exps NO_EXPS{XENT_NO_EXP, XENT_NO_EXP, XENT_NO_EXP};
+
+// Row m's loss and the factors of its gradient from the others' sum.
+__device__ __forceinline__ float finish_row(const XentArgs& a, int64_t r0, int m, Sum others, Exps& exps) {
   // the others' sum is sum * 2^top, the target's exponential 2^(top - d)
   const float top = others.top, sum = others.sum;
   float lt = a.at_target[r0 + m], slope = 1.0f;
@@ -357,37 +387,27 @@ __device__ __forceinline__ float finish_row(const XentArgs& a, int64_t r0, int m
     r.scale = g / whole;
     r.at_target = -g * (sum / whole) * slope;
     r.target = a.target[r0 + m];
-    r.exp = 0;
-    r.x_factor = XENT_NO_EXP;
+    r.e = r.g = XENT_NO_EXP;
     if (a.planes != 1) {
       // no |dz| of the row is above |g| times the others' share
       const float most = __builtin_fabsf(g) * (sum / whole);
       if (most > 0.0f && most < __builtin_inff()) {
         int e;
         (void)frexpf(most, &e);
-        r.exp = e + w_top - 15;
-        r.x_factor = r.exp + a.x_exp[r0 + m];
+        r.g = e - 15;
+        (void)frexpf(r.scale, &e);
+        const int of_others = others.exp > XENT_NO_EXP / 2 ? others.exp + e - 15 : XENT_NO_EXP;
+        (void)frexpf(r.at_target, &e);
+        const int w = a.w_exp[r.target];
+        const int of_target = w < XENT_INF && r.at_target != 0.0f ? w + e - 15 : XENT_NO_EXP;
+        r.e = max(of_others, of_target);
+        const int low = of_others > XENT_NO_EXP ? of_others : of_target;
+        exps.take({low > XENT_NO_EXP ? low - r.g - XENT_SLACK : XENT_NO_EXP, r.e + a.x_exp[r0 + m], r.g + a.x_exp[r0 + m]});
       }
-      r.at_target = ldexpf(r.at_target, a.w_exp[r.target] - r.exp);
     }
-    x_factor = r.x_factor;
     a.row[r0 + m] = r;
   }
   return loss;
-}
-
-// The largest w of all that packed the table (0: none but zeros and infinities).
-template <int T>
-__device__ __forceinline__ int largest_w(const XentArgs& a, int* lds) {
-  if (!a.backward || a.planes == 1) return 0;
-  int most = XENT_NO_EXP;
-  for (int i = threadIdx.x; i < a.w_parts; i += T) most = max(most, a.w_part[i]);
-  most = wave_max(most);
-  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = most;
-  __syncthreads();
-  for (int i = 0; i < T / 64; ++i) most = max(most, lds[i]);
-  __syncthreads();
-  return most == XENT_NO_EXP ? 0 : most;
 }
 
 // Few rows: a wave each.  With one workgroup for all of them it also sums the total.
@@ -395,28 +415,26 @@ constexpr int JOIN_WAVES = 16, JOIN_FEW = 512;
 __global__ __launch_bounds__(64 * JOIN_WAVES) void xent_join_few_kernel(XentArgs a, int64_t r0, int blocks,
                                                                         bool total) {
   __shared__ double part[JOIN_WAVES];
-  __shared__ int exps[JOIN_WAVES];
+  __shared__ Exps each[JOIN_WAVES];
   const int rows = mxm_xent_rows(a, r0), lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int m = blockIdx.x * JOIN_WAVES + wave;
-  const int w_top = largest_w<64 * JOIN_WAVES>(a, exps);
-  int x_factor = XENT_NO_EXP;
+  Exps exps = NO_EXPS;
   double sum = 0.0;
   if (m < rows) {
     Sum s = blocks_of(a, m, lane, 64, blocks);
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) s = join(s, {__shfl_xor(s.top, o), __shfl_xor(s.sum, o)});
+    for (int o = 1; o < 64; o <<= 1) s = join(s, of_lane(s, o));
     if (lane == 0) {
-      const float loss = finish_row(a, r0, m, s, w_top, x_factor);
+      const float loss = finish_row(a, r0, m, s, exps);
       sum = (double)loss * (a.row_weights ? (double)a.row_weights[a.map[r0 + m]] : 1.0);
     }
   }
   if (a.backward && a.planes != 1) {
-    if (lane == 0) exps[wave] = x_factor;
+    if (lane == 0) each[wave] = exps;
     __syncthreads();
     if (threadIdx.x == 0) {
-      int most = exps[0];
-      for (int i = 1; i < JOIN_WAVES; ++i) most = max(most, exps[i]);
-      a.c_part[blockIdx.x] = most;
+      for (int i = 1; i < JOIN_WAVES; ++i) exps.take(each[i]);
+      a.c_part[blockIdx.x] = make_int4(exps.low, exps.e, exps.g, 0);
     }
   }
   if (!total) return;
@@ -434,35 +452,34 @@ __global__ __launch_bounds__(64 * JOIN_WAVES) void xent_join_few_kernel(XentArgs
 constexpr int JOIN_ROWS = 16;
 __global__ __launch_bounds__(NT) void xent_join_kernel(XentArgs a, int64_t r0, int blocks) {
   __shared__ Sum red[4][JOIN_ROWS];
-  __shared__ int exps[4];
   const int rows = mxm_xent_rows(a, r0);
   const int k = threadIdx.x & 15, m = blockIdx.x * JOIN_ROWS + k;
   const bool exponents = a.backward && a.planes != 1;
   if (blockIdx.x * JOIN_ROWS >= rows) {
-    if (exponents && threadIdx.x == 0) a.c_part[blockIdx.x] = XENT_NO_EXP;
+    if (exponents && threadIdx.x == 0) a.c_part[blockIdx.x] = make_int4(XENT_NO_EXP, XENT_NO_EXP, XENT_NO_EXP, 0);
     return;
   }
-  const int w_top = largest_w<NT>(a, exps);
   Sum s = blocks_of(a, min(m, rows - 1), threadIdx.x >> 4, 16, blocks);
-  s = join(s, {__shfl_xor(s.top, 16), __shfl_xor(s.sum, 16)});
-  s = join(s, {__shfl_xor(s.top, 32), __shfl_xor(s.sum, 32)});
+  s = join(s, of_lane(s, 16));
+  s = join(s, of_lane(s, 32));
   if ((threadIdx.x & 63) < 16) red[threadIdx.x >> 6][k] = s;
   __syncthreads();
   if (threadIdx.x >= 64) return;
-  int x_factor = XENT_NO_EXP;
+  Exps exps = NO_EXPS;
   if (threadIdx.x < 16 && m < rows)
-    finish_row(a, r0, m, join(join(red[0][k], red[1][k]), join(red[2][k], red[3][k])), w_top, x_factor);
+    finish_row(a, r0, m, join(join(red[0][k], red[1][k]), join(red[2][k], red[3][k])), exps);
   if (exponents) {
-    x_factor = wave_max(x_factor);
-    if (threadIdx.x == 0) a.c_part[blockIdx.x] = x_factor;
+    exps.take_wave();
+    if (threadIdx.x == 0) a.c_part[blockIdx.x] = make_int4(exps.low, exps.e, exps.g, 0);
   }
 }
 
 // The summands of a piece to dz, 8 of a row per thread; under fp32 the first workgroups
-// of the rows also take x' to x'' (in place: the piece's logits are done).
-// ONCE: past the last-level cache.
+// of the rows also take x' to x'', and all of them the rows of W' below L to it (in
+// place: the piece's logits are done).  ONCE: past the last-level cache.
 template <bool F16, bool ONCE>
-__global__ __launch_bounds__(NT) void xent_finish_kernel(XentArgs a, int64_t r0, int block) {
+__global__ __launch_bounds__(NT) void xent_finish_kernel(XentArgs a, int64_t r0, int block, int parity,
+                                                           bool first) {
   constexpr int AHEAD = ONCE ? 4 : 1;  // units of a thread in flight
   const auto put = [](u32x4_t v, u32x4_t* to) {
     if constexpr (ONCE)
@@ -471,32 +488,69 @@ __global__ __launch_bounds__(NT) void xent_finish_kernel(XentArgs a, int64_t r0,
       *to = v;
   };
   const int rows = mxm_xent_rows(a, r0), units = a.Vp / 8;
-  int c_top = 0;
+  int c_top = 0, low = XENT_NO_EXP;
   if constexpr (F16) {
-    __shared__ int exps[4];
-    if (blockIdx.x == 0 && a.dw) {
-      c_top = XENT_NO_EXP;
-      for (int i = threadIdx.x; i < a.c_parts; i += NT) c_top = max(c_top, a.c_part[i]);
-      c_top = wave_max(c_top);
-      if ((threadIdx.x & 63) == 0) exps[threadIdx.x >> 6] = c_top;
-      __syncthreads();
-      c_top = max(max(exps[0], exps[1]), max(exps[2], exps[3]));
-      if (blockIdx.y == 0 && threadIdx.x == 0) a.scalars->dw_exp = c_top == XENT_NO_EXP ? 0 : c_top;
+    __shared__ Exps each[NT / 64];
+    Exps all = NO_EXPS;
+    for (int i = threadIdx.x; i < a.c_parts; i += NT) {
+      const int4 c = a.c_part[i];
+      all.take({c.x, c.y, c.z});
+    }
+    all.take_wave();
+    if ((threadIdx.x & 63) == 0) each[threadIdx.x >> 6] = all;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < NT / 64; ++i) all.take(each[i]);
+    const int before = first ? XENT_NO_EXP : a.scalars->low[parity ^ 1];
+    low = max(all.low, before);
+    c_top = all.g == XENT_NO_EXP ? 0 : max(all.e, all.g + max(low, XENT_ZERO));
+    const int id = blockIdx.y * gridDim.x + blockIdx.x;
+    if (id == 0 && threadIdx.x == 0) {
+      a.scalars->dw_exp = c_top;
+      a.scalars->low[parity] = low;
+    }
+    if (a.dx) {
+      const int lane = threadIdx.x & 63;
+      // (four rows a wave: where many need it, in a small table, all waves work)
+      for (int v0 = (id * (NT / 64) + (threadIdx.x >> 6)) * 4; v0 < a.V; v0 += gridDim.x * gridDim.y * (NT / 16)) {
+        const int v = v0 + (lane & 3), w = v < a.V ? a.w_exp[v] : XENT_ZERO;
+        const int now = max(w, before);
+        unsigned todo = (unsigned)__ballot(w != XENT_ZERO && now < low) & 15u;
+        while (todo != 0) {
+          const int at = __ffs(todo) - 1;
+          todo &= todo - 1;
+          const int64_t row = v0 + at;
+          const int by = __shfl(now, at) - low;
+          for (int u = lane; u < 2 * (a.Dp / 8); u += 64) {
+            const int pl = u >= a.Dp / 8;
+            f16x8_t* q = reinterpret_cast<f16x8_t*>(a.w_pack + (pl * (int64_t)a.V + row) * a.Dp) + (u - pl * (a.Dp / 8));
+            f16x8_t h = *q;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) h[i] = (_Float16)ldexpf((float)h[i], by);
+            *q = h;
+          }
+        }
+      }
     }
   }
   for (int m = blockIdx.y; m < rows; m += gridDim.y) {
     const XentRow r = a.row[r0 + m];
+    int row_exp = 0;
     if constexpr (F16) {
-      if (blockIdx.x == 0 && a.dw) {
-        const float f = r.x_factor == XENT_NO_EXP ? 0.0f : ldexpf(1.0f, r.x_factor - c_top);
-        for (int u = threadIdx.x; u < 2 * (a.Dp / 8); u += NT) {
-          const int pl = u >= a.Dp / 8;
-          f16x8_t* q = reinterpret_cast<f16x8_t*>(a.x_pack + pl * (a.x_rows * a.Dp) + (r0 + m) * a.Dp) +
-                       (u - pl * (a.Dp / 8));
-          f16x8_t v = *q;
+      if (r.g != XENT_NO_EXP) row_exp = max(r.e, r.g + max(low, XENT_ZERO));
+      if (blockIdx.x == 0) {
+        if (threadIdx.x == 0) a.e_row[r0 + m] = row_exp;
+        if (a.dw) {
+          const float f = r.g == XENT_NO_EXP ? 0.0f : ldexpf(1.0f, row_exp + a.x_exp[r0 + m] - c_top);
+          for (int u = threadIdx.x; u < 2 * (a.Dp / 8); u += NT) {
+            const int pl = u >= a.Dp / 8;
+            f16x8_t* q = reinterpret_cast<f16x8_t*>(a.x_pack + pl * (a.x_rows * a.Dp) + (r0 + m) * a.Dp) +
+                         (u - pl * (a.Dp / 8));
+            f16x8_t v = *q;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) v[i] = (_Float16)((float)v[i] * f);
-          *q = v;
+            for (int i = 0; i < 8; ++i) v[i] = (_Float16)((float)v[i] * f);
+            *q = v;
+          }
         }
       }
     }
@@ -534,11 +588,15 @@ __global__ __launch_bounds__(NT) void xent_finish_kernel(XentArgs a, int64_t r0,
         } else {
 #pragma unroll
           for (int i = 0; i < 8; ++i)
-            e[i] = ldexpf(mxm_u2f(raw[k][i / 4][i % 4]) * f, we[k][i / 4][i % 4] - r.exp);
+            e[i] = ldexpf(mxm_u2f(raw[k][i / 4][i % 4]) * f, max(we[k][i / 4][i % 4], low) - row_exp);
         }
         const int t = r.target - v;
+        float at_target = r.at_target;
+        if constexpr (F16) {
+          if (t >= 0 && t < 8) at_target = ldexpf(at_target, max(a.w_exp[r.target], low) - row_exp);
+        }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) e[i] = i == t ? r.at_target : (v + i < a.V ? e[i] : 0.0f);
+        for (int i = 0; i < 8; ++i) e[i] = i == t ? at_target : (v + i < a.V ? e[i] : 0.0f);
         if constexpr (!F16) {
           u32x4_t o;
 #pragma unroll
@@ -581,8 +639,7 @@ void mxm_launch_xent(const XentArgs& a0, hipStream_t s) {
   const bool plan = a.rows > 0 && a.rows <= PLAN_ROWS;
   if (!plan) xent_plan_kernel<<<1, PLAN_NT, 0, s>>>(a);
   if (a.rows > 0) {
-    const unsigned gx = rows_grid(a.rows), gw = a.w_direct ? 0 : std::min<unsigned>(rows_grid(a.V), XENT_W_PARTS);
-    a.w_parts = (int)gw;
+    const unsigned gx = rows_grid(a.rows), gw = a.w_direct ? 0 : rows_grid(a.V);
     if (plan)
       xent_pack_kernel<true><<<gx + gw, NT, 0, s>>>(a, (int)gx);
     else
@@ -592,10 +649,11 @@ void mxm_launch_xent(const XentArgs& a0, hipStream_t s) {
   const bool total_there = a.total && a.rows > 0 && a.rows <= JOIN_WAVES;  // (one piece)
   for (int64_t p = 0; p < pieces; ++p) {
     const int64_t r0 = p * a.piece_rows, rows = std::min(a.rows - r0, a.piece_rows);
+    const int parity = (int)(p & 1);
     if (rows > 0) {
       const int block = mxm_xent_block(rows, a.V, a.n_cu);
       a.stat_ld = rows;
-      mxm_launch_xent_logits(a, r0, rows, s);
+      mxm_launch_xent_logits(a, r0, rows, a.planes != 1 && a.dx && p > 0 ? a.scalars->low + (parity ^ 1) : nullptr, s);
       const int blocks = (a.V + block - 1) / block;
       if (rows <= JOIN_FEW) {
         a.c_parts = (int)((rows + JOIN_WAVES - 1) / JOIN_WAVES);
@@ -611,7 +669,7 @@ void mxm_launch_xent(const XentArgs& a0, hipStream_t s) {
         const int per = NT * (once ? 4 : 1);
         const unsigned gx = (unsigned)std::min((a.Vp / 8 + per - 1) / per, 64);
         const dim3 grid(gx, (unsigned)std::min<int64_t>(rows, std::max(1u, (unsigned)a.n_cu * 32 / gx)));
-        const auto launch = [&](auto kernel) { kernel<<<grid, NT, 0, s>>>(a, r0, block); };
+        const auto launch = [&](auto kernel) { kernel<<<grid, NT, 0, s>>>(a, r0, block, parity, p == 0); };
         if (a.planes == 1)
           once ? launch(xent_finish_kernel<false, true>) : launch(xent_finish_kernel<false, false>);
         else
@@ -619,7 +677,7 @@ void mxm_launch_xent(const XentArgs& a0, hipStream_t s) {
       }
       if (a.dx) mxm_launch_xent_dx(a, r0, rows, s);
     }
-    if (a.dw) mxm_launch_xent_dw(a, r0, rows, p == pieces - 1, s);
+    if (a.dw) mxm_launch_xent_dw(a, r0, rows, p == pieces - 1, a.scalars->low + parity, s);
   }
   if (a.total && !total_there) xent_total_kernel<<<1, PLAN_NT, 0, s>>>(a);
 }

@@ -436,7 +436,9 @@ struct LogitsArgs {
   float softcap;
   const int32_t *target, *x_exp, *w_exp;
   float* at_target;
+  const int32_t* low;
   float2* stat;
+  int32_t* stat_exp;
   int64_t stat_ld;
   void* summands;
 };
@@ -478,7 +480,10 @@ __global__ __launch_bounds__(TL::NT, TL::WPS) void xent_logits_kernel(LogitsArgs
     }
     // (the sum's barriers stand between this and the epilogue)
     if constexpr (F16)
-      for (int i = threadIdx.x; i < TL::BM; i += TL::NT) w_exp[i] = a.w_exp[m0 + i];
+      for (int i = threadIdx.x; i < TL::BM; i += TL::NT) {
+        const int e = a.w_exp[m0 + i];
+        w_exp[i] = a.low ? max(e, *a.low) : e;
+      }
     f32x16_t acc[TM][TN];
     product_tile<TL, true, true, F16>(p, lds, m0, n0, 0, p.nk * p.pairs, acc);
     const int mw = m0 + wm * TM * 32;  // the wave's block of the vocabulary
@@ -552,8 +557,23 @@ __global__ __launch_bounds__(TL::NT, TL::WPS) void xent_logits_kernel(LogitsArgs
       }
       float sum = s[0] + s[1];
       sum += mxm_xor_lane_f(sum, 32);
-      if (n < rows && mw < a.V && lane < 32)
-        a.stat[(int64_t)(mw / (TM * 32)) * a.stat_ld + n] = make_float2(sum, ref);
+      const int64_t at_stat = (int64_t)(mw / (TM * 32)) * a.stat_ld + n;
+      if (n < rows && mw < a.V && lane < 32) a.stat[at_stat] = make_float2(sum, ref);
+      if constexpr (F16 && STORE) {
+        // (2^(w - 1): none overflows)
+        float big = 0.0f;
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const i32x4_t we = *reinterpret_cast<const i32x4_t*>(w_exp + first - m0 + i * 32 + q * 8);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) big = fmaxf(big, ldexpf(acc[i][j][q * 4 + k], we[k] - 1));
+          }
+        big = fmaxf(big, mxm_xor_lane_f(big, 32));
+        if (n < rows && mw < a.V && lane < 32)
+          a.stat_exp[at_stat] = big > 0.0f ? __builtin_amdgcn_frexp_expf(big) + 1 : XENT_NO_EXP;
+      }
       if constexpr (STORE) {
         constexpr int BITS = F16 ? 32 : 16, PER = 128 / BITS;
         using R = Rows<TM, BITS>;
@@ -585,18 +605,23 @@ struct Out {
   void* out;
   const float* add;      // earlier sums of the same elements, or null
   const int32_t* map;    // the row that n is, or null: n
-  const XentRow* row;    // fp32: the exponents of n's sums: dx's E,
-  const int32_t* w_exp;  // or dw's C - w
+  const int32_t* e_row;  // fp32: the exponents of n's sums: dx's E,
+  const int32_t* w_exp;  // or dw's C - max(w, L)
+  const int32_t* low;
   const XentScalars* scalars;
   int M;
   bool bf16, vec;        // vec: rows of whole aligned 16 bytes
 };
 
+__device__ __forceinline__ int exp_of(const Out& o, int n) {
+  return o.e_row ? o.e_row[n] : o.scalars->dw_exp - max(o.w_exp[n], *o.low);
+}
+
 // Row n's elements m .. m + 3 of an MFMA tile, as each quad of registers holds them.
 template <bool F16>
 __device__ __forceinline__ void put_tile(const Out& o, int m_first, int n, bool in, int lane, f32x16_t c) {
   if constexpr (F16) {
-    const int e = !in ? 0 : o.row ? o.row[n].exp : o.scalars->dw_exp - o.w_exp[n];
+    const int e = !in ? 0 : exp_of(o, n);
 #pragma unroll
     for (int r = 0; r < 16; ++r) c[r] = ldexpf(c[r], e);
   }
@@ -650,7 +675,7 @@ template <bool F16>
 __device__ __forceinline__ void put_quad(const Out& o, int m, int n, f32x4_t c) {
   if (m >= o.M) return;
   if constexpr (F16) {
-    const int e = o.row ? o.row[n].exp : o.scalars->dw_exp - o.w_exp[n];
+    const int e = exp_of(o, n);
 #pragma unroll
     for (int k = 0; k < 4; ++k) c[k] = ldexpf(c[k], e);
   }
@@ -834,10 +859,12 @@ Shape logits_shape(int64_t rows, int V, int n_cu) {
 }
 
 template <class TL>
-void launch_logits(const XentArgs& a, const Product& p, int64_t r0, int64_t rows, int per_cu, hipStream_t s) {
+void launch_logits(const XentArgs& a, const Product& p, int64_t r0, int64_t rows, const int32_t* low, int per_cu,
+                   hipStream_t s) {
   const unsigned grid = grid_of(tiles_of(a.V, rows, TL::BM, TL::BN), (int64_t)a.n_cu * per_cu);
   const LogitsArgs l{a.scalars, r0, a.piece_rows, a.V, a.Vp, a.softcap, a.target + r0,
-                     a.x_exp ? a.x_exp + r0 : nullptr, a.w_exp, a.at_target + r0, a.stat, a.stat_ld, a.summands};
+                     a.x_exp ? a.x_exp + r0 : nullptr, a.w_exp, a.at_target + r0, low, a.stat, a.stat_exp,
+                     a.stat_ld, a.summands};
   const auto launch = [&](auto kernel) { kernel<<<grid, TL::NT, 0, s>>>(l, p); };
   const auto typed = [&](auto cap) {
     constexpr bool CAP = decltype(cap)::value;
@@ -918,16 +945,16 @@ int64_t mxm_xent_stats(int64_t rows, int V, int n_cu) {
   return std::max({of(rows, 128), of(std::min(rows, small), 64), of(std::min(rows, few), 32)});
 }
 
-void mxm_launch_xent_logits(const XentArgs& a, int64_t r0, int64_t rows, hipStream_t s) {
+void mxm_launch_xent_logits(const XentArgs& a, int64_t r0, int64_t rows, const int32_t* low, hipStream_t s) {
   Product p{};
   set_planes(a, p);
   p.a = table(a, true);
   p.b = hidden(a, true, r0);
   p.nk = a.Dp / BK;
   switch (logits_shape(rows, a.V, a.n_cu)) {
-    case FEW: return launch_logits<Few>(a, p, r0, rows, 2, s);
-    case SMALL: return launch_logits<Small>(a, p, r0, rows, 2, s);
-    default: return launch_logits<Big>(a, p, r0, rows, 1, s);
+    case FEW: return launch_logits<Few>(a, p, r0, rows, low, 2, s);
+    case SMALL: return launch_logits<Small>(a, p, r0, rows, low, 2, s);
+    default: return launch_logits<Big>(a, p, r0, rows, low, 1, s);
   }
 }
 
@@ -940,14 +967,15 @@ void mxm_launch_xent_dx(const XentArgs& a, int64_t r0, int64_t rows, hipStream_t
   Out o{};
   o.out = a.dx;
   o.map = a.map + r0;
-  o.row = a.row + r0;
+  o.e_row = a.e_row + r0;
   o.M = a.D;
   o.bf16 = a.dx_bf16;
   o.vec = aligned(a.dx) && a.D % (a.dx_bf16 ? 8 : 4) == 0;
   launch_grad<false>(a, p, o, r0, rows, s);
 }
 
-void mxm_launch_xent_dw(const XentArgs& a, int64_t r0, int64_t rows, bool last, hipStream_t s) {
+void mxm_launch_xent_dw(const XentArgs& a, int64_t r0, int64_t rows, bool last, const int32_t* low,
+                        hipStream_t s) {
   Product p{};
   set_planes(a, p);
   p.a = hidden(a, false, r0);
@@ -958,6 +986,7 @@ void mxm_launch_xent_dw(const XentArgs& a, int64_t r0, int64_t rows, bool last, 
   o.bf16 = last && a.dw_bf16;
   o.add = r0 > 0 ? sums : nullptr;
   o.w_exp = a.w_exp;
+  o.low = low;
   o.scalars = a.scalars;
   o.M = a.D;
   o.vec = aligned(o.out) && a.D % (o.bf16 ? 8 : 4) == 0;

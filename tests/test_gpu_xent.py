@@ -29,26 +29,39 @@ def tolerances(x, w, ref, dtype, softcap, V):
     aw, ax = np.abs(w), np.abs(x)
     xtop, wtop = ax.max(axis=1, keepdims=True), aw.max(axis=1, keepdims=True)
     low = 2.0 ** -39
+    dz, dl = np.abs(ref["dz"]), np.abs(ref["dl"])
+    # |g| times the others' share bounds a row's |dl|; the target's is that
+    most = dl.max(axis=1, keepdims=True)
+    if fp32:
+        # the least exponent of a row of the table: smaller ones are taken down to it (at
+        # most: it has some slack)
+        others = np.where(ref["dl"] * ref["g"][:, None] > 0, dz, 0.0)
+        least = np.divide(others * wtop.T, most, out=np.zeros_like(dl), where=most > 0).max()
+        wtop = np.maximum(wtop, least)
     el = (2 * (D + 8) * (3 if fp32 else 1) + (8 if fp32 else 4)) * U32 * ref["mass"]
     if fp32:
         el = el + low * (xtop * aw.sum(axis=1) + ax.sum(axis=1, keepdims=True) * wtop.T)
     if softcap:
         el = el + 8 * U32 * softcap
-    size = np.abs(ref["l"]).max(axis=1, keepdims=True)
-    top = el.max(axis=1, keepdims=True)
+    # an entry whose logit is over 60 below the largest, whatever its error, has a share
+    # below 2^-86
+    alive = ref["l"] + 2 * el > (ref["l"] - 2 * el).max(axis=1, keepdims=True) - 60
+    size = np.where(alive, np.abs(ref["l"]), 0.0).max(axis=1, keepdims=True)
+    top = np.where(alive, el, 0.0).max(axis=1, keepdims=True)
     steps = U32 * (8 * size + 2 * (V / 64 + 160))
-    row = (2 * top + steps)[:, 0]
+    # (the target's own logit is in the loss; of lse it is not asked for)
+    at_target = np.where(ref["dl"] * ref["g"][:, None] > 0, 0.0, el + 8 * U32 * np.abs(ref["l"])).max(axis=1)
+    row = (2 * top + steps)[:, 0] + at_target
     ep = (2 * top + steps) * 1.1            # of p, relative
     rounding = 8 * U32 if fp32 else UBF + UBF / 4
-    dz, dl = np.abs(ref["dz"]), np.abs(ref["dl"])
-    edz = dz * (ep + rounding)
-    # |g| times the others' share bounds a row's |dl|; the target's is that
-    most = dl.max(axis=1, keepdims=True)
+    edz = dz * (ep + rounding) + most * 2.0 ** -86
     if fp32:
-        # dz is kept in planes too, in units that the row's bound and the table's largest
-        # row set: half a subnormal step is 2^-39 of them, for entry v as many times more
-        # as its row of the table is smaller (powers of two: within a factor of 4)
-        edz = edz + low * 4 * most * (wtop.max() / np.maximum(wtop, 1e-300)).T
+        # dz is kept in planes too, in units of the row's largest |dz| times its row of the
+        # table, or of the largest |dz| times the least exponent (a power of two from each:
+        # within a factor of 8; the slack of four bits); half a subnormal step is 2^-39 of them
+        scale = np.maximum((dz * wtop.T).max(axis=1, keepdims=True), most * least)
+        scale = np.where(scale > 0, scale, most)  # (a table of zeros)
+        edz = edz + low * 8 * 16 * scale / np.where(wtop.T > 0, wtop.T, 1.0)
     else:
         # p is kept in fp16 between its two passes, in units of which the largest of a
         # block of the vocabulary is over 2^14: half a step of fp16's subnormal numbers,
@@ -62,9 +75,9 @@ def tolerances(x, w, ref, dtype, softcap, V):
     bw = edz.T @ ax + per * (N + 64) * U32 * ((dz + edz).T @ ax)
     if fp32:
         bx = bx + dz @ (4 * U32 * aw + low * wtop)
-        # dw's rows of x share one exponent, set by the largest bound times row of x
-        share = np.divide(dz, most, out=np.zeros_like(dz), where=most > 0)
-        bw = bw + dz.T @ (4 * U32 * ax) + (low * 4 * (most * xtop).max()) * share.sum(axis=0)[:, None]
+        # dw's rows of x share one exponent, set by the largest of those units times row of x
+        share = np.divide(dz, scale, out=np.zeros_like(dz), where=scale > 0)
+        bw = bw + dz.T @ (4 * U32 * ax) + (low * 8 * (scale * xtop).max()) * share.sum(axis=0)[:, None]
     return row, bx, bw
 
 
