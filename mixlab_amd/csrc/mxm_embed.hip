@@ -386,16 +386,18 @@ __global__ __launch_bounds__(NT) void embed_join_kernel(EmbedArgs a, int T, int 
   }
 }
 
-// Elements per thread and step: 4 where fp32 is among the tensors (16 bytes of it, so
-// that a wave's accesses lie side by side: two halves of 32 bytes a lane took 221 us for
-// a backward's sums of 65536 x 2048, against 197), 8 of bf16 alone, 1 of rows that no
-// aligned unit divides.
+// Elements per thread and step: 8 where both tensors are bf16, 4 where fp32 is among
+// them (16 bytes of it, so that a wave's accesses lie side by side: two halves of 32 bytes
+// a lane took 221 us for a backward's sums of 65536 x 2048, against 197) or 8 do not
+// divide the rows or their places, 1 where 4 do not.
 int unit_of(int D, const void* p, bool p_bf16, const void* q, bool q_bf16) {
-  const int u = p_bf16 && q_bf16 ? 8 : 4;
-  const auto fits = [&](const void* at, bool bf16) {
-    return reinterpret_cast<uintptr_t>(at) % (u * (bf16 ? 2 : 4) < 16 ? u * (bf16 ? 2 : 4) : 16) == 0;
-  };
-  return D % u == 0 && fits(p, p_bf16) && fits(q, q_bf16) ? u : 1;
+  for (int u = p_bf16 && q_bf16 ? 8 : 4; u >= 4; u /= 2) {
+    const auto fits = [&](const void* at, bool bf16) {
+      return reinterpret_cast<uintptr_t>(at) % (u * (bf16 ? 2 : 4)) == 0;
+    };
+    if (D % u == 0 && fits(p, p_bf16) && fits(q, q_bf16)) return u;
+  }
+  return 1;
 }
 
 // Threads that walk one row of `units`: the least power of two that covers it, at

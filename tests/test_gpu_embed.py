@@ -38,6 +38,9 @@ def tokens_of(kind, rng, N, V):
     (100, 544, 300, "bf16", "fp32", 1, "extremes"),
     (64, 136, 40, "fp32", "fp32", 3, "outside"),
     (3000, 8, 5000, "bf16", "bf16", 0, "uniform"),
+    (130, 100, 90, "bf16", "bf16", 0, "skewed"),
+    (130, 72, 90, "bf16", "bf16", 4, "skewed"),
+    (20000, 300, 50, "bf16", "bf16", 2, "skewed"),
 ])
 def test_forward(gpu_lib, N, D, V, table, out, shift, kind):
     rng = np.random.default_rng(N + D)
@@ -67,6 +70,9 @@ def test_forward(gpu_lib, N, D, V, table, out, shift, kind):
     (40001, 16, 9000, "fp32", "fp32", 0, "skewed", False),
     (33000, 9, 1, "bf16", "fp32", 0, "one", False),
     (65, 8, 20000, "fp32", "fp32", 0, "uniform", False),
+    (700, 100, 90, "bf16", "bf16", 0, "skewed", True),
+    (700, 72, 90, "bf16", "bf16", 4, "skewed", False),
+    (700, 72, 90, "bf16", "fp32", 2, "skewed", False),
 ])
 def test_backward(gpu_lib, N, D, V, grad, dtable, shift, kind, add):
     rng = np.random.default_rng(N + 3 * D)
