@@ -160,11 +160,20 @@ __device__ __forceinline__ void each_group(const int32_t* tokens, int64_t from, 
 }
 
 template <int SORT_WAVES>
-__global__ __launch_bounds__(64 * SORT_WAVES) void embed_sort_kernel(EmbedArgs a, int span) {
-  __shared__ int cnt[SORT_WAVES][SORT_SPAN];
-  __shared__ unsigned long long same[SORT_WAVES][SORT_SPAN];
-  __shared__ int tot[SORT_SPAN];
-  __shared__ int lower[SORT_WAVES];
+struct SortLds {
+  int cnt[SORT_WAVES][SORT_SPAN];
+  unsigned long long same[SORT_WAVES][SORT_SPAN];
+  int tot[SORT_SPAN + 1];  // where each owned token starts, and the end
+  int lower[SORT_WAVES];
+};
+// put(sorted place, place, token) for every owned place; LOCAL: the sorted places start at
+// the workgroup's own.
+template <int SORT_WAVES, bool LOCAL, class Put>
+__device__ __forceinline__ void sort_span(const EmbedArgs& a, int span, SortLds<SORT_WAVES>& lds, Put put) {
+  auto& cnt = lds.cnt;
+  auto& same = lds.same;
+  auto& tot = lds.tot;
+  auto& lower = lds.lower;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int lo = blockIdx.x * span, own = min(span, a.V - lo);
   // stretches of whole groups of 64
@@ -201,8 +210,10 @@ __global__ __launch_bounds__(64 * SORT_WAVES) void embed_sort_kernel(EmbedArgs a
   __syncthreads();
   if (wave == 0) {
     int base = 0;
+    if constexpr (!LOCAL) {
 #pragma unroll
-    for (int w = 0; w < SORT_WAVES; ++w) base += lower[w];
+      for (int w = 0; w < SORT_WAVES; ++w) base += lower[w];
+    }
     for (int b0 = 0; b0 < own; b0 += 64) {
       const int b = b0 + lane, c = b < own ? tot[b] : 0;
       int x = c;
@@ -211,13 +222,10 @@ __global__ __launch_bounds__(64 * SORT_WAVES) void embed_sort_kernel(EmbedArgs a
         const int y = __shfl_up(x, o);
         if (lane >= o) x += y;
       }
-      if (b < own) {
-        tot[b] = base + x - c;
-        a.starts[lo + b] = base + x - c;
-      }
+      if (b < own) tot[b] = base + x - c;
       base += __shfl(x, 63);
     }
-    if (lane == 0 && lo + own == a.V) a.starts[a.V] = base;
+    if (lane == 0) tot[own] = base;
   }
   __syncthreads();
   each_group<8>(a.tokens, from, to, lane, [&](int64_t n, unsigned v) {
@@ -238,7 +246,7 @@ __global__ __launch_bounds__(64 * SORT_WAVES) void embed_sort_kernel(EmbedArgs a
       const unsigned long long m = one ? any : same[wave][b];
       before = __popcll(m & ((1ull << lane) - 1));
       all = __popcll(m);
-      a.sorted[tot[b] + cnt[wave][b] + before] = make_int2((int)(n + lane), (int)v);
+      put(tot[b] + cnt[wave][b] + before, (int)(n + lane), (int)v);
     }
     wave_lds_sync();  // every lane has read its word and count
     if (mine && before == 0) {
@@ -248,6 +256,23 @@ __global__ __launch_bounds__(64 * SORT_WAVES) void embed_sort_kernel(EmbedArgs a
     wave_lds_sync();
   });
 }
+
+template <int SORT_WAVES>
+__global__ __launch_bounds__(64 * SORT_WAVES) void embed_sort_kernel(EmbedArgs a, int span) {
+  __shared__ SortLds<SORT_WAVES> lds;
+  sort_span<SORT_WAVES, false>(a, span, lds, [&](int at, int n, int v) { a.sorted[at] = make_int2(n, v); });
+  const int lo = blockIdx.x * span, own = min(span, a.V - lo);
+  for (int b = threadIdx.x; b < own + (lo + own == a.V); b += blockDim.x) a.starts[lo + b] = lds.tot[b];
+}
+
+// The sorted places as the sums see them: place and token of one, where a token starts
+// and ends, and the chunks' sums.
+struct Runs {
+  const EmbedArgs& a;
+  __device__ __forceinline__ int2 at(int64_t p) const { return a.sorted[p]; }
+  __device__ __forceinline__ int64_t start(int v) const { return a.starts[v]; }
+  __device__ __forceinline__ float* part(int64_t row) const { return a.part + row * a.D; }
+};
 
 // Sorted places [c * C, (c + 1) * C) per T threads: each run of one token that lies
 // within them to the table, the first and last run's sums to part where they go on
@@ -268,8 +293,7 @@ __device__ __forceinline__ void put_row(const EmbedArgs& a, int v, int d, float 
 
 // (read again by the join: kept in the caches)
 template <int U>
-__device__ __forceinline__ void store_part(const EmbedArgs& a, int64_t row, int d, const float (&s)[U]) {
-  float* q = a.part + row * a.D + d;
+__device__ __forceinline__ void store_part(float* q, const float (&s)[U]) {
   if constexpr (U == 1) {
     q[0] = s[0];
   } else {
@@ -282,29 +306,30 @@ __device__ __forceinline__ void store_part(const EmbedArgs& a, int64_t row, int 
 }
 
 constexpr int AHEAD = 8;  // rows in flight
-template <int U>
-__device__ __forceinline__ void sum_chunk(const EmbedArgs& a, int T, int t, int C, int64_t c, int64_t all) {
+template <int U, class R>
+__device__ __forceinline__ void sum_chunk(const EmbedArgs& a, const R& runs, int T, int t, int C, int64_t c,
+                                          int64_t all) {
   const int64_t from = c * C, to = min(from + C, all);
   if (from >= to) return;
   for (int d = t * U; d < a.D; d += T * U) {
     float s[U];
 #pragma unroll
     for (int i = 0; i < U; ++i) s[i] = 0.0f;
-    int v = a.sorted[from].y;
+    int v = runs.at(from).y;
     bool first = true;  // the chunk's first run
     for (int64_t p0 = from; p0 < to; p0 += AHEAD) {
       int2 e[AHEAD];
       float g[AHEAD][U];
 #pragma unroll
-      for (int k = 0; k < AHEAD; ++k) e[k] = a.sorted[min(p0 + k, to - 1)];
+      for (int k = 0; k < AHEAD; ++k) e[k] = runs.at(min(p0 + k, to - 1));
 #pragma unroll
       for (int k = 0; k < AHEAD; ++k) load_once<U>(a.d_out, a.grad_bf16, (int64_t)e[k].x * a.D + d, g[k]);
 #pragma unroll
       for (int k = 0; k < AHEAD; ++k) {
         if (p0 + k >= to) break;
         if (e[k].y != v) {
-          if (first && a.starts[v] < from) {
-            store_part<U>(a, c * 2, d, s);
+          if (first && runs.start(v) < from) {
+            store_part<U>(runs.part(c * 2) + d, s);
           } else {
             put_row<U>(a, v, d, s);
           }
@@ -317,9 +342,9 @@ __device__ __forceinline__ void sum_chunk(const EmbedArgs& a, int T, int t, int 
         for (int i = 0; i < U; ++i) s[i] += g[k][i];
       }
     }
-    const bool before = first && a.starts[v] < from, after = a.starts[v + 1] > to;
+    const bool before = first && runs.start(v) < from, after = runs.start(v + 1) > to;
     if (before || after) {
-      store_part<U>(a, c * 2 + (before ? 0 : 1), d, s);
+      store_part<U>(runs.part(c * 2 + (before ? 0 : 1)) + d, s);
     } else {
       put_row<U>(a, v, d, s);
     }
@@ -331,26 +356,27 @@ __global__ __launch_bounds__(NT) void embed_sum_kernel(EmbedArgs a, int T, int C
   const int per = NT / T, sub = threadIdx.x / T, t = threadIdx.x % T;
   const int64_t all = a.starts[a.V];
   for (int64_t c = (int64_t)blockIdx.x * per + sub; c < chunks; c += (int64_t)gridDim.x * per)
-    sum_chunk<U>(a, T, t, C, c, all);
+    sum_chunk<U>(a, Runs{a}, T, t, C, c, all);
 }
 
 // The run that starts in chunk c and goes on behind it: its sums in order.
 constexpr int JOIN_AHEAD = 16;
-template <int U>
-__device__ __forceinline__ void join_chunk(const EmbedArgs& a, int T, int t, int C, int64_t c, int64_t all) {
+template <int U, class R>
+__device__ __forceinline__ void join_chunk(const EmbedArgs& a, const R& runs, int T, int t, int C, int64_t c,
+                                           int64_t all) {
   if ((c + 1) * C >= all) return;
-  const int v = a.sorted[(c + 1) * C - 1].y;
-  const int64_t from = a.starts[v], to = a.starts[v + 1];
+  const int v = runs.at((c + 1) * C - 1).y;
+  const int64_t from = runs.start(v), to = runs.start(v + 1);
   if (from < c * C || to <= (c + 1) * C) return;
   const int64_t last = (to - 1) / C;
   for (int d = t * U; d < a.D; d += T * U) {
     float s[U];
-    load_unit<U>(a.part, false, (c * 2 + 1) * a.D + d, s);
+    load_unit<U>(runs.part(c * 2 + 1), false, d, s);
     int64_t k = c + 1;
     for (; k + JOIN_AHEAD <= last + 1; k += JOIN_AHEAD) {
       float e[JOIN_AHEAD][U];
 #pragma unroll
-      for (int h = 0; h < JOIN_AHEAD; ++h) load_unit<U>(a.part, false, (k + h) * 2 * a.D + d, e[h]);
+      for (int h = 0; h < JOIN_AHEAD; ++h) load_unit<U>(runs.part((k + h) * 2), false, d, e[h]);
 #pragma unroll
       for (int h = 0; h < JOIN_AHEAD; ++h)
 #pragma unroll
@@ -358,7 +384,7 @@ __device__ __forceinline__ void join_chunk(const EmbedArgs& a, int T, int t, int
     }
     for (; k <= last; ++k) {
       float e[U];
-      load_unit<U>(a.part, false, k * 2 * a.D + d, e);
+      load_unit<U>(runs.part(k * 2), false, d, e);
 #pragma unroll
       for (int i = 0; i < U; ++i) s[i] += e[i];
     }
@@ -374,7 +400,7 @@ __global__ __launch_bounds__(NT) void embed_join_kernel(EmbedArgs a, int T, int 
   const int64_t all = a.starts[a.V];
   for (int64_t i = (int64_t)blockIdx.x * per + sub; i < items; i += (int64_t)gridDim.x * per) {
     if (i < joins) {
-      join_chunk<U>(a, T, t, C, i, all);
+      join_chunk<U>(a, Runs{a}, T, t, C, i, all);
     } else {
       const int64_t v = i - joins;
       if (a.starts[v] != a.starts[v + 1]) continue;
@@ -383,6 +409,50 @@ __global__ __launch_bounds__(NT) void embed_join_kernel(EmbedArgs a, int T, int 
       for (int k = 0; k < U; ++k) z[k] = 0.0f;
       for (int d = t * U; d < a.D; d += T * U) store_unit<U>(a.d_table, a.dtable_bf16, v * a.D + d, z);
     }
+  }
+}
+
+// A batch whose chunks' sums fit into LDS, in one launch: a workgroup per span of tokens
+// sorts its places and sums them.  1024 rows of D 64 into 1024 tokens take 13.6 us in
+// three launches, 9.3 so; 8 rows of D 2048 on top of a table 14.3 and 8.4.  Zeros for a
+// large table keep to the join, whose many workgroups write them faster (8 rows into 50257
+// tokens of D 2048 84 us there, 92 so).
+constexpr int FEW_SUMS = 16384;                 // floats of LDS for them
+constexpr int FEW_CHUNK = 8;
+constexpr int64_t FEW_ZEROS = (int64_t)1 << 25; // elements of a table that it writes zeros to
+struct LocalRuns {
+  const EmbedArgs& a;
+  const int* list;  // place | token of the span << 16
+  const int* tot;
+  float* sums;
+  int lo;
+  __device__ __forceinline__ int2 at(int64_t p) const {
+    return make_int2(list[p] & 0xffff, lo + (list[p] >> 16));
+  }
+  __device__ __forceinline__ int64_t start(int v) const { return tot[v - lo]; }
+  __device__ __forceinline__ float* part(int64_t row) const { return sums + row * a.D; }
+};
+template <int U>
+__global__ __launch_bounds__(NT) void embed_few_kernel(EmbedArgs a, int span, int T) {
+  __shared__ SortLds<NT / 64> lds;
+  __shared__ int list[SORT_FEW];
+  __shared__ __attribute__((aligned(16))) float sums[FEW_SUMS];
+  const int lo = blockIdx.x * span, own = min(span, a.V - lo);
+  sort_span<NT / 64, true>(a, span, lds, [&](int at, int n, int v) { list[at] = n | (v - lo) << 16; });
+  __syncthreads();
+  const LocalRuns runs{a, list, lds.tot, sums, lo};
+  const int all = lds.tot[own], chunks = (all + FEW_CHUNK - 1) / FEW_CHUNK;
+  const int per = NT / T, sub = threadIdx.x / T, t = threadIdx.x % T;
+  for (int c = sub; c < chunks; c += per) sum_chunk<U>(a, runs, T, t, FEW_CHUNK, c, all);
+  __syncthreads();
+  for (int c = sub; c < chunks - 1; c += per) join_chunk<U>(a, runs, T, t, FEW_CHUNK, c, all);
+  if (a.accumulate) return;
+  float z[U];
+#pragma unroll
+  for (int k = 0; k < U; ++k) z[k] = 0.0f;
+  for (int b = sub; b < own; b += per) {
+    if (lds.tot[b] != lds.tot[b + 1]) continue;
+    for (int d = t * U; d < a.D; d += T * U) store_unit<U>(a.d_table, a.dtable_bf16, (int64_t)(lo + b) * a.D + d, z);
   }
 }
 
@@ -417,7 +487,18 @@ unsigned grid_of(int64_t items, int per, int n_cu) {
 }
 
 template <int U>
-void launch_bw(const EmbedArgs& a, hipStream_t s) {
+void launch_bw(const EmbedArgs& a, int span, hipStream_t s) {
+  const unsigned spans = (unsigned)((a.V + span - 1) / span);
+  // (a chunk has two sums)
+  if (a.rows <= SORT_FEW && (a.rows + FEW_CHUNK - 1) / FEW_CHUNK * 2 * a.D <= FEW_SUMS &&
+      (a.accumulate || (int64_t)a.V * a.D <= FEW_ZEROS)) {
+    embed_few_kernel<U><<<spans, NT, 0, s>>>(a, span, threads_per_row(a.D / U));
+    return;
+  }
+  if (a.rows <= SORT_FEW)
+    embed_sort_kernel<4><<<spans, 256, 0, s>>>(a, span);
+  else
+    embed_sort_kernel<16><<<spans, 1024, 0, s>>>(a, span);
   const int T = threads_per_row(a.D / U), per = NT / T, C = chunk_rows(a.rows);
   const int64_t chunks = (a.rows + C - 1) / C, joins = chunks > 1 ? chunks - 1 : 0;
   const int64_t items = joins + (a.accumulate ? 0 : a.V);
@@ -445,17 +526,12 @@ void mxm_launch_embed(const EmbedArgs& a, hipStream_t s) {
 }
 
 void mxm_launch_embed_bw(const EmbedArgs& a, hipStream_t s) {
-  const int span = std::min(SORT_SPAN, std::max(16, (a.V + a.n_cu - 1) / a.n_cu));
-  const unsigned grid = (unsigned)((a.V + span - 1) / span);
-  if (a.rows <= SORT_FEW)
-    embed_sort_kernel<4><<<grid, 256, 0, s>>>(a, span);
-  else
-    embed_sort_kernel<16><<<grid, 1024, 0, s>>>(a, span);
+  const int span = std::min(SORT_SPAN, (a.V + a.n_cu - 1) / a.n_cu);
   const int U = unit_of(a.D, a.d_out, a.grad_bf16, a.d_table, a.dtable_bf16);
   if (U == 8)
-    launch_bw<8>(a, s);
+    launch_bw<8>(a, span, s);
   else if (U == 4)
-    launch_bw<4>(a, s);
+    launch_bw<4>(a, span, s);
   else
-    launch_bw<1>(a, s);
+    launch_bw<1>(a, span, s);
 }

@@ -71,6 +71,13 @@ def test_forward(gpu_lib, N, D, V, table, out, shift, kind):
     (33000, 9, 1, "bf16", "fp32", 0, "one", False),
     (65, 8, 20000, "fp32", "fp32", 0, "uniform", False),
     (700, 100, 90, "bf16", "bf16", 0, "skewed", True),
+    (1024, 64, 1024, "fp32", "fp32", 0, "one", False),
+    (2048, 32, 1, "bf16", "fp32", 0, "one", True),
+    (2048, 32, 1000, "fp32", "bf16", 0, "skewed", False),
+    (2047, 24, 300, "bf16", "bf16", 1, "extremes", True),
+    (9, 1024, 5000, "fp32", "fp32", 0, "extremes", True),
+    (8, 2048, 20000, "fp32", "bf16", 0, "uniform", False),
+    (2049, 32, 700, "fp32", "fp32", 0, "skewed", True),
     (700, 72, 90, "bf16", "bf16", 4, "skewed", False),
     (700, 72, 90, "bf16", "fp32", 2, "skewed", False),
 ])
