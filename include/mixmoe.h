@@ -441,10 +441,15 @@ int mxm_embed_backward(int64_t h, int64_t rows, const int32_t* tokens, const voi
  *   total = sum of row_weights[n] * loss[n]    MXM_XENT_MEAN: / sum of row_weights[n]
  * over the rows that take part (0 where none does).
  * params = [V, D, maxRows, dtype, dxDtype, dwDtype, flags]; dtype is that of x and
- * weight.  Under fp32 the products are as exact as fp32 ones; under bf16 they are
- * exact products summed in fp32, and the backward rounds the logits' gradient to
- * bf16 before the products with it.  softcap 0: none.  Returns a handle, 0 on
- * failure. */
+ * weight.  Under bf16 the products are exact and summed in fp32, and the backward
+ * rounds the logits' gradient to bf16 before the products with it.  Under fp32 a
+ * row's elements keep 22 bits down to 2^-17 of its largest and 2^-40 of it below,
+ * and so does a row's gradient of the logits.  An entry (row of weight) that minus
+ * infinity or the type's lowest value keeps from coming has no share in any result
+ * (but that dx of a bf16 table with infinities is not a number, 0 times those);
+ * as a target it makes the loss infinite (or as large), and then dx and dw are of no
+ * use.  A row of x that is not finite spoils its own results and dw.  softcap 0:
+ * none.  Returns a handle, 0 on failure. */
 #define MXM_XENT_MEAN 1
 #define MXM_XENT_BACKWARD 2 /* the handle also runs backward (holds its workspace) */
 int64_t mxm_xent_create(const int64_t* params, int n_params, float softcap, int64_t stream_of);

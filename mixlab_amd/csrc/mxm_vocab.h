@@ -144,11 +144,23 @@ int64_t mxm_xent_stats(int64_t rows, int V, int n_cu);
 // Columns of the vocabulary per block of stat, for a piece of `rows` rows.
 int mxm_xent_block(int64_t rows, int V, int n_cu);
 // low: where the pieces before left L, or null.
-void mxm_launch_xent_logits(const XentArgs& a, int64_t r0, int64_t rows, const int32_t* low, hipStream_t s);
+// gather: the kernel itself finds the rows that take part and reads them in place.
+void mxm_launch_xent_logits(const XentArgs& a, int64_t r0, int64_t rows, const int32_t* low, bool gather,
+                            hipStream_t s);
+// Most rows of a forward that are read in place.
+constexpr int XENT_GATHER = 32;
 void mxm_launch_xent_dx(const XentArgs& a, int64_t r0, int64_t rows, hipStream_t s);
 void mxm_launch_xent_dw(const XentArgs& a, int64_t r0, int64_t rows, bool last, const int32_t* low,
                         hipStream_t s);
 void mxm_launch_xent(const XentArgs& a, hipStream_t s);
+
+// Whether a row of weight w and target t takes part.
+__device__ __forceinline__ bool mxm_xent_takes_part(const int32_t* targets, const float* row_weights, int V,
+                                                    int64_t n, int& t, float& w) {
+  t = targets[n];
+  w = row_weights ? row_weights[n] : 1.0f;
+  return t >= 0 && t < V && w != 0.0f;
+}
 
 // Rows of the piece that starts at row r0 of those that take part.
 __device__ __forceinline__ int mxm_xent_rows(const XentArgs& a, int64_t r0) {

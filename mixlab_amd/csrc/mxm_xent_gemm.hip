@@ -134,13 +134,16 @@ struct Loads {
   unsigned off[Q];       // bytes from the stage's base
   int k[EVEN ? 1 : Q];   // the lane's k in the stage: of load 0, or of each
   const uint16_t* base;  // of the next stage to load
-  __device__ __forceinline__ void init(const Operand& o, int x0, int wave, int lane) {
+  // row: the one that the lane loads of (k-inner, one load), or -1
+  __device__ __forceinline__ void init(const Operand& o, int x0, int wave, int lane, int row) {
     if constexpr (INNER) {
       const int r0 = wave * 8 + lane / 8, chunk = ((lane % 8) ^ ((r0 / 2) % 8)) * 8;
       k[0] = chunk;
 #pragma unroll
-      for (int q = 0; q < Q; ++q)
-        off[q] = 2u * ((unsigned)min(r0 + q * NW * 8, o.rows - 1 - x0) * (unsigned)o.ld + (unsigned)chunk);
+      for (int q = 0; q < Q; ++q) {
+        const int r = row >= 0 ? row : min(r0 + q * NW * 8, o.rows - 1 - x0);
+        off[q] = 2u * ((unsigned)r * (unsigned)o.ld + (unsigned)chunk);
+      }
     } else {
 #pragma unroll
       for (int q = 0; q < Q; ++q) {
@@ -202,7 +205,8 @@ __device__ __forceinline__ f32x16_t mfma(u32x4_t a, u32x4_t b, f32x16_t c) {
 // Stages s_lo .. s_hi - 1 (of pairs * nk) of the tile at (m0, n0) into acc.
 template <class TL, bool AIN, bool BIN, bool F16>
 __device__ __forceinline__ void product_tile(const Product& p, unsigned char* lds, int m0, int n0,
-                                             int s_lo, int s_hi, f32x16_t (&acc)[TL::TM][TL::TN]) {
+                                             int s_lo, int s_hi, f32x16_t (&acc)[TL::TM][TL::TN],
+                                             int row_b = -1) {
   constexpr int TM = TL::TM, TN = TL::TN, NW = TL::NW, NS = TL::NS, KS = BK / 16;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / TL::WN, wn = wave % TL::WN;
@@ -212,8 +216,8 @@ __device__ __forceinline__ void product_tile(const Product& p, unsigned char* ld
   static_assert((NS - 1) * LDPS <= 63, "vmcnt counts");
   LA la;
   LB lb;
-  la.init(p.a, m0, wave, lane);
-  lb.init(p.b, n0, wave, lane);
+  la.init(p.a, m0, wave, lane, -1);
+  lb.init(p.b, n0, wave, lane, row_b);
 #pragma unroll
   for (int i = 0; i < TM; ++i)
 #pragma unroll
@@ -442,6 +446,15 @@ struct LogitsArgs {
   int64_t stat_ld;
   void* summands;
 };
+// The rows as a forward of few gets them (GATHER).
+struct GatherArgs {
+  const int32_t* targets;
+  const float* row_weights;
+  int rows;
+  XentScalars* scalars;
+  int32_t *map, *target;
+  float *loss, *lse;
+};
 struct GradArgs {
   const XentScalars* scalars;
   int64_t r0, piece_rows;
@@ -455,12 +468,56 @@ __device__ __forceinline__ int rows_of(const A& a) {
   return left <= 0 ? 0 : (int)(left < a.piece_rows ? left : a.piece_rows);
 }
 
-template <class TL, bool STORE, bool F16, bool CAP>
-__global__ __launch_bounds__(TL::NT, TL::WPS) void xent_logits_kernel(LogitsArgs a, Product p) {
+// What the packing's launch does for more rows (the plan, in order; zeros for the rows
+// that take no part), by every workgroup for itself and by the first for the join.
+struct Gathered {
+  int at[XENT_GATHER], target[XENT_GATHER], rows;
+};
+__device__ __forceinline__ void gather_rows(const GatherArgs& g, int V, Gathered& lds) {
+  if (threadIdx.x < 64) {
+    const int n = threadIdx.x;
+    int t = -1;
+    float w = 0.0f;
+    const bool in = n < g.rows && mxm_xent_takes_part(g.targets, g.row_weights, V, n, t, w);
+    const unsigned long long m = __ballot(in);
+    const int to = __popcll(m & ((1ull << n) - 1));
+    if (in) lds.at[to] = n, lds.target[to] = t;
+    if (n == 0) lds.rows = __popcll(m);
+    if (blockIdx.x == 0) {
+      double sum = in ? (double)w : 0.0;
+#pragma unroll
+      for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
+      if (n == 0) g.scalars->rows = __popcll(m), g.scalars->weight_sum = sum;
+      if (in) {
+        g.map[to] = n;
+        g.target[to] = t;
+      } else if (n < g.rows) {
+        if (g.loss) g.loss[n] = 0.0f;
+        if (g.lse) g.lse[n] = 0.0f;
+      }
+    }
+  }
+  __syncthreads();
+}
+
+// (four stages of 20 KB and the exponents under fp32: one workgroup per CU)
+template <class TL, bool STORE, bool F16, bool CAP, bool GATHER = false>
+__global__ __launch_bounds__(TL::NT, F16 && TL::NS == 4 ? 1 : TL::WPS) void xent_logits_kernel(LogitsArgs a, Product p, GatherArgs g) {
   __shared__ __attribute__((aligned(1024))) unsigned char lds[TL::NS * TL::BUF];
   __shared__ __attribute__((aligned(16))) int w_exp[F16 ? TL::BM : 4];
   constexpr int TM = TL::TM, TN = TL::TN;
-  const int rows = rows_of(a);
+  int rows, row_b = -1, own_target = -1;
+  if constexpr (GATHER) {
+    static_assert(TN == 1 && TL::WN == 1 && TL::BN / 8 == TL::NW, "a row's loads by one lane each");
+    Gathered& own = *reinterpret_cast<Gathered*>(lds);
+    gather_rows(g, a.V, own);
+    rows = __builtin_amdgcn_readfirstlane(own.rows);
+    row_b = own.at[max(min((int)threadIdx.x / 8, rows - 1), 0)];
+    if ((int)(threadIdx.x & 31) < rows) own_target = own.target[threadIdx.x & 31];
+    __syncthreads();
+  } else {
+    rows = rows_of(a);
+  }
   p.b.rows = rows;
   const int mt = (a.V + TL::BM - 1) / TL::BM, nt = (rows + TL::BN - 1) / TL::BN;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -475,7 +532,7 @@ __global__ __launch_bounds__(TL::NT, TL::WPS) void xent_logits_kernel(LogitsArgs
 #pragma unroll
     for (int j = 0; j < TN; ++j) {
       const int n = n0 + (wn * TN + j) * 32 + (lane & 31);
-      targets[j] = n < rows ? a.target[n] : -1;
+      targets[j] = n < rows ? (GATHER ? own_target : a.target[n]) : -1;
       if constexpr (F16) x_exps[j] = n < rows ? a.x_exp[n] : 0;
     }
     // (the sum's barriers stand between this and the epilogue)
@@ -485,7 +542,7 @@ __global__ __launch_bounds__(TL::NT, TL::WPS) void xent_logits_kernel(LogitsArgs
         w_exp[i] = a.low ? max(e, *a.low) : e;
       }
     f32x16_t acc[TM][TN];
-    product_tile<TL, true, true, F16>(p, lds, m0, n0, 0, p.nk * p.pairs, acc);
+    product_tile<TL, true, true, F16>(p, lds, m0, n0, 0, p.nk * p.pairs, acc, row_b);
     const int mw = m0 + wm * TM * 32;  // the wave's block of the vocabulary
     const int first = mw + (lane >> 5) * 4;
 #pragma unroll
@@ -860,14 +917,18 @@ Shape logits_shape(int64_t rows, int V, int n_cu) {
 
 template <class TL>
 void launch_logits(const XentArgs& a, const Product& p, int64_t r0, int64_t rows, const int32_t* low, int per_cu,
-                   hipStream_t s) {
+                   bool gather, hipStream_t s) {
   const unsigned grid = grid_of(tiles_of(a.V, rows, TL::BM, TL::BN), (int64_t)a.n_cu * per_cu);
   const LogitsArgs l{a.scalars, r0, a.piece_rows, a.V, a.Vp, a.softcap, a.target + r0,
                      a.x_exp ? a.x_exp + r0 : nullptr, a.w_exp, a.at_target + r0, low, a.stat, a.stat_exp,
                      a.stat_ld, a.summands};
-  const auto launch = [&](auto kernel) { kernel<<<grid, TL::NT, 0, s>>>(l, p); };
+  const GatherArgs g{a.targets, a.row_weights, (int)a.rows, a.scalars, a.map, a.target, a.loss, a.lse};
+  const auto launch = [&](auto kernel) { kernel<<<grid, TL::NT, 0, s>>>(l, p, g); };
   const auto typed = [&](auto cap) {
     constexpr bool CAP = decltype(cap)::value;
+    if constexpr (TL::BN == XENT_GATHER) {
+      if (gather) return launch(xent_logits_kernel<TL, false, false, CAP, true>);
+    }
     if (a.planes == 1)
       a.backward ? launch(xent_logits_kernel<TL, true, false, CAP>) : launch(xent_logits_kernel<TL, false, false, CAP>);
     else
@@ -945,16 +1006,21 @@ int64_t mxm_xent_stats(int64_t rows, int V, int n_cu) {
   return std::max({of(rows, 128), of(std::min(rows, small), 64), of(std::min(rows, few), 32)});
 }
 
-void mxm_launch_xent_logits(const XentArgs& a, int64_t r0, int64_t rows, const int32_t* low, hipStream_t s) {
+void mxm_launch_xent_logits(const XentArgs& a, int64_t r0, int64_t rows, const int32_t* low, bool gather,
+                            hipStream_t s) {
   Product p{};
   set_planes(a, p);
   p.a = table(a, true);
   p.b = hidden(a, true, r0);
+  if (gather) {
+    p.b.p = static_cast<const uint16_t*>(a.x);
+    p.b.ld = p.b.k = a.D;
+  }
   p.nk = a.Dp / BK;
   switch (logits_shape(rows, a.V, a.n_cu)) {
-    case FEW: return launch_logits<Few>(a, p, r0, rows, low, 2, s);
-    case SMALL: return launch_logits<Small>(a, p, r0, rows, low, 2, s);
-    default: return launch_logits<Big>(a, p, r0, rows, low, 1, s);
+    case FEW: return launch_logits<Few>(a, p, r0, rows, low, 2, gather, s);
+    case SMALL: return launch_logits<Small>(a, p, r0, rows, low, 2, false, s);
+    default: return launch_logits<Big>(a, p, r0, rows, low, 1, false, s);
   }
 }
 

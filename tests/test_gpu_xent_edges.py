@@ -48,17 +48,17 @@ def test_entries_of_zeros(gpu_lib, dtype, which):
     check(x, w, t, dtype=dtype)
 
 
-@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
-def test_entries_masked_by_the_lowest_value(gpu_lib, dtype, monkeypatch):
-    """Entries that a first channel of the type's lowest value keeps from coming (x's is
-    above zero): every other result is as without them, their own gradient is zero."""
+@pytest.mark.parametrize("dtype,lowest", [("bf16", -3.38e38), ("fp32", -3.38e38), ("fp32", -np.inf)])
+def test_masked_entries(gpu_lib, dtype, lowest, monkeypatch):
+    """Entries that a first channel of the type's lowest value, or less, keeps from coming
+    (x's is above zero): every other result is as without them, their gradient is zero."""
     N, D, V = 700, 72, 330
     x, w, t = inputs(N, D, V, dtype, 26, pad=0.2)
     x[:, 0] = np.abs(x[:, 0]) + 0.5
     x = as_kept(x, dtype)
     out = np.array([3, 77, 299])
     t[np.isin(t, out)] = 5
-    w[out, 0] = as_kept(np.array([-3.38e38]), dtype)
+    w[out, 0] = as_kept(np.array([lowest]), dtype)
     keep = np.setdiff1d(np.arange(V), out)
     took = (t >= 0) & (t < V)
     at = np.where(took, np.searchsorted(keep, np.clip(t, 0, V - 1)), -1)
@@ -99,6 +99,22 @@ def test_pieces_of_unlike_magnitude(gpu_lib, dx, dw, monkeypatch):
         x[:, 0] = -np.ldexp(1.0, at)
         t = np.array([rng.integers(0, np.searchsorted(ex, 2 - a)) for a in at])
         check(x, w, t, dtype="fp32", want_dx=dx, want_dw=dw)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("N,D,V,pad,weighted,shift", [
+    (1, 2048, 3000, 0.0, False, 0), (1, 64, 500, 1.0, False, 0), (2, 72, 40000, 0.0, True, 0),
+    (17, 136, 700, 0.4, True, 0), (32, 8, 130, 0.3, False, 0), (32, 520, 1000, 0.0, False, 8),
+    (31, 100, 400, 0.2, True, 0), (33, 136, 700, 0.4, True, 0), (20, 64, 128, 0.5, False, 1)])
+def test_few_rows(gpu_lib, N, D, V, pad, weighted, shift, dtype):
+    """Up to the few rows that a forward reads in place, in and out of order, and past them."""
+    x, w, t = inputs(N, D, V, dtype, 31 * N + V, pad=pad)
+    weights = None
+    if weighted:
+        weights = np.random.default_rng(N).uniform(0.5, 1.5, N).astype(np.float32)
+        weights[1::3] = 0.0
+        x[1::3] = np.nan
+    check(x, w, t, weights, dtype=dtype, softcap=25.0 if N % 2 else 0.0, shift=shift, calls=2)
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "fp32"])
