@@ -73,6 +73,14 @@ int item(bool bf16) { return bf16 ? 2 : 4; }
 // of which a tile's rows take more).
 constexpr int64_t XENT_PIECE_BYTES = (int64_t)2 << 30;
 
+// What a create returns; memory that there is not enough of leaves an error that the
+// next call's launch would take for its own.
+int64_t created(int rc, int64_t handle) {
+  if (rc == MXM_OK) return handle;
+  if (rc == MXM_ERR) (void)hipGetLastError();
+  return 0;
+}
+
 #define EMBED "TOKEN_EMBEDDING"
 #define XENT "TOKEN_LOSS"
 
@@ -165,7 +173,7 @@ int64_t mxm_embed_create(const int64_t* params, int n_params, float scale, int64
     handle = keep(std::move(e));
     return MXM_OK;
   });
-  return rc == MXM_OK ? handle : 0;
+  return created(rc, handle);
 }
 
 int mxm_embed_destroy(int64_t h) { return destroy<Embed>(h, EMBED); }
@@ -314,7 +322,7 @@ int64_t mxm_xent_create(const int64_t* params, int n_params, float softcap, int6
     handle = keep(std::move(x));
     return MXM_OK;
   });
-  return rc == MXM_OK ? handle : 0;
+  return created(rc, handle);
 }
 
 int mxm_xent_destroy(int64_t h) { return destroy<Xent>(h, XENT); }

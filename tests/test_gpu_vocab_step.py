@@ -279,3 +279,19 @@ def test_rows_of_a_step_do_not_depend_on_the_others(gpu_lib):
             mass = np.abs(x[n]) @ np.abs(w).T
             assert abs(one.get()[0] - every[n]) <= (2 * (D + 8) * 3 + 16) * 2 * U32 * mass.max()
             assert np.max(np.abs(gone.get()[0] - grads[n])) <= size * mass.max()
+
+
+def test_more_than_fits_is_refused_and_harms_nothing(gpu_lib):
+    e = Ends(100, 72, 300, "bf16")
+    e.fill(1)
+    e.run()
+    want = e.results()
+    with pytest.raises(_lib.MixMoEError, match="memory"):
+        TokenLoss(4_194_304, 16384, 1 << 30, dtype="fp32", share=e.emb)
+    e.run()
+    with pytest.raises(_lib.MixMoEError, match="memory"):
+        TokenEmbedding(4_194_304, 16384, 1 << 30, share=e.emb)
+    e.run()
+    for a, b in zip(e.results(), want):
+        np.testing.assert_array_equal(a, b)
+    e.close()
