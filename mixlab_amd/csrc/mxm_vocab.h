@@ -149,9 +149,9 @@ void mxm_launch_xent_logits(const XentArgs& a, int64_t r0, int64_t rows, const i
                             hipStream_t s);
 // Most rows of a forward that are read in place.
 constexpr int XENT_GATHER = 32;
-void mxm_launch_xent_dx(const XentArgs& a, int64_t r0, int64_t rows, hipStream_t s);
-void mxm_launch_xent_dw(const XentArgs& a, int64_t r0, int64_t rows, bool last, const int32_t* low,
-                        hipStream_t s);
+// dx and dw, as far as they are wanted; last: no piece comes after this one.
+void mxm_launch_xent_grads(const XentArgs& a, int64_t r0, int64_t rows, bool last, const int32_t* low,
+                           hipStream_t s);
 void mxm_launch_xent(const XentArgs& a, hipStream_t s);
 
 // Whether a row of weight w and target t takes part.

@@ -690,9 +690,8 @@ void mxm_launch_xent(const XentArgs& a0, hipStream_t s) {
         else
           once ? launch(xent_finish_kernel<true, true>) : launch(xent_finish_kernel<true, false>);
       }
-      if (a.dx) mxm_launch_xent_dx(a, r0, rows, s);
     }
-    if (a.dw) mxm_launch_xent_dw(a, r0, rows, p == pieces - 1, a.scalars->low + parity, s);
+    if (a.backward) mxm_launch_xent_grads(a, r0, rows, p == pieces - 1, a.scalars->low + parity, s);
   }
   if (a.total && !total_there && !(a.backward && a.rows > 0)) xent_total_kernel<<<1, PLAN_NT, 0, s>>>(a);
 }

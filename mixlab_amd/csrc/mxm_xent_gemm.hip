@@ -359,10 +359,13 @@ __device__ __forceinline__ void tile_at(int t, int mt, int nt, int& m, int& n) {
 // This workgroup's items of `items`: first, first + step, ... below end.
 struct Items {
   int first, step, end;
-  __device__ __forceinline__ explicit Items(int items) {
+  // behind: another list's items per XCD that start at the first workgroups
+  __device__ __forceinline__ explicit Items(int items, int behind = 0) {
     const int xcd = blockIdx.x % 8, per = (items + 7) / 8;
-    first = xcd * per + blockIdx.x / 8;
     step = gridDim.x / 8;
+    int at = blockIdx.x / 8;
+    if (behind != 0) at = (at + step - behind % step) % step;
+    first = xcd * per + at;
     end = min((xcd + 1) * per, items);
   }
 };
@@ -772,9 +775,10 @@ __device__ __forceinline__ void fit(const GradArgs& a, Product& p) {
   }
 }
 
+// The tiles of dx or dw; returns how many of its last round's items an XCD has.
 template <class TL, bool DW, bool F16>
-__global__ __launch_bounds__(TL::NT, TL::WPS) void xent_grad_kernel(GradArgs a, Product p, Out o) {
-  __shared__ __attribute__((aligned(1024))) unsigned char lds[TL::NS * TL::BUF];
+__device__ __forceinline__ int grad_tiles(const GradArgs& a, Product p, const Out& o, unsigned char* lds,
+                                          float* partial, int behind) {
   constexpr int TM = TL::TM, TN = TL::TN;
   fit<DW>(a, p);
   const int N = DW ? a.V : p.b.rows;
@@ -790,7 +794,7 @@ __global__ __launch_bounds__(TL::NT, TL::WPS) void xent_grad_kernel(GradArgs a, 
     product_tile<TL, false, !DW, F16>(p, lds, tm * TL::BM, tn * TL::BN, (int)((int64_t)split * stages / splits),
                                  (int)((int64_t)(split + 1) * stages / splits), acc);
     if (splits > 1) {
-      f32x4_t* to = reinterpret_cast<f32x4_t*>(a.partial) +
+      f32x4_t* to = reinterpret_cast<f32x4_t*>(partial) +
                     (int64_t)(split * plan.tail + tile - plan.whole) * (TL::BM * TL::BN / 4) +
                     wave * (TM * TN * 4 * 64) + lane;
 #pragma unroll
@@ -814,7 +818,7 @@ __global__ __launch_bounds__(TL::NT, TL::WPS) void xent_grad_kernel(GradArgs a, 
       }
   };
   // (one loop over both lists: the tile's code once)
-  const Items whole(plan.whole), tail(plan.tail * plan.splits);
+  const Items whole(plan.whole, behind), tail(plan.tail * plan.splits, behind);
   int item = whole.first;
   bool rest = item >= whole.end;
   if (rest) item = tail.first;
@@ -827,12 +831,31 @@ __global__ __launch_bounds__(TL::NT, TL::WPS) void xent_grad_kernel(GradArgs a, 
       item = tail.first;
     }
   }
+  return (plan.tail * plan.splits + 7) / 8;
 }
 
-// The splits of the last round's tiles added in order; a workgroup per MFMA tile of
-// each wave.
 template <class TL, bool DW, bool F16>
-__global__ __launch_bounds__(TL::NT) void xent_grad_join_kernel(GradArgs a, Product p, Out o) {
+__global__ __launch_bounds__(TL::NT, TL::WPS) void xent_grad_kernel(GradArgs a, Product p, Out o) {
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[TL::NS * TL::BUF];
+  (void)grad_tiles<TL, DW, F16>(a, p, o, lds, a.partial, 0);
+}
+// Both, of small tiles: dw's items start at the workgroups behind dx's last ones.  (A step
+// of 512 rows of D 512 and 8192 entries 67.6 us with two launches and their joins', 56.8
+// so; larger tiles' launches are long enough: 16384 rows of D 2048 and 50257 entries 8.97
+// ms with two, 9.03 with one.)
+template <class TL, bool F16>
+__global__ __launch_bounds__(TL::NT, TL::WPS) void xent_grads_kernel(GradArgs a, Product px, Out ox, Product pw,
+                                                                     Out ow) {
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[TL::NS * TL::BUF];
+  const int behind = grad_tiles<TL, false, F16>(a, px, ox, lds, a.partial, 0);
+  (void)grad_tiles<TL, true, F16>(a, pw, ow, lds, a.partial + (int64_t)a.scratch_tiles * (TL::BM * TL::BN), behind);
+}
+
+// The splits of the last round's tiles added in order; a workgroup per quad of registers
+// of all waves.
+template <class TL, bool DW, bool F16>
+__device__ __forceinline__ int grad_join(const GradArgs& a, Product p, const Out& o, const float* partial,
+                                         int item) {
   constexpr int TM = TL::TM, TN = TL::TN, AHEAD = 16;
   fit<DW>(a, p);
   const int N = DW ? a.V : p.b.rows;
@@ -840,16 +863,16 @@ __global__ __launch_bounds__(TL::NT) void xent_grad_join_kernel(GradArgs a, Prod
   const Split plan = split_of(mt * nt, p.nk * p.pairs, a.slots, a.scratch_tiles);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int wm = wave / TL::WN, wn = wave % TL::WN;
-  if (plan.splits == 1) return;
+  if (plan.splits == 1) return item;
   const int64_t step = (int64_t)plan.tail * (TL::BM * TL::BN / 4);
   // a quad of each lane's registers at a time
-  for (int item = blockIdx.x; item < plan.tail * (TM * TN * 4); item += gridDim.x) {
+  for (; item < plan.tail * (TM * TN * 4); item += gridDim.x) {
     const int tile = item / (TM * TN * 4), ijq = item % (TM * TN * 4);
     const int i = ijq / (TN * 4), j = ijq / 4 % TN, q = ijq % 4;
     int tm, tn;
     tile_at(plan.whole + tile, mt, nt, tm, tn);
     f32x4_t c = {0.0f, 0.0f, 0.0f, 0.0f};
-    const f32x4_t* from = reinterpret_cast<const f32x4_t*>(a.partial) + (int64_t)tile * (TL::BM * TL::BN / 4) +
+    const f32x4_t* from = reinterpret_cast<const f32x4_t*>(partial) + (int64_t)tile * (TL::BM * TL::BN / 4) +
                           wave * (TM * TN * 4 * 64) + ijq * 64 + lane;
     for (int s = 0; s < plan.splits; s += AHEAD) {
       f32x4_t v[AHEAD];
@@ -864,6 +887,16 @@ __global__ __launch_bounds__(TL::NT) void xent_grad_join_kernel(GradArgs a, Prod
     const int n = tn * TL::BN + (wn * TN + j) * 32 + (lane & 31);
     if (n < N) put_quad<F16>(o, tm * TL::BM + (wm * TM + i) * 32 + q * 8 + (lane >> 5) * 4, n, c);
   }
+  return item - plan.tail * (TM * TN * 4);
+}
+template <class TL, bool DW, bool F16>
+__global__ __launch_bounds__(TL::NT) void xent_grad_join_kernel(GradArgs a, Product p, Out o) {
+  (void)grad_join<TL, DW, F16>(a, p, o, a.partial, blockIdx.x);
+}
+template <class TL, bool F16>
+__global__ __launch_bounds__(TL::NT) void xent_grads_join_kernel(GradArgs a, Product px, Out ox, Product pw, Out ow) {
+  const int item = grad_join<TL, false, F16>(a, px, ox, a.partial, blockIdx.x);
+  (void)grad_join<TL, true, F16>(a, pw, ow, a.partial + (int64_t)a.scratch_tiles * (TL::BM * TL::BN), item);
 }
 
 // ---- launches ----
@@ -940,51 +973,72 @@ void launch_logits(const XentArgs& a, const Product& p, int64_t r0, int64_t rows
     typed(std::false_type{});
 }
 
-// The device counts the rows that take part, so it decides how tiles are split: the
-// second launch is there wherever it may.
-template <class TL, bool DW>
-void launch_grad(const XentArgs& a, const Product& p, const Out& o, int64_t r0, int64_t N, int per_cu,
-                 hipStream_t s) {
-  const int64_t tiles = tiles_of(a.D, N, TL::BM, TL::BN);
-  const int slots = a.n_cu * per_cu / 8 * 8;
-  const int scratch = (int)(mxm_xent_partial_bytes(a.n_cu) / (TL::BM * TL::BN * 4));
-  const int64_t most = std::min<int64_t>((DW ? tiles % slots : std::min<int64_t>(tiles, slots - 1)) * TL::TM * TL::TN * 4,
-                                         (int64_t)a.n_cu * 8);
-  const GradArgs g{a.scalars, r0, a.piece_rows, a.V, a.D, a.partial, slots, scratch};
-  const auto launch = [&](auto kernel, int64_t grid) {
-    if (grid > 0) kernel<<<(unsigned)grid, TL::NT, 0, s>>>(g, p, o);
-  };
-  if (a.planes == 1) {
-    launch(xent_grad_kernel<TL, DW, false>, slots);
-    launch(xent_grad_join_kernel<TL, DW, false>, most);
-  } else {
-    launch(xent_grad_kernel<TL, DW, true>, slots);
-    launch(xent_grad_join_kernel<TL, DW, true>, most);
-  }
-}
+// One product's launch.
+struct Grad {
+  Product p;
+  Out o;
+  int64_t N;
+};
+enum GradShape { G_SMALL, G_THIN, G_BIG };
 
 // The shape whose tiles take the least time by split_of's count of stages, at a stage's
 // time (Small: of two on a CU).  Measured: a step of 8192 rows and 32768 entries at D
 // 320 982 us in tiles of 256 channels, 930 of 192; D 384 1014 / 965; of 315 rows and 256
 // entries in fp32 at D 1528 89 us in tiles of 256, 76 so.
-template <bool DW>
-void launch_grad(const XentArgs& a, const Product& p, const Out& o, int64_t r0, int64_t rows, hipStream_t s) {
-  const int64_t N = DW ? a.V : rows;
-  const int stages = (int)(DW ? (rows + BK - 1) / BK : p.nk) * p.pairs;
+GradShape grad_shape(const XentArgs& a, const Grad& g, int64_t k) {
+  const int stages = (int)((k + BK - 1) / BK) * g.p.pairs;
   const auto time = [&](auto tile, int per_cu, double stage) {
     using TL = decltype(tile);
     const int slots = a.n_cu * per_cu / 8 * 8;
-    return stage * split_of((int)tiles_of(a.D, N, TL::BM, TL::BN), stages, slots,
+    return stage * split_of((int)tiles_of(a.D, g.N, TL::BM, TL::BN), stages, slots,
                             (int)(mxm_xent_partial_bytes(a.n_cu) / (TL::BM * TL::BN * 4)))
                        .cost;
   };
   const double big = time(Big{}, 1, 1.0), thin = time(Thin{}, 1, 0.8), small = time(Small{}, 2, 0.65);
-  if (small < big && small < thin)
-    launch_grad<Small, DW>(a, p, o, r0, N, 2, s);
-  else if (thin < big)
-    launch_grad<Thin, DW>(a, p, o, r0, N, 1, s);
+  return small < big && small < thin ? G_SMALL : thin < big ? G_THIN : G_BIG;
+}
+
+// The device counts the rows that take part, so it decides how tiles are split: the
+// second launch is there wherever it may.  dx, dw or (small tiles) both, null: not.
+template <class TL>
+void launch_grads(const XentArgs& a, const Grad* dx, const Grad* dw, int64_t r0, int per_cu, hipStream_t s) {
+  const int slots = a.n_cu * per_cu / 8 * 8;
+  const bool both = dx && dw;
+  const int scratch = (int)(mxm_xent_partial_bytes(a.n_cu) / (TL::BM * TL::BN * 4)) / (both ? 2 : 1);
+  int64_t joins = 0;
+  if (dx) joins += std::min<int64_t>(tiles_of(a.D, dx->N, TL::BM, TL::BN), slots - 1);
+  if (dw) joins += tiles_of(a.D, dw->N, TL::BM, TL::BN) % slots;
+  joins = std::min<int64_t>(joins * TL::TM * TL::TN * 4, (int64_t)a.n_cu * 8);
+  const GradArgs g{a.scalars, r0, a.piece_rows, a.V, a.D, a.partial, slots, scratch};
+  const auto typed = [&](auto f16) {
+    constexpr bool F16 = decltype(f16)::value;
+    if constexpr (std::is_same_v<TL, Small>) {
+      if (both) {
+        xent_grads_kernel<TL, F16><<<slots, TL::NT, 0, s>>>(g, dx->p, dx->o, dw->p, dw->o);
+        if (joins > 0)
+          xent_grads_join_kernel<TL, F16><<<(unsigned)joins, TL::NT, 0, s>>>(g, dx->p, dx->o, dw->p, dw->o);
+        return;
+      }
+    }
+    if (dx) {
+      xent_grad_kernel<TL, false, F16><<<slots, TL::NT, 0, s>>>(g, dx->p, dx->o);
+      if (joins > 0) xent_grad_join_kernel<TL, false, F16><<<(unsigned)joins, TL::NT, 0, s>>>(g, dx->p, dx->o);
+    } else {
+      xent_grad_kernel<TL, true, F16><<<slots, TL::NT, 0, s>>>(g, dw->p, dw->o);
+      if (joins > 0) xent_grad_join_kernel<TL, true, F16><<<(unsigned)joins, TL::NT, 0, s>>>(g, dw->p, dw->o);
+    }
+  };
+  if (a.planes == 1)
+    typed(std::false_type{});
   else
-    launch_grad<Big, DW>(a, p, o, r0, N, 1, s);
+    typed(std::true_type{});
+}
+void launch_grads(const XentArgs& a, GradShape shape, const Grad* dx, const Grad* dw, int64_t r0, hipStream_t s) {
+  switch (shape) {
+    case G_SMALL: return launch_grads<Small>(a, dx, dw, r0, 2, s);
+    case G_THIN: return launch_grads<Thin>(a, dx, dw, r0, 1, s);
+    default: return launch_grads<Big>(a, dx, dw, r0, 1, s);
+  }
 }
 
 }  // namespace
@@ -1024,37 +1078,49 @@ void mxm_launch_xent_logits(const XentArgs& a, int64_t r0, int64_t rows, const i
   }
 }
 
-void mxm_launch_xent_dx(const XentArgs& a, int64_t r0, int64_t rows, hipStream_t s) {
-  Product p{};
-  set_planes(a, p);
-  p.a = table(a, false);
-  p.b = grad(a);
-  p.nk = (a.V + BK - 1) / BK;
-  Out o{};
-  o.out = a.dx;
-  o.map = a.map + r0;
-  o.e_row = a.e_row + r0;
-  o.M = a.D;
-  o.bf16 = a.dx_bf16;
-  o.vec = aligned(a.dx) && a.D % (a.dx_bf16 ? 8 : 4) == 0;
-  launch_grad<false>(a, p, o, r0, rows, s);
-}
-
-void mxm_launch_xent_dw(const XentArgs& a, int64_t r0, int64_t rows, bool last, const int32_t* low,
-                        hipStream_t s) {
-  Product p{};
-  set_planes(a, p);
-  p.a = hidden(a, false, r0);
-  p.b = grad(a);
-  Out o{};
-  float* sums = a.dw32 ? a.dw32 : static_cast<float*>(a.dw);
-  o.out = last ? a.dw : sums;
-  o.bf16 = last && a.dw_bf16;
-  o.add = r0 > 0 ? sums : nullptr;
-  o.w_exp = a.w_exp;
-  o.low = low;
-  o.scalars = a.scalars;
-  o.M = a.D;
-  o.vec = aligned(o.out) && a.D % (o.bf16 ? 8 : 4) == 0;
-  launch_grad<true>(a, p, o, r0, rows, s);
+void mxm_launch_xent_grads(const XentArgs& a, int64_t r0, int64_t rows, bool last, const int32_t* low,
+                           hipStream_t s) {
+  Grad dx{}, dw{};
+  const bool want_dx = a.dx && rows > 0;
+  GradShape shape_dx = G_BIG, shape_dw = G_BIG;
+  if (want_dx) {
+    Product& p = dx.p;
+    Out& o = dx.o;
+    set_planes(a, p);
+    p.a = table(a, false);
+    p.b = grad(a);
+    p.nk = (a.V + BK - 1) / BK;
+    o.out = a.dx;
+    o.map = a.map + r0;
+    o.e_row = a.e_row + r0;
+    o.M = a.D;
+    o.bf16 = a.dx_bf16;
+    o.vec = aligned(a.dx) && a.D % (a.dx_bf16 ? 8 : 4) == 0;
+    dx.N = rows;
+    shape_dx = grad_shape(a, dx, a.V);
+  }
+  if (a.dw) {
+    Product& p = dw.p;
+    Out& o = dw.o;
+    set_planes(a, p);
+    p.a = hidden(a, false, r0);
+    p.b = grad(a);
+    float* sums = a.dw32 ? a.dw32 : static_cast<float*>(a.dw);
+    o.out = last ? a.dw : sums;
+    o.bf16 = last && a.dw_bf16;
+    o.add = r0 > 0 ? sums : nullptr;
+    o.w_exp = a.w_exp;
+    o.low = low;
+    o.scalars = a.scalars;
+    o.M = a.D;
+    o.vec = aligned(o.out) && a.D % (o.bf16 ? 8 : 4) == 0;
+    dw.N = a.V;
+    shape_dw = grad_shape(a, dw, rows);
+  }
+  if (want_dx && a.dw && shape_dx == G_SMALL && shape_dw == G_SMALL) {
+    launch_grads(a, G_SMALL, &dx, &dw, r0, s);
+    return;
+  }
+  if (want_dx) launch_grads(a, shape_dx, &dx, nullptr, r0, s);
+  if (a.dw) launch_grads(a, shape_dw, nullptr, &dw, r0, s);
 }
