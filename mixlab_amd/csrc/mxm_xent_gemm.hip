@@ -443,7 +443,7 @@ struct LogitsArgs {
   float softcap;
   const int32_t *target, *x_exp, *w_exp;
   float* at_target;
-  const int32_t* low;
+  const int32_t* low;      // L that the table's planes were taken down to, or null
   float2* stat;
   int32_t* stat_exp;
   int64_t stat_ld;

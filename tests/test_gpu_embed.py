@@ -41,6 +41,8 @@ def tokens_of(kind, rng, N, V):
     (130, 100, 90, "bf16", "bf16", 0, "skewed"),
     (130, 72, 90, "bf16", "bf16", 4, "skewed"),
     (20000, 300, 50, "bf16", "bf16", 2, "skewed"),
+    (7, 16384, 30, "bf16", "fp32", 0, "extremes"),
+    (9, 16383, 30, "fp32", "bf16", 0, "skewed"),
 ])
 def test_forward(gpu_lib, N, D, V, table, out, shift, kind):
     rng = np.random.default_rng(N + D)
@@ -78,6 +80,9 @@ def test_forward(gpu_lib, N, D, V, table, out, shift, kind):
     (9, 1024, 5000, "fp32", "fp32", 0, "extremes", True),
     (8, 2048, 20000, "fp32", "bf16", 0, "uniform", False),
     (2049, 32, 700, "fp32", "fp32", 0, "skewed", True),
+    (70, 16384, 9, "bf16", "fp32", 0, "skewed", True),
+    (50, 16383, 7, "fp32", "bf16", 0, "extremes", False),
+    (40000, 8, 700000, "fp32", "fp32", 0, "skewed", True),
     (700, 72, 90, "bf16", "bf16", 4, "skewed", False),
     (700, 72, 90, "bf16", "fp32", 2, "skewed", False),
 ])

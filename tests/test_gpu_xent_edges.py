@@ -118,6 +118,17 @@ def test_few_rows(gpu_lib, N, D, V, pad, weighted, shift, dtype):
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("N,D,V,weighted,pad", [
+    (40, 16384, 70, False, 0.0), (6, 16383, 130, True, 0.0), (300, 2056, 1, False, 0.2),
+    (4096, 40, 90, True, 0.3), (4097, 40, 90, True, 0.3), (9001, 24, 65, True, 0.6)])
+def test_extreme_sizes(gpu_lib, N, D, V, weighted, pad, dtype):
+    """The widest rows, a table of one entry, batches around the counts' own launch."""
+    x, w, t = inputs(N, D, V, dtype, N + D, pad=pad)
+    weights = np.random.default_rng(V).uniform(0.5, 1.5, N).astype(np.float32) if weighted else None
+    check(x, w, t, weights, dtype=dtype, calls=2)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
 def test_elements_of_unlike_magnitude(gpu_lib, dtype):
     """Within a row of x and of the table: below the planes' reach an element counts as
     far as its share of the row's largest."""
