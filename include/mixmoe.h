@@ -448,8 +448,9 @@ int mxm_embed_backward(int64_t h, int64_t rows, const int32_t* tokens, const voi
  * infinity or the type's lowest value keeps from coming has no share in any result
  * (but that dx of a bf16 table with infinities is not a number, 0 times those);
  * as a target it makes the loss infinite (or as large), and then dx and dw are of no
- * use.  A row of x that is not finite spoils its own results and dw.  softcap 0:
- * none.  Returns a handle, 0 on failure. */
+ * use.  A row of x that is not finite spoils its own results and dw.  softcap is
+ * 0 (none) or in [1/64, 1024]; capped logits are off by a few 2^-24 of it, and minus
+ * infinity is -softcap under it.  Returns a handle, 0 on failure. */
 #define MXM_XENT_MEAN 1
 #define MXM_XENT_BACKWARD 2 /* the handle also runs backward (holds its workspace) */
 int64_t mxm_xent_create(const int64_t* params, int n_params, float softcap, int64_t stream_of);

@@ -69,6 +69,9 @@ void check_rows(const char* what, int64_t rows, int64_t max_rows) {
 }
 int item(bool bf16) { return bf16 ? 2 : 4; }
 
+// Softcaps: a capped logit is off by a few 2^-24 of the cap, 1.2e-4 at the largest.
+constexpr float XENT_MIN_CAP = 1.0f / 64, XENT_MAX_CAP = 1024;
+
 // Bytes that a loss's workspace holds of a piece of the rows at most (but for tables
 // of which a tile's rows take more).
 constexpr int64_t XENT_PIECE_BYTES = (int64_t)2 << 30;
@@ -240,7 +243,8 @@ int64_t mxm_xent_create(const int64_t* params, int n_params, float softcap, int6
     for (int i = 3; i < 6; ++i) check_dtype(XENT, params[i]);
     if (flags & ~(int64_t)(MXM_XENT_MEAN | MXM_XENT_BACKWARD))
       fail(XENT " unknown flags 0x%llx", (unsigned long long)flags);
-    if (!(softcap >= 0.0f) || !std::isfinite(softcap)) fail(XENT " softcap must be finite and >= 0");
+    if (softcap != 0.0f && !(softcap >= XENT_MIN_CAP && softcap <= XENT_MAX_CAP))
+      fail(XENT " softcap must be 0 or in [%g,%g]", XENT_MIN_CAP, XENT_MAX_CAP);
     auto shared = shared_stream(XENT, stream_of);
 
     auto x = std::make_shared<Xent>();

@@ -431,8 +431,10 @@ struct Rows {
 
 // What bounds the epilogue is its transcendentals, one per logit and three with a
 // softcap, at a quarter of the other instructions' rate: about 4 us of a 256 x 256 tile
-// without and 8 with it, next to 1.5 us per stage of the sum.  The largest logit is
-// taken before the cap, which keeps their order.
+// without and 8 with it, next to 1.5 us per stage of the sum.  Under a softcap the
+// entries that do not count are put at a tanh far below any other, after it, where the
+// few blocks that have some do it: a comparison of every logit took 465 us of 16384 x
+// 50257 at D 64, 433 so.
 // (What the kernels take, and no more: every argument is a scalar register that the sum's
 // loop has to keep, and some forty more of them had it reading them back from vector
 // registers: 2720 us of 16384 x 50257 logits at D 2048 became 2940.)
@@ -563,26 +565,57 @@ __global__ __launch_bounds__(TL::NT, F16 && TL::NS == 4 ? 1 : TL::WPS) void xent
             for (int k = 0; k < 4; ++k) acc[i][j][q * 4 + k] = ldexpf(acc[i][j][q * 4 + k], we[k] + x_exps[j]);
           }
       }
-      // entries behind the vocabulary, and the target (whose logit is kept apart)
+      // entries behind the vocabulary, and the target (whose logit is kept apart), get one
+      // with an exponential of 0 (under a softcap a tanh, so small that no ref brings it
+      // back and no slope times 0 leaves 0: a logit of minus infinity is its lowest there)
+      const float none = CAP ? -(200.0f / cap2 + 4.0f) : -__builtin_inff();
+      const bool here = __ballot(target >= mw && target < mw + TM * 32) != 0;
+      const int at = target - first;
+      if (here) {
+        // (as branches with a softcap, and as selections without, the comparisons take some
+        // hundred scalar registers too many)
+        if constexpr (CAP) {
+          float z = 0.0f;
+#pragma unroll
+          for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) z = at == i * 32 + (r >> 2) * 8 + (r & 3) ? acc[i][j][r] : z;
+          // (of the two half-waves the one that holds it)
+          if (at >= 0 && at < TM * 32 && (at & 4) == 0) a.at_target[n] = z;
+        } else {
+#pragma unroll
+          for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+              if (at == i * 32 + (r >> 2) * 8 + (r & 3)) {
+                a.at_target[n] = acc[i][j][r];
+                acc[i][j][r] = none;
+              }
+        }
+      }
+      if constexpr (CAP) {
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) acc[i][j][r] = mxm_xent_capped(acc[i][j][r], k2);
+        if (here) {
+          int again = at;
+          asm volatile("" : "+v"(again));  // (else the comparisons above are kept, in 128 scalar registers)
+#pragma unroll
+          for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+              acc[i][j][r] = again == i * 32 + (r >> 2) * 8 + (r & 3) ? none : acc[i][j][r];
+        }
+      }
       if (mw + TM * 32 > a.V) {
         int end = a.V - first;
-        asm volatile("" : "+v"(end));  // (else the loop's comparisons move before it, into 128 scalar registers)
+        asm volatile("" : "+v"(end));  // (nor move before the branch)
 #pragma unroll
         for (int i = 0; i < TM; ++i)
 #pragma unroll
           for (int r = 0; r < 16; ++r)
-            acc[i][j][r] = i * 32 + (r >> 2) * 8 + (r & 3) >= end ? -__builtin_inff() : acc[i][j][r];
-      }
-      if (__ballot(target >= mw && target < mw + TM * 32) != 0) {
-        const int at = target - first;
-#pragma unroll
-        for (int i = 0; i < TM; ++i)
-#pragma unroll
-          for (int r = 0; r < 16; ++r)
-            if (at == i * 32 + (r >> 2) * 8 + (r & 3)) {
-              a.at_target[n] = acc[i][j][r];
-              acc[i][j][r] = -__builtin_inff();
-            }
+            acc[i][j][r] = i * 32 + (r >> 2) * 8 + (r & 3) >= end ? none : acc[i][j][r];
       }
       float top = acc[0][j][0];
 #pragma unroll
@@ -592,33 +625,21 @@ __global__ __launch_bounds__(TL::NT, F16 && TL::NS == 4 ? 1 : TL::WPS) void xent
       top = fmaxf(top, mxm_xor_lane_f(top, 32));
       // 2^(l log2 e - ref) lies in (0, 2^15]: fp16 keeps 12 bits of summands down to
       // 2^-29 of the block's largest and 2^-39 of it at all
-      float ref = -1.0e30f;  // (of a block of minus infinities)
-      if (top > -__builtin_inff()) ref = ceilf(CAP ? cap2 * mxm_xent_capped(top, k2) : top * LOG2E) - 15.0f;
+      const bool any = CAP ? top >= -2.0f : top > -__builtin_inff();
+      const float ref = any ? ceilf(CAP ? cap2 * top : top * LOG2E) - 15.0f : 0.0f;
       float s[2] = {0.0f, 0.0f};
-      if constexpr (CAP) {
 #pragma unroll
-        for (int i = 0; i < TM; ++i)
+      for (int i = 0; i < TM; ++i)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const float th = mxm_xent_capped(acc[i][j][r], k2);
-            float e = __builtin_amdgcn_exp2f(fmaf(th, cap2, -ref));
-            e = acc[i][j][r] == -__builtin_inff() ? 0.0f : e;
-            s[r & 1] += e;
-            acc[i][j][r] = e * fmaf(-th, th, 1.0f);
-          }
-      } else {
-#pragma unroll
-        for (int i = 0; i < TM; ++i)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            acc[i][j][r] = __builtin_amdgcn_exp2f(fmaf(acc[i][j][r], LOG2E, -ref));
-            s[r & 1] += acc[i][j][r];
-          }
-      }
+        for (int r = 0; r < 16; ++r) {
+          const float v = acc[i][j][r], e = __builtin_amdgcn_exp2f(fmaf(v, CAP ? cap2 : LOG2E, -ref));
+          s[r & 1] += e;
+          acc[i][j][r] = CAP ? e * fmaf(-v, v, 1.0f) : e;
+        }
       float sum = s[0] + s[1];
       sum += mxm_xor_lane_f(sum, 32);
       const int64_t at_stat = (int64_t)(mw / (TM * 32)) * a.stat_ld + n;
-      if (n < rows && mw < a.V && lane < 32) a.stat[at_stat] = make_float2(sum, ref);
+      if (n < rows && mw < a.V && lane < 32) a.stat[at_stat] = make_float2(sum, any ? ref : -1.0e30f);
       if constexpr (F16 && STORE) {
         // (2^(w - 1): none overflows)
         float big = 0.0f;

@@ -80,6 +80,42 @@ def test_masked_entries(gpu_lib, dtype, lowest, monkeypatch):
         assert not np.any(gw.get()[out])
 
 
+@pytest.mark.parametrize("cap", [4.0, 1.0])
+@pytest.mark.parametrize("dtype,lowest", [("bf16", -3.38e38), ("fp32", -3.38e38), ("fp32", -np.inf)])
+def test_masked_entries_under_a_softcap(gpu_lib, dtype, lowest, cap):
+    """Their logit is -softcap, as the formula has it, with a slope of zero."""
+    N, D, V = 300, 72, 330
+    x, w, t = inputs(N, D, V, dtype, 28)
+    x[:, 0] = np.abs(x[:, 0]) + 0.5
+    x = as_kept(x, dtype)
+    out = np.array([3, 77, 78, 299])
+    t[np.isin(t, out)] = 5
+    keep = np.setdiff1d(np.arange(V), out)
+    part = token_loss(x, w[keep], np.searchsorted(keep, t), softcap=cap)
+    row, bx, bw = tolerances(x, w[keep], part, dtype, cap, V)
+    w[out, 0] = -1e6  # (of a tanh of -1 too)
+    ref = token_loss(x, w, t, softcap=cap)
+    w[out, 0] = as_kept(np.array([lowest]), dtype)
+    dx_, dw_, dt = Dev(x, dtype), Dev(w, dtype), Dev(t.astype(np.int32), "int32")
+    loss, lse, gx, gw = Dev.out((N,)), Dev.out((N,)), Dev.out((N, D)), Dev.out((V, D))
+    with TokenLoss(V, D, N, dtype=dtype, softcap=cap) as h:
+        h.backward(N, dx_.ptr, dw_.ptr, dt.ptr, dx=gx.ptr, dw=gw.ptr, loss=loss.ptr, lse=lse.ptr)
+        h.synchronize()
+    assert cap > 1.0 or np.all(ref["lse"] - part["lse"] > row)  # (without their share lse is off by more)
+    close(loss.get(), ref["loss"], row, "fp32", "loss")
+    close(lse.get(), ref["lse"], row, "fp32", "lse")
+    close(gx.get(), ref["dx"], bx, "fp32", "dx")
+    close(gw.get()[keep], ref["dw"][keep], bw, "fp32", "dw")
+    assert not np.any(gw.get()[out])
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("cap", [1 / 64, 0.5, 1024.0])
+def test_caps(gpu_lib, dtype, cap):
+    x, w, t = inputs(150, 72, 330, dtype, 29, pad=0.1)
+    check(x, w, t, dtype=dtype, softcap=cap)
+
+
 @pytest.mark.parametrize("dx,dw", [(True, True), (True, False), (False, True)])
 def test_pieces_of_unlike_magnitude(gpu_lib, dx, dw, monkeypatch):
     """Under fp32, pieces whose gradients reach rows of the table of ever larger or ever

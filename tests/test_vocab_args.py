@@ -44,7 +44,7 @@ def test_embed_create_refuses(kw, want):
     (dict(n=6), "requires V,D,maxRows"), (dict(dtypes=(0, F32, F32)), "dtype 0 unsupported"),
     (dict(dtypes=(BF16, F32, 3)), "dtype 3 unsupported"),
     (dict(softcap=-1.0), "softcap"), (dict(softcap=float("nan")), "softcap"),
-    (dict(softcap=float("inf")), "softcap"),
+    (dict(softcap=float("inf")), "softcap"), (dict(softcap=0.01), "softcap"), (dict(softcap=1025.0), "softcap"),
 ])
 def test_xent_create_refuses(kw, want):
     assert _xent(**kw) == 0
