@@ -112,9 +112,10 @@ struct XentArgs {
   // workspace
   int Dp, Vp;               // D rounded up to whole stages; V to an odd number of them
   int planes;               // 1 (bf16) or 2 (fp32)
-  int32_t* slot;            // [rows] a row's place among those that take part, or -1
-  int32_t* map;             // [rows] and back
+  int32_t* map;             // [rows] a row that takes part, by its place among those
   int32_t* target;          // [rows] of those that take part
+  int32_t* counts;          // [XENT_CHUNKS] of rows that take part, and their weights' sums
+  double* weights;
   XentScalars* scalars;
   float* nll;               // [rows] loss of the rows that take part
   float* at_target;         // [rows] their target's logit, before the cap
@@ -137,6 +138,7 @@ struct XentArgs {
   int64_t piece_rows, stat_ld;
   int n_cu;
 };
+constexpr int XENT_CHUNKS = 4096;  // most chunks of a call's rows
 // Bytes of partial, for handles that run backward.
 int64_t mxm_xent_partial_bytes(int n_cu);
 // Most blocks of stat times rows, for pieces of `rows`.

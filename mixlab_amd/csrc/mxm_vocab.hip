@@ -26,7 +26,7 @@ struct Xent : TrainHandle {
   XentArgs base{};
   int64_t max_rows = 0;
   bool backward = false;
-  DevBuf slot, map, target, scalars, nll, at_target, row, x_pack, w_pack, exps, parts, stat, stat_exp, summands, dz, partial, dw32, zeros;
+  DevBuf counts, weights, map, target, scalars, nll, at_target, row, x_pack, w_pack, exps, parts, stat, stat_exp, summands, dz, partial, dw32, zeros;
   ~Xent() override {
     if (stream_ref) (void)hipStreamSynchronize(stream());
   }
@@ -276,7 +276,8 @@ int64_t mxm_xent_create(const int64_t* params, int n_params, float softcap, int6
     const int64_t row_bytes = (V + 127) / 128 * (x->backward && !a.bf16 ? 12 : 8) + (x->backward ? a.Vp * (int64_t)(a.bf16 ? 2 : 8) : 0);
     a.piece_rows = std::max<int64_t>(256, std::min(up(rows), bytes / row_bytes / 256 * 256));
     if (rows < a.piece_rows) a.piece_rows = std::max<int64_t>(64, up(rows));
-    x->slot.alloc((size_t)rows * 4);
+    x->counts.alloc(XENT_CHUNKS * 4);
+    x->weights.alloc(XENT_CHUNKS * 8);
     x->map.alloc((size_t)rows * 4);
     x->target.alloc((size_t)rows * 4);
     x->scalars.alloc(sizeof(XentScalars));
@@ -300,7 +301,8 @@ int64_t mxm_xent_create(const int64_t* params, int n_params, float softcap, int6
     }
     x->zeros.alloc(4096);
     HIPCK(hipMemsetAsync(x->zeros.p, 0, 4096, x->stream()));
-    a.slot = x->slot.as<int32_t>();
+    a.counts = x->counts.as<int32_t>();
+    a.weights = x->weights.as<double>();
     a.map = x->map.as<int32_t>();
     a.target = x->target.as<int32_t>();
     a.scalars = x->scalars.as<XentScalars>();

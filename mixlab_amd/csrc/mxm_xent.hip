@@ -21,68 +21,30 @@ __device__ __forceinline__ void leave_out(const XentArgs& a, int64_t n) {
   if (a.lse) a.lse[n] = 0.0f;
 }
 
-// The rows that take part, in order, and the sum of their weights; zeros for the
-// others' loss and lse.
-constexpr int PLAN_NT = 1024;
-__global__ __launch_bounds__(PLAN_NT) void xent_plan_kernel(XentArgs a) {
-  constexpr int EACH = 8;  // rows per thread and turn, PLAN_NT apart
-  __shared__ int wave_count[2][EACH][16];
-  __shared__ double wave_weight[16];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int64_t base = 0;
+// How many rows of each chunk take part, and the sum of their weights; a wave per chunk.
+constexpr int NT = 256;
+__global__ __launch_bounds__(NT) void xent_count_kernel(XentArgs a, int64_t chunk, int chunks) {
+  const int lane = threadIdx.x & 63, c = blockIdx.x * (NT / 64) + (threadIdx.x >> 6);
+  if (c >= chunks) return;
+  int count = 0;
   double sum = 0.0;
-  int turn = 0;
-  for (int64_t n0 = 0; n0 < a.rows; n0 += PLAN_NT * EACH, turn ^= 1) {
-    int t[EACH];
-    float w[EACH];
-    bool in[EACH];
-    unsigned long long m[EACH];
-#pragma unroll
-    for (int k = 0; k < EACH; ++k) {
-      const int64_t n = n0 + k * PLAN_NT + threadIdx.x;
-      w[k] = 0.0f;
-      in[k] = n < a.rows && takes_part(a, n, t[k], w[k]);
-    }
-#pragma unroll
-    for (int k = 0; k < EACH; ++k) {
-      sum += in[k] ? (double)w[k] : 0.0;
-      m[k] = __ballot(in[k]);
-      if (lane == 0) wave_count[turn][k][wave] = __popcll(m[k]);
-    }
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < EACH; ++k) {
-      const int64_t n = n0 + k * PLAN_NT + threadIdx.x;
-      const int c = lane < 16 ? wave_count[turn][k][lane] : 0;
-      int before = lane < wave ? c : 0, all = c;
-#pragma unroll
-      for (int o = 1; o < 16; o <<= 1) {
-        before += __shfl_xor(before, o);
-        all += __shfl_xor(all, o);
-      }
-      before = __builtin_amdgcn_readfirstlane(before);
-      const int64_t at = base + before + __popcll(m[k] & ((1ull << lane) - 1));
-      if (n < a.rows) {
-        a.slot[n] = in[k] ? (int32_t)at : -1;
-        if (in[k]) {
-          a.map[at] = (int32_t)n;
-          a.target[at] = t[k];
-        } else {
-          leave_out(a, n);
-        }
-      }
-      base += __builtin_amdgcn_readfirstlane(all);
+  const int64_t from = c * chunk, to = min(from + chunk, a.rows);
+  for (int64_t n = from + lane; n < to; n += 64) {
+    int t;
+    float w;
+    if (takes_part(a, n, t, w)) {
+      ++count;
+      sum += (double)w;
     }
   }
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
-  if (lane == 0) wave_weight[wave] = sum;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    double s = 0.0;
-    for (int i = 0; i < 16; ++i) s += wave_weight[i];
-    a.scalars->weight_sum = s;
-    a.scalars->rows = (int32_t)base;
+  for (int o = 32; o > 0; o >>= 1) {
+    count += __shfl_xor(count, o);
+    sum += __shfl_xor(sum, o);
+  }
+  if (lane == 0) {
+    a.counts[c] = count;
+    a.weights[c] = sum;
   }
 }
 
@@ -102,8 +64,6 @@ __device__ __forceinline__ void planes2x8(const float (&v)[8], u32x4_t (&q)[2]) 
 #pragma unroll
     for (int i = 0; i < 4; ++i) q[k][i] = p[k][2 * i] | (uint32_t)p[k][2 * i + 1] << 16;
 }
-
-constexpr int NT = 256;
 
 // Row `src` of x or weight to row `to` of its pack of `rows` rows, zeros behind D, by a
 // wave; wide: rows of whole aligned 16 bytes.
@@ -195,14 +155,16 @@ __device__ __forceinline__ bool wide_rows(const XentArgs& a, const void* p) {
   return a.D % 8 == 0 && (reinterpret_cast<uintptr_t>(p) & 15) == 0;
 }
 
-// x's rows that take part to their places, dx's others to zeros; a wave per row.
-// PLAN: for up to PLAN_ROWS rows, every workgroup counts those before its own, and the
-// plan's launch is saved (the losses of 4000 rows of D 64 and 1000 entries take 22.1 us
-// with it, 19.2 so; of 8000 25.4, 27.4).
+// x's rows that take part to their places, dx's others to zeros; a workgroup per chunk
+// of rows, a wave per row.  The places are in the rows' order; every workgroup counts the
+// rows before its own: PLAN, for up to PLAN_ROWS rows, by itself, else from the chunks'
+// counts (the losses of 2000 rows of D 64 and 1000 entries take 18.1 us by chunks and 15.8
+// so; of 4000 21.2, 19.8; counted by one workgroup, those of 48000 took 89 us and by chunks
+// 71).
 constexpr int PLAN_ROWS = 4096;
 // The workgroups behind the first x_blocks pack the table.
 template <bool PLAN>
-__global__ __launch_bounds__(NT) void xent_pack_kernel(XentArgs a, int x_blocks) {
+__global__ __launch_bounds__(NT) void xent_pack_kernel(XentArgs a, int x_blocks, int64_t chunk) {
   __shared__ int count[2][4];
   __shared__ double weight[4];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -219,55 +181,62 @@ __global__ __launch_bounds__(NT) void xent_pack_kernel(XentArgs a, int x_blocks)
     return;
   }
   const bool wide = wide_rows(a, a.x);
-  for (int64_t first = (int64_t)blockIdx.x * 4; first < a.rows; first += (int64_t)x_blocks * 4) {
-    const int64_t n = first + wave;
-    int to = -1;
-    if constexpr (PLAN) {
-      int before = 0, all = 0;
-      double sum = 0.0;
+  const int64_t from = blockIdx.x * chunk, end = min(from + chunk, a.rows);
+  int before = 0, all = 0;
+  double sum = 0.0;
+  if constexpr (PLAN) {
 #pragma unroll 4
-      for (int k = threadIdx.x; k < (int)a.rows; k += NT) {
-        int t;
-        float w = 0.0f;
-        if (takes_part(a, k, t, w)) {
-          before += k < n - wave;
-          ++all;
-          sum += (double)w;
-        }
+    for (int k = threadIdx.x; k < (int)a.rows; k += NT) {
+      int t;
+      float w = 0.0f;
+      if (takes_part(a, k, t, w)) {
+        before += k < from;
+        ++all;
+        sum += (double)w;
       }
-#pragma unroll
-      for (int o = 32; o > 0; o >>= 1) {
-        before += __shfl_xor(before, o);
-        all += __shfl_xor(all, o);
-        sum += __shfl_xor(sum, o);
-      }
-      if (lane == 0) count[0][wave] = before, count[1][wave] = all, weight[wave] = sum;
-      __syncthreads();
-      if (first == 0 && threadIdx.x == 0) {
-        a.scalars->rows = count[1][0] + count[1][1] + count[1][2] + count[1][3];
-        a.scalars->weight_sum = ((weight[0] + weight[1]) + weight[2]) + weight[3];
-      }
-      int at = count[0][0] + count[0][1] + count[0][2] + count[0][3];
-      int t = -1;
-      for (int64_t k = first; k <= n && k < a.rows; ++k) {  // (uniform in the wave)
-        float w;
-        const bool in = takes_part(a, k, t, w);
-        if (k == n) to = in ? at : -1;
-        at += in;
-      }
-      if (n < a.rows && lane == 0) {
-        if (to >= 0) {
-          a.map[to] = (int32_t)n;
-          a.target[to] = t;
-        } else {
-          leave_out(a, n);
-        }
-      }
-      __syncthreads();
-    } else if (n < a.rows) {
-      to = a.slot[n];
     }
-    if (n >= a.rows) continue;
+  } else {
+#pragma unroll 4
+    for (int c = threadIdx.x; c < x_blocks; c += NT) {
+      const int n = a.counts[c];
+      before += c < (int)blockIdx.x ? n : 0;
+      all += n;
+      if (blockIdx.x == 0) sum += a.weights[c];
+    }
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    before += __shfl_xor(before, o);
+    all += __shfl_xor(all, o);
+    sum += __shfl_xor(sum, o);
+  }
+  if (lane == 0) count[0][wave] = before, count[1][wave] = all, weight[wave] = sum;
+  __syncthreads();
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    a.scalars->rows = count[1][0] + count[1][1] + count[1][2] + count[1][3];
+    a.scalars->weight_sum = ((weight[0] + weight[1]) + weight[2]) + weight[3];
+  }
+  int at = count[0][0] + count[0][1] + count[0][2] + count[0][3];
+  for (int64_t first = from; first < end; first += 4) {
+    const int64_t n = first + wave;
+    int to = -1, target = -1;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {  // (uniform in the wave)
+      int t;
+      float w;
+      const bool in = first + k < end && takes_part(a, first + k, t, w);
+      if (k == wave && in) to = at, target = t;
+      at += in;
+    }
+    if (n >= end) continue;
+    if (lane == 0) {
+      if (to >= 0) {
+        a.map[to] = (int32_t)n;
+        a.target[to] = target;
+      } else {
+        leave_out(a, n);
+      }
+    }
     if (to >= 0) {
       if (a.planes == 1) {
         pack_row(a, a.x, wide, n, a.x_pack, to, lane);
@@ -475,8 +444,10 @@ __global__ __launch_bounds__(NT) void xent_join_kernel(XentArgs a, int64_t r0, i
 // The total, by a workgroup.
 template <int T>
 __device__ __forceinline__ void sum_total(const XentArgs& a, double* part) {
+  const int rows = a.scalars->rows;
   double s = 0.0;
-  for (int i = threadIdx.x; i < a.scalars->rows; i += T)
+#pragma unroll 8
+  for (int i = threadIdx.x; i < rows; i += T)
     s += (double)a.nll[i] * (a.row_weights ? (double)a.row_weights[a.map[i]] : 1.0);
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
@@ -485,7 +456,7 @@ __device__ __forceinline__ void sum_total(const XentArgs& a, double* part) {
   if (threadIdx.x == 0) {
     s = 0.0;
     for (int i = 0; i < T / 64; ++i) s += part[i];
-    if (a.mean && a.scalars->rows > 0) s /= a.scalars->weight_sum;
+    if (a.mean && rows > 0) s /= a.scalars->weight_sum;
     a.total[0] = (float)s;
   }
 }
@@ -634,9 +605,10 @@ __global__ __launch_bounds__(NT) void xent_finish_kernel(XentArgs a, int64_t r0,
   }
 }
 
-__global__ __launch_bounds__(PLAN_NT) void xent_total_kernel(XentArgs a) {
-  __shared__ double part[PLAN_NT / 64];
-  sum_total<PLAN_NT>(a, part);
+constexpr int TOTAL_NT = 1024;
+__global__ __launch_bounds__(TOTAL_NT) void xent_total_kernel(XentArgs a) {
+  __shared__ double part[TOTAL_NT / 64];
+  sum_total<TOTAL_NT>(a, part);
 }
 
 }  // namespace
@@ -644,19 +616,21 @@ __global__ __launch_bounds__(PLAN_NT) void xent_total_kernel(XentArgs a) {
 void mxm_launch_xent(const XentArgs& a0, hipStream_t s) {
   XentArgs a = a0;
   a.w_direct = a.bf16 && a.D % 8 == 0 && (reinterpret_cast<uintptr_t>(a.weight) & 15) == 0;
-  const auto rows_grid = [&](int64_t n) { return (unsigned)std::min<int64_t>((n + 3) / 4, (int64_t)a.n_cu * 16); };
-  const bool plan = a.rows > 0 && a.rows <= PLAN_ROWS;
   // (one row's loss at D 2048 and 50257 entries, in the caches: 39.4 us with the
   // packing's launch, 36.4 without)
-  const bool gather = plan && !a.backward && a.w_direct && a.rows <= XENT_GATHER &&
+  const bool gather = a.rows > 0 && !a.backward && a.w_direct && a.rows <= XENT_GATHER &&
                       (reinterpret_cast<uintptr_t>(a.x) & 15) == 0;
-  if (!plan) xent_plan_kernel<<<1, PLAN_NT, 0, s>>>(a);
-  if (a.rows > 0 && !gather) {
-    const unsigned gx = rows_grid(a.rows), gw = a.w_direct ? 0 : rows_grid(a.V);
-    if (plan)
-      xent_pack_kernel<true><<<gx + gw, NT, 0, s>>>(a, (int)gx);
-    else
-      xent_pack_kernel<false><<<gx + gw, NT, 0, s>>>(a, (int)gx);
+  if (!gather) {
+    const auto waves = [&](int64_t n) { return std::min<int64_t>((n + 3) / 4, (int64_t)a.n_cu * 16); };
+    const int64_t chunk = ((a.rows + XENT_CHUNKS - 1) / XENT_CHUNKS + 3) / 4 * 4;
+    const int64_t gx = chunk ? (a.rows + chunk - 1) / chunk : 1, gw = a.w_direct || a.rows == 0 ? 0 : waves(a.V);
+    const auto pack = [&](auto kernel) { kernel<<<(unsigned)(gx + gw), NT, 0, s>>>(a, (int)gx, chunk); };
+    if (a.rows <= PLAN_ROWS) {
+      pack(xent_pack_kernel<true>);
+    } else {
+      xent_count_kernel<<<(unsigned)((gx + 3) / 4), NT, 0, s>>>(a, chunk, (int)gx);
+      pack(xent_pack_kernel<false>);
+    }
   }
   const int64_t pieces = std::max<int64_t>(1, (a.rows + a.piece_rows - 1) / a.piece_rows);
   const bool total_there = a.total && a.rows > 0 && a.rows <= JOIN_WAVES;  // (one piece)
@@ -693,5 +667,5 @@ void mxm_launch_xent(const XentArgs& a0, hipStream_t s) {
     }
     if (a.backward) mxm_launch_xent_grads(a, r0, rows, p == pieces - 1, a.scalars->low + parity, s);
   }
-  if (a.total && !total_there && !(a.backward && a.rows > 0)) xent_total_kernel<<<1, PLAN_NT, 0, s>>>(a);
+  if (a.total && !total_there && !(a.backward && a.rows > 0)) xent_total_kernel<<<1, TOTAL_NT, 0, s>>>(a);
 }
