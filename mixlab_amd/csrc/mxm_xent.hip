@@ -65,46 +65,58 @@ __device__ __forceinline__ void planes2x8(const float (&v)[8], u32x4_t (&q)[2]) 
     for (int i = 0; i < 4; ++i) q[k][i] = p[k][2 * i] | (uint32_t)p[k][2 * i + 1] << 16;
 }
 
+// The 8 elements at p, of which `left` are a row's, zeros behind them: vectors at the
+// elements' alignment, so that rows of any width and place are read alike (the losses of
+// 67 rows of D 1001 against 50257 entries 85 us with element loads, 65 so).
+__device__ __forceinline__ u32x4_t load8(const uint16_t* p, int left) {
+  typedef unsigned int at2_t __attribute__((ext_vector_type(4), aligned(2)));
+  if (left >= 8) return *reinterpret_cast<const at2_t*>(p);
+  u32x4_t q = {0, 0, 0, 0};
+#pragma unroll
+  for (int i = 0; i < 7; ++i)
+    if (i < left) q[i / 2] |= (uint32_t)p[i] << 16 * (i % 2);
+  return q;
+}
+__device__ __forceinline__ void load8(const float* p, int left, float (&v)[8]) {
+  typedef float at4_t __attribute__((ext_vector_type(4), aligned(4)));
+  if (left >= 8) {
+    const f32x4_t lo = *reinterpret_cast<const at4_t*>(p), hi = *reinterpret_cast<const at4_t*>(p + 4);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = lo[i], v[4 + i] = hi[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = i < left ? p[i] : 0.0f;
+  }
+}
+
 // Row `src` of x or weight to row `to` of its pack of `rows` rows, zeros behind D, by a
-// wave; wide: rows of whole aligned 16 bytes.
-__device__ __forceinline__ void pack_row(const XentArgs& a, const void* p, bool wide, int64_t src,
-                                         uint16_t* pack, int64_t to, int lane) {
+// wave.
+__device__ __forceinline__ void pack_row(const XentArgs& a, const void* p, int64_t src, uint16_t* pack, int64_t to,
+                                         int lane) {
   const uint16_t* from = static_cast<const uint16_t*>(p) + src * a.D;
   pack += to * a.Dp;
-  if (wide) {
-    for (int d = lane * 8; d < a.Dp; d += 512) {
-      u32x4_t q = {0, 0, 0, 0};
-      if (d < a.D) q = *reinterpret_cast<const u32x4_t*>(from + d);
-      *reinterpret_cast<u32x4_t*>(pack + d) = q;
-    }
-  } else {
-    for (int d = lane; d < a.Dp; d += 64) pack[d] = d < a.D ? from[d] : (uint16_t)0;
-  }
+  for (int d = lane * 8; d < a.Dp; d += 512) *reinterpret_cast<u32x4_t*>(pack + d) = load8(from + d, a.D - d);
 }
 
 // The same of an fp32 row, to planes; returns its exponent.
 template <bool WEIGHT>
-__device__ __forceinline__ int pack_row32(const XentArgs& a, const void* p, bool wide, int64_t src,
-                                          uint16_t* pack, int64_t rows, int64_t to, int lane) {
+__device__ __forceinline__ int pack_row32(const XentArgs& a, const void* p, int64_t src, uint16_t* pack, int64_t rows,
+                                          int64_t to, int lane) {
   const float* from = static_cast<const float*>(p) + src * a.D;
   const int64_t plane = rows * a.Dp;
   pack += to * a.Dp;
   // the largest finite element (of their bits, which are ordered alike), any infinity
   uint32_t top = 0;
   bool inf = false;
-  auto look = [&](float v) {
-    const uint32_t u = mxm_f2u(v) & 0x7fffffffu;
-    if (u < 0x7f800000u) top = max(top, u);
-    inf |= u == 0x7f800000u;
-  };
-  if (wide) {
-    for (int d = lane * 4; d < a.D; d += 256) {
-      const f32x4_t v = *reinterpret_cast<const f32x4_t*>(from + d);
+  for (int d = lane * 8; d < a.D; d += 512) {
+    float v[8];
+    load8(from + d, a.D - d, v);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) look(v[i]);
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t u = mxm_f2u(v[i]) & 0x7fffffffu;
+      if (u < 0x7f800000u) top = max(top, u);
+      inf |= u == 0x7f800000u;
     }
-  } else {
-    for (int d = lane; d < a.D; d += 64) look(from[d]);
   }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o));
@@ -118,29 +130,15 @@ __device__ __forceinline__ int pack_row32(const XentArgs& a, const void* p, bool
     if (!signs) return ldexpf(v, -e);
     return v != v ? v : __builtin_isinf(v) ? __builtin_copysignf(1.0f, v) : 0.0f;
   };
-  if (wide) {
-    for (int d = lane * 8; d < a.Dp; d += 512) {
-      float v[8];
+  for (int d = lane * 8; d < a.Dp; d += 512) {
+    float v[8];
+    load8(from + d, a.D - d, v);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = 0.0f;
-      if (d < a.D) {
-        const f32x4_t* f = reinterpret_cast<const f32x4_t*>(from + d);
-        const f32x4_t lo = f[0], hi = f[1];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = scaled(lo[i]), v[4 + i] = scaled(hi[i]);
-      }
-      u32x4_t q[2];
-      planes2x8(v, q);
-      *reinterpret_cast<u32x4_t*>(pack + d) = q[0];
-      *reinterpret_cast<u32x4_t*>(pack + plane + d) = q[1];
-    }
-  } else {
-    for (int d = lane; d < a.Dp; d += 64) {
-      uint16_t hi, lo;
-      planes2(d < a.D ? scaled(from[d]) : 0.0f, hi, lo);
-      pack[d] = hi;
-      pack[plane + d] = lo;
-    }
+    for (int i = 0; i < 8; ++i) v[i] = scaled(v[i]);
+    u32x4_t q[2];
+    planes2x8(v, q);
+    *reinterpret_cast<u32x4_t*>(pack + d) = q[0];
+    *reinterpret_cast<u32x4_t*>(pack + plane + d) = q[1];
   }
   return signs ? XENT_INF : e;
 }
@@ -149,10 +147,6 @@ __device__ __forceinline__ int wave_max(int v) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) v = max(v, __shfl_xor(v, o));
   return v;
-}
-
-__device__ __forceinline__ bool wide_rows(const XentArgs& a, const void* p) {
-  return a.D % 8 == 0 && (reinterpret_cast<uintptr_t>(p) & 15) == 0;
 }
 
 // x's rows that take part to their places, dx's others to zeros; a workgroup per chunk
@@ -169,18 +163,16 @@ __global__ __launch_bounds__(NT) void xent_pack_kernel(XentArgs a, int x_blocks,
   __shared__ double weight[4];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   if ((int)blockIdx.x >= x_blocks) {
-    const bool wide = wide_rows(a, a.weight);
     for (int64_t v = (int64_t)(blockIdx.x - x_blocks) * 4 + wave; v < a.V; v += (int64_t)(gridDim.x - x_blocks) * 4) {
       if (a.planes == 1) {
-        pack_row(a, a.weight, wide, v, a.w_pack, v, lane);
+        pack_row(a, a.weight, v, a.w_pack, v, lane);
       } else {
-        const int e = pack_row32<true>(a, a.weight, wide, v, a.w_pack, a.V, v, lane);
+        const int e = pack_row32<true>(a, a.weight, v, a.w_pack, a.V, v, lane);
         if (lane == 0) a.w_exp[v] = e;
       }
     }
     return;
   }
-  const bool wide = wide_rows(a, a.x);
   const int64_t from = blockIdx.x * chunk, end = min(from + chunk, a.rows);
   int before = 0, all = 0;
   double sum = 0.0;
@@ -239,9 +231,9 @@ __global__ __launch_bounds__(NT) void xent_pack_kernel(XentArgs a, int x_blocks,
     }
     if (to >= 0) {
       if (a.planes == 1) {
-        pack_row(a, a.x, wide, n, a.x_pack, to, lane);
+        pack_row(a, a.x, n, a.x_pack, to, lane);
       } else {
-        const int e = pack_row32<false>(a, a.x, wide, n, a.x_pack, a.x_rows, to, lane);
+        const int e = pack_row32<false>(a, a.x, n, a.x_pack, a.x_rows, to, lane);
         if (lane == 0) a.x_exp[to] = e;
       }
     } else if (a.dx) {
