@@ -8,72 +8,76 @@ namespace {
 
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 
-// U elements at p as fp32: 8 or 4 of rows of whole such units at aligned places, or 1.
-template <int U>
-__device__ __forceinline__ void load_unit(const void* p, bool bf16, int64_t at, float (&v)[U]) {
-  if constexpr (U == 1) {
-    v[0] = bf16 ? mxm_bf2f(static_cast<const uint16_t*>(p)[at]) : static_cast<const float*>(p)[at];
+// U elements of a row of fp32 or bf16 (ODD: at the elements' alignment, the row's last
+// unit of as many as are left).
+template <int N, bool ODD>
+struct Words {
+  typedef unsigned int type __attribute__((ext_vector_type(N)));
+};
+template <int N>
+struct Words<N, true> {
+  typedef unsigned int type __attribute__((ext_vector_type(N), aligned(2)));
+};
+template <bool ODD>
+struct Floats {
+  typedef float type __attribute__((ext_vector_type(4)));
+};
+template <>
+struct Floats<true> {
+  typedef float type __attribute__((ext_vector_type(4), aligned(4)));
+};
+// ONCE: read past the caches.
+template <int U, bool ODD, bool ONCE = false>
+__device__ __forceinline__ void load_unit(const void* p, bool bf16, int64_t at, int left, float (&v)[U]) {
+  if (ODD && left < U) {
+#pragma unroll
+    for (int i = 0; i < U; ++i)
+      v[i] = i >= left ? 0.0f
+             : bf16    ? mxm_bf2f(static_cast<const uint16_t*>(p)[at + i])
+                       : static_cast<const float*>(p)[at + i];
   } else if (bf16) {
-    typedef unsigned int words_t __attribute__((ext_vector_type(U / 2)));
-    const words_t q = *reinterpret_cast<const words_t*>(static_cast<const uint16_t*>(p) + at);
+    typedef typename Words<U / 2, ODD>::type words_t;
+    const words_t* from = reinterpret_cast<const words_t*>(static_cast<const uint16_t*>(p) + at);
+    const typename Words<U / 2, false>::type q = ONCE ? __builtin_nontemporal_load(from) : *from;
 #pragma unroll
     for (int i = 0; i < U / 2; ++i) {
       v[2 * i] = mxm_u2f(q[i] << 16);
       v[2 * i + 1] = mxm_u2f(q[i] & 0xffff0000u);
     }
   } else {
-    const f32x4_t* q = reinterpret_cast<const f32x4_t*>(static_cast<const float*>(p) + at);
+    typedef typename Floats<ODD>::type floats_t;
+    const floats_t* q = reinterpret_cast<const floats_t*>(static_cast<const float*>(p) + at);
 #pragma unroll
     for (int h = 0; h < U / 4; ++h) {
-      const f32x4_t a = q[h];
+      const f32x4_t a = ONCE ? __builtin_nontemporal_load(q + h) : q[h];
 #pragma unroll
       for (int i = 0; i < 4; ++i) v[4 * h + i] = a[i];
     }
   }
 }
-// (rows of gradients are read once)
-template <int U>
-__device__ __forceinline__ void load_once(const void* p, bool bf16, int64_t at, float (&v)[U]) {
-  if constexpr (U == 1) {
-    load_unit<U>(p, bf16, at, v);
-  } else if (bf16) {
-    typedef unsigned int words_t __attribute__((ext_vector_type(U / 2)));
-    const words_t q = __builtin_nontemporal_load(reinterpret_cast<const words_t*>(static_cast<const uint16_t*>(p) + at));
+template <int U, bool ODD>
+__device__ __forceinline__ void store_unit(void* p, bool bf16, int64_t at, int left, const float (&v)[U]) {
+  if (ODD && left < U) {
 #pragma unroll
-    for (int i = 0; i < U / 2; ++i) {
-      v[2 * i] = mxm_u2f(q[i] << 16);
-      v[2 * i + 1] = mxm_u2f(q[i] & 0xffff0000u);
+    for (int i = 0; i < U; ++i) {
+      if (i >= left) continue;
+      if (bf16)
+        static_cast<uint16_t*>(p)[at + i] = mxm_f2bf_fast(v[i]);
+      else
+        static_cast<float*>(p)[at + i] = v[i];
     }
-  } else {
-    const f32x4_t* q = reinterpret_cast<const f32x4_t*>(static_cast<const float*>(p) + at);
-#pragma unroll
-    for (int h = 0; h < U / 4; ++h) {
-      const f32x4_t a = __builtin_nontemporal_load(q + h);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v[4 * h + i] = a[i];
-    }
-  }
-}
-template <int U>
-__device__ __forceinline__ void store_unit(void* p, bool bf16, int64_t at, const float (&v)[U]) {
-  if constexpr (U == 1) {
-    if (bf16)
-      static_cast<uint16_t*>(p)[at] = mxm_f2bf_fast(v[0]);
-    else
-      static_cast<float*>(p)[at] = v[0];
   } else if (bf16) {
-    typedef unsigned int words_t __attribute__((ext_vector_type(U / 2)));
-    words_t q;
+    typename Words<U / 2, false>::type q;
 #pragma unroll
     for (int i = 0; i < U / 2; ++i) q[i] = mxm_pack_bf2_fast(v[2 * i], v[2 * i + 1]);
+    typedef typename Words<U / 2, ODD>::type words_t;
     __builtin_nontemporal_store(q, reinterpret_cast<words_t*>(static_cast<uint16_t*>(p) + at));
   } else {
-    f32x4_t* q = reinterpret_cast<f32x4_t*>(static_cast<float*>(p) + at);
+    typedef typename Floats<ODD>::type floats_t;
+    floats_t* q = reinterpret_cast<floats_t*>(static_cast<float*>(p) + at);
 #pragma unroll
     for (int h = 0; h < U / 4; ++h) {
-      f32x4_t a;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) a[i] = v[4 * h + i];
+      const f32x4_t a = {v[4 * h], v[4 * h + 1], v[4 * h + 2], v[4 * h + 3]};
       __builtin_nontemporal_store(a, q + h);
     }
   }
@@ -83,7 +87,7 @@ constexpr int NT = 256;
 
 // A row per T threads, ROWS of them in flight: their tokens, then their elements.
 constexpr int ROWS = 4;
-template <int U>
+template <int U, bool ODD>
 __global__ __launch_bounds__(NT) void embed_kernel(EmbedArgs a, int T) {
   const int per = NT / T, sub = threadIdx.x / T, t = threadIdx.x % T;
   const int64_t step = (int64_t)gridDim.x * per;
@@ -96,7 +100,7 @@ __global__ __launch_bounds__(NT) void embed_kernel(EmbedArgs a, int T) {
 #pragma unroll
       for (int k = 0; k < ROWS; ++k) {
         if (v[k] >= 0 && v[k] < a.V) {
-          load_unit<U>(a.table, a.table_bf16, (int64_t)v[k] * a.D + d, e[k]);
+          load_unit<U, ODD>(a.table, a.table_bf16, (int64_t)v[k] * a.D + d, a.D - d, e[k]);
 #pragma unroll
           for (int i = 0; i < U; ++i) e[k][i] *= a.scale;
         } else {
@@ -106,7 +110,7 @@ __global__ __launch_bounds__(NT) void embed_kernel(EmbedArgs a, int T) {
       }
 #pragma unroll
       for (int k = 0; k < ROWS; ++k)
-        if (n0 + k * step < a.rows) store_unit<U>(a.out, a.out_bf16, (n0 + k * step) * a.D + d, e[k]);
+        if (n0 + k * step < a.rows) store_unit<U, ODD>(a.out, a.out_bf16, (n0 + k * step) * a.D + d, a.D - d, e[k]);
     }
   }
 }
@@ -265,48 +269,47 @@ __global__ __launch_bounds__(64 * SORT_WAVES) void embed_sort_kernel(EmbedArgs a
   for (int b = threadIdx.x; b < own + (lo + own == a.V); b += blockDim.x) a.starts[lo + b] = lds.tot[b];
 }
 
+// Floats from one chunk's sum to the next: whole aligned units.
+__host__ __device__ inline int part_row(int D) { return (D + 7) / 8 * 8; }
+
 // The sorted places as the sums see them: place and token of one, where a token starts
 // and ends, and the chunks' sums.
 struct Runs {
   const EmbedArgs& a;
   __device__ __forceinline__ int2 at(int64_t p) const { return a.sorted[p]; }
   __device__ __forceinline__ int64_t start(int v) const { return a.starts[v]; }
-  __device__ __forceinline__ float* part(int64_t row) const { return a.part + row * a.D; }
+  __device__ __forceinline__ float* part(int64_t row) const { return a.part + row * part_row(a.D); }
 };
 
 // Sorted places [c * C, (c + 1) * C) per T threads: each run of one token that lies
 // within them to the table, the first and last run's sums to part where they go on
 // outside.
-template <int U>
+template <int U, bool ODD>
 __device__ __forceinline__ void put_row(const EmbedArgs& a, int v, int d, float (&s)[U]) {
 #pragma unroll
   for (int i = 0; i < U; ++i) s[i] *= a.scale;
   const int64_t at = (int64_t)v * a.D + d;
   if (a.accumulate) {
     float o[U];
-    load_unit<U>(a.d_table, a.dtable_bf16, at, o);
+    load_unit<U, ODD>(a.d_table, a.dtable_bf16, at, a.D - d, o);
 #pragma unroll
     for (int i = 0; i < U; ++i) s[i] += o[i];
   }
-  store_unit<U>(a.d_table, a.dtable_bf16, at, s);
+  store_unit<U, ODD>(a.d_table, a.dtable_bf16, at, a.D - d, s);
 }
 
 // (read again by the join: kept in the caches)
 template <int U>
 __device__ __forceinline__ void store_part(float* q, const float (&s)[U]) {
-  if constexpr (U == 1) {
-    q[0] = s[0];
-  } else {
 #pragma unroll
-    for (int h = 0; h < U / 4; ++h) {
-      const f32x4_t v = {s[4 * h], s[4 * h + 1], s[4 * h + 2], s[4 * h + 3]};
-      reinterpret_cast<f32x4_t*>(q)[h] = v;
-    }
+  for (int h = 0; h < U / 4; ++h) {
+    const f32x4_t v = {s[4 * h], s[4 * h + 1], s[4 * h + 2], s[4 * h + 3]};
+    reinterpret_cast<f32x4_t*>(q)[h] = v;
   }
 }
 
 constexpr int AHEAD = 8;  // rows in flight
-template <int U, class R>
+template <int U, bool ODD, class R>
 __device__ __forceinline__ void sum_chunk(const EmbedArgs& a, const R& runs, int T, int t, int C, int64_t c,
                                           int64_t all) {
   const int64_t from = c * C, to = min(from + C, all);
@@ -323,7 +326,7 @@ __device__ __forceinline__ void sum_chunk(const EmbedArgs& a, const R& runs, int
 #pragma unroll
       for (int k = 0; k < AHEAD; ++k) e[k] = runs.at(min(p0 + k, to - 1));
 #pragma unroll
-      for (int k = 0; k < AHEAD; ++k) load_once<U>(a.d_out, a.grad_bf16, (int64_t)e[k].x * a.D + d, g[k]);
+      for (int k = 0; k < AHEAD; ++k) load_unit<U, ODD, true>(a.d_out, a.grad_bf16, (int64_t)e[k].x * a.D + d, a.D - d, g[k]);
 #pragma unroll
       for (int k = 0; k < AHEAD; ++k) {
         if (p0 + k >= to) break;
@@ -331,7 +334,7 @@ __device__ __forceinline__ void sum_chunk(const EmbedArgs& a, const R& runs, int
           if (first && runs.start(v) < from) {
             store_part<U>(runs.part(c * 2) + d, s);
           } else {
-            put_row<U>(a, v, d, s);
+            put_row<U, ODD>(a, v, d, s);
           }
           first = false;
           v = e[k].y;
@@ -346,22 +349,22 @@ __device__ __forceinline__ void sum_chunk(const EmbedArgs& a, const R& runs, int
     if (before || after) {
       store_part<U>(runs.part(c * 2 + (before ? 0 : 1)) + d, s);
     } else {
-      put_row<U>(a, v, d, s);
+      put_row<U, ODD>(a, v, d, s);
     }
   }
 }
 
-template <int U>
+template <int U, bool ODD>
 __global__ __launch_bounds__(NT) void embed_sum_kernel(EmbedArgs a, int T, int C, int64_t chunks) {
   const int per = NT / T, sub = threadIdx.x / T, t = threadIdx.x % T;
   const int64_t all = a.starts[a.V];
   for (int64_t c = (int64_t)blockIdx.x * per + sub; c < chunks; c += (int64_t)gridDim.x * per)
-    sum_chunk<U>(a, Runs{a}, T, t, C, c, all);
+    sum_chunk<U, ODD>(a, Runs{a}, T, t, C, c, all);
 }
 
 // The run that starts in chunk c and goes on behind it: its sums in order.
 constexpr int JOIN_AHEAD = 16;
-template <int U, class R>
+template <int U, bool ODD, class R>
 __device__ __forceinline__ void join_chunk(const EmbedArgs& a, const R& runs, int T, int t, int C, int64_t c,
                                            int64_t all) {
   if ((c + 1) * C >= all) return;
@@ -371,12 +374,12 @@ __device__ __forceinline__ void join_chunk(const EmbedArgs& a, const R& runs, in
   const int64_t last = (to - 1) / C;
   for (int d = t * U; d < a.D; d += T * U) {
     float s[U];
-    load_unit<U>(runs.part(c * 2 + 1), false, d, s);
+    load_unit<U, false>(runs.part(c * 2 + 1), false, d, U, s);
     int64_t k = c + 1;
     for (; k + JOIN_AHEAD <= last + 1; k += JOIN_AHEAD) {
       float e[JOIN_AHEAD][U];
 #pragma unroll
-      for (int h = 0; h < JOIN_AHEAD; ++h) load_unit<U>(runs.part((k + h) * 2), false, d, e[h]);
+      for (int h = 0; h < JOIN_AHEAD; ++h) load_unit<U, false>(runs.part((k + h) * 2), false, d, U, e[h]);
 #pragma unroll
       for (int h = 0; h < JOIN_AHEAD; ++h)
 #pragma unroll
@@ -384,30 +387,30 @@ __device__ __forceinline__ void join_chunk(const EmbedArgs& a, const R& runs, in
     }
     for (; k <= last; ++k) {
       float e[U];
-      load_unit<U>(runs.part(k * 2), false, d, e);
+      load_unit<U, false>(runs.part(k * 2), false, d, U, e);
 #pragma unroll
       for (int i = 0; i < U; ++i) s[i] += e[i];
     }
-    put_row<U>(a, v, d, s);
+    put_row<U, ODD>(a, v, d, s);
   }
 }
 
 // The runs over several chunks, then zeros for the tokens that occur nowhere (behind the
 // runs, whose partials come one after the other: a launch of theirs took 15 us more).
-template <int U>
+template <int U, bool ODD>
 __global__ __launch_bounds__(NT) void embed_join_kernel(EmbedArgs a, int T, int C, int64_t joins, int64_t items) {
   const int per = NT / T, sub = threadIdx.x / T, t = threadIdx.x % T;
   const int64_t all = a.starts[a.V];
   for (int64_t i = (int64_t)blockIdx.x * per + sub; i < items; i += (int64_t)gridDim.x * per) {
     if (i < joins) {
-      join_chunk<U>(a, Runs{a}, T, t, C, i, all);
+      join_chunk<U, ODD>(a, Runs{a}, T, t, C, i, all);
     } else {
       const int64_t v = i - joins;
       if (a.starts[v] != a.starts[v + 1]) continue;
       float z[U];
 #pragma unroll
       for (int k = 0; k < U; ++k) z[k] = 0.0f;
-      for (int d = t * U; d < a.D; d += T * U) store_unit<U>(a.d_table, a.dtable_bf16, v * a.D + d, z);
+      for (int d = t * U; d < a.D; d += T * U) store_unit<U, ODD>(a.d_table, a.dtable_bf16, v * a.D + d, a.D - d, z);
     }
   }
 }
@@ -430,9 +433,9 @@ struct LocalRuns {
     return make_int2(list[p] & 0xffff, lo + (list[p] >> 16));
   }
   __device__ __forceinline__ int64_t start(int v) const { return tot[v - lo]; }
-  __device__ __forceinline__ float* part(int64_t row) const { return sums + row * a.D; }
+  __device__ __forceinline__ float* part(int64_t row) const { return sums + row * part_row(a.D); }
 };
-template <int U>
+template <int U, bool ODD>
 __global__ __launch_bounds__(NT) void embed_few_kernel(EmbedArgs a, int span, int T) {
   __shared__ SortLds<NT / 64> lds;
   __shared__ int list[SORT_FEW];
@@ -443,31 +446,31 @@ __global__ __launch_bounds__(NT) void embed_few_kernel(EmbedArgs a, int span, in
   const LocalRuns runs{a, list, lds.tot, sums, lo};
   const int all = lds.tot[own], chunks = (all + FEW_CHUNK - 1) / FEW_CHUNK;
   const int per = NT / T, sub = threadIdx.x / T, t = threadIdx.x % T;
-  for (int c = sub; c < chunks; c += per) sum_chunk<U>(a, runs, T, t, FEW_CHUNK, c, all);
+  for (int c = sub; c < chunks; c += per) sum_chunk<U, ODD>(a, runs, T, t, FEW_CHUNK, c, all);
   __syncthreads();
-  for (int c = sub; c < chunks - 1; c += per) join_chunk<U>(a, runs, T, t, FEW_CHUNK, c, all);
+  for (int c = sub; c < chunks - 1; c += per) join_chunk<U, ODD>(a, runs, T, t, FEW_CHUNK, c, all);
   if (a.accumulate) return;
   float z[U];
 #pragma unroll
   for (int k = 0; k < U; ++k) z[k] = 0.0f;
   for (int b = sub; b < own; b += per) {
     if (lds.tot[b] != lds.tot[b + 1]) continue;
-    for (int d = t * U; d < a.D; d += T * U) store_unit<U>(a.d_table, a.dtable_bf16, (int64_t)(lo + b) * a.D + d, z);
+    for (int d = t * U; d < a.D; d += T * U) store_unit<U, ODD>(a.d_table, a.dtable_bf16, (int64_t)(lo + b) * a.D + d, a.D - d, z);
   }
 }
 
 // Elements per thread and step: 8 where both tensors are bf16, 4 where fp32 is among
 // them (16 bytes of it, so that a wave's accesses lie side by side: two halves of 32 bytes
-// a lane took 221 us for a backward's sums of 65536 x 2048, against 197) or 8 do not
-// divide the rows or their places, 1 where 4 do not.
-int unit_of(int D, const void* p, bool p_bf16, const void* q, bool q_bf16) {
-  for (int u = p_bf16 && q_bf16 ? 8 : 4; u >= 4; u /= 2) {
-    const auto fits = [&](const void* at, bool bf16) {
-      return reinterpret_cast<uintptr_t>(at) % (u * (bf16 ? 2 : 4)) == 0;
-    };
-    if (D % u == 0 && fits(p, p_bf16) && fits(q, q_bf16)) return u;
-  }
-  return 1;
+// a lane took 221 us for a backward's sums of 65536 x 2048, against 197).
+int unit_of(bool p_bf16, bool q_bf16) { return p_bf16 && q_bf16 ? 8 : 4; }
+// Whether those do not divide the rows, or their places (an element a thread, such a
+// lookup of 65536 rows of D 1001 took 129 us, 67 in units at the elements' alignment; a
+// gradient of 20000 rows of D 1289 into 20000 tokens 103, 80).
+bool odd(int u, int D, const void* p, bool p_bf16, const void* q, bool q_bf16) {
+  const auto fits = [&](const void* at, bool bf16) {
+    return reinterpret_cast<uintptr_t>(at) % (u * (bf16 ? 2 : 4)) == 0;
+  };
+  return D % u != 0 || !fits(p, p_bf16) || !fits(q, q_bf16);
 }
 
 // Threads that walk one row of `units`: the least power of two that covers it, at
@@ -486,52 +489,53 @@ unsigned grid_of(int64_t items, int per, int n_cu) {
   return (unsigned)std::min<int64_t>((items + per - 1) / per, (int64_t)n_cu * 64);
 }
 
-template <int U>
+template <int U, bool ODD>
 void launch_bw(const EmbedArgs& a, int span, hipStream_t s) {
   const unsigned spans = (unsigned)((a.V + span - 1) / span);
   // (a chunk has two sums)
-  if (a.rows <= SORT_FEW && (a.rows + FEW_CHUNK - 1) / FEW_CHUNK * 2 * a.D <= FEW_SUMS &&
+  if (a.rows <= SORT_FEW && (a.rows + FEW_CHUNK - 1) / FEW_CHUNK * 2 * part_row(a.D) <= FEW_SUMS &&
       (a.accumulate || (int64_t)a.V * a.D <= FEW_ZEROS)) {
-    embed_few_kernel<U><<<spans, NT, 0, s>>>(a, span, threads_per_row(a.D / U));
+    embed_few_kernel<U, ODD><<<spans, NT, 0, s>>>(a, span, threads_per_row((a.D + U - 1) / U));
     return;
   }
   if (a.rows <= SORT_FEW)
     embed_sort_kernel<4><<<spans, 256, 0, s>>>(a, span);
   else
     embed_sort_kernel<16><<<spans, 1024, 0, s>>>(a, span);
-  const int T = threads_per_row(a.D / U), per = NT / T, C = chunk_rows(a.rows);
+  const int T = threads_per_row((a.D + U - 1) / U), per = NT / T, C = chunk_rows(a.rows);
   const int64_t chunks = (a.rows + C - 1) / C, joins = chunks > 1 ? chunks - 1 : 0;
   const int64_t items = joins + (a.accumulate ? 0 : a.V);
-  if (chunks > 0) embed_sum_kernel<U><<<grid_of(chunks, per, a.n_cu), NT, 0, s>>>(a, T, C, chunks);
-  if (items > 0) embed_join_kernel<U><<<grid_of(items, per, a.n_cu), NT, 0, s>>>(a, T, C, joins, items);
+  if (chunks > 0) embed_sum_kernel<U, ODD><<<grid_of(chunks, per, a.n_cu), NT, 0, s>>>(a, T, C, chunks);
+  if (items > 0) embed_join_kernel<U, ODD><<<grid_of(items, per, a.n_cu), NT, 0, s>>>(a, T, C, joins, items);
 }
 
 }  // namespace
 
-int64_t mxm_embed_max_chunks(int64_t max_rows) {
-  return std::max((std::min(max_rows, LONG_BATCH - 1) + 7) / 8, (max_rows + 31) / 32);
+int64_t mxm_embed_part_floats(int64_t max_rows, int D) {
+  return std::max((std::min(max_rows, LONG_BATCH - 1) + 7) / 8, (max_rows + 31) / 32) * 2 * part_row(D);
 }
 
 void mxm_launch_embed(const EmbedArgs& a, hipStream_t s) {
   if (a.rows == 0) return;
-  const int U = unit_of(a.D, a.table, a.table_bf16, a.out, a.out_bf16);
-  const int T = threads_per_row(a.D / U);
+  const int U = unit_of(a.table_bf16, a.out_bf16);
+  const int T = threads_per_row((a.D + U - 1) / U);
   const unsigned grid = grid_of(a.rows, NT / T, a.n_cu);
-  if (U == 8)
-    embed_kernel<8><<<grid, NT, 0, s>>>(a, T);
-  else if (U == 4)
-    embed_kernel<4><<<grid, NT, 0, s>>>(a, T);
+  const auto launch = [&](auto kernel) { kernel<<<grid, NT, 0, s>>>(a, T); };
+  if (odd(U, a.D, a.table, a.table_bf16, a.out, a.out_bf16))
+    U == 8 ? launch(embed_kernel<8, true>) : launch(embed_kernel<4, true>);
   else
-    embed_kernel<1><<<grid, NT, 0, s>>>(a, T);
+    U == 8 ? launch(embed_kernel<8, false>) : launch(embed_kernel<4, false>);
 }
 
 void mxm_launch_embed_bw(const EmbedArgs& a, hipStream_t s) {
   const int span = std::min(SORT_SPAN, (a.V + a.n_cu - 1) / a.n_cu);
-  const int U = unit_of(a.D, a.d_out, a.grad_bf16, a.d_table, a.dtable_bf16);
-  if (U == 8)
-    launch_bw<8>(a, span, s);
-  else if (U == 4)
-    launch_bw<4>(a, span, s);
+  // (bf16 rows of D 100, 5000 into 2000 tokens: 19.7 us in whole units of 4, 26.0 in 8 and
+  // a part)
+  const auto uneven = [&](int u) { return odd(u, a.D, a.d_out, a.grad_bf16, a.d_table, a.dtable_bf16); };
+  if (unit_of(a.grad_bf16, a.dtable_bf16) == 8 && !uneven(8))
+    launch_bw<8, false>(a, span, s);
+  else if (!uneven(4))
+    launch_bw<4, false>(a, span, s);
   else
-    launch_bw<1>(a, span, s);
+    launch_bw<4, true>(a, span, s);
 }

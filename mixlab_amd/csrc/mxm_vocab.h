@@ -28,14 +28,14 @@ struct EmbedArgs {
   // backward's workspace
   int2* sorted;           // [rows]: place, token
   int32_t* starts;        // [V + 1]: first sorted place of token v
-  float* part;            // [chunks][2][D]: sums of runs that a chunk shares
+  float* part;            // [chunks][2][D up to 8]: sums of runs that a chunk shares
   int64_t max_rows;
   int n_cu;
 };
 void mxm_launch_embed(const EmbedArgs& a, hipStream_t s);
 void mxm_launch_embed_bw(const EmbedArgs& a, hipStream_t s);
-// Most chunks of a backward of up to max_rows rows (part's first extent).
-int64_t mxm_embed_max_chunks(int64_t max_rows);
+// Floats of part, for a backward of up to max_rows rows.
+int64_t mxm_embed_part_floats(int64_t max_rows, int D);
 
 // ---- token loss ----
 //

@@ -168,7 +168,7 @@ int64_t mxm_embed_create(const int64_t* params, int n_params, float scale, int64
     if (e->backward) {
       e->sorted.alloc((size_t)rows * sizeof(int2));
       e->starts.alloc(((size_t)V + 1) * 4);
-      e->part.alloc((size_t)mxm_embed_max_chunks(rows) * 2 * (size_t)D * 4);
+      e->part.alloc((size_t)mxm_embed_part_floats(rows, (int)D) * 4);
       a.sorted = e->sorted.as<int2>();
       a.starts = e->starts.as<int32_t>();
       a.part = e->part.as<float>();
