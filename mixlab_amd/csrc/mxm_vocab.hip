@@ -293,7 +293,7 @@ int64_t mxm_xent_create(const int64_t* params, int n_params, float softcap, int6
       a.x_exp = a.w_exp + v_tiles;
       a.e_row = a.x_exp + n;
       if (x->backward) {
-        x->parts.alloc((n / 16 + 1) * sizeof(int4));
+        x->parts.alloc((n / 4 + 1) * sizeof(int4));  // (4 rows a workgroup at least)
         x->stat_exp.alloc((size_t)mxm_xent_stats(a.piece_rows, a.V, a.n_cu) * 4);
         a.c_part = x->parts.as<int4>();
         a.stat_exp = x->stat_exp.as<int32_t>();

@@ -369,24 +369,35 @@ __device__ __forceinline__ float finish_row(const XentArgs& a, int64_t r0, int m
   return loss;
 }
 
-// Few rows: a wave each.  With one workgroup for all of them it also sums the total.
-constexpr int JOIN_WAVES = 16, JOIN_FEW = 512;
+// Few rows: WAVES waves each (1, or 4 for sums of many blocks: 21 rows' of 1713 blocks took
+// 16.7 us with one, 12 so).  With one workgroup for all of them it also sums the total.
+constexpr int JOIN_WAVES = 16, JOIN_FEW = 512, LONG_JOIN = 512;
+template <int WAVES>
 __global__ __launch_bounds__(64 * JOIN_WAVES) void xent_join_few_kernel(XentArgs a, int64_t r0, int blocks,
                                                                         bool total) {
   __shared__ double part[JOIN_WAVES];
   __shared__ Exps each[JOIN_WAVES];
+  __shared__ Sum sums[JOIN_WAVES];
   const int rows = mxm_xent_rows(a, r0), lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int m = blockIdx.x * JOIN_WAVES + wave;
+  const int m = blockIdx.x * (JOIN_WAVES / WAVES) + wave / WAVES;
   Exps exps = NO_EXPS;
   double sum = 0.0;
+  Sum s = {-__builtin_inff(), 0.0f, XENT_NO_EXP};
   if (m < rows) {
-    Sum s = blocks_of(a, m, lane, 64, blocks);
+    s = blocks_of(a, m, wave % WAVES * 64 + lane, 64 * WAVES, blocks);
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) s = join(s, of_lane(s, o));
-    if (lane == 0) {
-      const float loss = finish_row(a, r0, m, s, exps);
-      sum = (double)loss * (a.row_weights ? (double)a.row_weights[a.map[r0 + m]] : 1.0);
-    }
+  }
+  if constexpr (WAVES > 1) {
+    if (lane == 0) sums[wave] = s;
+    __syncthreads();
+#pragma unroll
+    for (int i = 1; i < WAVES; ++i)
+      if (wave % WAVES == 0) s = join(s, sums[wave + i]);
+  }
+  if (m < rows && wave % WAVES == 0 && lane == 0) {
+    const float loss = finish_row(a, r0, m, s, exps);
+    sum = (double)loss * (a.row_weights ? (double)a.row_weights[a.map[r0 + m]] : 1.0);
   }
   if (a.backward && a.planes != 1) {
     if (lane == 0) each[wave] = exps;
@@ -495,15 +506,16 @@ __global__ __launch_bounds__(NT) void xent_finish_kernel(XentArgs a, int64_t r0,
     }
     if (a.dx) {
       const int lane = threadIdx.x & 63;
-      // (four rows a wave: where many need it, in a small table, all waves work)
-      for (int v0 = (id * (NT / 64) + (threadIdx.x >> 6)) * 4; v0 < a.V; v0 += gridDim.x * gridDim.y * (NT / 16)) {
-        const int v = v0 + (lane & 3), w = v < a.V ? a.w_exp[v] : XENT_ZERO;
+      // (neighbours go to different waves: where many need it, in a small table, all work)
+      const int waves = gridDim.x * gridDim.y * (NT / 64);
+      for (int v0 = id * (NT / 64) + (threadIdx.x >> 6); v0 < a.V; v0 += 64 * waves) {
+        const int v = v0 + lane * waves, w = v < a.V ? a.w_exp[v] : XENT_ZERO;
         const int now = max(w, before);
-        unsigned todo = (unsigned)__ballot(w != XENT_ZERO && now < low) & 15u;
+        unsigned long long todo = __ballot(w != XENT_ZERO && now < low);
         while (todo != 0) {
-          const int at = __ffs(todo) - 1;
+          const int at = __ffsll(todo) - 1;
           todo &= todo - 1;
-          const int64_t row = v0 + at;
+          const int64_t row = v0 + at * waves;
           const int by = __shfl(now, at) - low;
           for (int u = lane; u < 2 * (a.Dp / 8); u += 64) {
             const int pl = u >= a.Dp / 8;
@@ -625,7 +637,7 @@ void mxm_launch_xent(const XentArgs& a0, hipStream_t s) {
     }
   }
   const int64_t pieces = std::max<int64_t>(1, (a.rows + a.piece_rows - 1) / a.piece_rows);
-  const bool total_there = a.total && a.rows > 0 && a.rows <= JOIN_WAVES;  // (one piece)
+  bool total_there = false;  // one workgroup joins all rows and sums their total
   for (int64_t p = 0; p < pieces; ++p) {
     const int64_t r0 = p * a.piece_rows, rows = std::min(a.rows - r0, a.piece_rows);
     const int parity = (int)(p & 1);
@@ -636,8 +648,17 @@ void mxm_launch_xent(const XentArgs& a0, hipStream_t s) {
                              gather, s);
       const int blocks = (a.V + block - 1) / block;
       if (rows <= JOIN_FEW) {
-        a.c_parts = (int)((rows + JOIN_WAVES - 1) / JOIN_WAVES);
-        xent_join_few_kernel<<<a.c_parts, 64 * JOIN_WAVES, 0, s>>>(a, r0, blocks, total_there);
+        // (5 to 16 rows' losses with their total: one workgroup, without the total's launch,
+        // 12.7 us of 10 rows of D 192 and 58527 entries, 14.9 with four waves a row)
+        const bool long_joins = blocks > LONG_JOIN && (a.backward || !a.total || a.rows <= JOIN_WAVES / 4 ||
+                                                       a.rows > JOIN_WAVES);
+        const int each = long_joins ? JOIN_WAVES / 4 : JOIN_WAVES;
+        a.c_parts = (int)((rows + each - 1) / each);
+        total_there = a.total && a.rows <= each;
+        const auto launch = [&](auto kernel) {
+          kernel<<<a.c_parts, 64 * JOIN_WAVES, 0, s>>>(a, r0, blocks, total_there);
+        };
+        long_joins ? launch(xent_join_few_kernel<4>) : launch(xent_join_few_kernel<1>);
       } else {
         a.c_parts = (int)((rows + JOIN_ROWS - 1) / JOIN_ROWS);
         xent_join_kernel<<<a.c_parts, NT, 0, s>>>(a, r0, blocks);

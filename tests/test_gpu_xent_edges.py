@@ -141,6 +141,7 @@ def test_pieces_of_unlike_magnitude(gpu_lib, dx, dw, monkeypatch):
 @pytest.mark.parametrize("N,D,V,pad,weighted,shift", [
     (1, 2048, 3000, 0.0, False, 0), (1, 64, 500, 1.0, False, 0), (2, 72, 40000, 0.0, True, 0),
     (17, 136, 700, 0.4, True, 0), (32, 8, 130, 0.3, False, 0), (32, 520, 1000, 0.0, False, 8),
+    (4, 40, 33000, 0.0, False, 0), (5, 40, 33001, 0.2, False, 0), (16, 24, 40000, 0.0, True, 0),
     (31, 100, 400, 0.2, True, 0), (33, 136, 700, 0.4, True, 0), (20, 64, 128, 0.5, False, 1)])
 def test_few_rows(gpu_lib, N, D, V, pad, weighted, shift, dtype):
     """Up to the few rows that a forward reads in place, in and out of order, and past them."""
