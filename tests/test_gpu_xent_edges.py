@@ -177,7 +177,7 @@ def test_elements_of_unlike_magnitude(gpu_lib, dtype):
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "fp32"])
-@pytest.mark.parametrize("d_total", [-3.0, 65536.0, 2.0 ** -40, 2.0 ** 60])
+@pytest.mark.parametrize("d_total", [0.0, -3.0, 65536.0, 2.0 ** -40, 2.0 ** 60])
 def test_scales_of_the_gradient(gpu_lib, dtype, d_total):
     rng = np.random.default_rng(5)
     x, w, t = inputs(120, 64, 200, dtype, 24, pad=0.2)
