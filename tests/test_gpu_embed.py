@@ -23,6 +23,11 @@ def tokens_of(kind, rng, N, V):
         t = np.where(rng.random(N) < 0.5, -1, V + rng.integers(0, 3, N))
     elif kind == "extremes":
         t = rng.choice(np.array([-2 ** 31, -1, 0, V - 1, V, 2 ** 31 - 1]), N)
+    elif kind == "half":         # every other place or so of one token
+        t = np.where(rng.random(N) < 0.5, V // 3, rng.integers(0, V, N))
+    elif kind == "blocks":       # tokens that occur 64, 128 or 256 times, or one less or more
+        n = rng.choice(np.array([1, 63, 64, 65, 127, 128, 129, 256, 257]), N)
+        t = rng.permutation(np.repeat(np.arange(N), n)[:N] % V)
     else:                        # skewed, some of them padding
         t = np.minimum((V ** rng.random(N)).astype(np.int64) - 1, V - 1)
         t[rng.random(N) < 0.2] = -1
@@ -83,6 +88,13 @@ def test_forward(gpu_lib, N, D, V, table, out, shift, kind):
     (70, 16384, 9, "bf16", "fp32", 0, "skewed", True),
     (50, 16383, 7, "fp32", "bf16", 0, "extremes", False),
     (40000, 8, 700000, "fp32", "fp32", 0, "skewed", True),
+    (5000, 72, 40, "fp32", "fp32", 0, "half", False),
+    (20000, 260, 3000, "bf16", "fp32", 0, "half", True),
+    (50000, 40, 2000, "fp32", "bf16", 0, "half", False),
+    (9000, 24, 5000, "fp32", "fp32", 0, "blocks", False),
+    (36000, 24, 5000, "bf16", "bf16", 0, "blocks", True),
+    (1900, 32, 300, "fp32", "fp32", 0, "blocks", False),
+    (2000, 32, 200, "fp32", "fp32", 0, "half", True),
     (700, 72, 90, "bf16", "bf16", 4, "skewed", False),
     (700, 72, 90, "bf16", "fp32", 2, "skewed", False),
 ])
