@@ -85,6 +85,7 @@ constexpr int XENT_INF = 1 << 20;
 constexpr int XENT_ZERO = -(1 << 18);
 constexpr int XENT_SLACK = 4;
 constexpr int XENT_NO_EXP = -(1 << 20);  // of nothing
+constexpr float XENT_NO_REF = -3.4028235e38f;  // ref of a block without an entry: the least
 struct XentRow {            // of a row that takes part
   float ref;                // M: the summands' common exponent
   float scale;              // g / sum of all 2^(l log2 e - M)

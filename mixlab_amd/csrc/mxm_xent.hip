@@ -328,12 +328,14 @@ __device__ __forceinline__ float finish_row(const XentArgs& a, int64_t r0, int m
     lt = a.softcap * th;
     slope = fmaf(-th, th, 1.0f);
   }
-  const float d = fmaf(-lt, LOG2E, top);
+  // (no other entry comes: d is whatever makes the target's share one)
+  const bool alone = sum == 0.0f;
+  const float d = alone ? -200.0f : fmaf(-lt, LOG2E, top);
   const float et = __builtin_amdgcn_exp2f(-d), whole = sum + et;
   // (next to the target's probability of one the loss keeps its digits)
   const bool near = d <= 60.0f;
   const float over = logf(whole);
-  const float loss = near ? log1pf(sum * __builtin_amdgcn_exp2f(d)) : d * LN2 + over;
+  const float loss = alone ? lt - lt : near ? log1pf(sum * __builtin_amdgcn_exp2f(d)) : d * LN2 + over;
   const int64_t n = a.map[r0 + m];
   a.nll[r0 + m] = loss;
   if (a.loss) a.loss[n] = loss;

@@ -626,20 +626,39 @@ __global__ __launch_bounds__(TL::NT, F16 && TL::NS == 4 ? 1 : TL::WPS) void xent
       // 2^(l log2 e - ref) lies in (0, 2^15]: fp16 keeps 12 bits of summands down to
       // 2^-29 of the block's largest and 2^-39 of it at all
       const bool any = CAP ? top >= -2.0f : top > -__builtin_inff();
-      const float ref = any ? ceilf(CAP ? cap2 * top : top * LOG2E) - 15.0f : 0.0f;
+      const float t = CAP ? cap2 * top : top * LOG2E;
+      float ref = any ? ceilf(t) - 15.0f : 0.0f, sub = ref;
+      if constexpr (!CAP) {
+        // From 2^22 on ref and the exact product may lie further apart than a summand's
+        // range allows (a block of masked entries, say): such logits are taken less their
+        // largest first, whose summand is 2^15.  Their ref is finite, and above that of no
+        // entry at all.
+        const bool far = any && !(__builtin_fabsf(t) < 4194304.0f);
+        if (__ballot(far) != 0) {
+          const float by = far ? top : 0.0f;
+#pragma unroll
+          for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[i][j][r] -= by;
+          if (far) {
+            sub = -15.0f;
+            ref = fminf(fmaxf(t - 15.0f, 0.5f * XENT_NO_REF), -XENT_NO_REF);
+          }
+        }
+      }
       float s[2] = {0.0f, 0.0f};
 #pragma unroll
       for (int i = 0; i < TM; ++i)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          const float v = acc[i][j][r], e = __builtin_amdgcn_exp2f(fmaf(v, CAP ? cap2 : LOG2E, -ref));
+          const float v = acc[i][j][r], e = __builtin_amdgcn_exp2f(fmaf(v, CAP ? cap2 : LOG2E, -sub));
           s[r & 1] += e;
           acc[i][j][r] = CAP ? e * fmaf(-v, v, 1.0f) : e;
         }
       float sum = s[0] + s[1];
       sum += mxm_xor_lane_f(sum, 32);
       const int64_t at_stat = (int64_t)(mw / (TM * 32)) * a.stat_ld + n;
-      if (n < rows && mw < a.V && lane < 32) a.stat[at_stat] = make_float2(sum, any ? ref : -1.0e30f);
+      if (n < rows && mw < a.V && lane < 32) a.stat[at_stat] = make_float2(sum, any ? ref : XENT_NO_REF);
       if constexpr (F16 && STORE) {
         // (2^(w - 1): none overflows)
         float big = 0.0f;
