@@ -444,7 +444,8 @@ int mxm_embed_backward(int64_t h, int64_t rows, const int32_t* tokens, const voi
  * weight.  Under bf16 the products are exact and summed in fp32, and the backward
  * rounds the logits' gradient to bf16 before the products with it.  Under fp32 a
  * row's elements keep 22 bits down to 2^-17 of its largest and 2^-40 of it below,
- * and so does a row's gradient of the logits.  An entry (row of weight) that minus
+ * and so does a row's gradient of the logits (under a softcap, of what it is before
+ * the cap's slope).  An entry (row of weight) that minus
  * infinity or the type's lowest value keeps from coming has no share in any result
  * (but that dx of a bf16 table with infinities is not a number, 0 times those);
  * as a target it makes the loss infinite (or as large), and then dx and dw are of no

@@ -70,8 +70,9 @@ int64_t mxm_embed_part_floats(int64_t max_rows, int D);
 // Then, for a piece of the rows that take part at a time:
 //   product 1 (mxm_xent_gemm.hip): logits of a tile of vocabulary x rows in the
 //     accumulators; of each row and block of the vocabulary the sum over v != t of
-//     2^(l log2 e - ref) with a whole-number ref of the block; backwards also each
-//     summand (times 1 - (l / cap)^2), relative to that ref;
+//     2^(l log2 e - ref) with a ref of the block (a whole number, or next to one);
+//     backwards also each summand (under a softcap times a quarter of 1 - (l / cap)^2),
+//     relative to that ref;
 //   join (mxm_xent.hip): each row's loss and the factors of its gradient;
 //   finish: the summands to dz, in place (fp32: to planes; x' to x'');
 //   product 2: dx = dz W;  product 3: dW (+)= dz^T x.
@@ -88,7 +89,7 @@ constexpr int XENT_NO_EXP = -(1 << 20);  // of nothing
 constexpr float XENT_NO_REF = -3.4028235e38f;  // ref of a block without an entry: the least
 struct XentRow {            // of a row that takes part
   float ref;                // M: the summands' common exponent
-  float scale;              // g / sum of all 2^(l log2 e - M)
+  float scale;              // g / sum of all 2^(l log2 e - M), times 4 under a softcap
   float at_target;          // dz of the target
   int32_t target;
   // fp32: |dz| 2^w < 2^(e + 15) and |dz| < 2^(g + 15), XENT_NO_EXP for a row without a
@@ -176,3 +177,8 @@ __device__ __forceinline__ int mxm_xent_rows(const XentArgs& a, int64_t r0) {
 __device__ __forceinline__ float mxm_xent_capped(float z, float k2) {
   return fmaf(-2.0f, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * k2)), 1.0f);
 }
+
+// The slope 1 - tanh^2, as 4 times this, from e = exp(2 z / cap) and r = 1 / (1 + e), tanh =
+// 1 - 2 r: it keeps its digits where tanh is next to 1 or -1 (taken from tanh it is off by
+// 6e-5 at z = 4 cap, by 8e-3 at 7, and zero from 9 on).  e r is 1 where e is infinite.
+__device__ __forceinline__ float mxm_xent_cap_slope(float e, float r) { return r * fminf(e * r, 1.0f); }

@@ -324,9 +324,9 @@ __device__ __forceinline__ float finish_row(const XentArgs& a, int64_t r0, int m
   const float top = others.top, sum = others.sum;
   float lt = a.at_target[r0 + m], slope = 1.0f;
   if (a.softcap > 0.0f) {
-    const float th = mxm_xent_capped(lt, 2.0f * LOG2E / a.softcap);
-    lt = a.softcap * th;
-    slope = fmaf(-th, th, 1.0f);
+    const float e = __builtin_amdgcn_exp2f(lt * (2.0f * LOG2E / a.softcap)), r = __builtin_amdgcn_rcpf(1.0f + e);
+    lt = a.softcap * fmaf(-2.0f, r, 1.0f);
+    slope = 4.0f * mxm_xent_cap_slope(e, r);
   }
   // (no other entry comes: d is whatever makes the target's share one)
   const bool alone = sum == 0.0f;
@@ -345,7 +345,7 @@ __device__ __forceinline__ float finish_row(const XentArgs& a, int64_t r0, int m
     const float g = (float)((double)a.d_total * w / (a.mean ? a.scalars->weight_sum : 1.0));
     XentRow r;
     r.ref = top;
-    r.scale = g / whole;
+    r.scale = (a.softcap > 0.0f ? 4.0f * g : g) / whole;
     r.at_target = -g * (sum / whole) * slope;
     r.target = a.target[r0 + m];
     r.e = r.g = XENT_NO_EXP;

@@ -442,7 +442,7 @@ struct LogitsArgs {
   const XentScalars* scalars;
   int64_t r0, piece_rows;  // the piece; arrays of rows start at its first row
   int V, Vp;
-  float softcap;
+  float k2, cap2;          // 2 log2 e / softcap, softcap log2 e
   const int32_t *target, *x_exp, *w_exp;
   float* at_target;
   const int32_t* low;      // L that the table's planes were taken down to, or null
@@ -527,7 +527,7 @@ __global__ __launch_bounds__(TL::NT, F16 && TL::NS == 4 ? 1 : TL::WPS) void xent
   const int mt = (a.V + TL::BM - 1) / TL::BM, nt = (rows + TL::BN - 1) / TL::BN;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int wm = wave / TL::WN, wn = wave % TL::WN;
-  const float k2 = 2.0f * LOG2E / a.softcap, cap2 = a.softcap * LOG2E;  // (CAP)
+  const float k2 = a.k2, cap2 = a.cap2;  // (CAP)
   const Items items(mt * nt);
   for (int item = items.first; item < items.end; item += items.step) {
     int tm, tn;
@@ -566,9 +566,12 @@ __global__ __launch_bounds__(TL::NT, F16 && TL::NS == 4 ? 1 : TL::WPS) void xent
           }
       }
       // entries behind the vocabulary, and the target (whose logit is kept apart), get one
-      // with an exponential of 0 (under a softcap a tanh, so small that no ref brings it
-      // back and no slope times 0 leaves 0: a logit of minus infinity is its lowest there)
-      const float none = CAP ? -(200.0f / cap2 + 4.0f) : -__builtin_inff();
+      // with an exponential of 0.  Under a softcap that is a tanh so small that no ref brings
+      // it back and no slope times 0 leaves 0 (a logit of minus infinity is its lowest
+      // there: at the least cap, 1/64, this one is 2^-225), or where the summands are kept
+      // too, with their slope, the exp(2 z / cap) of about such a tanh: below zero.
+      constexpr bool SLOPE = CAP && STORE;
+      constexpr float none = SLOPE ? -0.9998f : CAP ? -1.0e4f : -__builtin_inff();
       const bool here = __ballot(target >= mw && target < mw + TM * 32) != 0;
       const int at = target - first;
       if (here) {
@@ -597,7 +600,8 @@ __global__ __launch_bounds__(TL::NT, F16 && TL::NS == 4 ? 1 : TL::WPS) void xent
 #pragma unroll
         for (int i = 0; i < TM; ++i)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) acc[i][j][r] = mxm_xent_capped(acc[i][j][r], k2);
+          for (int r = 0; r < 16; ++r)
+            acc[i][j][r] = SLOPE ? __builtin_amdgcn_exp2f(acc[i][j][r] * k2) : mxm_xent_capped(acc[i][j][r], k2);
         if (here) {
           int again = at;
           asm volatile("" : "+v"(again));  // (else the comparisons above are kept, in 128 scalar registers)
@@ -623,11 +627,20 @@ __global__ __launch_bounds__(TL::NT, F16 && TL::NS == 4 ? 1 : TL::WPS) void xent
 #pragma unroll
         for (int r = 0; r < 16; ++r) top = fmaxf(top, acc[i][j][r]);
       top = fmaxf(top, mxm_xor_lane_f(top, 32));
-      // 2^(l log2 e - ref) lies in (0, 2^15]: fp16 keeps 12 bits of summands down to
-      // 2^-29 of the block's largest and 2^-39 of it at all
-      const bool any = CAP ? top >= -2.0f : top > -__builtin_inff();
-      const float t = CAP ? cap2 * top : top * LOG2E;
-      float ref = any ? ceilf(t) - 15.0f : 0.0f, sub = ref;
+      const bool any = SLOPE ? top >= 0.0f : CAP ? top >= -2.0f : top > -__builtin_inff();
+      // 2^(l log2 e - ref) lies in (0, 2^15], or 2^17 where a quarter of the slope comes to
+      // it: fp16 keeps 12 bits of summands down to 2^-29 of the block's largest and 2^-39 of
+      // it at all
+      constexpr float UP = SLOPE ? 17.0f : 15.0f;
+      const float t = SLOPE ? fmaf(-2.0f * cap2, __builtin_amdgcn_rcpf(1.0f + top), cap2)
+                      : CAP ? cap2 * top
+                            : top * LOG2E;
+      float ref = any ? ceilf(t) - UP : 0.0f, sub = ref;
+      if constexpr (SLOPE) {
+        // l log2 e - ref = (cap2 - ref) - 2 cap2 r: ref is what the rounded difference makes it
+        sub = cap2 - ref;
+        ref = cap2 - sub;
+      }
       if constexpr (!CAP) {
         // From 2^22 on ref and the exact product may lie further apart than a summand's
         // range allows (a block of masked entries, say): such logits are taken less their
@@ -641,8 +654,8 @@ __global__ __launch_bounds__(TL::NT, F16 && TL::NS == 4 ? 1 : TL::WPS) void xent
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[i][j][r] -= by;
           if (far) {
-            sub = -15.0f;
-            ref = fminf(fmaxf(t - 15.0f, 0.5f * XENT_NO_REF), -XENT_NO_REF);
+            sub = -UP;
+            ref = fminf(fmaxf(t - UP, 0.5f * XENT_NO_REF), -XENT_NO_REF);
           }
         }
       }
@@ -651,9 +664,19 @@ __global__ __launch_bounds__(TL::NT, F16 && TL::NS == 4 ? 1 : TL::WPS) void xent
       for (int i = 0; i < TM; ++i)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          const float v = acc[i][j][r], e = __builtin_amdgcn_exp2f(fmaf(v, CAP ? cap2 : LOG2E, -sub));
-          s[r & 1] += e;
-          acc[i][j][r] = CAP ? e * fmaf(-v, v, 1.0f) : e;
+          const float v = acc[i][j][r];
+          if constexpr (SLOPE) {
+            const float w = __builtin_amdgcn_rcpf(1.0f + v), e = __builtin_amdgcn_exp2f(fmaf(-2.0f * cap2, w, sub));
+            s[r & 1] += e;
+            acc[i][j][r] = e * mxm_xent_cap_slope(v, w);
+            // (else the product moves to where the summands are stored, and its factors of
+            // all logits till there spill 300 registers)
+            asm("" : "+v"(acc[i][j][r]));
+          } else {
+            const float e = __builtin_amdgcn_exp2f(fmaf(v, CAP ? cap2 : LOG2E, -sub));
+            s[r & 1] += e;
+            acc[i][j][r] = e;
+          }
         }
       float sum = s[0] + s[1];
       sum += mxm_xor_lane_f(sum, 32);
@@ -988,7 +1011,7 @@ template <class TL>
 void launch_logits(const XentArgs& a, const Product& p, int64_t r0, int64_t rows, const int32_t* low, int per_cu,
                    bool gather, hipStream_t s) {
   const unsigned grid = grid_of(tiles_of(a.V, rows, TL::BM, TL::BN), (int64_t)a.n_cu * per_cu);
-  const LogitsArgs l{a.scalars, r0, a.piece_rows, a.V, a.Vp, a.softcap, a.target + r0,
+  const LogitsArgs l{a.scalars, r0, a.piece_rows, a.V, a.Vp, 2.0f * LOG2E / a.softcap, a.softcap * LOG2E, a.target + r0,
                      a.x_exp ? a.x_exp + r0 : nullptr, a.w_exp, a.at_target + r0, low, a.stat, a.stat_exp,
                      a.stat_ld, a.summands};
   const GatherArgs g{a.targets, a.row_weights, (int)a.rows, a.scalars, a.map, a.target, a.loss, a.lse};
