@@ -1,4 +1,7 @@
-"""The token loss against 64 bits, element by element and, in fp32, in the 2-norm."""
+"""The token loss in every shape of tiles that its rules choose between, against 64 bits:
+logits of few rows, of middling and of large ones, alone and with gradients, with and
+without a softcap; products for dx and dw in each of their shapes, whole and split along
+their sums.  The sizes are such that 256 compute units take the shapes named."""
 import numpy as np
 import pytest
 
@@ -50,6 +53,36 @@ def run(N, D, V, dtype, softcap=0.0, kept="fp32", pad=0.0, weighted=False, seed=
             off = errors({"loss": loss[took], "lse": lse[took], "dx": dx[took], "dw": dw}, ref)
             for k, most in norm_bounds(clean[took], w, ref, softcap).items():
                 assert off[k] <= most, (k, off[k] / most)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("softcap", [0.0, 30.0])
+# logits in tiles of 128 x 32, 128 x 128 and 256 x 256: of one stage of the sum, and of four
+@pytest.mark.parametrize("N,D,V", [(150, 64, 900), (40, 200, 900), (2100, 40, 1000), (1500, 200, 2100),
+                                   (300, 40, 16500), (700, 200, 12000)])
+def test_logits(gpu_lib, N, D, V, softcap, dtype):
+    run(N, D, V, dtype, softcap, pad=0.1 if D == 200 else 0.0, weighted=D == 40)
+
+
+@pytest.mark.parametrize("N,D,V,dtype,kept,softcap", [
+    (1500, 200, 16500, "bf16", "fp32", 0.0),   # dw in 256 x 256, split
+    (520, 392, 8300, "fp32", "fp32", 0.0),     # the same
+    (520, 1001, 13000, "bf16", "bf16", 0.0),   # dw in 256 x 256, whole
+    (520, 1000, 13000, "bf16", "bf16", 30.0),
+    (520, 1000, 13000, "fp32", "fp32", 0.0),
+    (4200, 1032, 2100, "bf16", "fp32", 30.0),  # dx in 256 x 256, split
+    (2100, 392, 4100, "fp32", "fp32", 0.0),    # the same, dw in 192 x 256, split
+    (13000, 1000, 520, "bf16", "bf16", 0.0),   # dx in 256 x 256, whole
+    (13000, 1001, 520, "fp32", "fp32", 30.0),
+    (4200, 136, 4100, "bf16", "fp32", 0.0),    # dx and dw in 192 x 256, split
+    (3000, 136, 2100, "fp32", "fp32", 0.0),    # dx in 192 x 256, split
+    (200, 392, 16500, "bf16", "bf16", 0.0),    # dw in 192 x 256, whole
+    (200, 392, 16500, "fp32", "fp32", 20.0),
+    (9000, 1800, 300, "bf16", "fp32", 0.0),    # dx in 192 x 256, whole
+    (700, 1032, 13200, "fp32", "bf16", 0.0),   # dw in 192 x 256, both
+])
+def test_gradients(gpu_lib, N, D, V, dtype, kept, softcap):
+    run(N, D, V, dtype, softcap, kept, pad=0.1 if N % 1000 else 0.0)
 
 
 # the small shapes' precision: losses and gradients of products in two planes each
