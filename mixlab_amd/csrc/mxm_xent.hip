@@ -650,10 +650,15 @@ void mxm_launch_xent(const XentArgs& a0, hipStream_t s) {
                              gather, s);
       const int blocks = (a.V + block - 1) / block;
       if (rows <= JOIN_FEW) {
-        // (5 to 16 rows' losses with their total: one workgroup, without the total's launch,
-        // 12.7 us of 10 rows of D 192 and 58527 entries, 14.9 with four waves a row)
-        const bool long_joins = blocks > LONG_JOIN && (a.backward || !a.total || a.rows <= JOIN_WAVES / 4 ||
-                                                       a.rows > JOIN_WAVES);
+        // Four waves a row for long sums; but up to 15 rows' losses with their total, of
+        // some 24000 blocks in all, take one workgroup with a wave a row and no launch for
+        // the total (us so / with four waves a row and that launch: 10 rows against 58527
+        // entries, 18000 blocks, 12.6 / 14.3; 13 rows, 24000, 15.0 / 15.1; 11 against 131072,
+        // 45000, 20.7 / 18.7; 16 rows against 33000, 16500, 16.1 / 14.1, and against a
+        // million 275 / 115).
+        const bool alone = !a.backward && a.total && a.rows > JOIN_WAVES / 4 && a.rows < JOIN_WAVES &&
+                           a.rows * blocks <= 24000;
+        const bool long_joins = blocks > LONG_JOIN && !alone;
         const int each = long_joins ? JOIN_WAVES / 4 : JOIN_WAVES;
         a.c_parts = (int)((rows + each - 1) / each);
         total_there = a.total && a.rows <= each;
