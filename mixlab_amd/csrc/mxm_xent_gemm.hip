@@ -1041,9 +1041,13 @@ struct Grad {
 enum GradShape { G_SMALL, G_THIN, G_BIG };
 
 // The shape whose tiles take the least time by split_of's count of stages, at a stage's
-// time (Small: of two on a CU).  Measured: a step of 8192 rows and 32768 entries at D
-// 320 982 us in tiles of 256 channels, 930 of 192; D 384 1014 / 965; of 315 rows and 256
-// entries in fp32 at D 1528 89 us in tiles of 256, 76 so.
+// time (Small: of two on a CU).  Those, measured: dw of D 1536 and 32768 entries, whole
+// rounds in every shape, 4 to 192 stages, takes 1.81-2.35 us a stage in tiles of Big,
+// 1.39-1.80 in Thin (0.79 of that on average) and 0.96-1.31 in Small (0.55).  What the rule
+// chooses between: a step of 4096 rows and 32768 entries at D 544 with dx in Big 508 us, Thin
+// 488, Small 496; 8192 and 32768 at D 1024 1256 / 1464 / 1387; dw of 4096 and 8192 at D 1024
+// 194 / 193 / 170; of 300 and 50257 at D 1000 155 / 151 / 136; of 1024 and 32768 at D 192 in
+// fp32, where it takes Thin, 229 / 219 / 205, its worst of 16 such sizes.
 GradShape grad_shape(const XentArgs& a, const Grad& g, int64_t k) {
   const int stages = (int)((k + BK - 1) / BK) * g.p.pairs;
   const auto time = [&](auto tile, int per_cu, double stage) {
@@ -1053,7 +1057,7 @@ GradShape grad_shape(const XentArgs& a, const Grad& g, int64_t k) {
                             (int)(mxm_xent_partial_bytes(a.n_cu) / (TL::BM * TL::BN * 4)))
                        .cost;
   };
-  const double big = time(Big{}, 1, 1.0), thin = time(Thin{}, 1, 0.8), small = time(Small{}, 2, 0.65);
+  const double big = time(Big{}, 1, 1.0), thin = time(Thin{}, 1, 0.79), small = time(Small{}, 2, 0.55);
   return small < big && small < thin ? G_SMALL : thin < big ? G_THIN : G_BIG;
 }
 

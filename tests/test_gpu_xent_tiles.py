@@ -65,24 +65,45 @@ def test_logits(gpu_lib, N, D, V, softcap, dtype):
 
 
 @pytest.mark.parametrize("N,D,V,dtype,kept,softcap", [
-    (1500, 200, 16500, "bf16", "fp32", 0.0),   # dw in 256 x 256, split
-    (520, 392, 8300, "fp32", "fp32", 0.0),     # the same
-    (520, 1001, 13000, "bf16", "bf16", 0.0),   # dw in 256 x 256, whole
-    (520, 1000, 13000, "bf16", "bf16", 30.0),
-    (520, 1000, 13000, "fp32", "fp32", 0.0),
-    (4200, 1032, 2100, "bf16", "fp32", 30.0),  # dx in 256 x 256, split
-    (2100, 392, 4100, "fp32", "fp32", 0.0),    # the same, dw in 192 x 256, split
-    (13000, 1000, 520, "bf16", "bf16", 0.0),   # dx in 256 x 256, whole
-    (13000, 1001, 520, "fp32", "fp32", 30.0),
-    (4200, 136, 4100, "bf16", "fp32", 0.0),    # dx and dw in 192 x 256, split
-    (3000, 136, 2100, "fp32", "fp32", 0.0),    # dx in 192 x 256, split
-    (200, 392, 16500, "bf16", "bf16", 0.0),    # dw in 192 x 256, whole
-    (200, 392, 16500, "fp32", "fp32", 20.0),
-    (9000, 1800, 300, "bf16", "fp32", 0.0),    # dx in 192 x 256, whole
-    (700, 1032, 13200, "fp32", "bf16", 0.0),   # dw in 192 x 256, both
+    (1500, 200, 16500, "bf16", "fp32", 0.0),    # dx in 128 x 128, split, dw in 128 x 128
+    (520, 392, 8300, "fp32", "fp32", 0.0),      # dx in 128 x 128, split, dw in 128 x 128
+    (520, 1001, 13000, "bf16", "bf16", 0.0),    # dx in 128 x 128, split, dw in 256 x 256
+    (520, 1000, 13000, "bf16", "bf16", 30.0),   # dx in 128 x 128, split, dw in 256 x 256
+    (520, 1000, 13000, "fp32", "fp32", 0.0),    # dx in 128 x 128, split, dw in 256 x 256
+    (4200, 1032, 2100, "bf16", "fp32", 30.0),   # dx in 128 x 128, split, dw in 128 x 128, split
+    (2100, 392, 4100, "fp32", "fp32", 0.0),     # dx in 128 x 128, split, dw in 192 x 256, split
+    (13000, 1000, 520, "bf16", "bf16", 0.0),    # dx in 256 x 256, dw in 128 x 128, split
+    (13000, 1001, 520, "fp32", "fp32", 30.0),   # dx in 256 x 256, dw in 128 x 128, split
+    (4200, 136, 4100, "bf16", "fp32", 0.0),     # dx in 128 x 128, split, dw in 128 x 128, split
+    (3000, 136, 2100, "fp32", "fp32", 0.0),     # dx in 128 x 128, split, dw in 128 x 128, split
+    (200, 392, 16500, "bf16", "bf16", 0.0),     # dx in 128 x 128, split, dw in 192 x 256
+    (200, 392, 16500, "fp32", "fp32", 20.0),    # dx in 128 x 128, split, dw in 192 x 256
+    (9000, 1800, 300, "bf16", "fp32", 0.0),     # dx in 192 x 256, dw in 128 x 128, split
+    (700, 1032, 13200, "fp32", "bf16", 0.0),    # dx in 192 x 256, split, dw in 128 x 128
 ])
 def test_gradients(gpu_lib, N, D, V, dtype, kept, softcap):
     run(N, D, V, dtype, softcap, kept, pad=0.1 if N % 1000 else 0.0)
+
+
+@pytest.mark.parametrize("N,D,V,dtype,kept,softcap", [
+    (200, 200, 33000, "bf16", "fp32", 0.0),    # dw in 256 x 256, whole
+    (200, 200, 33000, "fp32", "fp32", 0.0),
+    (13000, 392, 4100, "bf16", "fp32", 0.0),   # dw in 256 x 256, split
+    (1500, 392, 8300, "fp32", "fp32", 0.0),
+    (6500, 1800, 300, "bf16", "fp32", 0.0),    # dx in 256 x 256, whole
+    (6500, 1800, 300, "fp32", "fp32", 0.0),
+    (4200, 392, 13000, "bf16", "fp32", 0.0),   # dx in 256 x 256, split
+    (4200, 392, 4100, "fp32", "fp32", 0.0),
+    (200, 136, 33000, "bf16", "fp32", 20.0),   # dw in 192 x 256, whole
+    (1500, 136, 13000, "bf16", "fp32", 0.0),   # dw in 192 x 256, split
+    (520, 136, 13000, "fp32", "fp32", 0.0),
+    (9000, 1000, 300, "bf16", "bf16", 0.0),    # dx in 192 x 256, whole
+    (9000, 1000, 300, "fp32", "fp32", 0.0),
+    (13000, 136, 2100, "bf16", "fp32", 0.0),   # dx in 192 x 256, split
+    (13000, 136, 520, "fp32", "fp32", 0.0),
+])
+def test_gradients_of_large_tiles(gpu_lib, N, D, V, dtype, kept, softcap):
+    run(N, D, V, dtype, softcap, kept, seed=2)
 
 
 # the small shapes' precision: losses and gradients of products in two planes each
