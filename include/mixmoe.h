@@ -405,6 +405,7 @@ int mxm_grads_adamw(int64_t h, double lr, double beta1, double beta2, double eps
  * Handles as the residual norm's and the gradient set's above: shared streams,
  * asynchronous calls without allocation or waiting (all can be captured), contiguous
  * device tensors aligned to their elements, a workspace that is the handle's own.
+ * None is created on a stream that is being captured.
  * An output may not overlap any other tensor of its call.  Every sum is taken in
  * an order that the call's sizes and whole-number inputs decide: equal inputs give
  * equal bits. */

@@ -69,6 +69,14 @@ void check_rows(const char* what, int64_t rows, int64_t max_rows) {
 }
 int item(bool bf16) { return bf16 ? 2 : 4; }
 
+// A create allocates and clears memory on the stream, which a capture would only record.
+void refuse_capture(const char* what, const std::shared_ptr<StreamRef>& shared) {
+  if (!shared) return;
+  hipStreamCaptureStatus now = hipStreamCaptureStatusNone;
+  HIPCK(hipStreamIsCapturing(shared->stream, &now));
+  if (now != hipStreamCaptureStatusNone) fail("%s cannot be created on a stream that is being captured", what);
+}
+
 // Softcaps: a capped logit is off by a few 2^-24 of the cap, 1.2e-4 at the largest.
 constexpr float XENT_MIN_CAP = 1.0f / 64, XENT_MAX_CAP = 1024;
 
@@ -149,6 +157,7 @@ int64_t mxm_embed_create(const int64_t* params, int n_params, float scale, int64
     if (flags & ~(int64_t)MXM_EMBED_BACKWARD) fail(EMBED " unknown flags 0x%llx", (unsigned long long)flags);
     if (!std::isfinite(scale)) fail(EMBED " scale must be finite");
     auto shared = shared_stream(EMBED, stream_of);
+    refuse_capture(EMBED, shared);
 
     auto e = std::make_shared<Embed>();
     const DeviceGuard guard(device_of(shared));
@@ -246,6 +255,7 @@ int64_t mxm_xent_create(const int64_t* params, int n_params, float softcap, int6
     if (softcap != 0.0f && !(softcap >= XENT_MIN_CAP && softcap <= XENT_MAX_CAP))
       fail(XENT " softcap must be 0 or in [%g,%g]", XENT_MIN_CAP, XENT_MAX_CAP);
     auto shared = shared_stream(XENT, stream_of);
+    refuse_capture(XENT, shared);
 
     auto x = std::make_shared<Xent>();
     const DeviceGuard guard(device_of(shared));
