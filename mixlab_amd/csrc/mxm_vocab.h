@@ -51,7 +51,7 @@ int64_t mxm_embed_part_floats(int64_t max_rows, int D);
 // fp32 operands become two fp16 planes: a row of x or weight is 2^exp (hi + lo) with
 // its largest element's hi in [2^14, 2^15), 22 bits of every element down to 2^-17 of
 // the largest and 2^-40 of the largest below.  Products of two such operands are
-// hi lo + lo hi + hi hi (lo lo is below 2^-23 of the product), each exact in fp32.
+// hi lo + lo hi + hi hi (lo lo, up to 2^-22 of the product, is left out), each exact in fp32.
 // Exponents of rows along m or n of a product are applied to its sums; along k they
 // have to agree.  With W_v = 2^c_v W'_v and x_n = 2^X_n x'_n:
 //   dz'[n, v] = dz 2^(c_v - E_n),  dx = 2^E_n dz' W'

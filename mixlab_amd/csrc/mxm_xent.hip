@@ -143,12 +143,6 @@ __device__ __forceinline__ int pack_row32(const XentArgs& a, const void* p, int6
   return signs ? XENT_INF : e;
 }
 
-__device__ __forceinline__ int wave_max(int v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v = max(v, __shfl_xor(v, o));
-  return v;
-}
-
 // x's rows that take part to their places, dx's others to zeros; a workgroup per chunk
 // of rows, a wave per row.  The places are in the rows' order; every workgroup counts the
 // rows before its own: PLAN, for up to PLAN_ROWS rows, by itself, else from the chunks'
@@ -596,6 +590,9 @@ __global__ __launch_bounds__(NT) void xent_finish_kernel(XentArgs a, int64_t r0,
 #pragma unroll
         for (int i = 0; i < 8; ++i) e[i] = i == t ? at_target : (v + i < a.V ? e[i] : 0.0f);
         if constexpr (!F16) {
+          // (to bf16 as the table and x are, whose products are at the matrix cores' full
+          // rate and exact: this rounding and that of the results to bf16 leave 1.8e-3 to
+          // 2.3e-3 of dx and dw in the 2-norm, the results' alone 1.66e-3)
           u32x4_t o;
 #pragma unroll
           for (int i = 0; i < 4; ++i) o[i] = mxm_pack_bf2_fast(e[2 * i], e[2 * i + 1]);

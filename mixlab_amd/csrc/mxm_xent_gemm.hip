@@ -1,4 +1,5 @@
-// The token loss's three products on bf16 MFMA (gfx950, v_mfma_f32_32x32x16_bf16).
+// The token loss's three products on MFMA (gfx950, v_mfma_f32_32x32x16_bf16, or _f16 for
+// fp32 operands).
 //
 //   C[m][n] = sum over pairs of planes and k of A(m, k) B(n, k)
 //   logits:  m a vocabulary entry, n a row;  A = weight,        B = x

@@ -75,3 +75,11 @@ def test_a_closed_object_shares_no_stream():
         TokenEmbedding(8, 8, 1, share=Closed())
     with pytest.raises(ValueError, match="closed"):
         TokenLoss(8, 8, 1, share=Closed())
+
+
+@pytest.mark.parametrize("create", [_embed, _xent])
+@pytest.mark.parametrize("kw", [dict(V=_lib.MXM_VOCAB_MAX + 1), dict(D=_lib.MXM_RESNORM_MAX_D + 1),
+                                dict(V=-1), dict(D=-1), dict(rows=-2 ** 62), dict(V=2 ** 62), dict(D=2 ** 62)])
+def test_sizes_right_behind_the_limits(create, kw):
+    assert create(**kw) == 0
+    assert "invalid dimensions (V in [1,4194304], D in [1,16384], maxRows in [0,2^30])" in _lib.last_error()
