@@ -446,8 +446,8 @@ int mxm_embed_backward(int64_t h, int64_t rows, const int32_t* tokens, const voi
  * rounds the logits' gradient to bf16 before the products with it.  Under fp32 a
  * row's elements keep 22 bits down to 2^-17 of its largest and 2^-40 of it below,
  * and so does a row's gradient of the logits (under a softcap, of what it is before
- * the cap's slope); the dw of an entry whose share is 2^-k of every row's largest
- * keeps some 36 - k bits.  An entry (row of weight) that minus infinity or the type's
+ * the cap's slope); the dw of an entry whose gradient is 2^-k of every row's largest
+ * keeps 36 - k bits at least, of 22.  An entry (row of weight) that minus infinity or the type's
  * lowest value keeps from coming has no share in any result (but that dx of a bf16
  * table with infinities is not a number, 0 times those; under fp32 the logit of an
  * entry with infinities has the sign of their sum times x, and is 0 where that is 0);

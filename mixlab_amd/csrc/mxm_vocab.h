@@ -60,10 +60,13 @@ int64_t mxm_embed_part_floats(int64_t max_rows, int D);
 // any size without a share in the gradient has none in it.  c_v is the exponent w_v of
 // the row of weight, but where that is so small that dz' would lose digits, which dW_v
 // needs whatever the row holds (zeros, say): no smaller than L = max_n of the others'
-// largest |dz| 2^w_v over the largest |dz|, less XENT_SLACK (rows of W' below L are taken
-// down to it before product 2: with the slack, few if any of a table of alike rows; a
-// step of 733 rows of D 1528 and 256 entries took 206 us without, 76 with it).  So dx's
-// terms keep 2^-40 of their largest, and dW's 2^-36.
+// largest |dz| 2^w_v over the others' largest |dz| (under a softcap, before its slope),
+// less XENT_SLACK: next to the exponents of the rows that the gradients go to.  Rows of
+// W' below L are taken down to it before product 2 (with the slack, few if any of a table
+// of alike rows; a step of 733 rows of D 1528 and 256 entries took 206 us without, 76 with
+// it).  So dz' keeps 2^-36 of a row's largest |dz|, whatever the entry's row of weight.
+// (Over the largest |dz| of all, the target's, L was lower by the others' shares: with
+// 50257 entries dW of rows of zeros was off by 1.6e-4 of it, 4e-7 so.)
 // A row of weight with infinite elements is its infinities' signs and the exponent
 // XENT_INF, one of zeros has XENT_ZERO.
 //

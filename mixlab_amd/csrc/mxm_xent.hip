@@ -344,20 +344,22 @@ __device__ __forceinline__ float finish_row(const XentArgs& a, int64_t r0, int m
     r.target = a.target[r0 + m];
     r.e = r.g = XENT_NO_EXP;
     if (a.planes != 1) {
-      // no |dz| of the row is above |g| times the others' share
+      // no |dz| of the row is above |g| times the others' share, none of the others' above
+      // 2^15 (a summand's most) times scale
       const float most = __builtin_fabsf(g) * (sum / whole);
       if (most > 0.0f && most < __builtin_inff()) {
-        int e;
-        (void)frexpf(most, &e);
-        r.g = e - 15;
-        (void)frexpf(r.scale, &e);
-        const int of_others = others.exp > XENT_NO_EXP / 2 ? others.exp + e - 15 : XENT_NO_EXP;
-        (void)frexpf(r.at_target, &e);
+        int e_most, e_scale, e_target;
+        (void)frexpf(most, &e_most);
+        (void)frexpf(r.scale, &e_scale);
+        (void)frexpf(r.at_target, &e_target);
         const int w = a.w_exp[r.target];
-        const int of_target = w < XENT_INF && r.at_target != 0.0f ? w + e - 15 : XENT_NO_EXP;
-        r.e = max(of_others, of_target);
-        const int low = of_others > XENT_NO_EXP ? of_others : of_target;
-        exps.take({low > XENT_NO_EXP ? low - r.g - XENT_SLACK : XENT_NO_EXP, r.e + a.x_exp[r0 + m], r.g + a.x_exp[r0 + m]});
+        const bool any = others.exp > XENT_NO_EXP / 2, at = w < XENT_INF && r.at_target != 0.0f;
+        r.e = max(any ? others.exp + e_scale - 15 : XENT_NO_EXP, at ? w + e_target - 15 : XENT_NO_EXP);
+        r.g = max(min(e_most, e_scale + 15), at ? e_target : XENT_NO_EXP) - 15;
+        exps.take({any  ? others.exp - 15 - XENT_SLACK
+                   : at ? w - XENT_SLACK
+                        : XENT_NO_EXP,
+                   r.e + a.x_exp[r0 + m], r.g + a.x_exp[r0 + m]});
       }
     }
     a.row[r0 + m] = r;
@@ -673,7 +675,11 @@ void mxm_launch_xent(const XentArgs& a0, hipStream_t s) {
         const bool once = rows * a.Vp * (a.planes == 1 ? 2 : 8) > (int64_t)1 << 30;
         const int per = NT * (once ? 4 : 1);
         const unsigned gx = (unsigned)std::min((a.Vp / 8 + per - 1) / per, 64);
-        const dim3 grid(gx, (unsigned)std::min<int64_t>(rows, std::max(1u, (unsigned)a.n_cu * 32 / gx)));
+        unsigned gy = (unsigned)std::min<int64_t>(rows, std::max(1u, (unsigned)a.n_cu * 32 / gx));
+        // (few rows' workgroups would be few for the rows of W' below L: a step of one row
+        // against 32768 entries at D 512, whose rows' sizes spread over 2^8, 250-296 us, 112 so)
+        if (a.planes != 1 && a.dx) gy = std::max(gy, (unsigned)std::min(a.n_cu * 4, (a.V + 3) / 4) / gx);
+        const dim3 grid(gx, gy);
         const bool total_late = a.total && !total_there && p == pieces - 1;
         const auto launch = [&](auto kernel) { kernel<<<grid, NT, 0, s>>>(a, r0, block, parity, p == 0, total_late); };
         if (a.planes == 1)

@@ -85,3 +85,36 @@ def test_rows_that_are_not_numbers(gpu_lib, N, dtype):
     for a, b in zip(*outs):
         np.testing.assert_array_equal(a[others], b[others])
         assert np.all(np.isnan(b[bad]))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("N,V", [(20, 300), (520, 16500)])
+def test_logits_far_past_the_cap(gpu_lib, N, V, dtype):
+    """Where the exponential of the cap is infinite, or zero: a capped logit is the cap, its
+    slope zero, of others and of targets."""
+    cap, D = 2.0, 8
+    w = np.zeros((V, D), np.float32)
+    kinds = np.array([0.0, 100.0, -100.0, 1e30, -1e30, 1.0], np.float32)
+    w[:, 0] = as_kept(kinds[np.arange(V) % 6], dtype)
+    x = np.zeros((N, D), np.float32)
+    x[:, 0] = 1.0
+    t = (np.arange(N) % 6).astype(np.int32)
+    dx_, dw_, dt = Dev(x, dtype), Dev(w, dtype), Dev(t, "int32")
+    gw, loss, one = Dev.out((V, D)), Dev.out((N,)), Dev.out((N,))
+    with TokenLoss(V, D, N, dtype=dtype, softcap=cap, mean=False) as h:
+        h.backward(N, dx_.ptr, dw_.ptr, dt.ptr, dw=gw.ptr, loss=loss.ptr)
+        h.forward(N, dx_.ptr, dw_.ptr, dt.ptr, loss=one.ptr)
+        h.synchronize()
+    l = cap * np.tanh(w[:, 0].astype(np.float64) / cap)
+    p = np.exp(l) / np.exp(l).sum()
+    want = np.log(np.exp(l).sum()) - l[t]
+    off = U32 * (64 * cap + 2 * (V / 64 + 160))
+    for o in (loss, one):
+        close(o.get(), want, off, "fp32", "loss")
+    slope = 1 - np.tanh(w[:, 0].astype(np.float64) / cap) ** 2
+    dw = N * p
+    dw[:6] -= np.bincount(t, minlength=6)
+    # (zero within what the slope of 50 caps is, e^-100 and so 2^-144)
+    bound = (np.abs(dw) * slope + N * p * slope) * (off + (UBF + UBF / 4 if dtype == "bf16" else 16 * U32) + 2 * N * U32)
+    close(gw.get()[:, 0], dw * slope, bound + N * 2.0 ** -39 * p.max() * (slope > 1e-30) + 1e-30, "fp32", "dw")
+    assert not np.any(gw.get()[:, 1:])

@@ -5,8 +5,10 @@ import numpy as np
 from tests.train_testutil import U32
 
 
-def norm_bounds(x, w, ref, softcap=0.0):
-    """Of loss, lse, dx and dw of the rows that take part (x and ref's), as 2-norms over all.
+def rms_bounds(x, w, ref, softcap=0.0, floor=0.0):
+    """Of loss, lse, dx and dw of the rows that take part (x and ref's), element by element,
+    for 2-norms over many of them.  floor: what the logits' gradient is off by at least, of
+    its row's largest.
 
     Roundings of different elements are independent: they add up by squares.  A logit's
     error: of each product of elements the operands' half steps of 2^-23 and the product of
@@ -27,12 +29,16 @@ def norm_bounds(x, w, ref, softcap=0.0):
     rel = np.sqrt(el ** 2 + common[:, None] ** 2) + 8 * U32
     if softcap:
         rel = rel + 2 * el / softcap + U32 * (4 * np.abs(z) / softcap + 8)
-    edz = dz * rel
+    edz = dz * rel + floor * dl.max(axis=1, keepdims=True)
     dx = np.sqrt(edz ** 2 @ w ** 2) + 8 * U32 * np.sqrt(dz ** 2 @ w ** 2) + 4 * U32 * np.abs(ref["dx"][rows])
     dw = np.sqrt((edz ** 2).T @ x ** 2) + 8 * U32 * np.sqrt((dz ** 2).T @ x ** 2) + 4 * U32 * np.abs(ref["dw"])
-    return {"loss": np.linalg.norm(common + few + 4 * U32 * ref["loss"][rows]),
-            "lse": np.linalg.norm(np.sqrt(((p * el) ** 2).sum(axis=1)) + few),
-            "dx": np.linalg.norm(dx), "dw": np.linalg.norm(dw)}
+    return {"loss": common + few + 4 * U32 * ref["loss"][rows],
+            "lse": np.sqrt(((p * el) ** 2).sum(axis=1)) + few, "dx": dx, "dw": dw}
+
+
+def norm_bounds(x, w, ref, softcap=0.0):
+    """The same as 2-norms over all."""
+    return {k: np.linalg.norm(v) for k, v in rms_bounds(x, w, ref, softcap).items()}
 
 
 def errors(got, ref):
