@@ -326,7 +326,8 @@ __device__ __forceinline__ float finish_row(const XentArgs& a, int64_t r0, int m
   const bool alone = sum == 0.0f;
   const float d = alone ? -200.0f : fmaf(-lt, LOG2E, top);
   const float et = __builtin_amdgcn_exp2f(-d), whole = sum + et;
-  // (next to the target's probability of one the loss keeps its digits)
+  // (next to the target's probability of one the loss keeps its digits; a share of the
+  // others' below 2^-113 leaves no gradient)
   const bool near = d <= 60.0f;
   const float over = logf(whole);
   const float loss = alone ? lt - lt : near ? log1pf(sum * __builtin_amdgcn_exp2f(d)) : d * LN2 + over;
