@@ -443,7 +443,8 @@ int mxm_embed_backward(int64_t h, int64_t rows, const int32_t* tokens, const voi
  * over the rows that take part (0 where none does).
  * params = [V, D, maxRows, dtype, dxDtype, dwDtype, flags]; dtype is that of x and
  * weight.  Under bf16 the products are exact and summed in fp32, and the backward
- * rounds the logits' gradient to bf16 before the products with it.  Under fp32 a
+ * rounds the logits' gradient to bf16 before the products with it (from fp16: what is
+ * below 2^-29 of a row's largest keeps fewer bits, below 2^-39 of it none).  Under fp32 a
  * row's elements keep 22 bits down to 2^-17 of its largest and 2^-40 of it below,
  * and so does a row's gradient of the logits (under a softcap, of what it is before
  * the cap's slope); the dw of an entry whose gradient is 2^-k of every row's largest
